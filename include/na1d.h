@@ -383,6 +383,52 @@ int na1d_train_context_backward(void *dx, const void *dctx, const void *x, const
                                 int64_t T, float eps, int dtype, void *stream);
 
 /*
+ * Losses over a large number of classes, forward and backward, without the logits in memory.  They replace the classification
+ * heads of models/SoftMaxLoss.py:7-138 (and add a teacher's): x [N, D] are embeddings or hidden states, w [V * subcenters, D]
+ * the classes' weight rows, both 16-bit with contiguous channels and rows x_stride, w_stride elements apart.
+ *   kind NA1D_HEAD_TARGETS: z = scale * x . w, loss of a row: log sum exp z - z[target]
+ *   kind NA1D_HEAD_MARGIN:  cos = max over a class's subcenters of x . w / (|x| |w|); z = scale * cos, at the target
+ *          scale * cos(theta + margin) where cos > cos(pi - margin), else scale * (cos - margin * sin(pi - margin)).  The derivative
+ *          of cos(theta + margin) takes the squared sine as 1e-6 at least; a row of zeros has cosine 0 and no gradient.
+ *   kind NA1D_HEAD_TEACHER: z = x . w / temperature (`scale` is the temperature); q = softmax(teacher / temperature) over
+ *          the row's `top` entries (ids [N, top], teacher [N, top]; ids below 0 are no entries, a class may be there
+ *          twice); loss of a row: temperature^2 * sum of q (log q - log softmax(z)[id])
+ * A row whose target is ignore_index, or whose teacher has no entry, has loss 0 and no gradient and does not count in a mean
+ * (0 if none counts).  Any other target outside [0, V), and a teacher's id of V or more, makes the row's loss NaN; it has no gradient.
+ *   loss  : fp32 [N] (NA1D_HEAD_NONE) or [1] (_MEAN, _SUM); dloss the same in the backward
+ *   saved : what a forward leaves for its backward, na1d_head_saved_bytes() bytes; a forward needs it in any case
+ *   dx, dw: 16-bit, packed [N, D] and [V * subcenters, D]; either may be NULL
+ * Sums are in fp32; the gradients of the logits are rounded to 16 bits (fp16: scaled by a power of two first) before they
+ * are multiplied.  Nothing uses atomics: results are the same from call to call.
+ * D % 8 == 0; x, w, dx, dw, saved and the workspace 16-byte aligned, strides multiples of 8 and at least D.  Limits
+ * (NA1D_ERR_UNSUPPORTED): N up to 2^20, V * subcenters up to 2^24, w_stride * subcenters and x_stride up to 2^20, N * V, N * D and
+ * V * subcenters * D up to 2^37, subcenters up to 255, top up to NA1D_HEAD_MAX_TOP.
+ */
+#define NA1D_FP32 2              /* teacher_type only */
+#define NA1D_HEAD_TARGETS 0
+#define NA1D_HEAD_MARGIN  1
+#define NA1D_HEAD_TEACHER 2
+#define NA1D_HEAD_NONE 0
+#define NA1D_HEAD_MEAN 1
+#define NA1D_HEAD_SUM  2
+#define NA1D_HEAD_MAX_TOP 256
+typedef struct na1d_head {
+    int32_t dtype, kind, reduction;
+    int32_t subcenters;                 /* 1 except with a margin */
+    int32_t top, teacher_type;          /* teacher only: entries of a row; NA1D_BF16, NA1D_FP16 or NA1D_FP32 */
+    int32_t ids_64;                     /* targets and ids are int64, else int32 */
+    float scale, margin;                /* finite and above 0; 0 <= margin < pi / 2 */
+    int64_t ignore_index;
+    int64_t N, V, D, x_stride, w_stride;
+} na1d_head;
+int64_t na1d_head_saved_bytes(const na1d_head *h);
+int64_t na1d_head_workspace_bytes(const na1d_head *h, int backward);
+int na1d_head_forward(const na1d_head *h, float *loss, const void *x, const void *w, const void *ids, const void *teacher, void *saved,
+                      int64_t saved_bytes, void *workspace, int64_t workspace_bytes, void *stream);
+int na1d_head_backward(const na1d_head *h, void *dx, void *dw, const float *dloss, const void *x, const void *w, const void *ids, const void *saved,
+                       int64_t saved_bytes, void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
  * Profiling hook; no counterpart in the reference.  From this call on, the matrix-core fused kernels that the
  * CALLING THREAD launches record `start` just before and `stop` just after the kernel itself (hipEvent_t handles,
  * recorded by hipExtLaunchKernel: the dispatch's own begin and end, i.e. what a profiler's kernel trace reports,

@@ -565,6 +565,51 @@ int na1d_train_layer_backward(const na1d_train_layer *l, void *dx, const void *d
     return na1d::train::run_backward(*l, dx, dout, x, saved, workspace, N, T, (hipStream_t)stream);
 }
 
+static int head_check(const na1d_head *h) {
+    if (!h) return NA1D_ERR_NULL;
+    if (h->dtype != NA1D_BF16 && h->dtype != NA1D_FP16) return NA1D_ERR_DTYPE;
+    const bool teaches = h->kind == NA1D_HEAD_TEACHER, cosines = h->kind == NA1D_HEAD_MARGIN;
+    if (h->kind < NA1D_HEAD_TARGETS || h->kind > NA1D_HEAD_TEACHER || h->reduction < NA1D_HEAD_NONE || h->reduction > NA1D_HEAD_SUM) return NA1D_ERR_SHAPE;
+    if (teaches && (h->teacher_type < NA1D_BF16 || h->teacher_type > NA1D_FP32)) return NA1D_ERR_DTYPE;
+    if (h->N < 1 || h->V < 1 || h->subcenters < 1 || (teaches && h->top < 1)) return NA1D_ERR_SHAPE;
+    if (h->D < 1 || h->D % 8) return NA1D_ERR_HEAD_DIM;
+    if (h->x_stride < h->D || h->w_stride < h->D) return NA1D_ERR_SHAPE;
+    if (h->x_stride % 8 || h->w_stride % 8) return NA1D_ERR_ALIGN;
+    if (bad_scale(h->scale) || (cosines && !(h->margin >= 0.f && h->margin < 1.5707963f))) return NA1D_ERR_SCALE;
+    const int64_t most = 1ll << 37, widest = 1ll << 20;
+    if (h->subcenters > (cosines ? 255 : 1) || (teaches && h->top > NA1D_HEAD_MAX_TOP)) return NA1D_ERR_UNSUPPORTED;
+    if (h->N > widest || h->V > (1ll << 24) / h->subcenters || h->x_stride > widest || h->w_stride > widest / h->subcenters) return NA1D_ERR_UNSUPPORTED;
+    if (h->N * h->V > most || h->N * h->D > most || h->V * h->subcenters * h->D > most) return NA1D_ERR_UNSUPPORTED;
+    return NA1D_OK;
+}
+int64_t na1d_head_saved_bytes(const na1d_head *h) {
+    const int st = head_check(h);
+    return st == NA1D_OK ? na1d::loss::saved_bytes(*h) : st;
+}
+int64_t na1d_head_workspace_bytes(const na1d_head *h, int backward) {
+    const int st = head_check(h);
+    return st == NA1D_OK ? na1d::loss::scratch_bytes(*h, backward != 0) : st;
+}
+int na1d_head_forward(const na1d_head *h, float *loss, const void *x, const void *w, const void *ids, const void *teacher, void *saved,
+                      int64_t saved_bytes, void *workspace, int64_t workspace_bytes, void *stream) {
+    const int st = head_check(h);
+    if (st != NA1D_OK) return st;
+    if (!loss || !x || !w || !ids || !saved || !workspace || (h->kind == NA1D_HEAD_TEACHER && !teacher)) return NA1D_ERR_NULL;
+    if (misaligned(x) || misaligned(w) || misaligned(saved) || misaligned(workspace)) return NA1D_ERR_ALIGN;
+    if (saved_bytes < na1d::loss::saved_bytes(*h) || workspace_bytes < na1d::loss::scratch_bytes(*h, false)) return NA1D_ERR_WORKSPACE;
+    return na1d::loss::run_forward(*h, loss, x, w, ids, teacher, saved, workspace, (hipStream_t)stream);
+}
+int na1d_head_backward(const na1d_head *h, void *dx, void *dw, const float *dloss, const void *x, const void *w, const void *ids, const void *saved,
+                       int64_t saved_bytes, void *workspace, int64_t workspace_bytes, void *stream) {
+    const int st = head_check(h);
+    if (st != NA1D_OK) return st;
+    if (!dloss || !x || !w || !ids || !saved || !workspace) return NA1D_ERR_NULL;
+    if (misaligned(x) || misaligned(w) || misaligned(saved) || misaligned(workspace) || misaligned(dx) || misaligned(dw)) return NA1D_ERR_ALIGN;
+    if (saved_bytes < na1d::loss::saved_bytes(*h) || workspace_bytes < na1d::loss::scratch_bytes(*h, true)) return NA1D_ERR_WORKSPACE;
+    if (!dx && !dw) return NA1D_OK;
+    return na1d::loss::run_backward(*h, dx, dw, dloss, x, w, ids, saved, workspace, (hipStream_t)stream);
+}
+
 int na1d_fused_backward_noalloc(void *dq, void *dk, void *dv, float *drpb, const void *q, const void *k, const void *v,
                                 const void *out, const void *dout, const float *lse, const float *rpb,
                                 const int32_t *t_valid, int64_t B, int64_t H, int64_t T, int64_t C, int64_t W,

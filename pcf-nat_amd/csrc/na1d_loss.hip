@@ -1,0 +1,1097 @@
+// Losses over a large number of classes, forward and backward, without the logits in memory: softmax cross entropy of a linear
+// head, the additive angular margin of models/SoftMaxLoss.py:99-138 on cosines with several weight rows to a class, and the
+// divergence from a teacher of which the largest logits are kept.
+//
+// With z_nc = scale * x_n . w_c, o_n = log of the sum of exp(z_nc) over the classes that are not the row's target t:
+//   loss_n = log(1 + exp(o_n - z_nt)),   dz_nc = P_nc - [c = t],   P = softmax(z),   dx = dz W,   dW = dz^T x.
+// The target is kept out of the sum so that neither the loss of a row that is nearly certain nor its P_nt - 1 is the difference
+// of two numbers that are nearly the same.  The forward is one product x W^T whose tiles leave as a maximum and a sum of
+// exponentials to a row (logits_kernel), and a kernel that puts a row's tiles together (finish_kernel).  The backward works the
+// logits out again, a range of classes at a time, rounds dz to the operands' type - what a head that keeps its logits would have
+// handed its products - and multiplies it twice (product_kernel): by W for dx, transposed by x for dW.
+#include <cmath>
+
+#include "na1d_encoder.h"
+
+namespace na1d {
+namespace loss {
+
+using namespace enc;
+
+// =============================================================================
+// Tiles
+// =============================================================================
+// Every operand comes through LDS in pieces of 64 rows of 128 bytes, written there by the loads themselves; what a step of 64 of
+// the contraction needs of a tile is extent / 64 such pieces.  An operand whose contraction runs along its rows in memory has
+// the tile's rows (64 to a piece) and 64 values of each; one whose contraction runs from row to row ("turned") has 64 rows of
+// the contraction and 64 of the tile's columns, which come out of LDS transposed (ds_read_b64_tr_b16).  The 16-byte units of a
+// row are XOR-swizzled by three bits of its number so that both ways of reading spread over all banks: rows 0 .. 15 at one unit
+// (row operands), and rows {0-3, 8-11} or {4-7, 12-15} at 32 bytes (half a wave's transposed read).
+constexpr int kStep = 64;                     // of the contraction
+constexpr int kPieceRow = 2 * kStep;          // bytes
+constexpr int kPiece = 64 * kPieceRow;
+__device__ inline int swizzle(int row) { return ((row >> 3) & 1) << 2 | ((row >> 1) & 1) << 1 | ((row >> 2) & 1); }
+
+// Where an operand's tile comes from.  All members but the lane's are wave-uniform.
+template <int EXTENT, int NW, bool TURNED> struct Source {
+    static constexpr int kLoads = EXTENT * kPieceRow / kChunk / NW;          // of a wave in a step
+    static constexpr int kBytes = EXTENT * kPieceRow;
+    static_assert(EXTENT * kPieceRow % (kChunk * NW) == 0 && (!TURNED || EXTENT % 64 == 0) && NW % 4 == 0, "whole chunks");
+    const char *at;          // first byte of the tile
+    int64_t bytes, step;     // from there to the end of what may be read; from one step to the next
+    int pitch, width;        // bytes: from row to row; of a row, from the tile's first one on
+    int lane_at, unit;       // this lane's place in chunk `wave`
+    // `rows`: rows that exist from the tile's first one on (of the tile, or, turned, of the contraction)
+    __device__ inline void init(const char *first, int64_t rows, int64_t row_pitch, int64_t row_width, int wave, int lane) {
+        at = first;
+        pitch = (int)row_pitch;
+        width = (int)row_width;
+        bytes = rows > 0 ? (rows - 1) * row_pitch + row_width : 0;
+        step = TURNED ? kStep * row_pitch : kPieceRow;
+        unit = ((lane & 7) ^ swizzle(8 * wave + (lane >> 3))) * 16;          // chunks of a wave differ by multiples of 16 rows or of 32
+        lane_at = (8 * wave + (lane >> 3)) * pitch + unit;
+    }
+    __device__ inline void load(LDS_PTR(char) to, int s, int wave) const {
+        const int64_t left = bytes - s * step;
+        const Rsrc src = make_rsrc(at + s * step, (int)(left < 0 ? 0 : left < (1 << 30) ? left : (1 << 30)));
+        const int from = TURNED || s * kPieceRow + unit < width ? lane_at : kNowhere;
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+            const int c = j * NW;                                            // + wave
+            int off = from;
+            if constexpr (TURNED) {
+                off += c % 8 * 8 * pitch + c / 8 * kPieceRow;
+                if (c / 8 * kPieceRow + unit >= width) off = kNowhere;
+            } else {
+                off += c * 8 * pitch;
+            }
+            load_to_lds<16, kReadShared>(src, to + (c + wave) * kChunk, off);
+        }
+    }
+};
+// Operands of the 16 x 16 x 32 product out of such a tile: 16 of its extent (number t) and half h of the step's 64.
+template <bool TURNED> struct Reader;
+template <> struct Reader<false> {
+    int lane_at;
+    __device__ inline void init(int n, int g) { lane_at = n * kPieceRow + ((g ^ swizzle(n)) << 4); }
+    __device__ inline u32x4 read(LDS_PTR(char) tile, int t, int h) const {
+        return *reinterpret_cast<LDS_PTR(u32x4)>(tile + t * 16 * kPieceRow + (lane_at ^ h * 64));
+    }
+};
+template <> struct Reader<true> {
+    int lane_at;
+    __device__ inline void init(int n, int g) {
+        const int row = 8 * g + (n >> 2);
+        lane_at = row * kPieceRow + ((((n & 3) >> 1) ^ swizzle(row)) << 4) + 8 * (n & 1);
+    }
+    __device__ inline u32x4 read(LDS_PTR(char) tile, int t, int h) const {
+        LDS_PTR(char) p = tile + (t >> 2) * kPiece + h * 32 * kPieceRow;
+        const int at = lane_at ^ (t & 3) * 32;
+        const u32x2 a = read_tr(p + at), b = read_tr(p + 4 * kPieceRow + (at ^ 16));
+        return u32x4{a.x, a.y, b.x, b.y};
+    }
+};
+
+// A workgroup's tile: WM x WN waves of MT x NT products of 16 x 16; STAGES steps of operands in LDS.
+template <int MT_, int NT_, int WM_, int WN_, int STAGES_> struct Shape {
+    static constexpr int MT = MT_, NT = NT_, WM = WM_, WN = WN_, STAGES = STAGES_;
+    static constexpr int kWavesOf = WM * WN, kThreadsOf = 64 * kWavesOf, BM = 16 * MT * WM, BN = 16 * NT * WN;
+    static constexpr int kSlot = (BM + BN) * kPieceRow, kLds = STAGES * kSlot;
+};
+__device__ inline float sum_of_16(float x) {                                   // over the lanes of one g
+    x += __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), 0xb1, 0xf, 0xf, true));
+    x += __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), 0x4e, 0xf, 0xf, true));
+    x += __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), 0x141, 0xf, 0xf, true));
+    return x + __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), 0x140, 0xf, 0xf, true));
+}
+template <int COUNT> __device__ inline void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(COUNT) : "memory"); }
+
+// acc[i][j] += A[16 of M, number wm * MT + i] . B[16 of N, number wn * NT + j]^T; lane (n, g) holds M 4g .. 4g + 3 and N n.
+// A step's operands are asked for STAGES - 1 steps ahead; one barrier to a step.
+template <class DT, class S, class A, class B, class RA, class RB>
+__device__ inline void accumulate(f32x4 (&acc)[S::MT][S::NT], const A &a, const B &b, const RA &ra, const RB &rb, int steps, LDS_PTR(char) lds, int wave, int wm,
+                                  int wn) {
+    constexpr int kAhead = S::STAGES - 1, kLoads = A::kLoads + B::kLoads;
+    auto stage = [&](int s, int slot) {
+        a.load(lds + slot * S::kSlot, s, wave);
+        b.load(lds + slot * S::kSlot + A::kBytes, s, wave);
+    };
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s)
+        if (s < steps) stage(s, s);
+    int slot = 0, next = kAhead;
+#pragma unroll 1
+    for (int s = 0; s < steps; ++s) {
+        if (s + kAhead <= steps)
+            wait_loads<(kAhead - 1) * kLoads>();
+        else
+            wait_loads<0>();
+        barrier_lds();                       // everyone's loads of this step are there, everyone is done with the step before
+        if (s + kAhead < steps) stage(s + kAhead, next);
+        LDS_PTR(char) from = lds + slot * S::kSlot;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            u32x4 x[S::MT], y[S::NT];
+#pragma unroll
+            for (int i = 0; i < S::MT; ++i) x[i] = ra.read(from, wm * S::MT + i, h);
+#pragma unroll
+            for (int j = 0; j < S::NT; ++j) y[j] = rb.read(from + A::kBytes, wn * S::NT + j, h);
+#pragma unroll
+            for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+                for (int j = 0; j < S::NT; ++j) acc[i][j] = Mma<DT>::k32(x[i], y[j], acc[i][j]);
+        }
+        slot = slot + 1 == S::STAGES ? 0 : slot + 1;
+        next = next + 1 == S::STAGES ? 0 : next + 1;
+    }
+}
+
+// =============================================================================
+// The heads
+// =============================================================================
+constexpr int kFar = 0x7f000000;             // no class
+// What a row has to do with its target, left by the forward for the backward.
+struct alignas(16) RowStat {
+    float lse2;        // log2 of the sum of exp(z) over all classes, the target's with its margin; +inf: the row does not count
+    float at_target;   // P_t - 1, times the margin's slope
+    int target;        // class, or kFar
+    int sub;           // of its weight rows the nearest
+};
+// The same as the backward's kernels take it.
+struct alignas(16) RowGrad {
+    float lse2, f, at_target;       // dz = f * exp2(z2 - lse2), at the target at_target
+    int target;
+};
+struct Head {
+    const char *x, *w;
+    int64_t x_pitch, w_pitch;       // bytes
+    int N, V, D, subs;
+    float scale2;                   // scale * log2(e)
+    const float *inv_x, *inv_w;     // 1 / |row| (cosines only)
+};
+// A class's index in ids of either width; what does not fit 32 bits is no class.
+__device__ inline int load_id(const void *ids, int64_t i, int wide) {
+    if (!wide) return reinterpret_cast<const int32_t *>(ids)[i];
+    const int64_t v = reinterpret_cast<const int64_t *>(ids)[i];
+    return v < INT32_MIN || v > INT32_MAX ? (v < 0 ? INT32_MIN : INT32_MAX) : (int)v;
+}
+// A row of zeros has cosine 0 with everything and no gradient.  The factor of its (zero) products is a small number and not 0, so
+// that a masked logit of -inf stays one.
+constexpr float kLeastNorm = 1e-12f, kNoNorm = 1e-30f;
+
+// 1 / |row| of 16-bit rows, a wave to a row; the first `rows_a` are a's.  And the largest of each workgroup's rows of b.
+template <class DT>
+__global__ void __launch_bounds__(256)
+norms_kernel(float *__restrict__ inv_a, float *__restrict__ inv_b, float *__restrict__ most_b, const char *__restrict__ a, const char *__restrict__ b, int64_t a_pitch,
+             int64_t b_pitch, int64_t rows_a, int64_t rows_b, int D) {
+    __shared__ float most[4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    float top = 0.f;
+    for (int64_t r = (int64_t)blockIdx.x * 4 + wave; r < rows_a + rows_b; r += (int64_t)gridDim.x * 4) {
+        const bool first = r < rows_a;
+        const char *row = first ? a + r * a_pitch : b + (r - rows_a) * b_pitch;
+        float s = 0.f;
+        for (int c = lane * 8; c < D; c += 512) {
+            const u32x4 v = *reinterpret_cast<const u32x4 *>(row + 2 * c);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f32x2 p = widen<DT>(v[i]);
+                s = __builtin_fmaf(p.x, p.x, s);
+                s = __builtin_fmaf(p.y, p.y, s);
+            }
+        }
+#pragma unroll
+        for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
+        const float inv = s > kLeastNorm * kLeastNorm ? 1.f / __builtin_sqrtf(s) : s != s ? s : kNoNorm;
+        if (lane == 0) (first ? inv_a[r] : inv_b[r - rows_a]) = inv;
+        if (!first) top = __builtin_fmaxf(top, inv);
+    }
+    if (lane == 0) most[wave] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) most_b[blockIdx.x] = __builtin_fmaxf(__builtin_fmaxf(most[0], most[1]), __builtin_fmaxf(most[2], most[3]));
+}
+
+// Tile number -> (class tile, row tile): groups of kGroup class tiles by all row tiles, so that what runs side by side on an XCD
+// shares both operands in its L2.
+constexpr int kGroup = 8;
+__device__ inline void tile_of(uint32_t item, int m_tiles, int n_tiles, int &m, int &n) {
+    const uint32_t per = (uint32_t)kGroup * n_tiles, group = item / per, in = item - group * per;
+    const uint32_t wide = min((uint32_t)kGroup, (uint32_t)m_tiles - group * kGroup);
+    n = (int)(in / wide);
+    m = (int)(group * kGroup + in - (uint32_t)n * wide);
+}
+
+struct Logits {
+    Head h;
+    int class0, classes;            // of this range; the tiles cut it up
+    int m_tiles, n_tiles;
+    // forward: a maximum and a sum (log2 domain) to a class tile and row
+    f32x2 *part;
+    const void *ids;                // targets, or NULL: no class is kept out
+    int ids_wide;
+    // backward
+    const RowGrad *rows;
+    const RowStat *stats;
+    char *dz;                       // 16-bit [N, subs, plane]
+    int64_t plane;                  // columns to a sub-centre, a multiple of 64
+    float *col_part;                // cosines: sums of dz * cosine over a wave's rows: [n_tiles * WN, subs, plane]
+};
+
+// Logits of a tile of classes (M) by rows (N).
+template <class DT, class S, bool COS, bool SUBS, bool BACK>
+__global__ void __launch_bounds__(S::kThreadsOf, 2)
+logits_kernel(Logits a) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    LDS_PTR(char) lds = (LDS_PTR(char))smem;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+    const int wm = wave % S::WM, wn = wave / S::WM;
+    int mt, nt;
+    tile_of(xcd_item(blockIdx.x, gridDim.x), a.m_tiles, a.n_tiles, mt, nt);
+    const int c0 = a.class0 + mt * S::BM, r0 = nt * S::BN;                     // first class and row
+    const int there = min(a.class0 + a.classes, a.h.V) - c0;                   // classes of the tile that exist
+    Source<S::BM, S::kWavesOf, false> ws;
+    Source<S::BN, S::kWavesOf, false> xs;
+    xs.init(a.h.x + r0 * a.h.x_pitch, min(S::BN, a.h.N - r0), a.h.x_pitch, 2 * (int64_t)a.h.D, wave, lane);
+    Reader<false> reader;
+    reader.init(n, g);
+    const int steps = (a.h.D + kStep - 1) / kStep;
+    f32x4 acc[S::MT][S::NT];
+    f32x4 best[SUBS ? S::MT : 1][SUBS ? S::NT : 1];                            // over the sub-centres, and which
+    uint32_t which[SUBS ? S::MT : 1][SUBS ? S::NT : 1];                        // a byte to a value
+    const int first = 16 * wm * S::MT + 4 * g;                                 // this lane's class of the tile for i = 0
+#pragma unroll 1
+    for (int sub = 0; sub < (SUBS ? a.h.subs : 1); ++sub) {
+        const int64_t pitch = a.h.w_pitch * (SUBS ? a.h.subs : 1);
+        ws.init(a.h.w + c0 * pitch + sub * a.h.w_pitch, min(S::BM, there), pitch, 2 * (int64_t)a.h.D, wave, lane);
+#pragma unroll
+        for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+            for (int j = 0; j < S::NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (SUBS && sub) barrier_lds();
+        accumulate<DT, S>(acc, ws, xs, reader, reader, steps, lds, wave, wm, wn);
+        if constexpr (COS) {
+#pragma unroll
+            for (int i = 0; i < S::MT; ++i) {
+                f32x4 inv;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int c = min(first + 16 * i + r, there - 1);
+                    inv[r] = a.h.inv_w[(int64_t)(c0 + c) * (SUBS ? a.h.subs : 1) + sub];
+                }
+#pragma unroll
+                for (int j = 0; j < S::NT; ++j) {
+                    acc[i][j] *= inv;
+                    if constexpr (SUBS) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const bool better = sub == 0 || acc[i][j][r] > best[i][j][r] || acc[i][j][r] != acc[i][j][r];
+                            best[i][j][r] = better ? acc[i][j][r] : best[i][j][r];
+                            which[i][j] = sub == 0 ? 0u : better ? (which[i][j] & ~(0xffu << 8 * r)) | (uint32_t)sub << 8 * r : which[i][j];
+                        }
+                    }
+                }
+            }
+        }
+    }
+    if constexpr (SUBS) {
+#pragma unroll
+        for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+            for (int j = 0; j < S::NT; ++j) acc[i][j] = best[i][j];
+    }
+
+    if constexpr (!BACK) {
+        barrier_lds();                                                          // the operands' place is taken over
+        LDS_PTR(f32x2) met = (LDS_PTR(f32x2))lds;                             // [WM][BN]
+#pragma unroll
+        for (int j = 0; j < S::NT; ++j) {
+            const int row = 16 * (wn * S::NT + j) + n;
+            const int64_t r = min(r0 + row, a.h.N - 1);
+            const float c2 = a.h.scale2 * (COS ? a.h.inv_x[r] : 1.f);
+            if (there < S::BM) {
+#pragma unroll
+                for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) acc[i][j][k] = first + 16 * i + k < there ? acc[i][j][k] : kNegInf;
+            }
+            if (a.ids) {
+                const int64_t t = (int64_t)load_id(a.ids, r, a.ids_wide) - c0;
+                const bool hit = t >= 16 * wm * S::MT && t < 16 * (wm + 1) * S::MT;
+                if (__builtin_amdgcn_ballot_w64(hit)) {
+#pragma unroll
+                    for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) acc[i][j][k] = first + 16 * i + k == t ? kNegInf : acc[i][j][k];
+                }
+            }
+            float top = kNegInf;
+#pragma unroll
+            for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) top = __builtin_fmaxf(top, acc[i][j][k]);
+            top = xor_max(top) * c2;
+            const float off = top == kNegInf ? 0.f : top;
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][k], c2, -off));
+            sum = xor_sum(sum);
+            if (g == 0) met[wm * S::BN + row] = f32x2{top, sum};
+        }
+        barrier_lds();
+        for (int row = threadIdx.x; row < S::BN; row += S::kThreadsOf) {
+            if (r0 + row >= a.h.N) break;
+            f32x2 v = met[row];
+#pragma unroll
+            for (int i = 1; i < S::WM; ++i) {
+                const f32x2 o = met[i * S::BN + row];
+                const float top = __builtin_fmaxf(v.x, o.x), off = top == kNegInf ? 0.f : top;
+                v = f32x2{top, v.y * __builtin_amdgcn_exp2f(v.x - off) + o.y * __builtin_amdgcn_exp2f(o.x - off)};
+            }
+            a.part[(int64_t)mt * a.h.N + r0 + row] = v;
+        }
+    } else {
+        const int subs = SUBS ? a.h.subs : 1;
+        const int64_t pitch = 2 * a.plane * subs;                               // bytes of a row of dz
+        const int col = mt * S::BM + 16 * wm * S::MT;                           // this wave's first column of the range
+        const Rsrc out = make_rsrc(a.dz + r0 * pitch, (int)((int64_t)min(S::BN, a.h.N - r0) * pitch));
+        // dz for weights of length 1; in `best` stay the cosines that came with it
+        f32x4 sums[COS ? S::MT : 1];
+        if constexpr (COS)
+#pragma unroll
+            for (int i = 0; i < S::MT; ++i) sums[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < S::NT; ++j) {
+            const int row = 16 * (wn * S::NT + j) + n;
+            const int64_t r = min(r0 + row, a.h.N - 1);
+            const RowGrad rg = a.rows[r];
+            const bool exists = r0 + row < a.h.N;                               // rows behind the last have no share in the sums
+            const float c2 = a.h.scale2 * (COS ? a.h.inv_x[r] : 1.f), f = exists ? rg.f : 0.f, e = exists ? rg.at_target : 0.f;
+            const int64_t t = (int64_t)rg.target - c0;
+            const bool hit = t >= 16 * wm * S::MT && t < 16 * (wm + 1) * S::MT;
+            const bool any = __builtin_amdgcn_ballot_w64(hit) != 0;
+            const int near = SUBS && any ? a.stats[r].sub : 0;
+#pragma unroll
+            for (int i = 0; i < S::MT; ++i) {
+                f32x4 d;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) d[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][k], c2, -rg.lse2)) * f;
+                if (any) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const bool at = first + 16 * i + k == t;
+                        d[k] = at ? e : d[k];
+                        if constexpr (SUBS) which[i][j] = at ? (which[i][j] & ~(0xffu << 8 * k)) | (uint32_t)near << 8 * k : which[i][j];
+                    }
+                }
+                if (there < S::BM) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) d[k] = first + 16 * i + k < there ? d[k] : 0.f;
+                }
+                if constexpr (COS && !SUBS) sums[i] += d * acc[i][j];
+                acc[i][j] = d;
+            }
+        }
+        const int width = (int)max((int64_t)0, min((int64_t)32 * S::MT, 2 * (a.plane - col)));
+#pragma unroll 1
+        for (int sub = 0; sub < subs; ++sub) {
+            f32x4 inv[COS ? S::MT : 1];
+            if constexpr (COS)
+#pragma unroll
+                for (int i = 0; i < S::MT; ++i) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) inv[i][k] = a.h.inv_w[(int64_t)(c0 + min(first + 16 * i + k, there - 1)) * subs + sub];
+                    if constexpr (SUBS) sums[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+                }
+#pragma unroll
+            for (int j = 0; j < S::NT; ++j) {
+                u32x2 o[S::MT];
+#pragma unroll
+                for (int i = 0; i < S::MT; ++i) {
+                    f32x4 d = acc[i][j];
+                    if constexpr (SUBS) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) d[k] = (which[i][j] >> 8 * k & 0xffu) == (uint32_t)sub ? d[k] : 0.f;
+                        sums[i] += d * best[i][j];
+                    }
+                    if constexpr (COS) d *= inv[i];
+                    o[i] = narrow4<DT>(d);
+                }
+                const int at = (int)((16 * (wn * S::NT + j) + n) * pitch + 2 * (sub * a.plane + col));
+                if constexpr (S::MT == 1)
+                    __builtin_amdgcn_raw_buffer_store_b64(o[0], out, g * 8 < width ? at + g * 8 : kNowhere, 0, 0);
+                else
+                    store_tile<16 * S::MT, 0>(out, at, o, g, width);
+            }
+            if constexpr (COS)
+                if (a.col_part) {
+#pragma unroll
+                    for (int i = 0; i < S::MT; ++i) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) sums[i][k] = sum_of_16(sums[i][k]);
+                        if (n == 0 && 32 * i + 8 * g < width)
+                            *reinterpret_cast<f32x4 *>(a.col_part + ((int64_t)(nt * S::WN + wn) * subs + sub) * a.plane + col + 16 * i + 4 * g) = sums[i];
+                    }
+                }
+        }
+    }
+}
+
+// =============================================================================
+// A row's tiles put together, the target's logit, the loss
+// =============================================================================
+struct Finish {
+    Head h;
+    const f32x2 *part;
+    int m_tiles, rows;              // rows to a workgroup, a power of two up to 16
+    const void *ids;
+    int ids_wide, top;              // teacher's entries of a row, 0: targets
+    const void *teacher;
+    int teacher_type;               // NA1D_BF16, NA1D_FP16, NA1D_FP32
+    int64_t ignore;
+    int cosines;
+    float cos_m, sin_m, threshold, drop, scale, temperature;
+    RowStat *stats;
+    float *coeff;                   // teacher: p - q of every entry, [N, top]
+    float *loss;                    // [N]
+};
+__device__ inline float teacher_value(const void *p, int64_t i, int type) {
+    if (type == NA1D_FP32) return reinterpret_cast<const float *>(p)[i];
+    const uint16_t v = reinterpret_cast<const uint16_t *>(p)[i];
+    return type == NA1D_BF16 ? BF16::to_f32(v) : FP16::to_f32(v);
+}
+__device__ inline float over_wave(float x, bool max) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) {
+        const float y = __shfl_xor(x, o);
+        x = max ? __builtin_fmaxf(x, y) : x + y;
+    }
+    return x;
+}
+constexpr int kFinishThreads = 256, kMostRows = 16;
+// The derivative of the margin's cosine has the sine in its denominator; it is bounded there.
+constexpr float kLeastSine2 = 1e-6f;
+
+template <class DT>
+__global__ void __launch_bounds__(kFinishThreads)
+finish_kernel(Finish a) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    f32x2 *met = reinterpret_cast<f32x2 *>(smem);                             // [lanes][rows]: 256 of them
+    float *z = reinterpret_cast<float *>(smem + kFinishThreads * sizeof(f32x2));     // [rows][entries], log2 domain
+    float *lse = z + a.rows * (a.top ? a.top : a.h.subs);                       // [rows]
+    const int R = a.rows, lanes = kFinishThreads / R, r = threadIdx.x & (R - 1), l = threadIdx.x / R;
+    const int64_t r0 = (int64_t)blockIdx.x * R;
+    {
+        f32x2 v = {kNegInf, 0.f};
+        const int64_t row = min(r0 + r, (int64_t)a.h.N - 1);
+        for (int t = l; t < a.m_tiles; t += lanes) {
+            const f32x2 o = a.part[(int64_t)t * a.h.N + row];
+            const float top = __builtin_fmaxf(v.x, o.x), off = top == kNegInf ? 0.f : top;
+            v = f32x2{top, v.y * __builtin_amdgcn_exp2f(v.x - off) + o.y * __builtin_amdgcn_exp2f(o.x - off)};
+        }
+        met[threadIdx.x] = v;
+    }
+    // logits of the entries: 16 lanes to an entry
+    const int entries = a.top ? a.top : a.h.subs, lane16 = threadIdx.x & 15;
+    for (int e = threadIdx.x >> 4; e < R * entries; e += kFinishThreads / 16) {
+        const int64_t row = r0 + e / entries;
+        const int k = e % entries;
+        float s = 0.f;
+        if (row < a.h.N) {
+            const int id = load_id(a.ids, a.top ? row * a.top + k : row, a.ids_wide);
+            if (id >= 0 && id < a.h.V) {
+                const int64_t wr = a.top ? id : (int64_t)id * a.h.subs + k;
+                const char *xr = a.h.x + row * a.h.x_pitch, *w = a.h.w + wr * a.h.w_pitch;
+#pragma unroll 2
+                for (int c = lane16 * 8; c < a.h.D; c += 128) {
+                    const u32x4 p = *reinterpret_cast<const u32x4 *>(xr + 2 * c), q = *reinterpret_cast<const u32x4 *>(w + 2 * c);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const f32x2 u = widen<DT>(p[i]), v = widen<DT>(q[i]);
+                        s = __builtin_fmaf(u.x, v.x, s);
+                        s = __builtin_fmaf(u.y, v.y, s);
+                    }
+                }
+                if (a.cosines) s *= a.h.inv_w[wr];
+            }
+        }
+        s = sum_of_16(s);
+        if (lane16 == 0) z[e] = s;
+    }
+    __syncthreads();
+    // The tiles' sums meet, R rows at a time.
+    for (int half = lanes / 2; half; half >>= 1) {
+        if (l < half) {
+            const f32x2 v = met[threadIdx.x], o = met[threadIdx.x + half * R];
+            const float top = __builtin_fmaxf(v.x, o.x), off = top == kNegInf ? 0.f : top;
+            met[threadIdx.x] = f32x2{top, v.y * __builtin_amdgcn_exp2f(v.x - off) + o.y * __builtin_amdgcn_exp2f(o.x - off)};
+        }
+        __syncthreads();
+    }
+    if ((int)threadIdx.x < R) lse[threadIdx.x] = met[threadIdx.x].x + __builtin_log2f(met[threadIdx.x].y);
+    __syncthreads();
+    if (!a.top) {
+        const int64_t row = r0 + threadIdx.x;
+        if ((int)threadIdx.x >= R || row >= a.h.N) return;
+        const int64_t raw = a.ids_wide ? reinterpret_cast<const int64_t *>(a.ids)[row] : (int64_t)reinterpret_cast<const int32_t *>(a.ids)[row];
+        RowStat st = {__builtin_inff(), 0.f, kFar, -1};
+        float loss = raw == a.ignore ? 0.f : __builtin_nanf("");
+        if (raw != a.ignore && raw >= 0 && raw < a.h.V) {
+            float best = z[threadIdx.x * entries], slope = 1.f;
+            st.sub = 0;
+            for (int k = 1; k < entries; ++k)
+                if (z[threadIdx.x * entries + k] > best) best = z[threadIdx.x * entries + k], st.sub = k;
+            if (a.cosines) {
+                const float c = best * a.h.inv_x[row], sine2 = 1.f - c * c;
+                best = c;
+                if (c > a.threshold) {
+                    best = c * a.cos_m - __builtin_sqrtf(__builtin_fmaxf(sine2, 0.f)) * a.sin_m;
+                    slope = a.cos_m + a.sin_m * c / __builtin_sqrtf(__builtin_fmaxf(sine2, kLeastSine2));
+                } else if (c <= a.threshold) {
+                    best = c - a.drop;
+                }
+            }
+            const float zt = best * a.h.scale2, others = lse[threadIdx.x], d = others - zt;         // log2 domain
+            const float e = __builtin_amdgcn_exp2f(-__builtin_fabsf(d)), more = log1pf(e);
+            loss = __builtin_fmaxf(d, 0.f) * kLn2 + more;
+            if (d != d) loss = d;
+            st.lse2 = (d > 0.f ? others : zt) + more * kLog2e;
+            st.at_target = -(d > 0.f ? 1.f : e) / (1.f + e) * slope;
+            st.target = (int)raw;
+        }
+        a.stats[row] = st;
+        a.loss[row] = loss;
+        return;
+    }
+    // A teacher's row: a wave to each.
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int q0 = wave; q0 < R; q0 += kFinishThreads / 64) {
+        const int64_t row = r0 + q0;
+        if (row >= a.h.N) break;
+        constexpr int kEach = NA1D_HEAD_MAX_TOP / 64;
+        int id[kEach];
+        float t[kEach], q[kEach], top = kNegInf;
+        bool bad = false, nan = false;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int k = i * 64 + lane;
+            id[i] = k < a.top ? load_id(a.ids, row * a.top + k, a.ids_wide) : -1;
+            bad |= id[i] >= a.h.V;
+            t[i] = id[i] >= 0 && id[i] < a.h.V ? teacher_value(a.teacher, row * a.top + k, a.teacher_type) * (1.f / a.temperature) : kNegInf;
+            nan |= t[i] != t[i];
+            top = __builtin_fmaxf(top, t[i]);
+        }
+        top = over_wave(top, true);
+        float total = 0.f;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) total += q[i] = t[i] == kNegInf ? 0.f : __builtin_amdgcn_exp2f((t[i] - top) * kLog2e);
+        total = over_wave(total, false);
+        bad = __builtin_amdgcn_ballot_w64(bad) != 0;
+        nan = __builtin_amdgcn_ballot_w64(nan) != 0;
+        RowStat st = {__builtin_inff(), 0.f, kFar, -1};
+        float loss = bad ? __builtin_nanf("") : 0.f;
+        const bool counts = !bad && (top > kNegInf || nan);
+        const float log_total = __builtin_log2f(total), lse2 = lse[q0];
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int k = i * 64 + lane;
+            if (k >= a.top) continue;
+            const float z2 = z[q0 * a.top + k] * a.h.scale2, p = __builtin_amdgcn_exp2f(z2 - lse2);
+            q[i] /= total;
+            if (t[i] != kNegInf) sum += q[i] == 0.f ? 0.f : q[i] * ((t[i] - top) * kLog2e - log_total - (z2 - lse2));
+            float same = 0.f;                                                   // an entry that is there twice has both shares
+            for (int m = 0; m < a.top; ++m) {
+                const int64_t at = row * a.top + m;
+                if (load_id(a.ids, at, a.ids_wide) == id[i]) {
+                    const float u = teacher_value(a.teacher, at, a.teacher_type) * (1.f / a.temperature);
+                    same += u == kNegInf ? 0.f : __builtin_amdgcn_exp2f((u - top) * kLog2e);
+                }
+            }
+            a.coeff[row * a.top + k] = counts && id[i] >= 0 ? p - same / total : 0.f;
+        }
+        sum = over_wave(sum, false);
+        if (counts) {
+            loss = sum * kLn2 * a.temperature * a.temperature;
+            st.lse2 = lse2;
+            st.sub = 0;
+        }
+        if (lane == 0) a.stats[row] = st, a.loss[row] = loss;
+    }
+}
+
+// Sum or mean of the rows' losses; and of how many rows.
+__global__ void __launch_bounds__(1024)
+reduce_kernel(float *__restrict__ loss, float *__restrict__ count, const float *__restrict__ rows, const RowStat *__restrict__ stats, int N, int mean) {
+    __shared__ double sums[16];
+    __shared__ int counts[16];
+    double s = 0.0;
+    int c = 0;
+    for (int r = threadIdx.x; r < N; r += 1024) {
+        s += (double)rows[r];
+        c += stats[r].sub >= 0;
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o), c += __shfl_xor(c, o);
+    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s, counts[threadIdx.x >> 6] = c;
+    __syncthreads();
+    if (threadIdx.x) return;
+    for (int i = 1; i < 16; ++i) s += sums[i], c += counts[i];
+    *count = (float)(c > 1 ? c : 1);
+    *loss = (float)(mean ? s / (double)(c > 1 ? c : 1) : s);
+}
+
+// =============================================================================
+// Backward
+// =============================================================================
+struct Rows {
+    RowGrad *rows;
+    float *unscale;
+    const RowStat *stats;
+    const float *dloss, *count, *inv_x, *most_w;      // count NULL: dloss has a value for every row
+    int N, most_count, mean, half;
+    float factor;
+};
+// What a row multiplies its probabilities by.  fp16 gradients of single logits would be lost below 6e-8: they are multiplied by the
+// power of two that brings the largest that may come to 2^13 or more, which the products' ends take away again.
+__global__ void __launch_bounds__(1024)
+rows_kernel(Rows a) {
+    __shared__ float tops[16];
+    auto factor = [&](int r) {
+        const RowStat st = a.stats[r];
+        if (st.sub < 0) return 0.f;
+        float f = a.factor * (a.count ? a.dloss[0] / (a.mean ? a.count[0] : 1.f) : a.dloss[r]);
+        if (a.inv_x) f = a.inv_x[r] == kNoNorm ? 0.f : f * a.inv_x[r];
+        return f;
+    };
+    float scale = 1.f;
+    if (a.half) {
+        float top = 0.f, most = a.most_w ? 0.f : 1.f;
+        for (int r = threadIdx.x; r < a.N; r += 1024) {
+            const float f = __builtin_fabsf(factor(r));
+            top = __builtin_fmaxf(top, f * __builtin_fmaxf(1.f, __builtin_fabsf(a.stats[r].at_target)));
+        }
+        for (int i = threadIdx.x; i < a.most_count; i += 1024) most = __builtin_fmaxf(most, a.most_w[i]);
+        top = over_wave(top, true);
+        most = over_wave(most, true);
+        __shared__ float mosts[16];
+        if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top, mosts[threadIdx.x >> 6] = most;
+        __syncthreads();
+        for (int i = 0; i < 16; ++i) top = __builtin_fmaxf(top, tops[i]), most = __builtin_fmaxf(most, mosts[i]);
+        top *= most;
+        if (top > 0.f && top < 3.0e38f) scale = __builtin_ldexpf(1.f, max(-120, min(120, 13 + 127 - (int)(__float_as_uint(top) >> 23))));
+    }
+    if (threadIdx.x == 0 && blockIdx.x == 0) *a.unscale = 1.f / scale;
+    for (int r = blockIdx.x * 1024 + threadIdx.x; r < a.N; r += gridDim.x * 1024) {
+        const RowStat st = a.stats[r];
+        const float f = factor(r) * scale;
+        a.rows[r] = RowGrad{st.lse2, f, f * st.at_target, st.target};
+    }
+}
+
+// The teacher's entries of dz, which the logits' kernel left as those of any class.  Entries of one class write the same value.
+template <class DT>
+__global__ void __launch_bounds__(256)
+entries_kernel(uint16_t *__restrict__ dz, const float *__restrict__ coeff, const RowGrad *__restrict__ rows, const void *__restrict__ ids, int ids_wide, int N, int top,
+               int class0, int classes, int64_t plane) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= (int64_t)N * top) return;
+    const int64_t row = i / top, c = (int64_t)load_id(ids, i, ids_wide) - class0;
+    if (c < 0 || c >= classes) return;
+    dz[row * plane + c] = (uint16_t)Mma<DT>::pack(coeff[i] * rows[row].f, 0.f);
+}
+
+// dx (fp32, all ranges' and splits' shares): x rows (N side) by channels (M side), contracted over a range's classes; and dW:
+// weight rows by channels, contracted over the rows.
+struct Product {
+    const char *dz, *other;         // other: W, or x
+    int64_t plane, other_pitch;     // of dz; bytes from one row of `other` to the next
+    int N, D, subs;
+    int classes, columns, class0;   // of this range; its columns of dz, whole steps
+    int m_tiles, n_tiles, splits, per;          // per: of the contraction to a split, a multiple of kStep
+    float *part;                    // fp32 [splits, rows, D]
+    int64_t part_stride;
+    int add;                        // to what is there
+    // dW without splits
+    char *out;                      // 16-bit [V * subs, D], or NULL: to part
+    const float *unscale;
+    const char *w;                  // cosines: dW loses its part along w
+    int64_t w_pitch;
+    const float *inv_w, *col_part;
+    int col_parts;
+};
+template <class DT, class S, bool DW>
+__global__ void __launch_bounds__(S::kThreadsOf, 2)
+product_kernel(Product a) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    LDS_PTR(char) lds = (LDS_PTR(char))smem;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+    const int wm = wave % S::WM, wn = wave / S::WM;
+    const uint32_t item = xcd_item(blockIdx.x, gridDim.x), mt = item % (uint32_t)a.m_tiles, rest = item / (uint32_t)a.m_tiles;
+    const int nt = (int)(rest % (uint32_t)a.n_tiles), split = (int)(rest / (uint32_t)a.n_tiles);
+    const int d0 = (int)mt * S::BM;
+    const int64_t pitch = 2 * a.plane * a.subs;
+    f32x4 acc[S::MT][S::NT];
+#pragma unroll
+    for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+        for (int j = 0; j < S::NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    Reader<true> turned;
+    turned.init(n, g);
+    Source<S::BM, S::kWavesOf, true> as;
+    const int tiles_of_plane = DW ? a.n_tiles / a.subs : 1;
+    const int sub = DW ? nt / tiles_of_plane : 0, col0 = DW ? (nt - sub * tiles_of_plane) * S::BN : 0, r0 = DW ? 0 : nt * S::BN;
+    if constexpr (DW) {
+        const int64_t first = (int64_t)split * a.per, rows = min((int64_t)a.per, a.N - first);
+        Source<S::BN, S::kWavesOf, true> bs;
+        as.init(a.other + first * a.other_pitch + 2 * d0, rows, a.other_pitch, 2 * (int64_t)(a.D - d0), wave, lane);
+        bs.init(a.dz + first * pitch + 2 * (sub * a.plane + col0), rows, pitch, 2 * (a.plane - col0), wave, lane);
+        accumulate<DT, S>(acc, as, bs, turned, turned, (int)((rows + kStep - 1) / kStep), lds, wave, wm, wn);
+    } else {
+        Reader<false> straight;
+        straight.init(n, g);
+        Source<S::BN, S::kWavesOf, false> bs;
+        const int first = split * a.per, wide = min(a.per, a.columns - first);
+#pragma unroll 1
+        for (int k = 0; k < a.subs; ++k) {
+            if (k) barrier_lds();
+            as.init(a.other + ((int64_t)(a.class0 + first) * a.subs + k) * a.other_pitch + 2 * d0, min(wide, a.classes - first), a.other_pitch * a.subs,
+                    2 * (int64_t)(a.D - d0), wave, lane);
+            bs.init(a.dz + r0 * pitch + 2 * (k * a.plane + first), min(S::BN, a.N - r0), pitch, 2 * (int64_t)wide, wave, lane);
+            accumulate<DT, S>(acc, as, bs, turned, straight, (wide + kStep - 1) / kStep, lds, wave, wm, wn);
+        }
+    }
+    const int m0 = d0 + 16 * wm * S::MT;                                        // this wave's channels
+    if (DW && a.out) {
+        const float unscale = *a.unscale;
+        const int left = a.classes - col0;                                      // classes of the tile
+        const int64_t row0 = (int64_t)(a.class0 + col0) * a.subs + sub;
+        const int out_pitch = 2 * a.D * a.subs, width = max(0, min(32 * S::MT, 2 * (a.D - m0)));
+        const Rsrc os = make_rsrc(a.out + row0 * 2 * a.D, left > 0 ? (int)min((int64_t)(min(left, S::BN) - 1) * out_pitch + 2 * a.D, (int64_t)1 << 30) : 0);
+        const Rsrc wr = make_rsrc(a.w ? a.w + row0 * a.w_pitch : a.other, a.w && left > 0 ? (int)((min(left, S::BN) - 1) * a.w_pitch * a.subs + 2 * a.D) : 0);
+#pragma unroll
+        for (int j = 0; j < S::NT; ++j) {
+            const int c = 16 * (wn * S::NT + j) + n;
+            float along = 0.f;
+            if (a.w && c < left) {
+                for (int p = 0; p < a.col_parts; ++p) along += a.col_part[((int64_t)p * a.subs + sub) * a.plane + col0 + c];
+                const float inv = a.inv_w[row0 + (int64_t)c * a.subs];
+                along *= inv == kNoNorm ? 0.f : inv * inv;
+            }
+            const float f = a.w && c < left && a.inv_w[row0 + (int64_t)c * a.subs] == kNoNorm ? 0.f : unscale;
+            u32x2 o[S::MT];
+#pragma unroll
+            for (int i = 0; i < S::MT; ++i) {
+                f32x4 v = acc[i][j];
+                if (a.w) {
+                    const int at = 32 * i + 8 * g;
+                    v -= along * widen4<DT>(__builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(wr, at < width ? (int)(c * a.w_pitch * a.subs) + 2 * m0 + at : kNowhere, 0, 0)));
+                }
+                o[i] = narrow4<DT>(v * f);
+            }
+            if constexpr (S::MT == 1)
+                __builtin_amdgcn_raw_buffer_store_b64(o[0], os, g * 8 < width ? c * out_pitch + 2 * m0 + g * 8 : kNowhere, 0, 0);
+            else
+                store_tile<16 * S::MT, 0>(os, c * out_pitch + 2 * m0, o, g, width);
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < S::NT; ++j) {
+        const int in = 16 * (wn * S::NT + j) + n;
+        const int64_t row = DW ? (int64_t)(a.class0 + col0 + in) * a.subs + sub : r0 + in;
+        if (DW ? col0 + in >= a.classes : r0 + in >= a.N) continue;
+        float *to = a.part + split * a.part_stride + row * a.D;
+#pragma unroll
+        for (int i = 0; i < S::MT; ++i) {
+            const int d = m0 + 16 * i + 4 * g;
+            if (d >= a.D) continue;
+            f32x4 v = acc[i][j];
+            if (a.add) v += *reinterpret_cast<const f32x4 *>(to + d);
+            *reinterpret_cast<f32x4 *>(to + d) = v;
+        }
+    }
+}
+
+// The shares of all splits of a row put together (a wave to a row), less their part along the row's own vector (cosines).
+struct Fold {
+    char *out;
+    const float *part;
+    int64_t stride, rows;
+    int splits, D;
+    const float *unscale;
+    const char *own;                // cosines: the rows themselves, and 1 / their length
+    int64_t own_pitch;
+    const float *inv;
+};
+template <class DT>
+__global__ void __launch_bounds__(256)
+fold_kernel(Fold a) {
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= a.rows) return;
+    const float *part = a.part + row * a.D;
+    float f = *a.unscale;
+    auto sum = [&](int d) {
+        f32x4 v = *reinterpret_cast<const f32x4 *>(part + d);
+#pragma unroll 4
+        for (int s = 1; s < a.splits; ++s) v += *reinterpret_cast<const f32x4 *>(part + s * a.stride + d);
+        return v;
+    };
+    auto own = [&](int d) { return widen4<DT>(*reinterpret_cast<const u32x2 *>(a.own + row * a.own_pitch + 2 * d)); };
+    float along = 0.f;
+    if (a.own) {
+        for (int d = lane * 4; d < a.D; d += 256) {
+            const f32x4 v = sum(d) * own(d);
+            along += v[0] + v[1] + (v[2] + v[3]);
+        }
+        const float inv = a.inv[row];
+        along = over_wave(along, false) * inv * inv;
+        if (inv == kNoNorm) f = 0.f, along = 0.f;
+    }
+    for (int d = lane * 4; d < a.D; d += 256) {
+        f32x4 v = sum(d);
+        if (a.own) v -= along * own(d);
+        *reinterpret_cast<u32x2 *>(a.out + (row * a.D + d) * 2) = narrow4<DT>(v * f);
+    }
+}
+__global__ void __launch_bounds__(256)
+clear_kernel(u32x4 *__restrict__ out, int64_t units) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i < units) out[i] = u32x4{0, 0, 0, 0};
+}
+
+// =============================================================================
+// Plans and launches
+// =============================================================================
+template <class T> inline T ceil_div(T a, T b) { return (a + b - 1) / b; }
+inline int64_t round_up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
+constexpr int kNormBlocks = 1024;
+
+// Places of the forward's results in `saved`, which the backward reads.
+struct Saved {
+    int64_t count, stats, coeff, inv_x, inv_w, most, bytes;
+    explicit Saved(const na1d_head &h) {
+        int64_t at = 0;
+        auto take = [&](int64_t n) { const int64_t p = at; at += round_up(n, 256); return p; };
+        const bool cosines = h.kind == NA1D_HEAD_MARGIN, teacher = h.kind == NA1D_HEAD_TEACHER;
+        count = take(16);
+        stats = take(h.N * (int64_t)sizeof(RowStat));
+        coeff = take(teacher ? 4 * h.N * h.top : 0);
+        inv_x = take(cosines ? 4 * h.N : 0);
+        inv_w = take(cosines ? 4 * h.V * h.subcenters : 0);
+        most = take(cosines ? 4 * kNormBlocks : 0);
+        bytes = at;
+    }
+};
+
+// Tile shapes: classes by rows of the logits, channels by rows (dx) or weight rows (dW) of the products.
+using Few = Shape<1, 2, 4, 1, 4>;             // 64 x 32
+using Batch = Shape<2, 4, 2, 2, 3>;           // 64 x 128
+using Many = Shape<4, 4, 2, 2, 2>;            // 128 x 128
+
+enum Pick { kFew, kBatch, kMany };
+struct Plan {
+    Pick logits, dx, dw;
+    int bm, bn;                               // of the logits' tiles
+    int wn;                                   // waves along the rows
+    int64_t m_tiles;
+    // backward: ranges of classes
+    int64_t plane;                            // columns to a sub-centre: a range's classes, rounded up to whole steps
+    int64_t ranges;
+    int dx_bm, dx_bn, dx_splits, dx_per;
+    int dw_bm, dw_bn, dw_splits, dw_per;
+};
+constexpr int64_t kMostDz = 256ll << 20;      // bytes of dz: what the last level of cache holds
+constexpr int kFullLaunch = 512;              // workgroups: two to a CU
+inline void shape_of(Pick p, int &bm, int &bn) { bm = p == kMany ? 128 : 64, bn = p == kFew ? 32 : 128; }
+inline Plan plan_of(const na1d_head &h) {
+    Plan p{};
+    p.logits = h.N <= 32 ? kFew : ceil_div<int64_t>(h.V, 128) * ceil_div<int64_t>(h.N, 128) < kFullLaunch || h.subcenters > 1 ? kBatch : kMany;     // two sets of sums
+    shape_of(p.logits, p.bm, p.bn);
+    p.wn = p.logits == kFew ? 1 : 2;
+    p.m_tiles = ceil_div<int64_t>(h.V, p.bm);
+    const int64_t fits = std::min<int64_t>(kMostDz / (2 * h.N * h.subcenters), (1 << 20) / h.subcenters);
+    p.plane = std::min(round_up(h.V, kStep), std::max<int64_t>(fits / 256 * 256, 256));
+    p.ranges = ceil_div(h.V, p.plane);
+    const bool narrow = round_up(h.D, 64) < round_up(h.D, 128);
+    p.dx = h.N <= 32 ? kFew : narrow ? kBatch : kMany;
+    shape_of(p.dx, p.dx_bm, p.dx_bn);
+    const int64_t dx_tiles = ceil_div<int64_t>(h.D, p.dx_bm) * ceil_div<int64_t>(h.N, p.dx_bn);
+    auto split = [&](int64_t tiles, int64_t length, int &splits, int &per) {
+        const int64_t steps = ceil_div<int64_t>(length, kStep), want = std::max<int64_t>(1, std::min<int64_t>(kFullLaunch / tiles, steps / 4));
+        per = (int)(ceil_div(steps, want) * kStep);
+        splits = (int)ceil_div<int64_t>(length, per);
+    };
+    split(dx_tiles, p.plane, p.dx_splits, p.dx_per);
+    p.dw = narrow ? kBatch : kMany;
+    shape_of(p.dw, p.dw_bm, p.dw_bn);
+    const int64_t dw_tiles = ceil_div<int64_t>(h.D, p.dw_bm) * h.subcenters * ceil_div<int64_t>(p.plane, p.dw_bn);
+    split(dw_tiles, h.N, p.dw_splits, p.dw_per);
+    return p;
+}
+struct ForwardScratch {
+    int64_t part, rows, bytes;
+    ForwardScratch(const na1d_head &h, const Plan &p) {
+        part = 0;
+        rows = round_up(p.m_tiles * h.N * (int64_t)sizeof(f32x2), 256);
+        bytes = rows + round_up(4 * h.N, 256);
+    }
+};
+struct BackwardScratch {
+    int64_t unscale, rows, dz, dx, dw, cols, bytes;
+    BackwardScratch(const na1d_head &h, const Plan &p) {
+        int64_t at = 0;
+        auto take = [&](int64_t n) { const int64_t q = at; at += round_up(n, 256); return q; };
+        unscale = take(16);
+        rows = take(h.N * (int64_t)sizeof(RowGrad));
+        dz = take(2 * h.N * h.subcenters * p.plane);
+        dx = take(4 * h.N * h.D * p.dx_splits);
+        dw = take(p.dw_splits > 1 ? 4 * h.V * h.subcenters * h.D * p.dw_splits : 0);
+        cols = take(h.kind == NA1D_HEAD_MARGIN && p.dw_splits == 1 ? 4 * ceil_div<int64_t>(h.N, p.bn) * p.wn * h.subcenters * p.plane : 0);
+        bytes = at;
+    }
+};
+
+#define NA1D_TRY(x)                      \
+    do {                                 \
+        const int st_ = (x);             \
+        if (st_ != NA1D_OK) return st_;  \
+    } while (0)
+
+template <class K, class A> int launch(K kern, unsigned grid, unsigned block, size_t lds, hipStream_t s, const A &a) {
+    if (!allow_lds(kern, lds)) return NA1D_ERR_LAUNCH;
+    kern<<<grid, block, lds, s>>>(a);
+    return launch_status();
+}
+template <class DT, class S, bool BACK> int launch_logits_of(const na1d_head &h, const Logits &a, hipStream_t s) {
+    const unsigned grid = (unsigned)(a.m_tiles * a.n_tiles);
+    if (h.kind != NA1D_HEAD_MARGIN) return launch(logits_kernel<DT, S, false, false, BACK>, grid, S::kThreadsOf, S::kLds, s, a);
+    if (h.subcenters == 1) return launch(logits_kernel<DT, S, true, false, BACK>, grid, S::kThreadsOf, S::kLds, s, a);
+    if constexpr (S::MT * S::NT <= 8) return launch(logits_kernel<DT, S, true, true, BACK>, grid, S::kThreadsOf, S::kLds, s, a);
+    return NA1D_ERR_UNSUPPORTED;
+}
+template <class DT, bool BACK> int launch_logits(const na1d_head &h, const Plan &p, Logits a, hipStream_t s) {
+    a.m_tiles = (int)ceil_div(a.classes, p.bm);
+    a.n_tiles = (int)ceil_div<int64_t>(h.N, p.bn);
+    return p.logits == kFew ? launch_logits_of<DT, Few, BACK>(h, a, s) : p.logits == kBatch ? launch_logits_of<DT, Batch, BACK>(h, a, s) : launch_logits_of<DT, Many, BACK>(h, a, s);
+}
+template <class DT, bool DW> int launch_product(Pick pick, const Product &a, hipStream_t s) {
+    const unsigned grid = (unsigned)((int64_t)a.m_tiles * a.n_tiles * a.splits);
+    if constexpr (!DW)
+        if (pick == kFew) return launch(product_kernel<DT, Few, DW>, grid, Few::kThreadsOf, Few::kLds, s, a);
+    if (pick == kBatch) return launch(product_kernel<DT, Batch, DW>, grid, Batch::kThreadsOf, Batch::kLds, s, a);
+    return launch(product_kernel<DT, Many, DW>, grid, Many::kThreadsOf, Many::kLds, s, a);
+}
+inline Head head_of(const na1d_head &h, const void *x, const void *w, const char *saved, const Saved &o) {
+    const bool cosines = h.kind == NA1D_HEAD_MARGIN;
+    const float scale = h.kind == NA1D_HEAD_TEACHER ? 1.f / h.scale : h.scale;             // a teacher's is the temperature
+    return Head{(const char *)x, (const char *)w, 2 * h.x_stride, 2 * h.w_stride, (int)h.N, (int)h.V, (int)h.D, h.subcenters, scale * kLog2e,
+                cosines ? reinterpret_cast<const float *>(saved + o.inv_x) : nullptr, cosines ? reinterpret_cast<const float *>(saved + o.inv_w) : nullptr};
+}
+
+template <class DT>
+int forward(const na1d_head &h, float *loss, const void *x, const void *w, const void *ids, const void *teacher, char *saved, char *ws, hipStream_t s) {
+    const Saved o(h);
+    const Plan p = plan_of(h);
+    const ForwardScratch f(h, p);
+    const bool cosines = h.kind == NA1D_HEAD_MARGIN, teaches = h.kind == NA1D_HEAD_TEACHER;
+    Logits a{};
+    a.h = head_of(h, x, w, saved, o);
+    if (cosines) {
+        norms_kernel<DT><<<kNormBlocks, 256, 0, s>>>(reinterpret_cast<float *>(saved + o.inv_x), reinterpret_cast<float *>(saved + o.inv_w),
+                                                     reinterpret_cast<float *>(saved + o.most), a.h.x, a.h.w, a.h.x_pitch, a.h.w_pitch, h.N, h.V * h.subcenters, (int)h.D);
+        NA1D_TRY(launch_status());
+    }
+    a.classes = (int)h.V;
+    a.part = reinterpret_cast<f32x2 *>(ws + f.part);
+    a.ids = teaches ? nullptr : ids, a.ids_wide = h.ids_64;
+    NA1D_TRY((launch_logits<DT, false>(h, p, a, s)));
+    Finish e{};
+    e.h = a.h, e.part = a.part, e.m_tiles = (int)p.m_tiles;
+    e.rows = h.N >= 4096 ? 16 : h.N >= 1024 ? 4 : 1;
+    e.ids = ids, e.ids_wide = h.ids_64, e.top = teaches ? h.top : 0, e.teacher = teacher, e.teacher_type = h.teacher_type;
+    e.ignore = h.ignore_index, e.cosines = cosines, e.scale = h.scale, e.temperature = h.scale;
+    e.cos_m = (float)cos(h.margin), e.sin_m = (float)sin(h.margin), e.threshold = (float)cos(M_PI - h.margin), e.drop = (float)(sin(M_PI - h.margin) * h.margin);
+    e.stats = reinterpret_cast<RowStat *>(saved + o.stats), e.coeff = reinterpret_cast<float *>(saved + o.coeff);
+    float *rows = reinterpret_cast<float *>(ws + f.rows);
+    e.loss = h.reduction == NA1D_HEAD_NONE ? loss : rows;
+    const size_t lds = kFinishThreads * sizeof(f32x2) + 4 * (size_t)e.rows * ((teaches ? h.top : h.subcenters) + 1);
+    NA1D_TRY(launch(finish_kernel<DT>, (unsigned)ceil_div<int64_t>(h.N, e.rows), kFinishThreads, lds, s, e));
+    if (h.reduction == NA1D_HEAD_NONE) return NA1D_OK;
+    reduce_kernel<<<1, 1024, 0, s>>>(loss, reinterpret_cast<float *>(saved + o.count), rows, e.stats, (int)h.N, h.reduction == NA1D_HEAD_MEAN);
+    return launch_status();
+}
+
+template <class DT>
+int backward(const na1d_head &h, char *dx, char *dw, const float *dloss, const void *x, const void *w, const void *ids, const char *saved, char *ws, hipStream_t s) {
+    const Saved o(h);
+    const Plan p = plan_of(h);
+    const BackwardScratch b(h, p);
+    const bool cosines = h.kind == NA1D_HEAD_MARGIN;
+    float *unscale = reinterpret_cast<float *>(ws + b.unscale);
+    const RowStat *stats = reinterpret_cast<const RowStat *>(saved + o.stats);
+    Logits a{};
+    a.h = head_of(h, x, w, saved, o);
+    Rows r{};
+    r.rows = reinterpret_cast<RowGrad *>(ws + b.rows), r.unscale = unscale, r.stats = stats, r.dloss = dloss;
+    r.count = h.reduction == NA1D_HEAD_NONE ? nullptr : reinterpret_cast<const float *>(saved + o.count);
+    r.inv_x = a.h.inv_x, r.most_w = cosines ? reinterpret_cast<const float *>(saved + o.most) : nullptr, r.most_count = cosines ? kNormBlocks : 0;
+    r.N = (int)h.N, r.mean = h.reduction == NA1D_HEAD_MEAN, r.half = DT::tag == NA1D_FP16;
+    r.factor = h.scale;                                                                   // a teacher's: temperature^2 / temperature
+    rows_kernel<<<r.half ? 1 : (unsigned)ceil_div<int64_t>(h.N, 1024), 1024, 0, s>>>(r);
+    NA1D_TRY(launch_status());
+    a.rows = r.rows, a.stats = stats, a.dz = ws + b.dz, a.plane = p.plane;
+    a.col_part = cosines && dw && p.dw_splits == 1 ? reinterpret_cast<float *>(ws + b.cols) : nullptr;
+    Product g{};
+    g.dz = a.dz, g.plane = p.plane, g.N = (int)h.N, g.D = (int)h.D, g.subs = h.subcenters, g.unscale = unscale;
+    for (int64_t range = 0; range < p.ranges; ++range) {
+        a.class0 = g.class0 = (int)(range * p.plane);
+        a.classes = g.classes = (int)std::min(p.plane, h.V - a.class0);
+        g.columns = (int)round_up(a.classes, kStep);
+        NA1D_TRY((launch_logits<DT, true>(h, p, a, s)));
+        if (h.kind == NA1D_HEAD_TEACHER) {
+            entries_kernel<DT><<<(unsigned)ceil_div<int64_t>(h.N * h.top, 256), 256, 0, s>>>(
+                (uint16_t *)a.dz, reinterpret_cast<const float *>(saved + o.coeff), r.rows, ids, h.ids_64, (int)h.N, h.top, a.class0, a.classes, p.plane);
+            NA1D_TRY(launch_status());
+        }
+        if (dx) {
+            g.other = a.h.w, g.other_pitch = a.h.w_pitch;
+            g.m_tiles = (int)ceil_div<int64_t>(h.D, p.dx_bm), g.n_tiles = (int)ceil_div<int64_t>(h.N, p.dx_bn), g.splits = p.dx_splits, g.per = p.dx_per;
+            g.part = reinterpret_cast<float *>(ws + b.dx), g.part_stride = h.N * h.D, g.add = range > 0, g.out = nullptr;
+            NA1D_TRY((launch_product<DT, false>(p.dx, g, s)));
+        }
+        if (dw) {
+            g.other = a.h.x, g.other_pitch = a.h.x_pitch;
+            g.m_tiles = (int)ceil_div<int64_t>(h.D, p.dw_bm), g.n_tiles = (int)(h.subcenters * ceil_div(g.columns, p.dw_bn)), g.splits = p.dw_splits, g.per = p.dw_per;
+            g.part = reinterpret_cast<float *>(ws + b.dw), g.part_stride = h.V * h.subcenters * h.D, g.add = 0, g.out = p.dw_splits == 1 ? dw : nullptr;
+            g.w = cosines ? a.h.w : nullptr, g.w_pitch = a.h.w_pitch, g.inv_w = a.h.inv_w, g.col_part = a.col_part, g.col_parts = (int)ceil_div<int64_t>(h.N, p.bn) * p.wn;
+            NA1D_TRY((launch_product<DT, true>(p.dw, g, s)));
+        }
+    }
+    auto fold = [&](char *out, int64_t part, int64_t rows, int splits, const char *own, int64_t own_pitch, const float *inv) {
+        const Fold f{out, reinterpret_cast<const float *>(ws + part), rows * h.D, rows, splits, (int)h.D, unscale, cosines ? own : nullptr, own_pitch, inv};
+        return launch(fold_kernel<DT>, (unsigned)ceil_div<int64_t>(rows, 4), 256, 0, s, f);
+    };
+    if (dx) NA1D_TRY(fold(dx, b.dx, h.N, p.dx_splits, a.h.x, a.h.x_pitch, a.h.inv_x));
+    if (dw && p.dw_splits > 1) NA1D_TRY(fold(dw, b.dw, h.V * h.subcenters, p.dw_splits, a.h.w, a.h.w_pitch, a.h.inv_w));
+    return NA1D_OK;
+}
+
+int64_t saved_bytes(const na1d_head &h) { return Saved(h).bytes; }
+int64_t scratch_bytes(const na1d_head &h, bool back) {
+    const Plan p = plan_of(h);
+    return back ? BackwardScratch(h, p).bytes : ForwardScratch(h, p).bytes;
+}
+int run_forward(const na1d_head &h, float *loss, const void *x, const void *w, const void *ids, const void *teacher, void *saved, void *ws, hipStream_t s) {
+    return h.dtype == NA1D_BF16 ? forward<BF16>(h, loss, x, w, ids, teacher, (char *)saved, (char *)ws, s)
+                                : forward<FP16>(h, loss, x, w, ids, teacher, (char *)saved, (char *)ws, s);
+}
+int run_backward(const na1d_head &h, void *dx, void *dw, const float *dloss, const void *x, const void *w, const void *ids, const void *saved, void *ws, hipStream_t s) {
+    return h.dtype == NA1D_BF16 ? backward<BF16>(h, (char *)dx, (char *)dw, dloss, x, w, ids, (const char *)saved, (char *)ws, s)
+                                : backward<FP16>(h, (char *)dx, (char *)dw, dloss, x, w, ids, (const char *)saved, (char *)ws, s);
+}
+
+}  // namespace loss
+}  // namespace na1d

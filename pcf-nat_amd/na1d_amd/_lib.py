@@ -31,7 +31,8 @@ SYMBOLS = _UNFUSED + ("na1d_fused_forward", "na1d_fused_backward", "na1d_fused_b
                       "na1d_fused_backward_dilated_workspace_bytes", "na1d_encode", "na1d_encode_workspace_bytes",
                       "na1d_train_layer_saved_bytes", "na1d_train_layer_workspace_bytes", "na1d_train_layer_forward",
                       "na1d_train_to_channels", "na1d_train_pool_backward", "na1d_train_context_backward", "na1d_train_context",
-                      "na1d_train_layer_backward", "na1d_version", "na1d_status_string")
+                      "na1d_train_layer_backward", "na1d_head_saved_bytes", "na1d_head_workspace_bytes", "na1d_head_forward",
+                      "na1d_head_backward", "na1d_version", "na1d_status_string")
 UNSUPPORTED = -8
 
 _lib = None
@@ -113,6 +114,12 @@ def load():
     lib.na1d_train_pool_backward.argtypes = [_ptr] * 6 + [_i64] * 3 + [_f32, _int, _ptr]
     lib.na1d_train_context_backward.argtypes = [_ptr] * 5 + [_i64] * 3 + [_f32, _int, _ptr]
     lib.na1d_train_layer_backward.argtypes = [_ptr] * 5 + [_i64, _ptr, _i64, _i64, _i64, _ptr]
+    lib.na1d_head_saved_bytes.restype = lib.na1d_head_workspace_bytes.restype = _i64
+    lib.na1d_head_saved_bytes.argtypes = [_ptr]
+    lib.na1d_head_workspace_bytes.argtypes = [_ptr, _int]
+    lib.na1d_head_forward.restype = lib.na1d_head_backward.restype = _int
+    lib.na1d_head_forward.argtypes = [_ptr] * 7 + [_i64, _ptr, _i64, _ptr]
+    lib.na1d_head_backward.argtypes = [_ptr] * 8 + [_i64, _ptr, _i64, _ptr]
     lib.na1d_fused_backward_noalloc.restype = _int
     lib.na1d_fused_backward_noalloc.argtypes = [_ptr] * 12 + [_i64] * 6 + [_f32, _int, _ptr]
     lib.na1d_force_generic.restype = _int
