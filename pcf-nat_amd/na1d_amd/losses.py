@@ -111,6 +111,12 @@ class _HeadLoss(torch.autograd.Function):
         return (dx if want[0] else None, dw if want[1] else None) + (None,) * 7
 
 
+def _loss(x, weight, ids, teacher, *args):
+    nodes = _lib.nodes()
+    out = None if nodes is None else nodes.head(x, weight, ids, teacher, *args)
+    return _HeadLoss.apply(x, weight, ids, teacher, *args) if out is None else out
+
+
 def check_arguments(x, weight, ids, reduction, ids_shape, weight_dims=(2,), what="target"):
     """What the losses ask of their arguments; the sizes' limits are the native call's."""
     if reduction not in _REDUCTIONS:
@@ -144,7 +150,7 @@ def linear_cross_entropy(x, weight, target, scale=1.0, ignore_index=-100, reduct
     ones too: they take part in the weight's gradient with a factor of zero.
     """
     check_arguments(x, weight, target, reduction, x.shape[:-1])
-    return _HeadLoss.apply(x, weight, target, None, _TARGETS, float(scale), 0.0, int(ignore_index), _REDUCTIONS[reduction])
+    return _loss(x, weight, target, None, _TARGETS, float(scale), 0.0, int(ignore_index), _REDUCTIONS[reduction])
 
 
 def margin_cross_entropy(x, weight, target, margin=0.2, scale=32.0, ignore_index=-100, reduction="mean"):
@@ -156,7 +162,7 @@ def margin_cross_entropy(x, weight, target, margin=0.2, scale=32.0, ignore_index
     with everything and no gradient.  Other arguments as in :func:`linear_cross_entropy`.
     """
     check_arguments(x, weight, target, reduction, x.shape[:-1], weight_dims=(2, 3))
-    return _HeadLoss.apply(x, weight, target, None, _MARGIN, float(scale), float(margin), int(ignore_index), _REDUCTIONS[reduction])
+    return _loss(x, weight, target, None, _MARGIN, float(scale), float(margin), int(ignore_index), _REDUCTIONS[reduction])
 
 
 def linear_distillation(x, weight, teacher_logits, teacher_ids, temperature=1.0, reduction="mean"):
@@ -176,4 +182,4 @@ def linear_distillation(x, weight, teacher_logits, teacher_ids, temperature=1.0,
     check_arguments(x, weight, teacher_ids, reduction, x.shape[:-1] + teacher_logits.shape[-1:], what="teacher_ids")
     if teacher_logits.device != x.device:
         raise _lib.NA1DError("x and teacher_logits must be on one device")
-    return _HeadLoss.apply(x, weight, teacher_ids, teacher_logits.detach(), _TEACHER, float(temperature), 0.0, 0, _REDUCTIONS[reduction])
+    return _loss(x, weight, teacher_ids, teacher_logits.detach(), _TEACHER, float(temperature), 0.0, 0, _REDUCTIONS[reduction])

@@ -124,3 +124,14 @@ def test_distillation(size, top, dtype):
         delta = O.logit_bound(x, w, 1 / temperature) + 2.0 ** -18
         more = lambda f: tuple(a + b for a, b in zip(magnitudes(f), both(2 * delta + 2.0 ** -18)))
         _check(loss, grads, rows, ok, reduction, dx, dw, more, 2 * delta, up, dtype, extra_loss=temperature ** 2)
+
+
+def test_gradients_that_are_differentiated_again_are_refused():
+    x, w, target = _inputs(33, 64, 63, torch.float16, 4)
+    x.requires_grad_(True)
+    for call in (lambda: losses.linear_cross_entropy(x, w, target), lambda: losses.linear_cross_entropy(x[:, :], w.t().contiguous().t(), target)):
+        plain = torch.autograd.grad(call(), x)[0]
+        (dx,) = torch.autograd.grad(call(), x, create_graph=True)
+        assert torch.equal(dx, plain) and dx.requires_grad
+        with pytest.raises(RuntimeError, match="differentia"):
+            dx.sum().backward()
