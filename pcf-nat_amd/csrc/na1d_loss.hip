@@ -9,6 +9,7 @@
 // exponentials to a row (logits_kernel), and a kernel that puts a row's tiles together (finish_kernel).  The backward works the
 // logits out again, a range of classes at a time, rounds dz to the operands' type - what a head that keeps its logits would have
 // handed its products - and multiplies it twice (product_kernel): by W for dx, transposed by x for dW.
+#include <atomic>
 #include <cmath>
 
 #include "na1d_encoder.h"
@@ -157,10 +158,22 @@ struct alignas(16) RowStat {
     int target;        // class, or kFar
     int sub;           // of its weight rows the nearest
 };
-// The same as the backward's kernels take it.
-struct alignas(16) RowGrad {
-    float lse2, f, at_target;       // dz = f * exp2(z2 - lse2), at the target at_target
-    int target;
+// What a row multiplies its probabilities by: dz = f exp2(z2 - lse2).  Gradients of single logits are rounded to 16 bits, where fp16
+// ends at 6e-8 and either type is at its most exact just below a power of two; so all are multiplied by one number, which the
+// products' ends take away again, that brings the largest there may be to kTopDz.  Most rows' largest (the target's, -(1 - P_t) of a
+// whole) comes close to it: of the target's share in the gradients a third less is lost than on average.
+constexpr float kTopDz = 16320.f;            // 255 * 2^6
+struct Upstream {
+    const float *dloss, *count;     // count NULL: dloss has a value for every row
+    const float *most;              // the largest a row's factor may come to for an upstream gradient of 1 (with `count`) or as it is
+    float factor;
+    int mean;
+    __device__ inline float base() const { return count ? factor * (mean ? dloss[0] / count[0] : dloss[0]) : factor; }
+    __device__ inline float up(float base) const {
+        const float top = __builtin_fabsf(base) * *most;
+        return top > 0.f && top < 3.0e38f ? __builtin_fminf(kTopDz / top, 0x1p100f) : 1.f;
+    }
+    __device__ inline float down() const { return 1.f / up(base()); }
 };
 struct Head {
     const char *x, *w;
@@ -179,6 +192,7 @@ __device__ inline int load_id(const void *ids, int64_t i, int wide) {
 // that a masked logit of -inf stays one.
 constexpr float kLeastNorm = 1e-12f, kNoNorm = 1e-30f;
 
+constexpr int kNormBlocks = 1024;
 // 1 / |row| of 16-bit rows, a wave to a row; the first `rows_a` are a's.  And the largest of each workgroup's rows of b.
 template <class DT>
 __global__ void __launch_bounds__(256)
@@ -230,7 +244,7 @@ struct Logits {
     const void *ids;                // targets, or NULL: no class is kept out
     int ids_wide;
     // backward
-    const RowGrad *rows;
+    Upstream up;
     const RowStat *stats;
     char *dz;                       // 16-bit [N, subs, plane]
     int64_t plane;                  // columns to a sub-centre, a multiple of 64
@@ -361,17 +375,20 @@ logits_kernel(Logits a) {
         if constexpr (COS)
 #pragma unroll
             for (int i = 0; i < S::MT; ++i) sums[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const float base = a.up.base(), common = base * a.up.up(base);
 #pragma unroll
         for (int j = 0; j < S::NT; ++j) {
             const int row = 16 * (wn * S::NT + j) + n;
             const int64_t r = min(r0 + row, a.h.N - 1);
-            const RowGrad rg = a.rows[r];
-            const bool exists = r0 + row < a.h.N;                               // rows behind the last have no share in the sums
-            const float c2 = a.h.scale2 * (COS ? a.h.inv_x[r] : 1.f), f = exists ? rg.f : 0.f, e = exists ? rg.at_target : 0.f;
+            const RowStat rg = a.stats[r];
+            const float ix = COS ? a.h.inv_x[r] : 1.f, c2 = a.h.scale2 * ix;
+            float f = common * (a.up.count ? 1.f : a.up.dloss[r]) * ix;
+            if (r0 + row >= a.h.N || rg.sub < 0 || (COS && ix == kNoNorm)) f = 0.f;           // rows behind the last have no share in the sums
+            const float e = f * rg.at_target;
             const int64_t t = (int64_t)rg.target - c0;
             const bool hit = t >= 16 * wm * S::MT && t < 16 * (wm + 1) * S::MT;
             const bool any = __builtin_amdgcn_ballot_w64(hit) != 0;
-            const int near = SUBS && any ? a.stats[r].sub : 0;
+            const int near = rg.sub;
 #pragma unroll
             for (int i = 0; i < S::MT; ++i) {
                 f32x4 d;
@@ -469,7 +486,7 @@ __device__ inline float over_wave(float x, bool max) {
     }
     return x;
 }
-constexpr int kFinishThreads = 256, kMostRows = 16;
+constexpr int kFinishThreads = 256;
 // The derivative of the margin's cosine has the sine in its denominator; it is bounded there.
 constexpr float kLeastSine2 = 1e-6f;
 
@@ -477,14 +494,18 @@ template <class DT>
 __global__ void __launch_bounds__(kFinishThreads)
 finish_kernel(Finish a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    f32x2 *met = reinterpret_cast<f32x2 *>(smem);                             // [lanes][rows]: 256 of them
-    float *z = reinterpret_cast<float *>(smem + kFinishThreads * sizeof(f32x2));     // [rows][entries], log2 domain
-    float *lse = z + a.rows * (a.top ? a.top : a.h.subs);                       // [rows]
+    const int entries = a.top ? a.top : a.h.subs;
+    f32x2 *met = reinterpret_cast<f32x2 *>(smem);                               // [lanes][rows]: 256 of them
+    float *z = reinterpret_cast<float *>(met + kFinishThreads);                 // [rows][entries], log2 domain
+    float *lse = z + a.rows * entries;                                          // [rows]
+    int *ids = reinterpret_cast<int *>(lse + a.rows);                           // teacher: [rows][entries] ...
+    float *share = reinterpret_cast<float *>(ids + a.rows * entries);           // ... and their q, before the sum is divided out
     const int R = a.rows, lanes = kFinishThreads / R, r = threadIdx.x & (R - 1), l = threadIdx.x / R;
     const int64_t r0 = (int64_t)blockIdx.x * R;
     {
         f32x2 v = {kNegInf, 0.f};
         const int64_t row = min(r0 + r, (int64_t)a.h.N - 1);
+#pragma unroll 4
         for (int t = l; t < a.m_tiles; t += lanes) {
             const f32x2 o = a.part[(int64_t)t * a.h.N + row];
             const float top = __builtin_fmaxf(v.x, o.x), off = top == kNegInf ? 0.f : top;
@@ -493,17 +514,18 @@ finish_kernel(Finish a) {
         met[threadIdx.x] = v;
     }
     // logits of the entries: 16 lanes to an entry
-    const int entries = a.top ? a.top : a.h.subs, lane16 = threadIdx.x & 15;
+    const int lane16 = threadIdx.x & 15;
     for (int e = threadIdx.x >> 4; e < R * entries; e += kFinishThreads / 16) {
         const int64_t row = r0 + e / entries;
         const int k = e % entries;
         float s = 0.f;
+        int id = -1;
         if (row < a.h.N) {
-            const int id = load_id(a.ids, a.top ? row * a.top + k : row, a.ids_wide);
+            id = load_id(a.ids, a.top ? row * a.top + k : row, a.ids_wide);
             if (id >= 0 && id < a.h.V) {
                 const int64_t wr = a.top ? id : (int64_t)id * a.h.subs + k;
                 const char *xr = a.h.x + row * a.h.x_pitch, *w = a.h.w + wr * a.h.w_pitch;
-#pragma unroll 2
+#pragma unroll 4
                 for (int c = lane16 * 8; c < a.h.D; c += 128) {
                     const u32x4 p = *reinterpret_cast<const u32x4 *>(xr + 2 * c), q = *reinterpret_cast<const u32x4 *>(w + 2 * c);
 #pragma unroll
@@ -517,7 +539,10 @@ finish_kernel(Finish a) {
             }
         }
         s = sum_of_16(s);
-        if (lane16 == 0) z[e] = s;
+        if (lane16 == 0) {
+            z[e] = s;
+            if (a.top) ids[e] = id;
+        }
     }
     __syncthreads();
     // The tiles' sums meet, R rows at a time.
@@ -533,173 +558,140 @@ finish_kernel(Finish a) {
     __syncthreads();
     if (!a.top) {
         const int64_t row = r0 + threadIdx.x;
-        if ((int)threadIdx.x >= R || row >= a.h.N) return;
-        const int64_t raw = a.ids_wide ? reinterpret_cast<const int64_t *>(a.ids)[row] : (int64_t)reinterpret_cast<const int32_t *>(a.ids)[row];
-        RowStat st = {__builtin_inff(), 0.f, kFar, -1};
-        float loss = raw == a.ignore ? 0.f : __builtin_nanf("");
-        if (raw != a.ignore && raw >= 0 && raw < a.h.V) {
-            float best = z[threadIdx.x * entries], slope = 1.f;
-            st.sub = 0;
-            for (int k = 1; k < entries; ++k)
-                if (z[threadIdx.x * entries + k] > best) best = z[threadIdx.x * entries + k], st.sub = k;
-            if (a.cosines) {
-                const float c = best * a.h.inv_x[row], sine2 = 1.f - c * c;
-                best = c;
-                if (c > a.threshold) {
-                    best = c * a.cos_m - __builtin_sqrtf(__builtin_fmaxf(sine2, 0.f)) * a.sin_m;
-                    slope = a.cos_m + a.sin_m * c / __builtin_sqrtf(__builtin_fmaxf(sine2, kLeastSine2));
-                } else if (c <= a.threshold) {
-                    best = c - a.drop;
+        if ((int)threadIdx.x < R && row < a.h.N) {
+            const int64_t raw = a.ids_wide ? reinterpret_cast<const int64_t *>(a.ids)[row] : (int64_t)reinterpret_cast<const int32_t *>(a.ids)[row];
+            RowStat st = {__builtin_inff(), 0.f, kFar, -1};
+            float loss = raw == a.ignore ? 0.f : __builtin_nanf("");
+            if (raw != a.ignore && raw >= 0 && raw < a.h.V) {
+                float best = z[threadIdx.x * entries], slope = 1.f;
+                st.sub = 0;
+                for (int k = 1; k < entries; ++k)
+                    if (z[threadIdx.x * entries + k] > best) best = z[threadIdx.x * entries + k], st.sub = k;
+                if (a.cosines) {
+                    const float c = best * a.h.inv_x[row], sine2 = 1.f - c * c;
+                    best = c;
+                    if (c > a.threshold) {
+                        best = c * a.cos_m - __builtin_sqrtf(__builtin_fmaxf(sine2, 0.f)) * a.sin_m;
+                        slope = a.cos_m + a.sin_m * c / __builtin_sqrtf(__builtin_fmaxf(sine2, kLeastSine2));
+                    } else if (c <= a.threshold) {
+                        best = c - a.drop;
+                    }
                 }
+                const float zt = best * a.h.scale2, others = lse[threadIdx.x], d = others - zt;         // log2 domain
+                const float e = __builtin_amdgcn_exp2f(-__builtin_fabsf(d)), more = log1pf(e);
+                loss = __builtin_fmaxf(d, 0.f) * kLn2 + more;
+                if (d != d) loss = d;
+                st.lse2 = (d > 0.f ? others : zt) + more * kLog2e;
+                st.at_target = -(d > 0.f ? 1.f : e) / (1.f + e) * slope;
+                st.target = (int)raw;
             }
-            const float zt = best * a.h.scale2, others = lse[threadIdx.x], d = others - zt;         // log2 domain
-            const float e = __builtin_amdgcn_exp2f(-__builtin_fabsf(d)), more = log1pf(e);
-            loss = __builtin_fmaxf(d, 0.f) * kLn2 + more;
-            if (d != d) loss = d;
-            st.lse2 = (d > 0.f ? others : zt) + more * kLog2e;
-            st.at_target = -(d > 0.f ? 1.f : e) / (1.f + e) * slope;
-            st.target = (int)raw;
+            a.stats[row] = st;
+            a.loss[row] = loss;
         }
-        a.stats[row] = st;
-        a.loss[row] = loss;
-        return;
-    }
-    // A teacher's row: a wave to each.
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int q0 = wave; q0 < R; q0 += kFinishThreads / 64) {
-        const int64_t row = r0 + q0;
-        if (row >= a.h.N) break;
-        constexpr int kEach = NA1D_HEAD_MAX_TOP / 64;
-        int id[kEach];
-        float t[kEach], q[kEach], top = kNegInf;
-        bool bad = false, nan = false;
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            const int k = i * 64 + lane;
-            id[i] = k < a.top ? load_id(a.ids, row * a.top + k, a.ids_wide) : -1;
-            bad |= id[i] >= a.h.V;
-            t[i] = id[i] >= 0 && id[i] < a.h.V ? teacher_value(a.teacher, row * a.top + k, a.teacher_type) * (1.f / a.temperature) : kNegInf;
-            nan |= t[i] != t[i];
-            top = __builtin_fmaxf(top, t[i]);
-        }
-        top = over_wave(top, true);
-        float total = 0.f;
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) total += q[i] = t[i] == kNegInf ? 0.f : __builtin_amdgcn_exp2f((t[i] - top) * kLog2e);
-        total = over_wave(total, false);
-        bad = __builtin_amdgcn_ballot_w64(bad) != 0;
-        nan = __builtin_amdgcn_ballot_w64(nan) != 0;
-        RowStat st = {__builtin_inff(), 0.f, kFar, -1};
-        float loss = bad ? __builtin_nanf("") : 0.f;
-        const bool counts = !bad && (top > kNegInf || nan);
-        const float log_total = __builtin_log2f(total), lse2 = lse[q0];
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            const int k = i * 64 + lane;
-            if (k >= a.top) continue;
-            const float z2 = z[q0 * a.top + k] * a.h.scale2, p = __builtin_amdgcn_exp2f(z2 - lse2);
-            q[i] /= total;
-            if (t[i] != kNegInf) sum += q[i] == 0.f ? 0.f : q[i] * ((t[i] - top) * kLog2e - log_total - (z2 - lse2));
-            float same = 0.f;                                                   // an entry that is there twice has both shares
-            for (int m = 0; m < a.top; ++m) {
-                const int64_t at = row * a.top + m;
-                if (load_id(a.ids, at, a.ids_wide) == id[i]) {
-                    const float u = teacher_value(a.teacher, at, a.teacher_type) * (1.f / a.temperature);
-                    same += u == kNegInf ? 0.f : __builtin_amdgcn_exp2f((u - top) * kLog2e);
-                }
+    } else {
+        // A teacher's row: a wave to each.
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        for (int q0 = wave; q0 < R; q0 += kFinishThreads / 64) {
+            const int64_t row = r0 + q0;
+            if (row >= a.h.N) break;
+            const int *id = ids + q0 * a.top;
+            float *q = share + q0 * a.top;
+            float top = kNegInf, total = 0.f;
+            bool bad = false, nan = false;
+            for (int k = lane; k < a.top; k += 64) {
+                const float t = id[k] >= 0 && id[k] < a.h.V ? teacher_value(a.teacher, row * a.top + k, a.teacher_type) * (1.f / a.temperature) : kNegInf;
+                bad |= id[k] >= a.h.V;
+                nan |= t != t;
+                top = __builtin_fmaxf(top, t);
+                q[k] = t;
             }
-            a.coeff[row * a.top + k] = counts && id[i] >= 0 ? p - same / total : 0.f;
+            top = over_wave(top, true);
+            const float off = top == kNegInf ? 0.f : top;
+            for (int k = lane; k < a.top; k += 64) total += __builtin_amdgcn_exp2f((q[k] - off) * kLog2e);
+            total = over_wave(total, false);
+            bad = __builtin_amdgcn_ballot_w64(bad) != 0;
+            nan = __builtin_amdgcn_ballot_w64(nan) != 0;
+            const bool counts = !bad && (top > kNegInf || nan);
+            const float log_total = __builtin_log2f(total), inv = 1.f / total, lse2 = lse[q0];
+            float sum = 0.f;
+            for (int k = lane; k < a.top; k += 64) {
+                const float logq = (q[k] - off) * kLog2e - log_total, share = __builtin_amdgcn_exp2f((q[k] - off) * kLog2e) * inv, z2 = z[q0 * a.top + k] * a.h.scale2;
+                if (share != 0.f) sum += share * (logq - (z2 - lse2));
+                q[k] = share;
+            }
+            for (int k = lane; k < a.top; k += 64) {
+                float same = 0.f;                                               // an entry that is there twice has both shares
+                for (int m = 0; m < a.top; ++m) same += id[m] == id[k] ? q[m] : 0.f;
+                a.coeff[row * a.top + k] = counts && id[k] >= 0 ? __builtin_amdgcn_exp2f(z[q0 * a.top + k] * a.h.scale2 - lse2) - same : 0.f;
+            }
+            sum = over_wave(sum, false);
+            RowStat st = {__builtin_inff(), 0.f, kFar, -1};
+            float loss = bad ? __builtin_nanf("") : 0.f;
+            if (counts) {
+                loss = sum * kLn2 * a.temperature * a.temperature;
+                st.lse2 = lse2;
+                st.sub = 0;
+            }
+            if (lane == 0) a.stats[row] = st, a.loss[row] = loss;
         }
-        sum = over_wave(sum, false);
-        if (counts) {
-            loss = sum * kLn2 * a.temperature * a.temperature;
-            st.lse2 = lse2;
-            st.sub = 0;
-        }
-        if (lane == 0) a.stats[row] = st, a.loss[row] = loss;
     }
 }
 
-// Sum or mean of the rows' losses; and of how many rows.
+// The sum or mean of the rows' losses in a fixed order, how many rows count, and the largest their factors may come to (Upstream).
+// (As the work of the finish kernel's last workgroup it is no launch of its own, but the fences of all the others cost more than
+// that: 128 rows 15.8 us against 5.2 + 1.9, 999 rows 50 against 9.)
+struct Reduce {
+    float *total, *count, *most;
+    const float *loss, *dloss, *inv_x, *most_w;       // dloss: of every row, in a backward (NULL otherwise); most_w [kNormBlocks]; either may be NULL
+    const RowStat *stats;
+    int N, mean;
+};
 __global__ void __launch_bounds__(1024)
-reduce_kernel(float *__restrict__ loss, float *__restrict__ count, const float *__restrict__ rows, const RowStat *__restrict__ stats, int N, int mean) {
+reduce_kernel(Reduce a) {
     __shared__ double sums[16];
     __shared__ int counts[16];
+    __shared__ float tops[16], mosts[16];
     double s = 0.0;
     int c = 0;
-    for (int r = threadIdx.x; r < N; r += 1024) {
-        s += (double)rows[r];
-        c += stats[r].sub >= 0;
+    float top = 0.f, most = a.most_w ? 0.f : 1.f;
+#pragma unroll 4
+    for (int r = threadIdx.x; r < a.N; r += 1024) {
+        const RowStat st = a.stats[r];
+        if (a.loss) s += (double)a.loss[r];
+        const float f = __builtin_fmaxf(1.f, __builtin_fabsf(st.at_target)) * (a.inv_x ? a.inv_x[r] : 1.f) * (a.dloss ? __builtin_fabsf(a.dloss[r]) : 1.f);
+        c += st.sub >= 0;
+        top = __builtin_fmaxf(top, st.sub >= 0 ? f : 0.f);
     }
+    if (a.most_w) most = a.most_w[threadIdx.x];
+    static_assert(kNormBlocks == 1024, "one to a thread");
 #pragma unroll
     for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o), c += __shfl_xor(c, o);
-    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s, counts[threadIdx.x >> 6] = c;
+    top = over_wave(top, true), most = over_wave(most, true);
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) sums[wave] = s, counts[wave] = c, tops[wave] = top, mosts[wave] = most;
     __syncthreads();
     if (threadIdx.x) return;
-    for (int i = 1; i < 16; ++i) s += sums[i], c += counts[i];
-    *count = (float)(c > 1 ? c : 1);
-    *loss = (float)(mean ? s / (double)(c > 1 ? c : 1) : s);
+    for (int i = 1; i < 16; ++i) s += sums[i], c += counts[i], top = __builtin_fmaxf(top, tops[i]), most = __builtin_fmaxf(most, mosts[i]);
+    *a.most = top * most;
+    if (!a.loss) return;
+    *a.count = (float)(c > 1 ? c : 1);
+    *a.total = (float)(a.mean ? s / (double)(c > 1 ? c : 1) : s);
 }
 
 // =============================================================================
 // Backward
 // =============================================================================
-struct Rows {
-    RowGrad *rows;
-    float *unscale;
-    const RowStat *stats;
-    const float *dloss, *count, *inv_x, *most_w;      // count NULL: dloss has a value for every row
-    int N, most_count, mean, half;
-    float factor;
-};
-// What a row multiplies its probabilities by.  fp16 gradients of single logits would be lost below 6e-8: they are multiplied by the
-// power of two that brings the largest that may come to 2^13 or more, which the products' ends take away again.
-__global__ void __launch_bounds__(1024)
-rows_kernel(Rows a) {
-    __shared__ float tops[16];
-    auto factor = [&](int r) {
-        const RowStat st = a.stats[r];
-        if (st.sub < 0) return 0.f;
-        float f = a.factor * (a.count ? a.dloss[0] / (a.mean ? a.count[0] : 1.f) : a.dloss[r]);
-        if (a.inv_x) f = a.inv_x[r] == kNoNorm ? 0.f : f * a.inv_x[r];
-        return f;
-    };
-    float scale = 1.f;
-    if (a.half) {
-        float top = 0.f, most = a.most_w ? 0.f : 1.f;
-        for (int r = threadIdx.x; r < a.N; r += 1024) {
-            const float f = __builtin_fabsf(factor(r));
-            top = __builtin_fmaxf(top, f * __builtin_fmaxf(1.f, __builtin_fabsf(a.stats[r].at_target)));
-        }
-        for (int i = threadIdx.x; i < a.most_count; i += 1024) most = __builtin_fmaxf(most, a.most_w[i]);
-        top = over_wave(top, true);
-        most = over_wave(most, true);
-        __shared__ float mosts[16];
-        if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top, mosts[threadIdx.x >> 6] = most;
-        __syncthreads();
-        for (int i = 0; i < 16; ++i) top = __builtin_fmaxf(top, tops[i]), most = __builtin_fmaxf(most, mosts[i]);
-        top *= most;
-        if (top > 0.f && top < 3.0e38f) scale = __builtin_ldexpf(1.f, max(-120, min(120, 13 + 127 - (int)(__float_as_uint(top) >> 23))));
-    }
-    if (threadIdx.x == 0 && blockIdx.x == 0) *a.unscale = 1.f / scale;
-    for (int r = blockIdx.x * 1024 + threadIdx.x; r < a.N; r += gridDim.x * 1024) {
-        const RowStat st = a.stats[r];
-        const float f = factor(r) * scale;
-        a.rows[r] = RowGrad{st.lse2, f, f * st.at_target, st.target};
-    }
-}
-
 // The teacher's entries of dz, which the logits' kernel left as those of any class.  Entries of one class write the same value.
 template <class DT>
 __global__ void __launch_bounds__(256)
-entries_kernel(uint16_t *__restrict__ dz, const float *__restrict__ coeff, const RowGrad *__restrict__ rows, const void *__restrict__ ids, int ids_wide, int N, int top,
-               int class0, int classes, int64_t plane) {
+entries_kernel(uint16_t *__restrict__ dz, const float *__restrict__ coeff, Upstream up, const void *__restrict__ ids, int ids_wide, int N, int top, int class0, int classes,
+               int64_t plane) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= (int64_t)N * top) return;
     const int64_t row = i / top, c = (int64_t)load_id(ids, i, ids_wide) - class0;
     if (c < 0 || c >= classes) return;
-    dz[row * plane + c] = (uint16_t)Mma<DT>::pack(coeff[i] * rows[row].f, 0.f);
+    const float base = up.base();
+    dz[row * plane + c] = (uint16_t)Mma<DT>::pack(coeff[i] * (base * up.up(base) * (up.count ? 1.f : up.dloss[row])), 0.f);
 }
 
 // dx (fp32, all ranges' and splits' shares): x rows (N side) by channels (M side), contracted over a range's classes; and dW:
@@ -713,22 +705,19 @@ struct Product {
     float *part;                    // fp32 [splits, rows, D]
     int64_t part_stride;
     int add;                        // to what is there
+    Upstream up;
     // dW without splits
     char *out;                      // 16-bit [V * subs, D], or NULL: to part
-    const float *unscale;
     const char *w;                  // cosines: dW loses its part along w
     int64_t w_pitch;
     const float *inv_w, *col_part;
     int col_parts;
 };
 template <class DT, class S, bool DW>
-__global__ void __launch_bounds__(S::kThreadsOf, 2)
-product_kernel(Product a) {
-    extern __shared__ __attribute__((aligned(16))) char smem[];
-    LDS_PTR(char) lds = (LDS_PTR(char))smem;
+__device__ inline void product(const Product &a, uint32_t item, LDS_PTR(char) lds) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
     const int wm = wave % S::WM, wn = wave / S::WM;
-    const uint32_t item = xcd_item(blockIdx.x, gridDim.x), mt = item % (uint32_t)a.m_tiles, rest = item / (uint32_t)a.m_tiles;
+    const uint32_t mt = item % (uint32_t)a.m_tiles, rest = item / (uint32_t)a.m_tiles;
     const int nt = (int)(rest % (uint32_t)a.n_tiles), split = (int)(rest / (uint32_t)a.n_tiles);
     const int d0 = (int)mt * S::BM;
     const int64_t pitch = 2 * a.plane * a.subs;
@@ -764,7 +753,7 @@ product_kernel(Product a) {
     }
     const int m0 = d0 + 16 * wm * S::MT;                                        // this wave's channels
     if (DW && a.out) {
-        const float unscale = *a.unscale;
+        const float unscale = a.up.down();
         const int left = a.classes - col0;                                      // classes of the tile
         const int64_t row0 = (int64_t)(a.class0 + col0) * a.subs + sub;
         const int out_pitch = 2 * a.D * a.subs, width = max(0, min(32 * S::MT, 2 * (a.D - m0)));
@@ -814,35 +803,59 @@ product_kernel(Product a) {
     }
 }
 
-// The shares of all splits of a row put together (a wave to a row), less their part along the row's own vector (cosines).
+// Both in one launch, the dx part's workgroups first.  (Either may be empty.)
+template <class DT, class SX, class SW>
+__global__ void __launch_bounds__(SX::kThreadsOf, 2)
+products_kernel(Product dx, Product dw, uint32_t dx_items, uint32_t dw_items) {
+    static_assert(SX::kThreadsOf == SW::kThreadsOf, "one launch");
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    LDS_PTR(char) lds = (LDS_PTR(char))smem;
+    if (blockIdx.x < dx_items)
+        product<DT, SX, false>(dx, xcd_item(blockIdx.x, dx_items), lds);
+    else
+        product<DT, SW, true>(dw, xcd_item(blockIdx.x - dx_items, dw_items), lds);
+}
+
+// The shares of all splits of a row put together, less their part along the row's own vector (cosines).  WAVES waves to a row share
+// its splits.
 struct Fold {
     char *out;
     const float *part;
     int64_t stride, rows;
     int splits, D;
-    const float *unscale;
+    Upstream up;
     const char *own;                // cosines: the rows themselves, and 1 / their length
     int64_t own_pitch;
     const float *inv;
 };
-template <class DT>
+template <class DT, int WAVES>
 __global__ void __launch_bounds__(256)
 fold_kernel(Fold a) {
-    const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    __shared__ f32x4 met[WAVES > 1 ? WAVES : 1][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t row = WAVES > 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
     if (row >= a.rows) return;
     const float *part = a.part + row * a.D;
-    float f = *a.unscale;
+    float f = a.up.down();
     auto sum = [&](int d) {
-        f32x4 v = *reinterpret_cast<const f32x4 *>(part + d);
-#pragma unroll 4
-        for (int s = 1; s < a.splits; ++s) v += *reinterpret_cast<const f32x4 *>(part + s * a.stride + d);
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        if (d < a.D)
+#pragma unroll 8
+            for (int s = WAVES > 1 ? wave : 0; s < a.splits; s += WAVES) v += *reinterpret_cast<const f32x4 *>(part + s * a.stride + d);
+        if constexpr (WAVES > 1) {
+            __syncthreads();
+            met[wave][lane] = v;
+            __syncthreads();
+            v = met[0][lane];
+#pragma unroll
+            for (int i = 1; i < WAVES; ++i) v += met[i][lane];
+        }
         return v;
     };
-    auto own = [&](int d) { return widen4<DT>(*reinterpret_cast<const u32x2 *>(a.own + row * a.own_pitch + 2 * d)); };
+    auto own = [&](int d) { return d < a.D ? widen4<DT>(*reinterpret_cast<const u32x2 *>(a.own + row * a.own_pitch + 2 * d)) : f32x4{0.f, 0.f, 0.f, 0.f}; };
     float along = 0.f;
     if (a.own) {
-        for (int d = lane * 4; d < a.D; d += 256) {
+        for (int d = lane * 4; d < a.D + lane * 4; d += 256) {
             const f32x4 v = sum(d) * own(d);
             along += v[0] + v[1] + (v[2] + v[3]);
         }
@@ -850,16 +863,11 @@ fold_kernel(Fold a) {
         along = over_wave(along, false) * inv * inv;
         if (inv == kNoNorm) f = 0.f, along = 0.f;
     }
-    for (int d = lane * 4; d < a.D; d += 256) {
+    for (int d = lane * 4; d < a.D + lane * 4; d += 256) {
         f32x4 v = sum(d);
         if (a.own) v -= along * own(d);
-        *reinterpret_cast<u32x2 *>(a.out + (row * a.D + d) * 2) = narrow4<DT>(v * f);
+        if (d < a.D && (WAVES == 1 || wave == 0)) *reinterpret_cast<u32x2 *>(a.out + (row * a.D + d) * 2) = narrow4<DT>(v * f);
     }
-}
-__global__ void __launch_bounds__(256)
-clear_kernel(u32x4 *__restrict__ out, int64_t units) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i < units) out[i] = u32x4{0, 0, 0, 0};
 }
 
 // =============================================================================
@@ -867,11 +875,9 @@ clear_kernel(u32x4 *__restrict__ out, int64_t units) {
 // =============================================================================
 template <class T> inline T ceil_div(T a, T b) { return (a + b - 1) / b; }
 inline int64_t round_up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
-constexpr int kNormBlocks = 1024;
-
 // Places of the forward's results in `saved`, which the backward reads.
 struct Saved {
-    int64_t count, stats, coeff, inv_x, inv_w, most, bytes;
+    int64_t count, stats, coeff, inv_x, inv_w, most, bytes;     // count: and the largest factor behind it
     explicit Saved(const na1d_head &h) {
         int64_t at = 0;
         auto take = [&](int64_t n) { const int64_t p = at; at += round_up(n, 256); return p; };
@@ -940,12 +946,11 @@ struct ForwardScratch {
     }
 };
 struct BackwardScratch {
-    int64_t unscale, rows, dz, dx, dw, cols, bytes;
+    int64_t most, dz, dx, dw, cols, bytes;
     BackwardScratch(const na1d_head &h, const Plan &p) {
         int64_t at = 0;
         auto take = [&](int64_t n) { const int64_t q = at; at += round_up(n, 256); return q; };
-        unscale = take(16);
-        rows = take(h.N * (int64_t)sizeof(RowGrad));
+        most = take(16);
         dz = take(2 * h.N * h.subcenters * p.plane);
         dx = take(4 * h.N * h.D * p.dx_splits);
         dw = take(p.dw_splits > 1 ? 4 * h.V * h.subcenters * h.D * p.dw_splits : 0);
@@ -960,16 +965,22 @@ struct BackwardScratch {
         if (st_ != NA1D_OK) return st_;  \
     } while (0)
 
-template <class K, class A> int launch(K kern, unsigned grid, unsigned block, size_t lds, hipStream_t s, const A &a) {
-    if (!allow_lds(kern, lds)) return NA1D_ERR_LAUNCH;
-    kern<<<grid, block, lds, s>>>(a);
+// A kernel's limit of LDS is raised once on every device.
+template <auto KERNEL, class... A> int launch(unsigned grid, unsigned block, size_t lds, hipStream_t s, const A &...a) {
+    static std::atomic<uint64_t> raised{0};
+    int device = 0;
+    if (lds > 64 * 1024 && (hipGetDevice(&device) != hipSuccess || device > 63 || !(raised.load(std::memory_order_relaxed) >> device & 1))) {
+        if (!allow_lds(KERNEL, lds)) return NA1D_ERR_LAUNCH;
+        if (device <= 63) raised.fetch_or(1ull << device, std::memory_order_relaxed);
+    }
+    KERNEL<<<grid, block, lds, s>>>(a...);
     return launch_status();
 }
 template <class DT, class S, bool BACK> int launch_logits_of(const na1d_head &h, const Logits &a, hipStream_t s) {
     const unsigned grid = (unsigned)(a.m_tiles * a.n_tiles);
-    if (h.kind != NA1D_HEAD_MARGIN) return launch(logits_kernel<DT, S, false, false, BACK>, grid, S::kThreadsOf, S::kLds, s, a);
-    if (h.subcenters == 1) return launch(logits_kernel<DT, S, true, false, BACK>, grid, S::kThreadsOf, S::kLds, s, a);
-    if constexpr (S::MT * S::NT <= 8) return launch(logits_kernel<DT, S, true, true, BACK>, grid, S::kThreadsOf, S::kLds, s, a);
+    if (h.kind != NA1D_HEAD_MARGIN) return launch<logits_kernel<DT, S, false, false, BACK>>(grid, S::kThreadsOf, S::kLds, s, a);
+    if (h.subcenters == 1) return launch<logits_kernel<DT, S, true, false, BACK>>(grid, S::kThreadsOf, S::kLds, s, a);
+    if constexpr (S::MT * S::NT <= 8) return launch<logits_kernel<DT, S, true, true, BACK>>(grid, S::kThreadsOf, S::kLds, s, a);
     return NA1D_ERR_UNSUPPORTED;
 }
 template <class DT, bool BACK> int launch_logits(const na1d_head &h, const Plan &p, Logits a, hipStream_t s) {
@@ -977,12 +988,13 @@ template <class DT, bool BACK> int launch_logits(const na1d_head &h, const Plan 
     a.n_tiles = (int)ceil_div<int64_t>(h.N, p.bn);
     return p.logits == kFew ? launch_logits_of<DT, Few, BACK>(h, a, s) : p.logits == kBatch ? launch_logits_of<DT, Batch, BACK>(h, a, s) : launch_logits_of<DT, Many, BACK>(h, a, s);
 }
-template <class DT, bool DW> int launch_product(Pick pick, const Product &a, hipStream_t s) {
-    const unsigned grid = (unsigned)((int64_t)a.m_tiles * a.n_tiles * a.splits);
-    if constexpr (!DW)
-        if (pick == kFew) return launch(product_kernel<DT, Few, DW>, grid, Few::kThreadsOf, Few::kLds, s, a);
-    if (pick == kBatch) return launch(product_kernel<DT, Batch, DW>, grid, Batch::kThreadsOf, Batch::kLds, s, a);
-    return launch(product_kernel<DT, Many, DW>, grid, Many::kThreadsOf, Many::kLds, s, a);
+template <class DT, class SX, class SW> int launch_products_of(const Product &dx, const Product &dw, hipStream_t s) {
+    const uint32_t nx = (uint32_t)((int64_t)dx.m_tiles * dx.n_tiles * dx.splits), nw = (uint32_t)((int64_t)dw.m_tiles * dw.n_tiles * dw.splits);
+    return launch<products_kernel<DT, SX, SW>>(nx + nw, SX::kThreadsOf, std::max(SX::kLds, SW::kLds), s, dx, dw, nx, nw);
+}
+template <class DT> int launch_products(const Plan &p, const Product &dx, const Product &dw, hipStream_t s) {
+    if (p.dx == kFew) return p.dw == kBatch ? launch_products_of<DT, Few, Batch>(dx, dw, s) : launch_products_of<DT, Few, Many>(dx, dw, s);
+    return p.dw == kBatch ? launch_products_of<DT, Batch, Batch>(dx, dw, s) : launch_products_of<DT, Many, Many>(dx, dw, s);      // both by the channels
 }
 inline Head head_of(const na1d_head &h, const void *x, const void *w, const char *saved, const Saved &o) {
     const bool cosines = h.kind == NA1D_HEAD_MARGIN;
@@ -1010,18 +1022,19 @@ int forward(const na1d_head &h, float *loss, const void *x, const void *w, const
     NA1D_TRY((launch_logits<DT, false>(h, p, a, s)));
     Finish e{};
     e.h = a.h, e.part = a.part, e.m_tiles = (int)p.m_tiles;
-    e.rows = h.N >= 4096 ? 16 : h.N >= 1024 ? 4 : 1;
+    e.rows = h.N >= 4096 && !teaches ? 16 : h.N >= 1024 ? 4 : 1;
     e.ids = ids, e.ids_wide = h.ids_64, e.top = teaches ? h.top : 0, e.teacher = teacher, e.teacher_type = h.teacher_type;
     e.ignore = h.ignore_index, e.cosines = cosines, e.scale = h.scale, e.temperature = h.scale;
     e.cos_m = (float)cos(h.margin), e.sin_m = (float)sin(h.margin), e.threshold = (float)cos(M_PI - h.margin), e.drop = (float)(sin(M_PI - h.margin) * h.margin);
     e.stats = reinterpret_cast<RowStat *>(saved + o.stats), e.coeff = reinterpret_cast<float *>(saved + o.coeff);
     float *rows = reinterpret_cast<float *>(ws + f.rows);
     e.loss = h.reduction == NA1D_HEAD_NONE ? loss : rows;
-    const size_t lds = kFinishThreads * sizeof(f32x2) + 4 * (size_t)e.rows * ((teaches ? h.top : h.subcenters) + 1);
-    NA1D_TRY(launch(finish_kernel<DT>, (unsigned)ceil_div<int64_t>(h.N, e.rows), kFinishThreads, lds, s, e));
+    const size_t lds = kFinishThreads * sizeof(f32x2) + 4 * (size_t)e.rows * (teaches ? 3 * h.top + 1 : h.subcenters + 1);
+    NA1D_TRY(launch<finish_kernel<DT>>((unsigned)ceil_div<int64_t>(h.N, e.rows), kFinishThreads, lds, s, e));
     if (h.reduction == NA1D_HEAD_NONE) return NA1D_OK;
-    reduce_kernel<<<1, 1024, 0, s>>>(loss, reinterpret_cast<float *>(saved + o.count), rows, e.stats, (int)h.N, h.reduction == NA1D_HEAD_MEAN);
-    return launch_status();
+    float *count = reinterpret_cast<float *>(saved + o.count);
+    return launch<reduce_kernel>(1, 1024, 0, s, Reduce{loss, count, count + 1, rows, nullptr, a.h.inv_x, cosines ? reinterpret_cast<const float *>(saved + o.most) : nullptr,
+                                                       e.stats, (int)h.N, h.reduction == NA1D_HEAD_MEAN});
 }
 
 template <class DT>
@@ -1030,49 +1043,49 @@ int backward(const na1d_head &h, char *dx, char *dw, const float *dloss, const v
     const Plan p = plan_of(h);
     const BackwardScratch b(h, p);
     const bool cosines = h.kind == NA1D_HEAD_MARGIN;
-    float *unscale = reinterpret_cast<float *>(ws + b.unscale);
     const RowStat *stats = reinterpret_cast<const RowStat *>(saved + o.stats);
+    const float *most_w = cosines ? reinterpret_cast<const float *>(saved + o.most) : nullptr;
     Logits a{};
     a.h = head_of(h, x, w, saved, o);
-    Rows r{};
-    r.rows = reinterpret_cast<RowGrad *>(ws + b.rows), r.unscale = unscale, r.stats = stats, r.dloss = dloss;
-    r.count = h.reduction == NA1D_HEAD_NONE ? nullptr : reinterpret_cast<const float *>(saved + o.count);
-    r.inv_x = a.h.inv_x, r.most_w = cosines ? reinterpret_cast<const float *>(saved + o.most) : nullptr, r.most_count = cosines ? kNormBlocks : 0;
-    r.N = (int)h.N, r.mean = h.reduction == NA1D_HEAD_MEAN, r.half = DT::tag == NA1D_FP16;
-    r.factor = h.scale;                                                                   // a teacher's: temperature^2 / temperature
-    rows_kernel<<<r.half ? 1 : (unsigned)ceil_div<int64_t>(h.N, 1024), 1024, 0, s>>>(r);
-    NA1D_TRY(launch_status());
-    a.rows = r.rows, a.stats = stats, a.dz = ws + b.dz, a.plane = p.plane;
+    Upstream up{};
+    up.dloss = dloss, up.factor = h.scale, up.mean = h.reduction == NA1D_HEAD_MEAN;           // a teacher's: temperature^2 / temperature
+    if (h.reduction == NA1D_HEAD_NONE) {
+        up.most = reinterpret_cast<const float *>(ws + b.most);
+        NA1D_TRY(launch<reduce_kernel>(1, 1024, 0, s, Reduce{nullptr, nullptr, reinterpret_cast<float *>(ws + b.most), nullptr, dloss, a.h.inv_x, most_w, stats, (int)h.N, 0}));
+    } else {
+        up.count = reinterpret_cast<const float *>(saved + o.count), up.most = up.count + 1;
+    }
+    a.up = up, a.stats = stats, a.dz = ws + b.dz, a.plane = p.plane;
     a.col_part = cosines && dw && p.dw_splits == 1 ? reinterpret_cast<float *>(ws + b.cols) : nullptr;
     Product g{};
-    g.dz = a.dz, g.plane = p.plane, g.N = (int)h.N, g.D = (int)h.D, g.subs = h.subcenters, g.unscale = unscale;
+    g.dz = a.dz, g.plane = p.plane, g.N = (int)h.N, g.D = (int)h.D, g.subs = h.subcenters, g.up = up;
     for (int64_t range = 0; range < p.ranges; ++range) {
         a.class0 = g.class0 = (int)(range * p.plane);
         a.classes = g.classes = (int)std::min(p.plane, h.V - a.class0);
         g.columns = (int)round_up(a.classes, kStep);
         NA1D_TRY((launch_logits<DT, true>(h, p, a, s)));
         if (h.kind == NA1D_HEAD_TEACHER) {
-            entries_kernel<DT><<<(unsigned)ceil_div<int64_t>(h.N * h.top, 256), 256, 0, s>>>(
-                (uint16_t *)a.dz, reinterpret_cast<const float *>(saved + o.coeff), r.rows, ids, h.ids_64, (int)h.N, h.top, a.class0, a.classes, p.plane);
+            entries_kernel<DT><<<(unsigned)ceil_div<int64_t>(h.N * h.top, 256), 256, 0, s>>>((uint16_t *)a.dz, reinterpret_cast<const float *>(saved + o.coeff), up, ids,
+                                                                                             h.ids_64, (int)h.N, h.top, a.class0, a.classes, p.plane);
             NA1D_TRY(launch_status());
         }
+        Product gx = g, gw = g;                                                               // what is not asked for has no workgroups
         if (dx) {
-            g.other = a.h.w, g.other_pitch = a.h.w_pitch;
-            g.m_tiles = (int)ceil_div<int64_t>(h.D, p.dx_bm), g.n_tiles = (int)ceil_div<int64_t>(h.N, p.dx_bn), g.splits = p.dx_splits, g.per = p.dx_per;
-            g.part = reinterpret_cast<float *>(ws + b.dx), g.part_stride = h.N * h.D, g.add = range > 0, g.out = nullptr;
-            NA1D_TRY((launch_product<DT, false>(p.dx, g, s)));
+            gx.other = a.h.w, gx.other_pitch = a.h.w_pitch;
+            gx.m_tiles = (int)ceil_div<int64_t>(h.D, p.dx_bm), gx.n_tiles = (int)ceil_div<int64_t>(h.N, p.dx_bn), gx.splits = p.dx_splits, gx.per = p.dx_per;
+            gx.part = reinterpret_cast<float *>(ws + b.dx), gx.part_stride = h.N * h.D, gx.add = range > 0;
         }
         if (dw) {
-            g.other = a.h.x, g.other_pitch = a.h.x_pitch;
-            g.m_tiles = (int)ceil_div<int64_t>(h.D, p.dw_bm), g.n_tiles = (int)(h.subcenters * ceil_div(g.columns, p.dw_bn)), g.splits = p.dw_splits, g.per = p.dw_per;
-            g.part = reinterpret_cast<float *>(ws + b.dw), g.part_stride = h.V * h.subcenters * h.D, g.add = 0, g.out = p.dw_splits == 1 ? dw : nullptr;
-            g.w = cosines ? a.h.w : nullptr, g.w_pitch = a.h.w_pitch, g.inv_w = a.h.inv_w, g.col_part = a.col_part, g.col_parts = (int)ceil_div<int64_t>(h.N, p.bn) * p.wn;
-            NA1D_TRY((launch_product<DT, true>(p.dw, g, s)));
+            gw.other = a.h.x, gw.other_pitch = a.h.x_pitch;
+            gw.m_tiles = (int)ceil_div<int64_t>(h.D, p.dw_bm), gw.n_tiles = (int)(h.subcenters * ceil_div(g.columns, p.dw_bn)), gw.splits = p.dw_splits, gw.per = p.dw_per;
+            gw.part = reinterpret_cast<float *>(ws + b.dw), gw.part_stride = h.V * h.subcenters * h.D, gw.out = p.dw_splits == 1 ? dw : nullptr;
+            gw.w = cosines ? a.h.w : nullptr, gw.w_pitch = a.h.w_pitch, gw.inv_w = a.h.inv_w, gw.col_part = a.col_part, gw.col_parts = (int)ceil_div<int64_t>(h.N, p.bn) * p.wn;
         }
+        NA1D_TRY(launch_products<DT>(p, gx, gw, s));
     }
     auto fold = [&](char *out, int64_t part, int64_t rows, int splits, const char *own, int64_t own_pitch, const float *inv) {
-        const Fold f{out, reinterpret_cast<const float *>(ws + part), rows * h.D, rows, splits, (int)h.D, unscale, cosines ? own : nullptr, own_pitch, inv};
-        return launch(fold_kernel<DT>, (unsigned)ceil_div<int64_t>(rows, 4), 256, 0, s, f);
+        const Fold f{out, reinterpret_cast<const float *>(ws + part), rows * h.D, rows, splits, (int)h.D, up, cosines ? own : nullptr, own_pitch, inv};
+        return splits >= 8 ? launch<fold_kernel<DT, 4>>((unsigned)rows, 256, 0, s, f) : launch<fold_kernel<DT, 1>>((unsigned)ceil_div<int64_t>(rows, 4), 256, 0, s, f);
     };
     if (dx) NA1D_TRY(fold(dx, b.dx, h.N, p.dx_splits, a.h.x, a.h.x_pitch, a.h.inv_x));
     if (dw && p.dw_splits > 1) NA1D_TRY(fold(dw, b.dw, h.V * h.subcenters, p.dw_splits, a.h.w, a.h.w_pitch, a.h.inv_w));
