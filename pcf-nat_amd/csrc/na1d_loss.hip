@@ -26,12 +26,15 @@ using namespace enc;
 // the contraction needs of a tile is extent / 64 such pieces.  An operand whose contraction runs along its rows in memory has
 // the tile's rows (64 to a piece) and 64 values of each; one whose contraction runs from row to row ("turned") has 64 rows of
 // the contraction and 64 of the tile's columns, which come out of LDS transposed (ds_read_b64_tr_b16).  The 16-byte units of a
-// row are XOR-swizzled by three bits of its number so that both ways of reading spread over all banks: rows 0 .. 15 at one unit
-// (row operands), and rows {0-3, 8-11} or {4-7, 12-15} at 32 bytes (half a wave's transposed read).
+// row are XOR-swizzled by three bits of its number, by which the sixteen rows of a row operand's read, and the rows {0-3, 8-11} or
+// {4-7, 12-15} of half a wave's transposed read, spread over all banks; no one choice of bits does for both (counted: an operand's
+// read takes 4 cycles and a transposed one 2, with the other's choice 8 and 4).
 constexpr int kStep = 64;                     // of the contraction
 constexpr int kPieceRow = 2 * kStep;          // bytes
 constexpr int kPiece = 64 * kPieceRow;
-__device__ inline int swizzle(int row) { return ((row >> 3) & 1) << 2 | ((row >> 1) & 1) << 1 | ((row >> 2) & 1); }
+template <bool TURNED> __device__ inline int swizzle(int row) {
+    return TURNED ? ((row >> 3) & 1) << 2 | ((row >> 1) & 1) << 1 | ((row >> 2) & 1) : (row >> 1) & 7;
+}
 
 // Where an operand's tile comes from.  All members but the lane's are wave-uniform.
 template <int EXTENT, int NW, bool TURNED> struct Source {
@@ -49,7 +52,7 @@ template <int EXTENT, int NW, bool TURNED> struct Source {
         width = (int)row_width;
         bytes = rows > 0 ? (rows - 1) * row_pitch + row_width : 0;
         step = TURNED ? kStep * row_pitch : kPieceRow;
-        unit = ((lane & 7) ^ swizzle(8 * wave + (lane >> 3))) * 16;          // chunks of a wave differ by multiples of 16 rows or of 32
+        unit = ((lane & 7) ^ swizzle<TURNED>(8 * wave + (lane >> 3))) * 16;          // chunks of a wave are 32 rows apart, or 64
         lane_at = (8 * wave + (lane >> 3)) * pitch + unit;
     }
     __device__ inline void load(LDS_PTR(char) to, int s, int wave) const {
@@ -74,7 +77,7 @@ template <int EXTENT, int NW, bool TURNED> struct Source {
 template <bool TURNED> struct Reader;
 template <> struct Reader<false> {
     int lane_at;
-    __device__ inline void init(int n, int g) { lane_at = n * kPieceRow + ((g ^ swizzle(n)) << 4); }
+    __device__ inline void init(int n, int g) { lane_at = n * kPieceRow + ((g ^ swizzle<false>(n)) << 4); }
     __device__ inline u32x4 read(LDS_PTR(char) tile, int t, int h) const {
         return *reinterpret_cast<LDS_PTR(u32x4)>(tile + t * 16 * kPieceRow + (lane_at ^ h * 64));
     }
@@ -83,7 +86,7 @@ template <> struct Reader<true> {
     int lane_at;
     __device__ inline void init(int n, int g) {
         const int row = 8 * g + (n >> 2);
-        lane_at = row * kPieceRow + ((((n & 3) >> 1) ^ swizzle(row)) << 4) + 8 * (n & 1);
+        lane_at = row * kPieceRow + ((((n & 3) >> 1) ^ swizzle<true>(row)) << 4) + 8 * (n & 1);
     }
     __device__ inline u32x4 read(LDS_PTR(char) tile, int t, int h) const {
         LDS_PTR(char) p = tile + (t >> 2) * kPiece + h * 32 * kPieceRow;
@@ -105,13 +108,15 @@ __device__ inline float sum_of_16(float x) {                                   /
     x += __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), 0x141, 0xf, 0xf, true));
     return x + __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), 0x140, 0xf, 0xf, true));
 }
+__device__ inline void turn_over() { asm volatile("s_barrier" ::: "memory"); }
 template <int COUNT> __device__ inline void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(COUNT) : "memory"); }
 
 // acc[i][j] += A[16 of M, number wm * MT + i] . B[16 of N, number wn * NT + j]^T; lane (n, g) holds M 4g .. 4g + 3 and N n.
-// A step's operands are asked for STAGES - 1 steps ahead; one barrier to a step.
+//
+// Four waves: a step's operands are asked for STAGES - 1 steps ahead; one barrier to a step.  Two workgroups to a CU overlap.
 template <class DT, class S, class A, class B, class RA, class RB>
-__device__ inline void accumulate(f32x4 (&acc)[S::MT][S::NT], const A &a, const B &b, const RA &ra, const RB &rb, int steps, LDS_PTR(char) lds, int wave, int wm,
-                                  int wn) {
+__device__ inline void accumulate_ahead(f32x4 (&acc)[S::MT][S::NT], const A &a, const B &b, const RA &ra, const RB &rb, int steps, LDS_PTR(char) lds, int wave, int wm,
+                                        int wn) {
     constexpr int kAhead = S::STAGES - 1, kLoads = A::kLoads + B::kLoads;
     auto stage = [&](int s, int slot) {
         a.load(lds + slot * S::kSlot, s, wave);
@@ -145,6 +150,65 @@ __device__ inline void accumulate(f32x4 (&acc)[S::MT][S::NT], const A &a, const 
         slot = slot + 1 == S::STAGES ? 0 : slot + 1;
         next = next + 1 == S::STAGES ? 0 : next + 1;
     }
+}
+
+// Eight waves, one workgroup to a CU: two groups of four, a wave of each on every SIMD, which take turns.  A step is four quarters
+// of MT / 2 x NT products; while one group multiplies, the other reads the next quarter's operands out of LDS and asks for the next
+// step's from memory.  A group's reads have returned before the barrier that ends its turn, so its turn at the next step may write
+// where the other group's last turn has read; a step's loads are waited for at the end of its last reading turn, a barrier before
+// anyone reads them.  16384 x 1024 by 8192 x 1024 rows, with the softmax: 1130 TFLOP/s (four waves in tiles of 128 x 128: 960; eight
+// waves that read and multiply as the compiler orders it: 1085).
+template <class DT, class S, class A, class B, class RA, class RB>
+__device__ inline void accumulate_in_turns(f32x4 (&acc)[S::MT][S::NT], const A &a, const B &b, const RA &ra, const RB &rb, int steps, LDS_PTR(char) lds, int wave, int wm,
+                                           int wn) {
+    static_assert(S::kWavesOf == 8 && S::STAGES == 2 && S::MT % 2 == 0, "two groups of four waves, two steps in LDS");
+    constexpr int kHalf = S::MT / 2;
+    if (steps <= 0) return;
+    a.load(lds, 0, wave);
+    b.load(lds + A::kBytes, 0, wave);
+    wait_loads<0>();
+    barrier_lds();
+    if (wave >= 4) turn_over();
+#pragma unroll 1
+    for (int s = 0; s < steps; ++s) {
+        LDS_PTR(char) from = lds + (s & 1) * S::kSlot;
+        LDS_PTR(char) to = lds + (~s & 1) * S::kSlot;
+        u32x4 y[S::NT];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const int h = c >> 1, i0 = (c & 1) * kHalf;
+            u32x4 x[kHalf];
+            if ((c & 1) == 0) {
+#pragma unroll
+                for (int j = 0; j < S::NT; ++j) y[j] = rb.read(from + A::kBytes, wn * S::NT + j, h);
+            }
+#pragma unroll
+            for (int i = 0; i < kHalf; ++i) x[i] = ra.read(from, wm * S::MT + i0 + i, h);
+            __builtin_amdgcn_sched_barrier(0);
+            if (c == 0 && s + 1 < steps) b.load(to + A::kBytes, s + 1, wave);
+            if (c == 1 && s + 1 < steps) a.load(to, s + 1, wave);
+            if (c == 3) wait_loads<0>();
+            barrier_lds();
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+            for (int i = 0; i < kHalf; ++i)
+#pragma unroll
+                for (int j = 0; j < S::NT; ++j) acc[i0 + i][j] = Mma<DT>::k32(x[i], y[j], acc[i0 + i][j]);
+            __builtin_amdgcn_s_setprio(0);
+            __builtin_amdgcn_sched_barrier(0);
+            turn_over();
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    if (wave < 4) turn_over();
+}
+template <class DT, class S, class A, class B, class RA, class RB>
+__device__ inline void accumulate(f32x4 (&acc)[S::MT][S::NT], const A &a, const B &b, const RA &ra, const RB &rb, int steps, LDS_PTR(char) lds, int wave, int wm, int wn) {
+    if constexpr (S::kWavesOf == 8)
+        accumulate_in_turns<DT, S>(acc, a, b, ra, rb, steps, lds, wave, wm, wn);
+    else
+        accumulate_ahead<DT, S>(acc, a, b, ra, rb, steps, lds, wave, wm, wn);
 }
 
 // =============================================================================
@@ -764,6 +828,7 @@ __device__ inline void product(const Product &a, uint32_t item, LDS_PTR(char) ld
             const int c = 16 * (wn * S::NT + j) + n;
             float along = 0.f;
             if (a.w && c < left) {
+                #pragma unroll 8
                 for (int p = 0; p < a.col_parts; ++p) along += a.col_part[((int64_t)p * a.subs + sub) * a.plane + col0 + c];
                 const float inv = a.inv_w[row0 + (int64_t)c * a.subs];
                 along *= inv == kNoNorm ? 0.f : inv * inv;
@@ -896,46 +961,83 @@ struct Saved {
 using Few = Shape<1, 2, 4, 1, 4>;             // 64 x 32
 using Batch = Shape<2, 4, 2, 2, 3>;           // 64 x 128
 using Many = Shape<4, 4, 2, 2, 2>;            // 128 x 128
+using Vast = Shape<8, 4, 2, 4, 2>;            // 256 x 256
 
-enum Pick { kFew, kBatch, kMany };
-struct Plan {
-    Pick logits, dx, dw;
-    int bm, bn;                               // of the logits' tiles
+enum Pick { kFew, kBatch, kMany, kVast };
+struct Tiling {
+    Pick pick;
+    int bm, bn;
     int wn;                                   // waves along the rows
+    Tiling(Pick p = kFew) : pick(p) { bm = p == kVast ? 256 : p == kMany ? 128 : 64, bn = p == kVast ? 256 : p == kFew ? 32 : 128, wn = p == kVast ? 4 : p == kFew ? 1 : 2; }
+    int64_t tiles(int64_t m, int64_t n) const { return (m + bm - 1) / bm * ((n + bn - 1) / bn); }
+};
+struct Plan {
+    Tiling logits, back;                      // of the forward, of the backward
     int64_t m_tiles;
     // backward: ranges of classes
     int64_t plane;                            // columns to a sub-centre: a range's classes, rounded up to whole steps
     int64_t ranges;
-    int dx_bm, dx_bn, dx_splits, dx_per;
-    int dw_bm, dw_bn, dw_splits, dw_per;
+    Tiling dx, dw;
+    int dx_splits, dx_per, dw_splits, dw_per;
 };
-constexpr int64_t kMostDz = 256ll << 20;      // bytes of dz: what the last level of cache holds
+constexpr int64_t kMostDz = 256ll << 20;      // bytes of dz: what the last level of cache holds (64 MB: +10 to 25 %, 1 GB: 0 to +2 %)
 constexpr int kFullLaunch = 512;              // workgroups: two to a CU
-inline void shape_of(Pick p, int &bm, int &bn) { bm = p == kMany ? 128 : 64, bn = p == kFew ? 32 : 128; }
+
+// How long a launch of `first` workgroups of `first_steps` and then `second` of `second_steps` takes, in us: CUs hold one workgroup
+// of 256 x 256 or two smaller ones, and take the next as they get free.  A step of 64 takes the former 1.6 us and two of 128 x 128
+// side by side 0.93 (1340 and 1150 TFLOP/s), the rest of a tile 4.9 and 2.7: fitted to forwards of 8192 x 65536 and 16384 x 32768
+// logits with 1024 and 512 channels (972 and 567 us against 1124 and 650), which it also orders at sizes where the larger tiles do
+// not fill their last round: 1000 x 20000, 1024 channels 70 us against 62; 500 x 60000 73 against 86.
+inline double time_of(Pick p, int64_t first, int64_t first_steps, int64_t second = 0, int64_t second_steps = 0) {
+    const int64_t slots = p == kVast ? 256 : 512;
+    const double step = p == kVast ? 1.6 : 0.93, rest = p == kVast ? 4.9 : 2.7, a = first_steps * step + rest, b = second_steps * step + rest;
+    const int64_t rounds = first / slots, over = first % slots;
+    if (!second) return (rounds + (over > 0)) * a;
+    double busy[2] = {(rounds + 1) * a, rounds * a};
+    const int64_t wide[2] = {over, slots - over};
+    for (int64_t left = second; left > 0;) {
+        const int next = over && busy[0] < busy[1] ? 0 : 1;
+        left -= wide[next];
+        busy[next] += b;
+    }
+    return over ? std::max(busy[0], busy[1]) : busy[1];
+}
 inline Plan plan_of(const na1d_head &h) {
     Plan p{};
-    p.logits = h.N <= 32 ? kFew : ceil_div<int64_t>(h.V, 128) * ceil_div<int64_t>(h.N, 128) < kFullLaunch || h.subcenters > 1 ? kBatch : kMany;     // two sets of sums
-    shape_of(p.logits, p.bm, p.bn);
-    p.wn = p.logits == kFew ? 1 : 2;
-    p.m_tiles = ceil_div<int64_t>(h.V, p.bm);
+    const int64_t steps = ceil_div<int64_t>(h.D, kStep);
+    // Logits.  Several weight rows to a class keep two sets of sums, and the backward of a margin twice its tile's cosines: no room in
+    // the larger tiles.
+    const Tiling many(kMany), vast(kVast);
+    const int64_t in_many = many.tiles(h.V, h.N), in_vast = vast.tiles(h.V, h.N);
+    const bool larger = time_of(kVast, in_vast, steps) < time_of(kMany, in_many, steps);
+    p.logits = Tiling(h.N <= 32 ? kFew : in_many < kFullLaunch || h.subcenters > 1 ? kBatch : larger ? kVast : kMany);
+    p.back = Tiling(p.logits.pick == kVast && h.kind == NA1D_HEAD_MARGIN ? kMany : p.logits.pick);
+    p.m_tiles = ceil_div<int64_t>(h.V, p.logits.bm);
     const int64_t fits = std::min<int64_t>(kMostDz / (2 * h.N * h.subcenters), (1 << 20) / h.subcenters);
-    p.plane = std::min(round_up(h.V, kStep), std::max<int64_t>(fits / 256 * 256, 256));
+    p.plane = std::max<int64_t>(fits / 256 * 256, 256);
     p.ranges = ceil_div(h.V, p.plane);
+    p.plane = std::min(round_up(h.V, kStep), round_up(ceil_div(h.V, p.ranges), 256));         // ranges alike
+    p.ranges = ceil_div(h.V, p.plane);
+    // Products.  Channels are cut in tiles of 64 where that leaves fewer idle than 128.
     const bool narrow = round_up(h.D, 64) < round_up(h.D, 128);
-    p.dx = h.N <= 32 ? kFew : narrow ? kBatch : kMany;
-    shape_of(p.dx, p.dx_bm, p.dx_bn);
-    const int64_t dx_tiles = ceil_div<int64_t>(h.D, p.dx_bm) * ceil_div<int64_t>(h.N, p.dx_bn);
-    auto split = [&](int64_t tiles, int64_t length, int &splits, int &per) {
-        const int64_t steps = ceil_div<int64_t>(length, kStep), want = std::max<int64_t>(1, std::min<int64_t>(kFullLaunch / tiles, steps / 4));
-        per = (int)(ceil_div(steps, want) * kStep);
+    auto split = [&](int64_t tiles, int64_t length, int64_t most, int &splits, int &per) {
+        const int64_t all = ceil_div<int64_t>(length, kStep), want = std::max<int64_t>(1, std::min<int64_t>(most / tiles, all / 4));
+        per = (int)(ceil_div(all, want) * kStep);
         splits = (int)ceil_div<int64_t>(length, per);
     };
-    split(dx_tiles, p.plane, p.dx_splits, p.dx_per);
-    p.dw = narrow ? kBatch : kMany;
-    shape_of(p.dw, p.dw_bm, p.dw_bn);
-    const int64_t dw_tiles = ceil_div<int64_t>(h.D, p.dw_bm) * h.subcenters * ceil_div<int64_t>(p.plane, p.dw_bn);
-    split(dw_tiles, h.N, p.dw_splits, p.dw_per);
-    return p;
+    auto products = [&](Plan &q, Pick x, Pick w) {
+        q.dx = Tiling(x), q.dw = Tiling(w);
+        const int64_t most = w == kVast ? kFullLaunch / 2 : kFullLaunch, dx_tiles = q.dx.tiles(h.D, h.N), dw_tiles = h.subcenters * q.dw.tiles(h.D, q.plane);
+        split(dx_tiles, q.plane, most, q.dx_splits, q.dx_per);
+        split(dw_tiles, h.N, most, q.dw_splits, q.dw_per);
+        // and what the sums of splits cost in memory, at 4 TB/s
+        const double fold = (8. * q.dx_splits * h.N * h.D + (q.dw_splits > 1 ? 8. * q.dw_splits * h.subcenters * q.plane * h.D : 0.)) / 4.0e6;
+        return fold + time_of(w, dx_tiles * q.dx_splits, (int64_t)h.subcenters * q.dx_per / kStep, dw_tiles * q.dw_splits, q.dw_per / kStep);
+    };
+    Plan large = p;
+    const double t_large = h.N > 128 ? products(large, kVast, kVast) : 1e30;
+    const double t = products(p, h.N <= 32 ? kFew : narrow ? kBatch : kMany, narrow ? kBatch : kMany);
+    return t_large < t * (narrow ? 0.75 : 1.) ? large : p;
 }
 struct ForwardScratch {
     int64_t part, rows, bytes;
@@ -954,7 +1056,7 @@ struct BackwardScratch {
         dz = take(2 * h.N * h.subcenters * p.plane);
         dx = take(4 * h.N * h.D * p.dx_splits);
         dw = take(p.dw_splits > 1 ? 4 * h.V * h.subcenters * h.D * p.dw_splits : 0);
-        cols = take(h.kind == NA1D_HEAD_MARGIN && p.dw_splits == 1 ? 4 * ceil_div<int64_t>(h.N, p.bn) * p.wn * h.subcenters * p.plane : 0);
+        cols = take(h.kind == NA1D_HEAD_MARGIN && p.dw_splits == 1 ? 4 * ceil_div<int64_t>(h.N, p.back.bn) * p.back.wn * h.subcenters * p.plane : 0);
         bytes = at;
     }
 };
@@ -979,22 +1081,29 @@ template <auto KERNEL, class... A> int launch(unsigned grid, unsigned block, siz
 template <class DT, class S, bool BACK> int launch_logits_of(const na1d_head &h, const Logits &a, hipStream_t s) {
     const unsigned grid = (unsigned)(a.m_tiles * a.n_tiles);
     if (h.kind != NA1D_HEAD_MARGIN) return launch<logits_kernel<DT, S, false, false, BACK>>(grid, S::kThreadsOf, S::kLds, s, a);
-    if (h.subcenters == 1) return launch<logits_kernel<DT, S, true, false, BACK>>(grid, S::kThreadsOf, S::kLds, s, a);
+    if constexpr (!BACK || S::MT * S::NT <= 16)
+        if (h.subcenters == 1) return launch<logits_kernel<DT, S, true, false, BACK>>(grid, S::kThreadsOf, S::kLds, s, a);
     if constexpr (S::MT * S::NT <= 8) return launch<logits_kernel<DT, S, true, true, BACK>>(grid, S::kThreadsOf, S::kLds, s, a);
     return NA1D_ERR_UNSUPPORTED;
 }
-template <class DT, bool BACK> int launch_logits(const na1d_head &h, const Plan &p, Logits a, hipStream_t s) {
-    a.m_tiles = (int)ceil_div(a.classes, p.bm);
-    a.n_tiles = (int)ceil_div<int64_t>(h.N, p.bn);
-    return p.logits == kFew ? launch_logits_of<DT, Few, BACK>(h, a, s) : p.logits == kBatch ? launch_logits_of<DT, Batch, BACK>(h, a, s) : launch_logits_of<DT, Many, BACK>(h, a, s);
+template <class DT, bool BACK> int launch_logits(const na1d_head &h, const Tiling &t, Logits a, hipStream_t s) {
+    a.m_tiles = (int)ceil_div(a.classes, t.bm);
+    a.n_tiles = (int)ceil_div<int64_t>(h.N, t.bn);
+    switch (t.pick) {
+        case kFew: return launch_logits_of<DT, Few, BACK>(h, a, s);
+        case kBatch: return launch_logits_of<DT, Batch, BACK>(h, a, s);
+        case kMany: return launch_logits_of<DT, Many, BACK>(h, a, s);
+        default: return launch_logits_of<DT, Vast, BACK>(h, a, s);
+    }
 }
 template <class DT, class SX, class SW> int launch_products_of(const Product &dx, const Product &dw, hipStream_t s) {
     const uint32_t nx = (uint32_t)((int64_t)dx.m_tiles * dx.n_tiles * dx.splits), nw = (uint32_t)((int64_t)dw.m_tiles * dw.n_tiles * dw.splits);
     return launch<products_kernel<DT, SX, SW>>(nx + nw, SX::kThreadsOf, std::max(SX::kLds, SW::kLds), s, dx, dw, nx, nw);
 }
 template <class DT> int launch_products(const Plan &p, const Product &dx, const Product &dw, hipStream_t s) {
-    if (p.dx == kFew) return p.dw == kBatch ? launch_products_of<DT, Few, Batch>(dx, dw, s) : launch_products_of<DT, Few, Many>(dx, dw, s);
-    return p.dw == kBatch ? launch_products_of<DT, Batch, Batch>(dx, dw, s) : launch_products_of<DT, Many, Many>(dx, dw, s);      // both by the channels
+    if (p.dx.pick == kVast) return launch_products_of<DT, Vast, Vast>(dx, dw, s);
+    if (p.dx.pick == kFew) return p.dw.pick == kBatch ? launch_products_of<DT, Few, Batch>(dx, dw, s) : launch_products_of<DT, Few, Many>(dx, dw, s);
+    return p.dw.pick == kBatch ? launch_products_of<DT, Batch, Batch>(dx, dw, s) : launch_products_of<DT, Many, Many>(dx, dw, s);      // both by the channels
 }
 inline Head head_of(const na1d_head &h, const void *x, const void *w, const char *saved, const Saved &o) {
     const bool cosines = h.kind == NA1D_HEAD_MARGIN;
@@ -1019,7 +1128,7 @@ int forward(const na1d_head &h, float *loss, const void *x, const void *w, const
     a.classes = (int)h.V;
     a.part = reinterpret_cast<f32x2 *>(ws + f.part);
     a.ids = teaches ? nullptr : ids, a.ids_wide = h.ids_64;
-    NA1D_TRY((launch_logits<DT, false>(h, p, a, s)));
+    NA1D_TRY((launch_logits<DT, false>(h, p.logits, a, s)));
     Finish e{};
     e.h = a.h, e.part = a.part, e.m_tiles = (int)p.m_tiles;
     e.rows = h.N >= 4096 && !teaches ? 16 : h.N >= 1024 ? 4 : 1;
@@ -1063,7 +1172,7 @@ int backward(const na1d_head &h, char *dx, char *dw, const float *dloss, const v
         a.class0 = g.class0 = (int)(range * p.plane);
         a.classes = g.classes = (int)std::min(p.plane, h.V - a.class0);
         g.columns = (int)round_up(a.classes, kStep);
-        NA1D_TRY((launch_logits<DT, true>(h, p, a, s)));
+        NA1D_TRY((launch_logits<DT, true>(h, p.back, a, s)));
         if (h.kind == NA1D_HEAD_TEACHER) {
             entries_kernel<DT><<<(unsigned)ceil_div<int64_t>(h.N * h.top, 256), 256, 0, s>>>((uint16_t *)a.dz, reinterpret_cast<const float *>(saved + o.coeff), up, ids,
                                                                                              h.ids_64, (int)h.N, h.top, a.class0, a.classes, p.plane);
@@ -1072,14 +1181,14 @@ int backward(const na1d_head &h, char *dx, char *dw, const float *dloss, const v
         Product gx = g, gw = g;                                                               // what is not asked for has no workgroups
         if (dx) {
             gx.other = a.h.w, gx.other_pitch = a.h.w_pitch;
-            gx.m_tiles = (int)ceil_div<int64_t>(h.D, p.dx_bm), gx.n_tiles = (int)ceil_div<int64_t>(h.N, p.dx_bn), gx.splits = p.dx_splits, gx.per = p.dx_per;
+            gx.m_tiles = (int)ceil_div<int64_t>(h.D, p.dx.bm), gx.n_tiles = (int)ceil_div<int64_t>(h.N, p.dx.bn), gx.splits = p.dx_splits, gx.per = p.dx_per;
             gx.part = reinterpret_cast<float *>(ws + b.dx), gx.part_stride = h.N * h.D, gx.add = range > 0;
         }
         if (dw) {
             gw.other = a.h.x, gw.other_pitch = a.h.x_pitch;
-            gw.m_tiles = (int)ceil_div<int64_t>(h.D, p.dw_bm), gw.n_tiles = (int)(h.subcenters * ceil_div(g.columns, p.dw_bn)), gw.splits = p.dw_splits, gw.per = p.dw_per;
+            gw.m_tiles = (int)ceil_div<int64_t>(h.D, p.dw.bm), gw.n_tiles = (int)(h.subcenters * ceil_div(g.columns, p.dw.bn)), gw.splits = p.dw_splits, gw.per = p.dw_per;
             gw.part = reinterpret_cast<float *>(ws + b.dw), gw.part_stride = h.V * h.subcenters * h.D, gw.out = p.dw_splits == 1 ? dw : nullptr;
-            gw.w = cosines ? a.h.w : nullptr, gw.w_pitch = a.h.w_pitch, gw.inv_w = a.h.inv_w, gw.col_part = a.col_part, gw.col_parts = (int)ceil_div<int64_t>(h.N, p.bn) * p.wn;
+            gw.w = cosines ? a.h.w : nullptr, gw.w_pitch = a.h.w_pitch, gw.inv_w = a.h.inv_w, gw.col_part = a.col_part, gw.col_parts = (int)ceil_div<int64_t>(h.N, p.back.bn) * p.back.wn;
         }
         NA1D_TRY(launch_products<DT>(p, gx, gw, s));
     }

@@ -15,6 +15,9 @@ SIZES = [  # rows, channels, classes: one of each; below, at and above the tiles
     (1, 8, 1), (1, 192, 3001), (5, 16, 2), (32, 72, 65), (33, 64, 63), (31, 136, 300), (128, 192, 1000), (130, 200, 129), (129, 128, 64),
     (257, 328, 1211), (1030, 40, 300), (4100, 64, 130), (300, 1032, 501),
 ]
+LARGE = [  # launches that fill the card: tiles of 128 x 128 and of 256 x 256, products of either, several ranges of classes
+    (1000, 264, 9001), (2100, 72, 5003), (700, 1032, 13000), (2050, 512, 16390), (16390, 16, 8300),
+]
 
 
 def _inputs(N, D, V, dtype, seed, strength=3.0):
@@ -55,7 +58,7 @@ def _train(call, x, w, up):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=NAMES)
-@pytest.mark.parametrize("size", SIZES, ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("size", SIZES + LARGE, ids=lambda s: "x".join(map(str, s)))
 def test_cross_entropy(size, dtype):
     N, D, V = size
     print("cross entropy", size, dtype, flush=True)
@@ -73,6 +76,16 @@ def test_cross_entropy(size, dtype):
 @pytest.mark.parametrize("subs", [1, 2, 3, 5])
 @pytest.mark.parametrize("size", SIZES, ids=lambda s: "x".join(map(str, s)))
 def test_margin(size, subs, dtype):
+    _margin(size, subs, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=NAMES)
+@pytest.mark.parametrize("size,subs", [(s, 1) for s in LARGE] + [((2100, 72, 3003), 2), ((16390, 16, 4200), 3)], ids=lambda s: str(s))
+def test_margin_of_large_launches(size, subs, dtype):
+    _margin(size, subs, dtype)
+
+
+def _margin(size, subs, dtype):
     N, D, V = size
     print("margin", size, subs, dtype, flush=True)
     x, w, target = _inputs(N, D, V * subs, dtype, 2, strength=0.4 * D ** 0.5)
@@ -99,6 +112,16 @@ def test_margin(size, subs, dtype):
 @pytest.mark.parametrize("size", [(1, 8, 1), (1, 64, 500), (33, 72, 63), (128, 192, 1000), (1030, 40, 300), (4100, 64, 130)],
                          ids=lambda s: "x".join(map(str, s)))
 def test_distillation(size, top, dtype):
+    _distillation(size, top, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=NAMES)
+@pytest.mark.parametrize("size", LARGE, ids=lambda s: "x".join(map(str, s)))
+def test_distillation_of_large_launches(size, dtype):
+    _distillation(size, 5, dtype)
+
+
+def _distillation(size, top, dtype):
     N, D, V = size
     print("distillation", size, top, dtype, flush=True)
     x, w, target = _inputs(N, D, V, dtype, 3)
