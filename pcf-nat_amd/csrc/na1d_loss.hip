@@ -108,6 +108,14 @@ __device__ inline float sum_of_16(float x) {                                   /
     x += __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), 0x141, 0xf, 0xf, true));
     return x + __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), 0x140, 0xf, 0xf, true));
 }
+__device__ inline float over_wave(float x, bool max) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) {
+        const float y = __shfl_xor(x, o);
+        x = max ? __builtin_fmaxf(x, y) : x + y;
+    }
+    return x;
+}
 __device__ inline void turn_over() { asm volatile("s_barrier" ::: "memory"); }
 template <int COUNT> __device__ inline void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(COUNT) : "memory"); }
 
@@ -257,34 +265,45 @@ __device__ inline int load_id(const void *ids, int64_t i, int wide) {
 constexpr float kLeastNorm = 1e-12f, kNoNorm = 1e-30f;
 
 constexpr int kNormBlocks = 1024;
-// 1 / |row| of 16-bit rows, a wave to a row; the first `rows_a` are a's.  And the largest of each workgroup's rows of b.
+// 1 / |row| of 16-bit rows, sixteen lanes to a row; the first `rows_a` are a's.  And the largest of each workgroup's rows of b.
 template <class DT>
 __global__ void __launch_bounds__(256)
 norms_kernel(float *__restrict__ inv_a, float *__restrict__ inv_b, float *__restrict__ most_b, const char *__restrict__ a, const char *__restrict__ b, int64_t a_pitch,
              int64_t b_pitch, int64_t rows_a, int64_t rows_b, int D) {
+    constexpr int kAtOnce = 2;                                                  // rows of a lane in flight
     __shared__ float most[4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 15, wave = threadIdx.x >> 6;
+    const int64_t step = (int64_t)gridDim.x * 16, rows = rows_a + rows_b;
     float top = 0.f;
-    for (int64_t r = (int64_t)blockIdx.x * 4 + wave; r < rows_a + rows_b; r += (int64_t)gridDim.x * 4) {
-        const bool first = r < rows_a;
-        const char *row = first ? a + r * a_pitch : b + (r - rows_a) * b_pitch;
-        float s = 0.f;
-        for (int c = lane * 8; c < D; c += 512) {
-            const u32x4 v = *reinterpret_cast<const u32x4 *>(row + 2 * c);
+    for (int64_t r0 = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); r0 < rows; r0 += kAtOnce * step) {
+        float s[kAtOnce];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const f32x2 p = widen<DT>(v[i]);
-                s = __builtin_fmaf(p.x, p.x, s);
-                s = __builtin_fmaf(p.y, p.y, s);
+        for (int i = 0; i < kAtOnce; ++i) {
+            const int64_t r = min(r0 + i * step, rows - 1);
+            const char *row = r < rows_a ? a + r * a_pitch : b + (r - rows_a) * b_pitch;
+            s[i] = 0.f;
+#pragma unroll 2
+            for (int c = lane * 8; c < D; c += 128) {
+                const u32x4 v = *reinterpret_cast<const u32x4 *>(row + 2 * c);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const f32x2 p = widen<DT>(v[k]);
+                    s[i] = __builtin_fmaf(p.x, p.x, s[i]);
+                    s[i] = __builtin_fmaf(p.y, p.y, s[i]);
+                }
             }
         }
 #pragma unroll
-        for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
-        const float inv = s > kLeastNorm * kLeastNorm ? 1.f / __builtin_sqrtf(s) : s != s ? s : kNoNorm;
-        if (lane == 0) (first ? inv_a[r] : inv_b[r - rows_a]) = inv;
-        if (!first) top = __builtin_fmaxf(top, inv);
+        for (int i = 0; i < kAtOnce; ++i) {
+            const int64_t r = r0 + i * step;
+            const float sum = sum_of_16(s[i]), inv = sum > kLeastNorm * kLeastNorm ? 1.f / __builtin_sqrtf(sum) : sum != sum ? sum : kNoNorm;
+            if (r >= rows) continue;
+            if (lane == 0) (r < rows_a ? inv_a[r] : inv_b[r - rows_a]) = inv;
+            if (r >= rows_a) top = __builtin_fmaxf(top, inv);
+        }
     }
-    if (lane == 0) most[wave] = top;
+    top = over_wave(top, true);
+    if ((threadIdx.x & 63) == 0) most[wave] = top;
     __syncthreads();
     if (threadIdx.x == 0) most_b[blockIdx.x] = __builtin_fmaxf(__builtin_fmaxf(most[0], most[1]), __builtin_fmaxf(most[2], most[3]));
 }
@@ -482,7 +501,10 @@ logits_kernel(Logits a) {
 #pragma unroll
                 for (int i = 0; i < S::MT; ++i) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) inv[i][k] = a.h.inv_w[(int64_t)(c0 + min(first + 16 * i + k, there - 1)) * subs + sub];
+                    for (int k = 0; k < 4; ++k) {
+                        const float v = a.h.inv_w[(int64_t)(c0 + min(first + 16 * i + k, there - 1)) * subs + sub];
+                        inv[i][k] = v == kNoNorm ? 0.f : v;
+                    }
                     if constexpr (SUBS) sums[i] = f32x4{0.f, 0.f, 0.f, 0.f};
                 }
 #pragma unroll
@@ -541,14 +563,6 @@ __device__ inline float teacher_value(const void *p, int64_t i, int type) {
     if (type == NA1D_FP32) return reinterpret_cast<const float *>(p)[i];
     const uint16_t v = reinterpret_cast<const uint16_t *>(p)[i];
     return type == NA1D_BF16 ? BF16::to_f32(v) : FP16::to_f32(v);
-}
-__device__ inline float over_wave(float x, bool max) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) {
-        const float y = __shfl_xor(x, o);
-        x = max ? __builtin_fmaxf(x, y) : x + y;
-    }
-    return x;
 }
 constexpr int kFinishThreads = 256;
 // The derivative of the margin's cosine has the sine in its denominator; it is bounded there.
@@ -793,9 +807,16 @@ __device__ inline void product(const Product &a, uint32_t item, LDS_PTR(char) ld
     Reader<true> turned;
     turned.init(n, g);
     Source<S::BM, S::kWavesOf, true> as;
+    float along = 0.f;                                                          // cosines: of class threadIdx.x of the tile
     const int tiles_of_plane = DW ? a.n_tiles / a.subs : 1;
     const int sub = DW ? nt / tiles_of_plane : 0, col0 = DW ? (nt - sub * tiles_of_plane) * S::BN : 0, r0 = DW ? 0 : nt * S::BN;
     if constexpr (DW) {
+        if (a.out && a.w && (int)threadIdx.x < S::BN && col0 + (int)threadIdx.x < a.classes) {
+            const float *of = a.col_part + sub * a.plane + col0 + threadIdx.x, inv = a.inv_w[(int64_t)(a.class0 + col0 + threadIdx.x) * a.subs + sub];
+#pragma unroll 8
+            for (int p = 0; p < a.col_parts; ++p) along += of[(int64_t)p * a.subs * a.plane];
+            along *= inv == kNoNorm ? 0.f : inv * inv;
+        }
         const int64_t first = (int64_t)split * a.per, rows = min((int64_t)a.per, a.N - first);
         Source<S::BN, S::kWavesOf, true> bs;
         as.init(a.other + first * a.other_pitch + 2 * d0, rows, a.other_pitch, 2 * (int64_t)(a.D - d0), wave, lane);
@@ -822,32 +843,32 @@ __device__ inline void product(const Product &a, uint32_t item, LDS_PTR(char) ld
         const int64_t row0 = (int64_t)(a.class0 + col0) * a.subs + sub;
         const int out_pitch = 2 * a.D * a.subs, width = max(0, min(32 * S::MT, 2 * (a.D - m0)));
         const Rsrc os = make_rsrc(a.out + row0 * 2 * a.D, left > 0 ? (int)min((int64_t)(min(left, S::BN) - 1) * out_pitch + 2 * a.D, (int64_t)1 << 30) : 0);
-        const Rsrc wr = make_rsrc(a.w ? a.w + row0 * a.w_pitch : a.other, a.w && left > 0 ? (int)((min(left, S::BN) - 1) * a.w_pitch * a.subs + 2 * a.D) : 0);
+        LDS_PTR(float) part = (LDS_PTR(float))lds;
+        const int w_pitch = (int)(a.w_pitch * a.subs);
+        const Rsrc wr = make_rsrc(a.w ? a.w + row0 * a.w_pitch : a.other, a.w && left > 0 ? (min(left, S::BN) - 1) * w_pitch + 2 * a.D : 0);
+        if (a.w) {
+            barrier_lds();                                                      // the operands' place is taken over
+            if ((int)threadIdx.x < S::BN) part[threadIdx.x] = along;
+            barrier_lds();
+        }
 #pragma unroll
         for (int j = 0; j < S::NT; ++j) {
             const int c = 16 * (wn * S::NT + j) + n;
-            float along = 0.f;
-            if (a.w && c < left) {
-                #pragma unroll 8
-                for (int p = 0; p < a.col_parts; ++p) along += a.col_part[((int64_t)p * a.subs + sub) * a.plane + col0 + c];
-                const float inv = a.inv_w[row0 + (int64_t)c * a.subs];
-                along *= inv == kNoNorm ? 0.f : inv * inv;
+            if (a.w) {                                                          // the rows of w as store_tile's: 16 bytes to a lane
+                const float less = part[c];
+#pragma unroll
+                for (int p = 0; p < S::MT / 2; ++p) {
+                    const int at = (2 * p + (g & 1)) * 32 + (g >> 1) * 16;
+                    const u32x4 v = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(wr, at < width ? c * w_pitch + 2 * m0 + at : kNowhere, 0, 0));
+                    const u32x2 lo = __builtin_amdgcn_permlane16_swap(v.x, v.z, false, false), hi = __builtin_amdgcn_permlane16_swap(v.y, v.w, false, false);
+                    acc[2 * p][j] -= less * widen4<DT>(u32x2{lo.x, hi.x});
+                    acc[2 * p + 1][j] -= less * widen4<DT>(u32x2{lo.y, hi.y});
+                }
             }
-            const float f = a.w && c < left && a.inv_w[row0 + (int64_t)c * a.subs] == kNoNorm ? 0.f : unscale;
             u32x2 o[S::MT];
 #pragma unroll
-            for (int i = 0; i < S::MT; ++i) {
-                f32x4 v = acc[i][j];
-                if (a.w) {
-                    const int at = 32 * i + 8 * g;
-                    v -= along * widen4<DT>(__builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(wr, at < width ? (int)(c * a.w_pitch * a.subs) + 2 * m0 + at : kNowhere, 0, 0)));
-                }
-                o[i] = narrow4<DT>(v * f);
-            }
-            if constexpr (S::MT == 1)
-                __builtin_amdgcn_raw_buffer_store_b64(o[0], os, g * 8 < width ? c * out_pitch + 2 * m0 + g * 8 : kNowhere, 0, 0);
-            else
-                store_tile<16 * S::MT, 0>(os, c * out_pitch + 2 * m0, o, g, width);
+            for (int i = 0; i < S::MT; ++i) o[i] = narrow4<DT>(acc[i][j] * unscale);
+            store_tile<16 * S::MT, 0>(os, c * out_pitch + 2 * m0, o, g, width);
         }
         return;
     }
@@ -1131,7 +1152,7 @@ int forward(const na1d_head &h, float *loss, const void *x, const void *w, const
     NA1D_TRY((launch_logits<DT, false>(h, p.logits, a, s)));
     Finish e{};
     e.h = a.h, e.part = a.part, e.m_tiles = (int)p.m_tiles;
-    e.rows = h.N >= 4096 && !teaches ? 16 : h.N >= 1024 ? 4 : 1;
+    e.rows = teaches ? (h.N >= 8192 ? 4 : 1) : h.N >= 4096 ? 16 : h.N >= 1024 ? 4 : 1;          // a teacher of 100 entries in 1000 rows: 4 rows 68 us, 1 row 46
     e.ids = ids, e.ids_wide = h.ids_64, e.top = teaches ? h.top : 0, e.teacher = teacher, e.teacher_type = h.teacher_type;
     e.ignore = h.ignore_index, e.cosines = cosines, e.scale = h.scale, e.temperature = h.scale;
     e.cos_m = (float)cos(h.margin), e.sin_m = (float)sin(h.margin), e.threshold = (float)cos(M_PI - h.margin), e.drop = (float)(sin(M_PI - h.margin) * h.margin);
