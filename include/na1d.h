@@ -396,6 +396,8 @@ int na1d_train_context_backward(void *dx, const void *dctx, const void *x, const
  * A row whose target is ignore_index, or whose teacher has no entry, has loss 0 and no gradient and does not count in a mean
  * (0 if none counts).  Any other target outside [0, V), and a teacher's id of V or more, makes the row's loss NaN; it has no gradient.
  *   loss  : fp32 [N] (NA1D_HEAD_NONE) or [1] (_MEAN, _SUM); dloss the same in the backward
+ *   hits  : [N], or NULL: 1 where no class has a larger logit (cosine) than the target, which is taken without its margin; 0
+ *           elsewhere, where a row has no target, and for a teacher
  *   saved : what a forward leaves for its backward, na1d_head_saved_bytes() bytes; a forward needs it in any case
  *   dx, dw: 16-bit, packed [N, D] and [V * subcenters, D]; either may be NULL
  * Sums are in fp32; the gradients of the logits are rounded to 16 bits (fp16: scaled by a power of two first) before they
@@ -423,8 +425,8 @@ typedef struct na1d_head {
 } na1d_head;
 int64_t na1d_head_saved_bytes(const na1d_head *h);
 int64_t na1d_head_workspace_bytes(const na1d_head *h, int backward);
-int na1d_head_forward(const na1d_head *h, float *loss, const void *x, const void *w, const void *ids, const void *teacher, void *saved,
-                      int64_t saved_bytes, void *workspace, int64_t workspace_bytes, void *stream);
+int na1d_head_forward(const na1d_head *h, float *loss, uint8_t *hits, const void *x, const void *w, const void *ids, const void *teacher,
+                      void *saved, int64_t saved_bytes, void *workspace, int64_t workspace_bytes, void *stream);
 int na1d_head_backward(const na1d_head *h, void *dx, void *dw, const float *dloss, const void *x, const void *w, const void *ids, const void *saved,
                        int64_t saved_bytes, void *workspace, int64_t workspace_bytes, void *stream);
 

@@ -11,11 +11,12 @@ def softmax_targets(x, w, target, scale=1.0, ignore_index=-100):
     ok = target != ignore_index
     n, t = torch.arange(len(x), device=x.device), torch.where(ok, target, 0).long()
     lse = torch.logsumexp(z, 1)
-    rows = torch.where(ok, lse - z[n, t], 0.0)
     e = torch.exp(z - lse.unsqueeze(1))
     others = z.clone()
     others[n, t] = -math.inf
-    e[n, t] = -torch.sigmoid(torch.logsumexp(others, 1) - z[n, t])      # P - 1 without the difference
+    apart = torch.logsumexp(others, 1) - z[n, t]
+    rows = torch.where(ok, torch.logaddexp(apart, torch.zeros_like(apart)), 0.0)      # lse - z[t] and P - 1 without the differences
+    e[n, t] = -torch.sigmoid(apart)
     return rows, ok, torch.where(ok.unsqueeze(1), scale * e, 0.0)
 
 
@@ -48,11 +49,12 @@ def margin(x, w, target, m=0.2, scale=32.0, ignore_index=-100):
     z = scale * cosine
     z[n, t] = scale * moved
     lse = torch.logsumexp(z, 1)
-    rows = torch.where(ok, lse - z[n, t], 0.0)
     e = torch.exp(z - lse.unsqueeze(1))
     others = z.clone()
     others[n, t] = -math.inf
-    e[n, t] = -torch.sigmoid(torch.logsumexp(others, 1) - z[n, t]) * slope
+    apart = torch.logsumexp(others, 1) - z[n, t]
+    rows = torch.where(ok, torch.logaddexp(apart, torch.zeros_like(apart)), 0.0)
+    e[n, t] = -torch.sigmoid(apart) * slope
     e = torch.where(ok.unsqueeze(1), scale * e, 0.0)
     full = torch.zeros(len(x), V, K, dtype=torch.float64, device=x.device).scatter_(2, which.unsqueeze(2), e.unsqueeze(2))
     return rows, ok, full.view(-1, V * K), every

@@ -590,14 +590,14 @@ int64_t na1d_head_workspace_bytes(const na1d_head *h, int backward) {
     const int st = head_check(h);
     return st == NA1D_OK ? na1d::loss::scratch_bytes(*h, backward != 0) : st;
 }
-int na1d_head_forward(const na1d_head *h, float *loss, const void *x, const void *w, const void *ids, const void *teacher, void *saved,
-                      int64_t saved_bytes, void *workspace, int64_t workspace_bytes, void *stream) {
+int na1d_head_forward(const na1d_head *h, float *loss, uint8_t *hits, const void *x, const void *w, const void *ids, const void *teacher,
+                      void *saved, int64_t saved_bytes, void *workspace, int64_t workspace_bytes, void *stream) {
     const int st = head_check(h);
     if (st != NA1D_OK) return st;
     if (!loss || !x || !w || !ids || !saved || !workspace || (h->kind == NA1D_HEAD_TEACHER && !teacher)) return NA1D_ERR_NULL;
     if (misaligned(x) || misaligned(w) || misaligned(saved) || misaligned(workspace)) return NA1D_ERR_ALIGN;
     if (saved_bytes < na1d::loss::saved_bytes(*h) || workspace_bytes < na1d::loss::scratch_bytes(*h, false)) return NA1D_ERR_WORKSPACE;
-    return na1d::loss::run_forward(*h, loss, x, w, ids, teacher, saved, workspace, (hipStream_t)stream);
+    return na1d::loss::run_forward(*h, loss, hits, x, w, ids, teacher, saved, workspace, (hipStream_t)stream);
 }
 int na1d_head_backward(const na1d_head *h, void *dx, void *dw, const float *dloss, const void *x, const void *w, const void *ids, const void *saved,
                        int64_t saved_bytes, void *workspace, int64_t workspace_bytes, void *stream) {

@@ -237,7 +237,7 @@ int run_context_backward(void *dx, const void *dctx, const void *x, const void *
 namespace loss {
 int64_t saved_bytes(const na1d_head &h);
 int64_t scratch_bytes(const na1d_head &h, bool backward);
-int run_forward(const na1d_head &h, float *loss, const void *x, const void *w, const void *ids, const void *teacher, void *saved, void *ws, hipStream_t s);
+int run_forward(const na1d_head &h, float *loss, uint8_t *hits, const void *x, const void *w, const void *ids, const void *teacher, void *saved, void *ws, hipStream_t s);
 int run_backward(const na1d_head &h, void *dx, void *dw, const float *dloss, const void *x, const void *w, const void *ids, const void *saved, void *ws, hipStream_t s);
 }  // namespace loss
 

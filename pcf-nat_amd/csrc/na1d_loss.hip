@@ -326,6 +326,7 @@ struct Logits {
     f32x2 *part;
     const void *ids;                // targets, or NULL: no class is kept out
     int ids_wide;
+    f32x2 *at;                      // [N]: the target's product (cosines: over the weight's length) and which of its weight rows
     // backward
     Upstream up;
     const RowStat *stats;
@@ -418,7 +419,11 @@ logits_kernel(Logits a) {
 #pragma unroll
                     for (int i = 0; i < S::MT; ++i)
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) acc[i][j][k] = first + 16 * i + k == t ? kNegInf : acc[i][j][k];
+                        for (int k = 0; k < 4; ++k) {
+                            const bool here = first + 16 * i + k == t;
+                            if (here && r0 + row < a.h.N) a.at[r] = f32x2{acc[i][j][k], SUBS ? (float)(which[i][j] >> 8 * k & 0xffu) : 0.f};
+                            acc[i][j][k] = here ? kNegInf : acc[i][j][k];
+                        }
                 }
             }
             float top = kNegInf;
@@ -546,7 +551,7 @@ logits_kernel(Logits a) {
 // =============================================================================
 struct Finish {
     Head h;
-    const f32x2 *part;
+    const f32x2 *part, *at;
     int m_tiles, rows;              // rows to a workgroup, a power of two up to 16
     const void *ids;
     int ids_wide, top;              // teacher's entries of a row, 0: targets
@@ -558,6 +563,7 @@ struct Finish {
     RowStat *stats;
     float *coeff;                   // teacher: p - q of every entry, [N, top]
     float *loss;                    // [N]
+    uint8_t *hits;                  // [N], or NULL
 };
 __device__ inline float teacher_value(const void *p, int64_t i, int type) {
     if (type == NA1D_FP32) return reinterpret_cast<const float *>(p)[i];
@@ -572,12 +578,11 @@ template <class DT>
 __global__ void __launch_bounds__(kFinishThreads)
 finish_kernel(Finish a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    const int entries = a.top ? a.top : a.h.subs;
     f32x2 *met = reinterpret_cast<f32x2 *>(smem);                               // [lanes][rows]: 256 of them
-    float *z = reinterpret_cast<float *>(met + kFinishThreads);                 // [rows][entries], log2 domain
-    float *lse = z + a.rows * entries;                                          // [rows]
-    int *ids = reinterpret_cast<int *>(lse + a.rows);                           // teacher: [rows][entries] ...
-    float *share = reinterpret_cast<float *>(ids + a.rows * entries);           // ... and their q, before the sum is divided out
+    float *lse = reinterpret_cast<float *>(met + kFinishThreads);               // [rows]
+    float *z = lse + a.rows;                                                    // teacher, [rows][entries]: products,
+    int *ids = reinterpret_cast<int *>(z + a.rows * a.top);                     // classes,
+    float *share = reinterpret_cast<float *>(ids + a.rows * a.top);             // and their q
     const int R = a.rows, lanes = kFinishThreads / R, r = threadIdx.x & (R - 1), l = threadIdx.x / R;
     const int64_t r0 = (int64_t)blockIdx.x * R;
     {
@@ -591,18 +596,17 @@ finish_kernel(Finish a) {
         }
         met[threadIdx.x] = v;
     }
-    // logits of the entries: 16 lanes to an entry
+    // a teacher's entries: 16 lanes to an entry
     const int lane16 = threadIdx.x & 15;
-    for (int e = threadIdx.x >> 4; e < R * entries; e += kFinishThreads / 16) {
-        const int64_t row = r0 + e / entries;
-        const int k = e % entries;
+    for (int e = threadIdx.x >> 4; e < R * a.top; e += kFinishThreads / 16) {
+        const int64_t row = r0 + e / a.top;
+        const int k = e % a.top;
         float s = 0.f;
         int id = -1;
         if (row < a.h.N) {
-            id = load_id(a.ids, a.top ? row * a.top + k : row, a.ids_wide);
+            id = load_id(a.ids, row * a.top + k, a.ids_wide);
             if (id >= 0 && id < a.h.V) {
-                const int64_t wr = a.top ? id : (int64_t)id * a.h.subs + k;
-                const char *xr = a.h.x + row * a.h.x_pitch, *w = a.h.w + wr * a.h.w_pitch;
+                const char *xr = a.h.x + row * a.h.x_pitch, *w = a.h.w + id * a.h.w_pitch;
 #pragma unroll 4
                 for (int c = lane16 * 8; c < a.h.D; c += 128) {
                     const u32x4 p = *reinterpret_cast<const u32x4 *>(xr + 2 * c), q = *reinterpret_cast<const u32x4 *>(w + 2 * c);
@@ -613,14 +617,10 @@ finish_kernel(Finish a) {
                         s = __builtin_fmaf(u.y, v.y, s);
                     }
                 }
-                if (a.cosines) s *= a.h.inv_w[wr];
             }
         }
         s = sum_of_16(s);
-        if (lane16 == 0) {
-            z[e] = s;
-            if (a.top) ids[e] = id;
-        }
+        if (lane16 == 0) z[e] = s, ids[e] = id;
     }
     __syncthreads();
     // The tiles' sums meet, R rows at a time.
@@ -632,6 +632,7 @@ finish_kernel(Finish a) {
         }
         __syncthreads();
     }
+    const float largest = met[threadIdx.x & (R - 1)].x;                         // of the other classes' logits, for threads below R
     if ((int)threadIdx.x < R) lse[threadIdx.x] = met[threadIdx.x].x + __builtin_log2f(met[threadIdx.x].y);
     __syncthreads();
     if (!a.top) {
@@ -640,11 +641,11 @@ finish_kernel(Finish a) {
             const int64_t raw = a.ids_wide ? reinterpret_cast<const int64_t *>(a.ids)[row] : (int64_t)reinterpret_cast<const int32_t *>(a.ids)[row];
             RowStat st = {__builtin_inff(), 0.f, kFar, -1};
             float loss = raw == a.ignore ? 0.f : __builtin_nanf("");
+            bool hit = false;
             if (raw != a.ignore && raw >= 0 && raw < a.h.V) {
-                float best = z[threadIdx.x * entries], slope = 1.f;
-                st.sub = 0;
-                for (int k = 1; k < entries; ++k)
-                    if (z[threadIdx.x * entries + k] > best) best = z[threadIdx.x * entries + k], st.sub = k;
+                float best = a.at[row].x, slope = 1.f;
+                st.sub = (int)a.at[row].y;
+                hit = best * (a.h.scale2 * (a.cosines ? a.h.inv_x[row] : 1.f)) >= largest;         // as the tiles' maxima were worked out
                 if (a.cosines) {
                     const float c = best * a.h.inv_x[row], sine2 = 1.f - c * c;
                     best = c;
@@ -665,6 +666,7 @@ finish_kernel(Finish a) {
             }
             a.stats[row] = st;
             a.loss[row] = loss;
+            if (a.hits) a.hits[row] = hit;
         }
     } else {
         // A teacher's row: a wave to each.
@@ -711,6 +713,7 @@ finish_kernel(Finish a) {
                 st.sub = 0;
             }
             if (lane == 0) a.stats[row] = st, a.loss[row] = loss;
+            if (lane == 0 && a.hits) a.hits[row] = 0;
         }
     }
 }
@@ -1061,11 +1064,12 @@ inline Plan plan_of(const na1d_head &h) {
     return t_large < t * (narrow ? 0.75 : 1.) ? large : p;
 }
 struct ForwardScratch {
-    int64_t part, rows, bytes;
+    int64_t part, rows, at, bytes;
     ForwardScratch(const na1d_head &h, const Plan &p) {
         part = 0;
         rows = round_up(p.m_tiles * h.N * (int64_t)sizeof(f32x2), 256);
-        bytes = rows + round_up(4 * h.N, 256);
+        at = rows + round_up(4 * h.N, 256);
+        bytes = at + round_up(h.N * (int64_t)sizeof(f32x2), 256);
     }
 };
 struct BackwardScratch {
@@ -1134,7 +1138,7 @@ inline Head head_of(const na1d_head &h, const void *x, const void *w, const char
 }
 
 template <class DT>
-int forward(const na1d_head &h, float *loss, const void *x, const void *w, const void *ids, const void *teacher, char *saved, char *ws, hipStream_t s) {
+int forward(const na1d_head &h, float *loss, uint8_t *hits, const void *x, const void *w, const void *ids, const void *teacher, char *saved, char *ws, hipStream_t s) {
     const Saved o(h);
     const Plan p = plan_of(h);
     const ForwardScratch f(h, p);
@@ -1148,10 +1152,10 @@ int forward(const na1d_head &h, float *loss, const void *x, const void *w, const
     }
     a.classes = (int)h.V;
     a.part = reinterpret_cast<f32x2 *>(ws + f.part);
-    a.ids = teaches ? nullptr : ids, a.ids_wide = h.ids_64;
+    a.ids = teaches ? nullptr : ids, a.ids_wide = h.ids_64, a.at = reinterpret_cast<f32x2 *>(ws + f.at);
     NA1D_TRY((launch_logits<DT, false>(h, p.logits, a, s)));
     Finish e{};
-    e.h = a.h, e.part = a.part, e.m_tiles = (int)p.m_tiles;
+    e.h = a.h, e.part = a.part, e.at = a.at, e.m_tiles = (int)p.m_tiles;
     e.rows = teaches ? (h.N >= 8192 ? 4 : 1) : h.N >= 4096 ? 16 : h.N >= 1024 ? 4 : 1;          // a teacher of 100 entries in 1000 rows: 4 rows 68 us, 1 row 46
     e.ids = ids, e.ids_wide = h.ids_64, e.top = teaches ? h.top : 0, e.teacher = teacher, e.teacher_type = h.teacher_type;
     e.ignore = h.ignore_index, e.cosines = cosines, e.scale = h.scale, e.temperature = h.scale;
@@ -1159,7 +1163,8 @@ int forward(const na1d_head &h, float *loss, const void *x, const void *w, const
     e.stats = reinterpret_cast<RowStat *>(saved + o.stats), e.coeff = reinterpret_cast<float *>(saved + o.coeff);
     float *rows = reinterpret_cast<float *>(ws + f.rows);
     e.loss = h.reduction == NA1D_HEAD_NONE ? loss : rows;
-    const size_t lds = kFinishThreads * sizeof(f32x2) + 4 * (size_t)e.rows * (teaches ? 3 * h.top + 1 : h.subcenters + 1);
+    e.hits = hits;
+    const size_t lds = kFinishThreads * sizeof(f32x2) + 4 * (size_t)e.rows * (3 * e.top + 1);
     NA1D_TRY(launch<finish_kernel<DT>>((unsigned)ceil_div<int64_t>(h.N, e.rows), kFinishThreads, lds, s, e));
     if (h.reduction == NA1D_HEAD_NONE) return NA1D_OK;
     float *count = reinterpret_cast<float *>(saved + o.count);
@@ -1227,9 +1232,10 @@ int64_t scratch_bytes(const na1d_head &h, bool back) {
     const Plan p = plan_of(h);
     return back ? BackwardScratch(h, p).bytes : ForwardScratch(h, p).bytes;
 }
-int run_forward(const na1d_head &h, float *loss, const void *x, const void *w, const void *ids, const void *teacher, void *saved, void *ws, hipStream_t s) {
-    return h.dtype == NA1D_BF16 ? forward<BF16>(h, loss, x, w, ids, teacher, (char *)saved, (char *)ws, s)
-                                : forward<FP16>(h, loss, x, w, ids, teacher, (char *)saved, (char *)ws, s);
+int run_forward(const na1d_head &h, float *loss, uint8_t *hits, const void *x, const void *w, const void *ids, const void *teacher, void *saved, void *ws,
+                hipStream_t s) {
+    return h.dtype == NA1D_BF16 ? forward<BF16>(h, loss, hits, x, w, ids, teacher, (char *)saved, (char *)ws, s)
+                                : forward<FP16>(h, loss, hits, x, w, ids, teacher, (char *)saved, (char *)ws, s);
 }
 int run_backward(const na1d_head &h, void *dx, void *dw, const float *dloss, const void *x, const void *w, const void *ids, const void *saved, void *ws, hipStream_t s) {
     return h.dtype == NA1D_BF16 ? backward<BF16>(h, (char *)dx, (char *)dw, dloss, x, w, ids, (const char *)saved, (char *)ws, s)

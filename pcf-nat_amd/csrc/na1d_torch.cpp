@@ -396,10 +396,12 @@ struct HeadLoss : torch::autograd::Function<HeadLoss> {
         return {dx, dw, Tensor(), Tensor(), Tensor(), Tensor()};
     }
 };
-MaybeTensor head(const Tensor &x, const Tensor &weight, const Tensor &ids, const MaybeTensor &teacher, int kind, double scale, double margin, int64_t ignore, int reduction) {
+MaybeTensor head(const Tensor &x, const Tensor &weight, const Tensor &ids, const MaybeTensor &teacher, const MaybeTensor &hits, int kind, double scale, double margin,
+                 int64_t ignore, int reduction) {
     if (!plain_call() || !plain(x) || !half_type(x) || x.dim() < 1 || !x.is_contiguous() || !x.numel()) return std::nullopt;
     if (!on(weight, x) || weight.scalar_type() != x.scalar_type() || weight.dim() < 2 || weight.dim() > 3 || weight.size(-1) != x.size(-1)) return std::nullopt;
     if (!on(ids, x) || !index_type(ids)) return std::nullopt;
+    if (hits && (!on(*hits, x) || hits->scalar_type() != at::kBool || hits->numel() != x.numel() / x.size(-1))) return std::nullopt;
     int type = 0;
     if (teacher) {
         if (!on(*teacher, x) || (teacher->scalar_type() != at::kFloat && !half_type(*teacher)) || teacher->dim() < 1) return std::nullopt;
@@ -411,7 +413,7 @@ MaybeTensor head(const Tensor &x, const Tensor &weight, const Tensor &ids, const
     const c10::DeviceGuard guard(x.device());
     const Tensor loss = at::empty(reduction == NA1D_HEAD_NONE ? x.sizes().slice(0, x.dim() - 1) : at::IntArrayRef{}, x.options().dtype(at::kFloat));
     const Tensor saved = bytes_of(saved_bytes, x), ws = bytes_of(ws_bytes, x);
-    if (na1d_head_forward(&h, (float *)ptr(loss), ptr(x), ptr(weight), ptr(ids), teacher ? ptr(*teacher) : nullptr, ptr(saved), saved_bytes, ptr(ws), ws_bytes,
+    if (na1d_head_forward(&h, (float *)ptr(loss), hits ? (uint8_t *)ptr(*hits) : nullptr, ptr(x), ptr(weight), ptr(ids), teacher ? ptr(*teacher) : nullptr, ptr(saved), saved_bytes, ptr(ws), ws_bytes,
                           stream_of(x)) != NA1D_OK)
         return std::nullopt;
     if (!at::GradMode::is_enabled() || !(x.requires_grad() || weight.requires_grad())) return loss;

@@ -118,7 +118,7 @@ def load():
     lib.na1d_head_saved_bytes.argtypes = [_ptr]
     lib.na1d_head_workspace_bytes.argtypes = [_ptr, _int]
     lib.na1d_head_forward.restype = lib.na1d_head_backward.restype = _int
-    lib.na1d_head_forward.argtypes = [_ptr] * 7 + [_i64, _ptr, _i64, _ptr]
+    lib.na1d_head_forward.argtypes = [_ptr] * 8 + [_i64, _ptr, _i64, _ptr]
     lib.na1d_head_backward.argtypes = [_ptr] * 8 + [_i64, _ptr, _i64, _ptr]
     lib.na1d_fused_backward_noalloc.restype = _int
     lib.na1d_fused_backward_noalloc.argtypes = [_ptr] * 12 + [_i64] * 6 + [_f32, _int, _ptr]

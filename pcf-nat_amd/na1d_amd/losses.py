@@ -58,11 +58,14 @@ def _sizes(h, backward):
     return saved, ws
 
 
-def head_forward(x, weight, ids, teacher, kind, scale, margin, ignore_index, reduction):
-    """Loss, and what the backward needs of the forward.  Arguments as checked by the functions below."""
+def head_forward(x, weight, ids, teacher, hits, kind, scale, margin, ignore_index, reduction):
+    """Loss, and what the backward needs of the forward; `hits` (bool, a value to a row, or None) is written to.  Arguments as checked
+    by the functions below."""
     shape = x.shape[:-1] if reduction == 0 else ()
     loss = torch.empty(shape, dtype=torch.float32, device=x.device)
     if x.numel() == 0:
+        if hits is not None:
+            hits.zero_()
         return loss.zero_(), torch.empty(0, dtype=torch.uint8, device=x.device)
     h = _head(x, weight, ids, teacher, kind, scale, margin, ignore_index, reduction)
     xr, wr, ids = _rows(x), _rows(weight), ids.contiguous()
@@ -71,8 +74,8 @@ def head_forward(x, weight, ids, teacher, kind, scale, margin, ignore_index, red
     nsaved, nws = _sizes(h, 0)
     saved, ws = (torch.empty(n, dtype=torch.uint8, device=x.device) for n in (nsaved, nws))
     with torch.cuda.device(x.device):
-        _lib.check(_lib.load().na1d_head_forward(ctypes.byref(h), _lib._p(loss), _lib._p(xr), _lib._p(wr), _lib._p(ids), _lib._p(teacher),
-                                                 _lib._p(saved), nsaved, _lib._p(ws), nws, _lib._stream(x)), "na1d_head_forward")
+        _lib.check(_lib.load().na1d_head_forward(ctypes.byref(h), _lib._p(loss), _lib._p(hits), _lib._p(xr), _lib._p(wr), _lib._p(ids),
+                                                 _lib._p(teacher), _lib._p(saved), nsaved, _lib._p(ws), nws, _lib._stream(x)), "na1d_head_forward")
     return loss, saved
 
 
@@ -96,8 +99,8 @@ def head_backward(dloss, x, weight, ids, teacher, saved, kind, scale, margin, ig
 
 class _HeadLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, ids, teacher, *args):
-        loss, saved = head_forward(x, weight, ids, teacher, *args)
+    def forward(ctx, x, weight, ids, teacher, hits, *args):
+        loss, saved = head_forward(x, weight, ids, teacher, hits, *args)
         ctx.save_for_backward(x, weight, ids, teacher, saved)
         ctx.args = args
         return loss
@@ -108,13 +111,16 @@ class _HeadLoss(torch.autograd.Function):
         x, weight, ids, teacher, saved = ctx.saved_tensors
         want = ctx.needs_input_grad[:2]
         dx, dw = head_backward(dloss, x, weight, ids, teacher, saved, *ctx.args, *want)
-        return (dx if want[0] else None, dw if want[1] else None) + (None,) * 7
+        return (dx if want[0] else None, dw if want[1] else None) + (None,) * 8
 
 
-def _loss(x, weight, ids, teacher, *args):
+def _loss(x, weight, ids, teacher, return_hits, *args):
     nodes = _lib.nodes()
-    out = None if nodes is None else nodes.head(x, weight, ids, teacher, *args)
-    return _HeadLoss.apply(x, weight, ids, teacher, *args) if out is None else out
+    hits = torch.empty(x.shape[:-1], dtype=torch.bool, device=x.device) if return_hits else None
+    out = None if nodes is None else nodes.head(x, weight, ids, teacher, hits, *args)
+    if out is None:
+        out = _HeadLoss.apply(x, weight, ids, teacher, hits, *args)
+    return (out, hits) if return_hits else out
 
 
 def check_arguments(x, weight, ids, reduction, ids_shape, weight_dims=(2,), what="target"):
@@ -141,28 +147,40 @@ def check_arguments(x, weight, ids, reduction, ids_shape, weight_dims=(2,), what
         raise _lib.NA1DError("weight must have at least one class")
 
 
-def linear_cross_entropy(x, weight, target, scale=1.0, ignore_index=-100, reduction="mean"):
+def check_teacher(x, weight, teacher_logits, teacher_ids, reduction):
+    if teacher_logits.shape != teacher_ids.shape or teacher_logits.dim() < 1 or not 0 < teacher_logits.shape[-1] <= MAX_TOP:
+        raise ValueError("teacher_logits must be like teacher_ids, with 1 to %d entries to a row; got %s" % (MAX_TOP, list(teacher_logits.shape)))
+    if teacher_logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise TypeError("teacher_logits must be float32, bfloat16 or float16, got %s" % teacher_logits.dtype)
+    check_arguments(x, weight, teacher_ids, reduction, x.shape[:-1] + teacher_logits.shape[-1:], what="teacher_ids")
+    if teacher_logits.device != x.device:
+        raise _lib.NA1DError("x and teacher_logits must be on one device")
+
+
+def linear_cross_entropy(x, weight, target, scale=1.0, ignore_index=-100, reduction="mean", return_hits=False):
     """Softmax cross entropy of the logits ``scale * x @ weight.t()``.
 
     ``x [..., D]``, ``weight [V, D]``, ``target [...]`` (int32 or int64).  Rows whose target is ``ignore_index`` have loss 0 and no
     gradient and do not count in the mean (0 if no row counts); any other target outside ``[0, V)`` makes its row's loss NaN
     and has no gradient.  ``reduction``: "mean", "sum" or "none" (a loss to a row).  The rows themselves have to be finite, ignored
-    ones too: they take part in the weight's gradient with a factor of zero.
+    ones too: they take part in the weight's gradient with a factor of zero.  ``return_hits``: also a bool to a row that says whether
+    no class has a larger logit than the target (a row without a target is none).
     """
     check_arguments(x, weight, target, reduction, x.shape[:-1])
-    return _loss(x, weight, target, None, _TARGETS, float(scale), 0.0, int(ignore_index), _REDUCTIONS[reduction])
+    return _loss(x, weight, target, None, return_hits, _TARGETS, float(scale), 0.0, int(ignore_index), _REDUCTIONS[reduction])
 
 
-def margin_cross_entropy(x, weight, target, margin=0.2, scale=32.0, ignore_index=-100, reduction="mean"):
+def margin_cross_entropy(x, weight, target, margin=0.2, scale=32.0, ignore_index=-100, reduction="mean", return_hits=False):
     """Additive angular margin softmax (models/SoftMaxLoss.py:99-138) on the cosines of ``x [..., D]`` and ``weight [V, D]`` or
     ``[V, K, D]``, where a class's cosine is that of the nearest of its K rows (the lowest of equals).
 
     The target's cosine cos(theta) becomes cos(theta + margin) where theta + margin < pi, else cos(theta) - margin sin(pi - margin);
     the derivative takes the squared sine of theta as 1e-6 at least.  ``0 <= margin < pi / 2``.  A row of zeros has cosine 0
-    with everything and no gradient.  Other arguments as in :func:`linear_cross_entropy`.
+    with everything and no gradient.  Hits are by the cosines, without the margin.  Other arguments as in
+    :func:`linear_cross_entropy`.
     """
     check_arguments(x, weight, target, reduction, x.shape[:-1], weight_dims=(2, 3))
-    return _loss(x, weight, target, None, _MARGIN, float(scale), float(margin), int(ignore_index), _REDUCTIONS[reduction])
+    return _loss(x, weight, target, None, return_hits, _MARGIN, float(scale), float(margin), int(ignore_index), _REDUCTIONS[reduction])
 
 
 def linear_distillation(x, weight, teacher_logits, teacher_ids, temperature=1.0, reduction="mean"):
@@ -175,11 +193,5 @@ def linear_distillation(x, weight, teacher_logits, teacher_ids, temperature=1.0,
     and no gradient and does not count in the mean (0 if no row counts).  An id of V or more makes its row's loss NaN, without a
     gradient.  A class that is there twice has both entries' shares.
     """
-    if teacher_logits.shape != teacher_ids.shape or teacher_logits.dim() < 1 or not 0 < teacher_logits.shape[-1] <= MAX_TOP:
-        raise ValueError("teacher_logits must be like teacher_ids, with 1 to %d entries to a row; got %s" % (MAX_TOP, list(teacher_logits.shape)))
-    if teacher_logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
-        raise TypeError("teacher_logits must be float32, bfloat16 or float16, got %s" % teacher_logits.dtype)
-    check_arguments(x, weight, teacher_ids, reduction, x.shape[:-1] + teacher_logits.shape[-1:], what="teacher_ids")
-    if teacher_logits.device != x.device:
-        raise _lib.NA1DError("x and teacher_logits must be on one device")
-    return _loss(x, weight, teacher_ids, teacher_logits.detach(), _TEACHER, float(temperature), 0.0, 0, _REDUCTIONS[reduction])
+    check_teacher(x, weight, teacher_logits, teacher_ids, reduction)
+    return _loss(x, weight, teacher_ids, teacher_logits.detach(), False, _TEACHER, float(temperature), 0.0, 0, _REDUCTIONS[reduction])

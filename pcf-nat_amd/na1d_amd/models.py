@@ -33,6 +33,7 @@ import torch.nn.functional as F
 from .dense import global_attention
 from .encoder import embed as embed_natively
 from .fused import na1d_fused, na1d_fused_qkv
+from .losses import margin_cross_entropy
 from .nattn import getNA1dFunction
 from .train import layer as train_layer, pooled, pooled_of, pooling_context
 
@@ -793,10 +794,16 @@ def pcf_nat_6x4(**kw):
 
 
 class ArcMarginSubCenters(nn.Module):
-    """AAM-softmax with sub-centres (models/SoftMaxLoss.py:99-138)."""
+    """AAM-softmax with sub-centres (models/SoftMaxLoss.py:99-138).
 
-    def __init__(self, emb_size=192, n_classes=5994, m=0.2, s=32.0, subcenters=3):
+    ``head="fused"``: through :func:`na1d_amd.losses.margin_cross_entropy`, with products in ``dtype`` and neither the cosines nor the
+    logits in memory (an angle that the margin takes next to pi or 0 has a bounded derivative there); its ``acc1`` counts a
+    target that shares the first place."""
+
+    def __init__(self, emb_size=192, n_classes=5994, m=0.2, s=32.0, subcenters=3, head="torch", dtype=torch.bfloat16):
         super().__init__()
+        assert head in ("torch", "fused")
+        self.head, self.dtype = head, dtype
         self.s, self.m = s, m
         self.W = nn.Parameter(torch.empty(n_classes, subcenters, emb_size))
         nn.init.xavier_uniform_(self.W)
@@ -804,6 +811,9 @@ class ArcMarginSubCenters(nn.Module):
         self.th, self.mm = math.cos(math.pi - m), math.sin(math.pi - m) * m
 
     def forward(self, x, labels):
+        if self.head == "fused":
+            loss, hits = margin_cross_entropy(x.to(self.dtype), self.W.to(self.dtype), labels.long(), self.m, self.s, return_hits=True)
+            return loss, hits.sum()
         cosine = torch.einsum("ne,cse->ncs", F.normalize(x, dim=-1), F.normalize(self.W, dim=-1)).amax(-1)
         with torch.no_grad():
             acc1 = (cosine.argmax(1) == labels).sum()

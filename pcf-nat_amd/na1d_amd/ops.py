@@ -9,7 +9,8 @@ wrappers ``ana_qk`` / ``ana_av``).  The same names, schemas and semantics are re
 so code written against ``torch.ops.na_cuda.*`` runs unchanged; importing this module is what registers them.
 
 Beyond the reference, the fused operator is registered the same way:
-``na_cuda::na1d_fused_forward`` / ``na_cuda::na1d_fused_backward`` and the wrapper :func:`na1d_fused_op`.
+``na_cuda::na1d_fused_forward`` / ``na_cuda::na1d_fused_backward`` and the wrapper :func:`na1d_fused_op`; the dense
+operator and the losses over many classes (``na_cuda::class_loss_forward`` / ``class_loss_backward``) too.
 """
 from __future__ import annotations
 
@@ -18,7 +19,7 @@ from typing import Optional
 import torch
 from torch import Tensor
 
-from . import _lib
+from . import _lib, losses
 
 NAMESPACE = "na_cuda"
 _SIG = "int N, int T, int C, int win_size, int left"
@@ -289,3 +290,72 @@ def global_attention_op(q: Tensor, k: Tensor, v: Tensor, num_heads: int = 1, t_v
                         scale: float = 1.0) -> Tensor:
     """:func:`na1d_amd.dense.global_attention` through the registered op (traceable by ``torch.compile``)."""
     return getattr(torch.ops, NAMESPACE).global_attention_forward(q, k, v, t_valid, num_heads, float(scale))[0]
+
+
+# --------------------------------------------------------------------------- losses over many classes
+_HEAD = "int kind, float scale, float margin, int ignore_index, int reduction"
+_library.define("class_loss_forward(Tensor x, Tensor weight, Tensor ids, Tensor? teacher, %s) -> (Tensor, Tensor)" % _HEAD)
+_library.define("class_loss_backward(Tensor dloss, Tensor x, Tensor weight, Tensor ids, Tensor? teacher, Tensor saved, %s, bool want_x, "
+                "bool want_weight) -> (Tensor, Tensor)" % _HEAD)
+
+
+def _class_loss_forward(x, weight, ids, teacher, *args):
+    return losses.head_forward(x, weight, ids, teacher, None, *args)
+
+
+def _class_loss_forward_fake(x, weight, ids, teacher, kind, scale, margin, ignore_index, reduction):
+    loss = torch.empty(x.shape[:-1] if reduction == 0 else (), dtype=torch.float32, device=x.device)
+    h = losses._head(x, weight, ids, teacher, kind, scale, margin, ignore_index, reduction)
+    h.x_stride = h.w_stride = h.D
+    return loss, torch.empty(losses._sizes(h, 0)[0] if x.numel() else 0, dtype=torch.uint8, device=x.device)
+
+
+def _class_loss_backward_fake(dloss, x, weight, ids, teacher, saved, kind, scale, margin, ignore_index, reduction, want_x, want_weight):
+    return (torch.empty(x.shape if want_x else (0,), dtype=x.dtype, device=x.device),
+            torch.empty(weight.shape if want_weight else (0,), dtype=weight.dtype, device=x.device))
+
+
+_library.impl("class_loss_forward", _class_loss_forward, "CUDA")
+_library.impl("class_loss_backward", losses.head_backward, "CUDA")
+torch.library.register_fake(NAMESPACE + "::class_loss_forward", _class_loss_forward_fake, lib=_library)
+torch.library.register_fake(NAMESPACE + "::class_loss_backward", _class_loss_backward_fake, lib=_library)
+
+
+def _class_loss_setup(ctx, inputs, output):
+    x, weight, ids, teacher, *ctx.args = inputs
+    ctx.teaches = teacher is not None
+    ctx.save_for_backward(*[t for t in (x, weight, ids, output[1], teacher) if t is not None])
+
+
+def _class_loss_autograd(ctx, dloss, _dsaved):
+    x, weight, ids, saved, *teacher = ctx.saved_tensors
+    want = ctx.needs_input_grad[:2]
+    dx, dw = getattr(torch.ops, NAMESPACE).class_loss_backward(dloss, x, weight, ids, teacher[0] if ctx.teaches else None, saved, *ctx.args, *want)
+    return (dx if want[0] else None, dw if want[1] else None) + (None,) * 7
+
+
+torch.library.register_autograd(NAMESPACE + "::class_loss_forward", _class_loss_autograd, setup_context=_class_loss_setup, lib=_library)
+
+
+def _class_loss(x, weight, ids, teacher, *args):
+    return getattr(torch.ops, NAMESPACE).class_loss_forward(x, weight, ids, teacher, *args)[0]
+
+
+def linear_cross_entropy_op(x: Tensor, weight: Tensor, target: Tensor, scale: float = 1.0, ignore_index: int = -100, reduction: str = "mean") -> Tensor:
+    """:func:`na1d_amd.losses.linear_cross_entropy` through the registered op (traceable by ``torch.compile``)."""
+    losses.check_arguments(x, weight, target, reduction, x.shape[:-1])
+    return _class_loss(x, weight, target, None, losses._TARGETS, float(scale), 0.0, ignore_index, losses._REDUCTIONS[reduction])
+
+
+def margin_cross_entropy_op(x: Tensor, weight: Tensor, target: Tensor, margin: float = 0.2, scale: float = 32.0, ignore_index: int = -100,
+                            reduction: str = "mean") -> Tensor:
+    """:func:`na1d_amd.losses.margin_cross_entropy` through the registered op."""
+    losses.check_arguments(x, weight, target, reduction, x.shape[:-1], weight_dims=(2, 3))
+    return _class_loss(x, weight, target, None, losses._MARGIN, float(scale), float(margin), ignore_index, losses._REDUCTIONS[reduction])
+
+
+def linear_distillation_op(x: Tensor, weight: Tensor, teacher_logits: Tensor, teacher_ids: Tensor, temperature: float = 1.0,
+                           reduction: str = "mean") -> Tensor:
+    """:func:`na1d_amd.losses.linear_distillation` through the registered op."""
+    losses.check_teacher(x, weight, teacher_logits, teacher_ids, reduction)
+    return _class_loss(x, weight, teacher_ids, teacher_logits.detach(), losses._TEACHER, float(temperature), 0.0, 0, losses._REDUCTIONS[reduction])

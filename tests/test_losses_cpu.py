@@ -92,7 +92,7 @@ def test_sizes_that_the_native_call_refuses(status, change):
     lib, h = _lib.load(), _head(**change)
     ref, fake = ctypes.byref(h), ctypes.c_void_p(0x1000)
     assert lib.na1d_head_saved_bytes(ref) == status and lib.na1d_head_workspace_bytes(ref, 1) == status
-    assert lib.na1d_head_forward(ref, fake, fake, fake, fake, fake, fake, 1 << 40, fake, 1 << 40, None) == status
+    assert lib.na1d_head_forward(ref, fake, None, fake, fake, fake, fake, fake, 1 << 40, fake, 1 << 40, None) == status
     assert lib.na1d_head_backward(ref, fake, fake, fake, fake, fake, fake, fake, 1 << 40, fake, 1 << 40, None) == status
 
 
@@ -101,7 +101,7 @@ def test_pointers_and_workspaces_that_the_native_call_refuses():
     ref, ok, odd, big = ctypes.byref(h), ctypes.c_void_p(0x1000), ctypes.c_void_p(0x1008), 1 << 40
     saved, ws, back = lib.na1d_head_saved_bytes(ref), lib.na1d_head_workspace_bytes(ref, 0), lib.na1d_head_workspace_bytes(ref, 1)
     assert min(saved, ws, back) > 0
-    f = lambda *a: lib.na1d_head_forward(ref, *a, None)
+    f = lambda loss, *a: lib.na1d_head_forward(ref, loss, None, *a, None)
     for i in (0, 1, 2, 3, 5):
         a = [ok, ok, ok, ok, None, ok]
         a[i] = None
@@ -114,7 +114,7 @@ def test_pointers_and_workspaces_that_the_native_call_refuses():
     assert b(ok, ok, ok, ok, ok, ok, ok, saved - 1, ok, big) == -10 and b(ok, ok, ok, ok, ok, ok, ok, big, ok, back - 1) == -10
     assert b(None, None, ok, ok, ok, ok, ok, big, ok, big) == 0                     # nothing asked for
     teacher = _head(kind=2, top=4)
-    assert lib.na1d_head_forward(ctypes.byref(teacher), ok, ok, ok, ok, None, ok, big, ok, big, None) == -1
+    assert lib.na1d_head_forward(ctypes.byref(teacher), ok, None, ok, ok, ok, None, ok, big, ok, big, None) == -1
 
 
 def test_arguments_that_the_functions_refuse():
