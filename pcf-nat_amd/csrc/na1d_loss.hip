@@ -985,14 +985,15 @@ struct Saved {
 using Few = Shape<1, 2, 4, 1, 4>;             // 64 x 32
 using Batch = Shape<2, 4, 2, 2, 3>;           // 64 x 128
 using Many = Shape<4, 4, 2, 2, 2>;            // 128 x 128
+using Wide = Shape<6, 4, 2, 2, 2>;            // 192 x 128
 using Vast = Shape<8, 4, 2, 4, 2>;            // 256 x 256
 
-enum Pick { kFew, kBatch, kMany, kVast };
+enum Pick { kFew, kBatch, kMany, kWide, kVast };
 struct Tiling {
     Pick pick;
     int bm, bn;
     int wn;                                   // waves along the rows
-    Tiling(Pick p = kFew) : pick(p) { bm = p == kVast ? 256 : p == kMany ? 128 : 64, bn = p == kVast ? 256 : p == kFew ? 32 : 128, wn = p == kVast ? 4 : p == kFew ? 1 : 2; }
+    Tiling(Pick p = kFew) : pick(p) { bm = p == kVast ? 256 : p == kWide ? 192 : p == kMany ? 128 : 64, bn = p == kVast ? 256 : p == kFew ? 32 : 128, wn = p == kVast ? 4 : p == kFew ? 1 : 2; }
     int64_t tiles(int64_t m, int64_t n) const { return (m + bm - 1) / bm * ((n + bn - 1) / bn); }
 };
 struct Plan {
@@ -1008,17 +1009,29 @@ constexpr int64_t kMostDz = 256ll << 20;      // bytes of dz: what the last leve
 constexpr int kFullLaunch = 512;              // workgroups: two to a CU
 
 // How long a launch of `first` workgroups of `first_steps` and then `second` of `second_steps` takes, in us: CUs hold one workgroup
-// of 256 x 256 or two smaller ones, and take the next as they get free.  A step of 64 takes the former 1.6 us and two of 128 x 128
-// side by side 0.93 (1340 and 1150 TFLOP/s), the rest of a tile 4.9 and 2.7: fitted to forwards of 8192 x 65536 and 16384 x 32768
-// logits with 1024 and 512 channels (972 and 567 us against 1124 and 650), which it also orders at sizes where the larger tiles do
-// not fill their last round: 1000 x 20000, 1024 channels 70 us against 62; 500 x 60000 73 against 86.
-inline double time_of(Pick p, int64_t first, int64_t first_steps, int64_t second = 0, int64_t second_steps = 0) {
-    const int64_t slots = p == kVast ? 256 : 512;
-    const double step = p == kVast ? 1.6 : 0.93, rest = p == kVast ? 4.9 : 2.7, a = first_steps * step + rest, b = second_steps * step + rest;
-    const int64_t rounds = first / slots, over = first % slots;
+// of 256 x 256 or two smaller ones, and take the next as they get free.  What a step of 64 and the rest of a tile take is
+// fitted to forwards of 4096 x 32768 logits with 64, 256 and 1024 channels (64 x 128: 99, 152, 361 us; 128 x 128: 62, 101, 263; 192 x 128: 52, 92,
+// 250; 256 x 256: 61, 93, 235), that is 990, 1280, 1340 and 1460 TFLOP/s between the ends.  The model also orders what does
+// not fill a round: 1024 x 8000, 512 channels 25, 21, 25 and 27 us; 128 x 20000, 1024 channels 22, 25, 26, 36; 2000 x 1000 17, 20, 22, 29.
+struct Cost {
+    double step, rest;
+    int64_t slots;
+};
+inline Cost cost_of(Pick p) {
+    switch (p) {
+        case kMany: return {0.84, 3.0, 512};
+        case kWide: return {1.2, 3.5, 512};
+        case kVast: return {1.47, 6.0, 256};
+        default: return {0.55, 2.55, 512};
+    }
+}
+inline double time_of(Pick p, int64_t first, int64_t first_steps, int64_t second = 0, int64_t second_steps = 0, double more = 0.) {
+    const Cost c = cost_of(p);
+    const double a = first_steps * c.step + c.rest + more, b = second_steps * c.step + c.rest + more;
+    const int64_t rounds = first / c.slots, over = first % c.slots;
     if (!second) return (rounds + (over > 0)) * a;
     double busy[2] = {(rounds + 1) * a, rounds * a};
-    const int64_t wide[2] = {over, slots - over};
+    const int64_t wide[2] = {over, c.slots - over};
     for (int64_t left = second; left > 0;) {
         const int next = over && busy[0] < busy[1] ? 0 : 1;
         left -= wide[next];
@@ -1028,40 +1041,44 @@ inline double time_of(Pick p, int64_t first, int64_t first_steps, int64_t second
 }
 inline Plan plan_of(const na1d_head &h) {
     Plan p{};
+    // Logits.  Several weight rows to a class keep two sets of sums, and the backward of a margin its tile's cosines: there is no room
+    // for them in the larger tiles.
     const int64_t steps = ceil_div<int64_t>(h.D, kStep);
-    // Logits.  Several weight rows to a class keep two sets of sums, and the backward of a margin twice its tile's cosines: no room in
-    // the larger tiles.
-    const Tiling many(kMany), vast(kVast);
-    const int64_t in_many = many.tiles(h.V, h.N), in_vast = vast.tiles(h.V, h.N);
-    const bool larger = time_of(kVast, in_vast, steps) < time_of(kMany, in_many, steps);
-    p.logits = Tiling(h.N <= 32 ? kFew : in_many < kFullLaunch || h.subcenters > 1 ? kBatch : larger ? kVast : kMany);
-    p.back = Tiling(p.logits.pick == kVast && h.kind == NA1D_HEAD_MARGIN ? kMany : p.logits.pick);
+    auto shortest = [&](Pick largest) {
+        Pick best = kBatch;
+        double least = 1e30;
+        for (const Pick pick : {kBatch, kMany, kWide, kVast}) {
+            const double t = time_of(pick, Tiling(pick).tiles(h.V, h.N), steps);
+            if (pick <= largest && t < least) best = pick, least = t;
+        }
+        return Tiling(h.N <= 32 ? kFew : best);
+    };
+    p.logits = shortest(h.subcenters > 1 ? kBatch : kVast);
+    p.back = h.kind == NA1D_HEAD_MARGIN ? shortest(h.subcenters > 1 ? kBatch : kMany) : p.logits;
     p.m_tiles = ceil_div<int64_t>(h.V, p.logits.bm);
     const int64_t fits = std::min<int64_t>(kMostDz / (2 * h.N * h.subcenters), (1 << 20) / h.subcenters);
     p.plane = std::max<int64_t>(fits / 256 * 256, 256);
     p.ranges = ceil_div(h.V, p.plane);
     p.plane = std::min(round_up(h.V, kStep), round_up(ceil_div(h.V, p.ranges), 256));         // ranges alike
     p.ranges = ceil_div(h.V, p.plane);
-    // Products.  Channels are cut in tiles of 64 where that leaves fewer idle than 128.
-    const bool narrow = round_up(h.D, 64) < round_up(h.D, 128);
+    // Products: the tiles and splits that take least, with what the sums of splits cost in memory at 4 TB/s.
     auto split = [&](int64_t tiles, int64_t length, int64_t most, int &splits, int &per) {
         const int64_t all = ceil_div<int64_t>(length, kStep), want = std::max<int64_t>(1, std::min<int64_t>(most / tiles, all / 4));
         per = (int)(ceil_div(all, want) * kStep);
         splits = (int)ceil_div<int64_t>(length, per);
     };
-    auto products = [&](Plan &q, Pick x, Pick w) {
-        q.dx = Tiling(x), q.dw = Tiling(w);
-        const int64_t most = w == kVast ? kFullLaunch / 2 : kFullLaunch, dx_tiles = q.dx.tiles(h.D, h.N), dw_tiles = h.subcenters * q.dw.tiles(h.D, q.plane);
+    double least = 1e30;
+    for (const Pick pick : {kBatch, kMany, kWide, kVast}) {
+        Plan q = p;
+        q.dx = Tiling(h.N <= 32 ? kFew : pick), q.dw = Tiling(pick);
+        const int64_t dx_tiles = q.dx.tiles(h.D, h.N), dw_tiles = h.subcenters * q.dw.tiles(h.D, q.plane), most = cost_of(pick).slots;
         split(dx_tiles, q.plane, most, q.dx_splits, q.dx_per);
         split(dw_tiles, h.N, most, q.dw_splits, q.dw_per);
-        // and what the sums of splits cost in memory, at 4 TB/s
         const double fold = (8. * q.dx_splits * h.N * h.D + (q.dw_splits > 1 ? 8. * q.dw_splits * h.subcenters * q.plane * h.D : 0.)) / 4.0e6;
-        return fold + time_of(w, dx_tiles * q.dx_splits, (int64_t)h.subcenters * q.dx_per / kStep, dw_tiles * q.dw_splits, q.dw_per / kStep);
-    };
-    Plan large = p;
-    const double t_large = h.N > 128 ? products(large, kVast, kVast) : 1e30;
-    const double t = products(p, h.N <= 32 ? kFew : narrow ? kBatch : kMany, narrow ? kBatch : kMany);
-    return t_large < t * (narrow ? 0.75 : 1.) ? large : p;
+        const double t = fold + time_of(pick, dx_tiles * q.dx_splits, (int64_t)h.subcenters * q.dx_per / kStep, dw_tiles * q.dw_splits, q.dw_per / kStep, 2.);          // whose ends store more
+        if (t < least && (h.N > 32 || pick <= kMany)) p = q, least = t;
+    }
+    return p;
 }
 struct ForwardScratch {
     int64_t part, rows, at, bytes;
@@ -1118,6 +1135,7 @@ template <class DT, bool BACK> int launch_logits(const na1d_head &h, const Tilin
         case kFew: return launch_logits_of<DT, Few, BACK>(h, a, s);
         case kBatch: return launch_logits_of<DT, Batch, BACK>(h, a, s);
         case kMany: return launch_logits_of<DT, Many, BACK>(h, a, s);
+        case kWide: return launch_logits_of<DT, Wide, BACK>(h, a, s);
         default: return launch_logits_of<DT, Vast, BACK>(h, a, s);
     }
 }
@@ -1126,6 +1144,7 @@ template <class DT, class SX, class SW> int launch_products_of(const Product &dx
     return launch<products_kernel<DT, SX, SW>>(nx + nw, SX::kThreadsOf, std::max(SX::kLds, SW::kLds), s, dx, dw, nx, nw);
 }
 template <class DT> int launch_products(const Plan &p, const Product &dx, const Product &dw, hipStream_t s) {
+    if (p.dx.pick == kWide) return launch_products_of<DT, Wide, Wide>(dx, dw, s);
     if (p.dx.pick == kVast) return launch_products_of<DT, Vast, Vast>(dx, dw, s);
     if (p.dx.pick == kFew) return p.dw.pick == kBatch ? launch_products_of<DT, Few, Batch>(dx, dw, s) : launch_products_of<DT, Few, Many>(dx, dw, s);
     return p.dw.pick == kBatch ? launch_products_of<DT, Batch, Batch>(dx, dw, s) : launch_products_of<DT, Many, Many>(dx, dw, s);      // both by the channels

@@ -16,7 +16,7 @@ SIZES = [  # rows, channels, classes: one of each; below, at and above the tiles
     (257, 328, 1211), (1030, 40, 300), (4100, 64, 130), (300, 1032, 501),
 ]
 LARGE = [  # launches that fill the card: tiles of 128 x 128 and of 256 x 256, products of either, several ranges of classes
-    (1000, 264, 9001), (2100, 72, 5003), (700, 1032, 13000), (2050, 512, 16390), (16390, 16, 8300),
+    (1000, 264, 9001), (2100, 72, 5003), (700, 1032, 13000), (2050, 512, 16390), (16390, 16, 8300), (1500, 192, 9001), (1024, 512, 8000),
 ]
 
 
