@@ -17,6 +17,7 @@ SIZES = [  # rows, channels, classes: one of each; below, at and above the tiles
 ]
 LARGE = [  # launches that fill the card: tiles of 128 x 128 and of 256 x 256, products of either, several ranges of classes
     (1000, 264, 9001), (2100, 72, 5003), (700, 1032, 13000), (2050, 512, 16390), (16390, 16, 8300), (1500, 192, 9001), (1024, 512, 8000),
+    (1500, 192, 3000), (1500, 960, 9000), (2050, 1024, 12000), (3000, 1024, 16000),
 ]
 
 
@@ -80,7 +81,7 @@ def test_margin(size, subs, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=NAMES)
-@pytest.mark.parametrize("size,subs", [(s, 1) for s in LARGE] + [((2100, 72, 3003), 2), ((16390, 16, 4200), 3)], ids=lambda s: str(s))
+@pytest.mark.parametrize("size,subs", [(s, 1) for s in LARGE] + [((2100, 72, 3003), 2), ((16390, 16, 4200), 3), ((260, 1024, 3000), 3), ((260, 512, 3000), 3)], ids=lambda s: str(s))
 def test_margin_of_large_launches(size, subs, dtype):
     _margin(size, subs, dtype)
 
