@@ -335,6 +335,22 @@ struct Logits {
     float *col_part;                // cosines: sums of dz * cosine over a wave's rows: [n_tiles * WN, subs, plane]
 };
 
+// 1 / length of a tile's weight rows c .. c + 3 (classes from c0 on, `there` of them; 0 for those that there are not).  The places
+// behind the last class belong to `saved` too.
+template <bool SUBS> __device__ inline f32x4 inverse_lengths(const Head &h, int c0, int c, int there, int sub) {
+    f32x4 v;
+    if constexpr (SUBS) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = h.inv_w[(int64_t)(c0 + min(c + k, there - 1)) * h.subs + sub];
+    } else {
+        v = *reinterpret_cast<const f32x4 *>(h.inv_w + c0 + c);
+    }
+    if (c + 4 > there)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = c + k < there ? v[k] : 0.f;
+    return v;
+}
+
 // Logits of a tile of classes (M) by rows (N).
 template <class DT, class S, bool COS, bool SUBS, bool BACK>
 __global__ void __launch_bounds__(S::kThreadsOf, 2)
@@ -370,12 +386,7 @@ logits_kernel(Logits a) {
         if constexpr (COS) {
 #pragma unroll
             for (int i = 0; i < S::MT; ++i) {
-                f32x4 inv;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int c = min(first + 16 * i + r, there - 1);
-                    inv[r] = a.h.inv_w[(int64_t)(c0 + c) * (SUBS ? a.h.subs : 1) + sub];
-                }
+                const f32x4 inv = inverse_lengths<SUBS>(a.h, c0, first + 16 * i, there, sub);
 #pragma unroll
                 for (int j = 0; j < S::NT; ++j) {
                     acc[i][j] *= inv;
@@ -497,20 +508,25 @@ logits_kernel(Logits a) {
                 if constexpr (COS && !SUBS) sums[i] += d * acc[i][j];
                 acc[i][j] = d;
             }
+            if constexpr (COS) __builtin_amdgcn_sched_barrier(0);               // a column of tiles at a time: registers
         }
         const int width = (int)max((int64_t)0, min((int64_t)32 * S::MT, 2 * (a.plane - col)));
+        f32x4 invs[SUBS ? S::MT : 1];
 #pragma unroll 1
         for (int sub = 0; sub < subs; ++sub) {
-            f32x4 inv[COS ? S::MT : 1];
             if constexpr (COS)
 #pragma unroll
                 for (int i = 0; i < S::MT; ++i) {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const float v = a.h.inv_w[(int64_t)(c0 + min(first + 16 * i + k, there - 1)) * subs + sub];
-                        inv[i][k] = v == kNoNorm ? 0.f : v;
-                    }
                     if constexpr (SUBS) sums[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    f32x4 inv = inverse_lengths<SUBS>(a.h, c0, first + 16 * i, there, sub);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) inv[k] = inv[k] == kNoNorm ? 0.f : inv[k];
+                    if constexpr (SUBS) {
+                        invs[i] = inv;
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < S::NT; ++j) acc[i][j] *= inv;
+                    }
                 }
 #pragma unroll
             for (int j = 0; j < S::NT; ++j) {
@@ -522,8 +538,8 @@ logits_kernel(Logits a) {
 #pragma unroll
                         for (int k = 0; k < 4; ++k) d[k] = (which[i][j] >> 8 * k & 0xffu) == (uint32_t)sub ? d[k] : 0.f;
                         sums[i] += d * best[i][j];
+                        d *= invs[i];
                     }
-                    if constexpr (COS) d *= inv[i];
                     o[i] = narrow4<DT>(d);
                 }
                 const int at = (int)((16 * (wn * S::NT + j) + n) * pitch + 2 * (sub * a.plane + col));
@@ -1041,8 +1057,8 @@ inline double time_of(Pick p, int64_t first, int64_t first_steps, int64_t second
 }
 inline Plan plan_of(const na1d_head &h) {
     Plan p{};
-    // Logits.  Several weight rows to a class keep two sets of sums, and the backward of a margin its tile's cosines: there is no room
-    // for them in the larger tiles.
+    // Logits.  Several weight rows to a class keep two sets of sums, and the backward of a margin sums over its tile's classes: there is no
+    // room for them in the larger tiles.
     const int64_t steps = ceil_div<int64_t>(h.D, kStep);
     auto shortest = [&](Pick largest) {
         Pick best = kBatch;
@@ -1054,7 +1070,7 @@ inline Plan plan_of(const na1d_head &h) {
         return Tiling(h.N <= 32 ? kFew : best);
     };
     p.logits = shortest(h.subcenters > 1 ? kBatch : kVast);
-    p.back = h.kind == NA1D_HEAD_MARGIN ? shortest(h.subcenters > 1 ? kBatch : kMany) : p.logits;
+    p.back = h.kind == NA1D_HEAD_MARGIN ? shortest(h.subcenters > 1 ? kBatch : kWide) : p.logits;
     p.m_tiles = ceil_div<int64_t>(h.V, p.logits.bm);
     const int64_t fits = std::min<int64_t>(kMostDz / (2 * h.N * h.subcenters), (1 << 20) / h.subcenters);
     p.plane = std::max<int64_t>(fits / 256 * 256, 256);
@@ -1123,7 +1139,7 @@ template <auto KERNEL, class... A> int launch(unsigned grid, unsigned block, siz
 template <class DT, class S, bool BACK> int launch_logits_of(const na1d_head &h, const Logits &a, hipStream_t s) {
     const unsigned grid = (unsigned)(a.m_tiles * a.n_tiles);
     if (h.kind != NA1D_HEAD_MARGIN) return launch<logits_kernel<DT, S, false, false, BACK>>(grid, S::kThreadsOf, S::kLds, s, a);
-    if constexpr (!BACK || S::MT * S::NT <= 16)
+    if constexpr (!BACK || S::MT * S::NT <= 24)
         if (h.subcenters == 1) return launch<logits_kernel<DT, S, true, false, BACK>>(grid, S::kThreadsOf, S::kLds, s, a);
     if constexpr (S::MT * S::NT <= 8) return launch<logits_kernel<DT, S, true, true, BACK>>(grid, S::kThreadsOf, S::kLds, s, a);
     return NA1D_ERR_UNSUPPORTED;
