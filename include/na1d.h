@@ -404,7 +404,7 @@ int na1d_train_context_backward(void *dx, const void *dctx, const void *x, const
  * are multiplied.  Nothing uses atomics: results are the same from call to call.
  * D % 8 == 0; x, w, dx, dw, saved and the workspace 16-byte aligned, strides multiples of 8 and at least D.  Limits
  * (NA1D_ERR_UNSUPPORTED): N up to 2^20, V * subcenters up to 2^24, w_stride * subcenters and x_stride up to 2^20, N * V, N * D and
- * V * subcenters * D up to 2^37, subcenters up to 255, top up to NA1D_HEAD_MAX_TOP.
+ * V * subcenters * D up to 2^36, subcenters up to 255, top up to NA1D_HEAD_MAX_TOP.
  */
 #define NA1D_FP32 2              /* teacher_type only */
 #define NA1D_HEAD_TARGETS 0

@@ -8,7 +8,7 @@
 // of two numbers that are nearly the same.  The forward is one product x W^T whose tiles leave as a maximum and a sum of
 // exponentials to a row (logits_kernel), and a kernel that puts a row's tiles together (finish_kernel).  The backward works the
 // logits out again, a range of classes at a time, rounds dz to the operands' type - what a head that keeps its logits would have
-// handed its products - and multiplies it twice (product_kernel): by W for dx, transposed by x for dW.
+// handed its products - and multiplies it twice (products_kernel): by W for dx, transposed by x for dW.
 #include <atomic>
 #include <cmath>
 
@@ -381,12 +381,20 @@ logits_kernel(Logits a) {
         for (int i = 0; i < S::MT; ++i)
 #pragma unroll
             for (int j = 0; j < S::NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        f32x4 ahead[SUBS ? S::MT : 1];                                          // asked for in front of the product
+        if constexpr (SUBS)
+#pragma unroll
+            for (int i = 0; i < S::MT; ++i) ahead[i] = inverse_lengths<SUBS>(a.h, c0, first + 16 * i, there, sub);
         if (SUBS && sub) barrier_lds();
         accumulate<DT, S>(acc, ws, xs, reader, reader, steps, lds, wave, wm, wn);
         if constexpr (COS) {
 #pragma unroll
             for (int i = 0; i < S::MT; ++i) {
-                const f32x4 inv = inverse_lengths<SUBS>(a.h, c0, first + 16 * i, there, sub);
+                f32x4 inv;
+                if constexpr (SUBS)
+                    inv = ahead[i];
+                else
+                    inv = inverse_lengths<SUBS>(a.h, c0, first + 16 * i, there, sub);
 #pragma unroll
                 for (int j = 0; j < S::NT; ++j) {
                     acc[i][j] *= inv;
@@ -475,12 +483,20 @@ logits_kernel(Logits a) {
 #pragma unroll
             for (int i = 0; i < S::MT; ++i) sums[i] = f32x4{0.f, 0.f, 0.f, 0.f};
         const float base = a.up.base(), common = base * a.up.up(base);
+        RowStat row_stats[S::NT];                                               // all on their way at once
+        float row_inv[S::NT];
+#pragma unroll
+        for (int j = 0; j < S::NT; ++j) {
+            const int64_t r = min(r0 + 16 * (wn * S::NT + j) + n, a.h.N - 1);
+            row_stats[j] = a.stats[r];
+            row_inv[j] = COS ? a.h.inv_x[r] : 1.f;
+        }
 #pragma unroll
         for (int j = 0; j < S::NT; ++j) {
             const int row = 16 * (wn * S::NT + j) + n;
             const int64_t r = min(r0 + row, a.h.N - 1);
-            const RowStat rg = a.stats[r];
-            const float ix = COS ? a.h.inv_x[r] : 1.f, c2 = a.h.scale2 * ix;
+            const RowStat rg = row_stats[j];
+            const float ix = row_inv[j], c2 = a.h.scale2 * ix;
             float f = common * (a.up.count ? 1.f : a.up.dloss[r]) * ix;
             if (r0 + row >= a.h.N || rg.sub < 0 || (COS && ix == kNoNorm)) f = 0.f;           // rows behind the last have no share in the sums
             const float e = f * rg.at_target;
@@ -575,7 +591,7 @@ struct Finish {
     int teacher_type;               // NA1D_BF16, NA1D_FP16, NA1D_FP32
     int64_t ignore;
     int cosines;
-    float cos_m, sin_m, threshold, drop, scale, temperature;
+    float cos_m, sin_m, threshold, drop, temperature;
     RowStat *stats;
     float *coeff;                   // teacher: p - q of every entry, [N, top]
     float *loss;                    // [N]
@@ -1193,7 +1209,7 @@ int forward(const na1d_head &h, float *loss, uint8_t *hits, const void *x, const
     e.h = a.h, e.part = a.part, e.at = a.at, e.m_tiles = (int)p.m_tiles;
     e.rows = teaches ? (h.N >= 8192 ? 4 : 1) : h.N >= 4096 ? 16 : h.N >= 1024 ? 4 : 1;          // a teacher of 100 entries in 1000 rows: 4 rows 68 us, 1 row 46
     e.ids = ids, e.ids_wide = h.ids_64, e.top = teaches ? h.top : 0, e.teacher = teacher, e.teacher_type = h.teacher_type;
-    e.ignore = h.ignore_index, e.cosines = cosines, e.scale = h.scale, e.temperature = h.scale;
+    e.ignore = h.ignore_index, e.cosines = cosines, e.temperature = h.scale;
     e.cos_m = (float)cos(h.margin), e.sin_m = (float)sin(h.margin), e.threshold = (float)cos(M_PI - h.margin), e.drop = (float)(sin(M_PI - h.margin) * h.margin);
     e.stats = reinterpret_cast<RowStat *>(saved + o.stats), e.coeff = reinterpret_cast<float *>(saved + o.coeff);
     float *rows = reinterpret_cast<float *>(ws + f.rows);

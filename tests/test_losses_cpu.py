@@ -85,7 +85,7 @@ def _head(**kw):
     (-3, {"D": 60}), (-3, {"D": 0}), (-5, {"x_stride": 56}), (-6, {"w_stride": 68}), (-11, {"scale": 0.0}), (-11, {"scale": math.nan}),
     (-11, {"scale": math.inf}), (-11, {"kind": 1, "margin": -0.1}), (-11, {"kind": 1, "margin": 1.6}), (-11, {"kind": 1, "margin": math.nan}),
     (-8, {"subcenters": 2}), (-8, {"kind": 1, "subcenters": 256}), (-5, {"kind": 2, "top": 0}), (-8, {"kind": 2, "top": 257}), (-5, {"subcenters": 0}),
-    (-8, {"N": (1 << 20) + 1}), (-8, {"V": (1 << 24) + 1}), (-8, {"N": 1 << 20, "V": 1 << 18}), (-8, {"x_stride": (1 << 20) + 8}),
+    (-8, {"N": (1 << 20) + 1}), (-8, {"V": (1 << 24) + 1}), (-8, {"N": 1 << 20, "V": (1 << 16) + 1}), (-8, {"x_stride": (1 << 20) + 8}),
     (-8, {"V": 1 << 22, "D": 1 << 16, "x_stride": 1 << 16, "w_stride": 1 << 16}),
 ], ids=str)
 def test_sizes_that_the_native_call_refuses(status, change):
