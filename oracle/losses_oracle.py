@@ -94,6 +94,21 @@ def margin_gradients(x, w, e, g):
         ix * more(e.abs() * f.unsqueeze(1) @ uw.abs(), ux), iw * more((e.abs() * f.unsqueeze(1)).t() @ ux.abs(), uw))
 
 
+def undecided(x, w, e, cosines, g):
+    """What margin_gradients' two results may be off by where a class's two nearest rows are no further apart than their cosines'
+    errors in fp32 (D roundings of the sum's magnitudes and the last ones, for either): the class's share goes to either of the
+    two.  That is at most all of it, counted at both."""
+    V, K, D = w.shape
+    if K == 1:
+        return 0.0, 0.0
+    most = (unit(x.double()).abs() @ unit(w.double().view(V * K, D)).abs().t()).view(-1, V, K).amax(2)
+    two, at = cosines.view(-1, V, K).topk(2, 2)
+    close = two[..., 0] - two[..., 1] <= 2 * 2.0 ** -24 * (D * most + 4)
+    share = (e.view(-1, V, K).abs().sum(2) * close).unsqueeze(2).expand(-1, -1, 2)
+    both = torch.zeros(len(x), V, K, dtype=torch.float64, device=x.device).scatter_(2, at, share).view(-1, V * K)
+    return margin_gradients(x, w, both, g)[2](torch.ones(len(x), dtype=torch.float64, device=x.device))
+
+
 def logit_bound(x, w, scale):
     """How far a row's logits and the logarithm of its sum may be off in fp32: D roundings of a product's sums, relative to its
     magnitudes, and a few of the logarithm's, relative to itself (base 2: at most 2^-20 of it)."""

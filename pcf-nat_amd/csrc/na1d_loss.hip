@@ -11,6 +11,7 @@
 // handed its products - and multiplies it twice (products_kernel): by W for dx, transposed by x for dW.
 #include <atomic>
 #include <cmath>
+#include <type_traits>
 
 #include "na1d_encoder.h"
 
@@ -71,6 +72,37 @@ template <int EXTENT, int NW, bool TURNED> struct Source {
             }
             load_to_lds<16, kReadShared>(src, to + (c + wave) * kChunk, off);
         }
+    }
+};
+// A tile of weight rows of which K belong to a class: the 16-row tiles of a wave (MT of them, a multiple of K) are K of the same 16
+// classes, one behind the other, so that a lane has all of a class's products.  (Row operands only.)
+template <int EXTENT, int NW, int MT, int K> struct ClassSource {
+    static constexpr int kLoads = EXTENT * kPieceRow / kChunk / NW, kBytes = EXTENT * kPieceRow;
+    static_assert(EXTENT * kPieceRow % (kChunk * NW) == 0 && NW % 4 == 0 && MT % K == 0, "whole chunks, whole classes");
+    const char *at;
+    int64_t bytes;
+    int width, lane_at, unit;
+    int chunk_at[kLoads];
+    // `classes`: those that exist from the tile's first one on, row_pitch bytes from row to row
+    __device__ inline void init(const char *first, int64_t classes, int64_t row_pitch, int64_t row_width, int wave, int lane) {
+        const int pitch = (int)row_pitch * K;
+        at = first;
+        width = (int)row_width;
+        bytes = classes > 0 ? (classes - 1) * (int64_t)pitch + (K - 1) * row_pitch + row_width : 0;
+        unit = ((lane & 7) ^ swizzle<false>(8 * wave + (lane >> 3))) * 16;
+        lane_at = (lane >> 3) * pitch + unit;
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+            const int chunk = j * NW + wave, tile = chunk >> 1, of_wave = tile % MT;
+            chunk_at[j] = (tile / MT * (16 * MT / K) + of_wave / K * 16 + (chunk & 1) * 8) * pitch + of_wave % K * (int)row_pitch;
+        }
+    }
+    __device__ inline void load(LDS_PTR(char) to, int s, int wave) const {
+        const int64_t left = bytes - s * kPieceRow;
+        const Rsrc src = make_rsrc(at + s * kPieceRow, (int)(left < 0 ? 0 : left < (1 << 30) ? left : (1 << 30)));
+        const int from = s * kPieceRow + unit < width ? lane_at : kNowhere;
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) load_to_lds<16, kReadShared>(src, to + (j * NW + wave) * kChunk, from + chunk_at[j]);
     }
 };
 // Operands of the 16 x 16 x 32 product out of such a tile: 16 of its extent (number t) and half h of the step's 64.
@@ -337,9 +369,9 @@ struct Logits {
 
 // 1 / length of a tile's weight rows c .. c + 3 (classes from c0 on, `there` of them; 0 for those that there are not).  The places
 // behind the last class belong to `saved` too.
-template <bool SUBS> __device__ inline f32x4 inverse_lengths(const Head &h, int c0, int c, int there, int sub) {
+template <int SUBS> __device__ inline f32x4 inverse_lengths(const Head &h, int c0, int c, int there, int sub) {
     f32x4 v;
-    if constexpr (SUBS) {
+    if constexpr (SUBS != 0) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] = h.inv_w[(int64_t)(c0 + min(c + k, there - 1)) * h.subs + sub];
     } else {
@@ -351,54 +383,60 @@ template <bool SUBS> __device__ inline f32x4 inverse_lengths(const Head &h, int 
     return v;
 }
 
-// Logits of a tile of classes (M) by rows (N).
-template <class DT, class S, bool COS, bool SUBS, bool BACK>
+// Logits of a tile of classes (M) by rows (N).  SUBS: 0, one weight row to a class; 2 and more, that many, side by side in a lane's
+// sums (ClassSource); 1, any number, one product after the other with the largest kept (and which, a byte to a value).
+// 4000 x 20000 classes of 2 rows, 512 channels, bf16: forward 322 us one after the other in tiles of 64 x 128, 222 us side by side in
+// tiles of 128 x 128 (backward 706 and 654 us); 12562 x 2166 of 2, 224 channels: 98 and 73 us (175 and 153 us).
+template <class DT, class S, bool COS, int SUBS, bool BACK>
 __global__ void __launch_bounds__(S::kThreadsOf, 2)
 logits_kernel(Logits a) {
+    constexpr bool LOOP = SUBS == 1;
+    constexpr int K = SUBS > 1 ? SUBS : 1, CT = S::MT / K, BC = S::BM / K;     // rows in a lane's sums, 16-class tiles of a wave, classes of the tile
     extern __shared__ __attribute__((aligned(16))) char smem[];
     LDS_PTR(char) lds = (LDS_PTR(char))smem;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
     const int wm = wave % S::WM, wn = wave / S::WM;
     int mt, nt;
     tile_of(xcd_item(blockIdx.x, gridDim.x), a.m_tiles, a.n_tiles, mt, nt);
-    const int c0 = a.class0 + mt * S::BM, r0 = nt * S::BN;                     // first class and row
+    const int c0 = a.class0 + mt * BC, r0 = nt * S::BN;                        // first class and row
     const int there = min(a.class0 + a.classes, a.h.V) - c0;                   // classes of the tile that exist
-    Source<S::BM, S::kWavesOf, false> ws;
+    const int subs = SUBS ? a.h.subs : 1;
+    std::conditional_t<(K > 1), ClassSource<S::BM, S::kWavesOf, S::MT, K>, Source<S::BM, S::kWavesOf, false>> ws;
     Source<S::BN, S::kWavesOf, false> xs;
     xs.init(a.h.x + r0 * a.h.x_pitch, min(S::BN, a.h.N - r0), a.h.x_pitch, 2 * (int64_t)a.h.D, wave, lane);
     Reader<false> reader;
     reader.init(n, g);
     const int steps = (a.h.D + kStep - 1) / kStep;
     f32x4 acc[S::MT][S::NT];
-    f32x4 best[SUBS ? S::MT : 1][SUBS ? S::NT : 1];                            // over the sub-centres, and which
-    uint32_t which[SUBS ? S::MT : 1][SUBS ? S::NT : 1];                        // a byte to a value
-    const int first = 16 * wm * S::MT + 4 * g;                                 // this lane's class of the tile for i = 0
+    f32x4 best[LOOP ? S::MT : 1][LOOP ? S::NT : 1];
+    uint32_t which[LOOP ? S::MT : 1][LOOP ? S::NT : 1];
+    const int first = 16 * wm * CT + 4 * g;                                    // this lane's class of the tile in its first 16-class tile
 #pragma unroll 1
-    for (int sub = 0; sub < (SUBS ? a.h.subs : 1); ++sub) {
-        const int64_t pitch = a.h.w_pitch * (SUBS ? a.h.subs : 1);
-        ws.init(a.h.w + c0 * pitch + sub * a.h.w_pitch, min(S::BM, there), pitch, 2 * (int64_t)a.h.D, wave, lane);
+    for (int sub = 0; sub < (LOOP ? subs : 1); ++sub) {
+        const char *rows = a.h.w + (int64_t)c0 * subs * a.h.w_pitch + sub * a.h.w_pitch;
+        ws.init(rows, min(BC, there), K > 1 ? a.h.w_pitch : a.h.w_pitch * subs, 2 * (int64_t)a.h.D, wave, lane);
 #pragma unroll
         for (int i = 0; i < S::MT; ++i)
 #pragma unroll
             for (int j = 0; j < S::NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-        f32x4 ahead[SUBS ? S::MT : 1];                                          // asked for in front of the product
-        if constexpr (SUBS)
+        f32x4 ahead[LOOP ? S::MT : 1];                                          // asked for in front of the product
+        if constexpr (LOOP)
 #pragma unroll
             for (int i = 0; i < S::MT; ++i) ahead[i] = inverse_lengths<SUBS>(a.h, c0, first + 16 * i, there, sub);
-        if (SUBS && sub) barrier_lds();
+        if (LOOP && sub) barrier_lds();
         accumulate<DT, S>(acc, ws, xs, reader, reader, steps, lds, wave, wm, wn);
         if constexpr (COS) {
 #pragma unroll
             for (int i = 0; i < S::MT; ++i) {
                 f32x4 inv;
-                if constexpr (SUBS)
+                if constexpr (LOOP)
                     inv = ahead[i];
                 else
-                    inv = inverse_lengths<SUBS>(a.h, c0, first + 16 * i, there, sub);
+                    inv = inverse_lengths<SUBS>(a.h, c0, first + 16 * (i / K), there, i % K);
 #pragma unroll
                 for (int j = 0; j < S::NT; ++j) {
                     acc[i][j] *= inv;
-                    if constexpr (SUBS) {
+                    if constexpr (LOOP) {
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
                             const bool better = sub == 0 || acc[i][j][r] > best[i][j][r] || acc[i][j][r] != acc[i][j][r];
@@ -410,53 +448,66 @@ logits_kernel(Logits a) {
             }
         }
     }
-    if constexpr (SUBS) {
+    // Logits of 16-class tile p by the rows of column j, and (SUBS) of which weight row of the class each is.
+    auto logits_of = [&](int p, int j, uint32_t &of) {
+        f32x4 v = LOOP ? best[LOOP ? p : 0][LOOP ? j : 0] : acc[p * K][j];
+        of = LOOP ? which[LOOP ? p : 0][LOOP ? j : 0] : 0u;
 #pragma unroll
-        for (int i = 0; i < S::MT; ++i)
+        for (int i = 1; i < K; ++i)
 #pragma unroll
-            for (int j = 0; j < S::NT; ++j) acc[i][j] = best[i][j];
-    }
+            for (int r = 0; r < 4; ++r) {
+                const float o = acc[p * K + i][j][r];
+                const bool better = o > v[r] || o != o;
+                v[r] = better ? o : v[r];
+                of = better ? (of & ~(0xffu << 8 * r)) | (uint32_t)i << 8 * r : of;
+            }
+        return v;
+    };
 
     if constexpr (!BACK) {
         barrier_lds();                                                          // the operands' place is taken over
-        LDS_PTR(f32x2) met = (LDS_PTR(f32x2))lds;                             // [WM][BN]
+        LDS_PTR(f32x2) met = (LDS_PTR(f32x2))lds;                               // [WM][BN]
 #pragma unroll
         for (int j = 0; j < S::NT; ++j) {
             const int row = 16 * (wn * S::NT + j) + n;
             const int64_t r = min(r0 + row, a.h.N - 1);
             const float c2 = a.h.scale2 * (COS ? a.h.inv_x[r] : 1.f);
-            if (there < S::BM) {
+            f32x4 v[CT];
+            uint32_t of[CT];
 #pragma unroll
-                for (int i = 0; i < S::MT; ++i)
+            for (int p = 0; p < CT; ++p) v[p] = logits_of(p, j, of[p]);
+            if (there < BC) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) acc[i][j][k] = first + 16 * i + k < there ? acc[i][j][k] : kNegInf;
+                for (int p = 0; p < CT; ++p)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) v[p][k] = first + 16 * p + k < there ? v[p][k] : kNegInf;
             }
             if (a.ids) {
                 const int64_t t = (int64_t)load_id(a.ids, r, a.ids_wide) - c0;
-                const bool hit = t >= 16 * wm * S::MT && t < 16 * (wm + 1) * S::MT;
+                const bool hit = t >= 16 * wm * CT && t < 16 * (wm + 1) * CT;
                 if (__builtin_amdgcn_ballot_w64(hit)) {
 #pragma unroll
-                    for (int i = 0; i < S::MT; ++i)
+                    for (int p = 0; p < CT; ++p)
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
-                            const bool here = first + 16 * i + k == t;
-                            if (here && r0 + row < a.h.N) a.at[r] = f32x2{acc[i][j][k], SUBS ? (float)(which[i][j] >> 8 * k & 0xffu) : 0.f};
-                            acc[i][j][k] = here ? kNegInf : acc[i][j][k];
+                            const bool here = first + 16 * p + k == t;
+                            if (here && r0 + row < a.h.N) a.at[r] = f32x2{v[p][k], (float)(of[p] >> 8 * k & 0xffu)};
+                            v[p][k] = here ? kNegInf : v[p][k];
                         }
                 }
             }
             float top = kNegInf;
 #pragma unroll
-            for (int i = 0; i < S::MT; ++i)
+            for (int p = 0; p < CT; ++p)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) top = __builtin_fmaxf(top, acc[i][j][k]);
+                for (int k = 0; k < 4; ++k) top = __builtin_fmaxf(top, v[p][k]);
             top = xor_max(top) * c2;
             const float off = top == kNegInf ? 0.f : top;
             float sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < S::MT; ++i)
+            for (int p = 0; p < CT; ++p)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][k], c2, -off));
+                for (int k = 0; k < 4; ++k) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(v[p][k], c2, -off));
             sum = xor_sum(sum);
             if (g == 0) met[wm * S::BN + row] = f32x2{top, sum};
         }
@@ -473,11 +524,10 @@ logits_kernel(Logits a) {
             a.part[(int64_t)mt * a.h.N + r0 + row] = v;
         }
     } else {
-        const int subs = SUBS ? a.h.subs : 1;
         const int64_t pitch = 2 * a.plane * subs;                               // bytes of a row of dz
-        const int col = mt * S::BM + 16 * wm * S::MT;                           // this wave's first column of the range
+        const int col = mt * BC + 16 * wm * CT;                                 // this wave's first column of the range
         const Rsrc out = make_rsrc(a.dz + r0 * pitch, (int)((int64_t)min(S::BN, a.h.N - r0) * pitch));
-        // dz for weights of length 1; in `best` stay the cosines that came with it
+        // dz for weights of length 1 takes the products' place (LOOP: the largest ones stay in `best`); sums of dz times the cosine
         f32x4 sums[COS ? S::MT : 1];
         if constexpr (COS)
 #pragma unroll
@@ -501,79 +551,108 @@ logits_kernel(Logits a) {
             if (r0 + row >= a.h.N || rg.sub < 0 || (COS && ix == kNoNorm)) f = 0.f;           // rows behind the last have no share in the sums
             const float e = f * rg.at_target;
             const int64_t t = (int64_t)rg.target - c0;
-            const bool hit = t >= 16 * wm * S::MT && t < 16 * (wm + 1) * S::MT;
+            const bool hit = t >= 16 * wm * CT && t < 16 * (wm + 1) * CT;
             const bool any = __builtin_amdgcn_ballot_w64(hit) != 0;
-            const int near = rg.sub;
 #pragma unroll
-            for (int i = 0; i < S::MT; ++i) {
+            for (int p = 0; p < CT; ++p) {
+                uint32_t of;
+                const f32x4 v = logits_of(p, j, of);
                 f32x4 d;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) d[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][k], c2, -rg.lse2)) * f;
+                for (int k = 0; k < 4; ++k) d[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(v[k], c2, -rg.lse2)) * f;
                 if (any) {
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        const bool at = first + 16 * i + k == t;
+                        const bool at = first + 16 * p + k == t;
                         d[k] = at ? e : d[k];
-                        if constexpr (SUBS) which[i][j] = at ? (which[i][j] & ~(0xffu << 8 * k)) | (uint32_t)near << 8 * k : which[i][j];
+                        of = at ? (of & ~(0xffu << 8 * k)) | (uint32_t)rg.sub << 8 * k : of;
                     }
                 }
-                if (there < S::BM) {
+                if (there < BC) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) d[k] = first + 16 * i + k < there ? d[k] : 0.f;
+                    for (int k = 0; k < 4; ++k) d[k] = first + 16 * p + k < there ? d[k] : 0.f;
                 }
-                if constexpr (COS && !SUBS) sums[i] += d * acc[i][j];
-                acc[i][j] = d;
+                if constexpr (LOOP) {
+                    acc[p][j] = d;
+                    which[p][j] = of;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < K; ++i) {
+                        f32x4 own = d;
+                        if constexpr (K > 1)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) own[k] = (of >> 8 * k & 0xffu) == (uint32_t)i ? d[k] : 0.f;
+                        if constexpr (COS) sums[p * K + i] += own * v;
+                        acc[p * K + i][j] = own;
+                    }
+                }
             }
             if constexpr (COS) __builtin_amdgcn_sched_barrier(0);               // a column of tiles at a time: registers
         }
-        const int width = (int)max((int64_t)0, min((int64_t)32 * S::MT, 2 * (a.plane - col)));
-        f32x4 invs[SUBS ? S::MT : 1];
-#pragma unroll 1
-        for (int sub = 0; sub < subs; ++sub) {
-            if constexpr (COS)
+        auto scale_of = [&](int p, int sub) {                                   // a weight row of zeros has no gradient
+            f32x4 inv = inverse_lengths<SUBS>(a.h, c0, first + 16 * p, there, sub);
 #pragma unroll
-                for (int i = 0; i < S::MT; ++i) {
-                    if constexpr (SUBS) sums[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-                    f32x4 inv = inverse_lengths<SUBS>(a.h, c0, first + 16 * i, there, sub);
+            for (int k = 0; k < 4; ++k) inv[k] = inv[k] == kNoNorm ? 0.f : inv[k];
+            return inv;
+        };
+        const int width = (int)max((int64_t)0, min((int64_t)32 * CT, 2 * (a.plane - col)));
+        auto store = [&](int j, int sub, const u32x2 (&o)[CT]) {
+            const int at = (int)((16 * (wn * S::NT + j) + n) * pitch + 2 * (sub * a.plane + col));
+            if constexpr (CT == 1)
+                __builtin_amdgcn_raw_buffer_store_b64(o[0], out, g * 8 < width ? at + g * 8 : kNowhere, 0, 0);
+            else
+                store_tile<16 * CT, 0>(out, at, o, g, width);
+        };
+        auto store_sums = [&](int p, int sub, f32x4 v) {
+            if (!a.col_part) return;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) inv[k] = inv[k] == kNoNorm ? 0.f : inv[k];
-                    if constexpr (SUBS) {
-                        invs[i] = inv;
-                    } else {
+            for (int k = 0; k < 4; ++k) v[k] = sum_of_16(v[k]);
+            if (n == 0 && 32 * p + 8 * g < width)
+                *reinterpret_cast<f32x4 *>(a.col_part + ((int64_t)(nt * S::WN + wn) * subs + sub) * a.plane + col + 16 * p + 4 * g) = v;
+        };
+        if constexpr (!LOOP) {
 #pragma unroll
-                        for (int j = 0; j < S::NT; ++j) acc[i][j] *= inv;
+            for (int i = 0; i < K; ++i) {
+                if constexpr (COS)
+#pragma unroll
+                    for (int p = 0; p < CT; ++p) {
+                        const f32x4 inv = scale_of(p, i);
+#pragma unroll
+                        for (int j = 0; j < S::NT; ++j) acc[p * K + i][j] *= inv;
                     }
+#pragma unroll
+                for (int j = 0; j < S::NT; ++j) {
+                    u32x2 o[CT];
+#pragma unroll
+                    for (int p = 0; p < CT; ++p) o[p] = narrow4<DT>(acc[p * K + i][j]);
+                    store(j, i, o);
                 }
+                if constexpr (COS)
 #pragma unroll
-            for (int j = 0; j < S::NT; ++j) {
-                u32x2 o[S::MT];
-#pragma unroll
-                for (int i = 0; i < S::MT; ++i) {
-                    f32x4 d = acc[i][j];
-                    if constexpr (SUBS) {
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) d[k] = (which[i][j] >> 8 * k & 0xffu) == (uint32_t)sub ? d[k] : 0.f;
-                        sums[i] += d * best[i][j];
-                        d *= invs[i];
-                    }
-                    o[i] = narrow4<DT>(d);
-                }
-                const int at = (int)((16 * (wn * S::NT + j) + n) * pitch + 2 * (sub * a.plane + col));
-                if constexpr (S::MT == 1)
-                    __builtin_amdgcn_raw_buffer_store_b64(o[0], out, g * 8 < width ? at + g * 8 : kNowhere, 0, 0);
-                else
-                    store_tile<16 * S::MT, 0>(out, at, o, g, width);
+                    for (int p = 0; p < CT; ++p) store_sums(p, i, sums[p * K + i]);
             }
-            if constexpr (COS)
-                if (a.col_part) {
+        } else {
+#pragma unroll 1
+            for (int sub = 0; sub < subs; ++sub) {
+                f32x4 inv[CT];
 #pragma unroll
-                    for (int i = 0; i < S::MT; ++i) {
+                for (int p = 0; p < CT; ++p) inv[p] = scale_of(p, sub), sums[p] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) sums[i][k] = sum_of_16(sums[i][k]);
-                        if (n == 0 && 32 * i + 8 * g < width)
-                            *reinterpret_cast<f32x4 *>(a.col_part + ((int64_t)(nt * S::WN + wn) * subs + sub) * a.plane + col + 16 * i + 4 * g) = sums[i];
+                for (int j = 0; j < S::NT; ++j) {
+                    u32x2 o[CT];
+#pragma unroll
+                    for (int p = 0; p < CT; ++p) {
+                        f32x4 d = acc[p][j];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) d[k] = (which[p][j] >> 8 * k & 0xffu) == (uint32_t)sub ? d[k] : 0.f;
+                        sums[p] += d * best[p][j];
+                        o[p] = narrow4<DT>(d * inv[p]);
                     }
+                    store(j, sub, o);
                 }
+#pragma unroll
+                for (int p = 0; p < CT; ++p) store_sums(p, sub, sums[p]);
+            }
         }
     }
 }
@@ -1025,7 +1104,8 @@ struct Tiling {
     Pick pick;
     int bm, bn;
     int wn;                                   // waves along the rows
-    Tiling(Pick p = kFew) : pick(p) { bm = p == kVast ? 256 : p == kWide ? 192 : p == kMany ? 128 : 64, bn = p == kVast ? 256 : p == kFew ? 32 : 128, wn = p == kVast ? 4 : p == kFew ? 1 : 2; }
+    int side;                                 // weight rows of a class side by side in the tile (of whose classes bm is the number)
+    Tiling(Pick p = kFew, int rows = 1) : pick(p), side(rows) { bm = p == kVast ? 256 : p == kWide ? 192 : p == kMany ? 128 : 64, bn = p == kVast ? 256 : p == kFew ? 32 : 128, wn = p == kVast ? 4 : p == kFew ? 1 : 2, bm /= rows; }
     int64_t tiles(int64_t m, int64_t n) const { return (m + bm - 1) / bm * ((n + bn - 1) / bn); }
 };
 struct Plan {
@@ -1073,8 +1153,8 @@ inline double time_of(Pick p, int64_t first, int64_t first_steps, int64_t second
 }
 inline Plan plan_of(const na1d_head &h) {
     Plan p{};
-    // Logits.  Several weight rows to a class keep two sets of sums, and the backward of a margin sums over its tile's classes: there is no
-    // room for them in the larger tiles.
+    // Logits.  The backward of a margin sums over its tile's classes: there is no room for that in the largest tiles.  Two, three or four
+    // weight rows to a class come side by side in the tile whose waves they divide; otherwise they are worked on one after the other.
     const int64_t steps = ceil_div<int64_t>(h.D, kStep);
     auto shortest = [&](Pick largest) {
         Pick best = kBatch;
@@ -1083,10 +1163,11 @@ inline Plan plan_of(const na1d_head &h) {
             const double t = time_of(pick, Tiling(pick).tiles(h.V, h.N), steps);
             if (pick <= largest && t < least) best = pick, least = t;
         }
-        return Tiling(h.N <= 32 ? kFew : best);
+        return Tiling(best);
     };
-    p.logits = shortest(h.subcenters > 1 ? kBatch : kVast);
-    p.back = h.kind == NA1D_HEAD_MARGIN ? shortest(h.subcenters > 1 ? kBatch : kWide) : p.logits;
+    const bool side = h.subcenters >= 2 && h.subcenters <= 4;
+    p.logits = h.N <= 32 ? Tiling(kFew) : side ? Tiling(h.subcenters == 3 ? kWide : kMany, h.subcenters) : shortest(h.subcenters > 1 ? kBatch : kVast);
+    p.back = h.N > 32 && h.kind == NA1D_HEAD_MARGIN && h.subcenters == 1 ? shortest(kWide) : p.logits;
     p.m_tiles = ceil_div<int64_t>(h.V, p.logits.bm);
     const int64_t fits = std::min<int64_t>(kMostDz / (2 * h.N * h.subcenters), (1 << 20) / h.subcenters);
     p.plane = std::max<int64_t>(fits / 256 * 256, 256);
@@ -1152,23 +1233,30 @@ template <auto KERNEL, class... A> int launch(unsigned grid, unsigned block, siz
     KERNEL<<<grid, block, lds, s>>>(a...);
     return launch_status();
 }
-template <class DT, class S, bool BACK> int launch_logits_of(const na1d_head &h, const Logits &a, hipStream_t s) {
+template <class DT, class S, bool BACK> int launch_logits_of(const na1d_head &h, const Tiling &t, const Logits &a, hipStream_t s) {
     const unsigned grid = (unsigned)(a.m_tiles * a.n_tiles);
-    if (h.kind != NA1D_HEAD_MARGIN) return launch<logits_kernel<DT, S, false, false, BACK>>(grid, S::kThreadsOf, S::kLds, s, a);
+    if (h.kind != NA1D_HEAD_MARGIN) return launch<logits_kernel<DT, S, false, 0, BACK>>(grid, S::kThreadsOf, S::kLds, s, a);
     if constexpr (!BACK || S::MT * S::NT <= 24)
-        if (h.subcenters == 1) return launch<logits_kernel<DT, S, true, false, BACK>>(grid, S::kThreadsOf, S::kLds, s, a);
-    if constexpr (S::MT * S::NT <= 8) return launch<logits_kernel<DT, S, true, true, BACK>>(grid, S::kThreadsOf, S::kLds, s, a);
+        if (h.subcenters == 1) return launch<logits_kernel<DT, S, true, 0, BACK>>(grid, S::kThreadsOf, S::kLds, s, a);
+    if constexpr (S::MT == 4) {
+        if (t.side == 2) return launch<logits_kernel<DT, S, true, 2, BACK>>(grid, S::kThreadsOf, S::kLds, s, a);
+        if (t.side == 4) return launch<logits_kernel<DT, S, true, 4, BACK>>(grid, S::kThreadsOf, S::kLds, s, a);
+    }
+    if constexpr (S::MT == 6)
+        if (t.side == 3) return launch<logits_kernel<DT, S, true, 3, BACK>>(grid, S::kThreadsOf, S::kLds, s, a);
+    if constexpr (S::MT <= 2)
+        if (t.side == 1) return launch<logits_kernel<DT, S, true, 1, BACK>>(grid, S::kThreadsOf, S::kLds, s, a);
     return NA1D_ERR_UNSUPPORTED;
 }
 template <class DT, bool BACK> int launch_logits(const na1d_head &h, const Tiling &t, Logits a, hipStream_t s) {
-    a.m_tiles = (int)ceil_div(a.classes, t.bm);
+    a.m_tiles = (int)ceil_div<int64_t>(BACK ? round_up(a.classes, kStep) : a.classes, t.bm);           // dz: to the end of its last step
     a.n_tiles = (int)ceil_div<int64_t>(h.N, t.bn);
     switch (t.pick) {
-        case kFew: return launch_logits_of<DT, Few, BACK>(h, a, s);
-        case kBatch: return launch_logits_of<DT, Batch, BACK>(h, a, s);
-        case kMany: return launch_logits_of<DT, Many, BACK>(h, a, s);
-        case kWide: return launch_logits_of<DT, Wide, BACK>(h, a, s);
-        default: return launch_logits_of<DT, Vast, BACK>(h, a, s);
+        case kFew: return launch_logits_of<DT, Few, BACK>(h, t, a, s);
+        case kBatch: return launch_logits_of<DT, Batch, BACK>(h, t, a, s);
+        case kMany: return launch_logits_of<DT, Many, BACK>(h, t, a, s);
+        case kWide: return launch_logits_of<DT, Wide, BACK>(h, t, a, s);
+        default: return launch_logits_of<DT, Vast, BACK>(h, t, a, s);
     }
 }
 template <class DT, class SX, class SW> int launch_products_of(const Product &dx, const Product &dw, hipStream_t s) {
