@@ -690,10 +690,11 @@ __global__ void __launch_bounds__(kFinishThreads)
 finish_kernel(Finish a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     f32x2 *met = reinterpret_cast<f32x2 *>(smem);                               // [lanes][rows]: 256 of them
-    float *lse = reinterpret_cast<float *>(met + kFinishThreads);               // [rows]
-    float *z = lse + a.rows;                                                    // teacher, [rows][entries]: products,
-    int *ids = reinterpret_cast<int *>(z + a.rows * a.top);                     // classes,
-    float *share = reinterpret_cast<float *>(ids + a.rows * a.top);             // and their q
+    float *lse = reinterpret_cast<float *>(met + kFinishThreads);               // [16]
+    const int entries = (a.top + 3) & ~3;                                       // of a row here; the last ones may be of no class
+    float *z = lse + 16;                                                        // teacher, [rows][entries]: products,
+    int *ids = reinterpret_cast<int *>(z + a.rows * entries);                   // classes,
+    float *share = reinterpret_cast<float *>(ids + a.rows * entries);           // and their q
     const int R = a.rows, lanes = kFinishThreads / R, r = threadIdx.x & (R - 1), l = threadIdx.x / R;
     const int64_t r0 = (int64_t)blockIdx.x * R;
     {
@@ -709,12 +710,12 @@ finish_kernel(Finish a) {
     }
     // a teacher's entries: 16 lanes to an entry
     const int lane16 = threadIdx.x & 15;
-    for (int e = threadIdx.x >> 4; e < R * a.top; e += kFinishThreads / 16) {
-        const int64_t row = r0 + e / a.top;
-        const int k = e % a.top;
+    for (int e = threadIdx.x >> 4; e < R * entries; e += kFinishThreads / 16) {
+        const int64_t row = r0 + e / entries;
+        const int k = e % entries;
         float s = 0.f;
         int id = -1;
-        if (row < a.h.N) {
+        if (row < a.h.N && k < a.top) {
             id = load_id(a.ids, row * a.top + k, a.ids_wide);
             if (id >= 0 && id < a.h.V) {
                 const char *xr = a.h.x + row * a.h.x_pitch, *w = a.h.w + id * a.h.w_pitch;
@@ -785,8 +786,9 @@ finish_kernel(Finish a) {
         for (int q0 = wave; q0 < R; q0 += kFinishThreads / 64) {
             const int64_t row = r0 + q0;
             if (row >= a.h.N) break;
-            const int *id = ids + q0 * a.top;
-            float *q = share + q0 * a.top;
+            const int *id = ids + q0 * entries;
+            float *q = share + q0 * entries;
+            const float *zr = z + q0 * entries;
             float top = kNegInf, total = 0.f;
             bool bad = false, nan = false;
             for (int k = lane; k < a.top; k += 64) {
@@ -806,14 +808,23 @@ finish_kernel(Finish a) {
             const float log_total = __builtin_log2f(total), inv = 1.f / total, lse2 = lse[q0];
             float sum = 0.f;
             for (int k = lane; k < a.top; k += 64) {
-                const float logq = (q[k] - off) * kLog2e - log_total, share = __builtin_amdgcn_exp2f((q[k] - off) * kLog2e) * inv, z2 = z[q0 * a.top + k] * a.h.scale2;
+                const float logq = (q[k] - off) * kLog2e - log_total, share = __builtin_amdgcn_exp2f((q[k] - off) * kLog2e) * inv, z2 = zr[k] * a.h.scale2;
                 if (share != 0.f) sum += share * (logq - (z2 - lse2));
                 q[k] = share;
             }
+            if (lane < entries - a.top) q[a.top + lane] = 0.f;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");              // every lane reads the others' shares
             for (int k = lane; k < a.top; k += 64) {
                 float same = 0.f;                                               // an entry that is there twice has both shares
-                for (int m = 0; m < a.top; ++m) same += id[m] == id[k] ? q[m] : 0.f;
-                a.coeff[row * a.top + k] = counts && id[k] >= 0 ? __builtin_amdgcn_exp2f(z[q0 * a.top + k] * a.h.scale2 - lse2) - same : 0.f;
+                const int own = id[k];
+#pragma unroll 4
+                for (int m = 0; m < entries; m += 4) {
+                    const u32x4 them = *reinterpret_cast<const u32x4 *>(id + m);
+                    const f32x4 theirs = *reinterpret_cast<const f32x4 *>(q + m);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) same += (int)them[i] == own ? theirs[i] : 0.f;
+                }
+                a.coeff[row * a.top + k] = counts && own >= 0 ? __builtin_amdgcn_exp2f(zr[k] * a.h.scale2 - lse2) - same : 0.f;
             }
             sum = over_wave(sum, false);
             RowStat st = {__builtin_inff(), 0.f, kFar, -1};
@@ -846,7 +857,7 @@ reduce_kernel(Reduce a) {
     double s = 0.0;
     int c = 0;
     float top = 0.f, most = a.most_w ? 0.f : 1.f;
-#pragma unroll 4
+#pragma unroll 8
     for (int r = threadIdx.x; r < a.N; r += 1024) {
         const RowStat st = a.stats[r];
         if (a.loss) s += (double)a.loss[r];
@@ -1295,7 +1306,9 @@ int forward(const na1d_head &h, float *loss, uint8_t *hits, const void *x, const
     NA1D_TRY((launch_logits<DT, false>(h, p.logits, a, s)));
     Finish e{};
     e.h = a.h, e.part = a.part, e.at = a.at, e.m_tiles = (int)p.m_tiles;
-    e.rows = teaches ? (h.N >= 8192 ? 4 : 1) : h.N >= 4096 ? 16 : h.N >= 1024 ? 4 : 1;          // a teacher of 100 entries in 1000 rows: 4 rows 68 us, 1 row 46
+    // Rows to a workgroup: more read the tiles' results in longer pieces, fewer leave more of them at work.  A teacher's, whole forwards in
+    // us with 1, 2 and 4: 1000 rows of 16 entries 23, 25, 30; 2000 of 100 38, 35, 44; 10182 of 84 72, 66, 60; 7433 of 4 69, 53, 46.
+    e.rows = teaches ? (h.N >= 4096 ? 4 : h.N >= 1536 ? 2 : 1) : h.N >= 4096 ? 16 : h.N >= 1024 ? 4 : 1;
     e.ids = ids, e.ids_wide = h.ids_64, e.top = teaches ? h.top : 0, e.teacher = teacher, e.teacher_type = h.teacher_type;
     e.ignore = h.ignore_index, e.cosines = cosines, e.temperature = h.scale;
     e.cos_m = (float)cos(h.margin), e.sin_m = (float)sin(h.margin), e.threshold = (float)cos(M_PI - h.margin), e.drop = (float)(sin(M_PI - h.margin) * h.margin);
@@ -1303,7 +1316,7 @@ int forward(const na1d_head &h, float *loss, uint8_t *hits, const void *x, const
     float *rows = reinterpret_cast<float *>(ws + f.rows);
     e.loss = h.reduction == NA1D_HEAD_NONE ? loss : rows;
     e.hits = hits;
-    const size_t lds = kFinishThreads * sizeof(f32x2) + 4 * (size_t)e.rows * (3 * e.top + 1);
+    const size_t lds = kFinishThreads * sizeof(f32x2) + 64 + 12 * (size_t)e.rows * round_up(e.top, 4);
     NA1D_TRY(launch<finish_kernel<DT>>((unsigned)ceil_div<int64_t>(h.N, e.rows), kFinishThreads, lds, s, e));
     if (h.reduction == NA1D_HEAD_NONE) return NA1D_OK;
     float *count = reinterpret_cast<float *>(saved + o.count);
