@@ -21,6 +21,9 @@ LARGE = [  # launches that fill the card: tiles of 128 x 128 and of 256 x 256, p
 ]
 
 
+FEW_ROWS = [(1, 128, 50001), (20, 128, 50000), (32, 264, 30001), (31, 1032, 9000)]       # and a weight whose gradient fills the card
+
+
 def _inputs(N, D, V, dtype, seed, strength=3.0):
     g = torch.Generator().manual_seed(seed)
     w = (torch.randn(V, D, generator=g) * D ** -0.5).to(dtype)
@@ -59,7 +62,7 @@ def _train(call, x, w, up):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=NAMES)
-@pytest.mark.parametrize("size", SIZES + LARGE, ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("size", SIZES + LARGE + FEW_ROWS, ids=lambda s: "x".join(map(str, s)))
 def test_cross_entropy(size, dtype):
     N, D, V = size
     print("cross entropy", size, dtype, flush=True)

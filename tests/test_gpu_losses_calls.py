@@ -334,6 +334,32 @@ def test_compiled_ops_equal_the_functions():
         assert torch.equal(loss, 2 * want[0]) and _same(grads, want[1:]), kind
 
 
+def test_a_compiled_op_takes_batches_of_any_size():
+    from na1d_amd import ops
+    compiled = torch.compile(lambda x, w, t: ops.linear_cross_entropy_op(x, w, t), backend="aot_eager", fullgraph=True, dynamic=True)
+    for N in (33, 40, 7):
+        x, w, target, _, _ = _inputs(N=N)
+        got = _both(lambda a, b: compiled(a, b, target), x, w)
+        assert _same(got, _both(lambda a, b: losses.linear_cross_entropy(a, b, target), x, w)), N
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("kind", KINDS)
+def test_upstream_gradients_that_are_not_finite_or_zero(kind, dtype):
+    """A loss scale that has run over reaches the gradients, a zero leaves none; a row's own stays in its row of dx."""
+    x, w, target, ids, logits = _inputs(dtype=dtype)
+    for bad in (float("inf"), float("nan")):
+        for reduction in ("mean", "none"):
+            call = _calls(target, ids, logits, reduction)[kind]
+            up = torch.tensor(bad, device="cuda") if reduction == "mean" else torch.ones(33, device="cuda").index_fill(0, torch.tensor([4], device="cuda"), bad)
+            _, dx, dw = _both(call, x, w, up)
+            assert not torch.isfinite(dx[4]).all() and not torch.isfinite(dw).all()
+            if reduction == "none":
+                assert torch.isfinite(dx[:4]).all() and torch.isfinite(dx[5:]).all()
+    _, dx, dw = _both(_calls(target, ids, logits)[kind], x, w, torch.tensor(0.0, device="cuda"))
+    assert not dx.any() and not dw.any()
+
+
 @pytest.mark.parametrize("dtype", [BF16, FP16], ids=["bf16", "fp16"])
 def test_the_models_head(dtype):
     """The fused head beside the torch one: the same parameters, losses and gradients to what products in 16 bits give."""
