@@ -411,6 +411,16 @@ logits_kernel(Logits a) {
     f32x4 best[LOOP ? S::MT : 1][LOOP ? S::NT : 1];
     uint32_t which[LOOP ? S::MT : 1][LOOP ? S::NT : 1];
     const int first = 16 * wm * CT + 4 * g;                                    // this lane's class of the tile in its first 16-class tile
+    // What the ends read of the rows is asked for in front of the products.  Of a 64-bit target the lower half will do: a row whose
+    // upper half is not its sign has no target, and what it leaves is not read.
+    int target[S::NT];
+    float row_inv[S::NT];
+#pragma unroll
+    for (int j = 0; j < S::NT; ++j) {
+        const int64_t r = min(r0 + 16 * (wn * S::NT + j) + n, a.h.N - 1);
+        if constexpr (!BACK) target[j] = a.ids ? reinterpret_cast<const int32_t *>(a.ids)[a.ids_wide ? 2 * r : r] : -1;
+        row_inv[j] = COS ? a.h.inv_x[r] : 1.f;
+    }
 #pragma unroll 1
     for (int sub = 0; sub < (LOOP ? subs : 1); ++sub) {
         const char *rows = a.h.w + (int64_t)c0 * subs * a.h.w_pitch + sub * a.h.w_pitch;
@@ -471,7 +481,7 @@ logits_kernel(Logits a) {
         for (int j = 0; j < S::NT; ++j) {
             const int row = 16 * (wn * S::NT + j) + n;
             const int64_t r = min(r0 + row, a.h.N - 1);
-            const float c2 = a.h.scale2 * (COS ? a.h.inv_x[r] : 1.f);
+            const float c2 = a.h.scale2 * row_inv[j];
             f32x4 v[CT];
             uint32_t of[CT];
 #pragma unroll
@@ -482,19 +492,22 @@ logits_kernel(Logits a) {
 #pragma unroll
                     for (int k = 0; k < 4; ++k) v[p][k] = first + 16 * p + k < there ? v[p][k] : kNegInf;
             }
-            if (a.ids) {
-                const int64_t t = (int64_t)load_id(a.ids, r, a.ids_wide) - c0;
-                const bool hit = t >= 16 * wm * CT && t < 16 * (wm + 1) * CT;
-                if (__builtin_amdgcn_ballot_w64(hit)) {
+            const uint32_t t = (uint32_t)(target[j] - c0 - 16 * wm * CT);       // as a class of this wave's
+            if (a.ids && __builtin_amdgcn_ballot_w64(t < 16 * CT)) {
+                float mine = 0.f;
+                uint32_t of_mine = 0;
+                bool found = false;
 #pragma unroll
-                    for (int p = 0; p < CT; ++p)
+                for (int p = 0; p < CT; ++p)
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const bool here = first + 16 * p + k == t;
-                            if (here && r0 + row < a.h.N) a.at[r] = f32x2{v[p][k], (float)(of[p] >> 8 * k & 0xffu)};
-                            v[p][k] = here ? kNegInf : v[p][k];
-                        }
-                }
+                    for (int k = 0; k < 4; ++k) {
+                        const bool here = (uint32_t)(4 * g + 16 * p + k) == t;
+                        mine = here ? v[p][k] : mine;
+                        if constexpr (SUBS != 0) of_mine = here ? of[p] >> 8 * k & 0xffu : of_mine;
+                        found |= here;
+                        v[p][k] = here ? kNegInf : v[p][k];
+                    }
+                if (found && r0 + row < a.h.N) a.at[r] = f32x2{mine, (float)of_mine};
             }
             float top = kNegInf;
 #pragma unroll
@@ -534,13 +547,8 @@ logits_kernel(Logits a) {
             for (int i = 0; i < S::MT; ++i) sums[i] = f32x4{0.f, 0.f, 0.f, 0.f};
         const float base = a.up.base(), common = base * a.up.up(base);
         RowStat row_stats[S::NT];                                               // all on their way at once
-        float row_inv[S::NT];
 #pragma unroll
-        for (int j = 0; j < S::NT; ++j) {
-            const int64_t r = min(r0 + 16 * (wn * S::NT + j) + n, a.h.N - 1);
-            row_stats[j] = a.stats[r];
-            row_inv[j] = COS ? a.h.inv_x[r] : 1.f;
-        }
+        for (int j = 0; j < S::NT; ++j) row_stats[j] = a.stats[min(r0 + 16 * (wn * S::NT + j) + n, a.h.N - 1)];
 #pragma unroll
         for (int j = 0; j < S::NT; ++j) {
             const int row = 16 * (wn * S::NT + j) + n;
