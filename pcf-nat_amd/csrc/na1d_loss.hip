@@ -272,9 +272,13 @@ struct Upstream {
     const float *most;              // the largest a row's factor may come to for an upstream gradient of 1 (with `count`) or as it is
     float factor;
     int mean;
-    __device__ inline float base() const { return count ? factor * (mean ? dloss[0] / count[0] : dloss[0]) : factor; }
-    __device__ inline float up(float base) const {
-        const float top = __builtin_fabsf(base) * *most;
+    struct Read { float dloss, count, most; };                      // asked for, to be waited for later
+    __device__ inline Read read() const { return {count ? dloss[0] : 1.f, count ? count[0] : 1.f, *most}; }
+    __device__ inline float base(const Read &v) const { return count ? factor * (mean ? v.dloss / v.count : v.dloss) : factor; }
+    __device__ inline float base() const { return base(read()); }
+    __device__ inline float up(float base) const { return up(base, read()); }
+    __device__ inline float up(float base, const Read &v) const {
+        const float top = __builtin_fabsf(base) * v.most;
         return top > 0.f && top < 3.0e38f ? __builtin_fminf(kTopDz / top, 0x1p100f) : 1.f;
     }
     __device__ inline float down() const { return 1.f / up(base()); }
@@ -414,11 +418,15 @@ logits_kernel(Logits a) {
     // What the ends read of the rows is asked for in front of the products.  Of a 64-bit target the lower half will do: a row whose
     // upper half is not its sign has no target, and what it leaves is not read.
     int target[S::NT];
-    float row_inv[S::NT];
+    float row_inv[S::NT], row_up[S::NT];
+    RowStat row_stats[S::NT];
+    Upstream::Read up_read{};
+    if constexpr (BACK) up_read = a.up.read();
 #pragma unroll
     for (int j = 0; j < S::NT; ++j) {
         const int64_t r = min(r0 + 16 * (wn * S::NT + j) + n, a.h.N - 1);
         if constexpr (!BACK) target[j] = a.ids ? reinterpret_cast<const int32_t *>(a.ids)[a.ids_wide ? 2 * r : r] : -1;
+        if constexpr (BACK) row_stats[j] = a.stats[r], row_up[j] = a.up.count ? 1.f : a.up.dloss[r];
         row_inv[j] = COS ? a.h.inv_x[r] : 1.f;
     }
 #pragma unroll 1
@@ -545,17 +553,13 @@ logits_kernel(Logits a) {
         if constexpr (COS)
 #pragma unroll
             for (int i = 0; i < S::MT; ++i) sums[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-        const float base = a.up.base(), common = base * a.up.up(base);
-        RowStat row_stats[S::NT];                                               // all on their way at once
-#pragma unroll
-        for (int j = 0; j < S::NT; ++j) row_stats[j] = a.stats[min(r0 + 16 * (wn * S::NT + j) + n, a.h.N - 1)];
+        const float base = a.up.base(up_read), common = base * a.up.up(base, up_read);
 #pragma unroll
         for (int j = 0; j < S::NT; ++j) {
             const int row = 16 * (wn * S::NT + j) + n;
-            const int64_t r = min(r0 + row, a.h.N - 1);
             const RowStat rg = row_stats[j];
             const float ix = row_inv[j], c2 = a.h.scale2 * ix;
-            float f = common * (a.up.count ? 1.f : a.up.dloss[r]) * ix;
+            float f = common * row_up[j] * ix;
             if (r0 + row >= a.h.N || rg.sub < 0 || (COS && ix == kNoNorm)) f = 0.f;           // rows behind the last have no share in the sums
             const float e = f * rg.at_target;
             const int64_t t = (int64_t)rg.target - c0;
