@@ -302,6 +302,7 @@ constexpr float kLeastNorm = 1e-12f, kNoNorm = 1e-30f;
 
 constexpr int kNormBlocks = 1024;
 // 1 / |row| of 16-bit rows, sixteen lanes to a row; the first `rows_a` are a's.  And the largest of each workgroup's rows of b.
+// Bound by memory: 101024 rows of 512 channels 18 us, 5.8 TB/s.
 template <class DT>
 __global__ void __launch_bounds__(256)
 norms_kernel(float *__restrict__ inv_a, float *__restrict__ inv_b, float *__restrict__ most_b, const char *__restrict__ a, const char *__restrict__ b, int64_t a_pitch,
@@ -672,6 +673,8 @@ logits_kernel(Logits a) {
 // =============================================================================
 // A row's tiles put together, the target's logit, the loss
 // =============================================================================
+// Waits more than it works: 8192 rows of 256 tiles 6 us.  A teacher's entries are products of their own, read row by row: 4096 x 64 of 768
+// channels 70 us, 5.7 TB/s out of the last level of cache (the weight is 74 MB).
 struct Finish {
     Head h;
     const f32x2 *part, *at;
@@ -910,7 +913,9 @@ entries_kernel(uint16_t *__restrict__ dz, const float *__restrict__ coeff, Upstr
 }
 
 // dx (fp32, all ranges' and splits' shares): x rows (N side) by channels (M side), contracted over a range's classes; and dW:
-// weight rows by channels, contracted over the rows.
+// weight rows by channels, contracted over the rows.  Both in one launch, so that the one's last workgroups run beside the other's first.
+// Bound by the matrix cores where there are many rows: 8192 rows, 16384 classes, 1024 channels 450 us, 1220 TFLOP/s (the library's two products 895 and
+// 1087); by dz (read twice) and dW where there are few: 1024 rows, 100000 classes, 512 channels 288 us, 730 TFLOP/s.
 struct Product {
     const char *dz, *other;         // other: W, or x
     int64_t plane, other_pitch;     // of dz; bytes from one row of `other` to the next
@@ -1040,7 +1045,7 @@ products_kernel(Product dx, Product dw, uint32_t dx_items, uint32_t dw_items) {
 }
 
 // The shares of all splits of a row put together, less their part along the row's own vector (cosines).  WAVES waves to a row share
-// its splits.
+// its splits.  Bound by memory: 8192 rows of 1024 channels, two splits 15 us, 5.5 TB/s.
 struct Fold {
     char *out;
     const float *part;
@@ -1141,13 +1146,13 @@ struct Plan {
     int dx_splits, dx_per, dw_splits, dw_per;
 };
 constexpr int64_t kMostDz = 256ll << 20;      // bytes of dz: what the last level of cache holds (64 MB: +10 to 25 %, 1 GB: 0 to +2 %)
-constexpr int kFullLaunch = 512;              // workgroups: two to a CU
 
 // How long a launch of `first` workgroups of `first_steps` and then `second` of `second_steps` takes, in us: CUs hold one workgroup
 // of 256 x 256 or two smaller ones, and take the next as they get free.  What a step of 64 and the rest of a tile take is
-// fitted to forwards of 4096 x 32768 logits with 64, 256 and 1024 channels (64 x 128: 99, 152, 361 us; 128 x 128: 62, 101, 263; 192 x 128: 52, 92,
-// 250; 256 x 256: 61, 93, 235), that is 990, 1280, 1340 and 1460 TFLOP/s between the ends.  The model also orders what does
-// not fill a round: 1024 x 8000, 512 channels 25, 21, 25 and 27 us; 128 x 20000, 1024 channels 22, 25, 26, 36; 2000 x 1000 17, 20, 22, 29.
+// fitted to forwards of 4096 x 32768 logits with 64, 256 and 1024 channels (64 x 128: 94, 143, 358 us; 128 x 128: 64, 101, 263; 192 x 128: 56, 95,
+// 255; 256 x 256: 64, 99, 240), that is 990, 1280, 1340 and 1460 TFLOP/s between the ends.  The model also orders what does
+// not fill a round: 1024 x 8000, 512 channels 24, 20, 23 and 25 us; 128 x 20000, 1024 channels 21, 24, 25, 33; 300 x 5000, 256 channels 15, 15, 17, 20.
+// (It is not right everywhere: 2000 x 2000, 1000 channels take 26 us in the tiles that it picks, 64 x 128, and 24 in 128 x 128.)
 struct Cost {
     double step, rest;
     int64_t slots;
