@@ -134,19 +134,18 @@ template <int MT_, int NT_, int WM_, int WN_, int STAGES_> struct Shape {
     static constexpr int kWavesOf = WM * WN, kThreadsOf = 64 * kWavesOf, BM = 16 * MT * WM, BN = 16 * NT * WN;
     static constexpr int kSlot = (BM + BN) * kPieceRow, kLds = STAGES * kSlot;
 };
-__device__ inline float sum_of_16(float x) {                                   // over the lanes of one g
-    x += __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), 0xb1, 0xf, 0xf, true));
-    x += __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), 0x4e, 0xf, 0xf, true));
-    x += __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), 0x141, 0xf, 0xf, true));
-    return x + __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), 0x140, 0xf, 0xf, true));
+template <bool MAX> __device__ inline float joined(float x, float y) { return MAX ? __builtin_fmaxf(x, y) : x + y; }
+template <bool MAX = false> __device__ inline float sum_of_16(float x) {        // (or the largest) over the lanes of one g
+    x = joined<MAX>(x, __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), 0xb1, 0xf, 0xf, true)));
+    x = joined<MAX>(x, __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), 0x4e, 0xf, 0xf, true)));
+    x = joined<MAX>(x, __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), 0x141, 0xf, 0xf, true)));
+    return joined<MAX>(x, __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), 0x140, 0xf, 0xf, true)));
 }
-__device__ inline float over_wave(float x, bool max) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) {
-        const float y = __shfl_xor(x, o);
-        x = max ? __builtin_fmaxf(x, y) : x + y;
-    }
-    return x;
+template <bool MAX> __device__ inline float over_wave(float x) {
+    float a, b;
+    swap_rows16(sum_of_16<MAX>(x), a, b);
+    swap_rows32(joined<MAX>(a, b), a, b);
+    return joined<MAX>(a, b);
 }
 __device__ inline void turn_over() { asm volatile("s_barrier" ::: "memory"); }
 template <int COUNT> __device__ inline void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(COUNT) : "memory"); }
@@ -258,18 +257,20 @@ constexpr int kFar = 0x7f000000;             // no class
 // What a row has to do with its target, left by the forward for the backward.
 struct alignas(16) RowStat {
     float lse2;        // log2 of the sum of exp(z) over all classes, the target's with its margin; +inf: the row does not count
-    float at_target;   // P_t - 1, times the margin's slope
+    float at_target;   // P_t - 1, times the margin's slope; of a teacher's row the largest |P - q| of its entries
     int target;        // class, or kFar
     int sub;           // of its weight rows the nearest
 };
 // What a row multiplies its probabilities by: dz = f exp2(z2 - lse2).  Gradients of single logits are rounded to 16 bits, where fp16
 // ends at 6e-8 and either type is at its most exact just below a power of two; so all are multiplied by one number, which the
-// products' ends take away again, that brings the largest there may be to kTopDz.  Most rows' largest (the target's, -(1 - P_t) of a
-// whole) comes close to it: of the target's share in the gradients a third less is lost than on average.
-constexpr float kTopDz = 16320.f;            // 255 * 2^6
+// products' ends take away again.  It brings the largest that there may be to between kTopDz / 2 and kTopDz, and of the steps of a
+// factor of two it takes the eighth by which the rows' largest ones (the target's, -(1 - P_t) of a whole) lose least in
+// rounding: most of a gradient's length is theirs.  (Over 40 heads of random sizes a gradient was up to 1.52 times as far from 64 bits as
+// one that is rounded but once; 1.79 times with the largest brought to kTopDz itself.)
+constexpr float kTopDz = 32640.f;            // 255 * 2^7
 struct Upstream {
     const float *dloss, *count;     // count NULL: dloss has a value for every row
-    const float *most;              // the largest a row's factor may come to for an upstream gradient of 1 (with `count`) or as it is
+    const float *most;              // what to bring to kTopDz, for an upstream gradient of 1 (with `count`) or as it is
     float factor;
     int mean;
     struct Read { float dloss, count, most; };                      // asked for, to be waited for later
@@ -339,7 +340,7 @@ norms_kernel(float *__restrict__ inv_a, float *__restrict__ inv_b, float *__rest
             if (r >= rows_a) top = __builtin_fmaxf(top, inv);
         }
     }
-    top = over_wave(top, true);
+    top = over_wave<true>(top);
     if ((threadIdx.x & 63) == 0) most[wave] = top;
     __syncthreads();
     if (threadIdx.x == 0) most_b[blockIdx.x] = __builtin_fmaxf(__builtin_fmaxf(most[0], most[1]), __builtin_fmaxf(most[2], most[3]));
@@ -813,10 +814,10 @@ finish_kernel(Finish a) {
                 top = __builtin_fmaxf(top, t);
                 q[k] = t;
             }
-            top = over_wave(top, true);
+            top = over_wave<true>(top);
             const float off = top == kNegInf ? 0.f : top;
             for (int k = lane; k < a.top; k += 64) total += __builtin_amdgcn_exp2f((q[k] - off) * kLog2e);
-            total = over_wave(total, false);
+            total = over_wave<false>(total);
             bad = __builtin_amdgcn_ballot_w64(bad) != 0;
             nan = __builtin_amdgcn_ballot_w64(nan) != 0;
             const bool counts = !bad && (top > kNegInf || nan);
@@ -829,6 +830,7 @@ finish_kernel(Finish a) {
             }
             if (lane < entries - a.top) q[a.top + lane] = 0.f;
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");              // every lane reads the others' shares
+            float typical = 0.f;
             for (int k = lane; k < a.top; k += 64) {
                 float same = 0.f;                                               // an entry that is there twice has both shares
                 const int own = id[k];
@@ -839,14 +841,18 @@ finish_kernel(Finish a) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) same += (int)them[i] == own ? theirs[i] : 0.f;
                 }
-                a.coeff[row * a.top + k] = counts && own >= 0 ? __builtin_amdgcn_exp2f(zr[k] * a.h.scale2 - lse2) - same : 0.f;
+                const float d = counts && own >= 0 ? __builtin_amdgcn_exp2f(zr[k] * a.h.scale2 - lse2) - same : 0.f;
+                a.coeff[row * a.top + k] = d;
+                typical = __builtin_fmaxf(typical, __builtin_fabsf(d));
             }
-            sum = over_wave(sum, false);
+            sum = over_wave<false>(sum);
+            typical = over_wave<true>(typical);
             RowStat st = {__builtin_inff(), 0.f, kFar, -1};
             float loss = bad ? __builtin_nanf("") : 0.f;
             if (counts) {
                 loss = sum * kLn2 * a.temperature * a.temperature;
                 st.lse2 = lse2;
+                st.at_target = typical;
                 st.sub = 0;
             }
             if (lane == 0) a.stats[row] = st, a.loss[row] = loss;
@@ -855,28 +861,39 @@ finish_kernel(Finish a) {
     }
 }
 
-// The sum or mean of the rows' losses in a fixed order, how many rows count, and the largest their factors may come to (Upstream).
+// The sum or mean of the rows' losses in a fixed order, how many rows count, and what dz are to be scaled by (Upstream).  A number f
+// rounded to b bits is off by 2^-b of the power of two below it: for each of kSteps scales within a factor of two, the sum of those
+// powers squared over the typical f of up to 1024 rows (of all rows: 3 us more at 16000).
 // (As the work of the finish kernel's last workgroup it is no launch of its own, but the fences of all the others cost more than
 // that: 128 rows 15.8 us against 5.2 + 1.9, 999 rows 50 against 9.)
+constexpr int kSteps = 8;
 struct Reduce {
     float *total, *count, *most;
-    const float *loss, *dloss, *inv_x, *most_w;       // dloss: of every row, in a backward (NULL otherwise); most_w [kNormBlocks]; either may be NULL
+    const float *loss, *dloss, *inv_x, *inv_w, *most_w;       // dloss: of every row, in a backward (NULL otherwise); most_w [kNormBlocks]; all may be NULL
     const RowStat *stats;
-    int N, mean;
+    int N, subs, mean;
 };
 __global__ void __launch_bounds__(1024)
 reduce_kernel(Reduce a) {
     __shared__ double sums[16];
     __shared__ int counts[16];
-    __shared__ float tops[16], mosts[16];
+    __shared__ float tops[16], mosts[16], losts[16][kSteps];
     double s = 0.0;
     int c = 0;
-    float top = 0.f, most = a.most_w ? 0.f : 1.f;
+    float top = 0.f, most = a.most_w ? 0.f : 1.f, some = 0.f;
+    if (a.N > 1024 || (int)threadIdx.x < a.N) {
+        const int64_t r = a.N > 1024 ? (int64_t)threadIdx.x * a.N >> 10 : threadIdx.x;
+        const RowStat st = a.stats[r];
+        some = __builtin_fabsf(st.at_target) * (a.dloss ? __builtin_fabsf(a.dloss[r]) : 1.f);
+        if (a.inv_x && st.sub >= 0) some *= a.inv_x[r] * a.inv_w[(int64_t)st.target * a.subs + st.sub];
+        some = __builtin_fminf(some, 0x1p60f);
+    }
 #pragma unroll 8
     for (int r = threadIdx.x; r < a.N; r += 1024) {
         const RowStat st = a.stats[r];
         if (a.loss) s += (double)a.loss[r];
-        const float f = __builtin_fmaxf(1.f, __builtin_fabsf(st.at_target)) * (a.inv_x ? a.inv_x[r] : 1.f) * (a.dloss ? __builtin_fabsf(a.dloss[r]) : 1.f);
+        const float up = a.dloss ? __builtin_fabsf(a.dloss[r]) : 1.f;
+        const float f = __builtin_fmaxf(1.f, __builtin_fabsf(st.at_target)) * (a.inv_x ? a.inv_x[r] : 1.f) * up;
         c += st.sub >= 0;
         top = __builtin_fmaxf(top, st.sub >= 0 ? f : 0.f);
     }
@@ -884,13 +901,33 @@ reduce_kernel(Reduce a) {
     static_assert(kNormBlocks == 1024, "one to a thread");
 #pragma unroll
     for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o), c += __shfl_xor(c, o);
-    top = over_wave(top, true), most = over_wave(most, true);
-    const int wave = threadIdx.x >> 6;
-    if ((threadIdx.x & 63) == 0) sums[wave] = s, counts[wave] = c, tops[wave] = top, mosts[wave] = most;
+    top = over_wave<true>(top), most = over_wave<true>(most);
+    const float below = __uint_as_float(__float_as_uint(some) & 0x7f800000u);
+    float lost[kSteps];
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) lost[i] = over_wave<false>((some * __builtin_exp2f((float)i / kSteps) >= 2.f * below ? 4.f : 1.f) * (below * below));
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    if (lane == 0) {
+        sums[wave] = s, counts[wave] = c, tops[wave] = top, mosts[wave] = most;
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) losts[wave][i] = lost[i];
+    }
     __syncthreads();
-    if (threadIdx.x) return;
+    if (wave) return;
+    float mine = 0.f;                                                           // lanes 0 to 7: a scale each
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mine += losts[i][lane % kSteps];
+    mine *= __builtin_amdgcn_exp2f(-2.f / kSteps * (float)(lane % kSteps));
+    float least = mine;
+#pragma unroll
+    for (int o = 1; o < kSteps; o <<= 1) least = __builtin_fminf(least, __shfl_xor(least, o));
+    const uint64_t at = __builtin_amdgcn_ballot_w64(mine == least);             // none of numbers that are none
+    const float best = at ? __builtin_amdgcn_exp2f((float)(__builtin_ctzll(at) % kSteps) / kSteps) : 1.f;
+    if (lane) return;
+#pragma unroll
     for (int i = 1; i < 16; ++i) s += sums[i], c += counts[i], top = __builtin_fmaxf(top, tops[i]), most = __builtin_fmaxf(most, mosts[i]);
-    *a.most = top * most;
+    const float largest = top * most, all = kTopDz / (best * largest);          // rounded down to a power of two, all * best is the scale
+    *a.most = all > 1e-30f && all < 1e30f ? kTopDz / (best * __uint_as_float(__float_as_uint(all) & 0x7f800000u)) : largest;
     if (!a.loss) return;
     *a.count = (float)(c > 1 ? c : 1);
     *a.total = (float)(a.mean ? s / (double)(c > 1 ? c : 1) : s);
@@ -1088,7 +1125,7 @@ fold_kernel(Fold a) {
             along += v[0] + v[1] + (v[2] + v[3]);
         }
         const float inv = a.inv[row];
-        along = over_wave(along, false) * inv * inv;
+        along = over_wave<false>(along) * inv * inv;
         if (inv == kNoNorm) f = 0.f, along = 0.f;
     }
     for (int d = lane * 4; d < a.D + lane * 4; d += 256) {
@@ -1337,8 +1374,8 @@ int forward(const na1d_head &h, float *loss, uint8_t *hits, const void *x, const
     NA1D_TRY(launch<finish_kernel<DT>>((unsigned)ceil_div<int64_t>(h.N, e.rows), kFinishThreads, lds, s, e));
     if (h.reduction == NA1D_HEAD_NONE) return NA1D_OK;
     float *count = reinterpret_cast<float *>(saved + o.count);
-    return launch<reduce_kernel>(1, 1024, 0, s, Reduce{loss, count, count + 1, rows, nullptr, a.h.inv_x, cosines ? reinterpret_cast<const float *>(saved + o.most) : nullptr,
-                                                       e.stats, (int)h.N, h.reduction == NA1D_HEAD_MEAN});
+    return launch<reduce_kernel>(1, 1024, 0, s, Reduce{loss, count, count + 1, rows, nullptr, a.h.inv_x, a.h.inv_w, cosines ? reinterpret_cast<const float *>(saved + o.most) : nullptr,
+                                                       e.stats, (int)h.N, h.subcenters, h.reduction == NA1D_HEAD_MEAN});
 }
 
 template <class DT>
@@ -1355,7 +1392,7 @@ int backward(const na1d_head &h, char *dx, char *dw, const float *dloss, const v
     up.dloss = dloss, up.factor = h.scale, up.mean = h.reduction == NA1D_HEAD_MEAN;           // a teacher's: temperature^2 / temperature
     if (h.reduction == NA1D_HEAD_NONE) {
         up.most = reinterpret_cast<const float *>(ws + b.most);
-        NA1D_TRY(launch<reduce_kernel>(1, 1024, 0, s, Reduce{nullptr, nullptr, reinterpret_cast<float *>(ws + b.most), nullptr, dloss, a.h.inv_x, most_w, stats, (int)h.N, 0}));
+        NA1D_TRY(launch<reduce_kernel>(1, 1024, 0, s, Reduce{nullptr, nullptr, reinterpret_cast<float *>(ws + b.most), nullptr, dloss, a.h.inv_x, a.h.inv_w, most_w, stats, (int)h.N, h.subcenters, 0}));
     } else {
         up.count = reinterpret_cast<const float *>(saved + o.count), up.most = up.count + 1;
     }

@@ -123,6 +123,23 @@ def _margin(size, subs, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=NAMES)
+@pytest.mark.parametrize("seed", range(8))
+def test_a_single_rows_target_loses_little_in_rounding(seed, dtype):
+    """Gradients of logits are scaled so that the target's, one number here, lies in the last eighth of a factor of two, where half a
+    step is at most 2^(1/8) / 2 = 0.546 of u relative to it; the other classes' are off by u at most, each in a weight row of its own."""
+    x, w, target = _inputs(1, 64, 500, dtype, 40 + seed, strength=3.0)
+    w[(target + 1) % 500] *= 0.3 + 0.04 * seed                                           # a short row, by which alone no scale may go
+    rows, ok, e, _ = O.margin(x, w.view(500, 1, 64), target)
+    up = _upstream("mean", ok, dtype)
+    _, (_, dw) = _train(lambda a, b: losses.margin_cross_entropy(a, b, target), x, w, up)
+    _, want, _ = O.margin_gradients(x, w, e, O.shares(ok, "mean", up))
+    u, mine = torch.finfo(dtype).eps / 2, torch.arange(500, device="cuda") == target
+    once = (want.to(dtype).double() - want).norm()
+    bound = u * torch.sqrt((0.546 * want[mine].norm()) ** 2 + want[~mine].norm() ** 2) + 1.1 * once + 2.0 ** -13 * want.norm() * u
+    assert (dw.double() - want).norm() <= bound + 2.0 ** -17 * want.norm()               # and what fp32 logits are off
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=NAMES)
 @pytest.mark.parametrize("top", [1, 3, 64, 100, 256])
 @pytest.mark.parametrize("size", [(1, 8, 1), (1, 64, 500), (33, 72, 63), (128, 192, 1000), (1030, 40, 300), (4100, 64, 130)],
                          ids=lambda s: "x".join(map(str, s)))
