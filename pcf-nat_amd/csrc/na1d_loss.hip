@@ -1230,8 +1230,10 @@ inline Plan plan_of(const na1d_head &h) {
         }
         return Tiling(best);
     };
-    const bool side = h.subcenters >= 2 && h.subcenters <= 4;
-    p.logits = h.N <= 32 ? Tiling(kFew) : side ? Tiling(h.subcenters == 3 ? kWide : kMany, h.subcenters) : shortest(h.subcenters > 1 ? kBatch : kVast);
+    // (Unless that takes 2^24 workgroups, as 2^36 cosines of 4 rows do: a launch has less than 2^32 threads.)
+    const Tiling side(h.subcenters == 3 ? kWide : kMany, h.subcenters);
+    const bool fits_side = h.subcenters >= 2 && h.subcenters <= 4 && side.tiles(h.V, h.N) < 1 << 24;
+    p.logits = h.N <= 32 ? Tiling(kFew) : fits_side ? side : shortest(h.subcenters > 1 ? kBatch : kVast);
     p.back = h.N > 32 && h.kind == NA1D_HEAD_MARGIN && h.subcenters == 1 ? shortest(kWide) : p.logits;
     p.m_tiles = ceil_div<int64_t>(h.V, p.logits.bm);
     const int64_t fits = std::min<int64_t>(kMostDz / (2 * h.N * h.subcenters), (1 << 20) / h.subcenters);

@@ -294,6 +294,30 @@ def test_offsets_past_32_bits():
     assert ((dx[tail].double() - want).abs() <= O.gradient_bounds(want, want_dw, magnitudes, O.logit_bound(x[tail], w, 1.0), BF16)[0]).all()
 
 
+def test_the_largest_launches():
+    """2^36 logits, and as many cosines of four weight rows: some rows against the same rows by themselves.  Losses are off by the
+    logits' fp32 sums (8 products) alone; gradients, in norm, by half a step of dz and one of their own on either side."""
+    g = torch.Generator(device="cuda").manual_seed(0)
+    for N, V, K in ((1 << 14, 1 << 22, 4), (1 << 20, 1 << 16, 1)):
+        x = torch.randn(N, 8, generator=g, device="cuda", dtype=BF16)
+        w = torch.randn(V, K, 8, generator=g, device="cuda", dtype=BF16)
+        target = torch.randint(0, V, (N,), generator=g, device="cuda")
+        call = losses.margin_cross_entropy if K > 1 else losses.linear_cross_entropy
+        some = torch.tensor([0, 1, 77, N // 2, *range(N - 40, N)], device="cuda")
+        if K > 1:
+            loss, few = call(x, w, target, reduction="none"), call(x[some], w, target[some], reduction="none")
+        else:
+            loss, dx, _ = _both(lambda a, b: call(a, b, target, reduction="none"), x, w[:, 0], torch.ones(N, device="cuda"))
+            few, dx_few, _ = _both(lambda a, b: call(a, b, target[some], reduction="none"), x[some], w[:, 0], torch.ones(len(some), device="cuda"))
+            assert ((dx[some].double() - dx_few.double()).norm(dim=1) <= 4 * 2.0 ** -8 * dx_few.double().norm(dim=1)).all()
+            up = torch.zeros(N, device="cuda")
+            up[some] = 1.0                                                   # the weight's gradient of these rows alone
+            _, _, dw = _both(lambda a, b: call(a, b, target, reduction="none"), x, w[:, 0], up)
+            _, _, dw_few = _both(lambda a, b: call(a, b, target[some], reduction="none"), x[some], w[:, 0], torch.ones(len(some), device="cuda"))
+            assert (dw.double() - dw_few.double()).norm() <= 4 * 2.0 ** -8 * dw_few.double().norm()
+        assert ((loss[some] - few).abs() <= 2.0 ** -17 * (few.abs() + 32 * 8)).all()
+
+
 def test_hits():
     x, w, target, _, _ = _inputs(N=500)
     target[::3] = torch.randint(0, 300, (167,), generator=torch.Generator().manual_seed(1)).cuda()
