@@ -1082,7 +1082,8 @@ products_kernel(Product dx, Product dw, uint32_t dx_items, uint32_t dw_items) {
 }
 
 // The shares of all splits of a row put together, less their part along the row's own vector (cosines).  WAVES waves to a row share
-// its splits.  Bound by memory: 8192 rows of 1024 channels, two splits 15 us, 5.5 TB/s.
+// its splits: four where there are 8 or more, sixteen where there are 32 and few rows (whole backwards with sixteen and with four: 20 rows of 512 channels, 61
+// splits 42 and 44 us; 700 of 96, 60 splits 83 and 76).  Bound by memory: 8192 rows of 1024 channels, two splits 15 us, 5.5 TB/s.
 struct Fold {
     char *out;
     const float *part;
@@ -1094,7 +1095,7 @@ struct Fold {
     const float *inv;
 };
 template <class DT, int WAVES>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(WAVES > 1 ? 64 * WAVES : 256)
 fold_kernel(Fold a) {
     __shared__ f32x4 met[WAVES > 1 ? WAVES : 1][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -1241,21 +1242,23 @@ inline Plan plan_of(const na1d_head &h) {
     p.ranges = ceil_div(h.V, p.plane);
     p.plane = std::min(round_up(h.V, kStep), round_up(ceil_div(h.V, p.ranges), 256));         // ranges alike
     p.ranges = ceil_div(h.V, p.plane);
-    // Products: the tiles and splits that take least, with what the sums of splits cost in memory at 4 TB/s.
-    auto split = [&](int64_t tiles, int64_t length, int64_t most, int &splits, int &per) {
-        const int64_t all = ceil_div<int64_t>(length, kStep), want = std::max<int64_t>(1, std::min<int64_t>(most / tiles, all / 4));
+    // Products: the tiles and splits (of 4, 8 or 16 steps at least) that take least, with what the sums of splits cost in memory at 4 TB/s and in
+    // waiting.  Against splits of 4 steps whatever they cost (whole backwards): 999 x 9973 of 136 channels 42 -> 35 us, 128 x 20000 of
+    // 1024 55 -> 47, 128 x 17982 of 192 23 -> 19.
+    auto split = [&](int64_t tiles, int64_t length, int64_t most, int64_t shortest_split, int &splits, int &per) {
+        const int64_t all = ceil_div<int64_t>(length, kStep), want = std::max<int64_t>(1, std::min<int64_t>(most / tiles, all / shortest_split));
         per = (int)(ceil_div(all, want) * kStep);
         splits = (int)ceil_div<int64_t>(length, per);
     };
     double least = 1e30;
-    for (const Pick pick : {kBatch, kMany, kWide, kVast}) {
+    for (const Pick pick : {kBatch, kMany, kWide, kVast}) for (const int64_t shortest_split : {4, 8, 16}) {
         Plan q = p;
         q.dx = Tiling(h.N <= 32 ? kFew : pick), q.dw = Tiling(pick);
         const int64_t dx_tiles = q.dx.tiles(h.D, h.N), dw_tiles = h.subcenters * q.dw.tiles(h.D, q.plane), most = cost_of(pick).slots;
-        split(dx_tiles, q.plane, most, q.dx_splits, q.dx_per);
-        split(dw_tiles, h.N, most, q.dw_splits, q.dw_per);
+        split(dx_tiles, q.plane, most, shortest_split, q.dx_splits, q.dx_per);
+        split(dw_tiles, h.N, most, shortest_split, q.dw_splits, q.dw_per);
         const double fold = (8. * q.dx_splits * h.N * h.D + (q.dw_splits > 1 ? 8. * q.dw_splits * h.subcenters * q.plane * h.D : 0.)) / 4.0e6;
-        const double t = fold + time_of(pick, dx_tiles * q.dx_splits, (int64_t)h.subcenters * q.dx_per / kStep, dw_tiles * q.dw_splits, q.dw_per / kStep, 2.);          // whose ends store more
+        const double t = fold + 0.05 * q.dx_splits + time_of(pick, dx_tiles * q.dx_splits, (int64_t)h.subcenters * q.dx_per / kStep, dw_tiles * q.dw_splits, q.dw_per / kStep, 2.);          // whose ends store more
         if (t < least && (h.N > 32 || pick <= kMany)) p = q, least = t;
     }
     return p;
@@ -1428,6 +1431,7 @@ int backward(const na1d_head &h, char *dx, char *dw, const float *dloss, const v
     }
     auto fold = [&](char *out, int64_t part, int64_t rows, int splits, const char *own, int64_t own_pitch, const float *inv) {
         const Fold f{out, reinterpret_cast<const float *>(ws + part), rows * h.D, rows, splits, (int)h.D, up, cosines ? own : nullptr, own_pitch, inv};
+        if (splits >= 32 && rows <= 512) return launch<fold_kernel<DT, 16>>((unsigned)rows, 1024, 0, s, f);
         return splits >= 8 ? launch<fold_kernel<DT, 4>>((unsigned)rows, 256, 0, s, f) : launch<fold_kernel<DT, 1>>((unsigned)ceil_div<int64_t>(rows, 4), 256, 0, s, f);
     };
     if (dx) NA1D_TRY(fold(dx, b.dx, h.N, p.dx_splits, a.h.x, a.h.x_pitch, a.h.inv_x));
