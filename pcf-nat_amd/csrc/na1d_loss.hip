@@ -1119,21 +1119,27 @@ fold_kernel(Fold a) {
         return v;
     };
     auto own = [&](int d) { return d < a.D ? widen4<DT>(*reinterpret_cast<const u32x2 *>(a.own + row * a.own_pitch + 2 * d)) : f32x4{0.f, 0.f, 0.f, 0.f}; };
+    constexpr int kKept = 2;                                                    // of a row's 256 channels, for the second look at them
+    f32x4 kept[kKept];
     float along = 0.f;
+    auto add = [&](f32x4 v) { along += v[0] + v[1] + (v[2] + v[3]); };
     if (a.own) {
-        for (int d = lane * 4; d < a.D + lane * 4; d += 256) {
-            const f32x4 v = sum(d) * own(d);
-            along += v[0] + v[1] + (v[2] + v[3]);
-        }
+#pragma unroll
+        for (int i = 0; i < kKept; ++i)
+            if (256 * i < a.D) kept[i] = sum(256 * i + lane * 4), add(kept[i] * own(256 * i + lane * 4));
+        for (int d = 256 * kKept; d < a.D; d += 256) add(sum(d + lane * 4) * own(d + lane * 4));
         const float inv = a.inv[row];
         along = over_wave<false>(along) * inv * inv;
         if (inv == kNoNorm) f = 0.f, along = 0.f;
     }
-    for (int d = lane * 4; d < a.D + lane * 4; d += 256) {
-        f32x4 v = sum(d);
+    auto store = [&](int d, f32x4 v) {
         if (a.own) v -= along * own(d);
         if (d < a.D && (WAVES == 1 || wave == 0)) *reinterpret_cast<u32x2 *>(a.out + (row * a.D + d) * 2) = narrow4<DT>(v * f);
-    }
+    };
+#pragma unroll
+    for (int i = 0; i < kKept; ++i)
+        if (256 * i < a.D) store(256 * i + lane * 4, a.own ? kept[i] : sum(256 * i + lane * 4));
+    for (int d = 256 * kKept; d < a.D; d += 256) store(d + lane * 4, sum(d + lane * 4));
 }
 
 // =============================================================================
