@@ -400,7 +400,7 @@ int na1d_train_context_backward(void *dx, const void *dctx, const void *x, const
  *           elsewhere, where a row has no target, and for a teacher
  *   saved : what a forward leaves for its backward, na1d_head_saved_bytes() bytes; a forward needs it in any case
  *   dx, dw: 16-bit, packed [N, D] and [V * subcenters, D]; either may be NULL
- * Sums are in fp32; the gradients of the logits are rounded to 16 bits (fp16: scaled by a power of two first) before they
+ * Sums are in fp32; the gradients of the logits are scaled as one and rounded to 16 bits before they
  * are multiplied.  Nothing uses atomics: results are the same from call to call.
  * D % 8 == 0; x, w, dx, dw, saved and the workspace 16-byte aligned, strides multiples of 8 and at least D.  Limits
  * (NA1D_ERR_UNSUPPORTED): N up to 2^20, V * subcenters up to 2^24, w_stride * subcenters and x_stride up to 2^20, N * V, N * D and
