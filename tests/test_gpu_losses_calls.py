@@ -1,9 +1,11 @@
 """Losses over many classes as they are called: layouts, masks, streams, graphs, compiled, in the models, and together."""
 import math
+import threading
 
 import pytest
 import torch
 import torch.nn.functional as F
+import torch.utils.checkpoint
 
 from na1d_amd import _lib, losses, models
 from oracle import losses_oracle as O
@@ -292,6 +294,50 @@ def test_offsets_past_32_bits():
     assert ((loss[tail] - rows).abs() <= O.logit_bound(x[tail], w, 1.0)).all()
     want, want_dw, magnitudes = O.linear_gradients(x[tail], w, e, torch.ones(1000, device="cuda"))
     assert ((dx[tail].double() - want).abs() <= O.gradient_bounds(want, want_dw, magnitudes, O.logit_bound(x[tail], w, 1.0), BF16)[0]).all()
+
+
+def test_calls_of_several_threads_at_once():
+    sizes = ((128, 192, 3000, BF16), (700, 256, 5001, FP16), (33, 64, 900, BF16), (1, 128, 21000, FP16))
+    cases = [_inputs(N, D, V, dtype, seed=i) for i, (N, D, V, dtype) in enumerate(sizes)]
+    pairs = [(_calls(target, ids, logits)["margin"], x, w) for x, w, target, ids, logits in cases]
+    want = [_both(*p) for p in pairs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(k):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            got = [((i + k) % 4, _both(*pairs[(i + k) % 4])) for i in range(20)]
+        stream.synchronize()
+        wrong.extend(j for j, g in got if not _same(g, want[j]))
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_a_graph_of_one_loss_and_other_nodes(kind):
+    """Kept for a second backward, recomputed under checkpointing, with a weight that makes x too, and one that is written to in between."""
+    x, w, target, ids, logits = _inputs()
+    call = _calls(target, ids, logits)[kind]
+    want = _both(call, x, w)[1:]
+    a, b = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    loss = call(a, b)
+    assert _same(torch.autograd.grad(loss, [a, b], retain_graph=True), want) and _same(torch.autograd.grad(loss, [a, b]), want)
+    loss = torch.utils.checkpoint.checkpoint(call, a, b, use_reentrant=False)
+    assert _same(torch.autograd.grad(loss, [a, b]), want)
+    tied, = torch.autograd.grad(call(b[:33], b), b)
+    apart = _both(call, w[:33], w)[1:]
+    assert torch.equal(tied, torch.cat([apart[1][:33] + apart[0], apart[1][33:]]))
+    loss = call(a, b)
+    with torch.no_grad():
+        b.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
 
 
 def test_the_largest_launches():
