@@ -886,7 +886,7 @@ reduce_kernel(Reduce a) {
         const RowStat st = a.stats[r];
         some = __builtin_fabsf(st.at_target) * (a.dloss ? __builtin_fabsf(a.dloss[r]) : 1.f);
         if (a.inv_x && st.sub >= 0) some *= a.inv_x[r] * a.inv_w[(int64_t)st.target * a.subs + st.sub];
-        some = __builtin_fminf(some, 0x1p60f);
+        some = st.sub < 0 ? 0.f : __builtin_fminf(some, 0x1p60f);              // (0 times what is no number is none)
     }
 #pragma unroll 8
     for (int r = threadIdx.x; r < a.N; r += 1024) {
@@ -936,15 +936,16 @@ reduce_kernel(Reduce a) {
 // =============================================================================
 // Backward
 // =============================================================================
-// The teacher's entries of dz, which the logits' kernel left as those of any class.  Entries of one class write the same value.
+// The teacher's entries of dz, which the logits' kernel left as those of any class.  Entries of one class write the same value.  A row
+// that does not count has its zeros already; its coefficients are zeros too, but what comes from upstream need not be a number.
 template <class DT>
 __global__ void __launch_bounds__(256)
-entries_kernel(uint16_t *__restrict__ dz, const float *__restrict__ coeff, Upstream up, const void *__restrict__ ids, int ids_wide, int N, int top, int class0, int classes,
-               int64_t plane) {
+entries_kernel(uint16_t *__restrict__ dz, const float *__restrict__ coeff, const RowStat *__restrict__ stats, Upstream up, const void *__restrict__ ids, int ids_wide, int N, int top,
+               int class0, int classes, int64_t plane) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= (int64_t)N * top) return;
     const int64_t row = i / top, c = (int64_t)load_id(ids, i, ids_wide) - class0;
-    if (c < 0 || c >= classes) return;
+    if (c < 0 || c >= classes || stats[row].sub < 0) return;
     const float base = up.base();
     dz[row * plane + c] = (uint16_t)Mma<DT>::pack(coeff[i] * (base * up.up(base) * (up.count ? 1.f : up.dloss[row])), 0.f);
 }
@@ -1417,8 +1418,8 @@ int backward(const na1d_head &h, char *dx, char *dw, const float *dloss, const v
         g.columns = (int)round_up(a.classes, kStep);
         NA1D_TRY((launch_logits<DT, true>(h, p.back, a, s)));
         if (h.kind == NA1D_HEAD_TEACHER) {
-            entries_kernel<DT><<<(unsigned)ceil_div<int64_t>(h.N * h.top, 256), 256, 0, s>>>((uint16_t *)a.dz, reinterpret_cast<const float *>(saved + o.coeff), up, ids,
-                                                                                             h.ids_64, (int)h.N, h.top, a.class0, a.classes, p.plane);
+            entries_kernel<DT><<<(unsigned)ceil_div<int64_t>(h.N * h.top, 256), 256, 0, s>>>((uint16_t *)a.dz, reinterpret_cast<const float *>(saved + o.coeff), stats,
+                                                                                             up, ids, h.ids_64, (int)h.N, h.top, a.class0, a.classes, p.plane);
             NA1D_TRY(launch_status());
         }
         Product gx = g, gw = g;                                                               // what is not asked for has no workgroups

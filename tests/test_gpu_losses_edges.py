@@ -1,0 +1,72 @@
+"""Losses over many classes at the edges of what they take: rows that do not count beside upstream gradients that are not finite,
+losses that are written to, rows far apart, workgroups' rows behind the last, the largest weights and batches, and ops called by themselves."""
+import math
+
+import pytest
+import torch
+
+from na1d_amd import losses, ops
+from oracle import losses_oracle as O
+
+pytestmark = pytest.mark.gpu
+
+BF16, FP16 = torch.bfloat16, torch.float16
+KINDS = ["ce", "margin", "distil"]
+
+
+def _inputs(N=33, D=72, V=300, dtype=BF16, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    w = (torch.randn(V, D, generator=g) * D ** -0.5).to(dtype).cuda()
+    target = torch.randint(0, V, (N,), generator=g).cuda()
+    x = (torch.randn(N, D, generator=g).cuda() + 3 * w[target].float()).to(dtype)
+    ids = torch.stack([torch.randperm(V, generator=g)[:6] for _ in range(N)]).cuda()
+    logits = torch.randn(N, 6, generator=g).cuda()
+    return x, w, target, ids, logits
+
+
+def _calls(target, ids, logits, reduction="mean"):
+    return {"ce": lambda x, w: losses.linear_cross_entropy(x, w, target, reduction=reduction),
+            "margin": lambda x, w: losses.margin_cross_entropy(x, w.unflatten(0, (-1, 3)), target // 3, reduction=reduction),
+            "distil": lambda x, w: losses.linear_distillation(x, w, logits, ids, 2.0, reduction)}
+
+
+def _both(call, x, w, up=None):
+    x, w = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+    loss = call(x, w)
+    return [loss.detach(), *torch.autograd.grad(loss, [x, w], up)]
+
+
+def _same(a, b):
+    return all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("kind", KINDS)
+def test_rows_that_do_not_count_have_no_use_for_an_upstream_gradient(kind, dtype):
+    """Whatever comes to such a row, its gradient is zero and the others' are the same to the bit.  (A bad target's loss is no number,
+    so what is built on it mostly hands none back.)"""
+    x, w, target, ids, logits = _inputs(N=130, dtype=dtype)
+    rows = torch.tensor([4, 60, 129], device="cuda")
+    ways = {"ignored": -100, "no class": 300} if kind != "distil" else {"absent": -1, "no class": 300, "all -inf": None}
+    for name, bad in ways.items():
+        t, i, l = target.clone(), ids.clone(), logits.clone()
+        if kind == "margin":
+            t[rows] = -100 if name == "ignored" else 900
+        elif kind == "ce":
+            t[rows] = bad
+        elif name == "all -inf":
+            l[rows] = -math.inf
+        elif name == "absent":
+            i[rows] = -1
+        else:
+            i[rows, 2] = bad
+        if kind == "margin":
+            call = lambda x, w: losses.margin_cross_entropy(x, w.unflatten(0, (-1, 3)), torch.where(t < 0, t, t // 3), reduction="none")
+        else:
+            call = _calls(t, i, l, "none")[kind]
+        up = torch.rand(130, generator=torch.Generator().manual_seed(2)).cuda()
+        want = _both(call, x, w, up)[1:]
+        assert not want[0][rows].any() and all(torch.isfinite(g).all() and g.any() for g in want)
+        for value in (math.nan, math.inf, -math.inf, 3e38, 0.0):
+            got = _both(call, x, w, up.index_fill(0, rows, value))[1:]
+            assert _same(got, want), (name, value)
