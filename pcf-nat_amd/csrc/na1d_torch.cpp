@@ -360,13 +360,17 @@ bool index_type(const Tensor &t) { return t.scalar_type() == at::kLong || t.scal
 bool on(const Tensor &t, const Tensor &like) { return plain(t) && t.is_contiguous() && t.device() == like.device(); }
 Tensor bytes_of(int64_t n, const Tensor &like) { return at::empty({n}, like.options().dtype(at::kByte)); }
 
+// (Not as tensors of their own: a loss that goes into a node's function and comes out of it would be a view, which refuses to be written to.)
+struct HeadDone {
+    Tensor loss, saved;
+};
 struct HeadLoss : torch::autograd::Function<HeadLoss> {
-    static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &weight, const Tensor &ids, const na1d_head &h, const Tensor &loss, const Tensor &saved) {
-        ctx->save_for_backward({x, weight, ids, saved});
+    static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &weight, const Tensor &ids, const na1d_head &h, const HeadDone &done) {
+        ctx->save_for_backward({x, weight, ids, done.saved});
         ctx->saved_data["whole"] = std::vector<int64_t>{h.kind, h.top, h.teacher_type, h.ignore_index, h.reduction};
         ctx->saved_data["scale"] = (double)h.scale;
         ctx->saved_data["margin"] = (double)h.margin;
-        return loss;
+        return done.loss;
     }
     static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
         const variable_list s = ctx->get_saved_variables();
@@ -393,7 +397,7 @@ struct HeadLoss : torch::autograd::Function<HeadLoss> {
                 *t = (*error)({t->set_requires_grad(true)})[0];
             }
         }
-        return {dx, dw, Tensor(), Tensor(), Tensor(), Tensor()};
+        return {dx, dw, Tensor(), Tensor(), Tensor()};
     }
 };
 MaybeTensor head(const Tensor &x, const Tensor &weight, const Tensor &ids, const MaybeTensor &teacher, const MaybeTensor &hits, int kind, double scale, double margin,
@@ -411,13 +415,13 @@ MaybeTensor head(const Tensor &x, const Tensor &weight, const Tensor &ids, const
     const int64_t saved_bytes = na1d_head_saved_bytes(&h), ws_bytes = na1d_head_workspace_bytes(&h, 0);
     if (saved_bytes < 0 || ws_bytes < 0) return std::nullopt;
     const c10::DeviceGuard guard(x.device());
-    const Tensor loss = at::empty(reduction == NA1D_HEAD_NONE ? x.sizes().slice(0, x.dim() - 1) : at::IntArrayRef{}, x.options().dtype(at::kFloat));
-    const Tensor saved = bytes_of(saved_bytes, x), ws = bytes_of(ws_bytes, x);
-    if (na1d_head_forward(&h, (float *)ptr(loss), hits ? (uint8_t *)ptr(*hits) : nullptr, ptr(x), ptr(weight), ptr(ids), teacher ? ptr(*teacher) : nullptr, ptr(saved), saved_bytes, ptr(ws), ws_bytes,
+    const Tensor ws = bytes_of(ws_bytes, x);
+    const HeadDone done{at::empty(reduction == NA1D_HEAD_NONE ? x.sizes().slice(0, x.dim() - 1) : at::IntArrayRef{}, x.options().dtype(at::kFloat)), bytes_of(saved_bytes, x)};
+    if (na1d_head_forward(&h, (float *)ptr(done.loss), hits ? (uint8_t *)ptr(*hits) : nullptr, ptr(x), ptr(weight), ptr(ids), teacher ? ptr(*teacher) : nullptr, ptr(done.saved), saved_bytes, ptr(ws), ws_bytes,
                           stream_of(x)) != NA1D_OK)
         return std::nullopt;
-    if (!at::GradMode::is_enabled() || !(x.requires_grad() || weight.requires_grad())) return loss;
-    return HeadLoss::apply(x, weight, ids, h, loss, saved);
+    if (!at::GradMode::is_enabled() || !(x.requires_grad() || weight.requires_grad())) return done.loss;
+    return HeadLoss::apply(x, weight, ids, h, done);
 }
 
 // ------------------------------------------------------------------------------------------------ an encoder layer in training

@@ -70,3 +70,22 @@ def test_rows_that_do_not_count_have_no_use_for_an_upstream_gradient(kind, dtype
         for value in (math.nan, math.inf, -math.inf, 3e38, 0.0):
             got = _both(call, x, w, up.index_fill(0, rows, value))[1:]
             assert _same(got, want), (name, value)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_losses_are_written_to(kind):
+    """A loss is a tensor of its own, whichever node it comes from: divided, added to and cut off in place."""
+    x, w, target, ids, logits = _inputs()
+    for reduction in ("mean", "none"):
+        call = _calls(target, ids, logits, reduction)[kind]
+        want = _both(lambda a, b: call(a, b).sum() / 4, x, w)
+        for lay in (lambda t: t.detach().clone(), lambda t: t.detach().t().contiguous().t()):          # by the native node, and the other
+            a, b = lay(x).requires_grad_(True), lay(w).requires_grad_(True)
+            loss = call(a, b)
+            assert not loss._is_view()
+            loss /= 4
+            total = loss.sum()
+            total += 1
+            assert _same(torch.autograd.grad(total, [a, b]), want[1:])
+            loss = call(a, b)
+            assert not loss.detach_().requires_grad
