@@ -8,7 +8,7 @@ the backward works the logits out again, a range of classes at a time.
 
 All take ``x [..., D]`` and ``weight`` in bfloat16 or float16 on the GPU, D a multiple of 8, and give fp32 losses and
 gradients in the types of x and weight (fp16: scale the loss as ever).  Rows may lie apart (any stride that is a multiple of 8
-elements); what is laid out otherwise is packed first.
+elements, a class's rows together up to 2^20 of them); what is laid out otherwise is packed first.
 """
 from __future__ import annotations
 
@@ -22,6 +22,7 @@ from . import _lib
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 _TARGETS, _MARGIN, _TEACHER = range(3)
 MAX_TOP = 256                                        # NA1D_HEAD_MAX_TOP
+_MAX_STRIDE = 1 << 20                                # elements from one row, or from one class's rows to the next, that the native call takes
 _FP32 = 2
 _IDS = (torch.int32, torch.int64)
 
@@ -32,10 +33,10 @@ class _Head(ctypes.Structure):                       # na1d_head
                 + [(n, ctypes.c_int64) for n in "ignore_index N V D x_stride w_stride".split()])
 
 
-def _rows(t):
-    """``t [..., D]`` as rows: their number apart, contiguous and 16-byte aligned."""
+def _rows(t, to_class=1):
+    """``t [..., D]`` as rows, ``to_class`` of them to a class: their number apart, contiguous and 16-byte aligned."""
     t = t.reshape(-1, t.shape[-1])
-    if t.stride(1) != 1 or (t.shape[0] > 1 and (t.stride(0) % 8 or t.stride(0) < t.shape[1])):
+    if t.stride(1) != 1 or (t.shape[0] > 1 and (t.stride(0) % 8 or not t.shape[1] <= t.stride(0) <= _MAX_STRIDE // to_class)):
         t = t.contiguous()
     return t.clone(memory_format=torch.contiguous_format) if t.data_ptr() % 16 else t
 
@@ -68,7 +69,7 @@ def head_forward(x, weight, ids, teacher, hits, kind, scale, margin, ignore_inde
             hits.zero_()
         return loss.zero_(), torch.empty(0, dtype=torch.uint8, device=x.device)
     h = _head(x, weight, ids, teacher, kind, scale, margin, ignore_index, reduction)
-    xr, wr, ids = _rows(x), _rows(weight), ids.contiguous()
+    xr, wr, ids = _rows(x), _rows(weight, h.subcenters), ids.contiguous()
     teacher = None if teacher is None else teacher.contiguous()
     h.x_stride, h.w_stride = _stride(xr), _stride(wr)
     nsaved, nws = _sizes(h, 0)
@@ -86,7 +87,7 @@ def head_backward(dloss, x, weight, ids, teacher, saved, kind, scale, margin, ig
     if x.numel() == 0:
         return dx.zero_(), dw.zero_()
     h = _head(x, weight, ids, teacher, kind, scale, margin, ignore_index, reduction)
-    xr, wr, ids, dloss = _rows(x), _rows(weight), ids.contiguous(), dloss.contiguous()
+    xr, wr, ids, dloss = _rows(x), _rows(weight, h.subcenters), ids.contiguous(), dloss.contiguous()
     h.x_stride, h.w_stride = _stride(xr), _stride(wr)
     _, nws = _sizes(h, 1)
     ws = torch.empty(nws, dtype=torch.uint8, device=x.device)

@@ -89,3 +89,23 @@ def test_losses_are_written_to(kind):
             assert _same(torch.autograd.grad(total, [a, b]), want[1:])
             loss = call(a, b)
             assert not loss.detach_().requires_grad
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_rows_very_far_apart(kind):
+    """The last state of long sequences is a view whose rows are more than 2^20 elements apart, and so may a weight's be."""
+    x, w, target, ids, logits = _inputs(N=5, V=30)
+    want = _both(_calls(target, ids, logits)[kind], x, w)
+    far = (1 << 20) + 8
+    hidden, table = torch.empty(5, far, dtype=BF16, device="cuda"), torch.empty(30, far, dtype=BF16, device="cuda")
+    last, rows = hidden[:, -72:], table[:, 8:80]
+    last.copy_(x), rows.copy_(w)
+    a, b = last.requires_grad_(True), rows.requires_grad_(True)
+    assert a.stride(0) == far and b.stride(0) == far
+    loss = _calls(target, ids, logits)[kind](a, b)
+    assert _same([loss.detach(), *torch.autograd.grad(loss, [a, b])], want)
+    if kind == "margin":                                                   # a class's three rows together reach further than that
+        near = torch.empty(30, 1 << 19, dtype=BF16, device="cuda")[:, :72].copy_(w).unflatten(0, (10, 3)).requires_grad_(True)
+        loss = losses.margin_cross_entropy(x, near, target // 3)
+        assert near.stride() == (3 << 19, 1 << 19, 1) and torch.equal(loss.detach(), want[0])
+        assert torch.equal(torch.autograd.grad(loss, near)[0].view(30, 72), want[2])
