@@ -559,10 +559,12 @@ logits_kernel(Logits a) {
 #pragma unroll
         for (int j = 0; j < S::NT; ++j) {
             const int row = 16 * (wn * S::NT + j) + n;
-            const RowStat rg = row_stats[j];
+            RowStat rg = row_stats[j];
             const float ix = row_inv[j], c2 = a.h.scale2 * ix;
             float f = common * row_up[j] * ix;
-            if (r0 + row >= a.h.N || rg.sub < 0 || (COS && ix == kNoNorm)) f = 0.f;           // rows behind the last have no share in the sums
+            if (rg.sub < 0 || (COS && ix == kNoNorm)) f = 0.f;
+            // Rows behind the last have no share in the sums.  Their products are 0, which may be far above the logarithm of the last row's sum.
+            if (r0 + row >= a.h.N) f = 0.f, rg.lse2 = __builtin_inff();
             const float e = f * rg.at_target;
             const int64_t t = (int64_t)rg.target - c0;
             const bool hit = t >= 16 * wm * CT && t < 16 * (wm + 1) * CT;

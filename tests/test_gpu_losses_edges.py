@@ -109,3 +109,27 @@ def test_rows_very_far_apart(kind):
         loss = losses.margin_cross_entropy(x, near, target // 3)
         assert near.stride() == (3 << 19, 1 << 19, 1) and torch.equal(loss.detach(), want[0])
         assert torch.equal(torch.autograd.grad(loss, near)[0].view(30, 72), want[2])
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("V,K", [(1, 1), (2, 1), (2, 2), (2, 3), (2, 5)])
+def test_a_last_row_that_is_far_from_every_class(V, K, dtype):
+    """All its cosines are near -1 and the scale is large, so that the logarithm of its sum is far below zero: what stands behind it in
+    its tile has no share in any gradient."""
+    g = torch.Generator().manual_seed(V * 10 + K)
+    for N in (1, 37, 130):
+        base = torch.randn(64, generator=g)
+        w = (base + 0.02 * torch.randn(V, K, 64, generator=g)).to(dtype).cuda()
+        x = (-base + 0.02 * torch.randn(N, 64, generator=g)).to(dtype).cuda()
+        target = torch.randint(0, V, (N,), generator=g).cuda()
+        for scale in (128.0, 500.0):
+            rows, ok, e, cosines = O.margin(x, w, target, scale=scale)
+            up = torch.full((N,), 16.0, device="cuda")
+            loss, dx, dw = _both(lambda a, b: losses.margin_cross_entropy(a, b, target, scale=scale, reduction="none"), x, w, up)
+            delta = O.logit_bound(O.unit(x.double()), O.unit(w.double().view(V * K, 64)), scale)
+            assert ((loss - rows).abs() <= 2 * delta + 2.0 ** -20 * rows).all()
+            gx, gw, magnitudes = O.margin_gradients(x, w, e, up)
+            far = O.undecided(x, w, e, cosines, up)
+            # fp16: half a step of the smallest dz, 2^-39 of the largest, in up to 130 terms
+            bx, bw = O.gradient_bounds(gx, gw, magnitudes, 2 * delta, dtype, 2.0 ** -31 * 4 * scale)
+            assert ((dx.double() - gx).abs() <= bx + far[0]).all() and ((dw.double().view(V * K, 64) - gw).abs() <= bw + far[1]).all()
