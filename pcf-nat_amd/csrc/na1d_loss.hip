@@ -1438,10 +1438,11 @@ int backward(const na1d_head &h, char *dx, char *dw, const float *dloss, const v
         }
         NA1D_TRY(launch_products<DT>(p, gx, gw, s));
     }
+    // (A launch has less than 2^32 threads.)
     auto fold = [&](char *out, int64_t part, int64_t rows, int splits, const char *own, int64_t own_pitch, const float *inv) {
         const Fold f{out, reinterpret_cast<const float *>(ws + part), rows * h.D, rows, splits, (int)h.D, up, cosines ? own : nullptr, own_pitch, inv};
         if (splits >= 32 && rows <= 512) return launch<fold_kernel<DT, 16>>((unsigned)rows, 1024, 0, s, f);
-        return splits >= 8 ? launch<fold_kernel<DT, 4>>((unsigned)rows, 256, 0, s, f) : launch<fold_kernel<DT, 1>>((unsigned)ceil_div<int64_t>(rows, 4), 256, 0, s, f);
+        return splits >= 8 && rows < 1 << 24 ? launch<fold_kernel<DT, 4>>((unsigned)rows, 256, 0, s, f) : launch<fold_kernel<DT, 1>>((unsigned)ceil_div<int64_t>(rows, 4), 256, 0, s, f);
     };
     if (dx) NA1D_TRY(fold(dx, b.dx, h.N, p.dx_splits, a.h.x, a.h.x_pitch, a.h.inv_x));
     if (dw && p.dw_splits > 1) NA1D_TRY(fold(dw, b.dw, h.V * h.subcenters, p.dw_splits, a.h.w, a.h.w_pitch, a.h.inv_w));

@@ -133,3 +133,22 @@ def test_a_last_row_that_is_far_from_every_class(V, K, dtype):
             # fp16: half a step of the smallest dz, 2^-39 of the largest, in up to 130 terms
             bx, bw = O.gradient_bounds(gx, gw, magnitudes, 2 * delta, dtype, 2.0 ** -31 * 4 * scale)
             assert ((dx.double() - gx).abs() <= bx + far[0]).all() and ((dw.double().view(V * K, 64) - gw).abs() <= bw + far[1]).all()
+
+
+def test_the_largest_weight_that_many_rows_share():
+    """2^24 weight rows, four to a class, and a batch of which the weight's gradient is summed in parts: some rows' share of both
+    gradients against the same rows by themselves.  In norm they differ by half a step of dz and one of their own on either side."""
+    g = torch.Generator(device="cuda").manual_seed(0)
+    N, V, K = 1 << 14, 1 << 22, 4
+    x = torch.randn(N, 8, generator=g, device="cuda", dtype=BF16)
+    w = torch.randn(V, K, 8, generator=g, device="cuda", dtype=BF16)
+    target = torch.randint(0, V, (N,), generator=g, device="cuda")
+    some = torch.tensor([0, 1, 77, N // 2, *range(N - 40, N)], device="cuda")
+    up = torch.zeros(N, device="cuda").index_fill(0, some, 1.0)
+    call = lambda t: lambda a, b: losses.margin_cross_entropy(a, b, t, reduction="none")
+    loss, dx, dw = _both(call(target), x, w, up)
+    few, dx_few, dw_few = _both(call(target[some]), x[some], w, torch.ones(len(some), device="cuda"))
+    # A row's two nearest of a class may be closer than fp32 tells: tiles of either batch add in another order.
+    assert ((loss[some] - few).abs() <= 2.0 ** -17 * (few.abs() + 32 * 8)).all()
+    assert ((dx[some].double() - dx_few.double()).norm(dim=1) <= 4 * 2.0 ** -8 * dx_few.double().norm(dim=1)).all()
+    assert (dw.double() - dw_few.double()).norm() <= 4 * 2.0 ** -8 * dw_few.double().norm()
