@@ -962,11 +962,11 @@ struct Product {
     int N, D, subs;
     int classes, columns, class0;   // of this range; its columns of dz, whole steps
     int m_tiles, n_tiles, splits, per;          // per: of the contraction to a split, a multiple of kStep
-    float *part;                    // fp32 [splits, rows, D]
+    float *part;                    // fp32 [splits, rows, D]; dW: the range's rows
     int64_t part_stride;
     int add;                        // to what is there
     Upstream up;
-    // dW without splits
+    // dW at once
     char *out;                      // 16-bit [V * subs, D], or NULL: to part
     const char *w;                  // cosines: dW loses its part along w
     int64_t w_pitch;
@@ -1057,7 +1057,7 @@ __device__ inline void product(const Product &a, uint32_t item, LDS_PTR(char) ld
 #pragma unroll
     for (int j = 0; j < S::NT; ++j) {
         const int in = 16 * (wn * S::NT + j) + n;
-        const int64_t row = DW ? (int64_t)(a.class0 + col0 + in) * a.subs + sub : r0 + in;
+        const int64_t row = DW ? (int64_t)(col0 + in) * a.subs + sub : r0 + in;
         if (DW ? col0 + in >= a.classes : r0 + in >= a.N) continue;
         float *to = a.part + split * a.part_stride + row * a.D;
 #pragma unroll
@@ -1186,9 +1186,10 @@ struct Tiling {
 struct Plan {
     Tiling logits, back;                      // of the forward, of the backward
     int64_t m_tiles;
-    // backward: ranges of classes
+    // backward: ranges of classes, and within each, batches of rows
     int64_t plane;                            // columns to a sub-centre: a range's classes, rounded up to whole steps
-    int64_t ranges;
+    int64_t ranges, rows, batches;
+    bool dw_at_once() const { return dw_splits == 1 && batches == 1; }        // else in parts, which are put together behind each range
     Tiling dx, dw;
     int dx_splits, dx_per, dw_splits, dw_per;
 };
@@ -1251,6 +1252,11 @@ inline Plan plan_of(const na1d_head &h) {
     p.ranges = ceil_div(h.V, p.plane);
     p.plane = std::min(round_up(h.V, kStep), round_up(ceil_div(h.V, p.ranges), 256));         // ranges alike
     p.ranges = ceil_div(h.V, p.plane);
+    // More than 2^19 rows (times sub-centres) do not fit with 256 classes, and with fewer dx would be read and written in fp32 all the more often: such
+    // rows are taken in batches, alike too.
+    p.batches = ceil_div<int64_t>(2 * h.N * h.subcenters * p.plane, kMostDz);
+    p.rows = p.batches > 1 ? round_up(ceil_div(h.N, p.batches), 256) : h.N;
+    p.batches = ceil_div(h.N, p.rows);
     // Products: the tiles and splits (of 4, 8 or 16 steps at least) that take least, with what the sums of splits cost in memory at 4 TB/s and in
     // waiting.  Against splits of 4 steps whatever they cost (whole backwards): 999 x 9973 of 136 channels 42 -> 35 us, 128 x 20000 of
     // 1024 55 -> 47, 128 x 17982 of 192 23 -> 19.
@@ -1263,10 +1269,10 @@ inline Plan plan_of(const na1d_head &h) {
     for (const Pick pick : {kBatch, kMany, kWide, kVast}) for (const int64_t shortest_split : {4, 8, 16}) {
         Plan q = p;
         q.dx = Tiling(h.N <= 32 ? kFew : pick), q.dw = Tiling(pick);
-        const int64_t dx_tiles = q.dx.tiles(h.D, h.N), dw_tiles = h.subcenters * q.dw.tiles(h.D, q.plane), most = cost_of(pick).slots;
+        const int64_t dx_tiles = q.dx.tiles(h.D, p.rows), dw_tiles = h.subcenters * q.dw.tiles(h.D, q.plane), most = cost_of(pick).slots;
         split(dx_tiles, q.plane, most, shortest_split, q.dx_splits, q.dx_per);
-        split(dw_tiles, h.N, most, shortest_split, q.dw_splits, q.dw_per);
-        const double fold = (8. * q.dx_splits * h.N * h.D + (q.dw_splits > 1 ? 8. * q.dw_splits * h.subcenters * q.plane * h.D : 0.)) / 4.0e6;
+        split(dw_tiles, p.rows, most, shortest_split, q.dw_splits, q.dw_per);
+        const double fold = (8. * q.dx_splits * p.rows * h.D + (q.dw_splits > 1 ? 8. * q.dw_splits * h.subcenters * q.plane * h.D : 0.)) / 4.0e6;
         const double t = fold + 0.05 * q.dx_splits + time_of(pick, dx_tiles * q.dx_splits, (int64_t)h.subcenters * q.dx_per / kStep, dw_tiles * q.dw_splits, q.dw_per / kStep, 2.);          // whose ends store more
         if (t < least && (h.N > 32 || pick <= kMany)) p = q, least = t;
     }
@@ -1287,10 +1293,10 @@ struct BackwardScratch {
         int64_t at = 0;
         auto take = [&](int64_t n) { const int64_t q = at; at += round_up(n, 256); return q; };
         most = take(16);
-        dz = take(2 * h.N * h.subcenters * p.plane);
+        dz = take(2 * p.rows * h.subcenters * p.plane);
         dx = take(4 * h.N * h.D * p.dx_splits);
-        dw = take(p.dw_splits > 1 ? 4 * h.V * h.subcenters * h.D * p.dw_splits : 0);
-        cols = take(h.kind == NA1D_HEAD_MARGIN && p.dw_splits == 1 ? 4 * ceil_div<int64_t>(h.N, p.back.bn) * p.back.wn * h.subcenters * p.plane : 0);
+        dw = take(p.dw_at_once() ? 0 : 4 * p.plane * h.subcenters * h.D * p.dw_splits);
+        cols = take(h.kind == NA1D_HEAD_MARGIN && p.dw_at_once() ? 4 * ceil_div<int64_t>(h.N, p.back.bn) * p.back.wn * h.subcenters * p.plane : 0);
         bytes = at;
     }
 };
@@ -1329,7 +1335,7 @@ template <class DT, class S, bool BACK> int launch_logits_of(const na1d_head &h,
 }
 template <class DT, bool BACK> int launch_logits(const na1d_head &h, const Tiling &t, Logits a, hipStream_t s) {
     a.m_tiles = (int)ceil_div<int64_t>(BACK ? round_up(a.classes, kStep) : a.classes, t.bm);           // dz: to the end of its last step
-    a.n_tiles = (int)ceil_div<int64_t>(h.N, t.bn);
+    a.n_tiles = ceil_div(a.h.N, t.bn);
     switch (t.pick) {
         case kFew: return launch_logits_of<DT, Few, BACK>(h, t, a, s);
         case kBatch: return launch_logits_of<DT, Batch, BACK>(h, t, a, s);
@@ -1410,42 +1416,58 @@ int backward(const na1d_head &h, char *dx, char *dw, const float *dloss, const v
     } else {
         up.count = reinterpret_cast<const float *>(saved + o.count), up.most = up.count + 1;
     }
-    a.up = up, a.stats = stats, a.dz = ws + b.dz, a.plane = p.plane;
-    a.col_part = cosines && dw && p.dw_splits == 1 ? reinterpret_cast<float *>(ws + b.cols) : nullptr;
+    a.up = up, a.dz = ws + b.dz, a.plane = p.plane;
+    a.col_part = cosines && dw && p.dw_at_once() ? reinterpret_cast<float *>(ws + b.cols) : nullptr;
     Product g{};
-    g.dz = a.dz, g.plane = p.plane, g.N = (int)h.N, g.D = (int)h.D, g.subs = h.subcenters, g.up = up;
+    g.dz = a.dz, g.plane = p.plane, g.D = (int)h.D, g.subs = h.subcenters, g.up = up;
+    // (Of at most 2^20 rows, those of dx or of a range's weight: a launch has less than 2^32 threads.)
+    auto fold = [&](char *out, int64_t part, int64_t stride, int64_t rows, int splits, const char *own, int64_t own_pitch, const float *inv) {
+        const Fold f{out, reinterpret_cast<const float *>(ws + part), stride, rows, splits, (int)h.D, up, cosines ? own : nullptr, own_pitch, inv};
+        if (splits >= 32 && rows <= 512) return launch<fold_kernel<DT, 16>>((unsigned)rows, 1024, 0, s, f);
+        return splits >= 8 ? launch<fold_kernel<DT, 4>>((unsigned)rows, 256, 0, s, f) : launch<fold_kernel<DT, 1>>((unsigned)ceil_div<int64_t>(rows, 4), 256, 0, s, f);
+    };
+    const int64_t dw_stride = p.plane * h.subcenters * h.D;
     for (int64_t range = 0; range < p.ranges; ++range) {
         a.class0 = g.class0 = (int)(range * p.plane);
         a.classes = g.classes = (int)std::min(p.plane, h.V - a.class0);
         g.columns = (int)round_up(a.classes, kStep);
-        NA1D_TRY((launch_logits<DT, true>(h, p.back, a, s)));
-        if (h.kind == NA1D_HEAD_TEACHER) {
-            entries_kernel<DT><<<(unsigned)ceil_div<int64_t>(h.N * h.top, 256), 256, 0, s>>>((uint16_t *)a.dz, reinterpret_cast<const float *>(saved + o.coeff), stats,
-                                                                                             up, ids, h.ids_64, (int)h.N, h.top, a.class0, a.classes, p.plane);
-            NA1D_TRY(launch_status());
+        const int64_t w0 = (int64_t)a.class0 * h.subcenters;                                  // first weight row
+        for (int64_t batch = 0; batch < p.batches; ++batch) {
+            const int64_t r0 = batch * p.rows;
+            const Head whole = a.h;
+            a.h.N = g.N = (int)std::min(p.rows, h.N - r0);
+            a.h.x += r0 * a.h.x_pitch;
+            if (cosines) a.h.inv_x += r0;
+            a.stats = stats + r0;
+            a.up = up;
+            if (!up.count) a.up.dloss += r0;                                                  // of every row
+            NA1D_TRY((launch_logits<DT, true>(h, p.back, a, s)));
+            if (h.kind == NA1D_HEAD_TEACHER) {
+                entries_kernel<DT><<<(unsigned)ceil_div<int64_t>((int64_t)g.N * h.top, 256), 256, 0, s>>>(
+                    (uint16_t *)a.dz, reinterpret_cast<const float *>(saved + o.coeff) + r0 * h.top, a.stats, a.up,
+                    (const char *)ids + r0 * h.top * (h.ids_64 ? 8 : 4), h.ids_64, g.N, h.top, a.class0, a.classes, p.plane);
+                NA1D_TRY(launch_status());
+            }
+            Product gx = g, gw = g;                                                           // what is not asked for has no workgroups
+            if (dx) {
+                gx.other = a.h.w, gx.other_pitch = a.h.w_pitch;
+                gx.m_tiles = (int)ceil_div<int64_t>(h.D, p.dx.bm), gx.n_tiles = (int)ceil_div<int64_t>(g.N, p.dx.bn), gx.splits = p.dx_splits, gx.per = p.dx_per;
+                gx.part = reinterpret_cast<float *>(ws + b.dx) + r0 * h.D, gx.part_stride = h.N * h.D, gx.add = range > 0;
+            }
+            if (dw) {
+                gw.other = a.h.x, gw.other_pitch = a.h.x_pitch;
+                gw.m_tiles = (int)ceil_div<int64_t>(h.D, p.dw.bm), gw.n_tiles = (int)(h.subcenters * ceil_div(g.columns, p.dw.bn)), gw.splits = p.dw_splits, gw.per = p.dw_per;
+                gw.part = reinterpret_cast<float *>(ws + b.dw), gw.part_stride = dw_stride, gw.add = batch > 0, gw.out = p.dw_at_once() ? dw : nullptr;
+                gw.w = cosines ? a.h.w : nullptr, gw.w_pitch = a.h.w_pitch, gw.inv_w = a.h.inv_w, gw.col_part = a.col_part, gw.col_parts = (int)ceil_div<int64_t>(h.N, p.back.bn) * p.back.wn;
+            }
+            NA1D_TRY(launch_products<DT>(p, gx, gw, s));
+            a.h = whole;
         }
-        Product gx = g, gw = g;                                                               // what is not asked for has no workgroups
-        if (dx) {
-            gx.other = a.h.w, gx.other_pitch = a.h.w_pitch;
-            gx.m_tiles = (int)ceil_div<int64_t>(h.D, p.dx.bm), gx.n_tiles = (int)ceil_div<int64_t>(h.N, p.dx.bn), gx.splits = p.dx_splits, gx.per = p.dx_per;
-            gx.part = reinterpret_cast<float *>(ws + b.dx), gx.part_stride = h.N * h.D, gx.add = range > 0;
-        }
-        if (dw) {
-            gw.other = a.h.x, gw.other_pitch = a.h.x_pitch;
-            gw.m_tiles = (int)ceil_div<int64_t>(h.D, p.dw.bm), gw.n_tiles = (int)(h.subcenters * ceil_div(g.columns, p.dw.bn)), gw.splits = p.dw_splits, gw.per = p.dw_per;
-            gw.part = reinterpret_cast<float *>(ws + b.dw), gw.part_stride = h.V * h.subcenters * h.D, gw.out = p.dw_splits == 1 ? dw : nullptr;
-            gw.w = cosines ? a.h.w : nullptr, gw.w_pitch = a.h.w_pitch, gw.inv_w = a.h.inv_w, gw.col_part = a.col_part, gw.col_parts = (int)ceil_div<int64_t>(h.N, p.back.bn) * p.back.wn;
-        }
-        NA1D_TRY(launch_products<DT>(p, gx, gw, s));
+        if (dw && !p.dw_at_once())
+            NA1D_TRY(fold(dw + 2 * w0 * h.D, b.dw, dw_stride, a.classes * (int64_t)h.subcenters, p.dw_splits, a.h.w + w0 * a.h.w_pitch, a.h.w_pitch,
+                          cosines ? a.h.inv_w + w0 : nullptr));
     }
-    // (A launch has less than 2^32 threads.)
-    auto fold = [&](char *out, int64_t part, int64_t rows, int splits, const char *own, int64_t own_pitch, const float *inv) {
-        const Fold f{out, reinterpret_cast<const float *>(ws + part), rows * h.D, rows, splits, (int)h.D, up, cosines ? own : nullptr, own_pitch, inv};
-        if (splits >= 32 && rows <= 512) return launch<fold_kernel<DT, 16>>((unsigned)rows, 1024, 0, s, f);
-        return splits >= 8 && rows < 1 << 24 ? launch<fold_kernel<DT, 4>>((unsigned)rows, 256, 0, s, f) : launch<fold_kernel<DT, 1>>((unsigned)ceil_div<int64_t>(rows, 4), 256, 0, s, f);
-    };
-    if (dx) NA1D_TRY(fold(dx, b.dx, h.N, p.dx_splits, a.h.x, a.h.x_pitch, a.h.inv_x));
-    if (dw && p.dw_splits > 1) NA1D_TRY(fold(dw, b.dw, h.V * h.subcenters, p.dw_splits, a.h.w, a.h.w_pitch, a.h.inv_w));
+    if (dx) NA1D_TRY(fold(dx, b.dx, h.N * h.D, h.N, p.dx_splits, a.h.x, a.h.x_pitch, a.h.inv_x));
     return NA1D_OK;
 }
 

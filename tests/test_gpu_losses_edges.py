@@ -152,3 +152,40 @@ def test_the_largest_weight_that_many_rows_share():
     assert ((loss[some] - few).abs() <= 2.0 ** -17 * (few.abs() + 32 * 8)).all()
     assert ((dx[some].double() - dx_few.double()).norm(dim=1) <= 4 * 2.0 ** -8 * dx_few.double().norm(dim=1)).all()
     assert (dw.double() - dw_few.double()).norm() <= 4 * 2.0 ** -8 * dw_few.double().norm()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16], ids=["bf16", "fp16"])
+def test_rows_that_the_backward_takes_in_batches(dtype, monkeypatch):
+    """More than 2^19 rows, or rows times weight rows of a class, are worked on some at a time: the whole against 64 bits.
+
+    In fp16 a class has up to some 1500 rows whose upstream gradients are 16 each: with 1 - P up to 1 and |x| beyond 3, elements of its
+    gradient pass 65504, fp16's largest, and have to be infinite (or, within the bound of that, may be)."""
+    import test_gpu_losses as T
+    near = T._near
+
+    def near_or_beyond(name, got, want, bound):
+        beyond = got.isinf() & (got.sign() == want.sign()) & (want.abs() + bound > torch.finfo(got.dtype).max)
+        near(name, torch.where(beyond, want.to(torch.float64), got.double()), want, bound)
+
+    monkeypatch.setattr(T, "_near", near_or_beyond)
+    T.test_cross_entropy((530_001, 8, 300), dtype)
+    T._distillation((530_001, 8, 300), 3, dtype)
+    for size, subs in (((600_000, 8, 300), 1), ((270_001, 16, 300), 2), ((3000, 16, 300), 200)):
+        T._margin(size, subs, dtype)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_weights_whose_gradient_is_summed_in_parts_range_by_range(kind):
+    """So many rows that a range has few classes, and its weight rows' gradients are sums of many parts: against 64 bits in the norm, by
+    what rounding once leaves (half a step of dz in every term, and of the sum at the end)."""
+    x, w, target, ids, logits = _inputs(N=70_000, D=64, V=9_000)
+    call = _calls(target, ids, logits)[kind]
+    _, dx, dw = _both(call, x, w)
+    if kind == "margin":
+        rows, ok, e, _ = O.margin(x, w.view(3000, 3, 64), target // 3)
+        want = O.margin_gradients(x, w, e, O.shares(ok, "mean", 1.0))[:2]
+    else:
+        rows, ok, e = O.softmax_targets(x, w, target) if kind == "ce" else O.teacher(x, w, logits, ids, 2.0)
+        want = O.linear_gradients(x, w, e, O.shares(ok, "mean", 1.0))[:2]
+    for got, exact in zip((dx, dw), want):
+        assert (got.double() - exact).norm() <= 2 * 2.0 ** -8 * exact.norm()

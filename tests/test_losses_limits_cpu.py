@@ -1,0 +1,44 @@
+"""What the losses over many classes ask for and refuse at the ends of their range, without a GPU."""
+import ctypes
+import random
+
+import pytest
+import torch
+
+from na1d_amd import _lib, losses, ops
+
+
+def _head(**kw):
+    h = losses._Head(dtype=0, kind=0, reduction=1, subcenters=1, top=0, teacher_type=0, ids_64=1, scale=1.0, margin=0.0,
+                     ignore_index=-100, N=4, V=100, D=64, x_stride=64, w_stride=64)
+    for k, v in kw.items():
+        setattr(h, k, v)
+    h.x_stride = h.w_stride = h.D
+    return h
+
+
+def _most(N, D, K):
+    """512 MB, dx in fp32, and 256 classes' weight rows in fp32 where rows come in batches."""
+    return (1 << 29) + 4 * N * D + (1024 * K * D if N * K > 1 << 19 else 0)
+
+
+@pytest.mark.parametrize("N,V,K,D", [
+    (65536, 131072, 1, 1024), (131072, 262144, 1, 512), (262144, 262144, 1, 512), (65536, 128256, 1, 4096), (131072, 128256, 1, 4096), (131072, 65536, 1, 1024),
+    (1 << 14, 1 << 22, 4, 8), (1 << 15, 1 << 21, 8, 8), (1 << 16, 1 << 20, 16, 8), (1 << 20, 1 << 16, 1, 8), (1 << 20, 65536, 200, 64), (1 << 20, 65536, 255, 64),
+    (1 << 20, 65793, 255, 4112)])
+def test_a_backwards_workspace_does_not_grow_with_the_classes(N, V, K, D):
+    h = _head(N=N, V=min(V, (1 << 36) // N), subcenters=K, kind=int(K > 1), D=D)
+    nbytes = _lib.load().na1d_head_workspace_bytes(ctypes.byref(h), 1)
+    assert 0 < nbytes <= _most(N, D, K)
+
+
+def test_a_backwards_workspace_of_any_size():
+    rng, lib, taken = random.Random(0), _lib.load(), 0
+    for _ in range(400):
+        kind = rng.randrange(3)
+        K = int(2 ** rng.uniform(0, 8)) if kind == 1 else 1
+        N, V, D = int(2 ** rng.uniform(0, 20)), int(2 ** rng.uniform(0, 24)), 8 * int(2 ** rng.uniform(0, 10))
+        nbytes = lib.na1d_head_workspace_bytes(ctypes.byref(_head(kind=kind, N=N, V=V, D=D, subcenters=K, top=9, dtype=rng.randrange(2))), 1)
+        assert nbytes == _lib.UNSUPPORTED or 0 < nbytes <= _most(N, D, K), (kind, N, V, D, K)
+        taken += nbytes > 0
+    assert taken > 200
