@@ -962,7 +962,7 @@ struct Product {
     int N, D, subs;
     int classes, columns, class0;   // of this range; its columns of dz, whole steps
     int m_tiles, n_tiles, splits, per;          // per: of the contraction to a split, a multiple of kStep
-    float *part;                    // fp32 [splits, rows, D]; dW: the range's rows
+    float *part;                    // fp32 [splits, rows, D]; dW: rows from the range's first on
     int64_t part_stride;
     int add;                        // to what is there
     Upstream up;
@@ -1189,10 +1189,14 @@ struct Plan {
     // backward: ranges of classes, and within each, batches of rows
     int64_t plane;                            // columns to a sub-centre: a range's classes, rounded up to whole steps
     int64_t ranges, rows, batches;
-    bool dw_at_once() const { return dw_splits == 1 && batches == 1; }        // else in parts, which are put together behind each range
+    bool dw_at_once() const { return dw_splits == 1 && batches == 1; }        // else in parts
+    int64_t together;                         // ranges whose parts are put together at once
     Tiling dx, dw;
     int dx_splits, dx_per, dw_splits, dw_per;
 };
+// Bytes of dW's parts that are kept for a launch that puts them together (behind each range by itself: backwards of 16384 x 32768 of 256 channels
+// 1192 -> 1222 us, 40000 x 30000 of 128 2015 -> 2080).
+constexpr int64_t kMostParts = 128ll << 20;
 constexpr int64_t kMostDz = 256ll << 20;      // bytes of dz: what the last level of cache holds (64 MB: +10 to 25 %, 1 GB: 0 to +2 %)
 
 // How long a launch of `first` workgroups of `first_steps` and then `second` of `second_steps` takes, in us: CUs hold one workgroup
@@ -1252,9 +1256,10 @@ inline Plan plan_of(const na1d_head &h) {
     p.ranges = ceil_div(h.V, p.plane);
     p.plane = std::min(round_up(h.V, kStep), round_up(ceil_div(h.V, p.ranges), 256));         // ranges alike
     p.ranges = ceil_div(h.V, p.plane);
-    // More than 2^19 rows (times sub-centres) do not fit with 256 classes, and with fewer dx would be read and written in fp32 all the more often: such
-    // rows are taken in batches, alike too.
-    p.batches = ceil_div<int64_t>(2 * h.N * h.subcenters * p.plane, kMostDz);
+    // More than 2^19 rows (times sub-centres) do not fit with 256 classes, and with fewer dx would be read and written in fp32 all the more often. What
+    // takes more than four times the room, as only margins' can, goes in batches of rows, alike too: dW's sums are then read and written for each
+    // (10^6 x 10000 of 128 channels, 512 MB: 29.2 ms, in two batches 30.4; 40000 x 2000 of 40 rows and 64 channels, 820 MB: 6.8 and 7.9).
+    p.batches = ceil_div<int64_t>(2 * h.N * h.subcenters * p.plane, 4 * kMostDz);
     p.rows = p.batches > 1 ? round_up(ceil_div(h.N, p.batches), 256) : h.N;
     p.batches = ceil_div(h.N, p.rows);
     // Products: the tiles and splits (of 4, 8 or 16 steps at least) that take least, with what the sums of splits cost in memory at 4 TB/s and in
@@ -1276,6 +1281,7 @@ inline Plan plan_of(const na1d_head &h) {
         const double t = fold + 0.05 * q.dx_splits + time_of(pick, dx_tiles * q.dx_splits, (int64_t)h.subcenters * q.dx_per / kStep, dw_tiles * q.dw_splits, q.dw_per / kStep, 2.);          // whose ends store more
         if (t < least && (h.N > 32 || pick <= kMany)) p = q, least = t;
     }
+    p.together = std::max<int64_t>(1, std::min(p.ranges, kMostParts / (4 * p.plane * h.subcenters * h.D * p.dw_splits)));
     return p;
 }
 struct ForwardScratch {
@@ -1295,7 +1301,7 @@ struct BackwardScratch {
         most = take(16);
         dz = take(2 * p.rows * h.subcenters * p.plane);
         dx = take(4 * h.N * h.D * p.dx_splits);
-        dw = take(p.dw_at_once() ? 0 : 4 * p.plane * h.subcenters * h.D * p.dw_splits);
+        dw = take(p.dw_at_once() ? 0 : 4 * p.together * p.plane * h.subcenters * h.D * p.dw_splits);
         cols = take(h.kind == NA1D_HEAD_MARGIN && p.dw_at_once() ? 4 * ceil_div<int64_t>(h.N, p.back.bn) * p.back.wn * h.subcenters * p.plane : 0);
         bytes = at;
     }
@@ -1420,32 +1426,31 @@ int backward(const na1d_head &h, char *dx, char *dw, const float *dloss, const v
     a.col_part = cosines && dw && p.dw_at_once() ? reinterpret_cast<float *>(ws + b.cols) : nullptr;
     Product g{};
     g.dz = a.dz, g.plane = p.plane, g.D = (int)h.D, g.subs = h.subcenters, g.up = up;
-    // (Of at most 2^20 rows, those of dx or of a range's weight: a launch has less than 2^32 threads.)
+    // (Of at most 2^22 rows, those of dx or of kMostParts: a launch has less than 2^32 threads.)
     auto fold = [&](char *out, int64_t part, int64_t stride, int64_t rows, int splits, const char *own, int64_t own_pitch, const float *inv) {
         const Fold f{out, reinterpret_cast<const float *>(ws + part), stride, rows, splits, (int)h.D, up, cosines ? own : nullptr, own_pitch, inv};
         if (splits >= 32 && rows <= 512) return launch<fold_kernel<DT, 16>>((unsigned)rows, 1024, 0, s, f);
         return splits >= 8 ? launch<fold_kernel<DT, 4>>((unsigned)rows, 256, 0, s, f) : launch<fold_kernel<DT, 1>>((unsigned)ceil_div<int64_t>(rows, 4), 256, 0, s, f);
     };
-    const int64_t dw_stride = p.plane * h.subcenters * h.D;
+    const int64_t dw_stride = p.together * p.plane * h.subcenters * h.D;
     for (int64_t range = 0; range < p.ranges; ++range) {
         a.class0 = g.class0 = (int)(range * p.plane);
         a.classes = g.classes = (int)std::min(p.plane, h.V - a.class0);
         g.columns = (int)round_up(a.classes, kStep);
-        const int64_t w0 = (int64_t)a.class0 * h.subcenters;                                  // first weight row
+        const int64_t first = range / p.together * p.together * p.plane;                      // class of the parts
         for (int64_t batch = 0; batch < p.batches; ++batch) {
             const int64_t r0 = batch * p.rows;
             const Head whole = a.h;
             a.h.N = g.N = (int)std::min(p.rows, h.N - r0);
             a.h.x += r0 * a.h.x_pitch;
-            if (cosines) a.h.inv_x += r0;
+            if (cosines) a.h.inv_x += r0;                                                     // (no others come in batches)
             a.stats = stats + r0;
             a.up = up;
             if (!up.count) a.up.dloss += r0;                                                  // of every row
             NA1D_TRY((launch_logits<DT, true>(h, p.back, a, s)));
             if (h.kind == NA1D_HEAD_TEACHER) {
-                entries_kernel<DT><<<(unsigned)ceil_div<int64_t>((int64_t)g.N * h.top, 256), 256, 0, s>>>(
-                    (uint16_t *)a.dz, reinterpret_cast<const float *>(saved + o.coeff) + r0 * h.top, a.stats, a.up,
-                    (const char *)ids + r0 * h.top * (h.ids_64 ? 8 : 4), h.ids_64, g.N, h.top, a.class0, a.classes, p.plane);
+                entries_kernel<DT><<<(unsigned)ceil_div<int64_t>(h.N * h.top, 256), 256, 0, s>>>((uint16_t *)a.dz, reinterpret_cast<const float *>(saved + o.coeff), stats,
+                                                                                                 up, ids, h.ids_64, (int)h.N, h.top, a.class0, a.classes, p.plane);
                 NA1D_TRY(launch_status());
             }
             Product gx = g, gw = g;                                                           // what is not asked for has no workgroups
@@ -1457,15 +1462,16 @@ int backward(const na1d_head &h, char *dx, char *dw, const float *dloss, const v
             if (dw) {
                 gw.other = a.h.x, gw.other_pitch = a.h.x_pitch;
                 gw.m_tiles = (int)ceil_div<int64_t>(h.D, p.dw.bm), gw.n_tiles = (int)(h.subcenters * ceil_div(g.columns, p.dw.bn)), gw.splits = p.dw_splits, gw.per = p.dw_per;
-                gw.part = reinterpret_cast<float *>(ws + b.dw), gw.part_stride = dw_stride, gw.add = batch > 0, gw.out = p.dw_at_once() ? dw : nullptr;
+                gw.part = reinterpret_cast<float *>(ws + b.dw) + (a.class0 - first) * h.subcenters * h.D, gw.part_stride = dw_stride, gw.add = batch > 0, gw.out = p.dw_at_once() ? dw : nullptr;
                 gw.w = cosines ? a.h.w : nullptr, gw.w_pitch = a.h.w_pitch, gw.inv_w = a.h.inv_w, gw.col_part = a.col_part, gw.col_parts = (int)ceil_div<int64_t>(h.N, p.back.bn) * p.back.wn;
             }
             NA1D_TRY(launch_products<DT>(p, gx, gw, s));
             a.h = whole;
         }
-        if (dw && !p.dw_at_once())
-            NA1D_TRY(fold(dw + 2 * w0 * h.D, b.dw, dw_stride, a.classes * (int64_t)h.subcenters, p.dw_splits, a.h.w + w0 * a.h.w_pitch, a.h.w_pitch,
-                          cosines ? a.h.inv_w + w0 : nullptr));
+        if (dw && !p.dw_at_once() && ((range + 1) % p.together == 0 || range + 1 == p.ranges)) {
+            const int64_t w0 = first * h.subcenters, rows = (a.class0 + a.classes - first) * h.subcenters;
+            NA1D_TRY(fold(dw + 2 * w0 * h.D, b.dw, dw_stride, rows, p.dw_splits, a.h.w + w0 * a.h.w_pitch, a.h.w_pitch, cosines ? a.h.inv_w + w0 : nullptr));
+        }
     }
     if (dx) NA1D_TRY(fold(dx, b.dx, h.N * h.D, h.N, p.dx_splits, a.h.x, a.h.x_pitch, a.h.inv_x));
     return NA1D_OK;

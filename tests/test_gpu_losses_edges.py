@@ -156,7 +156,8 @@ def test_the_largest_weight_that_many_rows_share():
 
 @pytest.mark.parametrize("dtype", [BF16, FP16], ids=["bf16", "fp16"])
 def test_rows_that_the_backward_takes_in_batches(dtype, monkeypatch):
-    """More than 2^19 rows, or rows times weight rows of a class, are worked on some at a time: the whole against 64 bits.
+    """More than 2^19 rows have ranges of few classes, and more than 2^21 times weight rows of a class are worked on some at a time:
+    the whole against 64 bits.
 
     In fp16 a class has up to some 1500 rows whose upstream gradients are 16 each: with 1 - P up to 1 and |x| beyond 3, elements of its
     gradient pass 65504, fp16's largest, and have to be infinite (or, within the bound of that, may be)."""
@@ -170,7 +171,7 @@ def test_rows_that_the_backward_takes_in_batches(dtype, monkeypatch):
     monkeypatch.setattr(T, "_near", near_or_beyond)
     T.test_cross_entropy((530_001, 8, 300), dtype)
     T._distillation((530_001, 8, 300), 3, dtype)
-    for size, subs in (((600_000, 8, 300), 1), ((270_001, 16, 300), 2), ((3000, 16, 300), 200)):
+    for size, subs in (((600_000, 8, 300), 1), ((270_001, 16, 300), 2), ((3000, 16, 300), 200), ((11_001, 16, 300), 200)):
         T._margin(size, subs, dtype)
 
 

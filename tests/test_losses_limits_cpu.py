@@ -18,8 +18,8 @@ def _head(**kw):
 
 
 def _most(N, D, K):
-    """512 MB, dx in fp32, and 256 classes' weight rows in fp32 where rows come in batches."""
-    return (1 << 29) + 4 * N * D + (1024 * K * D if N * K > 1 << 19 else 0)
+    """512 MB, or 1.25 GB from 2^19 rows (times sub-centres) on, dx in fp32, and 256 classes' weight rows in fp32 where rows come in batches."""
+    return (5 << 28 if N * K > 1 << 19 else 1 << 29) + 4 * N * D + (1024 * K * D if N * K > 1 << 21 else 0)
 
 
 @pytest.mark.parametrize("N,V,K,D", [
