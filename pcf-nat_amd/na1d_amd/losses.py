@@ -15,7 +15,6 @@ from __future__ import annotations
 import ctypes
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -98,6 +97,16 @@ def head_backward(dloss, x, weight, ids, teacher, saved, kind, scale, margin, ig
     return dx, dw
 
 
+_AGAIN = "the gradients of na1d_amd's losses cannot be differentiated again"
+
+
+def _final(grad):
+    """A gradient that has none of its own: whoever asks for one is told, also where it is a part of a larger sum."""
+    if grad is None or not torch.is_grad_enabled():
+        return grad
+    return torch._C._functions.DelayedError(_AGAIN.encode(), 1)(grad.requires_grad_(True))
+
+
 class _HeadLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, ids, teacher, hits, *args):
@@ -107,12 +116,12 @@ class _HeadLoss(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dloss):
         x, weight, ids, teacher, saved = ctx.saved_tensors
         want = ctx.needs_input_grad[:2]
-        dx, dw = head_backward(dloss, x, weight, ids, teacher, saved, *ctx.args, *want)
-        return (dx if want[0] else None, dw if want[1] else None) + (None,) * 8
+        with torch.no_grad():
+            dx, dw = head_backward(dloss, x, weight, ids, teacher, saved, *ctx.args, *want)
+        return (_final(dx if want[0] else None), _final(dw if want[1] else None)) + (None,) * 8
 
 
 def _loss(x, weight, ids, teacher, return_hits, *args):

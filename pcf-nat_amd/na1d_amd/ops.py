@@ -334,7 +334,12 @@ def _class_loss_autograd(ctx, dloss, _dsaved):
     return (dx if want[0] else None, dw if want[1] else None) + (None,) * 7
 
 
+def _class_loss_again(ctx, *_grads):
+    raise RuntimeError(losses._AGAIN)
+
+
 torch.library.register_autograd(NAMESPACE + "::class_loss_forward", _class_loss_autograd, setup_context=_class_loss_setup, lib=_library)
+torch.library.register_autograd(NAMESPACE + "::class_loss_backward", _class_loss_again, lib=_library)
 
 
 def _class_loss(x, weight, ids, teacher, *args):

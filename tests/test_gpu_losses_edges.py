@@ -190,3 +190,24 @@ def test_weights_whose_gradient_is_summed_in_parts_range_by_range(kind):
         want = O.linear_gradients(x, w, e, O.shares(ok, "mean", 1.0))[:2]
     for got, exact in zip((dx, dw), want):
         assert (got.double() - exact).norm() <= 2 * 2.0 ** -8 * exact.norm()
+
+
+@pytest.mark.parametrize("way", ["native node", "Python node", "op"])
+@pytest.mark.parametrize("kind", KINDS)
+def test_a_penalty_on_a_gradient_is_refused(kind, way):
+    """The gradients are the same with create_graph, and a loss that holds them is not differentiated without them."""
+    x, w, target, ids, logits = _inputs()
+    call = _calls(target, ids, logits)[kind]
+    if way == "op":
+        call = {"ce": lambda x, w: ops.linear_cross_entropy_op(x, w, target), "margin": lambda x, w: ops.margin_cross_entropy_op(x, w.unflatten(0, (-1, 3)), target // 3),
+                "distil": lambda x, w: ops.linear_distillation_op(x, w, logits, ids, 2.0)}[kind]
+    lay = (lambda t: t.t().contiguous().t()) if way == "Python node" else (lambda t: t.clone())
+    want = _both(call, x, w)[1:]
+    for both in (True, False):
+        a, b = lay(x).requires_grad_(True), lay(w).requires_grad_(both)
+        leaves = [a, b] if both else [a]
+        loss = call(a, b)
+        grads = torch.autograd.grad(loss, leaves, create_graph=True)
+        assert _same(grads, want[:len(grads)])
+        with pytest.raises(RuntimeError, match="differentiated again"):
+            (loss + grads[0].float().square().sum()).backward()

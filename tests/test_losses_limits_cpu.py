@@ -42,3 +42,21 @@ def test_a_backwards_workspace_of_any_size():
         assert nbytes == _lib.UNSUPPORTED or 0 < nbytes <= _most(N, D, K), (kind, N, V, D, K)
         taken += nbytes > 0
     assert taken > 200
+
+
+def _on_meta(N=5, D=16, V=30, dtype=torch.bfloat16):
+    return (torch.empty(N, D, dtype=dtype, device="meta"), torch.empty(V, D, dtype=dtype, device="meta"), torch.empty(N, dtype=torch.int64, device="meta"))
+
+
+def test_a_second_derivative_of_the_op_is_refused():
+    """Also where a gradient is a part of a larger loss, which would be differentiated without it."""
+    x, w, target = _on_meta()
+    x.requires_grad_(True), w.requires_grad_(True)
+    for wanted in ([x], [w], [x, w]):
+        loss, _ = torch.ops.na_cuda.class_loss_forward(x, w, target, None, 0, 1.0, 0.0, -100, 1)
+        grads = torch.autograd.grad(loss, wanted, torch.empty((), device="meta"), create_graph=True)
+        penalty = sum(g.float().square().sum() for g in grads)
+        with pytest.raises(RuntimeError, match="differentiated again"):
+            torch.autograd.grad(loss + penalty, wanted, torch.empty((), device="meta"))
+        loss, _ = torch.ops.na_cuda.class_loss_forward(x, w, target, None, 0, 1.0, 0.0, -100, 1)
+        assert [g.shape for g in torch.autograd.grad(loss, wanted, torch.empty((), device="meta"))] == [t.shape for t in wanted]
