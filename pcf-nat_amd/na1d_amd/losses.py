@@ -133,10 +133,8 @@ def _loss(x, weight, ids, teacher, return_hits, *args):
     return (out, hits) if return_hits else out
 
 
-def check_arguments(x, weight, ids, reduction, ids_shape, weight_dims=(2,), what="target"):
-    """What the losses ask of their arguments; the sizes' limits are the native call's."""
-    if reduction not in _REDUCTIONS:
-        raise ValueError("reduction must be one of %s, got %r" % (", ".join(_REDUCTIONS), reduction))
+def check_operands(x, weight, ids, ids_shape, weight_dims=(2,), what="target"):
+    """What the losses and the registered ops ask of their tensors; the sizes' limits are the native call's."""
     if x.dim() < 1 or weight.dim() not in weight_dims or x.shape[-1] != weight.shape[-1]:
         raise ValueError("x must be [..., D] and weight %s, got %s and %s" % (
             " or ".join("[V, K, D]" if d == 3 else "[V, D]" for d in weight_dims), list(x.shape), list(weight.shape)))
@@ -149,22 +147,32 @@ def check_arguments(x, weight, ids, reduction, ids_shape, weight_dims=(2,), what
         raise TypeError("x and weight must have one dtype, got %s and %s" % (x.dtype, weight.dtype))
     if x.device != weight.device or x.device != ids.device:
         raise _lib.NA1DError("x, weight and %s must be on one device" % what)
-    if x.device.type != "cuda":
-        raise _lib.NA1DError("NA1D tensors must live on the GPU (got device %s); there is no CPU path" % x.device)
     if x.shape[-1] % 8 or x.shape[-1] == 0:
         raise _lib.NA1DError("the last dimension must be a positive multiple of 8, got %d" % x.shape[-1])
     if weight.numel() == 0:
         raise _lib.NA1DError("weight must have at least one class")
 
 
-def check_teacher(x, weight, teacher_logits, teacher_ids, reduction):
+def check_arguments(x, weight, ids, reduction, ids_shape, weight_dims=(2,), what="target"):
+    if reduction not in _REDUCTIONS:
+        raise ValueError("reduction must be one of %s, got %r" % (", ".join(_REDUCTIONS), reduction))
+    check_operands(x, weight, ids, ids_shape, weight_dims, what)
+    if x.device.type != "cuda":
+        raise _lib.NA1DError("NA1D tensors must live on the GPU (got device %s); there is no CPU path" % x.device)
+
+
+def check_entries(x, teacher_logits, teacher_ids):
     if teacher_logits.shape != teacher_ids.shape or teacher_logits.dim() < 1 or not 0 < teacher_logits.shape[-1] <= MAX_TOP:
         raise ValueError("teacher_logits must be like teacher_ids, with 1 to %d entries to a row; got %s" % (MAX_TOP, list(teacher_logits.shape)))
     if teacher_logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
         raise TypeError("teacher_logits must be float32, bfloat16 or float16, got %s" % teacher_logits.dtype)
-    check_arguments(x, weight, teacher_ids, reduction, x.shape[:-1] + teacher_logits.shape[-1:], what="teacher_ids")
     if teacher_logits.device != x.device:
         raise _lib.NA1DError("x and teacher_logits must be on one device")
+
+
+def check_teacher(x, weight, teacher_logits, teacher_ids, reduction):
+    check_entries(x, teacher_logits, teacher_ids)
+    check_arguments(x, weight, teacher_ids, reduction, x.shape[:-1] + teacher_logits.shape[-1:], what="teacher_ids")
 
 
 def linear_cross_entropy(x, weight, target, scale=1.0, ignore_index=-100, reduction="mean", return_hits=False):

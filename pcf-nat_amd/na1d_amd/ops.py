@@ -299,24 +299,49 @@ _library.define("class_loss_backward(Tensor dloss, Tensor x, Tensor weight, Tens
                 "bool want_weight) -> (Tensor, Tensor)" % _HEAD)
 
 
+def _class_loss_contract(x, weight, ids, teacher, kind, reduction):
+    """Shared by the real and the fake kernels; returns the loss's shape."""
+    torch._check(kind in (losses._TARGETS, losses._MARGIN, losses._TEACHER) and reduction in losses._REDUCTIONS.values(), lambda: "unknown kind or reduction")
+    torch._check((teacher is not None) == (kind == losses._TEACHER), lambda: "a teacher's loss has a teacher, the others have none")
+    if teacher is not None:
+        losses.check_entries(x, teacher, ids)
+    losses.check_operands(x, weight, ids, x.shape[:-1] + (() if teacher is None else teacher.shape[-1:]), (2, 3) if kind == losses._MARGIN else (2,), "ids")
+    return x.shape[:-1] if reduction == losses._REDUCTIONS["none"] else ()
+
+
+def _class_loss_backward_contract(dloss, x, weight, ids, teacher, saved, kind, reduction):
+    shape = _class_loss_contract(x, weight, ids, teacher, kind, reduction)
+    torch._check(dloss.dtype == torch.float32 and dloss.shape == shape, lambda: "dloss must be fp32 and like the loss")
+    torch._check(saved.dtype == torch.uint8 and saved.dim() == 1 and saved.is_contiguous(), lambda: "saved must be a forward's second result")
+    torch._check(dloss.device == x.device and saved.device == x.device, lambda: "NA1D operands must be on one device")
+
+
 def _class_loss_forward(x, weight, ids, teacher, *args):
+    _class_loss_contract(x, weight, ids, teacher, args[0], args[-1])
     return losses.head_forward(x, weight, ids, teacher, None, *args)
 
 
+def _class_loss_backward(dloss, x, weight, ids, teacher, saved, *args):
+    _class_loss_backward_contract(dloss, x, weight, ids, teacher, saved, args[0], args[4])
+    return losses.head_backward(dloss, x, weight, ids, teacher, saved, *args)
+
+
 def _class_loss_forward_fake(x, weight, ids, teacher, kind, scale, margin, ignore_index, reduction):
-    loss = torch.empty(x.shape[:-1] if reduction == 0 else (), dtype=torch.float32, device=x.device)
+    shape = _class_loss_contract(x, weight, ids, teacher, kind, reduction)
+    loss = torch.empty(shape, dtype=torch.float32, device=x.device)
     h = losses._head(x, weight, ids, teacher, kind, scale, margin, ignore_index, reduction)
     h.x_stride = h.w_stride = h.D
     return loss, torch.empty(losses._sizes(h, 0)[0] if x.numel() else 0, dtype=torch.uint8, device=x.device)
 
 
 def _class_loss_backward_fake(dloss, x, weight, ids, teacher, saved, kind, scale, margin, ignore_index, reduction, want_x, want_weight):
+    _class_loss_backward_contract(dloss, x, weight, ids, teacher, saved, kind, reduction)
     return (torch.empty(x.shape if want_x else (0,), dtype=x.dtype, device=x.device),
             torch.empty(weight.shape if want_weight else (0,), dtype=weight.dtype, device=x.device))
 
 
 _library.impl("class_loss_forward", _class_loss_forward, "CUDA")
-_library.impl("class_loss_backward", losses.head_backward, "CUDA")
+_library.impl("class_loss_backward", _class_loss_backward, "CUDA")
 torch.library.register_fake(NAMESPACE + "::class_loss_forward", _class_loss_forward_fake, lib=_library)
 torch.library.register_fake(NAMESPACE + "::class_loss_backward", _class_loss_backward_fake, lib=_library)
 

@@ -211,3 +211,27 @@ def test_a_penalty_on_a_gradient_is_refused(kind, way):
         assert _same(grads, want[:len(grads)])
         with pytest.raises(RuntimeError, match="differentiated again"):
             (loss + grads[0].float().square().sum()).backward()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_the_ops_by_themselves(kind):
+    """As torch.ops has them: schema and fake kernels, the functions' results, and operands that do not fit refused before any kernel."""
+    x, w, target, ids, logits = _inputs()
+    number = KINDS.index(kind)
+    operands = (x, w.unflatten(0, (-1, 3)) if kind == "margin" else w, ids if kind == "distil" else target // 3 if kind == "margin" else target,
+                logits if kind == "distil" else None)
+    rest = (number, {"ce": 1.0, "margin": 32.0, "distil": 2.0}[kind], 0.2 if kind == "margin" else 0.0, -100)
+    f, b = torch.ops.na_cuda.class_loss_forward, torch.ops.na_cuda.class_loss_backward
+    tests = ("test_schema", "test_faketensor")
+    torch.library.opcheck(f.default, (*operands, *rest, 1), test_utils=tests)
+    want = _both(_calls(target, ids, logits)[kind], x, w)
+    loss, saved = f(*operands, *rest, 1)
+    one = torch.ones((), device="cuda")
+    torch.library.opcheck(b.default, (one, *operands, saved, *rest, 1, True, True), test_utils=tests)
+    dx, dw = b(one, *operands, saved, *rest, 1, True, True)
+    assert _same([loss, dx, dw.view_as(w)], want)
+    short = (x, operands[1], operands[2][:30], None if operands[3] is None else operands[3][:30])
+    for call in (lambda: f(*short, *rest, 1), lambda: b(one, *short, saved, *rest, 1, True, True), lambda: b(one.expand(33), *operands, saved, *rest, 1, True, True),
+                 lambda: b(one, *operands, saved[:64], *rest, 1, True, True), lambda: f(x, operands[1].cpu(), *operands[2:], *rest, 1)):
+        with pytest.raises((RuntimeError, ValueError)):
+            call()

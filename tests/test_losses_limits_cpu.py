@@ -60,3 +60,27 @@ def test_a_second_derivative_of_the_op_is_refused():
             torch.autograd.grad(loss + penalty, wanted, torch.empty((), device="meta"))
         loss, _ = torch.ops.na_cuda.class_loss_forward(x, w, target, None, 0, 1.0, 0.0, -100, 1)
         assert [g.shape for g in torch.autograd.grad(loss, wanted, torch.empty((), device="meta"))] == [t.shape for t in wanted]
+
+
+def test_arguments_that_the_ops_refuse():
+    """Called by themselves they check what the losses check: the kernels read as many rows and ids as x and the sizes say."""
+    x, w, target = _on_meta()
+    ids, logits = torch.empty(5, 3, dtype=torch.int64, device="meta"), torch.empty(5, 3, device="meta")
+    f, b = torch.ops.na_cuda.class_loss_forward, torch.ops.na_cuda.class_loss_backward
+    rest = (1.0, 0.0, -100)
+    loss, saved = f(x, w, target, None, 0, *rest, 0)
+    assert loss.shape == (5,) and saved.numel() > 0
+    mean, _ = f(x, w, ids, logits, 2, *rest, 1)
+    assert mean.shape == ()
+    for call in (lambda: f(x, w, target[:4], None, 0, *rest, 1), lambda: f(x, w, ids, None, 0, *rest, 1), lambda: f(x, w, target.float(), None, 0, *rest, 1),
+                 lambda: f(x, w[:, :8], target, None, 0, *rest, 1), lambda: f(x, w.half(), target, None, 0, *rest, 1), lambda: f(x.float(), w.float(), target, None, 0, *rest, 1),
+                 lambda: f(x, w.view(10, 3, 16), target, None, 0, *rest, 1), lambda: f(x, w, target, None, 3, *rest, 1), lambda: f(x, w, target, None, 0, *rest, 3),
+                 lambda: f(x, w, target, logits, 0, *rest, 1), lambda: f(x, w, target, None, 2, *rest, 1), lambda: f(x, w, ids[:4], logits[:4], 2, *rest, 1),
+                 lambda: f(x, w, ids, logits[:, :2], 2, *rest, 1), lambda: f(x, w, ids, logits.double(), 2, *rest, 1),
+                 lambda: f(x, w[:0], target, None, 0, *rest, 1),
+                 lambda: b(loss[:4], x, w, target, None, saved, 0, *rest, 0, True, True), lambda: b(loss, x, w, target, None, saved, 0, *rest, 1, True, True),
+                 lambda: b(loss.double(), x, w, target, None, saved, 0, *rest, 0, True, True), lambda: b(loss, x, w, target[:4], None, saved, 0, *rest, 0, True, True),
+                 lambda: b(loss, x, w, target, None, saved.float(), 0, *rest, 0, True, True), lambda: b(loss, x, w, target, None, saved[::2], 0, *rest, 0, True, True)):
+        with pytest.raises((RuntimeError, ValueError, TypeError)):
+            call()
+    assert [g.shape for g in b(loss, x, w, target, None, saved, 0, *rest, 0, True, False)] == [(5, 16), (0,)]
