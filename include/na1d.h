@@ -421,7 +421,7 @@ typedef struct na1d_head {
     int32_t subcenters;                 /* 1 except with a margin */
     int32_t top, teacher_type;          /* teacher only: entries of a row; NA1D_BF16, NA1D_FP16 or NA1D_FP32 */
     int32_t ids_64;                     /* targets and ids are int64, else int32 */
-    float scale, margin;                /* finite and above 0; 0 <= margin < pi / 2 */
+    float scale, margin;                /* finite and above 0, a temperature's square and 1.5 * scale too; 0 <= margin < pi / 2 */
     int64_t ignore_index;
     int64_t N, V, D, x_stride, w_stride;
 } na1d_head;

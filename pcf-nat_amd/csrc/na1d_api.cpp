@@ -575,7 +575,7 @@ static int head_check(const na1d_head *h) {
     if (h->D < 1 || h->D % 8) return NA1D_ERR_HEAD_DIM;
     if (h->x_stride < h->D || h->w_stride < h->D) return NA1D_ERR_SHAPE;
     if (h->x_stride % 8 || h->w_stride % 8) return NA1D_ERR_ALIGN;
-    if (bad_scale(h->scale) || (cosines && !(h->margin >= 0.f && h->margin < 1.5707963f))) return NA1D_ERR_SCALE;
+    if (bad_scale(h->scale) || bad_scale(teaches ? h->scale * h->scale : 1.5f * h->scale) || (cosines && !(h->margin >= 0.f && h->margin < 1.5707963f))) return NA1D_ERR_SCALE;
     const int64_t most = 1ll << 36, widest = 1ll << 20;
     if (h->subcenters > (cosines ? 255 : 1) || (teaches && h->top > NA1D_HEAD_MAX_TOP)) return NA1D_ERR_UNSUPPORTED;
     if (h->N > widest || h->V > (1ll << 24) / h->subcenters || h->x_stride > widest || h->w_stride > widest / h->subcenters) return NA1D_ERR_UNSUPPORTED;

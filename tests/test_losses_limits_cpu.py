@@ -84,3 +84,11 @@ def test_arguments_that_the_ops_refuse():
         with pytest.raises((RuntimeError, ValueError, TypeError)):
             call()
     assert [g.shape for g in b(loss, x, w, target, None, saved, 0, *rest, 0, True, False)] == [(5, 16), (0,)]
+
+
+@pytest.mark.parametrize("kind,scale,fine", [(0, 2.9e38, False), (1, 2.9e38, False), (0, 1.9e38, True), (2, 1e-23, False), (2, 2e19, False), (2, 1e-18, True), (2, 1e18, True)])
+def test_scales_that_fp32_cannot_work_with(kind, scale, fine):
+    """The kernels work with scale * log2(e), and with a temperature's reciprocal and square: each has to be a number."""
+    ref = ctypes.byref(_head(kind=kind, scale=scale, top=3))
+    for nbytes in (_lib.load().na1d_head_saved_bytes(ref), _lib.load().na1d_head_workspace_bytes(ref, 1)):
+        assert nbytes > 0 if fine else nbytes == -11
