@@ -389,7 +389,8 @@ int na1d_train_context_backward(void *dx, const void *dctx, const void *x, const
  *   kind NA1D_HEAD_TARGETS: z = scale * x . w, loss of a row: log sum exp z - z[target]
  *   kind NA1D_HEAD_MARGIN:  cos = max over a class's subcenters of x . w / (|x| |w|); z = scale * cos, at the target
  *          scale * cos(theta + margin) where cos > cos(pi - margin), else scale * (cos - margin * sin(pi - margin)).  The derivative
- *          of cos(theta + margin) takes the squared sine as 1e-6 at least; a row of zeros has cosine 0 and no gradient.
+ *          of cos(theta + margin) takes the squared sine as 1e-6 at least; a row of zeros (no
+ *          longer than 1e-12) has cosine 0 and no gradient, one whose squares' sum is beyond fp32 (1.8e19 and longer) makes losses NaN.
  *   kind NA1D_HEAD_TEACHER: z = x . w / temperature (`scale` is the temperature); q = softmax(teacher / temperature) over
  *          the row's `top` entries (ids [N, top], teacher [N, top]; ids below 0 are no entries, a class may be there
  *          twice); loss of a row: temperature^2 * sum of q (log q - log softmax(z)[id])

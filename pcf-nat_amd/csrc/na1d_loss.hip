@@ -297,8 +297,8 @@ __device__ inline int load_id(const void *ids, int64_t i, int wide) {
     const int64_t v = reinterpret_cast<const int64_t *>(ids)[i];
     return v < INT32_MIN || v > INT32_MAX ? (v < 0 ? INT32_MIN : INT32_MAX) : (int)v;
 }
-// A row of zeros has cosine 0 with everything and no gradient.  The factor of its (zero) products is a small number and not 0, so
-// that a masked logit of -inf stays one.
+// A row of zeros (no longer than kLeastNorm) has cosine 0 with everything and no gradient.  The factor of its products is a small
+// number and not 0, so that a masked logit of -inf stays one.  A row whose squares have no sum in fp32 has no cosine.
 constexpr float kLeastNorm = 1e-12f, kNoNorm = 1e-30f;
 
 constexpr int kNormBlocks = 1024;
@@ -334,7 +334,7 @@ norms_kernel(float *__restrict__ inv_a, float *__restrict__ inv_b, float *__rest
 #pragma unroll
         for (int i = 0; i < kAtOnce; ++i) {
             const int64_t r = r0 + i * step;
-            const float sum = sum_of_16(s[i]), inv = sum > kLeastNorm * kLeastNorm ? 1.f / __builtin_sqrtf(sum) : sum != sum ? sum : kNoNorm;
+            const float sum = sum_of_16(s[i]), inv = !(sum <= 3.4e38f) ? __builtin_nanf("") : sum > kLeastNorm * kLeastNorm ? 1.f / __builtin_sqrtf(sum) : kNoNorm;
             if (r >= rows) continue;
             if (lane == 0) (r < rows_a ? inv_a[r] : inv_b[r - rows_a]) = inv;
             if (r >= rows_a) top = __builtin_fmaxf(top, inv);

@@ -235,3 +235,28 @@ def test_the_ops_by_themselves(kind):
                  lambda: b(one, *operands, saved[:64], *rest, 1, True, True), lambda: f(x, operands[1].cpu(), *operands[2:], *rest, 1)):
         with pytest.raises((RuntimeError, ValueError)):
             call()
+
+
+def test_rows_whose_length_fp32_does_not_hold():
+    """bfloat16 reaches 3e38, whose square fp32 does not: such a row's cosines are no numbers, where 0 would be a wrong one.  Short rows
+    have theirs down to 1e-12, below which a row counts as zeros."""
+    x, w, target, _, _ = _inputs()
+    x, w = torch.nn.functional.normalize(x.float()).to(BF16), torch.nn.functional.normalize(w.float()).to(BF16)
+    call = lambda a, b: losses.margin_cross_entropy(a, b, target, reduction="none")
+    want, up = call(x, w), torch.ones(33, device="cuda")
+    other = torch.arange(33, device="cuda") != 4
+    for size, fine in ((2.0 ** 62, True), (2.0 ** 66, False), (2.0 ** -38, True)):
+        a = torch.where(other.unsqueeze(1), x, x * size)
+        loss, dx, _ = _both(call, a, w, up)
+        assert torch.equal(loss[other], want[other])
+        if fine:
+            assert abs(loss[4] - want[4]) <= 1e-5 * want[4] and dx[4].any() and torch.isfinite(dx[4]).all()
+        else:
+            assert loss[4].isnan() and dx[4].isnan().all()
+    short = torch.where(other.unsqueeze(1), x, x * 2.0 ** -41)
+    loss, dx, _ = _both(call, short, w, up)
+    zeros = torch.where(other.unsqueeze(1), x, torch.zeros_like(x))
+    assert torch.equal(loss, call(zeros, w)) and not dx[4].any()
+    heavy = w.clone()
+    heavy[9] *= 2.0 ** 66
+    assert call(x, heavy).isnan().all()
