@@ -384,7 +384,8 @@ int na1d_train_context_backward(void *dx, const void *dctx, const void *x, const
 
 /*
  * Losses over a large number of classes, forward and backward, without the logits in memory.  They replace the classification
- * heads of models/SoftMaxLoss.py:7-138 (and add a teacher's): x [N, D] are embeddings or hidden states, w [V * subcenters, D]
+ * head of models/SoftMaxLoss.py:99-138 (its additive angular margin, with sub-centres; the same file's additive cosine margin is
+ * not among them) and add a plain softmax head's and a teacher's: x [N, D] are embeddings or hidden states, w [V * subcenters, D]
  * the classes' weight rows, both 16-bit with contiguous channels and rows x_stride, w_stride elements apart.
  *   kind NA1D_HEAD_TARGETS: z = scale * x . w, loss of a row: log sum exp z - z[target]
  *   kind NA1D_HEAD_MARGIN:  cos = max over a class's subcenters of x . w / (|x| |w|); z = scale * cos, at the target
