@@ -404,8 +404,8 @@ int na1d_train_context_backward(void *dx, const void *dctx, const void *x, const
  *   dx, dw: 16-bit, packed [N, D] and [V * subcenters, D]; either may be NULL
  * Sums are in fp32; the gradients of the logits are scaled as one and rounded to 16 bits before they
  * are multiplied.  Nothing uses atomics: results are the same from call to call.
- * A backward's workspace covers both gradients: at most 512 MB (1.25 GB from N * subcenters = 2^19 on), 4 N D bytes
- * and, from N * subcenters = 2^21 on, 1024 subcenters D.
+ * A forward's workspace is 8 bytes to a row and tile of 32 to 256 classes; a backward's covers both gradients: at most 512 MB
+ * (1.25 GB from N * subcenters = 2^19 on), 4 N D bytes and, from N * subcenters = 2^21 on, 1024 subcenters D.
  * D % 8 == 0; x, w, dx, dw, saved and the workspace 16-byte aligned, strides multiples of 8 and at least D.  Limits
  * (NA1D_ERR_UNSUPPORTED): N up to 2^20, V * subcenters up to 2^24, w_stride * subcenters and x_stride up to 2^20, N * V, N * D and
  * V * subcenters * D up to 2^36, subcenters up to 255, top up to NA1D_HEAD_MAX_TOP.

@@ -28,8 +28,8 @@ using namespace enc;
 // the tile's rows (64 to a piece) and 64 values of each; one whose contraction runs from row to row ("turned") has 64 rows of
 // the contraction and 64 of the tile's columns, which come out of LDS transposed (ds_read_b64_tr_b16).  The 16-byte units of a
 // row are XOR-swizzled by three bits of its number, by which the sixteen rows of a row operand's read, and the rows {0-3, 8-11} or
-// {4-7, 12-15} of half a wave's transposed read, spread over all banks; no one choice of bits does for both (counted: an operand's
-// read takes 4 cycles and a transposed one 2, with the other's choice 8 and 4).
+// {4-7, 12-15} of half a wave's transposed read, spread over all banks; no one choice of bits does for both (an operand's
+// read takes 4 cycles and a transposed one 2, with the other's choice 8 and 4; the kernels' counters show no conflicts).
 constexpr int kStep = 64;                     // of the contraction
 constexpr int kPieceRow = 2 * kStep;          // bytes
 constexpr int kPiece = 64 * kPieceRow;
@@ -677,7 +677,7 @@ logits_kernel(Logits a) {
 // A row's tiles put together, the target's logit, the loss
 // =============================================================================
 // Waits more than it works: 8192 rows of 256 tiles 6 us.  A teacher's entries are products of their own, read row by row: 4096 x 64 of 768
-// channels 70 us, 5.7 TB/s out of the last level of cache (the weight is 74 MB).
+// channels 74 us, 419 MB behind the L2s at 5.7 TB/s, out of the last level of cache (the weight is 74 MB).
 struct Finish {
     Head h;
     const f32x2 *part, *at;
@@ -1086,7 +1086,7 @@ products_kernel(Product dx, Product dw, uint32_t dx_items, uint32_t dw_items) {
 
 // The shares of all splits of a row put together, less their part along the row's own vector (cosines).  WAVES waves to a row share
 // its splits: four where there are 8 or more, sixteen where there are 32 and few rows (whole backwards with sixteen and with four: 20 rows of 512 channels, 61
-// splits 42 and 44 us; 700 of 96, 60 splits 83 and 76).  Bound by memory: 8192 rows of 1024 channels, two splits 15 us, 5.5 TB/s.
+// splits 42 and 44 us; 700 of 96, 60 splits 83 and 76).  Bound by memory: 8192 rows of 1024 channels, two splits 18 us, 84 MB at 4.7 TB/s.
 struct Fold {
     char *out;
     const float *part;
