@@ -298,7 +298,8 @@ __device__ inline int load_id(const void *ids, int64_t i, int wide) {
     return v < INT32_MIN || v > INT32_MAX ? (v < 0 ? INT32_MIN : INT32_MAX) : (int)v;
 }
 // A row of zeros (no longer than kLeastNorm) has cosine 0 with everything and no gradient.  The factor of its products is a small
-// number and not 0, so that a masked logit of -inf stays one.  A row whose squares have no sum in fp32 has no cosine.
+// number and not 0, so that a masked logit of -inf stays one.  A row whose squares have no sum in fp32 has no cosine: a weight's factor is no
+// number, a row's of x is 0, by which finish_kernel knows it - it need not count.
 constexpr float kLeastNorm = 1e-12f, kNoNorm = 1e-30f;
 
 constexpr int kNormBlocks = 1024;
@@ -334,7 +335,7 @@ norms_kernel(float *__restrict__ inv_a, float *__restrict__ inv_b, float *__rest
 #pragma unroll
         for (int i = 0; i < kAtOnce; ++i) {
             const int64_t r = r0 + i * step;
-            const float sum = sum_of_16(s[i]), inv = !(sum <= 3.4e38f) ? __builtin_nanf("") : sum > kLeastNorm * kLeastNorm ? 1.f / __builtin_sqrtf(sum) : kNoNorm;
+            const float sum = sum_of_16(s[i]), inv = sum > 3.4e38f ? (r < rows_a ? 0.f : __builtin_nanf("")) : sum > kLeastNorm * kLeastNorm ? 1.f / __builtin_sqrtf(sum) : sum != sum ? sum : kNoNorm;
             if (r >= rows) continue;
             if (lane == 0) (r < rows_a ? inv_a[r] : inv_b[r - rows_a]) = inv;
             if (r >= rows_a) top = __builtin_fmaxf(top, inv);
@@ -774,6 +775,7 @@ finish_kernel(Finish a) {
             bool hit = false;
             if (raw != a.ignore && raw >= 0 && raw < a.h.V) {
                 float best = a.at[row].x, slope = 1.f;
+                if (a.cosines && a.h.inv_x[row] == 0.f) best = __builtin_nanf("");
                 st.sub = (int)a.at[row].y;
                 hit = best * (a.h.scale2 * (a.cosines ? a.h.inv_x[row] : 1.f)) >= largest;         // as the tiles' maxima were worked out
                 if (a.cosines) {

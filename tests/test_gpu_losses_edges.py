@@ -257,6 +257,11 @@ def test_rows_whose_length_fp32_does_not_hold():
     loss, dx, _ = _both(call, short, w, up)
     zeros = torch.where(other.unsqueeze(1), x, torch.zeros_like(x))
     assert torch.equal(loss, call(zeros, w)) and not dx[4].any()
+    long = torch.where(other.unsqueeze(1), x, x * 2.0 ** 66)                # an ignored one has no say, as any other
+    ignored = target.masked_fill(~other, -100)
+    ignore = lambda a, b: losses.margin_cross_entropy(a, b, ignored, reduction="none", return_hits=True)[0]
+    assert _same(_both(ignore, long, w, up), _both(ignore, x, w, up))
+    assert not losses.margin_cross_entropy(long, w, target, return_hits=True)[1][4]
     heavy = w.clone()
     heavy[9] *= 2.0 ** 66
     assert call(x, heavy).isnan().all()
