@@ -194,7 +194,8 @@ def margin_cross_entropy(x, weight, target, margin=0.2, scale=32.0, ignore_index
 
     The target's cosine cos(theta) becomes cos(theta + margin) where theta + margin < pi, else cos(theta) - margin sin(pi - margin);
     the derivative takes the squared sine of theta as 1e-6 at least.  ``0 <= margin < pi / 2``.  A row of zeros (no longer
-    than 1e-12) has cosine 0 with everything and no gradient; one whose squares' sum is beyond fp32 (bfloat16, 1.8e19 and longer) has none: NaN.  Hits are by the cosines, without the margin.  Other arguments as in
+    than 1e-12) has cosine 0 with everything and no gradient; one whose squares' sum is beyond fp32 (bfloat16, 1.8e19 and longer)
+    has none, and what depends on it is NaN.  Hits are by the cosines, without the margin.  Other arguments as in
     :func:`linear_cross_entropy`.
     """
     check_arguments(x, weight, target, reduction, x.shape[:-1], weight_dims=(2, 3))

@@ -265,3 +265,15 @@ def test_rows_whose_length_fp32_does_not_hold():
     heavy = w.clone()
     heavy[9] *= 2.0 ** 66
     assert call(x, heavy).isnan().all()
+
+
+def test_under_compiled_autograd():
+    from torch._dynamo import compiled_autograd
+    x, w, target, ids, logits = _inputs()
+    for kind in KINDS:
+        call = _calls(target, ids, logits)[kind]
+        want = _both(call, x, w)
+        a, b = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        with compiled_autograd._enable(lambda graph: torch.compile(graph, backend="eager")):
+            call(a, b).backward()
+        assert torch.equal(a.grad, want[1]) and torch.equal(b.grad, want[2]), kind
