@@ -435,6 +435,38 @@ int na1d_head_backward(const na1d_head *h, void *dx, void *dw, const float *dlos
                        int64_t saved_bytes, void *workspace, int64_t workspace_bytes, void *stream);
 
 /*
+ * Causal attention with a sliding window of any length and a few first tokens that stay visible ("sinks"), for streams; no counterpart
+ * in the reference, whose windows are centred and at most NA1D_MAX_WINDOW long.  Query t of a sample sees key u where
+ *   u <= t  and  (t - u < window  or  u < sinks),
+ * P = softmax over those of scale * q . k, out = P v.  Queries have heads / kv_heads heads to every head of keys and values (head h
+ * goes with key head h / (heads / kv_heads)).
+ *   q [N, T, heads, head_dim], k, v [N, T, kv_heads, head_dim]: {sample, head, row} element strides, channels contiguous
+ *   out, dout, dq [N, T, heads, head_dim], dk, dv [N, T, kv_heads, head_dim]: packed
+ *   t_valid : int32 [N] or NULL; rows from there on do not exist: they may hold anything, their outputs and gradients are 0.
+ *             The rows before have to be finite.
+ *   saved   : what a forward leaves for its backward, na1d_sink_saved_bytes() bytes: 4 to a head's row and, with bf16, a byte to
+ *             a value of out; NULL for inference
+ * Scores, softmax and sums are in fp32; probabilities and their gradients are rounded to 16 bits where they are multiplied by v, k, q
+ * or dout.  Nothing uses atomics: results are the same from call to call.  A backward's workspace is 4 bytes to a head's row, and fp32 sums
+ * where several workgroups share the rows of a key head (those that are sinks, and all of them if there are few).
+ * head_dim % 8 == 0, up to 128 (NA1D_ERR_HEAD_DIM, NA1D_ERR_UNSUPPORTED); heads % kv_heads == 0, window >= 1, sinks >= 0
+ * (NA1D_ERR_SHAPE, NA1D_ERR_WINDOW); all pointers but t_valid 16-byte aligned, strides multiples of 8, row strides at least
+ * head_dim.  Limits (NA1D_ERR_UNSUPPORTED): T up to 2^24, row strides to 2^20, heads * head_dim too, N * T * heads to 2^36.
+ */
+typedef struct na1d_sink {
+    int32_t dtype, heads, kv_heads, head_dim;
+    float scale;                        /* finite and above 0 */
+    int64_t N, T, window, sinks;
+    int64_t q_strides[3], k_strides[3], v_strides[3];
+} na1d_sink;
+int64_t na1d_sink_saved_bytes(const na1d_sink *h);
+int64_t na1d_sink_backward_workspace_bytes(const na1d_sink *h);
+int na1d_sink_forward(const na1d_sink *h, void *out, void *saved, int64_t saved_bytes, const void *q, const void *k, const void *v, const int32_t *t_valid,
+                      void *stream);
+int na1d_sink_backward(const na1d_sink *h, void *dq, void *dk, void *dv, const void *q, const void *k, const void *v, const void *out, const void *dout,
+                       const void *saved, int64_t saved_bytes, const int32_t *t_valid, void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
  * Profiling hook; no counterpart in the reference.  From this call on, the matrix-core fused kernels that the
  * CALLING THREAD launches record `start` just before and `stop` just after the kernel itself (hipEvent_t handles,
  * recorded by hipExtLaunchKernel: the dispatch's own begin and end, i.e. what a profiler's kernel trace reports,

@@ -1,0 +1,74 @@
+"""Windowed causal attention with sinks in 64 bits by its formulas, with all pairs of a query and a key in memory; caches by a loop over
+positions; and how far results in the kernels' number formats may be off.  Test infrastructure only."""
+import torch
+
+# fp32 work on a score of at most `s` in size, relative to a probability: sums of up to 128 products, a scale, a power of two
+# to 2^-21, and row sums of up to 2^14 terms in a tree of chunks
+FP32 = 2.0 ** -16
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def visible(t, u, window, sinks):
+    """Whether the tokens at positions t see those at u."""
+    t, u = t.unsqueeze(-1), u.unsqueeze(-2)
+    return (u >= 0) & (u <= t) & ((t - u < window) | (u < sinks))
+
+
+def softmax_rows(scores, seen):
+    """Probabilities of what is seen; zeros for a row that sees nothing."""
+    scores = scores.masked_fill(~seen, -torch.inf)
+    high = scores.amax(-1, keepdim=True)
+    e = torch.where(seen, (scores - high).exp(), 0.0)
+    total = e.sum(-1, keepdim=True)
+    return torch.where(total > 0, e / total, 0.0)
+
+
+def _heads(x, H):
+    """[N, T, heads, C] in 64 bits as [N, H, T, C], every head as often as its group has heads."""
+    x = x.double().transpose(1, 2)
+    return x.repeat_interleave(H // x.shape[1], 1)
+
+
+def attention(q, k, v, window, sinks=0, t_valid=None, scale=None, dout=None):
+    """{"out", and with dout "dq", "dk", "dv"}: (value, how far a kernel's may be off), each like its tensor.
+
+    The bounds count half steps u of the 16-bit type: a probability is rounded where it is multiplied (u) and divided by a sum of rounded ones
+    (u); dS is rounded (u); an output is (u); delta = rowsum(dO O) has what O lost: u of it with fp16, and the byte that goes with
+    bf16 leaves 2^-16; the fp32 work, FP32 times the size of a score."""
+    N, T, H, C = q.shape
+    K, dtype, u = k.shape[2], q.dtype, half_step(q.dtype)
+    scale = C ** -0.5 if scale is None else scale
+    real = torch.ones(N, T, dtype=torch.bool, device=q.device) if t_valid is None else torch.arange(T, device=q.device) < t_valid.unsqueeze(1)
+    clean = lambda x: torch.where(real[:, :, None, None], x, torch.zeros_like(x))  # noqa: E731
+    q_, k_, v_ = (_heads(clean(x), H) for x in (q, k, v))
+    at = torch.arange(T, device=q.device)
+    seen = visible(at, at, window, sinks) & real[:, None, :, None] & real[:, None, None, :]
+    s = q_ @ k_.transpose(-1, -2) * scale
+    p = softmax_rows(s, seen)
+    f = FP32 * (1 + (q_.abs() @ k_.abs().transpose(-1, -2) * scale).amax().item())
+    out, size = p @ v_, p @ v_.abs()
+    got = {"out": (out, u * out.abs() + (2 * u + f) * size)}
+    if dout is not None:
+        g = _heads(clean(dout), H)
+        dp, delta = g @ v_.transpose(-1, -2), (g * out).sum(-1, keepdim=True)
+        ds = p * (dp - delta)
+        ddelta = ((2 * u + f) * (g.abs() * size) + ((u if dtype == torch.float16 else 2.0 ** -16) + f) * (g * out).abs()).sum(-1, keepdim=True)
+        dds = p * (ddelta + f * (g.abs() @ v_.abs().transpose(-1, -2))) + (2 * u + f) * ds.abs()
+        groups = lambda x: x.view(N, K, H // K, T, C).sum(2)  # noqa: E731
+        dq, dk, dv = scale * ds @ k_, groups(scale * ds.transpose(-1, -2) @ q_), groups(p.transpose(-1, -2) @ g)
+        got["dq"] = (dq, u * dq.abs() + scale * dds @ k_.abs())
+        got["dk"] = (dk, u * dk.abs() + groups(scale * dds.transpose(-1, -2) @ q_.abs()))
+        got["dv"] = (dv, u * dv.abs() + (2 * u + f) * groups(p.transpose(-1, -2) @ g.abs()))
+    # What is too small for its format.  A power of two below fp32's (and bf16's) least normal value, 2^-126, is 0, and so is a dS or a result: each is off
+    # by that at most.  fp16 rounds p, dS and results to multiples of 2^-24, half of one off.  A term's share counts times what it is multiplied by
+    # (dP - delta and then k or q, or dout, or v), for every term of a sum.
+    least = 2.0 ** -25 if dtype == torch.float16 else 2.0 ** -126
+    most = lambda x: float(x.double().nan_to_num(0, 0, 0).abs().max()) if x.numel() else 0.0  # noqa: E731
+    spread = 1 if dout is None else 1 + most(dp - delta)
+    times = {"out": 1 + T * most(v_), "dq": 1 + 2 * scale * T * spread * most(k_), "dk": 1 + 2 * scale * T * H * spread * most(q_)}
+    if dout is not None:
+        times["dv"] = 1 + T * H * most(g)
+    return {n: (a.transpose(1, 2), (b + least * times[n]).transpose(1, 2)) for n, (a, b) in got.items()}

@@ -610,6 +610,53 @@ int na1d_head_backward(const na1d_head *h, void *dx, void *dw, const float *dlos
     return na1d::loss::run_backward(*h, dx, dw, dloss, x, w, ids, saved, workspace, (hipStream_t)stream);
 }
 
+// +1: nothing to do
+static int sink_check(const na1d_sink *h) {
+    if (!h) return NA1D_ERR_NULL;
+    if (h->dtype != NA1D_BF16 && h->dtype != NA1D_FP16) return NA1D_ERR_DTYPE;
+    if (h->head_dim < 1 || h->head_dim % 8) return NA1D_ERR_HEAD_DIM;
+    if (h->window < 1 || h->sinks < 0) return NA1D_ERR_WINDOW;
+    if (h->N < 0 || h->T < 0 || h->heads < 1 || h->kv_heads < 1 || h->heads % h->kv_heads) return NA1D_ERR_SHAPE;
+    if (bad_scale(h->scale)) return NA1D_ERR_SCALE;
+    const int64_t widest = 1 << 20;
+    if (h->head_dim > 128 || h->T > (1 << 24) || (int64_t)h->heads * h->head_dim > widest) return NA1D_ERR_UNSUPPORTED;
+    if (h->N > (1ll << 36) / h->heads / (h->T > 0 ? h->T : 1)) return NA1D_ERR_UNSUPPORTED;
+    for (const int64_t *s : {h->q_strides, h->k_strides, h->v_strides}) {
+        if (s[0] < 0 || s[1] < 0 || s[2] < h->head_dim) return NA1D_ERR_SHAPE;
+        if (s[0] % 8 || s[1] % 8 || s[2] % 8) return NA1D_ERR_ALIGN;
+        if (s[2] > widest || s[1] > (1ll << 40) || s[0] > (1ll << 44)) return NA1D_ERR_UNSUPPORTED;
+    }
+    return h->N == 0 || h->T == 0;
+}
+int64_t na1d_sink_saved_bytes(const na1d_sink *h) {
+    const int st = sink_check(h);
+    return st == NA1D_OK ? na1d::mfma::sink_saved_bytes(*h) : st > 0 ? 0 : st;
+}
+int64_t na1d_sink_backward_workspace_bytes(const na1d_sink *h) {
+    const int st = sink_check(h);
+    return st == NA1D_OK ? na1d::mfma::sink_bwd_workspace_bytes(*h) : st > 0 ? 0 : st;
+}
+int na1d_sink_forward(const na1d_sink *h, void *out, void *saved, int64_t saved_bytes, const void *q, const void *k, const void *v, const int32_t *t_valid,
+                      void *stream) {
+    const int st = sink_check(h);
+    if (st != NA1D_OK) return st > 0 ? NA1D_OK : st;
+    if (!out || !q || !k || !v) return NA1D_ERR_NULL;
+    if (misaligned(out) || misaligned(saved) || misaligned(q) || misaligned(k) || misaligned(v)) return NA1D_ERR_ALIGN;
+    if (saved && saved_bytes < na1d::mfma::sink_saved_bytes(*h)) return NA1D_ERR_WORKSPACE;
+    return na1d::mfma::sink_fwd(*h, out, (float *)saved, q, k, v, t_valid, (hipStream_t)stream);
+}
+int na1d_sink_backward(const na1d_sink *h, void *dq, void *dk, void *dv, const void *q, const void *k, const void *v, const void *out, const void *dout,
+                       const void *saved, int64_t saved_bytes, const int32_t *t_valid, void *workspace, int64_t workspace_bytes, void *stream) {
+    const int st = sink_check(h);
+    if (st != NA1D_OK) return st > 0 ? NA1D_OK : st;
+    for (const void *p : {(const void *)dq, (const void *)dk, (const void *)dv, q, k, v, out, dout, saved, (const void *)workspace}) {
+        if (!p) return NA1D_ERR_NULL;
+        if (misaligned(p)) return NA1D_ERR_ALIGN;
+    }
+    if (saved_bytes < na1d::mfma::sink_saved_bytes(*h) || workspace_bytes < na1d::mfma::sink_bwd_workspace_bytes(*h)) return NA1D_ERR_WORKSPACE;
+    return na1d::mfma::sink_bwd(*h, dq, dk, dv, q, k, v, out, dout, (const float *)saved, t_valid, (float *)workspace, (hipStream_t)stream);
+}
+
 int na1d_fused_backward_noalloc(void *dq, void *dk, void *dv, float *drpb, const void *q, const void *k, const void *v,
                                 const void *out, const void *dout, const float *lse, const float *rpb,
                                 const int32_t *t_valid, int64_t B, int64_t H, int64_t T, int64_t C, int64_t W,

@@ -241,4 +241,13 @@ int run_forward(const na1d_head &h, float *loss, uint8_t *hits, const void *x, c
 int run_backward(const na1d_head &h, void *dx, void *dw, const float *dloss, const void *x, const void *w, const void *ids, const void *saved, void *ws, hipStream_t s);
 }  // namespace loss
 
+// ---- windowed causal attention with sinks: na1d_sink.hip ------------------
+namespace mfma {
+int64_t sink_saved_bytes(const na1d_sink &h);
+int64_t sink_bwd_workspace_bytes(const na1d_sink &h);
+int sink_fwd(const na1d_sink &h, void *out, float *saved, const void *q, const void *k, const void *v, const int32_t *t_valid, hipStream_t s);
+int sink_bwd(const na1d_sink &h, void *dq, void *dk, void *dv, const void *q, const void *k, const void *v, const void *out, const void *dout, const float *saved,
+             const int32_t *t_valid, float *ws, hipStream_t s);
+}  // namespace mfma
+
 }  // namespace na1d

@@ -24,34 +24,6 @@ namespace mfma {
 constexpr int kStripTiles = 4;      // tiles per strip (one per wave) and per chunk
 static_assert(kStripTiles == kWaves, "one tile of the strip per wave");
 
-// Two 16-bit values of a register as floats.
-template <class DT> __device__ inline f32x2 unpack2(uint32_t w);
-template <> __device__ inline f32x2 unpack2<BF16>(uint32_t w) {
-    return f32x2{__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)};
-}
-template <> __device__ inline f32x2 unpack2<FP16>(uint32_t w) {
-    return __builtin_convertvector(__builtin_bit_cast(f16x2, w), f32x2);
-}
-// sum over this lane's channels of a[c] * b[c] for two row operands
-template <class DT, int C>
-__device__ inline float dot_lane(const RowOperand<C> &a, const RowOperand<C> &b) {
-    float acc = 0.f;
-#pragma unroll
-    for (int s = 0; s < RowOperand<C>::k32; ++s)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const f32x2 x = unpack2<DT>(a.w32[s][i]), y = unpack2<DT>(b.w32[s][i]);
-            acc = __builtin_fmaf(x.x, y.x, __builtin_fmaf(x.y, y.y, acc));
-        }
-    if (RowOperand<C>::k16)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const f32x2 x = unpack2<DT>(a.w16[0][i]), y = unpack2<DT>(b.w16[0][i]);
-            acc = __builtin_fmaf(x.x, y.x, __builtin_fmaf(x.y, y.y, acc));
-        }
-    return acc;
-}
-
 // x *= a in the registers x lives in.  Written as plain C++ inside a branch, the compiler gives the products new
 // registers and pays for it with copies of every accumulator on both sides of the branch.  The accumulators are
 // results of matrix instructions the compiler cannot relate to this block: callers keep at least a dozen

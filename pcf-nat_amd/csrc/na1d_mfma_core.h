@@ -285,6 +285,34 @@ __device__ inline f32x4 dot_rows_mma(const RowOperand<C> &a, const RowOperand<C>
     return acc;
 }
 
+// Two 16-bit values of a register as floats.
+template <class DT> __device__ inline f32x2 unpack2(uint32_t w);
+template <> __device__ inline f32x2 unpack2<BF16>(uint32_t w) {
+    return f32x2{__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)};
+}
+template <> __device__ inline f32x2 unpack2<FP16>(uint32_t w) {
+    return __builtin_convertvector(__builtin_bit_cast(f16x2, w), f32x2);
+}
+// sum over this lane's channels of a[c] * b[c] for two row operands
+template <class DT, int C>
+__device__ inline float dot_lane(const RowOperand<C> &a, const RowOperand<C> &b) {
+    float acc = 0.f;
+#pragma unroll
+    for (int s = 0; s < RowOperand<C>::k32; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f32x2 x = unpack2<DT>(a.w32[s][i]), y = unpack2<DT>(b.w32[s][i]);
+            acc = __builtin_fmaf(x.x, y.x, __builtin_fmaf(x.y, y.y, acc));
+        }
+    if (RowOperand<C>::k16)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const f32x2 x = unpack2<DT>(a.w16[0][i]), y = unpack2<DT>(b.w16[0][i]);
+            acc = __builtin_fmaf(x.x, y.x, __builtin_fmaf(x.y, y.y, acc));
+        }
+    return acc;
+}
+
 // Transposed operand: output lane (n, g) receives tile[row 4g+0..3][chan 16*ct + n];
 // the lane supplies the address of row 4g + (n>>2), byte 32*ct + 8*(n&3).
 template <int C, int CS = C> struct TrLane {

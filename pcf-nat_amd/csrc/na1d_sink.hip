@@ -1,0 +1,715 @@
+// Causal attention with a sliding window of any length and a few first tokens that stay visible (sinks), forward and backward, on the
+// matrix cores (gfx950):
+//   P = softmax over the visible keys of q k^T * scale,  O = P v;   query t sees key u where u <= t and (t - u < window or u < sinks)
+// Queries have `group` heads to every head of keys and values.  Built from the tile machinery of na1d_mfma_core.h, like the dense
+// attention of na1d_global.hip: S^T tiles of 16 keys x 16 queries, an online softmax whose row statistics are lane-local up to a
+// reduction over the four lane groups, and the rounded probabilities fed straight back as the B operand of O^T += V^T P^T.
+//
+// A workgroup of the forward and of dQ owns a strip of one head's queries and walks the keys in chunks of 64 that its four waves share
+// through LDS: the chunks that hold sinks, then those that the strip's windows reach.  A workgroup of dK and dV owns a strip of
+// one key head's rows and walks the queries of all the heads of its group.  A chunk that all rows of a wave see whole needs no mask, one that
+// none of them sees is passed over by that wave.
+//
+// Rows from a sample's t_valid on do not exist: they are read as zeros whatever they hold (the buffer resources end there), and
+// their outputs and gradients are zeros.
+#include <type_traits>
+
+#include "na1d_mfma_core.h"
+
+namespace na1d {
+namespace mfma {
+namespace {
+
+constexpr int kChunkTiles = 4, kChunkRows = 16 * kChunkTiles;
+static_assert(kChunkTiles == kWaves, "row constants of a chunk are loaded by one wave to a tile");
+constexpr float kNoMaximum = -3.4e38f;      // where a row's running maximum starts: finite, so that a chunk which a row does not see leaves it alone
+
+struct SinkRows {               // one tensor: bytes from one sample, head, row to the next
+    int64_t sample, head;
+    int pitch;
+};
+struct SinkArgs {
+    int T, H, K, group, strips, window, sinks, width;      // width: bytes of a row
+    float scale;
+    SinkRows q, k, v, o;        // o: out and dout, and dq
+    SinkRows dkv;               // dk and dv
+    // dK and dV: strips that hold sinks are shared by sink_parts workgroups, the others by parts; their sums go to `partial`
+    int sink_strips, sink_parts, parts;
+};
+
+struct SinkItem {
+    uint32_t sample, kv, g;
+    int strip;
+};
+// A value that is the same in all lanes, in a scalar register (divisions and loads leave it in vector registers, where buffer resources cannot start).
+__device__ inline int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+// Heads of a group run side by side, then strips: what runs together on an XCD reads the same keys.
+__device__ inline SinkItem sink_item(uint32_t wg, uint32_t items, const SinkArgs &a) {
+    const uint32_t lin = xcd_item(wg, items), rest = uniform(lin / (uint32_t)a.group), head = uniform(rest / (uint32_t)a.strips);
+    SinkItem i;
+    i.g = lin - rest * a.group;
+    i.strip = (int)(rest - head * a.strips);
+    i.sample = uniform(head / (uint32_t)a.K);
+    i.kv = head - i.sample * a.K;
+    return i;
+}
+
+// Chunks of keys that rows row0 .. row1 meet: those of the sinks, [0, sink_end), and those of the windows, [from, end).
+struct KeyChunks {
+    int sink_end, from, end;
+    __device__ inline KeyChunks(int row0, int row1, int tv, const SinkArgs &a) {
+        const int last = min(row1, tv - 1);
+        end = last < row0 ? 0 : last / kChunkRows + 1;                   // nothing for a strip without a valid row
+        from = max(0, row0 - a.window + 1) / kChunkRows;
+        sink_end = min((a.sinks + kChunkRows - 1) / kChunkRows, end);
+        from = min(max(from, sink_end), end);
+    }
+    __device__ inline int first() const { return sink_end > 0 ? 0 : from; }
+    __device__ inline int after(int c) const { return c + 1 == sink_end ? from : c + 1; }
+};
+enum Sight { kNothing, kPart, kAll };
+// What queries q0 .. q1 see of keys k0 .. k1.
+__device__ inline Sight sight(int q0, int q1, int k0, int k1, const SinkArgs &a) {
+    if (k0 > q1 || (k0 >= a.sinks && q0 - k1 >= a.window)) return kNothing;
+    return k1 <= q0 && (k1 < a.sinks || q1 - k0 < a.window) ? kAll : kPart;
+}
+
+// `rows` rows of a tensor from row `row` on as a buffer resource: at most a strip of them, so that its bytes fit 31 bits wherever it lies.
+__device__ inline Rsrc rows_of(const void *base, int64_t row, int rows, int pitch) {
+    const uint64_t at = (uint64_t)base + row * pitch;
+    return make_rsrc((const void *)((uint64_t)(uint32_t)uniform((int)(at >> 32)) << 32 | (uint32_t)uniform((int)at)), uniform(max(0, rows) * pitch));
+}
+
+// What bf16 outputs lose in rounding, for the backward: delta = rowsum(dO * O) is taken away from every dP of a row, and with O as it is
+// stored, 2^-9 off, that alone made dQ and dK 3.5e-3 wrong (as a norm; all else together 2e-3).  An fp32 value is its bf16 rounding plus a
+// signed byte, as integers, to 2^-17: the bytes of a tile of 16 rows lie as dQ's waves read them, channels 32 s + 8 g of row n in the eight bytes
+// of lane 16 g + n of step s (16 channels: four bytes of a lane).  fp16 rounds to 2^-12 and goes without.
+template <class DT> constexpr bool kKeepsRest = DT::tag == NA1D_BF16;
+template <int C> constexpr int kRestBytes = 16 * C;      // of a tile
+// Four products' roundings `w` and the bytes they lack.
+__device__ inline uint32_t rest_of(f32x4 x, float f, u32x2 w) {
+    uint32_t b[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) b[r] = (__float_as_uint(x[r] * f) - ((r & 1) ? w[r / 2] & 0xffff0000u : w[r / 2] << 16)) >> 8;
+    return (b[0] & 0xffu) | (b[1] & 0xffu) << 8 | (b[2] & 0xffu) << 16 | b[3] << 24;
+}
+// A rounding and its byte, byte `i` of `rest`.
+template <class DT> __device__ inline float with_rest(uint32_t half, uint32_t rest, int i) {
+    return __uint_as_float((half << 16) + (uint32_t)((int32_t)(rest << (24 - 8 * i)) >> 24 << 8));
+}
+// rowsum over this lane's channels of a row of dO and one of O
+template <class DT, int C> __device__ inline float dot_whole(const RowOperand<C> &a, const RowOperand<C> &o, const char *rest, int lane) {
+    if constexpr (!kKeepsRest<DT>) {
+        return dot_lane<DT, C>(a, o);
+    } else {
+        float acc = 0.f;
+        auto add = [&](uint32_t x, uint32_t y, uint32_t b, int i) {
+            const f32x2 d = unpack2<DT>(x);
+            acc = __builtin_fmaf(d.x, with_rest<DT>(y & 0xffffu, b, i), __builtin_fmaf(d.y, with_rest<DT>(y >> 16, b, i + 1), acc));
+        };
+#pragma unroll
+        for (int s = 0; s < RowOperand<C>::k32; ++s) {
+            const u32x2 b = *reinterpret_cast<const u32x2 *>(rest + s * 512 + lane * 8);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) add(a.w32[s][i], o.w32[s][i], b[i / 2], 2 * (i & 1));
+        }
+        if (RowOperand<C>::k16) {
+            const uint32_t b = *reinterpret_cast<const uint32_t *>(rest + lane * 4);
+            add(a.w16[0][0], o.w16[0][0], b, 0);
+            add(a.w16[0][1], o.w16[0][1], b, 2);
+        }
+        return acc;
+    }
+}
+template <int C> __device__ inline void store_rest(char *rest, const uint32_t (&b)[C / 16], int lane) {
+    if constexpr (C == 16) {
+        *reinterpret_cast<uint32_t *>(rest + lane * 4) = b[0];
+    } else {
+        const int g = lane >> 4, to = (lane & 15) + 16 * (g == 1 ? 2 : g == 2 ? 1 : g);
+#pragma unroll
+        for (int s = 0; s < C / 32; ++s) {      // even groups get the first tile's eight channels, odd ones the second's
+            const u32x2 both = __builtin_amdgcn_permlane16_swap(b[2 * s], b[2 * s + 1], false, false);
+            *reinterpret_cast<u32x2 *>(rest + s * 512 + to * 8) = both;
+        }
+    }
+}
+
+// =============================================================================
+// Forward
+// =============================================================================
+template <class DT, int C, int QT>
+__global__ void __launch_bounds__(kThreads)
+sink_fwd_kernel(char *__restrict__ out, float *__restrict__ lse, char *__restrict__ rest, const char *__restrict__ q, const char *__restrict__ k, const char *__restrict__ v,
+                const int32_t *__restrict__ t_valid, uint32_t items, SinkArgs a) {
+    using LL = Lds<C>;
+    constexpr int CT = C / 16, kStep = region_bytes<C>(kChunkTiles);
+    extern __shared__ __attribute__((aligned(16))) char smem[];          // 4 * kStep bytes: K and V of two chunks
+    LDS_PTR(char) kv_lds = (LDS_PTR(char))smem;
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 4, n = lane & 15;
+    const SinkItem it = sink_item(blockIdx.x, items, a);
+    const int head = it.kv * a.group + it.g, T = a.T, width = a.width;
+    int tv = T;
+    if (t_valid) tv = uniform(max(0, min(T, t_valid[it.sample])));
+    const int row0 = it.strip * (kChunkRows * QT), row_end = min(T, row0 + kChunkRows * QT);
+    const char *kb = k + it.sample * a.k.sample + it.kv * a.k.head, *vb = v + it.sample * a.v.sample + it.kv * a.v.head;
+    const int k_lane = direct_lane_offset<C>(wave, lane, a.k.pitch, width), v_lane = direct_lane_offset<C>(wave, lane, a.v.pitch, width);
+    auto stage = [&](int c, LDS_PTR(char) to) {
+        const int rows = min(kChunkRows, tv - c * kChunkRows);
+        stage_direct<C, kChunkTiles, kReadShared>(rows_of(kb, (int64_t)c * kChunkRows, rows, a.k.pitch), 0, to, kChunkTiles, wave, k_lane, a.k.pitch);
+        stage_direct<C, kChunkTiles, kReadShared>(rows_of(vb, (int64_t)c * kChunkRows, rows, a.v.pitch), 0, to + kStep, kChunkTiles, wave, v_lane, a.v.pitch);
+    };
+    const KeyChunks chunks(row0, row_end - 1, tv, a);
+    int c = chunks.first();
+    if (c < chunks.end) stage(c, kv_lds);
+    const int own = 16 * QT * wave, w0 = row0 + own, w1 = w0 + 16 * QT - 1;      // this wave's rows
+    const Rsrc qs = rows_of(q + it.sample * a.q.sample + head * a.q.head, row0, min(row_end, tv) - row0, a.q.pitch);
+    RowOperand<C> qop[QT];
+#pragma unroll
+    for (int h = 0; h < QT; ++h) load_rows<C, kReadOnce>(qop[h], qs, (own + 16 * h) * a.q.pitch, a.q.pitch, width, lane);
+    const float scale2 = a.scale * kLog2e;               // the scale is positive: checked at the C boundary
+
+    RowLane<C> row_lane;
+    TrLane<C> tr_lane;
+    row_lane.init(0, lane);
+    tr_lane.init(0, lane);
+    constexpr float kSlack = 6.f;
+    float m[QT];
+    f32x4 o[QT][CT], lsum[QT];                            // lsum: the row sum, in every register
+#pragma unroll
+    for (int h = 0; h < QT; ++h) {
+        m[h] = kNoMaximum;
+        lsum[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) o[h][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    int at = 0;                                           // byte offset of the chunk's pair of regions: 0 or 2 * kStep
+    while (c < chunks.end) {
+        wait_direct();
+        barrier_lds();      // this chunk has landed, and every wave is done with the one before, whose regions the next takes
+        const int next = chunks.after(c), k0 = c * kChunkRows;
+        if (next < chunks.end) stage(next, kv_lds + (at ^ 2 * kStep));
+        LDS_PTR(char) k_lds = kv_lds + at;
+        LDS_PTR(char) v_lds = k_lds + kStep;
+        at ^= 2 * kStep;
+        c = next;
+        const Sight see = w0 < tv ? sight(w0, w1, k0, k0 + kChunkRows - 1, a) : kNothing;
+        if (see == kNothing) continue;
+        f32x4 s[QT][kChunkTiles];
+#pragma unroll
+        for (int kt = 0; kt < kChunkTiles; ++kt) {
+            RowOperand<C> kop;
+            read_rows<C>(kop, k_lds + kt * LL::kTileBytes, row_lane);
+#pragma unroll
+            for (int h = 0; h < QT; ++h) s[h][kt] = dot_rows_mma<DT, C>(kop, qop[h]);
+        }
+        if (see == kPart) {
+#pragma unroll
+            for (int h = 0; h < QT; ++h) {
+                const int row = w0 + 16 * h + n, d = row - k0 - 4 * g, stay = min(a.sinks, row + 1) - k0 - 4 * g;
+#pragma unroll
+                for (int kt = 0; kt < kChunkTiles; ++kt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (!((uint32_t)(d - 16 * kt - r) < (uint32_t)a.window || 16 * kt + r < stay)) s[h][kt][r] = kNegInf;
+            }
+        }
+        u32x4 pp[QT][kChunkTiles / 2];          // probabilities of two key tiles: the B operand of a 32-deep product
+#pragma unroll
+        for (int h = 0; h < QT; ++h) {
+            float mc = kNegInf;
+#pragma unroll
+            for (int kt = 0; kt < kChunkTiles; ++kt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) mc = __builtin_fmaxf(mc, s[h][kt][r]);
+            mc = xor_max(mc) * scale2;
+            // The reference point of the exponentials moves only when a row's maximum has outgrown it by more than
+            // kSlack (probabilities then stay below 2^kSlack, which every format here holds): most chunks leave
+            // the accumulators as they are.
+            if (__builtin_amdgcn_ballot_w64(mc > m[h] + kSlack)) {
+                const float m_new = max2(m[h], mc);
+                const float alpha = __builtin_amdgcn_exp2f(m[h] - m_new);
+                m[h] = m_new;
+                lsum[h] *= alpha;
+#pragma unroll
+                for (int ct = 0; ct < CT; ++ct) o[h][ct] *= alpha;
+            }
+            const float ref = -m[h];
+#pragma unroll
+            for (int kt = 0; kt < kChunkTiles; ++kt) {
+                float p[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][kt][r], scale2, ref));
+                pp[h][kt / 2][2 * (kt & 1)] = Mma<DT>::pack(p[0], p[1]);
+                pp[h][kt / 2][2 * (kt & 1) + 1] = Mma<DT>::pack(p[2], p[3]);
+            }
+        }
+        // O^T += V^T P^T over two key tiles at a time; the row sums come from the same instruction with ones in place of V^T.
+#pragma unroll
+        for (int kt = 0; kt < kChunkTiles; kt += 2) {
+            LDS_PTR(char) blk = v_lds + kt * LL::kTileBytes;
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+                const u32x2 v0 = read_tr(blk + tr_lane.off[ct]), v1 = read_tr(blk + LL::kTileBytes + tr_lane.off[ct]);
+                const u32x4 vv = {v0.x, v0.y, v1.x, v1.y};
+#pragma unroll
+                for (int h = 0; h < QT; ++h) o[h][ct] = Mma<DT>::k32(vv, pp[h][kt / 2], o[h][ct]);
+            }
+            const uint32_t one = Mma<DT>::pack(1.f, 1.f);
+            const u32x4 ones = {one, one, one, one};
+#pragma unroll
+            for (int h = 0; h < QT; ++h) lsum[h] = Mma<DT>::k32(ones, pp[h][kt / 2], lsum[h]);
+        }
+    }
+    const Rsrc os = rows_of(out + it.sample * a.o.sample + head * a.o.head, row0, row_end - row0, a.o.pitch);
+    const Rsrc ls = make_rsrc(lse ? lse + ((int64_t)it.sample * a.H + head) * T + row0 : nullptr, lse ? (row_end - row0) * 4 : 0);
+#pragma unroll
+    for (int h = 0; h < QT; ++h) {
+        const int at_row = own + 16 * h + n;
+        const bool valid = row0 + at_row < tv;
+        const float l = lsum[h][0], inv = __builtin_amdgcn_rcpf(l);
+        u32x2 ow[CT];
+        uint32_t rw[CT];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+            ow[ct] = pack_acc<DT>(o[h][ct], inv);
+            if constexpr (kKeepsRest<DT>) rw[ct] = rest_of(o[h][ct], inv, ow[ct]);
+            if (!valid) ow[ct] = u32x2{0u, 0u}, rw[ct] = 0u;
+        }
+        if (kKeepsRest<DT> && rest && w0 + 16 * h < T)
+            store_rest<C>(rest + (((int64_t)it.sample * a.H + head) * ((T + 15) / 16) + (w0 / 16 + h)) * kRestBytes<C>, rw, lane);
+        store_tile<C>(os, at_row * a.o.pitch, ow, g, stores_whole_lines(a.o.pitch, C, 0), width);   // rows past T are dropped
+        // log2 of the row's sum of exponentials; 0 for a row that does not exist, whose q and dO the backward reads as zeros
+        if (g == 0) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(valid ? m[h] + __builtin_amdgcn_logf(l) : 0.f), ls, at_row * 4, 0, 0);
+    }
+}
+
+// =============================================================================
+// Backward, query side: delta = rowsum(dO * O) and dQ = scale * dS K,  dS = P (dO V^T - delta)
+// =============================================================================
+template <class DT, int C, int QT>
+__global__ void __launch_bounds__(kThreads)
+sink_dq_kernel(char *__restrict__ dq, float *__restrict__ delta, const char *__restrict__ q, const char *__restrict__ k, const char *__restrict__ v,
+               const char *__restrict__ out, const char *__restrict__ dout, const float *__restrict__ lse, const char *__restrict__ rest, const int32_t *__restrict__ t_valid,
+               uint32_t items, SinkArgs a) {
+    using LL = Lds<C>;
+    constexpr int CT = C / 16, kStep = region_bytes<C>(kChunkTiles);
+    extern __shared__ __attribute__((aligned(16))) char smem[];          // 4 * kStep bytes
+    LDS_PTR(char) kv_lds = (LDS_PTR(char))smem;
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 4, n = lane & 15;
+    const SinkItem it = sink_item(blockIdx.x, items, a);
+    const int head = it.kv * a.group + it.g, T = a.T, width = a.width;
+    int tv = T;
+    if (t_valid) tv = uniform(max(0, min(T, t_valid[it.sample])));
+    const int row0 = it.strip * (kChunkRows * QT), row_end = min(T, row0 + kChunkRows * QT);
+    const char *kb = k + it.sample * a.k.sample + it.kv * a.k.head, *vb = v + it.sample * a.v.sample + it.kv * a.v.head;
+    const int k_lane = direct_lane_offset<C>(wave, lane, a.k.pitch, width), v_lane = direct_lane_offset<C>(wave, lane, a.v.pitch, width);
+    auto stage = [&](int c, LDS_PTR(char) to) {
+        const int rows = min(kChunkRows, tv - c * kChunkRows);
+        stage_direct<C, kChunkTiles, kReadShared>(rows_of(kb, (int64_t)c * kChunkRows, rows, a.k.pitch), 0, to, kChunkTiles, wave, k_lane, a.k.pitch);
+        stage_direct<C, kChunkTiles, kReadShared>(rows_of(vb, (int64_t)c * kChunkRows, rows, a.v.pitch), 0, to + kStep, kChunkTiles, wave, v_lane, a.v.pitch);
+    };
+    const KeyChunks chunks(row0, row_end - 1, tv, a);
+    int c = chunks.first();
+    if (c < chunks.end) stage(c, kv_lds);
+    const int own = 16 * QT * wave, w0 = row0 + own, w1 = w0 + 16 * QT - 1;
+    const int64_t o_off = it.sample * a.o.sample + head * a.o.head, stat = ((int64_t)it.sample * a.H + head) * T + row0;
+    const int valid_rows = min(row_end, tv) - row0;
+    const Rsrc qs = rows_of(q + it.sample * a.q.sample + head * a.q.head, row0, valid_rows, a.q.pitch);
+    const Rsrc os = rows_of(out + o_off, row0, valid_rows, a.o.pitch), gs = rows_of(dout + o_off, row0, valid_rows, a.o.pitch);
+    const Rsrc ls = make_rsrc(lse + stat, (row_end - row0) * 4), ds = make_rsrc(delta + stat, (row_end - row0) * 4);
+    RowOperand<C> qop[QT], gop[QT], oop[QT];
+    float ref[QT];                                        // minus the row's log2 of its sum
+#pragma unroll
+    for (int h = 0; h < QT; ++h) {
+        const int r0 = own + 16 * h;
+        load_rows<C, kReadShared>(qop[h], qs, r0 * a.q.pitch, a.q.pitch, width, lane);
+        load_rows<C, kReadShared>(gop[h], gs, r0 * a.o.pitch, a.o.pitch, width, lane);
+        load_rows<C, kReadOnce>(oop[h], os, r0 * a.o.pitch, a.o.pitch, width, lane);
+        ref[h] = -__uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(ls, (r0 + n) * 4, 0, 0));
+    }
+    const float scale2 = a.scale * kLog2e;
+    RowLane<C> row_lane;
+    TrLane<C> tr_lane;
+    row_lane.init(0, lane);
+    tr_lane.init(0, lane);
+    f32x4 acc[QT][CT], minus_dl[QT];                      // the product dO . V^T starts at minus delta
+#pragma unroll
+    for (int h = 0; h < QT; ++h) {
+        const int tile = min(w0 / 16 + h, (T - 1) / 16);   // a tile past the last reads the last's bytes, with zeros for dO
+        const char *bytes = kKeepsRest<DT> ? rest + (((int64_t)it.sample * a.H + head) * ((T + 15) / 16) + tile) * kRestBytes<C> : nullptr;
+        const float dl = xor_sum(dot_whole<DT, C>(gop[h], oop[h], bytes, lane));   // lane (n, g) holds a quarter of row n's channels
+        minus_dl[h] = f32x4{-dl, -dl, -dl, -dl};
+        if (g == 0) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(dl), ds, (own + 16 * h + n) * 4, 0, 0);
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) acc[h][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    int at = 0;
+    while (c < chunks.end) {
+        wait_direct();
+        barrier_lds();
+        const int next = chunks.after(c), k0 = c * kChunkRows;
+        if (next < chunks.end) stage(next, kv_lds + (at ^ 2 * kStep));
+        LDS_PTR(char) k_lds = kv_lds + at;
+        LDS_PTR(char) v_lds = k_lds + kStep;
+        at ^= 2 * kStep;
+        c = next;
+        const Sight see = w0 < tv ? sight(w0, w1, k0, k0 + kChunkRows - 1, a) : kNothing;
+        if (see == kNothing) continue;
+#pragma unroll
+        for (int kt = 0; kt < kChunkTiles; kt += 2) {
+            u32x4 db[QT];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                RowOperand<C> kop, vop;
+                read_rows<C>(kop, k_lds + (kt + j) * LL::kTileBytes, row_lane);
+                read_rows<C>(vop, v_lds + (kt + j) * LL::kTileBytes, row_lane);
+#pragma unroll
+                for (int h = 0; h < QT; ++h) {
+                    const f32x4 s = dot_rows_mma<DT, C>(kop, qop[h]);
+                    const f32x4 dp = dot_rows_mma<DT, C>(vop, gop[h], minus_dl[h]);
+                    float p[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], scale2, ref[h]));
+                    if (see == kPart) {
+                        const int row = w0 + 16 * h + n, d = row - k0 - 4 * g - 16 * (kt + j), stay = min(a.sinks, row + 1) - k0 - 4 * g - 16 * (kt + j);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (!((uint32_t)(d - r) < (uint32_t)a.window || r < stay)) p[r] = 0.f;
+                    }
+                    db[h][2 * j] = Mma<DT>::pack(p[0] * dp[0], p[1] * dp[1]);
+                    db[h][2 * j + 1] = Mma<DT>::pack(p[2] * dp[2], p[3] * dp[3]);
+                }
+            }
+            LDS_PTR(char) blk = k_lds + kt * LL::kTileBytes;
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+                const u32x2 k0t = read_tr(blk + tr_lane.off[ct]), k1t = read_tr(blk + LL::kTileBytes + tr_lane.off[ct]);
+                const u32x4 kk = {k0t.x, k0t.y, k1t.x, k1t.y};
+#pragma unroll
+                for (int h = 0; h < QT; ++h) acc[h][ct] = Mma<DT>::k32(kk, db[h], acc[h][ct]);
+            }
+        }
+    }
+    const Rsrc dqs = rows_of(dq + o_off, row0, row_end - row0, a.o.pitch);
+#pragma unroll
+    for (int h = 0; h < QT; ++h) {
+        const int at_row = own + 16 * h + n;
+        u32x2 qw[CT];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+            qw[ct] = pack_acc<DT>(acc[h][ct], a.scale);
+            if (row0 + at_row >= tv) qw[ct] = u32x2{0u, 0u};
+        }
+        store_tile<C>(dqs, at_row * a.o.pitch, qw, g, stores_whole_lines(a.o.pitch, C, 0), width);
+    }
+}
+
+// =============================================================================
+// Backward, key side: dV = P^T dO and dK = scale * dS^T Q, summed over the heads of the group
+// =============================================================================
+// A workgroup owns a strip of keys, whose K and V rows stay in registers, and walks units of (head of the group, chunk of 64
+// queries): Q and dO through LDS, double-buffered.  The score product is taken with Q and K swapped, so that P and dS come out as
+// B operands.  Sinks are seen by all the queries behind them, other keys by a window of them: strips that hold sinks are shared by more
+// workgroups, which add up in fp32 through `partial` in a fixed order (sink_join_kernel).
+template <class DT, int C, int QT>
+__global__ void __launch_bounds__(kThreads)
+sink_dkv_kernel(char *__restrict__ dk, char *__restrict__ dv, float *__restrict__ partial, const char *__restrict__ q, const char *__restrict__ k,
+                const char *__restrict__ v, const char *__restrict__ dout, const float *__restrict__ lse, const float *__restrict__ delta,
+                const int32_t *__restrict__ t_valid, uint32_t items, SinkArgs a) {
+    using LL = Lds<C>;
+    constexpr int CT = C / 16, kStep = region_bytes<C>(kChunkTiles), kBuf = 2 * kStep + 2 * kChunkRows * 4;
+    extern __shared__ __attribute__((aligned(16))) char smem[];          // 2 * kBuf bytes: Q, dO and the rows' constants of two chunks
+    LDS_PTR(char) buf_lds = (LDS_PTR(char))smem;
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 4, n = lane & 15;
+    // work items of a key head: the strips with sinks, sink_parts to each, then the others, parts to each
+    const uint32_t lin = xcd_item(blockIdx.x, items), sink_items = a.sink_strips * a.sink_parts;
+    const uint32_t per_head = sink_items + (a.strips - a.sink_strips) * a.parts;
+    const uint32_t sh = uniform(lin / per_head), rest = lin - sh * per_head, sample = uniform(sh / (uint32_t)a.K), kv = sh - sample * a.K;
+    const bool of_sinks = rest < sink_items;
+    const uint32_t each = of_sinks ? a.sink_parts : a.parts, r_in = of_sinks ? rest : rest - sink_items;
+    const int strip = uniform((int)(r_in / each)) + (of_sinks ? 0 : a.sink_strips), part = uniform((int)(r_in % each));
+    const int T = a.T, width = a.width;
+    int tv = T;
+    if (t_valid) tv = uniform(max(0, min(T, t_valid[sample])));
+    const int row0 = strip * (kChunkRows * QT), row_end = min(T, row0 + kChunkRows * QT);
+    // chunks of queries that see something of the strip
+    const int last_key = min(row_end, tv) - 1;
+    int c_from = row0 / kChunkRows, c_end = c_from;
+    if (last_key >= row0) c_end = (int)min((int64_t)tv - 1, row0 < a.sinks ? (int64_t)tv - 1 : (int64_t)last_key + a.window - 1) / kChunkRows + 1;
+    const int nc = c_end - c_from;
+    const int units = nc * a.group, u_end = uniform((int)((int64_t)units * (part + 1) / each));
+    int u = uniform((int)((int64_t)units * part / each));
+    int hg = nc ? uniform(u / nc) : 0, c = nc ? c_from + u - hg * nc : 0;
+
+    const int q_lane = direct_lane_offset<C>(wave, lane, a.q.pitch, width), g_lane = direct_lane_offset<C>(wave, lane, a.o.pitch, width);
+    const char *qb = q + sample * a.q.sample, *gb = dout + sample * a.o.sample;
+    float row_lse, row_delta;                             // of row 16 * wave + n of the chunk in flight
+    auto stage = [&](int hg_, int c_, LDS_PTR(char) to) {
+        const int head = kv * a.group + hg_, rows = min(kChunkRows, tv - c_ * kChunkRows);
+        const int64_t r0 = (int64_t)c_ * kChunkRows, stat = ((int64_t)sample * a.H + head) * T + r0;
+        stage_direct<C, kChunkTiles, kReadShared>(rows_of(qb + head * a.q.head, r0, rows, a.q.pitch), 0, to, kChunkTiles, wave, q_lane, a.q.pitch);
+        stage_direct<C, kChunkTiles, kReadShared>(rows_of(gb + head * a.o.head, r0, rows, a.o.pitch), 0, to + kStep, kChunkTiles, wave, g_lane, a.o.pitch);
+        const Rsrc ls = make_rsrc(lse + stat, max(0, rows) * 4), ds = make_rsrc(delta + stat, max(0, rows) * 4);
+        row_lse = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(ls, (16 * wave + n) * 4, 0, 0));
+        row_delta = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(ds, (16 * wave + n) * 4, 0, 0));
+    };
+    if (u < u_end) stage(hg, c, buf_lds);
+    const int own = 16 * QT * wave, w0 = row0 + own, w1 = w0 + 16 * QT - 1;
+    const Rsrc ks = rows_of(k + sample * a.k.sample + kv * a.k.head, row0, last_key + 1 - row0, a.k.pitch);
+    const Rsrc vs = rows_of(v + sample * a.v.sample + kv * a.v.head, row0, last_key + 1 - row0, a.v.pitch);
+    RowOperand<C> kop[QT], vop[QT];
+#pragma unroll
+    for (int h = 0; h < QT; ++h) {
+        load_rows<C, kReadShared>(kop[h], ks, (own + 16 * h) * a.k.pitch, a.k.pitch, width, lane);
+        load_rows<C, kReadShared>(vop[h], vs, (own + 16 * h) * a.v.pitch, a.v.pitch, width, lane);
+    }
+    const float scale2 = a.scale * kLog2e;
+    RowLane<C> row_lane;
+    TrLane<C> tr_lane;
+    row_lane.init(0, lane);
+    tr_lane.init(0, lane);
+    f32x4 acck[QT][CT], accv[QT][CT];
+#pragma unroll
+    for (int h = 0; h < QT; ++h)
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) acck[h][ct] = accv[h][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    int at = 0;
+    for (; u < u_end; ++u) {
+        wait_direct();
+        {
+            // rows past tv: q and dO are zeros there, and so are these
+            const float constant = g == 0 ? -row_lse : -row_delta;
+            if (g < 2) *reinterpret_cast<LDS_PTR(float)>(buf_lds + at + 2 * kStep + (g * kChunkRows + 16 * wave + n) * 4) = constant;
+        }
+        barrier_lds();
+        const int q0 = c * kChunkRows;
+        if (++c == c_end) c = c_from, ++hg;
+        if (u + 1 < u_end) stage(hg, c, buf_lds + (kBuf - at));
+        LDS_PTR(char) q_lds = buf_lds + at;
+        LDS_PTR(char) g_lds = q_lds + kStep;
+        LDS_PTR(char) ref_lds = q_lds + 2 * kStep + 16 * g;
+        at = kBuf - at;
+        const Sight see = w0 < tv ? sight(q0, q0 + kChunkRows - 1, w0, w1, a) : kNothing;
+        if (see == kNothing) continue;
+#pragma unroll
+        for (int qi = 0; qi < kChunkTiles; qi += 2) {
+            u32x4 pb[QT], db[QT];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                RowOperand<C> qop, gop;
+                read_rows<C>(qop, q_lds + (qi + j) * LL::kTileBytes, row_lane);
+                read_rows<C>(gop, g_lds + (qi + j) * LL::kTileBytes, row_lane);
+                const f32x4 ref = *reinterpret_cast<LDS_PTR(f32x4)>(ref_lds + 64 * (qi + j));
+                const f32x4 del4 = *reinterpret_cast<LDS_PTR(f32x4)>(ref_lds + kChunkRows * 4 + 64 * (qi + j));
+#pragma unroll
+                for (int h = 0; h < QT; ++h) {
+                    const f32x4 s = dot_rows_mma<DT, C>(qop, kop[h]);        // [query 4g+r][key n]
+                    const f32x4 dp = dot_rows_mma<DT, C>(gop, vop[h], del4);
+                    float p[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], scale2, ref[r]));
+                    if (see == kPart) {
+                        const int key = w0 + 16 * h + n, d = q0 + 16 * (qi + j) + 4 * g - key;      // query 4g less the key
+                        const uint32_t reach = key < a.sinks ? 0x7fffffffu : (uint32_t)a.window;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (!((uint32_t)(d + r) < reach)) p[r] = 0.f;
+                    }
+                    pb[h][2 * j] = Mma<DT>::pack(p[0], p[1]);
+                    pb[h][2 * j + 1] = Mma<DT>::pack(p[2], p[3]);
+                    db[h][2 * j] = Mma<DT>::pack(p[0] * dp[0], p[1] * dp[1]);
+                    db[h][2 * j + 1] = Mma<DT>::pack(p[2] * dp[2], p[3] * dp[3]);
+                }
+            }
+            LDS_PTR(char) qtile = q_lds + qi * LL::kTileBytes;
+            LDS_PTR(char) gtile = g_lds + qi * LL::kTileBytes;
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+                const u32x2 g0 = read_tr(gtile + tr_lane.off[ct]), g1 = read_tr(gtile + LL::kTileBytes + tr_lane.off[ct]);
+                const u32x2 q0t = read_tr(qtile + tr_lane.off[ct]), q1t = read_tr(qtile + LL::kTileBytes + tr_lane.off[ct]);
+                const u32x4 gg = {g0.x, g0.y, g1.x, g1.y}, qq = {q0t.x, q0t.y, q1t.x, q1t.y};
+#pragma unroll
+                for (int h = 0; h < QT; ++h) {
+                    accv[h][ct] = Mma<DT>::k32(gg, pb[h], accv[h][ct]);
+                    acck[h][ct] = Mma<DT>::k32(qq, db[h], acck[h][ct]);
+                }
+            }
+        }
+    }
+    if (each > 1) {          // fp32 sums of this part: [head, strip's parts][dk, dv][row of the strip][C]
+        const uint32_t slot = a.parts > 1 ? sh * per_head + rest : sh * sink_items + rest;
+        float *to = partial + (int64_t)slot * (2 * kChunkRows * QT * C);
+#pragma unroll
+        for (int h = 0; h < QT; ++h) {
+            float *row = to + (own + 16 * h + n) * C + 4 * g;
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+                *reinterpret_cast<f32x4 *>(row + 16 * ct) = acck[h][ct];
+                *reinterpret_cast<f32x4 *>(row + kChunkRows * QT * C + 16 * ct) = accv[h][ct];
+            }
+        }
+        return;
+    }
+    const int64_t off = sample * a.dkv.sample + kv * a.dkv.head;
+    const Rsrc dks = rows_of(dk + off, row0, row_end - row0, a.dkv.pitch), dvs = rows_of(dv + off, row0, row_end - row0, a.dkv.pitch);
+    const bool stream = stores_whole_lines(a.dkv.pitch, C, 0);
+#pragma unroll
+    for (int h = 0; h < QT; ++h) {
+        const int at_row = own + 16 * h + n;
+        const bool valid = row0 + at_row < tv;
+        u32x2 kw[CT], vw[CT];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+            kw[ct] = pack_acc<DT>(acck[h][ct], a.scale);
+            vw[ct] = pack_acc<DT>(accv[h][ct], 1.f);
+            if (!valid) kw[ct] = vw[ct] = u32x2{0u, 0u};
+        }
+        store_tile<C>(dks, at_row * a.dkv.pitch, kw, g, stream, width);      // rows past T are dropped
+        store_tile<C>(dvs, at_row * a.dkv.pitch, vw, g, stream, width);
+    }
+}
+
+// The parts of a strip's dK and dV, added up in a fixed order: four channels of a row to a thread.
+template <class DT, int C, int QT>
+__global__ void __launch_bounds__(kThreads)
+sink_join_kernel(char *__restrict__ dk, char *__restrict__ dv, const float *__restrict__ partial, const int32_t *__restrict__ t_valid, SinkArgs a) {
+    constexpr int kRows = kChunkRows * QT, kQuads = C / 4;
+    const uint32_t sink_items = a.sink_strips * a.sink_parts, joined = a.parts > 1 ? a.strips : a.sink_strips;
+    const uint32_t per_head = sink_items + (a.parts > 1 ? (a.strips - a.sink_strips) * a.parts : 0);
+    constexpr uint32_t kBlocks = (kRows * kQuads + kThreads - 1) / kThreads;     // workgroups to a strip
+    const uint32_t block = blockIdx.x % kBlocks, unit = blockIdx.x / kBlocks, sh = unit / joined, strip = unit - sh * joined;
+    const uint32_t sample = sh / (uint32_t)a.K, kv = sh - sample * a.K;
+    const int i = block * kThreads + threadIdx.x, r = i / kQuads, ch = (i % kQuads) * 4, row = strip * kRows + r;
+    if (i >= kRows * kQuads || row >= a.T || 2 * ch >= a.width) return;
+    const bool of_sinks = strip < (uint32_t)a.sink_strips;
+    const int each = of_sinks ? a.sink_parts : a.parts;
+    const uint32_t slot = sh * per_head + (of_sinks ? strip * a.sink_parts : sink_items + (strip - a.sink_strips) * a.parts);
+    const float *from = partial + (int64_t)slot * (2 * kRows * C) + r * C + ch;
+    f32x4 sk = {0.f, 0.f, 0.f, 0.f}, sv = sk;
+    for (int p = 0; p < each; ++p, from += 2 * kRows * C) {
+        sk += *reinterpret_cast<const f32x4 *>(from);
+        sv += *reinterpret_cast<const f32x4 *>(from + kRows * C);
+    }
+    u32x2 kw = pack_acc<DT>(sk, a.scale), vw = pack_acc<DT>(sv, 1.f);
+    if (t_valid && row >= t_valid[sample]) kw = vw = u32x2{0u, 0u};
+    const int64_t off = sample * a.dkv.sample + kv * a.dkv.head + (int64_t)row * a.dkv.pitch + 2 * ch;
+    *reinterpret_cast<u32x2 *>(dk + off) = kw;
+    *reinterpret_cast<u32x2 *>(dv + off) = vw;
+}
+
+// ----------------------------------------------------------------------------- launchers
+// Two tiles of 16 rows to a wave (strips of 128 rows) where that leaves every CU a workgroup or more: each operand read from LDS then
+// feeds two products.
+bool two_tiles(const na1d_sink &h, int64_t heads) { return h.N * heads * ((h.T + 127) / 128) >= 256; }
+
+SinkArgs sink_args(const na1d_sink &h, bool two, bool keys) {
+    SinkArgs a{};
+    const int64_t rows = kChunkRows * (two ? 2 : 1);
+    a.T = (int)h.T, a.H = h.heads, a.K = h.kv_heads, a.group = h.heads / h.kv_heads, a.strips = (int)((h.T + rows - 1) / rows);
+    a.window = (int)std::min(h.window, h.T), a.sinks = (int)std::min(h.sinks, h.T), a.width = 2 * h.head_dim, a.scale = h.scale;
+    auto strided = [](const int64_t (&s)[3]) { return SinkRows{2 * s[0], 2 * s[1], (int)(2 * s[2])}; };
+    auto packed = [&](int heads) { return SinkRows{2 * h.T * heads * h.head_dim, 2 * h.head_dim, 2 * heads * h.head_dim}; };
+    a.q = strided(h.q_strides), a.k = strided(h.k_strides), a.v = strided(h.v_strides), a.o = packed(h.heads), a.dkv = packed(h.kv_heads);
+    if (keys) {
+        // A strip's work is its chunks of queries times the heads of the group.  Strips are shared where there are too few of them
+        // to occupy every CU twice, and those with sinks so that none of their parts is longer than the others' work.
+        const int64_t chunks = (h.T + kChunkRows - 1) / kChunkRows, others = std::min<int64_t>(chunks, (a.window + rows - 1) / kChunkRows + 2);
+        const int64_t wgs = h.N * h.kv_heads * a.strips;
+        a.sink_strips = (int)((a.sinks + rows - 1) / rows);
+        a.parts = (int)std::min<int64_t>({std::max<int64_t>(1, 512 / wgs), std::max<int64_t>(1, others * a.group / 4), 16});
+        const int64_t sharing = h.N * h.kv_heads * std::max(a.sink_strips, 1);
+        a.sink_parts = (int)std::min((chunks * a.parts + others - 1) / others, std::max<int64_t>(a.parts, 1024 / sharing));
+    }
+    return a;
+}
+// fp32 sums that the workgroups which share a strip leave
+int64_t partial_floats(const na1d_sink &h, const SinkArgs &a, bool two, int C) {
+    const int64_t slots = (a.sink_parts > 1 || a.parts > 1 ? (int64_t)a.sink_strips * a.sink_parts : 0) + (a.parts > 1 ? (int64_t)(a.strips - a.sink_strips) * a.parts : 0);
+    return h.N * h.kv_heads * slots * (2 * kChunkRows * (two ? 2 : 1) * (int64_t)C);
+}
+int64_t lse_floats(const na1d_sink &h) { return (h.N * h.heads * h.T + 3) / 4 * 4; }
+bool countable(int64_t items) { return items <= 0x7fffff00LL; }
+
+template <class DT, int C>
+int launch_sink_fwd(const na1d_sink &h, void *out, float *saved, const void *q, const void *k, const void *v, const int32_t *t_valid, hipStream_t s) {
+    const bool two = two_tiles(h, h.heads);
+    const SinkArgs a = sink_args(h, two, false);
+    const int64_t items = h.N * h.heads * a.strips;
+    if (!countable(items)) return NA1D_ERR_UNSUPPORTED;
+    const size_t lds = 4 * (size_t)region_bytes<C>(kChunkTiles);
+    auto go = [&](auto kern) {
+        if (!allow_lds(kern, lds)) return (int)NA1D_ERR_LAUNCH;
+        note_kernel_as("sink_fwd_kernel<%s, %d, %d>", DT::tag == NA1D_BF16 ? "BF16" : "FP16", C, two ? 2 : 1);
+        launch_kernel(kern, (unsigned)items, lds, s, (char *)out, saved, saved ? (char *)(saved + lse_floats(h)) : nullptr, (const char *)q, (const char *)k,
+                      (const char *)v, t_valid, (uint32_t)items, a);
+        return launch_status();
+    };
+    return two ? go(sink_fwd_kernel<DT, C, 2>) : go(sink_fwd_kernel<DT, C, 1>);
+}
+
+template <class DT, int C>
+int launch_sink_bwd(const na1d_sink &h, void *dq, void *dk, void *dv, const void *q, const void *k, const void *v, const void *out, const void *dout,
+                    const float *saved, const int32_t *t_valid, float *ws, hipStream_t s) {
+    const bool two_q = two_tiles(h, h.heads), two_k = two_tiles(h, h.kv_heads);
+    const SinkArgs a = sink_args(h, two_q, false), b = sink_args(h, two_k, true);
+    const int64_t items = h.N * h.heads * a.strips;
+    const int64_t key_items = h.N * h.kv_heads * ((int64_t)b.sink_strips * b.sink_parts + (int64_t)(b.strips - b.sink_strips) * b.parts);
+    const bool joins = b.parts > 1 || (b.sink_parts > 1 && b.sink_strips > 0);
+    const int64_t rows = kChunkRows * (two_k ? 2 : 1);
+    const int64_t join_items = !joins ? 0 : h.N * h.kv_heads * (b.parts > 1 ? b.strips : b.sink_strips) * ((rows * (C / 4) + kThreads - 1) / kThreads);
+    if (!countable(items) || !countable(key_items) || !countable(join_items)) return NA1D_ERR_UNSUPPORTED;
+    float *const delta = ws, *const partial = ws + lse_floats(h);
+    const size_t dq_lds = 4 * (size_t)region_bytes<C>(kChunkTiles), dkv_lds = 2 * (2 * (size_t)region_bytes<C>(kChunkTiles) + 2 * kChunkRows * sizeof(float));
+    auto go = [&](auto dq_kern, auto dkv_kern, auto join_kern) {
+        if (!allow_lds(dq_kern, dq_lds) || !allow_lds(dkv_kern, dkv_lds)) return (int)NA1D_ERR_LAUNCH;
+        note_kernel_as("sink_dq_kernel + sink_dkv_kernel<%s, %d, %d>", DT::tag == NA1D_BF16 ? "BF16" : "FP16", C, two_k ? 2 : 1);
+        launch_kernel_span(1, dq_kern, (unsigned)items, (unsigned)kThreads, dq_lds, s, (char *)dq, delta, (const char *)q, (const char *)k, (const char *)v,
+                           (const char *)out, (const char *)dout, saved, (const char *)(saved + lse_floats(h)), t_valid, (uint32_t)items, a);
+        launch_kernel_span(joins ? 0 : 2, dkv_kern, (unsigned)key_items, (unsigned)kThreads, dkv_lds, s, (char *)dk, (char *)dv, partial, (const char *)q, (const char *)k,
+                           (const char *)v, (const char *)dout, saved, (const float *)delta, t_valid, (uint32_t)key_items, b);
+        if (joins) launch_kernel_span(2, join_kern, (unsigned)join_items, (unsigned)kThreads, 0, s, (char *)dk, (char *)dv, (const float *)partial, t_valid, b);
+        return launch_status();
+    };
+    if (two_q)
+        return two_k ? go(sink_dq_kernel<DT, C, 2>, sink_dkv_kernel<DT, C, 2>, sink_join_kernel<DT, C, 2>)
+                     : go(sink_dq_kernel<DT, C, 2>, sink_dkv_kernel<DT, C, 1>, sink_join_kernel<DT, C, 1>);
+    return two_k ? go(sink_dq_kernel<DT, C, 1>, sink_dkv_kernel<DT, C, 2>, sink_join_kernel<DT, C, 2>)
+                 : go(sink_dq_kernel<DT, C, 1>, sink_dkv_kernel<DT, C, 1>, sink_join_kernel<DT, C, 1>);
+}
+
+}  // namespace
+
+int64_t sink_saved_bytes(const na1d_sink &h) {
+    return 4 * lse_floats(h) + (h.dtype == NA1D_BF16 ? h.N * h.heads * ((h.T + 15) / 16) * 16 * padded_width(h.head_dim) : 0);
+}
+int64_t sink_bwd_workspace_bytes(const na1d_sink &h) {
+    const bool two = two_tiles(h, h.kv_heads);
+    return 4 * (lse_floats(h) + partial_floats(h, sink_args(h, two, true), two, padded_width(h.head_dim)));
+}
+
+int sink_fwd(const na1d_sink &h, void *out, float *saved, const void *q, const void *k, const void *v, const int32_t *t_valid, hipStream_t s) {
+    const int dtype = h.dtype;
+    const struct { int C; } g{h.head_dim};
+    NA1D_MFMA_DISPATCH(launch_sink_fwd, h, out, saved, q, k, v, t_valid, s);
+}
+
+int sink_bwd(const na1d_sink &h, void *dq, void *dk, void *dv, const void *q, const void *k, const void *v, const void *out, const void *dout, const float *saved,
+             const int32_t *t_valid, float *ws, hipStream_t s) {
+    const int dtype = h.dtype;
+    const struct { int C; } g{h.head_dim};
+    NA1D_MFMA_DISPATCH(launch_sink_bwd, h, dq, dk, dv, q, k, v, out, dout, saved, t_valid, ws, s);
+}
+
+}  // namespace mfma
+}  // namespace na1d

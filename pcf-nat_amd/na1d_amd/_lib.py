@@ -32,7 +32,8 @@ SYMBOLS = _UNFUSED + ("na1d_fused_forward", "na1d_fused_backward", "na1d_fused_b
                       "na1d_train_layer_saved_bytes", "na1d_train_layer_workspace_bytes", "na1d_train_layer_forward",
                       "na1d_train_to_channels", "na1d_train_pool_backward", "na1d_train_context_backward", "na1d_train_context",
                       "na1d_train_layer_backward", "na1d_head_saved_bytes", "na1d_head_workspace_bytes", "na1d_head_forward",
-                      "na1d_head_backward", "na1d_version", "na1d_status_string")
+                      "na1d_head_backward", "na1d_sink_saved_bytes", "na1d_sink_backward_workspace_bytes", "na1d_sink_forward", "na1d_sink_backward",
+                      "na1d_version", "na1d_status_string")
 UNSUPPORTED = -8
 
 _lib = None
@@ -120,6 +121,11 @@ def load():
     lib.na1d_head_forward.restype = lib.na1d_head_backward.restype = _int
     lib.na1d_head_forward.argtypes = [_ptr] * 8 + [_i64, _ptr, _i64, _ptr]
     lib.na1d_head_backward.argtypes = [_ptr] * 8 + [_i64, _ptr, _i64, _ptr]
+    lib.na1d_sink_saved_bytes.restype = lib.na1d_sink_backward_workspace_bytes.restype = _i64
+    lib.na1d_sink_saved_bytes.argtypes = lib.na1d_sink_backward_workspace_bytes.argtypes = [_ptr]
+    lib.na1d_sink_forward.restype = lib.na1d_sink_backward.restype = _int
+    lib.na1d_sink_forward.argtypes = [_ptr] * 3 + [_i64] + [_ptr] * 5
+    lib.na1d_sink_backward.argtypes = [_ptr] * 10 + [_i64, _ptr, _ptr, _i64, _ptr]
     lib.na1d_fused_backward_noalloc.restype = _int
     lib.na1d_fused_backward_noalloc.argtypes = [_ptr] * 12 + [_i64] * 6 + [_f32, _int, _ptr]
     lib.na1d_force_generic.restype = _int
