@@ -467,6 +467,40 @@ int na1d_sink_backward(const na1d_sink *h, void *dq, void *dk, void *dv, const v
                        const void *saved, int64_t saved_bytes, const int32_t *t_valid, void *workspace, int64_t workspace_bytes, void *stream);
 
 /*
+ * A cache of what a window with sinks can see, for streams that go on a few tokens at a time.  Position p of a sequence is in row p where
+ * p < sinks, else in row sinks + (p - sinks) mod (capacity - sinks).  lengths [N]: tokens that the sequences have seen; a negative number, or more
+ * than 2^30, marks an idle one, whose rows stay as they are and whose output is 0.
+ *   bits 16: k, v [N, kv_heads, capacity, head_dim] of `dtype`, ranges NULL
+ *   bits 4 : k, v [N, kv_heads, capacity, head_dim / 2], byte i of a row holds channel 2 i in its low four bits and 2 i + 1 in its high ones;
+ *            ranges [N, kv_heads, capacity, 2] of `dtype`: a row's step and its least value.  A code c stands for least + step * c;
+ *            step = (largest - least) / 15 rounded to `dtype`, c = (x - least) / step in fp32, rounded to the nearest of 0 .. 15
+ *            (0 where the step is 0).  head_dim is 32, 64, 96 or 128.  Rows have to be finite, largest - least within fp32.
+ * append: tokens [N, T, kv_heads, head_dim] of k and v become positions lengths[n] .. lengths[n] + t_valid[n] - 1 (lengths NULL: from 0 on,
+ *   t_valid NULL: all T); of those only sinks and the last capacity - sinks are kept.
+ * attend: the `fresh` newest tokens of each sequence, q [N, fresh, heads, head_dim], out alike and packed, attend to the tokens that they see (as
+ *   in na1d_sink_forward), the first of them at lengths[n] - fresh (a token before position 0 has output 0).  They are in the cache already.
+ * step: the same for tokens that are not: k, v [N, fresh, kv_heads, head_dim] become positions lengths[n] .. lengths[n] + fresh - 1 and are
+ *   attended to as the cache holds them.
+ * Strides as in na1d_sink.  capacity - sinks >= window + fresh - 1 (NA1D_ERR_WINDOW).  capacity * head_dim up to 2^29, N * kv_heads to 2^24,
+ * fresh * heads / kv_heads to 2^20 (NA1D_ERR_UNSUPPORTED).  All pointers but lengths and t_valid 16-byte aligned.  A workspace is needed where
+ * na1d_sink_attend_workspace_bytes() is above 0.  rows: what `rows` rows of codes stand for, in `dtype`.
+ */
+typedef struct na1d_sink_cache {
+    int32_t dtype, bits, kv_heads, head_dim;
+    int64_t N, capacity, sinks;
+    void *k, *v, *k_ranges, *v_ranges;
+} na1d_sink_cache;
+int64_t na1d_sink_attend_workspace_bytes(const na1d_sink_cache *c, int64_t fresh, int64_t heads, int64_t window);
+int na1d_sink_append(const na1d_sink_cache *c, const void *k, const void *v, const int64_t k_strides[3], const int64_t v_strides[3], const int32_t *lengths,
+                     const int32_t *t_valid, int64_t T, void *stream);
+int na1d_sink_attend(const na1d_sink_cache *c, void *out, const void *q, const int64_t q_strides[3], const int32_t *lengths, int64_t fresh, int64_t heads, int64_t window,
+                     float scale, void *workspace, int64_t workspace_bytes, void *stream);
+int na1d_sink_step(const na1d_sink_cache *c, void *out, const void *q, const void *k, const void *v, const int64_t q_strides[3], const int64_t k_strides[3],
+                   const int64_t v_strides[3], const int32_t *lengths, int64_t fresh, int64_t heads, int64_t window, float scale, void *workspace, int64_t workspace_bytes,
+                   void *stream);
+int na1d_sink_rows(void *out, const void *codes, const void *ranges, int64_t rows, int64_t head_dim, int dtype, void *stream);
+
+/*
  * Profiling hook; no counterpart in the reference.  From this call on, the matrix-core fused kernels that the
  * CALLING THREAD launches record `start` just before and `stop` just after the kernel itself (hipEvent_t handles,
  * recorded by hipExtLaunchKernel: the dispatch's own begin and end, i.e. what a profiler's kernel trace reports,

@@ -72,3 +72,40 @@ def attention(q, k, v, window, sinks=0, t_valid=None, scale=None, dout=None):
     if dout is not None:
         times["dv"] = 1 + T * H * most(g)
     return {n: (a.transpose(1, 2), (b + least * times[n]).transpose(1, 2)) for n, (a, b) in got.items()}
+
+
+def in_4_bits(x):
+    """Rows as a cache in 4 bits holds them: codes, step and least value (as fp32 steps of the stated arithmetic), and the values in 64 bits."""
+    low, high = x.amin(-1, keepdim=True), x.amax(-1, keepdim=True)
+    step = ((high.float() - low.float()) / 15).to(x.dtype)
+    code = torch.where(step > 0, torch.round((x.float() - low.float()) / step.float()).clamp(0, 15), 0.0)
+    return code, step, low, low.double() + code.double() * step.double()
+
+
+def over_history(q, k, v, window, sinks, ends, scale=None, four=False):
+    """The last tokens `q [N, n, H, C]` of sequences whose tokens have been `k[i], v[i] [>= ends[i], K, C]`: (value, how far a kernel's may be off).
+
+    p is rounded where it meets v, in 16 bits (u sum p |v|); rows in 4 bits have p times the step rounded, which meets a code less 7.5
+    (u sum p 7.5 step), and their scores and sums are made of parts up to 31 steps and |least| in size (fp32, counted in f)."""
+    N, n, H, C = q.shape
+    u, scale = half_step(q.dtype), C ** -0.5 if scale is None else scale
+    out, bound = torch.zeros(q.shape, dtype=torch.float64, device=q.device), torch.zeros(q.shape, dtype=torch.float64, device=q.device)
+    for i in range(N):
+        end = max(0, int(ends[i]))
+        t = torch.arange(end - n, end, device=q.device)
+        at = torch.arange(end, device=q.device)
+        seen = visible(t, at, window, sinks)
+        if end == 0:
+            continue
+        values = lambda x: in_4_bits(x[:end])[3] if four else x[:end].double()  # noqa: E731
+        wide = lambda x: (lambda c, s, low, _: 31 * s.double() + low.double().abs())(*in_4_bits(x[:end])).expand(x[:end].shape) if four else x[:end].double().abs()  # noqa: E731
+        heads = lambda x: x.transpose(0, 1).repeat_interleave(H // x.shape[1], 0)  # noqa: E731
+        qi = q[i].double().transpose(0, 1)
+        p = softmax_rows(qi @ heads(values(k[i])).transpose(-1, -2) * scale, seen)
+        o = p @ heads(values(v[i]))
+        f = FP32 * (1 + (qi.abs() @ heads(wide(k[i])).transpose(-1, -2) * scale).amax().item())
+        rounded = heads((7.5 * in_4_bits(v[i][:end])[1].double()).expand(v[i][:end].shape)) if four else heads(values(v[i]).abs())
+        out[i] = o.transpose(0, 1)
+        bound[i] = (u * o.abs() + u * (p @ rounded) + f * (p @ heads(wide(v[i])))).transpose(0, 1)
+    least = 2.0 ** -25 if q.dtype == torch.float16 else 2.0 ** -126
+    return out, bound + least * (1 + 16 * sum(x.shape[0] for x in v))

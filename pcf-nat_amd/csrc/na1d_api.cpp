@@ -610,6 +610,12 @@ int na1d_head_backward(const na1d_head *h, void *dx, void *dw, const float *dlos
     return na1d::loss::run_backward(*h, dx, dw, dloss, x, w, ids, saved, workspace, (hipStream_t)stream);
 }
 
+static int strides_check(const int64_t *s, int64_t head_dim) {
+    if (!s) return NA1D_ERR_NULL;
+    if (s[0] < 0 || s[1] < 0 || s[2] < head_dim) return NA1D_ERR_SHAPE;
+    if (s[0] % 8 || s[1] % 8 || s[2] % 8) return NA1D_ERR_ALIGN;
+    return s[0] > (1ll << 44) || s[1] > (1ll << 40) || s[2] > (1ll << 20) ? NA1D_ERR_UNSUPPORTED : NA1D_OK;
+}
 // +1: nothing to do
 static int sink_check(const na1d_sink *h) {
     if (!h) return NA1D_ERR_NULL;
@@ -621,11 +627,8 @@ static int sink_check(const na1d_sink *h) {
     const int64_t widest = 1 << 20;
     if (h->head_dim > 128 || h->T > (1 << 24) || (int64_t)h->heads * h->head_dim > widest) return NA1D_ERR_UNSUPPORTED;
     if (h->N > (1ll << 36) / h->heads / (h->T > 0 ? h->T : 1)) return NA1D_ERR_UNSUPPORTED;
-    for (const int64_t *s : {h->q_strides, h->k_strides, h->v_strides}) {
-        if (s[0] < 0 || s[1] < 0 || s[2] < h->head_dim) return NA1D_ERR_SHAPE;
-        if (s[0] % 8 || s[1] % 8 || s[2] % 8) return NA1D_ERR_ALIGN;
-        if (s[2] > widest || s[1] > (1ll << 40) || s[0] > (1ll << 44)) return NA1D_ERR_UNSUPPORTED;
-    }
+    for (const int64_t *s : {h->q_strides, h->k_strides, h->v_strides})
+        if (const int bad = strides_check(s, h->head_dim)) return bad;
     return h->N == 0 || h->T == 0;
 }
 int64_t na1d_sink_saved_bytes(const na1d_sink *h) {
@@ -655,6 +658,76 @@ int na1d_sink_backward(const na1d_sink *h, void *dq, void *dk, void *dv, const v
     }
     if (saved_bytes < na1d::mfma::sink_saved_bytes(*h) || workspace_bytes < na1d::mfma::sink_bwd_workspace_bytes(*h)) return NA1D_ERR_WORKSPACE;
     return na1d::mfma::sink_bwd(*h, dq, dk, dv, q, k, v, out, dout, (const float *)saved, t_valid, (float *)workspace, (hipStream_t)stream);
+}
+
+// +1: nothing to do
+static int cache_check(const na1d_sink_cache *c, int64_t fresh, int64_t heads, int64_t window) {
+    if (!c) return NA1D_ERR_NULL;
+    if (c->dtype != NA1D_BF16 && c->dtype != NA1D_FP16) return NA1D_ERR_DTYPE;
+    if (c->bits != 4 && c->bits != 16) return NA1D_ERR_DTYPE;
+    if (c->head_dim < 1 || c->head_dim % (c->bits == 4 ? 32 : 8)) return NA1D_ERR_HEAD_DIM;
+    if (c->N < 0 || fresh < 0 || c->kv_heads < 1 || heads < 1 || heads % c->kv_heads) return NA1D_ERR_SHAPE;
+    const int64_t most = 1ll << 29;
+    if (c->head_dim > 128 || c->capacity > most / c->head_dim || c->N > (1 << 24) / c->kv_heads || fresh > (1 << 20) / (heads / c->kv_heads)) return NA1D_ERR_UNSUPPORTED;
+    if (window < 1 || c->sinks < 0 || c->sinks >= c->capacity || window > c->capacity - c->sinks - (fresh > 0 ? fresh - 1 : 0)) return NA1D_ERR_WINDOW;
+    return c->N == 0 || fresh == 0;
+}
+static int cache_pointers(const na1d_sink_cache *c) {
+    if (!c->k || !c->v || (c->bits == 4 && (!c->k_ranges || !c->v_ranges))) return NA1D_ERR_NULL;
+    return misaligned(c->k) || misaligned(c->v) || (c->bits == 4 && (misaligned(c->k_ranges) || misaligned(c->v_ranges))) ? NA1D_ERR_ALIGN : NA1D_OK;
+}
+int64_t na1d_sink_attend_workspace_bytes(const na1d_sink_cache *c, int64_t fresh, int64_t heads, int64_t window) {
+    const int st = cache_check(c, fresh, heads, window);
+    return st == NA1D_OK ? na1d::mfma::cache_attend_workspace_bytes(*c, fresh, (int)heads, window) : st > 0 ? 0 : st;
+}
+int na1d_sink_append(const na1d_sink_cache *c, const void *k, const void *v, const int64_t k_strides[3], const int64_t v_strides[3], const int32_t *lengths,
+                     const int32_t *t_valid, int64_t T, void *stream) {
+    const int st = cache_check(c, 1, c ? c->kv_heads : 1, 1);
+    if (st < 0) return st;
+    if (T < 0) return NA1D_ERR_SHAPE;
+    if (st > 0 || T == 0) return NA1D_OK;
+    if (T > (1 << 24)) return NA1D_ERR_UNSUPPORTED;
+    if (!k || !v) return NA1D_ERR_NULL;
+    for (const int bad : {cache_pointers(c), strides_check(k_strides, c->head_dim), strides_check(v_strides, c->head_dim)})
+        if (bad) return bad;
+    if (misaligned(k) || misaligned(v)) return NA1D_ERR_ALIGN;
+    return na1d::mfma::cache_append(*c, k, v, k_strides, v_strides, lengths, t_valid, T, (hipStream_t)stream);
+}
+static int cache_call(const na1d_sink_cache *c, void *out, const void *q, const void *k, const void *v, const int64_t *q_strides, const int64_t *k_strides,
+                      const int64_t *v_strides, const int32_t *lengths, int64_t fresh, int64_t heads, int64_t window, float scale, void *workspace,
+                      int64_t workspace_bytes, void *stream, bool stores) {
+    const int st = cache_check(c, fresh, heads, window);
+    if (st < 0) return st;
+    if (bad_scale(scale)) return NA1D_ERR_SCALE;
+    if (st > 0) return NA1D_OK;
+    if (!out || !q || !lengths || (stores && (!k || !v))) return NA1D_ERR_NULL;
+    for (const int bad : {cache_pointers(c), strides_check(q_strides, c->head_dim), stores ? strides_check(k_strides, c->head_dim) : 0,
+                          stores ? strides_check(v_strides, c->head_dim) : 0})
+        if (bad) return bad;
+    if (misaligned(out) || misaligned(q) || misaligned(k) || misaligned(v) || misaligned(workspace)) return NA1D_ERR_ALIGN;
+    const int64_t need = na1d::mfma::cache_attend_workspace_bytes(*c, fresh, (int)heads, window);
+    if (need > 0 && !workspace) return NA1D_ERR_NULL;
+    if (workspace_bytes < need) return NA1D_ERR_WORKSPACE;
+    return na1d::mfma::cache_attend(*c, out, q, k, v, q_strides, k_strides, v_strides, lengths, fresh, (int)heads, window, scale, (float *)workspace, (hipStream_t)stream);
+}
+int na1d_sink_attend(const na1d_sink_cache *c, void *out, const void *q, const int64_t q_strides[3], const int32_t *lengths, int64_t fresh, int64_t heads, int64_t window,
+                     float scale, void *workspace, int64_t workspace_bytes, void *stream) {
+    return cache_call(c, out, q, nullptr, nullptr, q_strides, nullptr, nullptr, lengths, fresh, heads, window, scale, workspace, workspace_bytes, stream, false);
+}
+int na1d_sink_step(const na1d_sink_cache *c, void *out, const void *q, const void *k, const void *v, const int64_t q_strides[3], const int64_t k_strides[3],
+                   const int64_t v_strides[3], const int32_t *lengths, int64_t fresh, int64_t heads, int64_t window, float scale, void *workspace, int64_t workspace_bytes,
+                   void *stream) {
+    return cache_call(c, out, q, k, v, q_strides, k_strides, v_strides, lengths, fresh, heads, window, scale, workspace, workspace_bytes, stream, true);
+}
+int na1d_sink_rows(void *out, const void *codes, const void *ranges, int64_t rows, int64_t head_dim, int dtype, void *stream) {
+    if (dtype != NA1D_BF16 && dtype != NA1D_FP16) return NA1D_ERR_DTYPE;
+    if (head_dim < 1 || head_dim % 32) return NA1D_ERR_HEAD_DIM;
+    if (head_dim > 128 || rows > (1ll << 44)) return NA1D_ERR_UNSUPPORTED;
+    if (rows < 0) return NA1D_ERR_SHAPE;
+    if (rows == 0) return NA1D_OK;
+    if (!out || !codes || !ranges) return NA1D_ERR_NULL;
+    if (misaligned(out) || misaligned(codes) || misaligned(ranges)) return NA1D_ERR_ALIGN;
+    return na1d::mfma::cache_rows(out, codes, ranges, rows, (int)head_dim, dtype, (hipStream_t)stream);
 }
 
 int na1d_fused_backward_noalloc(void *dq, void *dk, void *dv, float *drpb, const void *q, const void *k, const void *v,

@@ -241,13 +241,20 @@ int run_forward(const na1d_head &h, float *loss, uint8_t *hits, const void *x, c
 int run_backward(const na1d_head &h, void *dx, void *dw, const float *dloss, const void *x, const void *w, const void *ids, const void *saved, void *ws, hipStream_t s);
 }  // namespace loss
 
-// ---- windowed causal attention with sinks: na1d_sink.hip ------------------
+// ---- windowed causal attention with sinks: na1d_sink.hip; over a cache: na1d_cache.hip ------------------
 namespace mfma {
 int64_t sink_saved_bytes(const na1d_sink &h);
 int64_t sink_bwd_workspace_bytes(const na1d_sink &h);
 int sink_fwd(const na1d_sink &h, void *out, float *saved, const void *q, const void *k, const void *v, const int32_t *t_valid, hipStream_t s);
 int sink_bwd(const na1d_sink &h, void *dq, void *dk, void *dv, const void *q, const void *k, const void *v, const void *out, const void *dout, const float *saved,
              const int32_t *t_valid, float *ws, hipStream_t s);
+int64_t cache_attend_workspace_bytes(const na1d_sink_cache &c, int64_t fresh, int heads, int64_t window);
+// `k` (and v) NULL: the call's tokens are in the cache
+int cache_attend(const na1d_sink_cache &c, void *out, const void *q, const void *k, const void *v, const int64_t *q_strides, const int64_t *k_strides, const int64_t *v_strides,
+                 const int32_t *lengths, int64_t fresh, int heads, int64_t window, float scale, float *ws, hipStream_t s);
+int cache_append(const na1d_sink_cache &c, const void *k, const void *v, const int64_t *k_strides, const int64_t *v_strides, const int32_t *lengths, const int32_t *t_valid, int64_t T,
+                 hipStream_t s);
+int cache_rows(void *out, const void *codes, const void *ranges, int64_t rows, int head_dim, int dtype, hipStream_t s);
 }  // namespace mfma
 
 }  // namespace na1d

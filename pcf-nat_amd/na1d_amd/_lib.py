@@ -33,6 +33,7 @@ SYMBOLS = _UNFUSED + ("na1d_fused_forward", "na1d_fused_backward", "na1d_fused_b
                       "na1d_train_to_channels", "na1d_train_pool_backward", "na1d_train_context_backward", "na1d_train_context",
                       "na1d_train_layer_backward", "na1d_head_saved_bytes", "na1d_head_workspace_bytes", "na1d_head_forward",
                       "na1d_head_backward", "na1d_sink_saved_bytes", "na1d_sink_backward_workspace_bytes", "na1d_sink_forward", "na1d_sink_backward",
+                      "na1d_sink_attend_workspace_bytes", "na1d_sink_append", "na1d_sink_attend", "na1d_sink_step", "na1d_sink_rows",
                       "na1d_version", "na1d_status_string")
 UNSUPPORTED = -8
 
@@ -126,6 +127,13 @@ def load():
     lib.na1d_sink_forward.restype = lib.na1d_sink_backward.restype = _int
     lib.na1d_sink_forward.argtypes = [_ptr] * 3 + [_i64] + [_ptr] * 5
     lib.na1d_sink_backward.argtypes = [_ptr] * 10 + [_i64, _ptr, _ptr, _i64, _ptr]
+    lib.na1d_sink_attend_workspace_bytes.restype = _i64
+    lib.na1d_sink_attend_workspace_bytes.argtypes = [_ptr] + [_i64] * 3
+    lib.na1d_sink_append.restype = lib.na1d_sink_attend.restype = lib.na1d_sink_step.restype = lib.na1d_sink_rows.restype = _int
+    lib.na1d_sink_append.argtypes = [_ptr] * 7 + [_i64, _ptr]
+    lib.na1d_sink_attend.argtypes = [_ptr] * 5 + [_i64] * 3 + [_f32, _ptr, _i64, _ptr]
+    lib.na1d_sink_step.argtypes = [_ptr] * 9 + [_i64] * 3 + [_f32, _ptr, _i64, _ptr]
+    lib.na1d_sink_rows.argtypes = [_ptr] * 3 + [_i64] * 2 + [_int, _ptr]
     lib.na1d_fused_backward_noalloc.restype = _int
     lib.na1d_fused_backward_noalloc.argtypes = [_ptr] * 12 + [_i64] * 6 + [_f32, _int, _ptr]
     lib.na1d_force_generic.restype = _int

@@ -109,3 +109,114 @@ def test_the_oracle_agrees_with_automatic_differentiation():
     got = O.attention(*[x.detach() for x in (q, k, v)], 5, 2, t_valid=lengths, dout=dout)
     for name, want in zip(("out", "dq", "dk", "dv"), (o,) + grads):
         assert torch.allclose(got[name][0], want, atol=1e-12), name
+
+
+# ------------------------------------------------------------------------------------------------ caches
+def _caches(bits=16, N=2, K=2, S=20, C=32, dtype=torch.bfloat16, device="meta"):
+    return streaming.new_cache(N, K, S, C, bits, dtype, device)
+
+
+def _call(q=None, k=None, v=None, caches=None, lengths=None, window=8, sinks=1, bits=16):
+    tokens = _on("meta", T=3, C=32)
+    q, k, v = (given if given is not None else x for given, x in zip((q, k, v), tokens))
+    caches = _caches(bits) if caches is None else caches
+    lengths = torch.zeros(2, dtype=torch.int32, device="meta") if lengths is None else lengths
+    return streaming.cache_step(q, k, v, *caches, lengths, window, sinks)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_caches_and_tokens_that_do_not_fit(bits):
+    meta = lambda *s, dtype=torch.bfloat16: torch.empty(*s, dtype=dtype, device="meta")  # noqa: E731
+    with pytest.raises(_lib.NA1DError, match="no CPU path"):        # everything but the device is right
+        _call(bits=bits)
+    for wrong, error in ((dict(q=meta(2, 3, 3, 32)), ValueError), (dict(q=meta(2, 2, 4, 32)), ValueError), (dict(k=meta(2, 3, 4, 32)), ValueError),
+                         (dict(v=meta(2, 4, 2, 32)), ValueError), (dict(k=meta(1, 3, 2, 32)), ValueError), (dict(q=meta(2, 3, 4, 64)), ValueError),
+                         (dict(q=meta(2, 3, 4, 32, dtype=torch.float16)), TypeError), (dict(k=torch.empty(2, 3, 2, 32, dtype=torch.bfloat16)), _lib.NA1DError),
+                         (dict(lengths=meta(2, dtype=torch.int64)), ValueError), (dict(lengths=meta(3, dtype=torch.int32)), ValueError),
+                         (dict(lengths=torch.zeros(2, dtype=torch.int32)), _lib.NA1DError), (dict(window=0), _lib.NA1DError), (dict(window=18), _lib.NA1DError),
+                         (dict(sinks=20, window=1), _lib.NA1DError), (dict(sinks=11), _lib.NA1DError), (dict(caches=(_caches(bits)[0], _caches(20 - bits)[1])), ValueError),
+                         (dict(caches=(_caches(bits)[0], _caches(bits, S=21)[1])), ValueError), (dict(caches=(_caches(bits)[0], _caches(bits, dtype=torch.float16)[1])), ValueError),
+                         (dict(caches=_caches(bits, K=0)), _lib.NA1DError)):
+        with pytest.raises(error):
+            _call(bits=bits, **wrong)
+    with pytest.raises(_lib.NA1DError, match="no CPU path"):
+        _call(bits=bits, window=17)                                 # 1 sink, 17, 2 more for three tokens at a time
+    with pytest.raises(ValueError, match="cache_attend"):
+        streaming.cache_step(_on("meta", C=32)[0], None, None, *_caches(bits), None, 4)
+    with pytest.raises(ValueError, match="lengths"):
+        streaming.cache_attend(_on("meta", T=3, C=32)[0], *_caches(bits), None, 4)
+
+
+def test_caches_that_cannot_be_written_to():
+    k, v = _caches(device="cpu")
+    with pytest.raises(_lib.NA1DError, match="contiguous"):
+        streaming._check_caches(k.transpose(1, 2), v.transpose(1, 2), 0)
+    with pytest.raises(_lib.NA1DError, match="aligned"):
+        streaming._check_caches(torch.zeros(k.numel() + 1, dtype=k.dtype)[1:].view(k.shape), v, 0)
+    with pytest.raises(_lib.NA1DError, match="gradient"):
+        streaming._check_caches(k.requires_grad_(True), v, 0)
+    codes, ranges = _caches(4, device="cpu")[0]
+    for bad in (streaming.Rows4(codes.to(torch.int8), ranges), streaming.Rows4(codes, ranges[..., :1]), streaming.Rows4(codes[0], ranges)):
+        with pytest.raises(ValueError):
+            streaming.cache_rows(bad)
+    with pytest.raises(_lib.NA1DError, match="head_dim"):
+        streaming.cache_rows(streaming.Rows4(codes[..., :10].contiguous(), ranges))
+    for bits, C in ((4, 40), (4, 256), (8, 64)):
+        with pytest.raises(_lib.NA1DError, match="bits"):
+            _caches(bits, C=C)
+
+
+def _native_cache(**kw):
+    args = dict(dtype=0, bits=16, kv_heads=2, head_dim=64, N=2, capacity=100, sinks=4, k=16, v=16, k_ranges=16, v_ranges=16)
+    args.update(kw)
+    return streaming._Cache(**args)
+
+
+@pytest.mark.parametrize("change,call,status", [
+    (dict(dtype=2), {}, -2), (dict(bits=8), {}, -2), (dict(head_dim=60), {}, -3), (dict(head_dim=136), {}, -8), (dict(bits=4, head_dim=40), {}, -3), (dict(N=-1), {}, -5),
+    (dict(kv_heads=0), {}, -5), ({}, dict(heads=3), -5), ({}, dict(fresh=-1), -5), (dict(sinks=100), {}, -4), (dict(sinks=-1), {}, -4), ({}, dict(window=0), -4),
+    ({}, dict(window=97), -4), ({}, dict(window=95, fresh=3), -4), (dict(capacity=(1 << 23) + 1), {}, -8), (dict(N=1 << 24), {}, -8), ({}, dict(fresh=1 << 20), -8)])
+def test_native_caches_refuse(change, call, status):
+    lib, c = _lib.load(), _native_cache(**change)
+    a = dict(fresh=1, heads=4, window=96)
+    a.update(call)
+    s = (ctypes.c_int64 * 3)(256, 64, 256)
+    ref = ctypes.byref(c)
+    assert lib.na1d_sink_attend_workspace_bytes(ref, a["fresh"], a["heads"], a["window"]) == status
+    assert lib.na1d_sink_attend(ref, 16, 16, s, 16, a["fresh"], a["heads"], a["window"], 0.1, 16, 1 << 40, None) == status
+    assert lib.na1d_sink_step(ref, 16, 16, 16, 16, s, s, s, 16, a["fresh"], a["heads"], a["window"], 0.1, 16, 1 << 40, None) == status
+    if not call:
+        assert lib.na1d_sink_append(ref, 16, 16, s, s, None, None, 5, None) == status
+
+
+def test_native_caches_ask_for_their_pointers():
+    lib, s = _lib.load(), (ctypes.c_int64 * 3)(256, 64, 256)
+    step = lambda c, *a: lib.na1d_sink_step(ctypes.byref(c), *a)  # noqa: E731
+    good = [16, 16, 16, 16, s, s, s, 16, 1, 4, 96, 0.1, 16, 1 << 40, None]
+    for i in (0, 1, 2, 3, 4, 5, 6, 7):
+        assert step(_native_cache(), *good[:i], None, *good[i + 1:]) == -1, i
+    for name in ("k", "v"):
+        assert step(_native_cache(**{name: None}), *good) == -1
+        assert step(_native_cache(**{name: 8}), *good) == -6
+        assert step(_native_cache(bits=4, **{name + "_ranges": None}), *good) == -1
+        assert step(_native_cache(bits=4, **{name + "_ranges": 8}), *good) == -6
+    for i in (0, 1, 2, 3):
+        assert step(_native_cache(), *good[:i], 24, *good[i + 1:]) == -6
+    for scale in (0.0, -1.0, float("nan"), float("inf")):
+        assert step(_native_cache(), *good[:11], scale, *good[12:]) == -11
+    for bad, status in (((256, 64, 56), -5), ((256, 64, 68), -6), ((-8, 64, 256), -5), ((256, 64, 1 << 21), -8)):
+        for i in (4, 5, 6):
+            assert step(_native_cache(), *good[:i], (ctypes.c_int64 * 3)(*bad), *good[i + 1:]) == status
+    long = _native_cache(capacity=5000)
+    need = lib.na1d_sink_attend_workspace_bytes(ctypes.byref(long), 1, 4, 4000)
+    assert need > 0
+    args = good[:8] + [1, 4, 4000, 0.1]
+    assert step(long, *args, 16, need - 1, None) == -10 and step(long, *args, None, need, None) == -1
+    assert step(_native_cache(N=0), *[None] * 4, s, s, s, None, 1, 4, 96, 0.1, None, 0, None) == 0
+    for a, status in (((16, 16, 16, 5, 60, 0), -3), ((16, 16, 16, 5, 64, 2), -2), ((16, 16, 16, -1, 64, 0), -5), ((None, 16, 16, 5, 64, 0), -1), ((16, 8, 16, 5, 64, 0), -6),
+                      ((16, 16, 16, 5, 160, 0), -8), ((None, None, None, 0, 64, 0), 0)):
+        assert lib.na1d_sink_rows(*a, None) == status
+    assert lib.na1d_sink_append(ctypes.byref(long), 16, 16, s, s, None, None, -1, None) == -5
+    assert lib.na1d_sink_append(ctypes.byref(long), 16, 16, s, s, None, None, (1 << 24) + 1, None) == -8
+    assert lib.na1d_sink_append(ctypes.byref(long), None, 16, s, s, None, None, 5, None) == -1
+    assert lib.na1d_sink_append(ctypes.byref(long), 16, 16, s, None, None, None, 5, None) == -1
