@@ -33,8 +33,8 @@ struct SinkArgs {
     float scale;
     SinkRows q, k, v, o;        // o: out and dout, and dq
     SinkRows dkv;               // dk and dv
-    // dK and dV: strips that hold sinks are shared by sink_parts workgroups, the others by parts; their sums go to `partial`
-    int sink_strips, sink_parts, parts;
+    // dK and dV (see there): strips of all heads up to `whole` have a workgroup each, the others `parts`; strips that hold sinks have `far` more
+    int whole, parts, sink_strips, sink_rows, far;
 };
 
 struct SinkItem {
@@ -414,15 +414,28 @@ sink_dq_kernel(char *__restrict__ dq, float *__restrict__ delta, const char *__r
 // =============================================================================
 // Backward, key side: dV = P^T dO and dK = scale * dS^T Q, summed over the heads of the group
 // =============================================================================
-// A workgroup owns a strip of keys, whose K and V rows stay in registers, and walks units of (head of the group, chunk of 64
-// queries): Q and dO through LDS, double-buffered.  The score product is taken with Q and K swapped, so that P and dS come out as
-// B operands.  Sinks are seen by all the queries behind them, other keys by a window of them: strips that hold sinks are shared by more
-// workgroups, which add up in fp32 through `partial` in a fixed order (sink_join_kernel).
-template <class DT, int C, int QT>
+// A workgroup owns a strip of 64 keys, a tile of them to a wave, whose K and V rows stay in registers, and walks units of (head of the group, chunk
+// of 64 queries): Q and dO through LDS, double-buffered.  The score product is taken with Q and K swapped, so that P and dS come out as B operands.
+// What bounds it is LDS: 64 KB of operands to a wave and unit.  Two tiles of keys to a wave would halve that, and need 308 registers at 128 channels, so
+// one wave to a SIMD: 2 x 8192 tokens, 16 heads of 128 over 4, window 1024 took 510 us in place of 435; at 64 channels 81 in place of 60 (16 x
+// 16 x 1000, window 128).
+//
+// A launch ends when its last workgroup does, so it is cut to fit the card: strips beyond a whole number of rounds of it are shared by `parts` workgroups
+// each.  Sinks are seen by all queries behind them, other keys by a window of them: the queries that see of a strip nothing but its sinks are left to
+// `far` workgroups.  What several workgroups have a share in they leave in fp32 in `partial`, and sink_join_kernel adds it up in a fixed order.
+struct Partial {                // floats from the start of `partial`: [parts of a shared strip][dk, dv][64][C], and twice [..][dk, dv][sink_rows][C]
+    int64_t shared, near, far;
+};
+template <int C> __device__ inline Partial partial_of(int64_t strip_id, int part, int64_t sink_strip, int far, int64_t heads, const SinkArgs &a) {
+    const int64_t shared_size = (heads * a.strips - a.whole) * a.parts * (2 * kChunkRows * C), slot = 2 * a.sink_rows * C;
+    return Partial{((strip_id - a.whole) * a.parts + part) * (2 * kChunkRows * C), shared_size + sink_strip * slot,
+                   shared_size + (heads * a.sink_strips + sink_strip * a.far + far) * slot};
+}
+template <class DT, int C>
 __global__ void __launch_bounds__(kThreads)
 sink_dkv_kernel(char *__restrict__ dk, char *__restrict__ dv, float *__restrict__ partial, const char *__restrict__ q, const char *__restrict__ k,
                 const char *__restrict__ v, const char *__restrict__ dout, const float *__restrict__ lse, const float *__restrict__ delta,
-                const int32_t *__restrict__ t_valid, uint32_t items, SinkArgs a) {
+                const int32_t *__restrict__ t_valid, uint32_t rest, uint32_t heads, SinkArgs a) {
     using LL = Lds<C>;
     constexpr int CT = C / 16, kStep = region_bytes<C>(kChunkTiles), kBuf = 2 * kStep + 2 * kChunkRows * 4;
     extern __shared__ __attribute__((aligned(16))) char smem[];          // 2 * kBuf bytes: Q, dO and the rows' constants of two chunks
@@ -431,23 +444,39 @@ sink_dkv_kernel(char *__restrict__ dk, char *__restrict__ dv, float *__restrict_
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, n = lane & 15;
-    // work items of a key head: the strips with sinks, sink_parts to each, then the others, parts to each
-    const uint32_t lin = xcd_item(blockIdx.x, items), sink_items = a.sink_strips * a.sink_parts;
-    const uint32_t per_head = sink_items + (a.strips - a.sink_strips) * a.parts;
-    const uint32_t sh = uniform(lin / per_head), rest = lin - sh * per_head, sample = uniform(sh / (uint32_t)a.K), kv = sh - sample * a.K;
-    const bool of_sinks = rest < sink_items;
-    const uint32_t each = of_sinks ? a.sink_parts : a.parts, r_in = of_sinks ? rest : rest - sink_items;
-    const int strip = uniform((int)(r_in / each)) + (of_sinks ? 0 : a.sink_strips), part = uniform((int)(r_in % each));
+    // strips with a workgroup of their own; then (`rest` of them) the parts of the others, and the far workgroups
+    uint32_t strip_id, part = 0, each = 1, head, strip;
+    bool far = false;
+    if (blockIdx.x < (uint32_t)a.whole) {
+        strip_id = xcd_item(blockIdx.x, a.whole);
+    } else {
+        const uint32_t lin = xcd_item(blockIdx.x - a.whole, rest), shared = (heads * a.strips - a.whole) * a.parts;
+        far = lin >= shared;
+        each = far ? a.far : a.parts;
+        const uint32_t i = far ? lin - shared : lin;
+        strip_id = uniform(i / each);
+        part = i - strip_id * each;
+        if (!far) strip_id += a.whole;
+    }
+    head = uniform(strip_id / (uint32_t)(far ? a.sink_strips : a.strips));
+    strip = strip_id - head * (far ? a.sink_strips : a.strips);
+    const uint32_t sample = uniform(head / (uint32_t)a.K), kv = head - sample * a.K;
     const int T = a.T, width = a.width;
     int tv = T;
     if (t_valid) tv = uniform(max(0, min(T, t_valid[sample])));
-    const int row0 = strip * (kChunkRows * QT), row_end = min(T, row0 + kChunkRows * QT);
-    // chunks of queries that see something of the strip
+    const int row0 = strip * kChunkRows, row_end = min(T, row0 + kChunkRows);
+    // chunks of queries that see something of the strip: [c_from, c_near) its windows, [c_near, c_end) its sinks
     const int last_key = min(row_end, tv) - 1;
     int c_from = row0 / kChunkRows, c_end = c_from;
-    if (last_key >= row0) c_end = (int)min((int64_t)tv - 1, row0 < a.sinks ? (int64_t)tv - 1 : (int64_t)last_key + a.window - 1) / kChunkRows + 1;
-    const int nc = c_end - c_from;
-    const int units = nc * a.group, u_end = uniform((int)((int64_t)units * (part + 1) / each));
+    if (last_key >= row0) {
+        const int chunks = (tv - 1) / kChunkRows + 1, near = (int)min((int64_t)chunks, ((int64_t)last_key + a.window - 1) / kChunkRows + 1);
+        if (far) {
+            c_from = near, c_end = chunks;
+        } else {
+            c_end = row0 < a.sinks && !a.far ? chunks : near;
+        }
+    }
+    const int nc = c_end - c_from, units = nc * a.group, u_end = uniform((int)((int64_t)units * (part + 1) / each));
     int u = uniform((int)((int64_t)units * part / each));
     int hg = nc ? uniform(u / nc) : 0, c = nc ? c_from + u - hg * nc : 0;
 
@@ -455,34 +484,30 @@ sink_dkv_kernel(char *__restrict__ dk, char *__restrict__ dv, float *__restrict_
     const char *qb = q + sample * a.q.sample, *gb = dout + sample * a.o.sample;
     float row_lse, row_delta;                             // of row 16 * wave + n of the chunk in flight
     auto stage = [&](int hg_, int c_, LDS_PTR(char) to) {
-        const int head = kv * a.group + hg_, rows = min(kChunkRows, tv - c_ * kChunkRows);
-        const int64_t r0 = (int64_t)c_ * kChunkRows, stat = ((int64_t)sample * a.H + head) * T + r0;
-        stage_direct<C, kChunkTiles, kReadShared>(rows_of(qb + head * a.q.head, r0, rows, a.q.pitch), 0, to, kChunkTiles, wave, q_lane, a.q.pitch);
-        stage_direct<C, kChunkTiles, kReadShared>(rows_of(gb + head * a.o.head, r0, rows, a.o.pitch), 0, to + kStep, kChunkTiles, wave, g_lane, a.o.pitch);
-        const Rsrc ls = make_rsrc(lse + stat, max(0, rows) * 4), ds = make_rsrc(delta + stat, max(0, rows) * 4);
+        const int h = kv * a.group + hg_, rows = min(kChunkRows, tv - c_ * kChunkRows);
+        const int64_t r0 = (int64_t)c_ * kChunkRows, stat = ((int64_t)sample * a.H + h) * T + r0;
+        stage_direct<C, kChunkTiles, kReadShared>(rows_of(qb + h * a.q.head, r0, rows, a.q.pitch), 0, to, kChunkTiles, wave, q_lane, a.q.pitch);
+        stage_direct<C, kChunkTiles, kReadShared>(rows_of(gb + h * a.o.head, r0, rows, a.o.pitch), 0, to + kStep, kChunkTiles, wave, g_lane, a.o.pitch);
+        const Rsrc ls = rows_of(lse + stat, 0, rows, 4), ds = rows_of(delta + stat, 0, rows, 4);
         row_lse = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(ls, (16 * wave + n) * 4, 0, 0));
         row_delta = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(ds, (16 * wave + n) * 4, 0, 0));
     };
     if (u < u_end) stage(hg, c, buf_lds);
-    const int own = 16 * QT * wave, w0 = row0 + own, w1 = w0 + 16 * QT - 1;
+    const int own = 16 * wave, w0 = row0 + own, w1 = w0 + 15, key = w0 + n;
     const Rsrc ks = rows_of(k + sample * a.k.sample + kv * a.k.head, row0, last_key + 1 - row0, a.k.pitch);
     const Rsrc vs = rows_of(v + sample * a.v.sample + kv * a.v.head, row0, last_key + 1 - row0, a.v.pitch);
-    RowOperand<C> kop[QT], vop[QT];
-#pragma unroll
-    for (int h = 0; h < QT; ++h) {
-        load_rows<C, kReadShared>(kop[h], ks, (own + 16 * h) * a.k.pitch, a.k.pitch, width, lane);
-        load_rows<C, kReadShared>(vop[h], vs, (own + 16 * h) * a.v.pitch, a.v.pitch, width, lane);
-    }
+    RowOperand<C> kop, vop;
+    load_rows<C, kReadShared>(kop, ks, own * a.k.pitch, a.k.pitch, width, lane);
+    load_rows<C, kReadShared>(vop, vs, own * a.v.pitch, a.v.pitch, width, lane);
     const float scale2 = a.scale * kLog2e;
+    const uint32_t reach = key < a.sinks ? 0x7fffffffu : (uint32_t)a.window;
     RowLane<C> row_lane;
     TrLane<C> tr_lane;
     row_lane.init(0, lane);
     tr_lane.init(0, lane);
-    f32x4 acck[QT][CT], accv[QT][CT];
+    f32x4 acck[CT], accv[CT];
 #pragma unroll
-    for (int h = 0; h < QT; ++h)
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) acck[h][ct] = accv[h][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int ct = 0; ct < CT; ++ct) acck[ct] = accv[ct] = f32x4{0.f, 0.f, 0.f, 0.f};
 
     int at = 0;
     for (; u < u_end; ++u) {
@@ -504,7 +529,7 @@ sink_dkv_kernel(char *__restrict__ dk, char *__restrict__ dv, float *__restrict_
         if (see == kNothing) continue;
 #pragma unroll
         for (int qi = 0; qi < kChunkTiles; qi += 2) {
-            u32x4 pb[QT], db[QT];
+            u32x4 pb, db;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 RowOperand<C> qop, gop;
@@ -512,25 +537,21 @@ sink_dkv_kernel(char *__restrict__ dk, char *__restrict__ dv, float *__restrict_
                 read_rows<C>(gop, g_lds + (qi + j) * LL::kTileBytes, row_lane);
                 const f32x4 ref = *reinterpret_cast<LDS_PTR(f32x4)>(ref_lds + 64 * (qi + j));
                 const f32x4 del4 = *reinterpret_cast<LDS_PTR(f32x4)>(ref_lds + kChunkRows * 4 + 64 * (qi + j));
+                const f32x4 s = dot_rows_mma<DT, C>(qop, kop);        // [query 4g+r][key n]
+                const f32x4 dp = dot_rows_mma<DT, C>(gop, vop, del4);
+                float p[4];
 #pragma unroll
-                for (int h = 0; h < QT; ++h) {
-                    const f32x4 s = dot_rows_mma<DT, C>(qop, kop[h]);        // [query 4g+r][key n]
-                    const f32x4 dp = dot_rows_mma<DT, C>(gop, vop[h], del4);
-                    float p[4];
+                for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], scale2, ref[r]));
+                if (see == kPart) {
+                    const int d = q0 + 16 * (qi + j) + 4 * g - key;      // query 4g less the key
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], scale2, ref[r]));
-                    if (see == kPart) {
-                        const int key = w0 + 16 * h + n, d = q0 + 16 * (qi + j) + 4 * g - key;      // query 4g less the key
-                        const uint32_t reach = key < a.sinks ? 0x7fffffffu : (uint32_t)a.window;
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (!((uint32_t)(d + r) < reach)) p[r] = 0.f;
-                    }
-                    pb[h][2 * j] = Mma<DT>::pack(p[0], p[1]);
-                    pb[h][2 * j + 1] = Mma<DT>::pack(p[2], p[3]);
-                    db[h][2 * j] = Mma<DT>::pack(p[0] * dp[0], p[1] * dp[1]);
-                    db[h][2 * j + 1] = Mma<DT>::pack(p[2] * dp[2], p[3] * dp[3]);
+                    for (int r = 0; r < 4; ++r)
+                        if (!((uint32_t)(d + r) < reach)) p[r] = 0.f;
                 }
+                pb[2 * j] = Mma<DT>::pack(p[0], p[1]);
+                pb[2 * j + 1] = Mma<DT>::pack(p[2], p[3]);
+                db[2 * j] = Mma<DT>::pack(p[0] * dp[0], p[1] * dp[1]);
+                db[2 * j + 1] = Mma<DT>::pack(p[2] * dp[2], p[3] * dp[3]);
             }
             LDS_PTR(char) qtile = q_lds + qi * LL::kTileBytes;
             LDS_PTR(char) gtile = g_lds + qi * LL::kTileBytes;
@@ -539,69 +560,72 @@ sink_dkv_kernel(char *__restrict__ dk, char *__restrict__ dv, float *__restrict_
                 const u32x2 g0 = read_tr(gtile + tr_lane.off[ct]), g1 = read_tr(gtile + LL::kTileBytes + tr_lane.off[ct]);
                 const u32x2 q0t = read_tr(qtile + tr_lane.off[ct]), q1t = read_tr(qtile + LL::kTileBytes + tr_lane.off[ct]);
                 const u32x4 gg = {g0.x, g0.y, g1.x, g1.y}, qq = {q0t.x, q0t.y, q1t.x, q1t.y};
-#pragma unroll
-                for (int h = 0; h < QT; ++h) {
-                    accv[h][ct] = Mma<DT>::k32(gg, pb[h], accv[h][ct]);
-                    acck[h][ct] = Mma<DT>::k32(qq, db[h], acck[h][ct]);
-                }
+                accv[ct] = Mma<DT>::k32(gg, pb, accv[ct]);
+                acck[ct] = Mma<DT>::k32(qq, db, acck[ct]);
             }
         }
     }
-    if (each > 1) {          // fp32 sums of this part: [head, strip's parts][dk, dv][row of the strip][C]
-        const uint32_t slot = a.parts > 1 ? sh * per_head + rest : sh * sink_items + rest;
-        float *to = partial + (int64_t)slot * (2 * kChunkRows * QT * C);
+    const bool shared = !far && strip_id >= (uint32_t)a.whole, sinking = a.far && w0 < a.sinks;
+    if (shared || far || sinking) {
+        if (far && !sinking) return;
+        const Partial at_ = partial_of<C>(strip_id, part, (int64_t)head * a.sink_strips + strip, part, heads, a);
+        const int rows = shared ? kChunkRows : a.sink_rows;
+        float *to = partial + (shared ? at_.shared : far ? at_.far : at_.near) + (own + n) * C + 4 * g;
 #pragma unroll
-        for (int h = 0; h < QT; ++h) {
-            float *row = to + (own + 16 * h + n) * C + 4 * g;
-#pragma unroll
-            for (int ct = 0; ct < CT; ++ct) {
-                *reinterpret_cast<f32x4 *>(row + 16 * ct) = acck[h][ct];
-                *reinterpret_cast<f32x4 *>(row + kChunkRows * QT * C + 16 * ct) = accv[h][ct];
-            }
+        for (int ct = 0; ct < CT; ++ct) {
+            *reinterpret_cast<f32x4 *>(to + 16 * ct) = acck[ct];
+            *reinterpret_cast<f32x4 *>(to + rows * C + 16 * ct) = accv[ct];
         }
         return;
     }
     const int64_t off = sample * a.dkv.sample + kv * a.dkv.head;
     const Rsrc dks = rows_of(dk + off, row0, row_end - row0, a.dkv.pitch), dvs = rows_of(dv + off, row0, row_end - row0, a.dkv.pitch);
     const bool stream = stores_whole_lines(a.dkv.pitch, C, 0);
+    u32x2 kw[CT], vw[CT];
 #pragma unroll
-    for (int h = 0; h < QT; ++h) {
-        const int at_row = own + 16 * h + n;
-        const bool valid = row0 + at_row < tv;
-        u32x2 kw[CT], vw[CT];
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-            kw[ct] = pack_acc<DT>(acck[h][ct], a.scale);
-            vw[ct] = pack_acc<DT>(accv[h][ct], 1.f);
-            if (!valid) kw[ct] = vw[ct] = u32x2{0u, 0u};
-        }
-        store_tile<C>(dks, at_row * a.dkv.pitch, kw, g, stream, width);      // rows past T are dropped
-        store_tile<C>(dvs, at_row * a.dkv.pitch, vw, g, stream, width);
+    for (int ct = 0; ct < CT; ++ct) {
+        kw[ct] = pack_acc<DT>(acck[ct], a.scale);
+        vw[ct] = pack_acc<DT>(accv[ct], 1.f);
+        if (key >= tv) kw[ct] = vw[ct] = u32x2{0u, 0u};
     }
+    store_tile<C>(dks, (own + n) * a.dkv.pitch, kw, g, stream, width);      // rows past T are dropped
+    store_tile<C>(dvs, (own + n) * a.dkv.pitch, vw, g, stream, width);
 }
 
-// The parts of a strip's dK and dV, added up in a fixed order: four channels of a row to a thread.
-template <class DT, int C, int QT>
+// Rows of dK and dV that several workgroups have a share in: strips in parts, and the tiles with sinks of the others.  Four channels of a row to a thread.
+template <class DT, int C>
 __global__ void __launch_bounds__(kThreads)
-sink_join_kernel(char *__restrict__ dk, char *__restrict__ dv, const float *__restrict__ partial, const int32_t *__restrict__ t_valid, SinkArgs a) {
-    constexpr int kRows = kChunkRows * QT, kQuads = C / 4;
-    const uint32_t sink_items = a.sink_strips * a.sink_parts, joined = a.parts > 1 ? a.strips : a.sink_strips;
-    const uint32_t per_head = sink_items + (a.parts > 1 ? (a.strips - a.sink_strips) * a.parts : 0);
-    constexpr uint32_t kBlocks = (kRows * kQuads + kThreads - 1) / kThreads;     // workgroups to a strip
-    const uint32_t block = blockIdx.x % kBlocks, unit = blockIdx.x / kBlocks, sh = unit / joined, strip = unit - sh * joined;
-    const uint32_t sample = sh / (uint32_t)a.K, kv = sh - sample * a.K;
-    const int i = block * kThreads + threadIdx.x, r = i / kQuads, ch = (i % kQuads) * 4, row = strip * kRows + r;
-    if (i >= kRows * kQuads || row >= a.T || 2 * ch >= a.width) return;
-    const bool of_sinks = strip < (uint32_t)a.sink_strips;
-    const int each = of_sinks ? a.sink_parts : a.parts;
-    const uint32_t slot = sh * per_head + (of_sinks ? strip * a.sink_parts : sink_items + (strip - a.sink_strips) * a.parts);
-    const float *from = partial + (int64_t)slot * (2 * kRows * C) + r * C + ch;
-    f32x4 sk = {0.f, 0.f, 0.f, 0.f}, sv = sk;
-    for (int p = 0; p < each; ++p, from += 2 * kRows * C) {
-        sk += *reinterpret_cast<const f32x4 *>(from);
-        sv += *reinterpret_cast<const f32x4 *>(from + kRows * C);
+sink_join_kernel(char *__restrict__ dk, char *__restrict__ dv, const float *__restrict__ partial, const int32_t *__restrict__ t_valid, uint32_t heads, SinkArgs a) {
+    constexpr int kQuads = C / 4;
+    constexpr uint32_t kBlocks = (kChunkRows * kQuads + kThreads - 1) / kThreads;     // workgroups to a strip
+    const uint32_t block = blockIdx.x % kBlocks, unit = blockIdx.x / kBlocks, shared = heads * a.strips - a.whole;
+    const int i = block * kThreads + threadIdx.x, r = i / kQuads, ch = (i % kQuads) * 4;
+    // the strips in parts, then those with sinks (which may be among them)
+    uint32_t head, strip;
+    if (unit < shared) {
+        head = (a.whole + unit) / (uint32_t)a.strips, strip = a.whole + unit - head * a.strips;
+    } else {
+        head = (unit - shared) / (uint32_t)a.sink_strips, strip = unit - shared - head * a.sink_strips;
     }
+    const uint32_t strip_id = head * a.strips + strip;
+    const bool in_parts = strip_id >= (uint32_t)a.whole, sinking = a.far && strip < (uint32_t)a.sink_strips && r < a.sink_rows && (int)(strip * kChunkRows) + (r & ~15) < a.sinks;
+    const int row = strip * kChunkRows + r;
+    if (i >= kChunkRows * kQuads || row >= a.T || 2 * ch >= a.width || (unit >= shared && (in_parts || !sinking))) return;
+    f32x4 sk = {0.f, 0.f, 0.f, 0.f}, sv = sk;
+    auto add = [&](int64_t from, int rows) {
+        sk += *reinterpret_cast<const f32x4 *>(partial + from + r * C + ch);
+        sv += *reinterpret_cast<const f32x4 *>(partial + from + (rows + r) * C + ch);
+    };
+    const int64_t sink_strip = (int64_t)head * a.sink_strips + strip;
+    if (in_parts) {
+        for (int p = 0; p < a.parts; ++p) add(partial_of<C>(strip_id, p, sink_strip, 0, heads, a).shared, kChunkRows);
+    } else {
+        add(partial_of<C>(strip_id, 0, sink_strip, 0, heads, a).near, a.sink_rows);
+    }
+    if (sinking)
+        for (int f = 0; f < a.far; ++f) add(partial_of<C>(strip_id, 0, sink_strip, f, heads, a).far, a.sink_rows);
     u32x2 kw = pack_acc<DT>(sk, a.scale), vw = pack_acc<DT>(sv, 1.f);
+    const uint32_t sample = head / (uint32_t)a.K, kv = head - sample * a.K;
     if (t_valid && row >= t_valid[sample]) kw = vw = u32x2{0u, 0u};
     const int64_t off = sample * a.dkv.sample + kv * a.dkv.head + (int64_t)row * a.dkv.pitch + 2 * ch;
     *reinterpret_cast<u32x2 *>(dk + off) = kw;
@@ -613,30 +637,45 @@ sink_join_kernel(char *__restrict__ dk, char *__restrict__ dv, const float *__re
 // feeds two products.
 bool two_tiles(const na1d_sink &h, int64_t heads) { return h.N * heads * ((h.T + 127) / 128) >= 256; }
 
-SinkArgs sink_args(const na1d_sink &h, bool two, bool keys) {
+SinkArgs sink_args(const na1d_sink &h, int tiles) {
     SinkArgs a{};
-    const int64_t rows = kChunkRows * (two ? 2 : 1);
+    const int64_t rows = kChunkRows * tiles;
     a.T = (int)h.T, a.H = h.heads, a.K = h.kv_heads, a.group = h.heads / h.kv_heads, a.strips = (int)((h.T + rows - 1) / rows);
     a.window = (int)std::min(h.window, h.T), a.sinks = (int)std::min(h.sinks, h.T), a.width = 2 * h.head_dim, a.scale = h.scale;
     auto strided = [](const int64_t (&s)[3]) { return SinkRows{2 * s[0], 2 * s[1], (int)(2 * s[2])}; };
     auto packed = [&](int heads) { return SinkRows{2 * h.T * heads * h.head_dim, 2 * h.head_dim, 2 * heads * h.head_dim}; };
     a.q = strided(h.q_strides), a.k = strided(h.k_strides), a.v = strided(h.v_strides), a.o = packed(h.heads), a.dkv = packed(h.kv_heads);
-    if (keys) {
-        // A strip's work is its chunks of queries times the heads of the group.  Strips are shared where there are too few of them
-        // to occupy every CU twice, and those with sinks so that none of their parts is longer than the others' work.
-        const int64_t chunks = (h.T + kChunkRows - 1) / kChunkRows, others = std::min<int64_t>(chunks, (a.window + rows - 1) / kChunkRows + 2);
-        const int64_t wgs = h.N * h.kv_heads * a.strips;
-        a.sink_strips = (int)((a.sinks + rows - 1) / rows);
-        a.parts = (int)std::min<int64_t>({std::max<int64_t>(1, 512 / wgs), std::max<int64_t>(1, others * a.group / 4), 16});
-        const int64_t sharing = h.N * h.kv_heads * std::max(a.sink_strips, 1);
-        a.sink_parts = (int)std::min((chunks * a.parts + others - 1) / others, std::max<int64_t>(a.parts, 1024 / sharing));
-    }
     return a;
 }
-// fp32 sums that the workgroups which share a strip leave
-int64_t partial_floats(const na1d_sink &h, const SinkArgs &a, bool two, int C) {
-    const int64_t slots = (a.sink_parts > 1 || a.parts > 1 ? (int64_t)a.sink_strips * a.sink_parts : 0) + (a.parts > 1 ? (int64_t)(a.strips - a.sink_strips) * a.parts : 0);
-    return h.N * h.kv_heads * slots * (2 * kChunkRows * (two ? 2 : 1) * (int64_t)C);
+// How dK and dV are cut into workgroups (see sink_dkv_kernel).
+struct KeyPlan {
+    SinkArgs a;
+    int64_t heads, rest, floats, joined;      // rest: workgroups beside the strips' own; floats of partial sums; strips that are joined
+};
+KeyPlan key_plan(const na1d_sink &h) {
+    KeyPlan p{};
+    SinkArgs &a = p.a;
+    a = sink_args(h, 1);
+    p.heads = h.N * h.kv_heads;
+    const int C = padded_width(h.head_dim);
+    const int64_t strips = p.heads * a.strips, round = 256 * (C == 128 ? 2 : C == 64 ? 4 : 6);      // workgroups that the card holds at once
+    const int64_t chunks = a.strips, near = std::min<int64_t>(chunks, (a.window + kChunkRows - 2) / kChunkRows + 1), units = near * a.group;      // a strip's
+    const int64_t over = strips % round;
+    a.parts = 1;
+    if (over > 0 && over <= round / 2) a.parts = (int)std::max<int64_t>(1, std::min<int64_t>({round / over, units / 4, 16}));
+    a.whole = (int)std::min<int64_t>(strips - (a.parts > 1 ? over : 0), INT32_MAX);
+    a.sink_strips = (int)((a.sinks + kChunkRows - 1) / kChunkRows);
+    a.sink_rows = std::min(kChunkRows, (a.sinks + 15) / 16 * 16);
+    // far workgroups fill the card once, or have as many units as the others where that makes more of them; from a thousand strips with sinks on there
+    // are enough of those as they are
+    const int64_t sinking = p.heads * a.sink_strips, beyond = chunks - near;
+    if (sinking > 0 && sinking < 1024 && beyond > 0)
+        a.far = (int)std::max<int64_t>(1, std::min<int64_t>({std::max((beyond + near - 1) / near, round / sinking), 1024 / sinking, beyond * a.group / 4}));
+    const int64_t shared = strips - a.whole;
+    p.rest = shared * a.parts + sinking * a.far;
+    p.floats = shared * a.parts * (2 * kChunkRows * (int64_t)C) + (a.far ? sinking * (1 + a.far) * (2 * a.sink_rows * (int64_t)C) : 0);
+    p.joined = shared + (a.far ? sinking : 0);
+    return p;
 }
 int64_t lse_floats(const na1d_sink &h) { return (h.N * h.heads * h.T + 3) / 4 * 4; }
 bool countable(int64_t items) { return items <= 0x7fffff00LL; }
@@ -644,7 +683,7 @@ bool countable(int64_t items) { return items <= 0x7fffff00LL; }
 template <class DT, int C>
 int launch_sink_fwd(const na1d_sink &h, void *out, float *saved, const void *q, const void *k, const void *v, const int32_t *t_valid, hipStream_t s) {
     const bool two = two_tiles(h, h.heads);
-    const SinkArgs a = sink_args(h, two, false);
+    const SinkArgs a = sink_args(h, two ? 2 : 1);
     const int64_t items = h.N * h.heads * a.strips;
     if (!countable(items)) return NA1D_ERR_UNSUPPORTED;
     const size_t lds = 4 * (size_t)region_bytes<C>(kChunkTiles);
@@ -661,31 +700,24 @@ int launch_sink_fwd(const na1d_sink &h, void *out, float *saved, const void *q, 
 template <class DT, int C>
 int launch_sink_bwd(const na1d_sink &h, void *dq, void *dk, void *dv, const void *q, const void *k, const void *v, const void *out, const void *dout,
                     const float *saved, const int32_t *t_valid, float *ws, hipStream_t s) {
-    const bool two_q = two_tiles(h, h.heads), two_k = two_tiles(h, h.kv_heads);
-    const SinkArgs a = sink_args(h, two_q, false), b = sink_args(h, two_k, true);
-    const int64_t items = h.N * h.heads * a.strips;
-    const int64_t key_items = h.N * h.kv_heads * ((int64_t)b.sink_strips * b.sink_parts + (int64_t)(b.strips - b.sink_strips) * b.parts);
-    const bool joins = b.parts > 1 || (b.sink_parts > 1 && b.sink_strips > 0);
-    const int64_t rows = kChunkRows * (two_k ? 2 : 1);
-    const int64_t join_items = !joins ? 0 : h.N * h.kv_heads * (b.parts > 1 ? b.strips : b.sink_strips) * ((rows * (C / 4) + kThreads - 1) / kThreads);
-    if (!countable(items) || !countable(key_items) || !countable(join_items)) return NA1D_ERR_UNSUPPORTED;
+    const bool two = two_tiles(h, h.heads);
+    const SinkArgs a = sink_args(h, two ? 2 : 1);
+    const KeyPlan p = key_plan(h);
+    const int64_t items = h.N * h.heads * a.strips, key_items = p.a.whole + p.rest, join_items = p.joined * ((kChunkRows * (C / 4) + kThreads - 1) / kThreads);
+    if (!countable(items) || !countable(p.heads * p.a.strips) || !countable(key_items) || !countable(join_items)) return NA1D_ERR_UNSUPPORTED;
     float *const delta = ws, *const partial = ws + lse_floats(h);
-    const size_t dq_lds = 4 * (size_t)region_bytes<C>(kChunkTiles), dkv_lds = 2 * (2 * (size_t)region_bytes<C>(kChunkTiles) + 2 * kChunkRows * sizeof(float));
-    auto go = [&](auto dq_kern, auto dkv_kern, auto join_kern) {
-        if (!allow_lds(dq_kern, dq_lds) || !allow_lds(dkv_kern, dkv_lds)) return (int)NA1D_ERR_LAUNCH;
-        note_kernel_as("sink_dq_kernel + sink_dkv_kernel<%s, %d, %d>", DT::tag == NA1D_BF16 ? "BF16" : "FP16", C, two_k ? 2 : 1);
-        launch_kernel_span(1, dq_kern, (unsigned)items, (unsigned)kThreads, dq_lds, s, (char *)dq, delta, (const char *)q, (const char *)k, (const char *)v,
-                           (const char *)out, (const char *)dout, saved, (const char *)(saved + lse_floats(h)), t_valid, (uint32_t)items, a);
-        launch_kernel_span(joins ? 0 : 2, dkv_kern, (unsigned)key_items, (unsigned)kThreads, dkv_lds, s, (char *)dk, (char *)dv, partial, (const char *)q, (const char *)k,
-                           (const char *)v, (const char *)dout, saved, (const float *)delta, t_valid, (uint32_t)key_items, b);
-        if (joins) launch_kernel_span(2, join_kern, (unsigned)join_items, (unsigned)kThreads, 0, s, (char *)dk, (char *)dv, (const float *)partial, t_valid, b);
-        return launch_status();
-    };
-    if (two_q)
-        return two_k ? go(sink_dq_kernel<DT, C, 2>, sink_dkv_kernel<DT, C, 2>, sink_join_kernel<DT, C, 2>)
-                     : go(sink_dq_kernel<DT, C, 2>, sink_dkv_kernel<DT, C, 1>, sink_join_kernel<DT, C, 1>);
-    return two_k ? go(sink_dq_kernel<DT, C, 1>, sink_dkv_kernel<DT, C, 2>, sink_join_kernel<DT, C, 2>)
-                 : go(sink_dq_kernel<DT, C, 1>, sink_dkv_kernel<DT, C, 1>, sink_join_kernel<DT, C, 1>);
+    constexpr size_t dq_lds = 4 * (size_t)region_bytes<C>(kChunkTiles), dkv_lds = 2 * (2 * (size_t)region_bytes<C>(kChunkTiles) + 2 * kChunkRows * sizeof(float));
+    auto dq_kern = two ? sink_dq_kernel<DT, C, 2> : sink_dq_kernel<DT, C, 1>;
+    if (!allow_lds(dq_kern, dq_lds) || !allow_lds(sink_dkv_kernel<DT, C>, dkv_lds)) return NA1D_ERR_LAUNCH;
+    note_kernel_as("sink_dq_kernel + sink_dkv_kernel<%s, %d>", DT::tag == NA1D_BF16 ? "BF16" : "FP16", C);
+    launch_kernel_span(1, dq_kern, (unsigned)items, (unsigned)kThreads, dq_lds, s, (char *)dq, delta, (const char *)q, (const char *)k, (const char *)v, (const char *)out,
+                       (const char *)dout, saved, (const char *)(saved + lse_floats(h)), t_valid, (uint32_t)items, a);
+    launch_kernel_span(p.joined ? 0 : 2, sink_dkv_kernel<DT, C>, (unsigned)key_items, (unsigned)kThreads, dkv_lds, s, (char *)dk, (char *)dv, partial, (const char *)q,
+                       (const char *)k, (const char *)v, (const char *)dout, saved, (const float *)delta, t_valid, (uint32_t)p.rest, (uint32_t)p.heads, p.a);
+    if (p.joined)
+        launch_kernel_span(2, sink_join_kernel<DT, C>, (unsigned)join_items, (unsigned)kThreads, 0, s, (char *)dk, (char *)dv, (const float *)partial, t_valid,
+                           (uint32_t)p.heads, p.a);
+    return launch_status();
 }
 
 }  // namespace
@@ -694,8 +726,7 @@ int64_t sink_saved_bytes(const na1d_sink &h) {
     return 4 * lse_floats(h) + (h.dtype == NA1D_BF16 ? h.N * h.heads * ((h.T + 15) / 16) * 16 * padded_width(h.head_dim) : 0);
 }
 int64_t sink_bwd_workspace_bytes(const na1d_sink &h) {
-    const bool two = two_tiles(h, h.kv_heads);
-    return 4 * (lse_floats(h) + partial_floats(h, sink_args(h, two, true), two, padded_width(h.head_dim)));
+    return 4 * (lse_floats(h) + key_plan(h).floats);
 }
 
 int sink_fwd(const na1d_sink &h, void *out, float *saved, const void *q, const void *k, const void *v, const int32_t *t_valid, hipStream_t s) {

@@ -1,4 +1,4 @@
-// The operators' autograd nodes for torch in C++: what fused.py, dense.py, nattn.py and losses.py do per call, without the
+// The operators' autograd nodes for torch in C++: what fused.py, dense.py, nattn.py, losses.py and streaming.py do per call, without the
 // interpreter.  A windowed layer's forward and backward at a training batch are 45 us of kernels; the same host path in
 // Python took 115 us (allocations, context managers, ctypes, and the engine's thread waiting for the interpreter lock).
 //
@@ -424,6 +424,152 @@ MaybeTensor head(const Tensor &x, const Tensor &weight, const Tensor &ids, const
     return HeadLoss::apply(x, weight, ids, h, done);
 }
 
+// ------------------------------------------------------------------------------------------------ attention of streams
+// streaming.py's calls: a step of one stream is 10 us of kernels and took 26 us through the interpreter, a training layer of 5 x 777 tokens 180.
+// Tokens [N, T, heads, C] whose strides the native call takes.
+bool tokens(const Tensor &t, const Tensor &like) {
+    if (!plain(t) || t.dim() != 4 || t.scalar_type() != like.scalar_type() || !half_type(t) || t.device() != like.device() || !t.numel()) return false;
+    const int64_t N = t.size(0), T = t.size(1), H = t.size(2), C = t.size(3);
+    const auto fits = [](int64_t n, int64_t stride, int64_t least, int64_t most) { return n == 1 || (stride % 8 == 0 && stride >= least && stride <= most); };
+    return (C == 1 || t.stride(3) == 1) && fits(N, t.stride(0), 0, 1ll << 40) && fits(T, t.stride(1), C, 1 << 20) && fits(H, t.stride(2), 0, 1ll << 40) && (uintptr_t)t.data_ptr() % 16 == 0;
+}
+void strides_into(int64_t (&to)[3], const Tensor &t) {       // {sample, head, row}; those of dimensions of one entry do not matter
+    to[0] = t.size(0) > 1 ? t.stride(0) : 0, to[1] = t.size(2) > 1 ? t.stride(2) : 0, to[2] = t.size(1) > 1 ? t.stride(1) : t.size(3);
+}
+bool lengths_for(const MaybeTensor &t, const Tensor &like) { return !t || (on(*t, like) && t->scalar_type() == at::kInt && t->dim() == 1 && t->size(0) == like.size(0)); }
+const int32_t *int_ptr(const MaybeTensor &t) { return t ? (const int32_t *)ptr(*t) : nullptr; }
+
+na1d_sink sink_of(const Tensor &q, const Tensor &k, const Tensor &v, int64_t window, int64_t sinks, double scale) {
+    na1d_sink h{};
+    h.dtype = tag(q), h.heads = (int32_t)q.size(2), h.kv_heads = (int32_t)k.size(2), h.head_dim = (int32_t)q.size(3), h.scale = (float)scale;
+    h.N = q.size(0), h.T = q.size(1), h.window = window, h.sinks = sinks;
+    strides_into(h.q_strides, q), strides_into(h.k_strides, k), strides_into(h.v_strides, v);
+    return h;
+}
+struct SinkDone {
+    Tensor out, saved;
+};
+struct SinkAttention : torch::autograd::Function<SinkAttention> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &q, const Tensor &k, const Tensor &v, const MaybeTensor &t_valid, int64_t window, int64_t sinks, double scale,
+                          const SinkDone &done) {
+        ctx->save_for_backward({q, k, v, t_valid ? *t_valid : Tensor(), done.out, done.saved});
+        ctx->saved_data["window"] = window;
+        ctx->saved_data["sinks"] = sinks;
+        ctx->saved_data["scale"] = scale;
+        return done.out;
+    }
+    static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
+        const variable_list s = ctx->get_saved_variables();
+        const Tensor &q = s[0], &k = s[1], &v = s[2];
+        const na1d_sink h = sink_of(q, k, v, ctx->saved_data["window"].toInt(), ctx->saved_data["sinks"].toInt(), ctx->saved_data["scale"].toDouble());
+        const c10::DeviceGuard guard(q.device());
+        Tensor d[3];
+        {
+            const at::AutoGradMode off(false);
+            Tensor dout = grads[0].contiguous();
+            if ((uintptr_t)dout.data_ptr() % 16) dout = dout.clone();
+            for (int i = 0; i < 3; ++i) d[i] = at::empty(s[i].sizes(), s[i].options());
+            const int64_t nbytes = na1d_sink_backward_workspace_bytes(&h);
+            check((int)std::min<int64_t>(nbytes, 0), "na1d_sink_backward_workspace_bytes");
+            const Tensor ws = bytes_of(nbytes, q);
+            check(na1d_sink_backward(&h, ptr(d[0]), ptr(d[1]), ptr(d[2]), ptr(q), ptr(k), ptr(v), ptr(s[4]), ptr(dout), ptr(s[5]), s[5].numel(), (const int32_t *)ptr(s[3]), ptr(ws),
+                                     nbytes, stream_of(q)),
+                  "na1d_sink_backward");
+        }
+        for (int i = 0; i < 3; ++i) {
+            if (!ctx->needs_input_grad(i)) {
+                d[i] = Tensor();
+            } else if (at::GradMode::is_enabled()) {         // these gradients have none of their own: whoever asks for them is told
+                const auto error = std::make_shared<torch::autograd::DelayedError>("the gradients of na1d_amd's sink_attention cannot be differentiated again", 1);
+                d[i] = (*error)({d[i].set_requires_grad(true)})[0];
+            }
+        }
+        return {d[0], d[1], d[2], Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+MaybeTensor sink(const Tensor &q, const Tensor &k, const Tensor &v, int64_t window, int64_t sinks, const MaybeTensor &t_valid, std::optional<double> scale) {
+    if (!plain_call() || !tokens(q, q) || !tokens(k, q) || !tokens(v, q) || k.sizes() != v.sizes() || q.size(0) != k.size(0) || q.size(1) != k.size(1) || q.size(3) != k.size(3) ||
+        q.size(2) % k.size(2) || q.size(2) > (1 << 20) || !lengths_for(t_valid, q))
+        return std::nullopt;
+    const double s = scale ? *scale : 1.0 / std::sqrt((double)q.size(3));
+    const na1d_sink h = sink_of(q, k, v, window, sinks, s);
+    const int64_t saved_bytes = na1d_sink_saved_bytes(&h);
+    if (saved_bytes < 0) return std::nullopt;
+    const c10::DeviceGuard guard(q.device());
+    const bool node = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad());
+    const SinkDone done{at::empty(q.sizes(), q.options()), node ? bytes_of(saved_bytes, q) : Tensor()};
+    if (na1d_sink_forward(&h, ptr(done.out), ptr(done.saved), node ? saved_bytes : 0, ptr(q), ptr(k), ptr(v), int_ptr(t_valid), stream_of(q)) != NA1D_OK) return std::nullopt;
+    return node ? SinkAttention::apply(q, k, v, t_valid, window, sinks, s, done) : done.out;
+}
+
+// A pair of caches, with their rows' ranges where they are held in 4 bits.
+bool cache_of(na1d_sink_cache &c, const Tensor &k, const Tensor &v, const MaybeTensor &kr, const MaybeTensor &vr, int64_t sinks) {
+    if (!plain(k) || !on(v, k) || !k.is_contiguous() || k.dim() != 4 || k.sizes() != v.sizes() || k.scalar_type() != v.scalar_type() || !k.numel() || kr.has_value() != vr.has_value())
+        return false;
+    if (k.requires_grad() || v.requires_grad()) return false;
+    if (kr) {
+        for (const Tensor *r : {&*kr, &*vr})
+            if (!on(*r, k) || !half_type(*r) || r->scalar_type() != kr->scalar_type() || r->dim() != 4 || r->size(0) != k.size(0) || r->size(1) != k.size(1) ||
+                r->size(2) != k.size(2) || r->size(3) != 2 || r->requires_grad())
+                return false;
+        if (k.scalar_type() != at::kByte) return false;
+    } else if (!half_type(k)) {
+        return false;
+    }
+    c = na1d_sink_cache{tag(kr ? *kr : k), kr ? 4 : 16, (int32_t)k.size(1), (int32_t)(k.size(3) * (kr ? 2 : 1)), k.size(0), k.size(2), sinks, ptr(k), ptr(v),
+                        kr ? ptr(*kr) : nullptr, vr ? ptr(*vr) : nullptr};
+    return k.size(1) <= 1 << 24;
+}
+bool goes_with(const Tensor &t, const na1d_sink_cache &c, const Tensor &cache, bool queries) {
+    return tokens(t, t) && tag(t) == c.dtype && t.device() == cache.device() && t.size(0) == c.N && t.size(3) == c.head_dim &&
+           (queries ? t.size(2) % c.kv_heads == 0 : t.size(2) == c.kv_heads);
+}
+void written(std::initializer_list<const Tensor *> ts) {
+    for (const Tensor *t : ts)
+        if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+MaybeTensor sink_over(const Tensor &q, const MaybeTensor &k, const MaybeTensor &v, const Tensor &kc, const Tensor &vc, const MaybeTensor &kr, const MaybeTensor &vr,
+                      const Tensor &lengths, int64_t window, int64_t sinks, std::optional<double> scale) {
+    na1d_sink_cache c;
+    if (!plain_call() || !cache_of(c, kc, vc, kr, vr, sinks) || !goes_with(q, c, kc, true) || !lengths_for(lengths, q)) return std::nullopt;
+    if (k && (!goes_with(*k, c, kc, false) || !goes_with(*v, c, kc, false) || k->size(1) != q.size(1) || v->size(1) != q.size(1))) return std::nullopt;
+    if (at::GradMode::is_enabled() && (q.requires_grad() || (k && (k->requires_grad() || v->requires_grad())))) return std::nullopt;
+    const int64_t fresh = q.size(1), heads = q.size(2), nbytes = na1d_sink_attend_workspace_bytes(&c, fresh, heads, window);
+    if (nbytes < 0) return std::nullopt;
+    const c10::DeviceGuard guard(q.device());
+    const Tensor out = at::empty(q.sizes(), q.options()), ws = nbytes ? bytes_of(nbytes, q) : Tensor();
+    const float s = (float)(scale ? *scale : 1.0 / std::sqrt((double)c.head_dim));
+    int64_t qs[3], ks[3], vs[3];
+    strides_into(qs, q);
+    int status;
+    if (k) {
+        strides_into(ks, *k), strides_into(vs, *v);
+        status = na1d_sink_step(&c, ptr(out), ptr(q), ptr(*k), ptr(*v), qs, ks, vs, (const int32_t *)ptr(lengths), fresh, heads, window, s, ptr(ws), nbytes, stream_of(q));
+    } else {
+        status = na1d_sink_attend(&c, ptr(out), ptr(q), qs, (const int32_t *)ptr(lengths), fresh, heads, window, s, ptr(ws), nbytes, stream_of(q));
+    }
+    if (status != NA1D_OK) return std::nullopt;
+    if (k) {
+        written({&kc, &vc});
+        if (kr) written({&*kr, &*vr});
+    }
+    return out;
+}
+bool sink_append(const Tensor &k, const Tensor &v, const Tensor &kc, const Tensor &vc, const MaybeTensor &kr, const MaybeTensor &vr, const MaybeTensor &lengths, int64_t sinks,
+                 const MaybeTensor &t_valid) {
+    na1d_sink_cache c;
+    if (!plain_call() || !cache_of(c, kc, vc, kr, vr, sinks) || !goes_with(k, c, kc, false) || !goes_with(v, c, kc, false) || k.size(1) != v.size(1) || !lengths_for(lengths, k) ||
+        !lengths_for(t_valid, k))
+        return false;
+    const c10::DeviceGuard guard(k.device());
+    int64_t ks[3], vs[3];
+    strides_into(ks, k), strides_into(vs, v);
+    if (na1d_sink_append(&c, ptr(k), ptr(v), ks, vs, int_ptr(lengths), int_ptr(t_valid), k.size(1), stream_of(k)) != NA1D_OK) return false;
+    written({&kc, &vc});
+    if (kr) written({&*kr, &*vr});
+    return true;
+}
+
 // ------------------------------------------------------------------------------------------------ an encoder layer in training
 // What train.py's node does between its checks and its bookkeeping.  A layer is some two dozen allocations and a dozen
 // launches each way: through the interpreter they took longer than the kernels of a small batch.
@@ -517,6 +663,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("qk", &qk);
     m.def("av", &av);
     m.def("head", &head);
+    m.def("sink", &sink);
+    m.def("sink_over", &sink_over);
+    m.def("sink_append", &sink_append);
     m.def("train_forward", &train_forward);
     m.def("train_backward", &train_backward);
 }

@@ -70,6 +70,18 @@ def _window(win_size, sinks):
     return min(int(win_size), 1 << 40), min(int(sinks), 1 << 40)
 
 
+def _nodes(win_size, sinks):
+    """The native path, where what it is given are numbers that it takes as they are."""
+    return _lib.nodes() if type(win_size) is type(sinks) is int and 0 < win_size < 1 << 40 and 0 <= sinks < 1 << 40 else None
+
+
+def _written(*caches):
+    for c in caches:
+        for t in c if isinstance(c, Rows4) else (c,):
+            if not t.is_inference():
+                torch.autograd.graph.increment_version(t)
+
+
 def _scale(scale, C):
     return float(C ** -0.5 if scale is None else scale)
 
@@ -179,15 +191,14 @@ def sink_attention(q, k, v, win_size, sinks=0, t_valid=None, scale=None):
     may hold anything, and their outputs and gradients are 0.  The tokens before have to be finite.  ``scale`` (finite and above
     0) defaults to ``C ** -0.5``.  Returns ``[N, T, heads, C]``.  The gradients cannot be differentiated again (asking for it raises).
     """
+    nodes = _nodes(win_size, sinks)
+    out = None if nodes is None else nodes.sink(q, k, v, win_size, sinks, t_valid, scale)
+    if out is not None:
+        return out
     check_operands(q, k, v, t_valid)
     _check_gpu(q)
     win_size, sinks = _window(win_size, sinks)
     scale = _scale(scale, q.shape[3])
-    nodes = _lib.nodes()
-    if nodes is not None and hasattr(nodes, "sink"):
-        out = nodes.sink(q, k, v, t_valid, win_size, sinks, scale)
-        if out is not None:
-            return out
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _SinkAttention.apply(q, k, v, t_valid, win_size, sinks, scale)
     return sink_forward(q, k, v, t_valid, win_size, sinks, scale, False)[0]
@@ -235,6 +246,12 @@ def _device(cache):
     return cache[0].device if isinstance(cache, Rows4) else cache.device
 
 
+def _parts(k_cache, v_cache):
+    """Codes or rows of both, and their ranges (None: rows in 16 bits)."""
+    k, v = (c if isinstance(c, Rows4) else (c, None) for c in (k_cache, v_cache))
+    return k[0], v[0], k[1], v[1]
+
+
 def _check_caches(k_cache, v_cache, sinks):
     (shape, dtype), other = _check_cache(k_cache, "k_cache"), _check_cache(v_cache, "v_cache")
     if (shape, dtype) != other or isinstance(k_cache, Rows4) != isinstance(v_cache, Rows4):
@@ -276,6 +293,9 @@ def cache_append(k, v, k_cache, v_cache, lengths=None, sinks=0, t_valid=None):
 
     ``t_valid`` int32 ``[N]``: only so many of a stream's tokens are there.  What a later token cannot see is not kept: of the tokens behind the
     sinks the last ``capacity - sinks`` are.  The caches are written to in place, and nothing is returned; no gradient goes through them."""
+    nodes = _nodes(1, sinks)
+    if nodes is not None and nodes.sink_append(k, v, *_parts(k_cache, v_cache), lengths, sinks, t_valid):
+        return
     _, sinks = _window(1, sinks)
     shape, dtype = _check_caches(k_cache, v_cache, sinks)
     device = _device(k_cache)
@@ -292,9 +312,14 @@ def cache_append(k, v, k_cache, v_cache, lengths=None, sinks=0, t_valid=None):
     with torch.cuda.device(device):
         _lib.check(_lib.load().na1d_sink_append(ctypes.byref(c), _lib._p(k), _lib._p(v), _strides(k), _strides(v), _lib._p(lengths), _lib._p(t_valid), k.shape[1],
                                                 _lib._stream(k)), "na1d_sink_append")
+    _written(k_cache, v_cache)
 
 
 def _over_cache(q, k, v, k_cache, v_cache, lengths, win_size, sinks, scale):
+    nodes = None if lengths is None else _nodes(win_size, sinks)
+    out = None if nodes is None else nodes.sink_over(q, k, v, *_parts(k_cache, v_cache), lengths, win_size, sinks, scale)
+    if out is not None:
+        return out
     win_size, sinks = _window(win_size, sinks)
     shape, dtype = _check_caches(k_cache, v_cache, sinks)
     device = _device(k_cache)
@@ -327,6 +352,7 @@ def _over_cache(q, k, v, k_cache, v_cache, lengths, win_size, sinks, scale):
         else:
             _lib.check(lib.na1d_sink_step(ctypes.byref(c), _lib._p(out), _lib._p(q), _lib._p(k), _lib._p(v), _strides(q), _strides(k), _strides(v), *tail),
                        "na1d_sink_step")
+            _written(k_cache, v_cache)
     return out
 
 
