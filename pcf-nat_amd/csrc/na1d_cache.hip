@@ -5,9 +5,9 @@
 // tokens see are numbered 0 .. total - 1: the sinks that lie before the window of the first of them, then the positions from there on.
 //
 // A workgroup has one head of keys of one sequence, 16 to 64 rows of queries (a token's heads of the group, then the next token's) and a share of
-// the keys.  What bounds these kernels is memory: every byte of the cache is used for a handful of queries.  So each of the four waves walks
-// its own units of keys and keeps the next one in flight, straight into a part of LDS of its own: no barriers, and every wave's loads overlap all other
-// work.  The waves join their sums at the end, workgroups that share a head's keys through memory (cache_join_kernel).
+// the keys.  What bounds these kernels is memory: every byte of the cache is used for a handful of queries.  So each wave walks its own units of
+// keys and keeps the next one in flight, straight into a part of LDS of its own: no barriers, and every wave's loads overlap all other work.  The
+// waves join their sums at the end, workgroups that share a head's keys through memory (cache_join_kernel).
 //
 // 4 bits: a row is codes c, two to a byte, with its least value and the step from one code to the next: x = low + step c.  Both products take the
 // codes as they are, exact in 16 bits:
@@ -70,34 +70,45 @@ __device__ inline void share_of(int split, int splits, int unit, const Seen &s, 
 }
 
 // ------------------------------------------------------------------------------------------------ rows in 4 bits
-// One row by one wave, two channels to a lane: its code's byte, and the row's step and least value.  The step is rounded to the rows' type; the codes
-// are of the step as it is stored.
-template <class DT> __device__ inline uint32_t quantized(uint32_t pair, bool there, uint32_t &range) {
-    const float x = DT::to_f32((uint16_t)(pair & 0xffffu)), y = DT::to_f32((uint16_t)(pair >> 16));
-    float low = there ? __builtin_fminf(x, y) : __builtin_inff(), high = there ? __builtin_fmaxf(x, y) : -__builtin_inff();
+// One row by as many lanes as have eight of its channels each (4, 8 or 16, from a multiple of that on; `there`: this lane has some): their codes, and the row's
+// step and least value.  The step is rounded to the rows' type; the codes are of the step as it is stored.
+template <int CTRL> __device__ inline float from_lane(float x) { return __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), CTRL, 0xf, 0xf, true)); }
+template <class DT> __device__ inline uint32_t quantized(const Chunk8 &c, bool there, int lanes, uint32_t &range) {
+    float x[8];
+    unpack8<DT>(c, x);
+    float low = __builtin_inff(), high = -__builtin_inff();
+    if (there) {
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        low = __builtin_fminf(low, __shfl_xor(low, d));
-        high = __builtin_fmaxf(high, __shfl_xor(high, d));
+        for (int i = 0; i < 8; ++i) low = __builtin_fminf(low, x[i]), high = __builtin_fmaxf(high, x[i]);
     }
+    auto meet = [&](float l, float h) { low = __builtin_fminf(low, l), high = __builtin_fmaxf(high, h); };
+    meet(from_lane<0xb1>(low), from_lane<0xb1>(high));           // lanes 1, 0, 3, 2 of four
+    meet(from_lane<0x4e>(low), from_lane<0x4e>(high));           // lanes 2, 3, 0, 1
+    if (lanes > 4) meet(from_lane<0x141>(low), from_lane<0x141>(high));       // eight lanes in reverse
+    if (lanes > 8) meet(from_lane<0x140>(low), from_lane<0x140>(high));       // sixteen
     const uint16_t step16 = DT::from_f32((high - low) / 15.f);
     const float step = DT::to_f32(step16);
     range = step16 | (uint32_t)DT::from_f32(low) << 16;
-    auto code = [&](float v) { return step > 0.f ? (uint32_t)__builtin_fminf(__builtin_fmaxf(__builtin_rintf((v - low) / step), 0.f), 15.f) : 0u; };
-    return code(x) | code(y) << 4;
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w |= (step > 0.f ? (uint32_t)__builtin_fminf(__builtin_fmaxf(__builtin_rintf((x[i] - low) / step), 0.f), 15.f) : 0u) << (4 * i);
+    return w;
 }
 
-// Tokens into the cache: row `token` of k or v by one wave (16 bits: 16 bytes to a lane; 4: two channels to a lane).
+// Tokens into the cache: lane `part` of those that a row has (8 channels each) stores its own.
+__device__ inline int lanes_to_row(int width) { return width <= 64 ? 4 : width <= 128 ? 8 : 16; }      // width: of 16-bit rows, bytes
 template <class DT, int BITS>
-__device__ inline void store_token(char *cache, char *ranges, int row, const char *x, int width, int lane) {
+__device__ inline void store_token(char *cache, char *ranges, int row, const char *x, int width, int part, int lanes) {
+    const bool there = part * 16 < width;
+    Chunk8 c = {{0u, 0u, 0u, 0u}};
+    if (there) c = *reinterpret_cast<const Chunk8 *>(x + part * 16);
     if constexpr (BITS == 16) {
-        if (lane * 16 < width) *reinterpret_cast<u32x4 *>(cache + (int64_t)row * width + lane * 16) = *reinterpret_cast<const u32x4 *>(x + lane * 16);
+        if (there) *reinterpret_cast<Chunk8 *>(cache + (int64_t)row * width + part * 16) = c;
     } else {
-        const bool there = lane * 4 < width;
         uint32_t range;
-        const uint32_t code = quantized<DT>(there ? *reinterpret_cast<const uint32_t *>(x + lane * 4) : 0u, there, range);
-        if (there) cache[(int64_t)row * (width / 4) + lane] = (char)code;
-        if (lane == 0) *reinterpret_cast<uint32_t *>(ranges + (int64_t)row * 4) = range;
+        const uint32_t w = quantized<DT>(c, there, lanes, range);
+        if (there) *reinterpret_cast<uint32_t *>(cache + (int64_t)row * (width / 4) + part * 4) = w;
+        if (part == 0) *reinterpret_cast<uint32_t *>(ranges + (int64_t)row * 4) = range;
     }
 }
 // Tokens of sample n at positions lengths[n] on: those that a later token can see, sinks and the last `ring` ones.
@@ -105,18 +116,19 @@ template <class DT, int BITS>
 __global__ void __launch_bounds__(kThreads)
 cache_append_kernel(char *__restrict__ kc, char *__restrict__ vc, char *__restrict__ kr, char *__restrict__ vr, const char *__restrict__ k, const char *__restrict__ v,
                     const int32_t *__restrict__ lengths, const int32_t *__restrict__ t_valid, int T, int blocks, CacheArgs a) {
-    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const uint32_t head = uniform(blockIdx.x / (uint32_t)blocks), sample = uniform(head / (uint32_t)a.K), kv = head - sample * a.K;
     const int block = (int)(blockIdx.x - head * blocks), start = lengths ? lengths[sample] : 0;
     const int tv = t_valid ? max(0, min(T, t_valid[sample])) : T;
     if (start < 0 || start > kLatest) return;
+    const int lanes = lanes_to_row(a.width), part = threadIdx.x & (lanes - 1), slot = (int)((uint32_t)threadIdx.x / (uint32_t)lanes), slots = kThreads / lanes;
     const char *kx = k + sample * a.k.sample + kv * a.k.head, *vx = v + sample * a.v.sample + kv * a.v.head;
+    kc += head * a.slice, vc += head * a.slice, kr += head * a.ranges, vr += head * a.ranges;
     // the last `ring` tokens, and before them those that are sinks
     const int tail = max(0, tv - a.ring), early = max(0, min(tail, a.sinks - start)), count = early + tv - tail;
-    for (int j = block * kWaves + wave; j < count; j += blocks * kWaves) {
+    for (int j = block * slots + slot; j < count; j += blocks * slots) {
         const int t = j < early ? j : tail + (j - early), row = row_of(start + t, a.sinks, a.ring);
-        store_token<DT, BITS>(kc + head * a.slice, kr + head * a.ranges, row, kx + t * a.k.row, a.width, lane);
-        store_token<DT, BITS>(vc + head * a.slice, vr + head * a.ranges, row, vx + t * a.v.row, a.width, lane);
+        store_token<DT, BITS>(kc, kr, row, kx + t * a.k.row, a.width, part, lanes);
+        store_token<DT, BITS>(vc, vr, row, vx + t * a.v.row, a.width, part, lanes);
     }
 }
 // Rows as the values that they stand for: eight channels to a thread.
@@ -162,14 +174,14 @@ template <int C, int QT> struct Sums {
     }
 };
 template <int C, int QT> constexpr int kJoinRow = C + 4;      // floats: rows of the waves' sums in LDS, apart from each other's banks
-template <int C, int QT> constexpr int kJoinBytes = kWaves * 16 * QT * (kJoinRow<C, QT> + 2) * 4;
+template <int C, int QT, int NW> constexpr int kJoinBytes = NW * 16 * QT * (kJoinRow<C, QT> + 2) * 4;
 
 // The waves' sums together: to the output, or (several shares) to memory.
-template <class DT, int C, int QT>
+template <class DT, int C, int QT, int NW>
 __device__ inline void join_waves(const Sums<C, QT> &s, char *smem, char *out, float *partial, uint32_t head, uint32_t sample, uint32_t kv, int block, int split, int wave, int lane,
                                   const CacheArgs &a) {
     constexpr int kRows = 16 * QT, kQuads = C / 4, kRow = kJoinRow<C, QT>;
-    float *rows = reinterpret_cast<float *>(smem), *stats = rows + kWaves * kRows * kRow;
+    float *rows = reinterpret_cast<float *>(smem), *stats = rows + NW * kRows * kRow;
     const int g = lane >> 4, n = lane & 15;
     __syncthreads();            // the waves are done with what they staged
 #pragma unroll
@@ -181,15 +193,15 @@ __device__ inline void join_waves(const Sums<C, QT> &s, char *smem, char *out, f
         if (g == 0) stats[2 * r] = s.m[h], stats[2 * r + 1] = l;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < kRows * kQuads; i += kThreads) {
+    for (int i = threadIdx.x; i < kRows * kQuads; i += 64 * NW) {
         const int r = i / kQuads, ch = (i % kQuads) * 4, row = block * kRows + r;
         if (row >= a.rows || 2 * ch >= a.width) continue;
         float m = kNoMaximum, l = 0.f;
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) m = __builtin_fmaxf(m, stats[2 * (w * kRows + r)]);
+        for (int w = 0; w < NW; ++w) m = __builtin_fmaxf(m, stats[2 * (w * kRows + r)]);
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
+        for (int w = 0; w < NW; ++w) {
             const float f = __builtin_amdgcn_exp2f(stats[2 * (w * kRows + r)] - m);
             l = __builtin_fmaf(stats[2 * (w * kRows + r) + 1], f, l);
             o += *reinterpret_cast<const f32x4 *>(rows + (w * kRows + r) * kRow + ch) * f;
@@ -242,19 +254,18 @@ struct Place {
         kv = head - sample * a.K;
     }
 };
-// The last share stores the call's tokens; they are read back like all others.  Workgroups of other blocks of queries store the same.
-template <class DT, int BITS>
-__device__ inline void store_fresh(char *kc, char *vc, char *kr, char *vr, const char *k, const char *v, const Place &p, const Seen &seen, int wave, int lane, const CacheArgs &a) {
+// The last share stores the call's tokens.  (Workgroups of other blocks of queries store the same.)
+template <class DT, int BITS, int NW>
+__device__ inline void store_fresh(char *kc, char *vc, char *kr, char *vr, const char *k, const char *v, const Place &p, const Seen &seen, const CacheArgs &a) {
     if (!a.stored || p.split + 1 < a.splits || seen.total == 0) return;
-    const char *kx = k + p.sample * a.k.sample + p.kv * a.k.head, *vx = v + p.sample * a.v.sample + p.kv * a.v.head;
-    for (int j = wave; j < 2 * a.stored; j += kWaves) {
+    const int lanes = lanes_to_row(a.width), part = threadIdx.x & (lanes - 1);
+    for (int j = (int)((uint32_t)threadIdx.x / (uint32_t)lanes); j < 2 * a.stored; j += 64 * NW / lanes) {
         const int t = j >> 1, row = row_of(seen.end - a.stored + t, a.sinks, a.ring);
-        if (j & 1)
-            store_token<DT, BITS>(vc + p.head * a.slice, vr + p.head * a.ranges, row, vx + t * a.v.row, a.width, lane);
-        else
-            store_token<DT, BITS>(kc + p.head * a.slice, kr + p.head * a.ranges, row, kx + t * a.k.row, a.width, lane);
+        const bool second = j & 1;
+        const Rows &from = second ? a.v : a.k;
+        store_token<DT, BITS>((second ? vc : kc) + p.head * a.slice, (second ? vr : kr) + p.head * a.ranges, row,
+                              (second ? v : k) + p.sample * from.sample + p.kv * from.head + t * from.row, a.width, part, lanes);
     }
-    __syncthreads();
 }
 // Rows n of the tiles of a block of queries: where they are, and when.
 struct QueryRow {
@@ -275,8 +286,15 @@ __device__ inline void reads_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "m
 // =============================================================================
 // Rows in 16 bits: units of 32 keys
 // =============================================================================
-template <class DT, int C, int QT>
-__global__ void __launch_bounds__(kThreads)
+// One load that writes LDS directly, from anywhere: lane l's 16 bytes land at lds + 16 * l.  As load_to_lds(), unknown to the compiler.
+__device__ inline void load_from(const char *p, LDS_PTR(char) lds) {
+    const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)reinterpret_cast<uintptr_t>(lds));
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(p) : "memory");
+}
+// A key's row is in the cache, or with the call's tokens: a step does not wait for its own stores.  Past the share's last key that one is loaded again, and
+// past a row's channels its first ones: finite, and met by probabilities and queries of zero.
+template <class DT, int C, int QT, int NW>
+__global__ void __launch_bounds__(64 * NW)
 cache_attend_kernel(char *__restrict__ out, float *__restrict__ partial, const char *__restrict__ q, const char *__restrict__ k, const char *__restrict__ v,
                     char *kc, char *vc, const int32_t *__restrict__ lengths, uint32_t items, CacheArgs a) {
     using LL = Lds<C>;
@@ -286,10 +304,8 @@ cache_attend_kernel(char *__restrict__ out, float *__restrict__ partial, const c
     LDS_PTR(char) mine = (LDS_PTR(char))smem + wave * 2 * kStage;
     const Place p(items, a);
     const Seen seen(uniform(lengths[p.sample]), a);
-    store_fresh<DT, 16>(kc, vc, nullptr, nullptr, k, v, p, seen, wave, lane, a);
     int i0, i1;
     share_of(p.split, a.splits, kUnit, seen, a.fresh, i0, i1);
-    const Rsrc ks = make_rsrc(kc + p.head * a.slice, (int)a.slice), vs = make_rsrc(vc + p.head * a.slice, (int)a.slice);
 
     RowOperand<C> qop[QT];
     int when[QT];
@@ -303,14 +319,18 @@ cache_attend_kernel(char *__restrict__ out, float *__restrict__ partial, const c
         if (RowOperand<C>::k16)
             qop[h].w16[0] = r.position >= 0 && 8 * g < a.width ? *reinterpret_cast<const u32x2 *>(q + r.at + 8 * g) : u32x2{0u, 0u};
     }
-    const int unit16 = lane % LL::kUnits;
+    const char *ks = kc + p.head * a.slice, *vs = vc + p.head * a.slice;
+    const char *kx = k + p.sample * a.k.sample + p.kv * a.k.head, *vx = v + p.sample * a.v.sample + p.kv * a.v.head;
+    const int old = seen.total - a.stored;
     auto stage = [&](int i, LDS_PTR(char) to) {
 #pragma unroll
         for (int c = 0; c < kRegion / kChunk; ++c) {
-            const int r = c * kChunkKeys + lane / LL::kUnits, unit = unit16 ^ LL::swz(r), key = i + r;
-            const int at = key < i1 && r < kUnit && unit * 16 < a.width ? seen.row(key) * a.width + unit * 16 : kNowhere;
-            load_to_lds<16, kReadShared>(ks, to + c * kChunk, at);
-            load_to_lds<16, kReadShared>(vs, to + kRegion + c * kChunk, at);
+            const int r = c * kChunkKeys + lane / LL::kUnits, unit = (lane % LL::kUnits) ^ LL::swz(r), key = min(i + r, i1 - 1);
+            const int byte = unit * 16 < a.width ? unit * 16 : 0;
+            const int64_t at = (int64_t)seen.row(key) * a.width + byte;
+            const bool fresh = key >= old;
+            load_from(fresh ? kx + (key - old) * a.k.row + byte : ks + at, to + c * kChunk);
+            load_from(fresh ? vx + (key - old) * a.v.row + byte : vs + at, to + kRegion + c * kChunk);
         }
     };
     RowLane<C> row_lane;
@@ -329,10 +349,15 @@ cache_attend_kernel(char *__restrict__ out, float *__restrict__ partial, const c
         for (int s = 0; s < RowOperand<C>::k32; ++s) settle(qop[h].w32[s]);
         if (RowOperand<C>::k16) settle(qop[h].w16[0]);
     }
-    for (; i < i1; i += kUnit * kWaves, at ^= kStage) {
+    store_fresh<DT, 16, NW>(kc, vc, nullptr, nullptr, k, v, p, seen, a);
+    for (; i < i1; i += kUnit * NW, at ^= kStage) {
         reads_done();
-        stage(i + kUnit * kWaves, mine + (at ^ kStage));      // past the share's end: nothing but zeros
-        wait_all_but<kLoads>();
+        if (i + kUnit * NW < i1) {
+            stage(i + kUnit * NW, mine + (at ^ kStage));
+            wait_all_but<kLoads>();
+        } else {
+            wait_direct();
+        }
         LDS_PTR(char) k_lds = mine + at;
         LDS_PTR(char) v_lds = k_lds + kRegion;
         f32x4 s[QT][2];
@@ -381,8 +406,7 @@ cache_attend_kernel(char *__restrict__ out, float *__restrict__ partial, const c
             for (int h = 0; h < QT; ++h) sums.o[h][ct] = Mma<DT>::k32(vv, pp[h], sums.o[h][ct]);
         }
     }
-    wait_direct();              // the last loads have landed before their place is used for something else
-    join_waves<DT, C, QT>(sums, smem, out, partial, p.head, p.sample, p.kv, p.block, p.split, wave, lane, a);
+    join_waves<DT, C, QT, NW>(sums, smem, out, partial, p.head, p.sample, p.kv, p.block, p.split, wave, lane, a);
 }
 
 // =============================================================================
@@ -411,8 +435,8 @@ __device__ inline int key_of_row(int row) {
     const int kt = row >> 4, g = (row >> 2) & 3, r = row & 3;
     return 16 * g + 8 * (kt >> 1) + 2 * (kt & 1) + (r >> 1) + 4 * (r & 1);
 }
-template <class DT, int C, int QT>
-__global__ void __launch_bounds__(kThreads)
+template <class DT, int C, int QT, int NW>
+__global__ void __launch_bounds__(64 * NW)
 cache_attend4_kernel(char *__restrict__ out, float *__restrict__ partial, const char *__restrict__ q, const char *__restrict__ k, const char *__restrict__ v,
                      char *kc, char *vc, char *kr, char *vr, const int32_t *__restrict__ lengths, uint32_t items, CacheArgs a) {
     constexpr int CT = C / 16, S = C / 32, kUnit = 64, kRow = C / 2, kUnits = kRow / 16;
@@ -423,7 +447,8 @@ cache_attend4_kernel(char *__restrict__ out, float *__restrict__ partial, const 
     LDS_PTR(char) mine = (LDS_PTR(char))smem + wave * 2 * kStage;
     const Place p(items, a);
     const Seen seen(uniform(lengths[p.sample]), a);
-    store_fresh<DT, 4>(kc, vc, kr, vr, k, v, p, seen, wave, lane, a);
+    store_fresh<DT, 4, NW>(kc, vc, kr, vr, k, v, p, seen, a);
+    if (a.stored) __syncthreads();      // the call's tokens are read back as the cache holds them
     int i0, i1;
     share_of(p.split, a.splits, kUnit, seen, a.fresh, i0, i1);
     const Rsrc ks = make_rsrc(kc + p.head * a.slice, (int)a.slice), vs = make_rsrc(vc + p.head * a.slice, (int)a.slice);
@@ -481,10 +506,14 @@ cache_attend4_kernel(char *__restrict__ out, float *__restrict__ partial, const 
         }
         qsum[h] = xor_sum(sum) * scale2;
     }
-    for (; i < i1; i += kUnit * kWaves, at ^= kStage) {
+    for (; i < i1; i += kUnit * NW, at ^= kStage) {
         reads_done();
-        stage(i + kUnit * kWaves, mine + (at ^ kStage));
-        wait_all_but<kLoads>();
+        if (i + kUnit * NW < i1) {
+            stage(i + kUnit * NW, mine + (at ^ kStage));
+            wait_all_but<kLoads>();
+        } else {
+            wait_direct();
+        }
         LDS_PTR(char) k_lds = mine + at;
         LDS_PTR(char) v_lds = k_lds + kCodes;
         LDS_PTR(char) r_lds = v_lds + kCodes;
@@ -568,24 +597,32 @@ cache_attend4_kernel(char *__restrict__ out, float *__restrict__ partial, const 
             }
         }
     }
-    wait_direct();
 #pragma unroll
     for (int h = 0; h < QT; ++h) {
         const float extra = __builtin_fmaf(-23.5f, steps[h][0], xor_sum(mids[h]));
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) sums.o[h][ct] += f32x4{extra, extra, extra, extra};
     }
-    join_waves<DT, C, QT>(sums, smem, out, partial, p.head, p.sample, p.kv, p.block, p.split, wave, lane, a);
+    join_waves<DT, C, QT, NW>(sums, smem, out, partial, p.head, p.sample, p.kv, p.block, p.split, wave, lane, a);
 }
 
 // ----------------------------------------------------------------------------- launchers
-// Blocks of 16, 32 or 64 rows of queries.  A head's keys are shared by as many workgroups as fill the card four times, each with two units of keys
-// for each of its waves at least.
+constexpr int kFewWaves = kWaves;
+// Bytes of LDS that a wave stages into, and the most waves of a workgroup that find room.
+constexpr int staged_bytes(int C, bool four) { return four ? 2 * 2 * (64 * (C / 2) + 64 * 4) : 2 * 2 * (C <= 16 ? kChunk : 64 * C); }
+constexpr int most_waves(int C, bool four) { return staged_bytes(C, four) > 20480 ? kFewWaves : staged_bytes(C, four) > 10240 ? 8 : 16; }
+int width_of(const na1d_sink_cache &c) { return c.bits == 4 ? c.head_dim : padded_width(c.head_dim); }
+
 struct CachePlan {
-    int tiles;
+    int tiles, waves;
     CacheArgs a;
     int64_t items;
 };
+// Blocks of 16, 32 or 64 rows of queries.  Where the card is not full with a workgroup to every head of keys, and a large one gets through them with at most
+// kSerial units to a wave, that one has them all, and a launch less: one stream's step over 1028 keys, 4 heads of 64, takes 10.4 us in two kernels of
+// 16 workgroups and then of one.  Otherwise workgroups of four waves, as many to a head as occupy the card in whole rounds, with two units of keys to a wave
+// at least.
+constexpr int kSerial = 5;
 CachePlan cache_plan(const na1d_sink_cache &c, int64_t fresh, int heads, int64_t window) {
     CachePlan p{};
     CacheArgs &a = p.a;
@@ -593,32 +630,43 @@ CachePlan cache_plan(const na1d_sink_cache &c, int64_t fresh, int heads, int64_t
     p.tiles = a.rows <= 16 ? 1 : a.rows <= 32 ? 2 : 4;
     a.blocks = (a.rows + 16 * p.tiles - 1) / (16 * p.tiles);
     a.window = (int)window, a.sinks = (int)c.sinks, a.ring = (int)(c.capacity - c.sinks), a.width = 2 * c.head_dim;
+    const bool four = c.bits == 4;
+    const int C = width_of(c), unit = four ? 64 : 32, wide = most_waves(C, four);
     const int64_t most = std::min(c.capacity, c.sinks + window + fresh - 1), heads_blocks = c.N * c.kv_heads * a.blocks;
-    const int64_t unit = c.bits == 4 ? 64 : 32;
-    a.splits = (int)std::max<int64_t>(1, std::min<int64_t>({1024 / std::max<int64_t>(1, heads_blocks), most / (2 * unit * kWaves), 256}));
-    a.slice = c.capacity * (c.bits == 4 ? c.head_dim / 2 : 2 * c.head_dim);
-    a.ranges = c.capacity * 4;
+    p.waves = kFewWaves, a.splits = 1;
+    if (p.tiles == 1 && wide > kFewWaves && heads_blocks <= 256 && most <= (int64_t)kSerial * unit * wide) {
+        p.waves = wide;
+    } else {
+        const int64_t slots = 256 * std::min(4, 160 * 1024 / (kFewWaves * staged_bytes(C, four))), longest = std::max<int64_t>(1, most / (2 * unit * kFewWaves));
+        auto wasted = [&](int64_t s) { return heads_blocks * s % slots ? slots - heads_blocks * s % slots : 0; };      // of the last round
+        int64_t s = std::max<int64_t>(1, slots / std::max<int64_t>(1, heads_blocks));
+        if (heads_blocks > slots / 2)
+            for (s = 1; s < 4 && wasted(s) * 10 > heads_blocks * s; ++s) {}
+        a.splits = (int)std::min<int64_t>({s, longest, 256});
+    }
+    a.slice = c.capacity * (four ? c.head_dim / 2 : 2 * c.head_dim);
+    a.ranges = four ? c.capacity * 4 : 0;
     p.items = heads_blocks * a.splits;
     return p;
 }
 Rows rows_by(const int64_t *s) { return Rows{2 * s[0], 2 * s[1], 2 * s[2]}; }
-int width_of(const na1d_sink_cache &c) { return c.bits == 4 ? c.head_dim : padded_width(c.head_dim); }
 
-template <class DT, int C, int QT, bool FOUR>
+template <class DT, int C, int QT, int NW, bool FOUR>
 int launch_attend(const na1d_sink_cache &c, const CachePlan &p, void *out, const void *q, const void *k, const void *v, const int32_t *lengths, float *ws, hipStream_t s) {
-    constexpr size_t staged = FOUR ? kWaves * 2 * 2 * (64 * (C / 2) + 64 * 4) : kWaves * 2 * 2 * (size_t)region_bytes<C>(2);
-    constexpr size_t lds = staged > (size_t)kJoinBytes<C, QT> ? staged : (size_t)kJoinBytes<C, QT>;
+    constexpr size_t staged = (size_t)NW * staged_bytes(C, FOUR);
+    constexpr size_t lds = staged > (size_t)kJoinBytes<C, QT, NW> ? staged : (size_t)kJoinBytes<C, QT, NW>;
+    static_assert(lds <= 160 * 1024, "a CU's LDS");
     const char *dt = DT::tag == NA1D_BF16 ? "BF16" : "FP16";
     const bool joins = p.a.splits > 1;
     if constexpr (FOUR) {
-        if (!allow_lds(cache_attend4_kernel<DT, C, QT>, lds)) return NA1D_ERR_LAUNCH;
-        note_kernel_as("cache_attend4_kernel<%s, %d, %d>", dt, C, QT);
-        launch_kernel_span(joins ? 1 : 3, cache_attend4_kernel<DT, C, QT>, (unsigned)p.items, (unsigned)kThreads, lds, s, (char *)out, ws, (const char *)q, (const char *)k,
+        if (!allow_lds(cache_attend4_kernel<DT, C, QT, NW>, lds)) return NA1D_ERR_LAUNCH;
+        note_kernel_as("cache_attend4_kernel<%s, %d, %d, %d>", dt, C, QT, NW);
+        launch_kernel_span(joins ? 1 : 3, cache_attend4_kernel<DT, C, QT, NW>, (unsigned)p.items, 64u * NW, lds, s, (char *)out, ws, (const char *)q, (const char *)k,
                            (const char *)v, (char *)c.k, (char *)c.v, (char *)c.k_ranges, (char *)c.v_ranges, lengths, (uint32_t)p.items, p.a);
     } else {
-        if (!allow_lds(cache_attend_kernel<DT, C, QT>, lds)) return NA1D_ERR_LAUNCH;
-        note_kernel_as("cache_attend_kernel<%s, %d, %d>", dt, C, QT);
-        launch_kernel_span(joins ? 1 : 3, cache_attend_kernel<DT, C, QT>, (unsigned)p.items, (unsigned)kThreads, lds, s, (char *)out, ws, (const char *)q, (const char *)k,
+        if (!allow_lds(cache_attend_kernel<DT, C, QT, NW>, lds)) return NA1D_ERR_LAUNCH;
+        note_kernel_as("cache_attend_kernel<%s, %d, %d, %d>", dt, C, QT, NW);
+        launch_kernel_span(joins ? 1 : 3, cache_attend_kernel<DT, C, QT, NW>, (unsigned)p.items, 64u * NW, lds, s, (char *)out, ws, (const char *)q, (const char *)k,
                            (const char *)v, (char *)c.k, (char *)c.v, lengths, (uint32_t)p.items, p.a);
     }
     if (joins) {
@@ -628,8 +676,10 @@ int launch_attend(const na1d_sink_cache &c, const CachePlan &p, void *out, const
     return launch_status();
 }
 template <class DT, int C, bool FOUR, class... A> int launch_tiles(const na1d_sink_cache &c, const CachePlan &p, A... args) {
-    if (p.tiles == 1) return launch_attend<DT, C, 1, FOUR>(c, p, args...);
-    return p.tiles == 2 ? launch_attend<DT, C, 2, FOUR>(c, p, args...) : launch_attend<DT, C, 4, FOUR>(c, p, args...);
+    if constexpr (most_waves(C, FOUR) > kFewWaves)
+        if (p.waves > kFewWaves) return launch_attend<DT, C, 1, most_waves(C, FOUR), FOUR>(c, p, args...);
+    if (p.tiles == 1) return launch_attend<DT, C, 1, kFewWaves, FOUR>(c, p, args...);
+    return p.tiles == 2 ? launch_attend<DT, C, 2, kFewWaves, FOUR>(c, p, args...) : launch_attend<DT, C, 4, kFewWaves, FOUR>(c, p, args...);
 }
 template <class DT, class... A> int launch_width(const na1d_sink_cache &c, const CachePlan &p, A... args) {
     const bool four = c.bits == 4;
@@ -661,9 +711,9 @@ int cache_append(const na1d_sink_cache &c, const void *k, const void *v, const i
                  hipStream_t s) {
     CachePlan p = cache_plan(c, 1, c.kv_heads, 1);
     p.a.k = rows_by(k_strides), p.a.v = rows_by(v_strides);
-    const int64_t heads = c.N * c.kv_heads, tokens = std::min(T, c.capacity);
-    // a wave to four tokens and more where there are enough of them to fill the card
-    const int64_t blocks = std::max<int64_t>(1, std::min((tokens + kWaves - 1) / kWaves, std::max<int64_t>((tokens + 4 * kWaves - 1) / (4 * kWaves), 4096 / heads)));
+    // workgroups fill the card eight times, where there are so many tokens
+    const int64_t heads = c.N * c.kv_heads, tokens = std::min(T, c.capacity), slots = kThreads / (c.head_dim <= 32 ? 4 : c.head_dim <= 64 ? 8 : 16);
+    const int64_t blocks = std::max<int64_t>(1, std::min((tokens + slots - 1) / slots, 16384 / heads));
     if (heads * blocks > 0x7fffff00LL) return NA1D_ERR_UNSUPPORTED;
     auto go = [&](auto kern) {
         launch_kernel(kern, (unsigned)(heads * blocks), 0, s, (char *)c.k, (char *)c.v, (char *)c.k_ranges, (char *)c.v_ranges, (const char *)k, (const char *)v, lengths, t_valid,

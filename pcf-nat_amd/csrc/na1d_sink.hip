@@ -5,7 +5,7 @@
 // attention of na1d_global.hip: S^T tiles of 16 keys x 16 queries, an online softmax whose row statistics are lane-local up to a
 // reduction over the four lane groups, and the rounded probabilities fed straight back as the B operand of O^T += V^T P^T.
 //
-// A workgroup of the forward and of dQ owns a strip of one head's queries and walks the keys in chunks of 64 that its four waves share
+// A workgroup of the forward and of dQ owns a strip of one head's queries and walks the keys in chunks of 32 that its four waves share
 // through LDS: the chunks that hold sinks, then those that the strip's windows reach.  A workgroup of dK and dV owns a strip of
 // one key head's rows and walks the queries of all the heads of its group.  A chunk that all rows of a wave see whole needs no mask, one that
 // none of them sees is passed over by that wave.
@@ -20,8 +20,11 @@ namespace na1d {
 namespace mfma {
 namespace {
 
-constexpr int kChunkTiles = 4, kChunkRows = 16 * kChunkTiles;
+constexpr int kChunkTiles = 4, kChunkRows = 16 * kChunkTiles;      // queries that dK and dV take at a time, and rows of a strip (twice that in large forwards)
 static_assert(kChunkTiles == kWaves, "row constants of a chunk are loaded by one wave to a tile");
+// Keys that the forward and dQ take at a time.  64 of them cost registers and LDS that another wave to a SIMD can have: forward of 16 x 16 x 1000, 64 channels,
+// window 128, 46.5 -> 43 us, 2 x 16 x 8192, 128 channels, window 1024, 191 -> 177.
+constexpr int kKeyTiles = 2, kKeyRows = 16 * kKeyTiles;
 constexpr float kNoMaximum = -3.4e38f;      // where a row's running maximum starts: finite, so that a chunk which a row does not see leaves it alone
 
 struct SinkRows {               // one tensor: bytes from one sample, head, row to the next
@@ -59,9 +62,9 @@ struct KeyChunks {
     int sink_end, from, end;
     __device__ inline KeyChunks(int row0, int row1, int tv, const SinkArgs &a) {
         const int last = min(row1, tv - 1);
-        end = last < row0 ? 0 : last / kChunkRows + 1;                   // nothing for a strip without a valid row
-        from = max(0, row0 - a.window + 1) / kChunkRows;
-        sink_end = min((a.sinks + kChunkRows - 1) / kChunkRows, end);
+        end = last < row0 ? 0 : last / kKeyRows + 1;                   // nothing for a strip without a valid row
+        from = max(0, row0 - a.window + 1) / kKeyRows;
+        sink_end = min((a.sinks + kKeyRows - 1) / kKeyRows, end);
         from = min(max(from, sink_end), end);
     }
     __device__ inline int first() const { return sink_end > 0 ? 0 : from; }
@@ -138,11 +141,11 @@ template <int C> __device__ inline void store_rest(char *rest, const uint32_t (&
 // Forward
 // =============================================================================
 template <class DT, int C, int QT>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 3)
 sink_fwd_kernel(char *__restrict__ out, float *__restrict__ lse, char *__restrict__ rest, const char *__restrict__ q, const char *__restrict__ k, const char *__restrict__ v,
                 const int32_t *__restrict__ t_valid, uint32_t items, SinkArgs a) {
     using LL = Lds<C>;
-    constexpr int CT = C / 16, kStep = region_bytes<C>(kChunkTiles);
+    constexpr int CT = C / 16, kStep = region_bytes<C>(kKeyTiles);
     extern __shared__ __attribute__((aligned(16))) char smem[];          // 4 * kStep bytes: K and V of two chunks
     LDS_PTR(char) kv_lds = (LDS_PTR(char))smem;
 
@@ -157,9 +160,9 @@ sink_fwd_kernel(char *__restrict__ out, float *__restrict__ lse, char *__restric
     const char *kb = k + it.sample * a.k.sample + it.kv * a.k.head, *vb = v + it.sample * a.v.sample + it.kv * a.v.head;
     const int k_lane = direct_lane_offset<C>(wave, lane, a.k.pitch, width), v_lane = direct_lane_offset<C>(wave, lane, a.v.pitch, width);
     auto stage = [&](int c, LDS_PTR(char) to) {
-        const int rows = min(kChunkRows, tv - c * kChunkRows);
-        stage_direct<C, kChunkTiles, kReadShared>(rows_of(kb, (int64_t)c * kChunkRows, rows, a.k.pitch), 0, to, kChunkTiles, wave, k_lane, a.k.pitch);
-        stage_direct<C, kChunkTiles, kReadShared>(rows_of(vb, (int64_t)c * kChunkRows, rows, a.v.pitch), 0, to + kStep, kChunkTiles, wave, v_lane, a.v.pitch);
+        const int rows = min(kKeyRows, tv - c * kKeyRows);
+        stage_direct<C, kKeyTiles, kReadShared>(rows_of(kb, (int64_t)c * kKeyRows, rows, a.k.pitch), 0, to, kKeyTiles, wave, k_lane, a.k.pitch);
+        stage_direct<C, kKeyTiles, kReadShared>(rows_of(vb, (int64_t)c * kKeyRows, rows, a.v.pitch), 0, to + kStep, kKeyTiles, wave, v_lane, a.v.pitch);
     };
     const KeyChunks chunks(row0, row_end - 1, tv, a);
     int c = chunks.first();
@@ -190,17 +193,17 @@ sink_fwd_kernel(char *__restrict__ out, float *__restrict__ lse, char *__restric
     while (c < chunks.end) {
         wait_direct();
         barrier_lds();      // this chunk has landed, and every wave is done with the one before, whose regions the next takes
-        const int next = chunks.after(c), k0 = c * kChunkRows;
+        const int next = chunks.after(c), k0 = c * kKeyRows;
         if (next < chunks.end) stage(next, kv_lds + (at ^ 2 * kStep));
         LDS_PTR(char) k_lds = kv_lds + at;
         LDS_PTR(char) v_lds = k_lds + kStep;
         at ^= 2 * kStep;
         c = next;
-        const Sight see = w0 < tv ? sight(w0, w1, k0, k0 + kChunkRows - 1, a) : kNothing;
+        const Sight see = w0 < tv ? sight(w0, w1, k0, k0 + kKeyRows - 1, a) : kNothing;
         if (see == kNothing) continue;
-        f32x4 s[QT][kChunkTiles];
+        f32x4 s[QT][kKeyTiles];
 #pragma unroll
-        for (int kt = 0; kt < kChunkTiles; ++kt) {
+        for (int kt = 0; kt < kKeyTiles; ++kt) {
             RowOperand<C> kop;
             read_rows<C>(kop, k_lds + kt * LL::kTileBytes, row_lane);
 #pragma unroll
@@ -211,18 +214,18 @@ sink_fwd_kernel(char *__restrict__ out, float *__restrict__ lse, char *__restric
             for (int h = 0; h < QT; ++h) {
                 const int row = w0 + 16 * h + n, d = row - k0 - 4 * g, stay = min(a.sinks, row + 1) - k0 - 4 * g;
 #pragma unroll
-                for (int kt = 0; kt < kChunkTiles; ++kt)
+                for (int kt = 0; kt < kKeyTiles; ++kt)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
                         if (!((uint32_t)(d - 16 * kt - r) < (uint32_t)a.window || 16 * kt + r < stay)) s[h][kt][r] = kNegInf;
             }
         }
-        u32x4 pp[QT][kChunkTiles / 2];          // probabilities of two key tiles: the B operand of a 32-deep product
+        u32x4 pp[QT][kKeyTiles / 2];          // probabilities of two key tiles: the B operand of a 32-deep product
 #pragma unroll
         for (int h = 0; h < QT; ++h) {
             float mc = kNegInf;
 #pragma unroll
-            for (int kt = 0; kt < kChunkTiles; ++kt)
+            for (int kt = 0; kt < kKeyTiles; ++kt)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) mc = __builtin_fmaxf(mc, s[h][kt][r]);
             mc = xor_max(mc) * scale2;
@@ -239,7 +242,7 @@ sink_fwd_kernel(char *__restrict__ out, float *__restrict__ lse, char *__restric
             }
             const float ref = -m[h];
 #pragma unroll
-            for (int kt = 0; kt < kChunkTiles; ++kt) {
+            for (int kt = 0; kt < kKeyTiles; ++kt) {
                 float p[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][kt][r], scale2, ref));
@@ -249,7 +252,7 @@ sink_fwd_kernel(char *__restrict__ out, float *__restrict__ lse, char *__restric
         }
         // O^T += V^T P^T over two key tiles at a time; the row sums come from the same instruction with ones in place of V^T.
 #pragma unroll
-        for (int kt = 0; kt < kChunkTiles; kt += 2) {
+        for (int kt = 0; kt < kKeyTiles; kt += 2) {
             LDS_PTR(char) blk = v_lds + kt * LL::kTileBytes;
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct) {
@@ -290,13 +293,15 @@ sink_fwd_kernel(char *__restrict__ out, float *__restrict__ lse, char *__restric
 // =============================================================================
 // Backward, query side: delta = rowsum(dO * O) and dQ = scale * dS K,  dS = P (dO V^T - delta)
 // =============================================================================
-template <class DT, int C, int QT>
+// One tile of 16 queries to a wave: with two, as in the forward, 228 registers leave two waves to a SIMD and not four, and the launches are half as
+// many workgroups: 16 x 16 x 1000, 64 channels, window 128 took 57 us and not 48, 5 x 10 x 777, 96 channels, window 100 24 and not 17.5.
+template <class DT, int C>
 __global__ void __launch_bounds__(kThreads)
 sink_dq_kernel(char *__restrict__ dq, float *__restrict__ delta, const char *__restrict__ q, const char *__restrict__ k, const char *__restrict__ v,
                const char *__restrict__ out, const char *__restrict__ dout, const float *__restrict__ lse, const char *__restrict__ rest, const int32_t *__restrict__ t_valid,
                uint32_t items, SinkArgs a) {
     using LL = Lds<C>;
-    constexpr int CT = C / 16, kStep = region_bytes<C>(kChunkTiles);
+    constexpr int CT = C / 16, kStep = region_bytes<C>(kKeyTiles);
     extern __shared__ __attribute__((aligned(16))) char smem[];          // 4 * kStep bytes
     LDS_PTR(char) kv_lds = (LDS_PTR(char))smem;
 
@@ -307,108 +312,91 @@ sink_dq_kernel(char *__restrict__ dq, float *__restrict__ delta, const char *__r
     const int head = it.kv * a.group + it.g, T = a.T, width = a.width;
     int tv = T;
     if (t_valid) tv = uniform(max(0, min(T, t_valid[it.sample])));
-    const int row0 = it.strip * (kChunkRows * QT), row_end = min(T, row0 + kChunkRows * QT);
+    const int row0 = it.strip * kChunkRows, row_end = min(T, row0 + kChunkRows);
     const char *kb = k + it.sample * a.k.sample + it.kv * a.k.head, *vb = v + it.sample * a.v.sample + it.kv * a.v.head;
     const int k_lane = direct_lane_offset<C>(wave, lane, a.k.pitch, width), v_lane = direct_lane_offset<C>(wave, lane, a.v.pitch, width);
     auto stage = [&](int c, LDS_PTR(char) to) {
-        const int rows = min(kChunkRows, tv - c * kChunkRows);
-        stage_direct<C, kChunkTiles, kReadShared>(rows_of(kb, (int64_t)c * kChunkRows, rows, a.k.pitch), 0, to, kChunkTiles, wave, k_lane, a.k.pitch);
-        stage_direct<C, kChunkTiles, kReadShared>(rows_of(vb, (int64_t)c * kChunkRows, rows, a.v.pitch), 0, to + kStep, kChunkTiles, wave, v_lane, a.v.pitch);
+        const int rows = min(kKeyRows, tv - c * kKeyRows);
+        stage_direct<C, kKeyTiles, kReadShared>(rows_of(kb, (int64_t)c * kKeyRows, rows, a.k.pitch), 0, to, kKeyTiles, wave, k_lane, a.k.pitch);
+        stage_direct<C, kKeyTiles, kReadShared>(rows_of(vb, (int64_t)c * kKeyRows, rows, a.v.pitch), 0, to + kStep, kKeyTiles, wave, v_lane, a.v.pitch);
     };
     const KeyChunks chunks(row0, row_end - 1, tv, a);
     int c = chunks.first();
     if (c < chunks.end) stage(c, kv_lds);
-    const int own = 16 * QT * wave, w0 = row0 + own, w1 = w0 + 16 * QT - 1;
+    const int own = 16 * wave, w0 = row0 + own, w1 = w0 + 15;
     const int64_t o_off = it.sample * a.o.sample + head * a.o.head, stat = ((int64_t)it.sample * a.H + head) * T + row0;
     const int valid_rows = min(row_end, tv) - row0;
     const Rsrc qs = rows_of(q + it.sample * a.q.sample + head * a.q.head, row0, valid_rows, a.q.pitch);
     const Rsrc os = rows_of(out + o_off, row0, valid_rows, a.o.pitch), gs = rows_of(dout + o_off, row0, valid_rows, a.o.pitch);
     const Rsrc ls = make_rsrc(lse + stat, (row_end - row0) * 4), ds = make_rsrc(delta + stat, (row_end - row0) * 4);
-    RowOperand<C> qop[QT], gop[QT], oop[QT];
-    float ref[QT];                                        // minus the row's log2 of its sum
-#pragma unroll
-    for (int h = 0; h < QT; ++h) {
-        const int r0 = own + 16 * h;
-        load_rows<C, kReadShared>(qop[h], qs, r0 * a.q.pitch, a.q.pitch, width, lane);
-        load_rows<C, kReadShared>(gop[h], gs, r0 * a.o.pitch, a.o.pitch, width, lane);
-        load_rows<C, kReadOnce>(oop[h], os, r0 * a.o.pitch, a.o.pitch, width, lane);
-        ref[h] = -__uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(ls, (r0 + n) * 4, 0, 0));
-    }
+    RowOperand<C> qop, gop, oop;
+    load_rows<C, kReadShared>(qop, qs, own * a.q.pitch, a.q.pitch, width, lane);
+    load_rows<C, kReadShared>(gop, gs, own * a.o.pitch, a.o.pitch, width, lane);
+    load_rows<C, kReadOnce>(oop, os, own * a.o.pitch, a.o.pitch, width, lane);
+    const float ref = -__uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(ls, (own + n) * 4, 0, 0));      // minus the row's log2 of its sum
     const float scale2 = a.scale * kLog2e;
     RowLane<C> row_lane;
     TrLane<C> tr_lane;
     row_lane.init(0, lane);
     tr_lane.init(0, lane);
-    f32x4 acc[QT][CT], minus_dl[QT];                      // the product dO . V^T starts at minus delta
+    const int tile = min(w0 / 16, (T - 1) / 16);          // a tile past the last reads the last's bytes, with zeros for dO
+    const char *bytes = kKeepsRest<DT> ? rest + (((int64_t)it.sample * a.H + head) * ((T + 15) / 16) + tile) * kRestBytes<C> : nullptr;
+    const float dl = xor_sum(dot_whole<DT, C>(gop, oop, bytes, lane));      // lane (n, g) holds a quarter of row n's channels
+    if (g == 0) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(dl), ds, (own + n) * 4, 0, 0);
+    const f32x4 minus_dl = {-dl, -dl, -dl, -dl};          // the product dO . V^T starts at minus delta
+    f32x4 acc[CT];
 #pragma unroll
-    for (int h = 0; h < QT; ++h) {
-        const int tile = min(w0 / 16 + h, (T - 1) / 16);   // a tile past the last reads the last's bytes, with zeros for dO
-        const char *bytes = kKeepsRest<DT> ? rest + (((int64_t)it.sample * a.H + head) * ((T + 15) / 16) + tile) * kRestBytes<C> : nullptr;
-        const float dl = xor_sum(dot_whole<DT, C>(gop[h], oop[h], bytes, lane));   // lane (n, g) holds a quarter of row n's channels
-        minus_dl[h] = f32x4{-dl, -dl, -dl, -dl};
-        if (g == 0) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(dl), ds, (own + 16 * h + n) * 4, 0, 0);
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) acc[h][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
+    for (int ct = 0; ct < CT; ++ct) acc[ct] = f32x4{0.f, 0.f, 0.f, 0.f};
     int at = 0;
     while (c < chunks.end) {
         wait_direct();
         barrier_lds();
-        const int next = chunks.after(c), k0 = c * kChunkRows;
+        const int next = chunks.after(c), k0 = c * kKeyRows;
         if (next < chunks.end) stage(next, kv_lds + (at ^ 2 * kStep));
         LDS_PTR(char) k_lds = kv_lds + at;
         LDS_PTR(char) v_lds = k_lds + kStep;
         at ^= 2 * kStep;
         c = next;
-        const Sight see = w0 < tv ? sight(w0, w1, k0, k0 + kChunkRows - 1, a) : kNothing;
+        const Sight see = w0 < tv ? sight(w0, w1, k0, k0 + kKeyRows - 1, a) : kNothing;
         if (see == kNothing) continue;
 #pragma unroll
-        for (int kt = 0; kt < kChunkTiles; kt += 2) {
-            u32x4 db[QT];
+        for (int kt = 0; kt < kKeyTiles; kt += 2) {
+            u32x4 db;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 RowOperand<C> kop, vop;
                 read_rows<C>(kop, k_lds + (kt + j) * LL::kTileBytes, row_lane);
                 read_rows<C>(vop, v_lds + (kt + j) * LL::kTileBytes, row_lane);
+                const f32x4 s = dot_rows_mma<DT, C>(kop, qop);
+                const f32x4 dp = dot_rows_mma<DT, C>(vop, gop, minus_dl);
+                float p[4];
 #pragma unroll
-                for (int h = 0; h < QT; ++h) {
-                    const f32x4 s = dot_rows_mma<DT, C>(kop, qop[h]);
-                    const f32x4 dp = dot_rows_mma<DT, C>(vop, gop[h], minus_dl[h]);
-                    float p[4];
+                for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], scale2, ref));
+                if (see == kPart) {
+                    const int row = w0 + n, d = row - k0 - 4 * g - 16 * (kt + j), stay = min(a.sinks, row + 1) - k0 - 4 * g - 16 * (kt + j);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], scale2, ref[h]));
-                    if (see == kPart) {
-                        const int row = w0 + 16 * h + n, d = row - k0 - 4 * g - 16 * (kt + j), stay = min(a.sinks, row + 1) - k0 - 4 * g - 16 * (kt + j);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (!((uint32_t)(d - r) < (uint32_t)a.window || r < stay)) p[r] = 0.f;
-                    }
-                    db[h][2 * j] = Mma<DT>::pack(p[0] * dp[0], p[1] * dp[1]);
-                    db[h][2 * j + 1] = Mma<DT>::pack(p[2] * dp[2], p[3] * dp[3]);
+                    for (int r = 0; r < 4; ++r)
+                        if (!((uint32_t)(d - r) < (uint32_t)a.window || r < stay)) p[r] = 0.f;
                 }
+                db[2 * j] = Mma<DT>::pack(p[0] * dp[0], p[1] * dp[1]);
+                db[2 * j + 1] = Mma<DT>::pack(p[2] * dp[2], p[3] * dp[3]);
             }
             LDS_PTR(char) blk = k_lds + kt * LL::kTileBytes;
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct) {
                 const u32x2 k0t = read_tr(blk + tr_lane.off[ct]), k1t = read_tr(blk + LL::kTileBytes + tr_lane.off[ct]);
-                const u32x4 kk = {k0t.x, k0t.y, k1t.x, k1t.y};
-#pragma unroll
-                for (int h = 0; h < QT; ++h) acc[h][ct] = Mma<DT>::k32(kk, db[h], acc[h][ct]);
+                acc[ct] = Mma<DT>::k32(u32x4{k0t.x, k0t.y, k1t.x, k1t.y}, db, acc[ct]);
             }
         }
     }
     const Rsrc dqs = rows_of(dq + o_off, row0, row_end - row0, a.o.pitch);
+    u32x2 qw[CT];
 #pragma unroll
-    for (int h = 0; h < QT; ++h) {
-        const int at_row = own + 16 * h + n;
-        u32x2 qw[CT];
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-            qw[ct] = pack_acc<DT>(acc[h][ct], a.scale);
-            if (row0 + at_row >= tv) qw[ct] = u32x2{0u, 0u};
-        }
-        store_tile<C>(dqs, at_row * a.o.pitch, qw, g, stores_whole_lines(a.o.pitch, C, 0), width);
+    for (int ct = 0; ct < CT; ++ct) {
+        qw[ct] = pack_acc<DT>(acc[ct], a.scale);
+        if (w0 + n >= tv) qw[ct] = u32x2{0u, 0u};
     }
+    store_tile<C>(dqs, (own + n) * a.o.pitch, qw, g, stores_whole_lines(a.o.pitch, C, 0), width);
 }
 
 // =============================================================================
@@ -686,7 +674,7 @@ int launch_sink_fwd(const na1d_sink &h, void *out, float *saved, const void *q, 
     const SinkArgs a = sink_args(h, two ? 2 : 1);
     const int64_t items = h.N * h.heads * a.strips;
     if (!countable(items)) return NA1D_ERR_UNSUPPORTED;
-    const size_t lds = 4 * (size_t)region_bytes<C>(kChunkTiles);
+    const size_t lds = 4 * (size_t)region_bytes<C>(kKeyTiles);
     auto go = [&](auto kern) {
         if (!allow_lds(kern, lds)) return (int)NA1D_ERR_LAUNCH;
         note_kernel_as("sink_fwd_kernel<%s, %d, %d>", DT::tag == NA1D_BF16 ? "BF16" : "FP16", C, two ? 2 : 1);
@@ -700,17 +688,15 @@ int launch_sink_fwd(const na1d_sink &h, void *out, float *saved, const void *q, 
 template <class DT, int C>
 int launch_sink_bwd(const na1d_sink &h, void *dq, void *dk, void *dv, const void *q, const void *k, const void *v, const void *out, const void *dout,
                     const float *saved, const int32_t *t_valid, float *ws, hipStream_t s) {
-    const bool two = two_tiles(h, h.heads);
-    const SinkArgs a = sink_args(h, two ? 2 : 1);
+    const SinkArgs a = sink_args(h, 1);
     const KeyPlan p = key_plan(h);
     const int64_t items = h.N * h.heads * a.strips, key_items = p.a.whole + p.rest, join_items = p.joined * ((kChunkRows * (C / 4) + kThreads - 1) / kThreads);
     if (!countable(items) || !countable(p.heads * p.a.strips) || !countable(key_items) || !countable(join_items)) return NA1D_ERR_UNSUPPORTED;
     float *const delta = ws, *const partial = ws + lse_floats(h);
-    constexpr size_t dq_lds = 4 * (size_t)region_bytes<C>(kChunkTiles), dkv_lds = 2 * (2 * (size_t)region_bytes<C>(kChunkTiles) + 2 * kChunkRows * sizeof(float));
-    auto dq_kern = two ? sink_dq_kernel<DT, C, 2> : sink_dq_kernel<DT, C, 1>;
-    if (!allow_lds(dq_kern, dq_lds) || !allow_lds(sink_dkv_kernel<DT, C>, dkv_lds)) return NA1D_ERR_LAUNCH;
+    constexpr size_t dq_lds = 4 * (size_t)region_bytes<C>(kKeyTiles), dkv_lds = 2 * (2 * (size_t)region_bytes<C>(kChunkTiles) + 2 * kChunkRows * sizeof(float));
+    if (!allow_lds(sink_dq_kernel<DT, C>, dq_lds) || !allow_lds(sink_dkv_kernel<DT, C>, dkv_lds)) return NA1D_ERR_LAUNCH;
     note_kernel_as("sink_dq_kernel + sink_dkv_kernel<%s, %d>", DT::tag == NA1D_BF16 ? "BF16" : "FP16", C);
-    launch_kernel_span(1, dq_kern, (unsigned)items, (unsigned)kThreads, dq_lds, s, (char *)dq, delta, (const char *)q, (const char *)k, (const char *)v, (const char *)out,
+    launch_kernel_span(1, sink_dq_kernel<DT, C>, (unsigned)items, (unsigned)kThreads, dq_lds, s, (char *)dq, delta, (const char *)q, (const char *)k, (const char *)v, (const char *)out,
                        (const char *)dout, saved, (const char *)(saved + lse_floats(h)), t_valid, (uint32_t)items, a);
     launch_kernel_span(p.joined ? 0 : 2, sink_dkv_kernel<DT, C>, (unsigned)key_items, (unsigned)kThreads, dkv_lds, s, (char *)dk, (char *)dv, partial, (const char *)q,
                        (const char *)k, (const char *)v, (const char *)dout, saved, (const float *)delta, t_valid, (uint32_t)p.rest, (uint32_t)p.heads, p.a);

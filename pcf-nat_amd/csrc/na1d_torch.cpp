@@ -570,6 +570,15 @@ bool sink_append(const Tensor &k, const Tensor &v, const Tensor &kc, const Tenso
     return true;
 }
 
+MaybeTensor sink_rows(const Tensor &codes, const Tensor &ranges) {
+    na1d_sink_cache c;
+    if (!plain_call() || !cache_of(c, codes, codes, ranges, ranges, 0)) return std::nullopt;
+    const c10::DeviceGuard guard(codes.device());
+    const Tensor out = at::empty({c.N, c.kv_heads, c.capacity, c.head_dim}, ranges.options());
+    if (na1d_sink_rows(ptr(out), c.k, c.k_ranges, c.N * c.kv_heads * c.capacity, c.head_dim, c.dtype, stream_of(codes)) != NA1D_OK) return std::nullopt;
+    return out;
+}
+
 // ------------------------------------------------------------------------------------------------ an encoder layer in training
 // What train.py's node does between its checks and its bookkeeping.  A layer is some two dozen allocations and a dozen
 // launches each way: through the interpreter they took longer than the kernels of a small batch.
@@ -666,6 +675,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("sink", &sink);
     m.def("sink_over", &sink_over);
     m.def("sink_append", &sink_append);
+    m.def("sink_rows", &sink_rows);
     m.def("train_forward", &train_forward);
     m.def("train_backward", &train_backward);
 }

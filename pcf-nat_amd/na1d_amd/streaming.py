@@ -374,6 +374,10 @@ def cache_attend(q, k_cache, v_cache, lengths, win_size, sinks=0, scale=None):
 
 def cache_rows(cache):
     """What the rows of a cache stand for, ``[N, kv_heads, capacity, C]``: a new tensor for :class:`Rows4`, a 16-bit cache itself."""
+    nodes = _lib.nodes() if isinstance(cache, Rows4) else None
+    out = None if nodes is None else nodes.sink_rows(*cache)
+    if out is not None:
+        return out
     shape, dtype = _check_cache(cache, "cache")
     if not isinstance(cache, Rows4):
         return cache
