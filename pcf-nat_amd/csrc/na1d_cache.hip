@@ -610,7 +610,7 @@ cache_attend4_kernel(char *__restrict__ out, float *__restrict__ partial, const 
 constexpr int kFewWaves = kWaves;
 // Bytes of LDS that a wave stages into, and the most waves of a workgroup that find room.
 constexpr int staged_bytes(int C, bool four) { return four ? 2 * 2 * (64 * (C / 2) + 64 * 4) : 2 * 2 * (C <= 16 ? kChunk : 64 * C); }
-constexpr int most_waves(int C, bool four) { return staged_bytes(C, four) > 20480 ? kFewWaves : staged_bytes(C, four) > 10240 ? 8 : 16; }
+constexpr int most_waves(int C, bool four) { return four || staged_bytes(C, four) > 20480 ? kFewWaves : staged_bytes(C, four) > 10240 ? 8 : 16; }
 int width_of(const na1d_sink_cache &c) { return c.bits == 4 ? c.head_dim : padded_width(c.head_dim); }
 
 struct CachePlan {
@@ -637,7 +637,7 @@ CachePlan cache_plan(const na1d_sink_cache &c, int64_t fresh, int heads, int64_t
     if (p.tiles == 1 && wide > kFewWaves && heads_blocks <= 256 && most <= (int64_t)kSerial * unit * wide) {
         p.waves = wide;
     } else {
-        const int64_t slots = 256 * std::min(4, 160 * 1024 / (kFewWaves * staged_bytes(C, four))), longest = std::max<int64_t>(1, most / (2 * unit * kFewWaves));
+        const int64_t slots = 256 * std::min(4, 160 * 1024 / (kFewWaves * staged_bytes(C, four))), longest = std::max<int64_t>(1, most / ((four ? 1 : 2) * unit * kFewWaves));
         auto wasted = [&](int64_t s) { return heads_blocks * s % slots ? slots - heads_blocks * s % slots : 0; };      // of the last round
         int64_t s = std::max<int64_t>(1, slots / std::max<int64_t>(1, heads_blocks));
         if (heads_blocks > slots / 2)

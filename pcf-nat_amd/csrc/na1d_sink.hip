@@ -606,12 +606,15 @@ sink_join_kernel(char *__restrict__ dk, char *__restrict__ dv, const float *__re
     };
     const int64_t sink_strip = (int64_t)head * a.sink_strips + strip;
     if (in_parts) {
+#pragma unroll 4
         for (int p = 0; p < a.parts; ++p) add(partial_of<C>(strip_id, p, sink_strip, 0, heads, a).shared, kChunkRows);
     } else {
         add(partial_of<C>(strip_id, 0, sink_strip, 0, heads, a).near, a.sink_rows);
     }
-    if (sinking)
+    if (sinking) {
+#pragma unroll 8
         for (int f = 0; f < a.far; ++f) add(partial_of<C>(strip_id, 0, sink_strip, f, heads, a).far, a.sink_rows);
+    }
     u32x2 kw = pack_acc<DT>(sk, a.scale), vw = pack_acc<DT>(sv, 1.f);
     const uint32_t sample = head / (uint32_t)a.K, kv = head - sample * a.K;
     if (t_valid && row >= t_valid[sample]) kw = vw = u32x2{0u, 0u};
@@ -621,9 +624,11 @@ sink_join_kernel(char *__restrict__ dk, char *__restrict__ dv, const float *__re
 }
 
 // ----------------------------------------------------------------------------- launchers
-// Two tiles of 16 rows to a wave (strips of 128 rows) where that leaves every CU a workgroup or more: each operand read from LDS then
-// feeds two products.
-bool two_tiles(const na1d_sink &h, int64_t heads) { return h.N * heads * ((h.T + 127) / 128) >= 256; }
+// The forward takes two tiles of 16 queries to a wave, strips of 128, where there are many of those and windows are long: each operand read from LDS then feeds
+// two products (window 2048, 16384 tokens, 32 heads of 128: 669 us and not 764; 8192 tokens, 2 x 16 heads of 32, window 1024: 88 and 102).  Fewer workgroups
+// are better off as twice as many (4096 tokens, 16 heads of 128, window 1024: 52.7 us and not 53.4; 6 x 12 x 1237, 72 channels, window 333: 23 and 27), and
+// windows of a few chunks spend their time on what the strip has to load and store (16 x 16 x 1000, 64 channels, window 128: 39.8 and 43).
+bool two_tiles(const na1d_sink &h) { return h.N * h.heads * ((h.T + 127) / 128) >= 1024 && std::min(h.window, h.T) >= 256; }
 
 SinkArgs sink_args(const na1d_sink &h, int tiles) {
     SinkArgs a{};
@@ -654,11 +659,11 @@ KeyPlan key_plan(const na1d_sink &h) {
     a.whole = (int)std::min<int64_t>(strips - (a.parts > 1 ? over : 0), INT32_MAX);
     a.sink_strips = (int)((a.sinks + kChunkRows - 1) / kChunkRows);
     a.sink_rows = std::min(kChunkRows, (a.sinks + 15) / 16 * 16);
-    // far workgroups fill the card once, or have as many units as the others where that makes more of them; from a thousand strips with sinks on there
-    // are enough of those as they are
+    // far workgroups are as many as there are CUs, or have as many units as the others where that makes more of them; from a thousand strips with sinks on
+    // there are enough of those as they are
     const int64_t sinking = p.heads * a.sink_strips, beyond = chunks - near;
     if (sinking > 0 && sinking < 1024 && beyond > 0)
-        a.far = (int)std::max<int64_t>(1, std::min<int64_t>({std::max((beyond + near - 1) / near, round / sinking), 1024 / sinking, beyond * a.group / 4}));
+        a.far = (int)std::max<int64_t>(1, std::min<int64_t>({std::max((beyond + near - 1) / near, 256 / sinking), 1024 / sinking, beyond * a.group / 4}));
     const int64_t shared = strips - a.whole;
     p.rest = shared * a.parts + sinking * a.far;
     p.floats = shared * a.parts * (2 * kChunkRows * (int64_t)C) + (a.far ? sinking * (1 + a.far) * (2 * a.sink_rows * (int64_t)C) : 0);
@@ -670,7 +675,7 @@ bool countable(int64_t items) { return items <= 0x7fffff00LL; }
 
 template <class DT, int C>
 int launch_sink_fwd(const na1d_sink &h, void *out, float *saved, const void *q, const void *k, const void *v, const int32_t *t_valid, hipStream_t s) {
-    const bool two = two_tiles(h, h.heads);
+    const bool two = two_tiles(h);
     const SinkArgs a = sink_args(h, two ? 2 : 1);
     const int64_t items = h.N * h.heads * a.strips;
     if (!countable(items)) return NA1D_ERR_UNSUPPORTED;
