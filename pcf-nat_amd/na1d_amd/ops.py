@@ -10,7 +10,8 @@ so code written against ``torch.ops.na_cuda.*`` runs unchanged; importing this m
 
 Beyond the reference, the fused operator is registered the same way:
 ``na_cuda::na1d_fused_forward`` / ``na_cuda::na1d_fused_backward`` and the wrapper :func:`na1d_fused_op`; the dense
-operator and the losses over many classes (``na_cuda::class_loss_forward`` / ``class_loss_backward``) too.
+operator, the losses over many classes (``na_cuda::class_loss_forward`` / ``class_loss_backward``) and the attention of
+streams (``na_cuda::sink_attention_forward`` / ``sink_attention_backward``) too.
 """
 from __future__ import annotations
 
@@ -19,7 +20,7 @@ from typing import Optional
 import torch
 from torch import Tensor
 
-from . import _lib, losses
+from . import _lib, losses, streaming
 
 NAMESPACE = "na_cuda"
 _SIG = "int N, int T, int C, int win_size, int left"
@@ -389,3 +390,72 @@ def linear_distillation_op(x: Tensor, weight: Tensor, teacher_logits: Tensor, te
     """:func:`na1d_amd.losses.linear_distillation` through the registered op."""
     losses.check_teacher(x, weight, teacher_logits, teacher_ids, reduction)
     return _class_loss(x, weight, teacher_ids, teacher_logits.detach(), losses._TEACHER, float(temperature), 0.0, 0, losses._REDUCTIONS[reduction])
+
+
+# --------------------------------------------------------------------------- windowed causal attention with sinks
+_library.define("sink_attention_forward(Tensor q, Tensor k, Tensor v, Tensor? t_valid, int win_size, int sinks, float scale) -> (Tensor, Tensor)")
+_library.define("sink_attention_backward(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor? t_valid, Tensor out, Tensor saved, int win_size, int sinks, "
+                "float scale) -> (Tensor, Tensor, Tensor)")
+
+
+def _sink_contract(q, k, v, t_valid, win_size, sinks, dout=None, out=None, saved=None):
+    """Shared by the real and the fake kernels."""
+    streaming.check_operands(q, k, v, t_valid)
+    torch._check(win_size >= 1 and sinks >= 0, lambda: "win_size must be at least 1 and sinks at least 0")
+    for t in (dout, out):
+        torch._check(t is None or (t.shape == q.shape and t.dtype == q.dtype and t.device == q.device), lambda: "dout and out must be like q")
+    torch._check(saved is None or (saved.dtype == torch.uint8 and saved.dim() == 1 and saved.is_contiguous() and saved.device == q.device),
+                 lambda: "saved must be a forward's second result")
+
+
+def _sink_forward(q, k, v, t_valid, win_size, sinks, scale):
+    _sink_contract(q, k, v, t_valid, win_size, sinks)
+    return streaming.sink_forward(q, k, v, t_valid, win_size, sinks, scale, True)
+
+
+def _sink_forward_fake(q, k, v, t_valid, win_size, sinks, scale):
+    _sink_contract(q, k, v, t_valid, win_size, sinks)
+    return torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(streaming.saved_bytes(q), dtype=torch.uint8, device=q.device)
+
+
+def _sink_backward(dout, q, k, v, t_valid, out, saved, win_size, sinks, scale):
+    _sink_contract(q, k, v, t_valid, win_size, sinks, dout, out, saved)
+    return streaming.sink_backward(dout, q, k, v, t_valid, out, saved, win_size, sinks, scale)
+
+
+def _sink_backward_fake(dout, q, k, v, t_valid, out, saved, win_size, sinks, scale):
+    _sink_contract(q, k, v, t_valid, win_size, sinks, dout, out, saved)
+    return tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+
+
+_library.impl("sink_attention_forward", _sink_forward, "CUDA")
+_library.impl("sink_attention_backward", _sink_backward, "CUDA")
+torch.library.register_fake(NAMESPACE + "::sink_attention_forward", _sink_forward_fake, lib=_library)
+torch.library.register_fake(NAMESPACE + "::sink_attention_backward", _sink_backward_fake, lib=_library)
+
+
+def _sink_setup(ctx, inputs, output):
+    q, k, v, t_valid, *ctx.args = inputs
+    ctx.has_lengths = t_valid is not None
+    ctx.save_for_backward(*[t for t in (q, k, v, *output, t_valid) if t is not None])
+
+
+def _sink_autograd(ctx, dout, _dsaved):
+    q, k, v, out, saved, *lengths = ctx.saved_tensors
+    grads = getattr(torch.ops, NAMESPACE).sink_attention_backward(dout, q, k, v, lengths[0] if ctx.has_lengths else None, out, saved, *ctx.args)
+    return tuple(g if want else None for g, want in zip(grads, ctx.needs_input_grad)) + (None,) * 4
+
+
+def _sink_again(ctx, *_grads):
+    raise RuntimeError(streaming._AGAIN)
+
+
+torch.library.register_autograd(NAMESPACE + "::sink_attention_forward", _sink_autograd, setup_context=_sink_setup, lib=_library)
+torch.library.register_autograd(NAMESPACE + "::sink_attention_backward", _sink_again, lib=_library)
+
+
+def sink_attention_op(q: Tensor, k: Tensor, v: Tensor, win_size: int, sinks: int = 0, t_valid: Optional[Tensor] = None,
+                      scale: Optional[float] = None) -> Tensor:
+    """:func:`na1d_amd.streaming.sink_attention` through the registered op (traceable by ``torch.compile``)."""
+    streaming.check_operands(q, k, v, t_valid)
+    return getattr(torch.ops, NAMESPACE).sink_attention_forward(q, k, v, t_valid, *streaming._window(win_size, sinks), streaming._scale(scale, q.shape[3]))[0]

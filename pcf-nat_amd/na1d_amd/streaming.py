@@ -127,6 +127,13 @@ def _bytes(name, h):
     return n
 
 
+def saved_bytes(q):
+    """na1d_sink_saved_bytes of a call on ``q``, in arithmetic that symbolic sizes go through too."""
+    N, T, H, C = q.shape
+    wide = next(w for w in (16, 32, 64, 128) if C <= w)
+    return 16 * ((N * H * T + 3) // 4) + (N * H * ((T + 15) // 16) * 16 * wide if q.dtype == torch.bfloat16 else 0)
+
+
 def sink_forward(q, k, v, t_valid, win_size, sinks, scale, want_saved):
     """Output and what a backward needs (nothing, if it is not wanted).  Arguments as checked by the functions below."""
     q, k, v = _rows(q), _rows(k), _rows(v)

@@ -220,3 +220,10 @@ def test_native_caches_ask_for_their_pointers():
     assert lib.na1d_sink_append(ctypes.byref(long), 16, 16, s, s, None, None, (1 << 24) + 1, None) == -8
     assert lib.na1d_sink_append(ctypes.byref(long), None, 16, s, s, None, None, 5, None) == -1
     assert lib.na1d_sink_append(ctypes.byref(long), 16, 16, s, None, None, None, 5, None) == -1
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_the_bytes_that_a_forward_saves(dtype):
+    for N, T, H, K, C in ((1, 1, 1, 1, 8), (3, 17, 6, 2, 40), (2, 100, 4, 4, 64), (5, 333, 8, 1, 128), (2, 64, 3, 3, 72)):
+        q, k, v = _on("meta", N, T, H, K, C, dtype)
+        assert streaming.saved_bytes(q) == streaming._bytes("na1d_sink_saved_bytes", streaming._sink(q, k, v, 5, 1, 0.1))
