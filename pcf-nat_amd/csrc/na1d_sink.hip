@@ -83,46 +83,50 @@ __device__ inline Rsrc rows_of(const void *base, int64_t row, int rows, int pitc
     return make_rsrc((const void *)((uint64_t)(uint32_t)uniform((int)(at >> 32)) << 32 | (uint32_t)uniform((int)at)), uniform(max(0, rows) * pitch));
 }
 
-// What bf16 outputs lose in rounding, for the backward: delta = rowsum(dO * O) is taken away from every dP of a row, and with O as it is
-// stored, 2^-9 off, that alone made dQ and dK 3.5e-3 wrong (as a norm; all else together 2e-3).  An fp32 value is its bf16 rounding plus a
-// signed byte, as integers, to 2^-17: the bytes of a tile of 16 rows lie as dQ's waves read them, channels 32 s + 8 g of row n in the eight bytes
-// of lane 16 g + n of step s (16 channels: four bytes of a lane).  fp16 rounds to 2^-12 and goes without.
-template <class DT> constexpr bool kKeepsRest = DT::tag == NA1D_BF16;
+// What outputs lose in rounding, for the backward: delta = rowsum(dO * O) is taken away from every dP of a row, and with O as it is stored, half a step off, that
+// alone made dQ and dK 3.5e-3 (bf16) and 4e-4 (fp16) wrong, as a norm; all else together 2e-3 and 2e-4.  As integers, an fp32 value and the fp32 value of its rounding are
+// apart by half a step of bf16 or fp16 at most, 2^15 or 2^12: a signed byte of that, 2^8 or 2^5 each, leaves 2^-17 or 2^-20 of the value.  (fp16 below its normal range has larger
+// steps: there the byte ends at its range.)  The bytes of a tile of 16 rows lie as dQ's waves read them: channels 32 s + 8 g of row n in the eight bytes of lane
+// 16 g + n of step s (16 channels: four bytes of a lane).
 template <int C> constexpr int kRestBytes = 16 * C;      // of a tile
+template <class DT> constexpr int kRestShift = DT::tag == NA1D_BF16 ? 8 : 5;
+template <class DT> __device__ inline uint32_t bits_of_half(uint32_t pair, int i) {      // of the fp32 value of half `i` of a pair
+    const f32x2 x = unpack2<DT>(pair);
+    return __float_as_uint(i ? x.y : x.x);
+}
 // Four products' roundings `w` and the bytes they lack.
-__device__ inline uint32_t rest_of(f32x4 x, float f, u32x2 w) {
+template <class DT> __device__ inline uint32_t rest_of(f32x4 x, float f, u32x2 w) {
     uint32_t b[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) b[r] = (__float_as_uint(x[r] * f) - ((r & 1) ? w[r / 2] & 0xffff0000u : w[r / 2] << 16)) >> 8;
-    return (b[0] & 0xffu) | (b[1] & 0xffu) << 8 | (b[2] & 0xffu) << 16 | b[3] << 24;
+    for (int r = 0; r < 4; ++r) {
+        const int32_t apart = (int32_t)(__float_as_uint(x[r] * f) - bits_of_half<DT>(w[r / 2], r & 1)) >> kRestShift<DT>;
+        b[r] = (uint32_t)max(-128, min(127, apart)) & 0xffu;
+    }
+    return b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24;
 }
-// A rounding and its byte, byte `i` of `rest`.
-template <class DT> __device__ inline float with_rest(uint32_t half, uint32_t rest, int i) {
-    return __uint_as_float((half << 16) + (uint32_t)((int32_t)(rest << (24 - 8 * i)) >> 24 << 8));
+// Half `i` of a pair and its byte, byte `j` of `rest`.
+template <class DT> __device__ inline float with_rest(uint32_t pair, int i, uint32_t rest, int j) {
+    return __uint_as_float(bits_of_half<DT>(pair, i) + (uint32_t)((int32_t)(rest << (24 - 8 * j)) >> 24 << kRestShift<DT>));
 }
 // rowsum over this lane's channels of a row of dO and one of O
 template <class DT, int C> __device__ inline float dot_whole(const RowOperand<C> &a, const RowOperand<C> &o, const char *rest, int lane) {
-    if constexpr (!kKeepsRest<DT>) {
-        return dot_lane<DT, C>(a, o);
-    } else {
-        float acc = 0.f;
-        auto add = [&](uint32_t x, uint32_t y, uint32_t b, int i) {
-            const f32x2 d = unpack2<DT>(x);
-            acc = __builtin_fmaf(d.x, with_rest<DT>(y & 0xffffu, b, i), __builtin_fmaf(d.y, with_rest<DT>(y >> 16, b, i + 1), acc));
-        };
+    float acc = 0.f;
+    auto add = [&](uint32_t x, uint32_t y, uint32_t b, int j) {
+        const f32x2 d = unpack2<DT>(x);
+        acc = __builtin_fmaf(d.x, with_rest<DT>(y, 0, b, j), __builtin_fmaf(d.y, with_rest<DT>(y, 1, b, j + 1), acc));
+    };
 #pragma unroll
-        for (int s = 0; s < RowOperand<C>::k32; ++s) {
-            const u32x2 b = *reinterpret_cast<const u32x2 *>(rest + s * 512 + lane * 8);
+    for (int s = 0; s < RowOperand<C>::k32; ++s) {
+        const u32x2 b = *reinterpret_cast<const u32x2 *>(rest + s * 512 + lane * 8);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) add(a.w32[s][i], o.w32[s][i], b[i / 2], 2 * (i & 1));
-        }
-        if (RowOperand<C>::k16) {
-            const uint32_t b = *reinterpret_cast<const uint32_t *>(rest + lane * 4);
-            add(a.w16[0][0], o.w16[0][0], b, 0);
-            add(a.w16[0][1], o.w16[0][1], b, 2);
-        }
-        return acc;
+        for (int i = 0; i < 4; ++i) add(a.w32[s][i], o.w32[s][i], b[i / 2], 2 * (i & 1));
     }
+    if (RowOperand<C>::k16) {
+        const uint32_t b = *reinterpret_cast<const uint32_t *>(rest + lane * 4);
+        add(a.w16[0][0], o.w16[0][0], b, 0);
+        add(a.w16[0][1], o.w16[0][1], b, 2);
+    }
+    return acc;
 }
 template <int C> __device__ inline void store_rest(char *rest, const uint32_t (&b)[C / 16], int lane) {
     if constexpr (C == 16) {
@@ -279,10 +283,10 @@ sink_fwd_kernel(char *__restrict__ out, float *__restrict__ lse, char *__restric
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
             ow[ct] = pack_acc<DT>(o[h][ct], inv);
-            if constexpr (kKeepsRest<DT>) rw[ct] = rest_of(o[h][ct], inv, ow[ct]);
+            rw[ct] = rest_of<DT>(o[h][ct], inv, ow[ct]);
             if (!valid) ow[ct] = u32x2{0u, 0u}, rw[ct] = 0u;
         }
-        if (kKeepsRest<DT> && rest && w0 + 16 * h < T)
+        if (rest && w0 + 16 * h < T)
             store_rest<C>(rest + (((int64_t)it.sample * a.H + head) * ((T + 15) / 16) + (w0 / 16 + h)) * kRestBytes<C>, rw, lane);
         store_tile<C>(os, at_row * a.o.pitch, ow, g, stores_whole_lines(a.o.pitch, C, 0), width);   // rows past T are dropped
         // log2 of the row's sum of exponentials; 0 for a row that does not exist, whose q and dO the backward reads as zeros
@@ -294,7 +298,10 @@ sink_fwd_kernel(char *__restrict__ out, float *__restrict__ lse, char *__restric
 // Backward, query side: delta = rowsum(dO * O) and dQ = scale * dS K,  dS = P (dO V^T - delta)
 // =============================================================================
 // One tile of 16 queries to a wave: with two, as in the forward, 228 registers leave two waves to a SIMD and not four, and the launches are half as
-// many workgroups: 16 x 16 x 1000, 64 channels, window 128 took 57 us and not 48, 5 x 10 x 777, 96 channels, window 100 24 and not 17.5.
+// many workgroups: 16 x 16 x 1000, 64 channels, window 128 took 57 us and not 48, 5 x 10 x 777, 96 channels, window 100 24 and not 17.5 (before the second product).
+// A row's dS sum to 0, so what all keys have in common drops out of dQ, but not out of the roundings of dS, and where one key (a sink) has half of a row's weight they
+// are large: dS goes into the product as two 16-bit numbers, the rounding and what it lost.  (2 x 16 x 8192, bf16, 16 sinks: dQ 3.2e-3 off, as a norm, without,
+// 2.1e-3 with it, of which 1.7e-3 are the rounding of dQ itself; 280 us and not 240.)
 template <class DT, int C>
 __global__ void __launch_bounds__(kThreads)
 sink_dq_kernel(char *__restrict__ dq, float *__restrict__ delta, const char *__restrict__ q, const char *__restrict__ k, const char *__restrict__ v,
@@ -340,7 +347,7 @@ sink_dq_kernel(char *__restrict__ dq, float *__restrict__ delta, const char *__r
     row_lane.init(0, lane);
     tr_lane.init(0, lane);
     const int tile = min(w0 / 16, (T - 1) / 16);          // a tile past the last reads the last's bytes, with zeros for dO
-    const char *bytes = kKeepsRest<DT> ? rest + (((int64_t)it.sample * a.H + head) * ((T + 15) / 16) + tile) * kRestBytes<C> : nullptr;
+    const char *bytes = rest + (((int64_t)it.sample * a.H + head) * ((T + 15) / 16) + tile) * kRestBytes<C>;
     const float dl = xor_sum(dot_whole<DT, C>(gop, oop, bytes, lane));      // lane (n, g) holds a quarter of row n's channels
     if (g == 0) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(dl), ds, (own + n) * 4, 0, 0);
     const f32x4 minus_dl = {-dl, -dl, -dl, -dl};          // the product dO . V^T starts at minus delta
@@ -361,7 +368,7 @@ sink_dq_kernel(char *__restrict__ dq, float *__restrict__ delta, const char *__r
         if (see == kNothing) continue;
 #pragma unroll
         for (int kt = 0; kt < kKeyTiles; kt += 2) {
-            u32x4 db;
+            u32x4 db, rb;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 RowOperand<C> kop, vop;
@@ -378,14 +385,22 @@ sink_dq_kernel(char *__restrict__ dq, float *__restrict__ delta, const char *__r
                     for (int r = 0; r < 4; ++r)
                         if (!((uint32_t)(d - r) < (uint32_t)a.window || r < stay)) p[r] = 0.f;
                 }
-                db[2 * j] = Mma<DT>::pack(p[0] * dp[0], p[1] * dp[1]);
-                db[2 * j + 1] = Mma<DT>::pack(p[2] * dp[2], p[3] * dp[3]);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float x = p[2 * i] * dp[2 * i], y = p[2 * i + 1] * dp[2 * i + 1];
+                    const uint32_t w = Mma<DT>::pack(x, y);
+                    const f32x2 there = unpack2<DT>(w);
+                    db[2 * j + i] = w;
+                    rb[2 * j + i] = Mma<DT>::pack(x - there.x, y - there.y);
+                }
             }
             LDS_PTR(char) blk = k_lds + kt * LL::kTileBytes;
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct) {
                 const u32x2 k0t = read_tr(blk + tr_lane.off[ct]), k1t = read_tr(blk + LL::kTileBytes + tr_lane.off[ct]);
-                acc[ct] = Mma<DT>::k32(u32x4{k0t.x, k0t.y, k1t.x, k1t.y}, db, acc[ct]);
+                const u32x4 kk = {k0t.x, k0t.y, k1t.x, k1t.y};
+                acc[ct] = Mma<DT>::k32(kk, db, acc[ct]);
+                acc[ct] = Mma<DT>::k32(kk, rb, acc[ct]);
             }
         }
     }
@@ -714,7 +729,7 @@ int launch_sink_bwd(const na1d_sink &h, void *dq, void *dk, void *dv, const void
 }  // namespace
 
 int64_t sink_saved_bytes(const na1d_sink &h) {
-    return 4 * lse_floats(h) + (h.dtype == NA1D_BF16 ? h.N * h.heads * ((h.T + 15) / 16) * 16 * padded_width(h.head_dim) : 0);
+    return 4 * lse_floats(h) + h.N * h.heads * ((h.T + 15) / 16) * 16 * padded_width(h.head_dim);
 }
 int64_t sink_bwd_workspace_bytes(const na1d_sink &h) {
     return 4 * (lse_floats(h) + key_plan(h).floats);
