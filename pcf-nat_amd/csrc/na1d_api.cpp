@@ -668,7 +668,7 @@ static int cache_check(const na1d_sink_cache *c, int64_t fresh, int64_t heads, i
     if (c->head_dim < 1 || c->head_dim % (c->bits == 4 ? 32 : 8)) return NA1D_ERR_HEAD_DIM;
     if (c->N < 0 || fresh < 0 || c->kv_heads < 1 || heads < 1 || heads % c->kv_heads) return NA1D_ERR_SHAPE;
     const int64_t most = 1ll << 29;
-    if (c->head_dim > 128 || c->capacity > most / c->head_dim || c->N > (1 << 24) / c->kv_heads || fresh > (1 << 20) / (heads / c->kv_heads)) return NA1D_ERR_UNSUPPORTED;
+    if (c->head_dim > 128 || c->capacity > most / c->head_dim || c->N > (1 << 24) / c->kv_heads || heads > (1 << 24) || fresh > (1 << 20) / (heads / c->kv_heads)) return NA1D_ERR_UNSUPPORTED;
     if (window < 1 || c->sinks < 0 || c->sinks >= c->capacity || window > c->capacity - c->sinks - (fresh > 0 ? fresh - 1 : 0)) return NA1D_ERR_WINDOW;
     return c->N == 0 || fresh == 0;
 }

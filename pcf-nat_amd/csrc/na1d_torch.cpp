@@ -502,7 +502,28 @@ MaybeTensor sink(const Tensor &q, const Tensor &k, const Tensor &v, int64_t wind
     return node ? SinkAttention::apply(q, k, v, t_valid, window, sinks, s, done) : done.out;
 }
 
-// A pair of caches, with their rows' ranges where they are held in 4 bits.
+// What a call writes to shares no memory with what else it takes.
+bool apart(std::initializer_list<const Tensor *> written, std::initializer_list<const Tensor *> read) {
+    const auto meet = [](const Tensor &a, const Tensor &b) {
+        const auto end = [](const Tensor &t) {
+            int64_t last = 1;
+            for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+            return (const char *)t.data_ptr() + last * t.element_size();
+        };
+        return (const char *)a.data_ptr() < end(b) && (const char *)b.data_ptr() < end(a);
+    };
+    for (auto i = written.begin(); i != written.end(); ++i) {
+        for (auto j = i + 1; j != written.end(); ++j)
+            if (meet(**i, **j)) return false;
+        for (const Tensor *t : read)
+            if (meet(**i, *t)) return false;
+    }
+    return true;
+}
+// A pair of caches, with their rows' ranges where they are held in 4 bits; `read`: what goes into them.
+bool separate(const Tensor &k, const Tensor &v, const MaybeTensor &kr, const MaybeTensor &vr, std::initializer_list<const Tensor *> read) {
+    return kr ? apart({&k, &v, &*kr, &*vr}, read) : apart({&k, &v}, read);
+}
 bool cache_of(na1d_sink_cache &c, const Tensor &k, const Tensor &v, const MaybeTensor &kr, const MaybeTensor &vr, int64_t sinks) {
     if (!plain(k) || !on(v, k) || !k.is_contiguous() || k.dim() != 4 || k.sizes() != v.sizes() || k.scalar_type() != v.scalar_type() || !k.numel() || kr.has_value() != vr.has_value())
         return false;
@@ -533,6 +554,7 @@ MaybeTensor sink_over(const Tensor &q, const MaybeTensor &k, const MaybeTensor &
     na1d_sink_cache c;
     if (!plain_call() || !cache_of(c, kc, vc, kr, vr, sinks) || !goes_with(q, c, kc, true) || !lengths_for(lengths, q)) return std::nullopt;
     if (k && (!goes_with(*k, c, kc, false) || !goes_with(*v, c, kc, false) || k->size(1) != q.size(1) || v->size(1) != q.size(1))) return std::nullopt;
+    if (k && !separate(kc, vc, kr, vr, {&q, &*k, &*v})) return std::nullopt;
     if (at::GradMode::is_enabled() && (q.requires_grad() || (k && (k->requires_grad() || v->requires_grad())))) return std::nullopt;
     const int64_t fresh = q.size(1), heads = q.size(2), nbytes = na1d_sink_attend_workspace_bytes(&c, fresh, heads, window);
     if (nbytes < 0) return std::nullopt;
@@ -559,7 +581,7 @@ bool sink_append(const Tensor &k, const Tensor &v, const Tensor &kc, const Tenso
                  const MaybeTensor &t_valid) {
     na1d_sink_cache c;
     if (!plain_call() || !cache_of(c, kc, vc, kr, vr, sinks) || !goes_with(k, c, kc, false) || !goes_with(v, c, kc, false) || k.size(1) != v.size(1) || !lengths_for(lengths, k) ||
-        !lengths_for(t_valid, k))
+        !lengths_for(t_valid, k) || !separate(kc, vc, kr, vr, {&k, &v}))
         return false;
     const c10::DeviceGuard guard(k.device());
     int64_t ks[3], vs[3];

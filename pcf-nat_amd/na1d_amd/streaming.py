@@ -272,6 +272,17 @@ def _check_caches(k_cache, v_cache, sinks):
     return shape, dtype
 
 
+def _check_apart(k_cache, v_cache, *read):
+    """What a call writes to shares no memory with what it reads or writes besides."""
+    def extent(t):
+        return t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+    there = [extent(t) for t in _parts(k_cache, v_cache) if t is not None and t.numel() and not t.is_meta]
+    rest = there + [extent(t) for t in read if t.numel() and not t.is_meta]
+    for i, (a, b) in enumerate(there):
+        if any(a < d and c < b for c, d in rest[i + 1:]):
+            raise _lib.NA1DError("k_cache and v_cache are written to: they must not share memory with each other or with q, k and v")
+
+
 def _check_tokens(t, shape, dtype, device, heads, what):
     N, K, _, C = shape
     if t.dim() != 4 or t.shape[0] != N or t.shape[3] != C or (t.shape[2] != K if heads == "kv_heads" else t.shape[2] == 0 or t.shape[2] % K):
@@ -299,7 +310,8 @@ def cache_append(k, v, k_cache, v_cache, lengths=None, sinks=0, t_valid=None):
     """Tokens ``k, v [N, T, kv_heads, C]`` become positions ``lengths[n]`` and following of their streams (``lengths`` None: from 0 on).
 
     ``t_valid`` int32 ``[N]``: only so many of a stream's tokens are there.  What a later token cannot see is not kept: of the tokens behind the
-    sinks the last ``capacity - sinks`` are.  The caches are written to in place, and nothing is returned; no gradient goes through them."""
+    sinks the last ``capacity - sinks`` are.  The caches are written to in place (they share no memory with each other or with the tokens), and nothing is
+    returned; no gradient goes through them."""
     nodes = _nodes(1, sinks)
     if nodes is not None and nodes.sink_append(k, v, *_parts(k_cache, v_cache), lengths, sinks, t_valid):
         return
@@ -312,6 +324,7 @@ def cache_append(k, v, k_cache, v_cache, lengths=None, sinks=0, t_valid=None):
         raise ValueError("k and v must have equally many tokens, got %d and %d" % (k.shape[1], v.shape[1]))
     check_lengths(lengths, k, "lengths")
     check_lengths(t_valid, k, "t_valid")
+    _check_apart(k_cache, v_cache, k, v)
     _check_gpu(k)
     k, v = _rows(k.detach()), _rows(v.detach())
     lengths, t_valid = (None if t is None else t.contiguous() for t in (lengths, t_valid))
@@ -335,6 +348,8 @@ def _over_cache(q, k, v, k_cache, v_cache, lengths, win_size, sinks, scale):
         _check_tokens(t, shape, dtype, device, "kv_heads", what)
         if t.shape[1] != q.shape[1]:
             raise ValueError("%s must have as many tokens as q, got %d and %d" % (what, t.shape[1], q.shape[1]))
+    if k is not None:
+        _check_apart(k_cache, v_cache, q, k, v)
     if lengths is None:
         raise ValueError("lengths must be int32 [%d]" % shape[0])
     check_lengths(lengths, q, "lengths")

@@ -192,3 +192,20 @@ def test_errors_of_the_native_call_carry_its_reason():
             streaming.sink_attention(q, k, v, 4, scale=scale)
         with pytest.raises(_lib.NA1DError, match="scale"):
             streaming.cache_step(q[:, :1], k[:, :1], v[:, :1], *streaming.new_cache(1, 2, 8, 32), torch.zeros(1, dtype=torch.int32, device="cuda"), 4, scale=scale)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_caches_that_share_memory_are_refused(bits):
+    """By the native path too, which passes them on to the checks."""
+    q, kx, vx, _ = _inputs(2, 3, 4, 2, 32, torch.bfloat16, 50)
+    k, v = streaming.new_cache(2, 2, 20, 32, bits)
+    lengths = torch.zeros(2, dtype=torch.int32, device="cuda")
+    rows = k.codes.view(torch.bfloat16).view(-1) if bits == 4 else k.view(-1)
+    inside = rows[-2 * 3 * 2 * 32:].view(2, 3, 2, 32)
+    for pair, tokens in (((k, k), (kx, vx)), ((k, v), (inside, vx)), ((v, k), (kx, inside))):
+        with pytest.raises(_lib.NA1DError, match="share memory"):
+            streaming.cache_append(*tokens, *pair)
+        with pytest.raises(_lib.NA1DError, match="share memory"):
+            streaming.cache_step(q, *tokens, *pair, lengths, 8)
+    both = streaming.cache_attend(q, k, k, lengths + 3, 8)                # read only
+    _same([both], [streaming.cache_attend(q, k, streaming.Rows4(*(t.clone() for t in k)) if bits == 4 else k.clone(), lengths + 3, 8)])

@@ -227,3 +227,31 @@ def test_the_bytes_that_a_forward_saves(dtype):
     for N, T, H, K, C in ((1, 1, 1, 1, 8), (3, 17, 6, 2, 40), (2, 100, 4, 4, 64), (5, 333, 8, 1, 128), (2, 64, 3, 3, 72)):
         q, k, v = _on("meta", N, T, H, K, C, dtype)
         assert streaming.saved_bytes(q) == streaming._bytes("na1d_sink_saved_bytes", streaming._sink(q, k, v, 5, 1, 0.1))
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_caches_that_share_memory(bits):
+    """Of the caches, and with what is put into them: refused wherever something is written."""
+    k, v = _caches(bits, device="cpu")
+    lengths = torch.zeros(2, dtype=torch.int32)
+    q, kx, vx = _on("cpu", T=3, C=32)
+    flat = torch.zeros(2 * 2 * 20 * 32 + 64, dtype=torch.bfloat16)                                # a cache that starts inside the other
+    near = flat[64:].view(2, 2, 20, 32), flat[:-64].view(2, 2, 20, 32)
+    pairs = [(k, k), (k, streaming.Rows4(v.codes, k.ranges)) if bits == 4 else near]
+    for pair in pairs:
+        with pytest.raises(_lib.NA1DError, match="share memory"):
+            streaming.cache_append(kx, vx, *pair)
+        with pytest.raises(_lib.NA1DError, match="share memory"):
+            streaming.cache_step(q, kx, vx, *pair, lengths, 8)
+        with pytest.raises(_lib.NA1DError, match="no CPU path"):                                 # nothing is written
+            streaming.cache_attend(q, *pair, lengths, 8)
+    rows = k.codes.view(torch.bfloat16).view(-1) if bits == 4 else k.view(-1)
+    inside = rows[:2 * 3 * 2 * 32].view(2, 3, 2, 32)
+    for tokens in ((inside, vx), (kx, inside)):
+        with pytest.raises(_lib.NA1DError, match="share memory"):
+            streaming.cache_append(*tokens, k, v)
+        with pytest.raises(_lib.NA1DError, match="share memory"):
+            streaming.cache_step(q, *tokens, k, v, lengths, 8)
+    both = torch.zeros(2, 2, 2, 20, 32, dtype=torch.bfloat16)                                    # halves of one tensor do not
+    with pytest.raises(_lib.NA1DError, match="no CPU path"):
+        streaming.cache_append(kx, vx, *both)
