@@ -219,25 +219,36 @@ __device__ inline void join_waves(const Sums<C, QT> &s, char *smem, char *out, f
 }
 // The shares of a head's keys, in a fixed order: four channels of a row to a thread.
 template <class DT, int C, int QT>
-__global__ void __launch_bounds__(kThreads) cache_join_kernel(char *__restrict__ out, const float *__restrict__ partial, int64_t quads, CacheArgs a) {
-    constexpr int kRows = 16 * QT;
-    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+__global__ void __launch_bounds__(kThreads) cache_join_kernel(char *__restrict__ out, const float *__restrict__ partial, uint32_t quads, CacheArgs a) {
+    constexpr int kRows = 16 * QT, kAtOnce = 8;
+    const uint32_t i = blockIdx.x * kThreads + threadIdx.x;      // (shares are many only where heads are few: 32 bits hold these)
     if (i >= quads) return;
-    const int per_row = a.width / 8, ch = (int)(i % per_row) * 4;
-    const int64_t hr = i / per_row;
-    const int row = (int)(hr % a.rows), block = row / kRows;
-    const int64_t head = hr / a.rows, sample = head / a.K, kv = head - sample * a.K;
-    const float *from = partial + (((head * a.blocks + block) * a.splits) * kRows + row - block * kRows) * (C + 4);
+    const uint32_t per_row = a.width / 8, hr = i / per_row, head = hr / (uint32_t)a.rows, row = hr - head * a.rows, sample = head / (uint32_t)a.K, kv = head - sample * a.K;
+    const uint32_t ch = (i - hr * per_row) * 4, block = row / kRows;
+    const float *from = partial + (((int64_t)(head * a.blocks + block) * a.splits) * kRows + row - block * kRows) * (C + 4);
     float m = kNoMaximum, l = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < a.splits; ++s) m = __builtin_fmaxf(m, from[(int64_t)s * kRows * (C + 4) + C]);
-    for (int s = 0; s < a.splits; ++s, from += kRows * (C + 4)) {
-        const float f = __builtin_amdgcn_exp2f(from[C] - m);
-        l = __builtin_fmaf(from[C + 1], f, l);
-        o += *reinterpret_cast<const f32x4 *>(from + ch) * f;
+    for (int s = 0; s < a.splits; s += kAtOnce) {
+        float ms[kAtOnce], ls[kAtOnce], high = m;
+        f32x4 os[kAtOnce];
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) {
+            const float *x = from + (int64_t)min(s + j, a.splits - 1) * (kRows * (C + 4));
+            ms[j] = x[C], ls[j] = x[C + 1], os[j] = *reinterpret_cast<const f32x4 *>(x + ch);
+        }
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) high = __builtin_fmaxf(high, ms[j]);      // (one share twice at the end: the same maximum)
+        const float alpha = __builtin_amdgcn_exp2f(m - high);
+        m = high, l *= alpha, o *= alpha;
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) {
+            const float f = s + j < a.splits ? __builtin_amdgcn_exp2f(ms[j] - m) : 0.f;
+            l = __builtin_fmaf(ls[j], f, l);
+            o += os[j] * f;
+        }
     }
-    const int token = row / a.group, gi = row - token * a.group;
-    const int64_t at = ((sample * a.fresh + token) * a.K * a.group + kv * a.group + gi) * a.width + 2 * ch;
+    const uint32_t token = row / (uint32_t)a.group, gi = row - token * a.group;
+    const int64_t at = (((int64_t)sample * a.fresh + token) * a.K * a.group + kv * a.group + gi) * a.width + 2 * ch;
     *reinterpret_cast<u32x2 *>(out + at) = l > 0.f ? pack_acc<DT>(o, 1.f / l) : u32x2{0u, 0u};
 }
 
@@ -671,7 +682,7 @@ int launch_attend(const na1d_sink_cache &c, const CachePlan &p, void *out, const
     }
     if (joins) {
         const int64_t quads = c.N * c.kv_heads * (int64_t)p.a.rows * (p.a.width / 8);
-        launch_kernel_span(2, cache_join_kernel<DT, C, QT>, (unsigned)((quads + kThreads - 1) / kThreads), (unsigned)kThreads, 0, s, (char *)out, (const float *)ws, quads, p.a);
+        launch_kernel_span(2, cache_join_kernel<DT, C, QT>, (unsigned)((quads + kThreads - 1) / kThreads), (unsigned)kThreads, 0, s, (char *)out, (const float *)ws, (uint32_t)quads, p.a);
     }
     return launch_status();
 }
