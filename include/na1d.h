@@ -445,7 +445,7 @@ int na1d_head_backward(const na1d_head *h, void *dx, void *dw, const float *dlos
  *   t_valid : int32 [N] or NULL; rows from there on do not exist: they may hold anything, their outputs and gradients are 0.
  *             The rows before have to be finite.
  *   saved   : what a forward leaves for its backward, na1d_sink_saved_bytes() bytes: 4 to a head's row and a byte to a value of out
- *             (what its rounding lost; head_dim counted as the next of 16, 32, 64, 128); NULL for inference
+ *             (what its rounding lost; head_dim counted as the next of 16, 32, 64, 96, 128); NULL for inference
  * Scores, softmax and sums are in fp32; probabilities, and their gradients for dk, are rounded to 16 bits where they are multiplied by v,
  * dout and q (their gradients for dq are taken as two such numbers).  Nothing uses atomics: results are the same from call to call.
  * A backward's workspace is 4 bytes to a head's row, and fp32 sums where several workgroups share the rows of a key head (those that are

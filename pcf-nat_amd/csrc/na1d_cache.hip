@@ -308,8 +308,9 @@ template <class DT, int C, int QT, int NW>
 __global__ void __launch_bounds__(64 * NW)
 cache_attend_kernel(char *__restrict__ out, float *__restrict__ partial, const char *__restrict__ q, const char *__restrict__ k, const char *__restrict__ v,
                     char *kc, char *vc, const int32_t *__restrict__ lengths, uint32_t items, CacheArgs a) {
-    using LL = Lds<C>;
-    constexpr int CT = C / 16, kUnit = 32, kRegion = region_bytes<C>(2), kStage = 2 * kRegion, kLoads = kStage / kChunk, kChunkKeys = kChunk / LL::kRowBytes;
+    constexpr int CS = kStaged<C>;
+    using LL = Lds<CS>;
+    constexpr int CT = C / 16, kUnit = 32, kRegion = region_bytes<CS>(2), kStage = 2 * kRegion, kLoads = kStage / kChunk, kChunkKeys = kChunk / LL::kRowBytes;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), g = lane >> 4, n = lane & 15;
     LDS_PTR(char) mine = (LDS_PTR(char))smem + wave * 2 * kStage;
@@ -344,8 +345,8 @@ cache_attend_kernel(char *__restrict__ out, float *__restrict__ partial, const c
             load_from(fresh ? vx + (key - old) * a.v.row + byte : vs + at, to + kRegion + c * kChunk);
         }
     };
-    RowLane<C> row_lane;
-    TrLane<C> tr_lane;
+    RowLane<C, CS> row_lane;
+    TrLane<C, CS> tr_lane;
     row_lane.init(0, lane);
     tr_lane.init(0, lane);
     const float scale2 = a.scale * kLog2e;
@@ -375,7 +376,7 @@ cache_attend_kernel(char *__restrict__ out, float *__restrict__ partial, const c
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
             RowOperand<C> kop;
-            read_rows<C>(kop, k_lds + kt * LL::kTileBytes, row_lane);
+            read_rows<C, CS>(kop, k_lds + kt * LL::kTileBytes, row_lane);
 #pragma unroll
             for (int h = 0; h < QT; ++h) s[h][kt] = dot_rows_mma<DT, C>(kop, qop[h]);
         }
@@ -620,9 +621,9 @@ cache_attend4_kernel(char *__restrict__ out, float *__restrict__ partial, const 
 // ----------------------------------------------------------------------------- launchers
 constexpr int kFewWaves = kWaves;
 // Bytes of LDS that a wave stages into, and the most waves of a workgroup that find room.
-constexpr int staged_bytes(int C, bool four) { return four ? 2 * 2 * (64 * (C / 2) + 64 * 4) : 2 * 2 * (C <= 16 ? kChunk : 64 * C); }
+constexpr int staged_bytes(int C, bool four) { return four ? 2 * 2 * (64 * (C / 2) + 64 * 4) : 2 * 2 * (C <= 16 ? kChunk : 64 * (C == 96 ? 128 : C)); }
 constexpr int most_waves(int C, bool four) { return four || staged_bytes(C, four) > 20480 ? kFewWaves : staged_bytes(C, four) > 10240 ? 8 : 16; }
-int width_of(const na1d_sink_cache &c) { return c.bits == 4 ? c.head_dim : padded_width(c.head_dim); }
+int width_of(const na1d_sink_cache &c) { return channels_of(c.head_dim); }
 
 struct CachePlan {
     int tiles, waves;
@@ -698,7 +699,7 @@ template <class DT, class... A> int launch_width(const na1d_sink_cache &c, const
         case 16: return launch_tiles<DT, 16, false>(c, p, args...);
         case 32: return four ? launch_tiles<DT, 32, true>(c, p, args...) : launch_tiles<DT, 32, false>(c, p, args...);
         case 64: return four ? launch_tiles<DT, 64, true>(c, p, args...) : launch_tiles<DT, 64, false>(c, p, args...);
-        case 96: return launch_tiles<DT, 96, true>(c, p, args...);
+        case 96: return four ? launch_tiles<DT, 96, true>(c, p, args...) : launch_tiles<DT, 96, false>(c, p, args...);
         case 128: return four ? launch_tiles<DT, 128, true>(c, p, args...) : launch_tiles<DT, 128, false>(c, p, args...);
     }
     return NA1D_ERR_UNSUPPORTED;

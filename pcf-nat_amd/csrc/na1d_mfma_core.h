@@ -714,6 +714,10 @@ inline int window_shift(const Geom &g) {
 
 // The kernels' C for a head_dim: the next of 16, 32, 64, 128 (0 above).
 inline int padded_width(int head_dim) { return head_dim <= 16 ? 16 : head_dim <= 32 ? 32 : head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 0; }
+// The same with 96 among them: rows of these lie in LDS as those of 128 do, kStaged, and nothing past their channels is read or multiplied
+// (a training pass over 5 x 10 x 777 rows of 96, window 100, is 57 us of kernels, and 67 with rows of 128; 6 x 12 x 1237 rows of 72, window 333, forward: 21.5 and 22.5).
+inline int channels_of(int head_dim) { return head_dim > 64 && head_dim <= 96 ? 96 : padded_width(head_dim); }
+template <int C> constexpr int kStaged = C == 96 ? 128 : C;
 
 #define NA1D_MFMA_DISPATCH(FN, ...)                                            \
     do {                                                                       \

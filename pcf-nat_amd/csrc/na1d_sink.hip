@@ -148,8 +148,8 @@ template <class DT, int C, int QT>
 __global__ void __launch_bounds__(kThreads, 3)
 sink_fwd_kernel(char *__restrict__ out, float *__restrict__ lse, char *__restrict__ rest, const char *__restrict__ q, const char *__restrict__ k, const char *__restrict__ v,
                 const int32_t *__restrict__ t_valid, uint32_t items, SinkArgs a) {
-    using LL = Lds<C>;
-    constexpr int CT = C / 16, kStep = region_bytes<C>(kKeyTiles);
+    constexpr int CT = C / 16, CS = kStaged<C>, kStep = region_bytes<CS>(kKeyTiles);
+    using LL = Lds<CS>;
     extern __shared__ __attribute__((aligned(16))) char smem[];          // 4 * kStep bytes: K and V of two chunks
     LDS_PTR(char) kv_lds = (LDS_PTR(char))smem;
 
@@ -162,11 +162,11 @@ sink_fwd_kernel(char *__restrict__ out, float *__restrict__ lse, char *__restric
     if (t_valid) tv = uniform(max(0, min(T, t_valid[it.sample])));
     const int row0 = it.strip * (kChunkRows * QT), row_end = min(T, row0 + kChunkRows * QT);
     const char *kb = k + it.sample * a.k.sample + it.kv * a.k.head, *vb = v + it.sample * a.v.sample + it.kv * a.v.head;
-    const int k_lane = direct_lane_offset<C>(wave, lane, a.k.pitch, width), v_lane = direct_lane_offset<C>(wave, lane, a.v.pitch, width);
+    const int k_lane = direct_lane_offset<CS>(wave, lane, a.k.pitch, width), v_lane = direct_lane_offset<CS>(wave, lane, a.v.pitch, width);
     auto stage = [&](int c, LDS_PTR(char) to) {
         const int rows = min(kKeyRows, tv - c * kKeyRows);
-        stage_direct<C, kKeyTiles, kReadShared>(rows_of(kb, (int64_t)c * kKeyRows, rows, a.k.pitch), 0, to, kKeyTiles, wave, k_lane, a.k.pitch);
-        stage_direct<C, kKeyTiles, kReadShared>(rows_of(vb, (int64_t)c * kKeyRows, rows, a.v.pitch), 0, to + kStep, kKeyTiles, wave, v_lane, a.v.pitch);
+        stage_direct<CS, kKeyTiles, kReadShared>(rows_of(kb, (int64_t)c * kKeyRows, rows, a.k.pitch), 0, to, kKeyTiles, wave, k_lane, a.k.pitch);
+        stage_direct<CS, kKeyTiles, kReadShared>(rows_of(vb, (int64_t)c * kKeyRows, rows, a.v.pitch), 0, to + kStep, kKeyTiles, wave, v_lane, a.v.pitch);
     };
     const KeyChunks chunks(row0, row_end - 1, tv, a);
     int c = chunks.first();
@@ -178,8 +178,8 @@ sink_fwd_kernel(char *__restrict__ out, float *__restrict__ lse, char *__restric
     for (int h = 0; h < QT; ++h) load_rows<C, kReadOnce>(qop[h], qs, (own + 16 * h) * a.q.pitch, a.q.pitch, width, lane);
     const float scale2 = a.scale * kLog2e;               // the scale is positive: checked at the C boundary
 
-    RowLane<C> row_lane;
-    TrLane<C> tr_lane;
+    RowLane<C, CS> row_lane;
+    TrLane<C, CS> tr_lane;
     row_lane.init(0, lane);
     tr_lane.init(0, lane);
     constexpr float kSlack = 6.f;
@@ -209,7 +209,7 @@ sink_fwd_kernel(char *__restrict__ out, float *__restrict__ lse, char *__restric
 #pragma unroll
         for (int kt = 0; kt < kKeyTiles; ++kt) {
             RowOperand<C> kop;
-            read_rows<C>(kop, k_lds + kt * LL::kTileBytes, row_lane);
+            read_rows<C, CS>(kop, k_lds + kt * LL::kTileBytes, row_lane);
 #pragma unroll
             for (int h = 0; h < QT; ++h) s[h][kt] = dot_rows_mma<DT, C>(kop, qop[h]);
         }
@@ -307,8 +307,8 @@ __global__ void __launch_bounds__(kThreads)
 sink_dq_kernel(char *__restrict__ dq, float *__restrict__ delta, const char *__restrict__ q, const char *__restrict__ k, const char *__restrict__ v,
                const char *__restrict__ out, const char *__restrict__ dout, const float *__restrict__ lse, const char *__restrict__ rest, const int32_t *__restrict__ t_valid,
                uint32_t items, SinkArgs a) {
-    using LL = Lds<C>;
-    constexpr int CT = C / 16, kStep = region_bytes<C>(kKeyTiles);
+    constexpr int CT = C / 16, CS = kStaged<C>, kStep = region_bytes<CS>(kKeyTiles);
+    using LL = Lds<CS>;
     extern __shared__ __attribute__((aligned(16))) char smem[];          // 4 * kStep bytes
     LDS_PTR(char) kv_lds = (LDS_PTR(char))smem;
 
@@ -321,11 +321,11 @@ sink_dq_kernel(char *__restrict__ dq, float *__restrict__ delta, const char *__r
     if (t_valid) tv = uniform(max(0, min(T, t_valid[it.sample])));
     const int row0 = it.strip * kChunkRows, row_end = min(T, row0 + kChunkRows);
     const char *kb = k + it.sample * a.k.sample + it.kv * a.k.head, *vb = v + it.sample * a.v.sample + it.kv * a.v.head;
-    const int k_lane = direct_lane_offset<C>(wave, lane, a.k.pitch, width), v_lane = direct_lane_offset<C>(wave, lane, a.v.pitch, width);
+    const int k_lane = direct_lane_offset<CS>(wave, lane, a.k.pitch, width), v_lane = direct_lane_offset<CS>(wave, lane, a.v.pitch, width);
     auto stage = [&](int c, LDS_PTR(char) to) {
         const int rows = min(kKeyRows, tv - c * kKeyRows);
-        stage_direct<C, kKeyTiles, kReadShared>(rows_of(kb, (int64_t)c * kKeyRows, rows, a.k.pitch), 0, to, kKeyTiles, wave, k_lane, a.k.pitch);
-        stage_direct<C, kKeyTiles, kReadShared>(rows_of(vb, (int64_t)c * kKeyRows, rows, a.v.pitch), 0, to + kStep, kKeyTiles, wave, v_lane, a.v.pitch);
+        stage_direct<CS, kKeyTiles, kReadShared>(rows_of(kb, (int64_t)c * kKeyRows, rows, a.k.pitch), 0, to, kKeyTiles, wave, k_lane, a.k.pitch);
+        stage_direct<CS, kKeyTiles, kReadShared>(rows_of(vb, (int64_t)c * kKeyRows, rows, a.v.pitch), 0, to + kStep, kKeyTiles, wave, v_lane, a.v.pitch);
     };
     const KeyChunks chunks(row0, row_end - 1, tv, a);
     int c = chunks.first();
@@ -342,8 +342,8 @@ sink_dq_kernel(char *__restrict__ dq, float *__restrict__ delta, const char *__r
     load_rows<C, kReadOnce>(oop, os, own * a.o.pitch, a.o.pitch, width, lane);
     const float ref = -__uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(ls, (own + n) * 4, 0, 0));      // minus the row's log2 of its sum
     const float scale2 = a.scale * kLog2e;
-    RowLane<C> row_lane;
-    TrLane<C> tr_lane;
+    RowLane<C, CS> row_lane;
+    TrLane<C, CS> tr_lane;
     row_lane.init(0, lane);
     tr_lane.init(0, lane);
     const int tile = min(w0 / 16, (T - 1) / 16);          // a tile past the last reads the last's bytes, with zeros for dO
@@ -372,8 +372,8 @@ sink_dq_kernel(char *__restrict__ dq, float *__restrict__ delta, const char *__r
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 RowOperand<C> kop, vop;
-                read_rows<C>(kop, k_lds + (kt + j) * LL::kTileBytes, row_lane);
-                read_rows<C>(vop, v_lds + (kt + j) * LL::kTileBytes, row_lane);
+                read_rows<C, CS>(kop, k_lds + (kt + j) * LL::kTileBytes, row_lane);
+                read_rows<C, CS>(vop, v_lds + (kt + j) * LL::kTileBytes, row_lane);
                 const f32x4 s = dot_rows_mma<DT, C>(kop, qop);
                 const f32x4 dp = dot_rows_mma<DT, C>(vop, gop, minus_dl);
                 float p[4];
@@ -439,8 +439,8 @@ __global__ void __launch_bounds__(kThreads)
 sink_dkv_kernel(char *__restrict__ dk, char *__restrict__ dv, float *__restrict__ partial, const char *__restrict__ q, const char *__restrict__ k,
                 const char *__restrict__ v, const char *__restrict__ dout, const float *__restrict__ lse, const float *__restrict__ delta,
                 const int32_t *__restrict__ t_valid, uint32_t rest, uint32_t heads, SinkArgs a) {
-    using LL = Lds<C>;
-    constexpr int CT = C / 16, kStep = region_bytes<C>(kChunkTiles), kBuf = 2 * kStep + 2 * kChunkRows * 4;
+    constexpr int CT = C / 16, CS = kStaged<C>, kStep = region_bytes<CS>(kChunkTiles), kBuf = 2 * kStep + 2 * kChunkRows * 4;
+    using LL = Lds<CS>;
     extern __shared__ __attribute__((aligned(16))) char smem[];          // 2 * kBuf bytes: Q, dO and the rows' constants of two chunks
     LDS_PTR(char) buf_lds = (LDS_PTR(char))smem;
 
@@ -483,14 +483,14 @@ sink_dkv_kernel(char *__restrict__ dk, char *__restrict__ dv, float *__restrict_
     int u = uniform((int)((int64_t)units * part / each));
     int hg = nc ? uniform(u / nc) : 0, c = nc ? c_from + u - hg * nc : 0;
 
-    const int q_lane = direct_lane_offset<C>(wave, lane, a.q.pitch, width), g_lane = direct_lane_offset<C>(wave, lane, a.o.pitch, width);
+    const int q_lane = direct_lane_offset<CS>(wave, lane, a.q.pitch, width), g_lane = direct_lane_offset<CS>(wave, lane, a.o.pitch, width);
     const char *qb = q + sample * a.q.sample, *gb = dout + sample * a.o.sample;
     float row_lse, row_delta;                             // of row 16 * wave + n of the chunk in flight
     auto stage = [&](int hg_, int c_, LDS_PTR(char) to) {
         const int h = kv * a.group + hg_, rows = min(kChunkRows, tv - c_ * kChunkRows);
         const int64_t r0 = (int64_t)c_ * kChunkRows, stat = ((int64_t)sample * a.H + h) * T + r0;
-        stage_direct<C, kChunkTiles, kReadShared>(rows_of(qb + h * a.q.head, r0, rows, a.q.pitch), 0, to, kChunkTiles, wave, q_lane, a.q.pitch);
-        stage_direct<C, kChunkTiles, kReadShared>(rows_of(gb + h * a.o.head, r0, rows, a.o.pitch), 0, to + kStep, kChunkTiles, wave, g_lane, a.o.pitch);
+        stage_direct<CS, kChunkTiles, kReadShared>(rows_of(qb + h * a.q.head, r0, rows, a.q.pitch), 0, to, kChunkTiles, wave, q_lane, a.q.pitch);
+        stage_direct<CS, kChunkTiles, kReadShared>(rows_of(gb + h * a.o.head, r0, rows, a.o.pitch), 0, to + kStep, kChunkTiles, wave, g_lane, a.o.pitch);
         const Rsrc ls = rows_of(lse + stat, 0, rows, 4), ds = rows_of(delta + stat, 0, rows, 4);
         row_lse = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(ls, (16 * wave + n) * 4, 0, 0));
         row_delta = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(ds, (16 * wave + n) * 4, 0, 0));
@@ -504,8 +504,8 @@ sink_dkv_kernel(char *__restrict__ dk, char *__restrict__ dv, float *__restrict_
     load_rows<C, kReadShared>(vop, vs, own * a.v.pitch, a.v.pitch, width, lane);
     const float scale2 = a.scale * kLog2e;
     const uint32_t reach = key < a.sinks ? 0x7fffffffu : (uint32_t)a.window;
-    RowLane<C> row_lane;
-    TrLane<C> tr_lane;
+    RowLane<C, CS> row_lane;
+    TrLane<C, CS> tr_lane;
     row_lane.init(0, lane);
     tr_lane.init(0, lane);
     f32x4 acck[CT], accv[CT];
@@ -536,8 +536,8 @@ sink_dkv_kernel(char *__restrict__ dk, char *__restrict__ dv, float *__restrict_
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 RowOperand<C> qop, gop;
-                read_rows<C>(qop, q_lds + (qi + j) * LL::kTileBytes, row_lane);
-                read_rows<C>(gop, g_lds + (qi + j) * LL::kTileBytes, row_lane);
+                read_rows<C, CS>(qop, q_lds + (qi + j) * LL::kTileBytes, row_lane);
+                read_rows<C, CS>(gop, g_lds + (qi + j) * LL::kTileBytes, row_lane);
                 const f32x4 ref = *reinterpret_cast<LDS_PTR(f32x4)>(ref_lds + 64 * (qi + j));
                 const f32x4 del4 = *reinterpret_cast<LDS_PTR(f32x4)>(ref_lds + kChunkRows * 4 + 64 * (qi + j));
                 const f32x4 s = dot_rows_mma<DT, C>(qop, kop);        // [query 4g+r][key n]
@@ -665,8 +665,8 @@ KeyPlan key_plan(const na1d_sink &h) {
     SinkArgs &a = p.a;
     a = sink_args(h, 1);
     p.heads = h.N * h.kv_heads;
-    const int C = padded_width(h.head_dim);
-    const int64_t strips = p.heads * a.strips, round = 256 * (C == 128 ? 2 : C == 64 ? 4 : 6);      // workgroups that the card holds at once
+    const int C = channels_of(h.head_dim);
+    const int64_t strips = p.heads * a.strips, round = 256 * (C >= 96 ? 2 : C == 64 ? 4 : 6);      // workgroups that the card holds at once
     const int64_t chunks = a.strips, near = std::min<int64_t>(chunks, (a.window + kChunkRows - 2) / kChunkRows + 1), units = near * a.group;      // a strip's
     const int64_t over = strips % round;
     a.parts = 1;
@@ -694,7 +694,7 @@ int launch_sink_fwd(const na1d_sink &h, void *out, float *saved, const void *q, 
     const SinkArgs a = sink_args(h, two ? 2 : 1);
     const int64_t items = h.N * h.heads * a.strips;
     if (!countable(items)) return NA1D_ERR_UNSUPPORTED;
-    const size_t lds = 4 * (size_t)region_bytes<C>(kKeyTiles);
+    const size_t lds = 4 * (size_t)region_bytes<kStaged<C>>(kKeyTiles);
     auto go = [&](auto kern) {
         if (!allow_lds(kern, lds)) return (int)NA1D_ERR_LAUNCH;
         note_kernel_as("sink_fwd_kernel<%s, %d, %d>", DT::tag == NA1D_BF16 ? "BF16" : "FP16", C, two ? 2 : 1);
@@ -713,7 +713,7 @@ int launch_sink_bwd(const na1d_sink &h, void *dq, void *dk, void *dv, const void
     const int64_t items = h.N * h.heads * a.strips, key_items = p.a.whole + p.rest, join_items = p.joined * ((kChunkRows * (C / 4) + kThreads - 1) / kThreads);
     if (!countable(items) || !countable(p.heads * p.a.strips) || !countable(key_items) || !countable(join_items)) return NA1D_ERR_UNSUPPORTED;
     float *const delta = ws, *const partial = ws + lse_floats(h);
-    constexpr size_t dq_lds = 4 * (size_t)region_bytes<C>(kKeyTiles), dkv_lds = 2 * (2 * (size_t)region_bytes<C>(kChunkTiles) + 2 * kChunkRows * sizeof(float));
+    constexpr size_t dq_lds = 4 * (size_t)region_bytes<kStaged<C>>(kKeyTiles), dkv_lds = 2 * (2 * (size_t)region_bytes<kStaged<C>>(kChunkTiles) + 2 * kChunkRows * sizeof(float));
     if (!allow_lds(sink_dq_kernel<DT, C>, dq_lds) || !allow_lds(sink_dkv_kernel<DT, C>, dkv_lds)) return NA1D_ERR_LAUNCH;
     note_kernel_as("sink_dq_kernel + sink_dkv_kernel<%s, %d>", DT::tag == NA1D_BF16 ? "BF16" : "FP16", C);
     launch_kernel_span(1, sink_dq_kernel<DT, C>, (unsigned)items, (unsigned)kThreads, dq_lds, s, (char *)dq, delta, (const char *)q, (const char *)k, (const char *)v, (const char *)out,
@@ -726,26 +726,36 @@ int launch_sink_bwd(const na1d_sink &h, void *dq, void *dk, void *dv, const void
     return launch_status();
 }
 
+template <class F> int by_width(const na1d_sink &h, F run) {
+    auto typed = [&](auto dt) {
+        switch (channels_of(h.head_dim)) {
+            case 16: return run(dt, std::integral_constant<int, 16>());
+            case 32: return run(dt, std::integral_constant<int, 32>());
+            case 64: return run(dt, std::integral_constant<int, 64>());
+            case 96: return run(dt, std::integral_constant<int, 96>());
+            case 128: return run(dt, std::integral_constant<int, 128>());
+        }
+        return (int)NA1D_ERR_UNSUPPORTED;
+    };
+    return h.dtype == NA1D_BF16 ? typed(BF16()) : typed(FP16());
+}
+
 }  // namespace
 
 int64_t sink_saved_bytes(const na1d_sink &h) {
-    return 4 * lse_floats(h) + h.N * h.heads * ((h.T + 15) / 16) * 16 * padded_width(h.head_dim);
+    return 4 * lse_floats(h) + h.N * h.heads * ((h.T + 15) / 16) * 16 * channels_of(h.head_dim);
 }
 int64_t sink_bwd_workspace_bytes(const na1d_sink &h) {
     return 4 * (lse_floats(h) + key_plan(h).floats);
 }
 
 int sink_fwd(const na1d_sink &h, void *out, float *saved, const void *q, const void *k, const void *v, const int32_t *t_valid, hipStream_t s) {
-    const int dtype = h.dtype;
-    const struct { int C; } g{h.head_dim};
-    NA1D_MFMA_DISPATCH(launch_sink_fwd, h, out, saved, q, k, v, t_valid, s);
+    return by_width(h, [&](auto dt, auto c) { return launch_sink_fwd<decltype(dt), decltype(c)::value>(h, out, saved, q, k, v, t_valid, s); });
 }
 
 int sink_bwd(const na1d_sink &h, void *dq, void *dk, void *dv, const void *q, const void *k, const void *v, const void *out, const void *dout, const float *saved,
              const int32_t *t_valid, float *ws, hipStream_t s) {
-    const int dtype = h.dtype;
-    const struct { int C; } g{h.head_dim};
-    NA1D_MFMA_DISPATCH(launch_sink_bwd, h, dq, dk, dv, q, k, v, out, dout, saved, t_valid, ws, s);
+    return by_width(h, [&](auto dt, auto c) { return launch_sink_bwd<decltype(dt), decltype(c)::value>(h, dq, dk, dv, q, k, v, out, dout, saved, t_valid, ws, s); });
 }
 
 }  // namespace mfma

@@ -130,7 +130,7 @@ def _bytes(name, h):
 def saved_bytes(q):
     """na1d_sink_saved_bytes of a call on ``q``, in arithmetic that symbolic sizes go through too."""
     N, T, H, C = q.shape
-    wide = next(w for w in (16, 32, 64, 128) if C <= w)
+    wide = next(w for w in (16, 32, 64, 96, 128) if C <= w)
     return 16 * ((N * H * T + 3) // 4) + N * H * ((T + 15) // 16) * 16 * wide
 
 
