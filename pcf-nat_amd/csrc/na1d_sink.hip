@@ -141,6 +141,16 @@ template <int C> __device__ inline void store_rest(char *rest, const uint32_t (&
     }
 }
 
+// Two values as a pair of 16-bit numbers each: the roundings, and those of what these lost.  A row's dS sum to 0, so what all keys have in common drops out of dQ (and of dK
+// what all queries have), but not out of roundings of dS: they go into the products twice, and so does P into dV's.  As norms against 64 bits, 2 x 16 x 8192 rows, bf16, 16 sinks:
+// dQ 3.2e-3 -> 2.1e-3, dK and dV 2.4e-3 -> 1.7e-3, where the rounding of the result alone is 1.7e-3.  It costs 280 us and not 240 (dQ) and 460 and not 405 (dK and
+// dV) there, at 128 channels, 52 and 48, 64 and 61 for 16 x 16 x 1000 rows of 64 channels, window 128.
+template <class DT> __device__ inline void pack_twice(float x, float y, uint32_t &w, uint32_t &rest) {
+    w = Mma<DT>::pack(x, y);
+    const f32x2 there = unpack2<DT>(w);
+    rest = Mma<DT>::pack(x - there.x, y - there.y);
+}
+
 // =============================================================================
 // Forward
 // =============================================================================
@@ -297,11 +307,9 @@ sink_fwd_kernel(char *__restrict__ out, float *__restrict__ lse, char *__restric
 // =============================================================================
 // Backward, query side: delta = rowsum(dO * O) and dQ = scale * dS K,  dS = P (dO V^T - delta)
 // =============================================================================
-// One tile of 16 queries to a wave: with two, as in the forward, 228 registers leave two waves to a SIMD and not four, and the launches are half as
-// many workgroups: 16 x 16 x 1000, 64 channels, window 128 took 57 us and not 48, 5 x 10 x 777, 96 channels, window 100 24 and not 17.5 (before the second product).
-// A row's dS sum to 0, so what all keys have in common drops out of dQ, but not out of the roundings of dS, and where one key (a sink) has half of a row's weight they
-// are large: dS goes into the product as two 16-bit numbers, the rounding and what it lost.  (2 x 16 x 8192, bf16, 16 sinks: dQ 3.2e-3 off, as a norm, without,
-// 2.1e-3 with it, of which 1.7e-3 are the rounding of dQ itself; 280 us and not 240.)
+// What bounds it is LDS: 24 KB of operands to a wave and 32 keys.  Two tiles of 16 queries to a wave, as in the forward, halve that, but 228 registers leave two waves to a SIMD and
+// not four, and the launches are half as many workgroups: 2 x 16 x 8192, 128 channels, window 1024, takes 310 us and not 280; 16 x 16 x 1000, 64 channels, window 128, took
+// 57 and not 48, 5 x 10 x 777, 96 channels, window 100, 24 and not 17.5 (these two before dS went into the product twice).
 template <class DT, int C>
 __global__ void __launch_bounds__(kThreads)
 sink_dq_kernel(char *__restrict__ dq, float *__restrict__ delta, const char *__restrict__ q, const char *__restrict__ k, const char *__restrict__ v,
@@ -385,14 +393,11 @@ sink_dq_kernel(char *__restrict__ dq, float *__restrict__ delta, const char *__r
                     for (int r = 0; r < 4; ++r)
                         if (!((uint32_t)(d - r) < (uint32_t)a.window || r < stay)) p[r] = 0.f;
                 }
+                uint32_t w[2], r_[2];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const float x = p[2 * i] * dp[2 * i], y = p[2 * i + 1] * dp[2 * i + 1];
-                    const uint32_t w = Mma<DT>::pack(x, y);
-                    const f32x2 there = unpack2<DT>(w);
-                    db[2 * j + i] = w;
-                    rb[2 * j + i] = Mma<DT>::pack(x - there.x, y - there.y);
-                }
+                for (int i = 0; i < 2; ++i) pack_twice<DT>(p[2 * i] * dp[2 * i], p[2 * i + 1] * dp[2 * i + 1], w[i], r_[i]);
+                db[2 * j] = w[0], db[2 * j + 1] = w[1];
+                rb[2 * j] = r_[0], rb[2 * j + 1] = r_[1];
             }
             LDS_PTR(char) blk = k_lds + kt * LL::kTileBytes;
 #pragma unroll
@@ -532,7 +537,7 @@ sink_dkv_kernel(char *__restrict__ dk, char *__restrict__ dv, float *__restrict_
         if (see == kNothing) continue;
 #pragma unroll
         for (int qi = 0; qi < kChunkTiles; qi += 2) {
-            u32x4 pb, db;
+            u32x4 pb, db, pr, dr;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 RowOperand<C> qop, gop;
@@ -551,10 +556,14 @@ sink_dkv_kernel(char *__restrict__ dk, char *__restrict__ dv, float *__restrict_
                     for (int r = 0; r < 4; ++r)
                         if (!((uint32_t)(d + r) < reach)) p[r] = 0.f;
                 }
-                pb[2 * j] = Mma<DT>::pack(p[0], p[1]);
-                pb[2 * j + 1] = Mma<DT>::pack(p[2], p[3]);
-                db[2 * j] = Mma<DT>::pack(p[0] * dp[0], p[1] * dp[1]);
-                db[2 * j + 1] = Mma<DT>::pack(p[2] * dp[2], p[3] * dp[3]);
+                uint32_t w[4], r_[4];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    pack_twice<DT>(p[2 * i], p[2 * i + 1], w[i], r_[i]);
+                    pack_twice<DT>(p[2 * i] * dp[2 * i], p[2 * i + 1] * dp[2 * i + 1], w[2 + i], r_[2 + i]);
+                }
+                pb[2 * j] = w[0], pb[2 * j + 1] = w[1], pr[2 * j] = r_[0], pr[2 * j + 1] = r_[1];
+                db[2 * j] = w[2], db[2 * j + 1] = w[3], dr[2 * j] = r_[2], dr[2 * j + 1] = r_[3];
             }
             LDS_PTR(char) qtile = q_lds + qi * LL::kTileBytes;
             LDS_PTR(char) gtile = g_lds + qi * LL::kTileBytes;
@@ -565,6 +574,8 @@ sink_dkv_kernel(char *__restrict__ dk, char *__restrict__ dv, float *__restrict_
                 const u32x4 gg = {g0.x, g0.y, g1.x, g1.y}, qq = {q0t.x, q0t.y, q1t.x, q1t.y};
                 accv[ct] = Mma<DT>::k32(gg, pb, accv[ct]);
                 acck[ct] = Mma<DT>::k32(qq, db, acck[ct]);
+                accv[ct] = Mma<DT>::k32(gg, pr, accv[ct]);
+                acck[ct] = Mma<DT>::k32(qq, dr, acck[ct]);
             }
         }
     }
