@@ -477,19 +477,20 @@ cache_attend4_kernel(char *__restrict__ out, float *__restrict__ partial, const 
 #pragma unroll
         for (int s = 0; s < S; ++s) qop[h][s] = r.position >= 0 ? *reinterpret_cast<const u32x4 *>(q + r.at + (C / 2) * g + 16 * s) : u32x4{0u, 0u, 0u, 0u};
     }
-    // V's rows have their 16-byte units swapped about so that the 16 rows a transposed read takes a unit of lie in distinct banks
+    // Rows have their 16-byte units swapped about so that the 16 rows a read takes a unit of lie in distinct banks
     auto swz = [](int row) { return kUnits == 4 ? row >> 2 & 3 : kUnits == 2 ? row >> 3 & 1 : 0; };
     auto stage = [&](int i, LDS_PTR(char) to) {
 #pragma unroll
         for (int c = 0; c < kCodes / kChunk; ++c) {
             const int u = 64 * c + lane, r = u / kUnits, unit = u % kUnits, kkey = i + key_of_row(r), vkey = i + r;
-            load_to_lds<16, kReadShared>(ks, to + c * kChunk, kkey < i1 ? seen.row(kkey) * kRow + unit * 16 : kNowhere);
+            load_to_lds<16, kReadShared>(ks, to + c * kChunk, kkey < i1 ? seen.row(kkey) * kRow + (unit ^ swz(r)) * 16 : kNowhere);
             load_to_lds<16, kReadShared>(vs, to + kCodes + c * kChunk, vkey < i1 ? seen.row(vkey) * kRow + (unit ^ swz(r)) * 16 : kNowhere);
         }
         const int key = i + key_of_row(lane), at = key < i1 ? seen.row(key) * 4 : kNowhere;
         load_to_lds<4, kReadShared>(krs, to + 2 * kCodes, at);
         load_to_lds<4, kReadShared>(vrs, to + 2 * kCodes + kRanges, at);
     };
+    const int k_off = n * kRow + ((((kRow / 4) * g >> 4) ^ swz(n)) << 4 | ((kRow / 4) * g & 15));      // of this lane's row n, channels (C / 4) g ..
     int v_off[CT];              // of this lane's row 16 g + n, channels 16 ct ..
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) v_off[ct] = (16 * g + n) * kRow + (((ct >> 1) ^ swz(16 * g + n)) << 4 | (ct & 1) << 3);
@@ -534,7 +535,7 @@ cache_attend4_kernel(char *__restrict__ out, float *__restrict__ partial, const 
         for (int kt = 0; kt < 4; ++kt) {
             uint32_t w[S];
 #pragma unroll
-            for (int s = 0; s < S; ++s) w[s] = *reinterpret_cast<LDS_PTR(uint32_t)>(k_lds + (16 * kt + n) * kRow + (kRow / 4) * g + 4 * s);
+            for (int s = 0; s < S; ++s) w[s] = *reinterpret_cast<LDS_PTR(uint32_t)>(k_lds + 16 * kt * kRow + k_off + 4 * s);
 #pragma unroll
             for (int h = 0; h < QT; ++h) z[h][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
