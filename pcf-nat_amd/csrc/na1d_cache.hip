@@ -480,6 +480,20 @@ cache_attend4_kernel(char *__restrict__ out, float *__restrict__ partial, const 
     // Rows have their 16-byte units swapped about so that the 16 rows a read takes a unit of lie in distinct banks
     auto swz = [](int row) { return kUnits == 4 ? row >> 2 & 3 : kUnits == 2 ? row >> 3 & 1 : 0; };
     auto stage = [&](int i, LDS_PTR(char) to) {
+        int row0 = seen.first + (i - seen.apart);
+        if (row0 >= seen.ring) row0 -= seen.ring;
+        if (i >= seen.apart && i + kUnit <= i1 && row0 + kUnit <= seen.ring) {      // rows one behind the other: what a lane adds to the first's place stays the same
+            row0 += seen.sinks;
+#pragma unroll
+            for (int c = 0; c < kCodes / kChunk; ++c) {
+                const int u = 64 * c + lane, r = u / kUnits, at = ((u % kUnits) ^ swz(r)) * 16;
+                load_to_lds<16, kReadShared>(ks, to + c * kChunk, row0 * kRow + (key_of_row(r) * kRow + at));
+                load_to_lds<16, kReadShared>(vs, to + kCodes + c * kChunk, row0 * kRow + (r * kRow + at));
+            }
+            load_to_lds<4, kReadShared>(krs, to + 2 * kCodes, row0 * 4 + key_of_row(lane) * 4);
+            load_to_lds<4, kReadShared>(vrs, to + 2 * kCodes + kRanges, row0 * 4 + key_of_row(lane) * 4);
+            return;
+        }
 #pragma unroll
         for (int c = 0; c < kCodes / kChunk; ++c) {
             const int u = 64 * c + lane, r = u / kUnits, unit = u % kUnits, kkey = i + key_of_row(r), vkey = i + r;
