@@ -544,6 +544,14 @@ cache_attend4_kernel(char *__restrict__ out, float *__restrict__ partial, const 
         LDS_PTR(char) k_lds = mine + at;
         LDS_PTR(char) v_lds = k_lds + kCodes;
         LDS_PTR(char) r_lds = v_lds + kCodes;
+        // What goes with a key, worked out by one lane for all: in the place of the ranges first K's numbers, then V's (the wave's own accesses stay in order, and all are of 32-bit integers).
+        const f32x2 of_k = unpack2<DT>(*reinterpret_cast<LDS_PTR(uint32_t)>(r_lds + 4 * lane)), of_v = unpack2<DT>(*reinterpret_cast<LDS_PTR(uint32_t)>(r_lds + kRanges + 4 * lane));
+        auto share = [&](float x, float y) {
+            *reinterpret_cast<LDS_PTR(uint32_t)>(r_lds + 4 * lane) = __float_as_uint(x);
+            *reinterpret_cast<LDS_PTR(uint32_t)>(r_lds + kRanges + 4 * lane) = __float_as_uint(y);
+        };
+        auto shared = [&](int which, int kt) { return __builtin_bit_cast(f32x4, *reinterpret_cast<LDS_PTR(u32x4)>(r_lds + which * kRanges + 64 * kt + 16 * g)); };
+        share(of_k.x * scale2, __builtin_fmaf(-16.f, of_k.x, of_k.y));
         f32x4 z[QT][4];
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt) {
@@ -558,15 +566,13 @@ cache_attend4_kernel(char *__restrict__ out, float *__restrict__ partial, const 
 #pragma unroll
                 for (int h = 0; h < QT; ++h) z[h][kt] = Mma<DT>::k32(kop, qop[h][s], z[h][kt]);
             }
-            const u32x4 range = *reinterpret_cast<LDS_PTR(u32x4)>(r_lds + 64 * kt + 16 * g);
+            const f32x4 by = shared(0, kt), and_ = shared(1, kt);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const f32x2 sl = unpack2<DT>(range[r]);         // step, low
-                const float a_ = sl.x * scale2, b_ = __builtin_fmaf(-16.f, sl.x, sl.y);
+            for (int r = 0; r < 4; ++r)
 #pragma unroll
-                for (int h = 0; h < QT; ++h) z[h][kt][r] = __builtin_fmaf(z[h][kt][r], a_, b_ * qsum[h]);
-            }
+                for (int h = 0; h < QT; ++h) z[h][kt][r] = __builtin_fmaf(z[h][kt][r], by[r], and_[r] * qsum[h]);
         }
+        share(of_v.x, __builtin_fmaf(7.5f, of_v.x, of_v.y));
         const bool ends = i + kUnit > i1;
         u32x4 pp[QT][2];
 #pragma unroll
@@ -591,15 +597,14 @@ cache_attend4_kernel(char *__restrict__ out, float *__restrict__ partial, const 
             const float m = sums.m[h];
 #pragma unroll
             for (int kt = 0; kt < 4; ++kt) {
-                const u32x4 range = *reinterpret_cast<LDS_PTR(u32x4)>(r_lds + kRanges + 64 * kt + 16 * g);
+                const f32x4 step = shared(0, kt), mid = shared(1, kt);
                 float e[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const f32x2 sl = unpack2<DT>(range[r]);
                     e[r] = __builtin_amdgcn_exp2f(z[h][kt][r] - m);
                     sums.l[h] += e[r];
-                    mids[h] = __builtin_fmaf(e[r], __builtin_fmaf(7.5f, sl.x, sl.y), mids[h]);
-                    e[r] *= sl.x;
+                    mids[h] = __builtin_fmaf(e[r], mid[r], mids[h]);
+                    e[r] *= step[r];
                 }
                 pp[h][kt >> 1][2 * (kt & 1)] = Mma<DT>::pack(e[0], e[1]);
                 pp[h][kt >> 1][2 * (kt & 1) + 1] = Mma<DT>::pack(e[2], e[3]);
