@@ -111,7 +111,8 @@ __device__ inline void store_token(char *cache, char *ranges, int row, const cha
         if (part == 0) *reinterpret_cast<uint32_t *>(ranges + (int64_t)row * 4) = range;
     }
 }
-// Tokens of sample n at positions lengths[n] on: those that a later token can see, sinks and the last `ring` ones.
+// Tokens of sample n at positions lengths[n] on: those that a later token can see, sinks and the last `ring` ones.  In 4 bits what bounds it is the vector unit: eight
+// divisions to a lane, since a code is a quotient's rounding (8 streams of up to 5000 tokens, 8 heads of 128: 32 us, 89 MB); with reciprocals, or two tokens at a time, 35 to 40.
 template <class DT, int BITS>
 __global__ void __launch_bounds__(kThreads)
 cache_append_kernel(char *__restrict__ kc, char *__restrict__ vc, char *__restrict__ kr, char *__restrict__ vr, const char *__restrict__ k, const char *__restrict__ v,
@@ -131,7 +132,7 @@ cache_append_kernel(char *__restrict__ kc, char *__restrict__ vc, char *__restri
         store_token<DT, BITS>(vc, vr, row, vx + t * a.v.row, a.width, part, lanes);
     }
 }
-// Rows as the values that they stand for: eight channels to a thread.
+// Rows as the values that they stand for: eight channels to a thread (8 x 8 x 4010 rows of 128: 16 us, 84 MB, 5.2 TB/s).
 template <class DT>
 __global__ void __launch_bounds__(kThreads) cache_rows_kernel(char *__restrict__ out, const char *__restrict__ codes, const char *__restrict__ ranges, int64_t words, int per_row) {
     for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < words; i += (int64_t)gridDim.x * kThreads) {
@@ -217,7 +218,7 @@ __device__ inline void join_waves(const Sums<C, QT> &s, char *smem, char *out, f
         }
     }
 }
-// The shares of a head's keys, in a fixed order: four channels of a row to a thread.
+// The shares of a head's keys, in a fixed order: four channels of a row to a thread, and eight shares on their way together (2 to 4 us, of which little is work).
 template <class DT, int C, int QT>
 __global__ void __launch_bounds__(kThreads) cache_join_kernel(char *__restrict__ out, const float *__restrict__ partial, uint32_t quads, CacheArgs a) {
     constexpr int kRows = 16 * QT, kAtOnce = 8;
@@ -302,7 +303,7 @@ __device__ inline void load_from(const char *p, LDS_PTR(char) lds) {
     const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)reinterpret_cast<uintptr_t>(lds));
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(p) : "memory");
 }
-// A key's row is in the cache, or with the call's tokens: a step does not wait for its own stores.  Past the share's last key that one is loaded again, and
+// 64 streams, 32 heads over 8 of 128 channels, 4100 keys: 178 us, 1.08 GB, 6.0 TB/s, more than a copy reaches.  A key's row is in the cache, or with the call's tokens: a step does not wait for its own stores.  Past the share's last key that one is loaded again, and
 // past a row's channels its first ones: finite, and met by probabilities and queries of zero.
 template <class DT, int C, int QT, int NW>
 __global__ void __launch_bounds__(64 * NW)
@@ -424,6 +425,8 @@ cache_attend_kernel(char *__restrict__ out, float *__restrict__ partial, const c
 // =============================================================================
 // Rows in 4 bits: units of 64 keys
 // =============================================================================
+// 64 streams, 32 heads over 8 of 128 channels, 8196 keys: 113 us, 572 MB, 5.1 TB/s.  What keeps it from the 6.0 of 16 bits is the vector unit: codes into values, and a softmax of
+// 16 rows where a group has four, about 550 instructions to a unit of 8.7 KB.
 // Values 16 + c of the eight codes of a word, channels (or keys) 0, 4, 1, 5, 2, 6, 3, 7 of it: codes four apart share a register.
 template <class DT> __device__ inline u32x4 of_codes(uint32_t w) {
     if constexpr (DT::tag == NA1D_BF16) {       // 16 (1 + c / 16): c at bit 3 of seven
@@ -650,10 +653,10 @@ struct CachePlan {
     CacheArgs a;
     int64_t items;
 };
-// Blocks of 16, 32 or 64 rows of queries.  Where the card is not full with a workgroup to every head of keys, and a large one gets through them with at most
-// kSerial units to a wave, that one has them all, and a launch less: one stream's step over 1028 keys, 4 heads of 64, takes 10.4 us in two kernels of
-// 16 workgroups and then of one.  Otherwise workgroups of four waves, as many to a head as occupy the card in whole rounds, with two units of keys to a wave
-// at least.
+// Blocks of 16, 32 or 64 rows of queries.  16-bit rows of up to 64 channels: where the card is not full with a workgroup to every head of keys, and a large one gets through them with at most
+// kSerial units to a wave, that one has them all, and a launch less: one stream's step over 1028 keys, 4 heads of 64, is 7.5 us in 4 workgroups of eight waves, and 6.2 and 3.6 in
+// 16 of four and a join.  (Rows in 4 bits, whose units take longer: 15.6 us in one workgroup of 16 waves to a head, 8.7 and 4.9 in shares, for 5 streams of 2 heads of 64, 2008 keys.)
+// Otherwise workgroups of four waves, as many to a head as occupy the card in whole rounds, with two units of keys to a wave at least, one in 4 bits.
 constexpr int kSerial = 5;
 CachePlan cache_plan(const na1d_sink_cache &c, int64_t fresh, int heads, int64_t window) {
     CachePlan p{};

@@ -154,6 +154,9 @@ template <class DT> __device__ inline void pack_twice(float x, float y, uint32_t
 // =============================================================================
 // Forward
 // =============================================================================
+// What bounds it: with long windows the matrix cores and what a softmax takes of the vector unit, which wait for each other (2 x 16 x 8192 rows of 128 channels, 4 key heads, window 1024:
+// 180 us, 0.72 PFLOP/s of what the mask leaves, matrix cores busy 0.41 of the time; 32 x 16384 over 8, window 2048: 540 us, 0.95 PFLOP/s, 0.49), with short ones memory (16 x 16 x 1000 rows of
+// 64 channels, window 128: 37 us, 154 MB behind the L2s, 4.2 TB/s), with few rows a chunk's way from memory (4 x 300 rows: 7 us).
 template <class DT, int C, int QT>
 __global__ void __launch_bounds__(kThreads, 3)
 sink_fwd_kernel(char *__restrict__ out, float *__restrict__ lse, char *__restrict__ rest, const char *__restrict__ q, const char *__restrict__ k, const char *__restrict__ v,
@@ -307,7 +310,7 @@ sink_fwd_kernel(char *__restrict__ out, float *__restrict__ lse, char *__restric
 // =============================================================================
 // Backward, query side: delta = rowsum(dO * O) and dQ = scale * dS K,  dS = P (dO V^T - delta)
 // =============================================================================
-// What bounds it is LDS: 24 KB of operands to a wave and 32 keys.  Two tiles of 16 queries to a wave, as in the forward, halve that, but 228 registers leave two waves to a SIMD and
+// What bounds it is LDS, 24 KB of operands to a wave and 32 keys, and the matrix cores (both busy 0.55 of the time at 2 x 16 x 8192 rows of 128, window 1024, 267 to 280 us).  Two tiles of 16 queries to a wave, as in the forward, halve that, but 228 registers leave two waves to a SIMD and
 // not four, and the launches are half as many workgroups: 2 x 16 x 8192, 128 channels, window 1024, takes 310 us and not 280; 16 x 16 x 1000, 64 channels, window 128, took
 // 57 and not 48, 5 x 10 x 777, 96 channels, window 100, 24 and not 17.5 (these two before dS went into the product twice).
 template <class DT, int C>
@@ -424,9 +427,9 @@ sink_dq_kernel(char *__restrict__ dq, float *__restrict__ delta, const char *__r
 // =============================================================================
 // A workgroup owns a strip of 64 keys, a tile of them to a wave, whose K and V rows stay in registers, and walks units of (head of the group, chunk
 // of 64 queries): Q and dO through LDS, double-buffered.  The score product is taken with Q and K swapped, so that P and dS come out as B operands.
-// What bounds it is LDS: 64 KB of operands to a wave and unit.  Two tiles of keys to a wave would halve that, and need 308 registers at 128 channels, so
-// one wave to a SIMD: 2 x 8192 tokens, 16 heads of 128 over 4, window 1024 took 510 us in place of 435; at 64 channels 81 in place of 60 (16 x
-// 16 x 1000, window 128).
+// What bounds it is LDS, 64 KB of operands to a wave and unit (busy 0.51 of the time), beside the matrix cores (0.46) and the waits of two waves to a SIMD for each other's: 2 x 8192 rows, 16
+// heads of 128 over 4, window 1024: 435 to 460 us; 16 x 16 x 1000 rows of 64, window 128: 64 us, 288 MB behind the L2s, 4.5 TB/s.  Two tiles of keys to a wave would halve what LDS gives,
+// and need 308 registers at 128 channels, so one wave to a SIMD: 510 us in place of 435 then, and at 64 channels 81 in place of 60.
 //
 // A launch ends when its last workgroup does, so it is cut to fit the card: strips beyond a whole number of rounds of it are shared by `parts` workgroups
 // each.  Sinks are seen by all queries behind them, other keys by a window of them: the queries that see of a strip nothing but its sinks are left to
