@@ -209,3 +209,43 @@ def test_caches_that_share_memory_are_refused(bits):
             streaming.cache_step(q, *tokens, *pair, lengths, 8)
     both = streaming.cache_attend(q, k, k, lengths + 3, 8)                # read only
     _same([both], [streaming.cache_attend(q, k, streaming.Rows4(*(t.clone() for t in k)) if bits == 4 else k.clone(), lengths + 3, 8)])
+
+
+def test_a_sequence_beyond_32_bits():
+    """Offsets of a head's rows pass 2^31 bytes: its last rows are those of a short sequence that ends with the same tokens.
+
+    Both round what differs by sums in another order (2^-20 of the value at most: some hundred fp32 terms) to bf16, half a step each: a step in all, 2^-8 * 2, of
+    which a norm keeps the same bound."""
+    T, part, W = 560128, 1024, 70                     # T a multiple of a strip
+    g = torch.Generator(device="cuda").manual_seed(51)
+    q, k, v, dout = (torch.randn(1, T, 16, 128, generator=g, device="cuda", dtype=torch.bfloat16) for _ in range(4))
+    assert q.numel() * 2 > 2 ** 31
+    whole = _grads(lambda *x: streaming.sink_attention(*x, W), q, k, v, dout)
+    short = _grads(lambda *x: streaming.sink_attention(*x, W), *(t[:, -part:].clone() for t in (q, k, v, dout)))
+    for name, a, b in zip(("out", "dq", "dk", "dv"), whole, short):
+        a, b = a[:, 2 * W - part:].double(), b[:, 2 * W:].double()
+        assert float((a - b).norm()) <= (2 ** -7 + 2 ** -20) * float(b.norm()), name
+    for t in whole:
+        assert bool(torch.isfinite(t[:, ::4097]).all()) and float(t[:, -part:].abs().max()) > 0
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_streams_of_two_to_the_thirty_tokens(bits):
+    """A stream's age matters by its place in the ring alone, up to 2^30 tokens; one that is older is idle."""
+    N, K, C, W, Z, n = 3, 2, 64, 40, 3, 2
+    ring = W + n - 1
+    q, k, v, _ = _inputs(N, 200, 4, K, C, torch.float16, 52)
+    old = 200 - n
+    laps = ((1 << 30) - n - old) // ring              # as many as leave the stream at 2^30 or just below once the step is done
+
+    def step(add):
+        caches = streaming.new_cache(N, K, Z + ring, C, bits, torch.float16)
+        streaming.cache_append(k[:, :old], v[:, :old], *caches, sinks=Z)
+        lengths = torch.full((N,), old + add, dtype=torch.int32, device="cuda")
+        outs = [streaming.cache_step(q[:, old:], k[:, old:], v[:, old:], *caches, lengths, W, Z), streaming.cache_attend(q[:, old:], *caches, lengths + n, W, Z)]
+        return outs + [t for c in caches for t in (c if bits == 4 else (c,))]
+    young = step(0)
+    _same(young, step(ring * laps))
+    assert old + ring * laps + n <= 1 << 30 < old + ring * (laps + 1) + n
+    over = step(ring * (laps + 2))
+    assert not bool(over[0].any()) and not bool(over[1].any()) and bool(young[0].any())
