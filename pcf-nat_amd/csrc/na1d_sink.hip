@@ -141,6 +141,13 @@ template <int C> __device__ inline void store_rest(char *rest, const uint32_t (&
     }
 }
 
+// What a wave has loaded for good is here before its loop: the compiler, which does not know of the loads that write LDS, would wait for it inside, where the chunk to come is on
+// its way, and so for that.
+template <int C> __device__ inline void settle_rows(RowOperand<C> &o) {
+#pragma unroll
+    for (int s = 0; s < RowOperand<C>::k32; ++s) settle(o.w32[s]);
+    if (RowOperand<C>::k16) settle(o.w16[0]);
+}
 // Two values as a pair of 16-bit numbers each: the roundings, and those of what these lost.  A row's dS sum to 0, so what all keys have in common drops out of dQ (and of dK
 // what all queries have), but not out of roundings of dS: they go into the products twice, and so does P into dV's.  As norms against 64 bits, 2 x 16 x 8192 rows, bf16, 16 sinks:
 // dQ 3.2e-3 -> 2.1e-3, dK and dV 2.4e-3 -> 1.7e-3, where the rounding of the result alone is 1.7e-3.  It costs 280 us and not 240 (dQ) and 460 and not 405 (dK and
@@ -206,6 +213,8 @@ sink_fwd_kernel(char *__restrict__ out, float *__restrict__ lse, char *__restric
         for (int ct = 0; ct < CT; ++ct) o[h][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
+#pragma unroll
+    for (int h = 0; h < QT; ++h) settle_rows<C>(qop[h]);
     int at = 0;                                           // byte offset of the chunk's pair of regions: 0 or 2 * kStep
     while (c < chunks.end) {
         wait_direct();
@@ -351,7 +360,7 @@ sink_dq_kernel(char *__restrict__ dq, float *__restrict__ delta, const char *__r
     load_rows<C, kReadShared>(qop, qs, own * a.q.pitch, a.q.pitch, width, lane);
     load_rows<C, kReadShared>(gop, gs, own * a.o.pitch, a.o.pitch, width, lane);
     load_rows<C, kReadOnce>(oop, os, own * a.o.pitch, a.o.pitch, width, lane);
-    const float ref = -__uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(ls, (own + n) * 4, 0, 0));      // minus the row's log2 of its sum
+    float ref = -__uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(ls, (own + n) * 4, 0, 0));      // minus the row's log2 of its sum
     const float scale2 = a.scale * kLog2e;
     RowLane<C, CS> row_lane;
     TrLane<C, CS> tr_lane;
@@ -365,6 +374,7 @@ sink_dq_kernel(char *__restrict__ dq, float *__restrict__ delta, const char *__r
     f32x4 acc[CT];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) acc[ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+    settle_rows<C>(qop), settle_rows<C>(gop), settle(ref);
     int at = 0;
     while (c < chunks.end) {
         wait_direct();
@@ -520,6 +530,7 @@ sink_dkv_kernel(char *__restrict__ dk, char *__restrict__ dv, float *__restrict_
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) acck[ct] = accv[ct] = f32x4{0.f, 0.f, 0.f, 0.f};
 
+    settle_rows<C>(kop), settle_rows<C>(vop);
     int at = 0;
     for (; u < u_end; ++u) {
         wait_direct();
