@@ -77,6 +77,20 @@ __device__ inline Sight sight(int q0, int q1, int k0, int k1, const SinkArgs &a)
     return k1 <= q0 && (k1 < a.sinks || q1 - k0 < a.window) ? kAll : kPart;
 }
 
+// The same for a wave's queries q0 .. q1 and chunks of keys by their number, worked out once: a chunk's turn is a chain of instructions, scalar ones among them.
+struct KeySight {
+    int last, sinks_end, passed, below, all_sinks, near;
+    __device__ inline KeySight(int q0, int q1, int tv, const SinkArgs &a)
+        : last(q0 < tv ? q1 / kKeyRows : -1), sinks_end((a.sinks + kKeyRows - 1) / kKeyRows), passed(floored(q0 - a.window - (kKeyRows - 1))), below(floored(q0 - (kKeyRows - 1))),
+          all_sinks(floored(a.sinks - kKeyRows)), near(floored(q1 - a.window) + 1) {}
+    __device__ static inline int floored(int x) { return x >> 5; }
+    __device__ inline Sight of(int c) const {
+        if (c > last || (c >= sinks_end && c <= passed)) return kNothing;
+        return c <= below && (c <= all_sinks || c >= near) ? kAll : kPart;
+    }
+};
+static_assert(kKeyRows == 32, "floored()");
+
 // `rows` rows of a tensor from row `row` on as a buffer resource: at most a strip of them, so that its bytes fit 31 bits wherever it lies.
 __device__ inline Rsrc rows_of(const void *base, int64_t row, int rows, int pitch) {
     const uint64_t at = (uint64_t)base + row * pitch;
@@ -175,6 +189,7 @@ sink_fwd_kernel(char *__restrict__ out, float *__restrict__ lse, char *__restric
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    __builtin_assume(wave >= 0 && wave < kWaves);
     const int g = lane >> 4, n = lane & 15;
     const SinkItem it = sink_item(blockIdx.x, items, a);
     const int head = it.kv * a.group + it.g, T = a.T, width = a.width;
@@ -213,6 +228,7 @@ sink_fwd_kernel(char *__restrict__ out, float *__restrict__ lse, char *__restric
         for (int ct = 0; ct < CT; ++ct) o[h][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
+    const KeySight sees(w0, w1, tv, a);
 #pragma unroll
     for (int h = 0; h < QT; ++h) settle_rows<C>(qop[h]);
     int at = 0;                                           // byte offset of the chunk's pair of regions: 0 or 2 * kStep
@@ -225,7 +241,7 @@ sink_fwd_kernel(char *__restrict__ out, float *__restrict__ lse, char *__restric
         LDS_PTR(char) v_lds = k_lds + kStep;
         at ^= 2 * kStep;
         c = next;
-        const Sight see = w0 < tv ? sight(w0, w1, k0, k0 + kKeyRows - 1, a) : kNothing;
+        const Sight see = sees.of(k0 / kKeyRows);
         if (see == kNothing) continue;
         f32x4 s[QT][kKeyTiles];
 #pragma unroll
@@ -334,6 +350,7 @@ sink_dq_kernel(char *__restrict__ dq, float *__restrict__ delta, const char *__r
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    __builtin_assume(wave >= 0 && wave < kWaves);
     const int g = lane >> 4, n = lane & 15;
     const SinkItem it = sink_item(blockIdx.x, items, a);
     const int head = it.kv * a.group + it.g, T = a.T, width = a.width;
@@ -374,6 +391,7 @@ sink_dq_kernel(char *__restrict__ dq, float *__restrict__ delta, const char *__r
     f32x4 acc[CT];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) acc[ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const KeySight sees(w0, w1, tv, a);
     settle_rows<C>(qop), settle_rows<C>(gop), settle(ref);
     int at = 0;
     while (c < chunks.end) {
@@ -385,7 +403,7 @@ sink_dq_kernel(char *__restrict__ dq, float *__restrict__ delta, const char *__r
         LDS_PTR(char) v_lds = k_lds + kStep;
         at ^= 2 * kStep;
         c = next;
-        const Sight see = w0 < tv ? sight(w0, w1, k0, k0 + kKeyRows - 1, a) : kNothing;
+        const Sight see = sees.of(k0 / kKeyRows);
         if (see == kNothing) continue;
 #pragma unroll
         for (int kt = 0; kt < kKeyTiles; kt += 2) {
@@ -464,6 +482,7 @@ sink_dkv_kernel(char *__restrict__ dk, char *__restrict__ dv, float *__restrict_
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    __builtin_assume(wave >= 0 && wave < kWaves);
     const int g = lane >> 4, n = lane & 15;
     // strips with a workgroup of their own; then (`rest` of them) the parts of the others, and the far workgroups
     uint32_t strip_id, part = 0, each = 1, head, strip;
