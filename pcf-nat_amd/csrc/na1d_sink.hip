@@ -91,10 +91,10 @@ struct KeySight {
 };
 static_assert(kKeyRows == 32, "floored()");
 
-// `rows` rows of a tensor from row `row` on as a buffer resource: at most a strip of them, so that its bytes fit 31 bits wherever it lies.
-__device__ inline Rsrc rows_of(const void *base, int64_t row, int rows, int pitch) {
-    const uint64_t at = (uint64_t)base + row * pitch;
-    return make_rsrc((const void *)((uint64_t)(uint32_t)uniform((int)(at >> 32)) << 32 | (uint32_t)uniform((int)at)), uniform(max(0, rows) * pitch));
+// `rows` rows (0 or more) of a tensor from row `row` on as a buffer resource: at most a strip of them, so that its bytes fit 31 bits wherever it lies.
+__device__ inline Rsrc rows_of(const void *base, int row, int rows, int pitch) {
+    const uint64_t at = (uint64_t)base + (int64_t)row * pitch;
+    return make_rsrc((const void *)((uint64_t)(uint32_t)uniform((int)(at >> 32)) << 32 | (uint32_t)uniform((int)at)), uniform(rows) * pitch);
 }
 
 // What outputs lose in rounding, for the backward: delta = rowsum(dO * O) is taken away from every dP of a row, and with O as it is stored, half a step off, that
@@ -200,14 +200,14 @@ sink_fwd_kernel(char *__restrict__ out, float *__restrict__ lse, char *__restric
     const int k_lane = direct_lane_offset<CS>(wave, lane, a.k.pitch, width), v_lane = direct_lane_offset<CS>(wave, lane, a.v.pitch, width);
     auto stage = [&](int c, LDS_PTR(char) to) {
         const int rows = min(kKeyRows, tv - c * kKeyRows);
-        stage_direct<CS, kKeyTiles, kReadShared>(rows_of(kb, (int64_t)c * kKeyRows, rows, a.k.pitch), 0, to, kKeyTiles, wave, k_lane, a.k.pitch);
-        stage_direct<CS, kKeyTiles, kReadShared>(rows_of(vb, (int64_t)c * kKeyRows, rows, a.v.pitch), 0, to + kStep, kKeyTiles, wave, v_lane, a.v.pitch);
+        stage_direct<CS, kKeyTiles, kReadShared>(rows_of(kb, c * kKeyRows, rows, a.k.pitch), 0, to, kKeyTiles, wave, k_lane, a.k.pitch);
+        stage_direct<CS, kKeyTiles, kReadShared>(rows_of(vb, c * kKeyRows, rows, a.v.pitch), 0, to + kStep, kKeyTiles, wave, v_lane, a.v.pitch);
     };
     const KeyChunks chunks(row0, row_end - 1, tv, a);
     int c = chunks.first();
     if (c < chunks.end) stage(c, kv_lds);
     const int own = 16 * QT * wave, w0 = row0 + own, w1 = w0 + 16 * QT - 1;      // this wave's rows
-    const Rsrc qs = rows_of(q + it.sample * a.q.sample + head * a.q.head, row0, min(row_end, tv) - row0, a.q.pitch);
+    const Rsrc qs = rows_of(q + it.sample * a.q.sample + head * a.q.head, row0, max(0, min(row_end, tv) - row0), a.q.pitch);
     RowOperand<C> qop[QT];
 #pragma unroll
     for (int h = 0; h < QT; ++h) load_rows<C, kReadOnce>(qop[h], qs, (own + 16 * h) * a.q.pitch, a.q.pitch, width, lane);
@@ -361,15 +361,15 @@ sink_dq_kernel(char *__restrict__ dq, float *__restrict__ delta, const char *__r
     const int k_lane = direct_lane_offset<CS>(wave, lane, a.k.pitch, width), v_lane = direct_lane_offset<CS>(wave, lane, a.v.pitch, width);
     auto stage = [&](int c, LDS_PTR(char) to) {
         const int rows = min(kKeyRows, tv - c * kKeyRows);
-        stage_direct<CS, kKeyTiles, kReadShared>(rows_of(kb, (int64_t)c * kKeyRows, rows, a.k.pitch), 0, to, kKeyTiles, wave, k_lane, a.k.pitch);
-        stage_direct<CS, kKeyTiles, kReadShared>(rows_of(vb, (int64_t)c * kKeyRows, rows, a.v.pitch), 0, to + kStep, kKeyTiles, wave, v_lane, a.v.pitch);
+        stage_direct<CS, kKeyTiles, kReadShared>(rows_of(kb, c * kKeyRows, rows, a.k.pitch), 0, to, kKeyTiles, wave, k_lane, a.k.pitch);
+        stage_direct<CS, kKeyTiles, kReadShared>(rows_of(vb, c * kKeyRows, rows, a.v.pitch), 0, to + kStep, kKeyTiles, wave, v_lane, a.v.pitch);
     };
     const KeyChunks chunks(row0, row_end - 1, tv, a);
     int c = chunks.first();
     if (c < chunks.end) stage(c, kv_lds);
     const int own = 16 * wave, w0 = row0 + own, w1 = w0 + 15;
     const int64_t o_off = it.sample * a.o.sample + head * a.o.head, stat = ((int64_t)it.sample * a.H + head) * T + row0;
-    const int valid_rows = min(row_end, tv) - row0;
+    const int valid_rows = max(0, min(row_end, tv) - row0);
     const Rsrc qs = rows_of(q + it.sample * a.q.sample + head * a.q.head, row0, valid_rows, a.q.pitch);
     const Rsrc os = rows_of(out + o_off, row0, valid_rows, a.o.pitch), gs = rows_of(dout + o_off, row0, valid_rows, a.o.pitch);
     const Rsrc ls = make_rsrc(lse + stat, (row_end - row0) * 4), ds = make_rsrc(delta + stat, (row_end - row0) * 4);
@@ -518,24 +518,28 @@ sink_dkv_kernel(char *__restrict__ dk, char *__restrict__ dv, float *__restrict_
     }
     const int nc = c_end - c_from, units = nc * a.group, u_end = uniform((int)((int64_t)units * (part + 1) / each));
     int u = uniform((int)((int64_t)units * part / each));
-    int hg = nc ? uniform(u / nc) : 0, c = nc ? c_from + u - hg * nc : 0;
+    const int hg = nc ? uniform(u / nc) : 0;
+    int c = nc ? c_from + u - hg * nc : 0;
 
     const int q_lane = direct_lane_offset<CS>(wave, lane, a.q.pitch, width), g_lane = direct_lane_offset<CS>(wave, lane, a.o.pitch, width);
     const char *qb = q + sample * a.q.sample, *gb = dout + sample * a.o.sample;
     float row_lse, row_delta;                             // of row 16 * wave + n of the chunk in flight
-    auto stage = [&](int hg_, int c_, LDS_PTR(char) to) {
-        const int h = kv * a.group + hg_, rows = min(kChunkRows, tv - c_ * kChunkRows);
-        const int64_t r0 = (int64_t)c_ * kChunkRows, stat = ((int64_t)sample * a.H + h) * T + r0;
-        stage_direct<CS, kChunkTiles, kReadShared>(rows_of(qb + h * a.q.head, r0, rows, a.q.pitch), 0, to, kChunkTiles, wave, q_lane, a.q.pitch);
-        stage_direct<CS, kChunkTiles, kReadShared>(rows_of(gb + h * a.o.head, r0, rows, a.o.pitch), 0, to + kStep, kChunkTiles, wave, g_lane, a.o.pitch);
-        const Rsrc ls = rows_of(lse + stat, 0, rows, 4), ds = rows_of(delta + stat, 0, rows, 4);
+    // of the head at hand: where it begins, and its rows' constants
+    const int first_head = kv * a.group + hg;
+    const char *qh = qb + first_head * a.q.head, *gh = gb + first_head * a.o.head;
+    const float *lse_h = lse + ((int64_t)sample * a.H + first_head) * T, *delta_h = delta + ((int64_t)sample * a.H + first_head) * T;
+    auto stage = [&](int c_, LDS_PTR(char) to) {
+        const int r0 = c_ * kChunkRows, rows = min(kChunkRows, tv - r0);
+        stage_direct<CS, kChunkTiles, kReadShared>(rows_of(qh, r0, rows, a.q.pitch), 0, to, kChunkTiles, wave, q_lane, a.q.pitch);
+        stage_direct<CS, kChunkTiles, kReadShared>(rows_of(gh, r0, rows, a.o.pitch), 0, to + kStep, kChunkTiles, wave, g_lane, a.o.pitch);
+        const Rsrc ls = rows_of(lse_h, r0, rows, 4), ds = rows_of(delta_h, r0, rows, 4);
         row_lse = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(ls, (16 * wave + n) * 4, 0, 0));
         row_delta = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(ds, (16 * wave + n) * 4, 0, 0));
     };
-    if (u < u_end) stage(hg, c, buf_lds);
+    if (u < u_end) stage(c, buf_lds);
     const int own = 16 * wave, w0 = row0 + own, w1 = w0 + 15, key = w0 + n;
-    const Rsrc ks = rows_of(k + sample * a.k.sample + kv * a.k.head, row0, last_key + 1 - row0, a.k.pitch);
-    const Rsrc vs = rows_of(v + sample * a.v.sample + kv * a.v.head, row0, last_key + 1 - row0, a.v.pitch);
+    const Rsrc ks = rows_of(k + sample * a.k.sample + kv * a.k.head, row0, max(0, last_key + 1 - row0), a.k.pitch);
+    const Rsrc vs = rows_of(v + sample * a.v.sample + kv * a.v.head, row0, max(0, last_key + 1 - row0), a.v.pitch);
     RowOperand<C> kop, vop;
     load_rows<C, kReadShared>(kop, ks, own * a.k.pitch, a.k.pitch, width, lane);
     load_rows<C, kReadShared>(vop, vs, own * a.v.pitch, a.v.pitch, width, lane);
@@ -560,8 +564,8 @@ sink_dkv_kernel(char *__restrict__ dk, char *__restrict__ dv, float *__restrict_
         }
         barrier_lds();
         const int q0 = c * kChunkRows;
-        if (++c == c_end) c = c_from, ++hg;
-        if (u + 1 < u_end) stage(hg, c, buf_lds + (kBuf - at));
+        if (++c == c_end) c = c_from, qh += a.q.head, gh += a.o.head, lse_h += T, delta_h += T;
+        if (u + 1 < u_end) stage(c, buf_lds + (kBuf - at));
         LDS_PTR(char) q_lds = buf_lds + at;
         LDS_PTR(char) g_lds = q_lds + kStep;
         LDS_PTR(char) ref_lds = q_lds + 2 * kStep + 16 * g;
