@@ -303,6 +303,12 @@ __device__ inline void load_from(const char *p, LDS_PTR(char) lds) {
     const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)reinterpret_cast<uintptr_t>(lds));
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(p) : "memory");
 }
+// The same from `offset` bytes behind a place that is the same in all lanes.
+__device__ inline void load_behind(const char *p, int offset, LDS_PTR(char) lds) {
+    const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)reinterpret_cast<uintptr_t>(lds));
+    const uint64_t base = (uint64_t)(uint32_t)uniform((int)((uint64_t)p >> 32)) << 32 | (uint32_t)uniform((int)(uint64_t)p);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(offset), "s"(base) : "memory");
+}
 // 64 streams, 32 heads over 8 of 128 channels, 4100 keys: 178 us, 1.08 GB, 6.0 TB/s, more than a copy reaches.  A key's row is in the cache, or with the call's tokens: a step does not wait for its own stores.  Past the share's last key that one is loaded again, and
 // past a row's channels its first ones: finite, and met by probabilities and queries of zero.
 template <class DT, int C, int QT, int NW>
@@ -336,6 +342,18 @@ cache_attend_kernel(char *__restrict__ out, float *__restrict__ partial, const c
     const char *kx = k + p.sample * a.k.sample + p.kv * a.k.head, *vx = v + p.sample * a.v.sample + p.kv * a.v.head;
     const int old = seen.total - a.stored;
     auto stage = [&](int i, LDS_PTR(char) to) {
+        int row0 = seen.first + (i - seen.apart);
+        if (row0 >= seen.ring) row0 -= seen.ring;
+        if (i >= seen.apart && i + kUnit <= min(i1, old) && row0 + kUnit <= seen.ring) {      // rows of the cache, one behind the other
+            const int64_t base = (int64_t)(seen.sinks + row0) * a.width;
+#pragma unroll
+            for (int c = 0; c < kRegion / kChunk; ++c) {
+                const int r = c * kChunkKeys + lane / LL::kUnits, unit = (lane % LL::kUnits) ^ LL::swz(r), offset = r * a.width + (unit * 16 < a.width ? unit * 16 : 0);
+                load_behind(ks + base, offset, to + c * kChunk);
+                load_behind(vs + base, offset, to + kRegion + c * kChunk);
+            }
+            return;
+        }
 #pragma unroll
         for (int c = 0; c < kRegion / kChunk; ++c) {
             const int r = c * kChunkKeys + lane / LL::kUnits, unit = (lane % LL::kUnits) ^ LL::swz(r), key = min(i + r, i1 - 1);
