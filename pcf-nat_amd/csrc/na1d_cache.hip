@@ -672,7 +672,7 @@ struct CachePlan {
     int64_t items;
 };
 // Blocks of 16, 32 or 64 rows of queries.  16-bit rows of up to 64 channels: where the card is not full with a workgroup to every head of keys, and a large one gets through them with at most
-// kSerial units to a wave, that one has them all, and a launch less: one stream's step over 1028 keys, 4 heads of 64, is 7.5 us in 4 workgroups of eight waves, and 6.2 and 3.6 in
+// kSerial units to a wave, that one has them all, and a launch less: one stream's step over 1028 keys, 4 heads of 64, was 7.5 us in 4 workgroups of eight waves (7.0 since), and 6.2 and 3.6 in
 // 16 of four and a join.  (Rows in 4 bits, whose units take longer: 15.6 us in one workgroup of 16 waves to a head, 8.7 and 4.9 in shares, for 5 streams of 2 heads of 64, 2008 keys.)
 // Otherwise workgroups of four waves, as many to a head as occupy the card in whole rounds, with two units of keys to a wave at least, one in 4 bits.
 constexpr int kSerial = 5;

@@ -164,7 +164,7 @@ template <int C> __device__ inline void settle_rows(RowOperand<C> &o) {
 }
 // Two values as a pair of 16-bit numbers each: the roundings, and those of what these lost.  A row's dS sum to 0, so what all keys have in common drops out of dQ (and of dK
 // what all queries have), but not out of roundings of dS: they go into the products twice, and so does P into dV's.  As norms against 64 bits, 2 x 16 x 8192 rows, bf16, 16 sinks:
-// dQ 3.2e-3 -> 2.1e-3, dK and dV 2.4e-3 -> 1.7e-3, where the rounding of the result alone is 1.7e-3.  It costs 280 us and not 240 (dQ) and 460 and not 405 (dK and
+// dQ 3.2e-3 -> 2.1e-3, dK and dV 2.4e-3 -> 1.7e-3, where the rounding of the result alone is 1.7e-3.  It cost 280 us and not 240 (dQ) and 460 and not 405 (dK and
 // dV) there, at 128 channels, 52 and 48, 64 and 61 for 16 x 16 x 1000 rows of 64 channels, window 128.
 template <class DT> __device__ inline void pack_twice(float x, float y, uint32_t &w, uint32_t &rest) {
     w = Mma<DT>::pack(x, y);
@@ -176,8 +176,9 @@ template <class DT> __device__ inline void pack_twice(float x, float y, uint32_t
 // Forward
 // =============================================================================
 // What bounds it: with long windows the matrix cores and what a softmax takes of the vector unit, which wait for each other (2 x 16 x 8192 rows of 128 channels, 4 key heads, window 1024:
-// 180 us, 0.72 PFLOP/s of what the mask leaves, matrix cores busy 0.41 of the time; 32 x 16384 over 8, window 2048: 540 us, 0.95 PFLOP/s, 0.49), with short ones memory (16 x 16 x 1000 rows of
-// 64 channels, window 128: 37 us, 154 MB behind the L2s, 4.2 TB/s), with few rows a chunk's way from memory (4 x 300 rows: 7 us).
+// 170 us, 0.77 PFLOP/s of what the mask leaves, matrix cores busy 0.44 of the time; 32 x 16384 over 8, window 2048: 513 us, 1.0 PFLOP/s, 0.53), with short ones memory (16 x 16 x 1000 rows of
+// 64 channels, window 128: 33 us, 153 MB behind the L2s, 4.6 TB/s), with few rows a chunk's turn, a chain of
+// dependent instructions (4 x 300 rows: 6.7 us; a third chunk on its way does nothing for them).
 template <class DT, int C, int QT>
 __global__ void __launch_bounds__(kThreads, 3)
 sink_fwd_kernel(char *__restrict__ out, float *__restrict__ lse, char *__restrict__ rest, const char *__restrict__ q, const char *__restrict__ k, const char *__restrict__ v,
@@ -335,8 +336,8 @@ sink_fwd_kernel(char *__restrict__ out, float *__restrict__ lse, char *__restric
 // =============================================================================
 // Backward, query side: delta = rowsum(dO * O) and dQ = scale * dS K,  dS = P (dO V^T - delta)
 // =============================================================================
-// What bounds it is LDS, 24 KB of operands to a wave and 32 keys, and the matrix cores (both busy 0.55 of the time at 2 x 16 x 8192 rows of 128, window 1024, 267 to 280 us).  Two tiles of 16 queries to a wave, as in the forward, halve that, but 228 registers leave two waves to a SIMD and
-// not four, and the launches are half as many workgroups: 2 x 16 x 8192, 128 channels, window 1024, takes 310 us and not 280; 16 x 16 x 1000, 64 channels, window 128, took
+// What bounds it is LDS, 24 KB of operands to a wave and 32 keys, and the matrix cores (both busy 0.6 of the time at 2 x 16 x 8192 rows of 128, window 1024, 254 to 272 us).  Two tiles of 16 queries to a wave, as in the forward, halve that, but 228 registers leave two waves to a SIMD and
+// not four, and the launches are half as many workgroups: 2 x 16 x 8192, 128 channels, window 1024, took 310 us and not 280; 16 x 16 x 1000, 64 channels, window 128, took
 // 57 and not 48, 5 x 10 x 777, 96 channels, window 100, 24 and not 17.5 (these two before dS went into the product twice).
 template <class DT, int C>
 __global__ void __launch_bounds__(kThreads)
@@ -455,8 +456,8 @@ sink_dq_kernel(char *__restrict__ dq, float *__restrict__ delta, const char *__r
 // =============================================================================
 // A workgroup owns a strip of 64 keys, a tile of them to a wave, whose K and V rows stay in registers, and walks units of (head of the group, chunk
 // of 64 queries): Q and dO through LDS, double-buffered.  The score product is taken with Q and K swapped, so that P and dS come out as B operands.
-// What bounds it is LDS, 64 KB of operands to a wave and unit (busy 0.51 of the time), beside the matrix cores (0.46) and the waits of two waves to a SIMD for each other's: 2 x 8192 rows, 16
-// heads of 128 over 4, window 1024: 435 to 460 us; 16 x 16 x 1000 rows of 64, window 128: 64 us, 288 MB behind the L2s, 4.5 TB/s.  Two tiles of keys to a wave would halve what LDS gives,
+// What bounds it is LDS, 64 KB of operands to a wave and unit (busy 0.54 of the time), beside the matrix cores (0.49) and the waits of two waves to a SIMD for each other's: 2 x 8192 rows, 16
+// heads of 128 over 4, window 1024: 425 to 460 us; 16 x 16 x 1000 rows of 64, window 128: 60 us, 289 MB behind the L2s, 4.8 TB/s.  Two tiles of keys to a wave would halve what LDS gives,
 // and need 308 registers at 128 channels, so one wave to a SIMD: 510 us in place of 435 then, and at 64 channels 81 in place of 60.
 //
 // A launch ends when its last workgroup does, so it is cut to fit the card: strips beyond a whole number of rounds of it are shared by `parts` workgroups
