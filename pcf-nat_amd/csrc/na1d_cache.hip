@@ -13,7 +13,8 @@
 // codes as they are, exact in 16 bits:
 //   q . k = step (q . (16 + c)) + (low - 16 step) sum(q),   sum p v = sum (p step)(16 + c) - 23.5 sum (p step) + sum p (low + 7.5 step)
 // where 16 + c costs two instructions for two codes: the code's bits shifted and put into the mantissa of 16.  (p step) is rounded to 16 bits, all else is
-// exact or fp32; with 16 for 23.5 and low for the middle of the row's range that rounding would weigh up to 15 steps in place of 7.5.
+// exact or fp32; with 16 for 23.5 and low for the middle of the row's range that rounding would weigh up to 15 steps in place of 7.5.  In fp16, where p may be
+// 2^6 and a step anything from 2^-24 to 2^13, steps count times a power of two that a wave chooses by the largest it has met.
 #include <type_traits>
 
 #include "na1d_mfma_core.h"
@@ -536,6 +537,10 @@ cache_attend4_kernel(char *__restrict__ out, float *__restrict__ partial, const 
     float mids[QT];             // this lane's part of sum p (low + 7.5 step)
 #pragma unroll
     for (int h = 0; h < QT; ++h) steps[h] = f32x4{0.f, 0.f, 0.f, 0.f}, mids[h] = 0.f;
+    // fp16: steps, and with them `o` and `steps`, count times 2^up.  The largest step is between 2^7 and 2^9 then: 2^15 with a p of 2^6, while a key is off by 2^-32 of it at most where
+    // its product is below fp16's normal range (as they were, products of steps above 1000 were infinite, and those of shares of 2^-12 with steps of 2^-11 a tenth off).
+    constexpr bool kLifts = DT::tag == NA1D_FP16;
+    int up = 31;                // has the least step there
     int at = 0;
     int i = i0 + kUnit * wave;
     if (i < i1) stage(i, mine);
@@ -567,6 +572,24 @@ cache_attend4_kernel(char *__restrict__ out, float *__restrict__ partial, const 
         LDS_PTR(char) r_lds = v_lds + kCodes;
         // What goes with a key, worked out by one lane for all: in the place of the ranges first K's numbers, then V's (the wave's own accesses stay in order, and all are of 32-bit integers).
         const f32x2 of_k = unpack2<DT>(*reinterpret_cast<LDS_PTR(uint32_t)>(r_lds + 4 * lane)), of_v = unpack2<DT>(*reinterpret_cast<LDS_PTR(uint32_t)>(r_lds + kRanges + 4 * lane));
+        float v_step = of_v.x;
+        if constexpr (kLifts) {
+            if (__builtin_amdgcn_ballot_w64(__builtin_amdgcn_ldexpf(v_step, up) > 512.f)) {
+                float most = v_step;
+#pragma unroll
+                for (int d = 1; d < 64; d *= 2) most = __builtin_fmaxf(most, __shfl_xor(most, d));
+                const int now = uniform(8 - __builtin_amdgcn_frexp_expf(most));       // between 2^7 and 2^8
+                const float by = __builtin_amdgcn_ldexpf(1.f, now - up);
+                up = now;
+#pragma unroll
+                for (int h = 0; h < QT; ++h) {
+                    steps[h] *= by;
+#pragma unroll
+                    for (int ct = 0; ct < CT; ++ct) sums.o[h][ct] *= by;
+                }
+            }
+            v_step = __builtin_amdgcn_ldexpf(v_step, up);
+        }
         auto share = [&](float x, float y) {
             *reinterpret_cast<LDS_PTR(uint32_t)>(r_lds + 4 * lane) = __float_as_uint(x);
             *reinterpret_cast<LDS_PTR(uint32_t)>(r_lds + kRanges + 4 * lane) = __float_as_uint(y);
@@ -593,7 +616,7 @@ cache_attend4_kernel(char *__restrict__ out, float *__restrict__ partial, const 
 #pragma unroll
                 for (int h = 0; h < QT; ++h) z[h][kt][r] = __builtin_fmaf(z[h][kt][r], by[r], and_[r] * qsum[h]);
         }
-        share(of_v.x, __builtin_fmaf(7.5f, of_v.x, of_v.y));
+        share(v_step, __builtin_fmaf(7.5f, of_v.x, of_v.y));
         const bool ends = i + kUnit > i1;
         u32x4 pp[QT][2];
 #pragma unroll
@@ -652,9 +675,11 @@ cache_attend4_kernel(char *__restrict__ out, float *__restrict__ partial, const 
     }
 #pragma unroll
     for (int h = 0; h < QT; ++h) {
-        const float extra = __builtin_fmaf(-23.5f, steps[h][0], xor_sum(mids[h]));
+        const float down = kLifts ? __builtin_amdgcn_ldexpf(1.f, -up) : 1.f, extra = __builtin_fmaf(-23.5f * down, steps[h][0], xor_sum(mids[h]));
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) sums.o[h][ct] += f32x4{extra, extra, extra, extra};
+        for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sums.o[h][ct][r] = __builtin_fmaf(sums.o[h][ct][r], down, extra);
     }
     join_waves<DT, C, QT, NW>(sums, smem, out, partial, p.head, p.sample, p.kv, p.block, p.split, wave, lane, a);
 }

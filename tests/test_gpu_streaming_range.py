@@ -1,0 +1,87 @@
+"""Attention of streams where numbers are large or small for their 16-bit type, against its formulas in 64 bits.
+
+`u` is half a step of the type.  fp16 rounds below 2^-14 to multiples of 2^-24, half of one off; the kernels lift what they round: a product with a step of 4 bits so that the
+largest step is 2^7 at least, so that it is off by 2^-32 of that step."""
+import pytest
+import torch
+
+from na1d_amd import streaming
+from oracle import streaming_oracle as O
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.bfloat16, torch.float16]
+NAMES = ["bf16", "fp16"]
+
+
+def _near(got, value, bound):
+    torch.cuda.synchronize()
+    off = (got.double() - value).abs()
+    if not bool((off <= bound).all()):
+        worst = (off / bound).nan_to_num(torch.inf).argmax()
+        pytest.fail("off by %.3g where %.3g is allowed, of %.3g" % (off.flatten()[worst], bound.flatten()[worst], value.flatten()[worst]))
+
+
+# ------------------------------------------------------------------------------------------------ rows in 4 bits
+def _over_four(q, k, v, W, Z, dtype, scale):
+    """One token's attention over a cache in 4 bits that the others have been put into, what it should be, and how far off it may be:
+    as over_history counts it, but for what is too small for fp16: 7.5 of 2^-32 of the largest step for every key, and half a step of the result's."""
+    N, T, K, C = k.shape
+    cache = streaming.new_cache(N, K, Z + W, C, 4, dtype)
+    streaming.cache_append(k, v, *cache, sinks=Z)
+    lengths = torch.full((N,), T, dtype=torch.int32, device="cuda")
+    got = streaming.cache_attend(q, *cache, lengths, W, Z, scale=scale)
+    value, bound = O.over_history(q, k, v, W, Z, [T] * N, scale=scale, four=True)
+    largest = O.in_4_bits(v)[1].double().max().item()
+    least = 2.0 ** -25 if dtype == torch.float16 else 2.0 ** -126
+    bound = bound - least * (1 + 16 * N * T) + least + (7.5 * 2.0 ** -32 * largest * T if dtype == torch.float16 else 0.0)
+    return got, value, bound
+
+
+def _rising(N, T, K, C, dtype, octaves):
+    """Keys whose scores, for queries of ones and a scale of 1 / C, rise by so many octaves from one unit of 64 keys to the next (a wave has every fourth)."""
+    rise = torch.arange(T) // 64 * (octaves * 0.6931)
+    return rise.view(1, T, 1, 1).expand(N, T, K, C).to(dtype).cuda().contiguous()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=NAMES)
+@pytest.mark.parametrize("N,H,K,C,T,W", [(2, 4, 2, 32, 500, 400), (32, 32, 32, 32, 1200, 1200), (16, 64, 64, 64, 700, 700), (16, 64, 64, 96, 600, 590), (8, 64, 64, 128, 1000, 900),
+                                         (2, 4, 2, 128, 2500, 2400)])
+def test_wide_values_in_4_bits(N, H, K, C, T, W, dtype):
+    """Scores that rise by less than what moves the softmax's reference, so that probabilities pass 1, and values whose steps are 1000 and more.  With many
+    heads a wave has several units of a head's keys, one after the other."""
+    g = torch.Generator().manual_seed(C)
+    q = torch.ones(N, 1, H, C, dtype=dtype, device="cuda")
+    v = (torch.randn(N, T, K, C, generator=g) * 4000).clamp(-65000, 65000)
+    v[:, T // 2:, 1] *= 4                                              # ranges up to all that fp16 has
+    v = v.clamp(-65000, 65000).to(dtype).cuda()
+    for octaves in (1.45, 0.7, 0.0):
+        got, value, bound = _over_four(q, _rising(N, T, K, C, dtype, octaves), v, W, 0, dtype, 1.0 / C)
+        _near(got, value, bound)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=NAMES)
+@pytest.mark.parametrize("N,H,K,C,T", [(2, 8, 2, 32, 500), (32, 64, 32, 32, 900), (2, 8, 2, 64, 1100), (16, 64, 64, 96, 600), (8, 64, 64, 128, 700)])
+def test_steps_of_very_different_sizes_in_4_bits(N, H, K, C, T, dtype):
+    g = torch.Generator().manual_seed(C)
+    q, k = (torch.randn(N, t, h, C, generator=g).to(dtype).cuda() for t, h in ((1, H), (T, K)))
+    order = torch.randperm(T, generator=g)
+    for sizes in (2.0 ** (torch.arange(T) / T * 24 - 12), 2.0 ** (12 - torch.arange(T) / T * 24), (2.0 ** (torch.arange(T) / T * 24 - 12))[order]):
+        v = (torch.randn(N, T, K, C, generator=g) * sizes.view(1, T, 1, 1)).to(dtype).cuda()
+        got, value, bound = _over_four(q, k, v, T, 0, dtype, None)
+        _near(got, value, bound)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=NAMES)
+@pytest.mark.parametrize("size", [2.0 ** -10, 1.0])
+def test_small_shares_in_4_bits(size, dtype):
+    """A sink without a value takes nearly all of every row; what is left are products of small probabilities and, possibly, small steps."""
+    N, H, K, C, T = 2, 4, 2, 64, 900
+    q = torch.ones(N, 1, H, C, dtype=dtype, device="cuda")
+    k, v = torch.zeros(N, T, K, C), torch.randn(1, 1, K, C, generator=torch.Generator().manual_seed(1)).expand(N, T, K, C) * size
+    k[:, 0] = 8.3                                                      # e^-8.3 is 2^-12
+    v = v.clone()
+    v[:, 0] = 0.0
+    got, value, bound = _over_four(q, k.to(dtype).cuda(), v.to(dtype).cuda(), T - 1, 1, dtype, 1.0 / C)
+    assert float(value.abs().max()) > 0.05 * size
+    _near(got, value, bound)
