@@ -484,7 +484,8 @@ int na1d_sink_backward(const na1d_sink *h, void *dq, void *dk, void *dv, const v
  *   attended to as the cache holds them.
  * Strides as in na1d_sink.  What a call writes to shares no memory with the rest.  capacity - sinks >= window + fresh - 1 (NA1D_ERR_WINDOW).  capacity * head_dim up to 2^29, N * kv_heads to 2^24,
  * fresh * heads / kv_heads to 2^20, heads to 2^24 (NA1D_ERR_UNSUPPORTED).  All pointers but lengths and t_valid 16-byte aligned.  A workspace is needed where
- * na1d_sink_attend_workspace_bytes() is above 0.  rows: what `rows` rows of codes stand for, in `dtype`.
+ * na1d_sink_attend_workspace_bytes() is above 0.  rows: what `rows` rows of codes stand for, in `dtype` (its largest number where the last code of a step that was rounded up
+ * stands for more).
  */
 typedef struct na1d_sink_cache {
     int32_t dtype, bits, kv_heads, head_dim;

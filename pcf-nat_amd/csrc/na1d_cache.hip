@@ -133,7 +133,9 @@ cache_append_kernel(char *__restrict__ kc, char *__restrict__ vc, char *__restri
         store_token<DT, BITS>(vc, vr, row, vx + t * a.v.row, a.width, part, lanes);
     }
 }
-// Rows as the values that they stand for: eight channels to a thread (8 x 8 x 4010 rows of 128: 16 us, 84 MB, 5.2 TB/s).
+// Rows as the values that they stand for, or the type's largest number where a step that was rounded up leads beyond it (an fp16 row of -65504 .. 65504 has steps of 8736): eight channels
+// to a thread (8 x 8 x 4010 rows of 128: 16 us, 84 MB, 5.2 TB/s).
+template <class DT> constexpr float kLargest = DT::tag == NA1D_BF16 ? 0x1.fep127f : 65504.f;
 template <class DT>
 __global__ void __launch_bounds__(kThreads) cache_rows_kernel(char *__restrict__ out, const char *__restrict__ codes, const char *__restrict__ ranges, int64_t words, int per_row) {
     for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < words; i += (int64_t)gridDim.x * kThreads) {
@@ -141,7 +143,7 @@ __global__ void __launch_bounds__(kThreads) cache_rows_kernel(char *__restrict__
         const float step = DT::to_f32((uint16_t)(range & 0xffffu)), low = DT::to_f32((uint16_t)(range >> 16));
         float x[8];
 #pragma unroll
-        for (int c = 0; c < 8; ++c) x[c] = __builtin_fmaf((float)(w >> (4 * c) & 15u), step, low);      // the product is exact
+        for (int c = 0; c < 8; ++c) x[c] = __builtin_fminf(__builtin_fmaf((float)(w >> (4 * c) & 15u), step, low), kLargest<DT>);      // the product is exact
         reinterpret_cast<Chunk8 *>(out)[i] = pack8<DT>(x);
     }
 }

@@ -395,7 +395,9 @@ def cache_attend(q, k_cache, v_cache, lengths, win_size, sinks=0, scale=None):
 
 
 def cache_rows(cache):
-    """What the rows of a cache stand for, ``[N, kv_heads, capacity, C]``: a new tensor for :class:`Rows4`, a 16-bit cache itself."""
+    """What the rows of a cache stand for, ``[N, kv_heads, capacity, C]``: a new tensor for :class:`Rows4`, a 16-bit cache itself.
+
+    Where a step was rounded up its last code may stand for more than the type's largest number: that number then."""
     nodes = _lib.nodes() if isinstance(cache, Rows4) else None
     out = None if nodes is None else nodes.sink_rows(*cache)
     if out is not None:

@@ -85,3 +85,22 @@ def test_small_shares_in_4_bits(size, dtype):
     got, value, bound = _over_four(q, k.to(dtype).cuda(), v.to(dtype).cuda(), T - 1, 1, dtype, 1.0 / C)
     assert float(value.abs().max()) > 0.05 * size
     _near(got, value, bound)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=NAMES)
+def test_rows_in_4_bits_to_the_ends_of_their_type(dtype):
+    """What a finite row stands for is finite: its last code is not beyond the type's largest number where the step was rounded up."""
+    largest, C, T = torch.finfo(dtype).max, 32, 64
+    x = torch.zeros(1, T, 1, C)
+    falls = (1 - torch.arange(T) / (4 * T)).view(1, T, 1, 1)
+    x[..., 1::2] = largest if dtype == torch.bfloat16 else largest * falls
+    # (bf16: a range that fp32 holds, 255.95 times 2^120 and less, a fifteenth of which is rounded from 17.06 to 17.125)
+    x[..., ::2] = -largest / 255 * (0.7 + falls / 4) if dtype == torch.bfloat16 else -largest * falls
+    x = x.to(dtype).cuda()
+    cache = streaming.new_cache(1, 1, T, C, 4, dtype)
+    streaming.cache_append(x, x, *cache)
+    value = O.in_4_bits(x)[3]
+    assert bool((value.to(dtype).double().abs() > largest).any())      # of these rows some would be
+    for c in cache:
+        got = streaming.cache_rows(c).transpose(1, 2)
+        assert torch.equal(got, value.clamp(-largest, largest).to(dtype))
