@@ -162,7 +162,7 @@ template <int C, int QT> struct Sums {
         }
     }
     // `high`: a row's largest score of the unit at hand.  The reference of its exponentials moves only when that has outgrown it by more than
-    // kSlack (probabilities stay below 2^kSlack, which every format here holds).
+    // kSlack (probabilities stay below 2^kSlack, which every format here holds, also 2^kLift times that).
     __device__ inline float move(int h, float high) {
         constexpr float kSlack = 6.f;
         float alpha = 1.f;
@@ -421,7 +421,7 @@ cache_attend_kernel(char *__restrict__ out, float *__restrict__ partial, const c
 #pragma unroll
                 for (int r = 0; r < 4; ++r) high = __builtin_fmaxf(high, s[h][kt][r]);
             sums.move(h, xor_max(high) * scale2);
-            const float ref = -sums.m[h];
+            const float ref = kLift<DT> - sums.m[h];
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt) {
                 float e[4];

@@ -285,6 +285,10 @@ __device__ inline f32x4 dot_rows_mma(const RowOperand<C> &a, const RowOperand<C>
     return acc;
 }
 
+// A probability that is rounded to fp16 beside one of 1 loses digits below 2^-14 and is 0 below 2^-25: a few first tokens that take nearly all of a row leave the
+// others there.  The attention of streams rounds 2^kLift times a probability: with a reference that lags by 2^6 that is 2^15 at most.
+template <class DT> constexpr float kLift = DT::tag == NA1D_FP16 ? 9.f : 0.f;
+
 // Two 16-bit values of a register as floats.
 template <class DT> __device__ inline f32x2 unpack2(uint32_t w);
 template <> __device__ inline f32x2 unpack2<BF16>(uint32_t w) {

@@ -273,8 +273,8 @@ sink_fwd_kernel(char *__restrict__ out, float *__restrict__ lse, char *__restric
                 for (int r = 0; r < 4; ++r) mc = __builtin_fmaxf(mc, s[h][kt][r]);
             mc = xor_max(mc) * scale2;
             // The reference point of the exponentials moves only when a row's maximum has outgrown it by more than
-            // kSlack (probabilities then stay below 2^kSlack, which every format here holds): most chunks leave
-            // the accumulators as they are.
+            // kSlack (probabilities then stay below 2^kSlack, which every format here holds, also 2^kLift times that): most
+            // chunks leave the accumulators as they are.
             if (__builtin_amdgcn_ballot_w64(mc > m[h] + kSlack)) {
                 const float m_new = max2(m[h], mc);
                 const float alpha = __builtin_amdgcn_exp2f(m[h] - m_new);
@@ -283,7 +283,7 @@ sink_fwd_kernel(char *__restrict__ out, float *__restrict__ lse, char *__restric
 #pragma unroll
                 for (int ct = 0; ct < CT; ++ct) o[h][ct] *= alpha;
             }
-            const float ref = -m[h];
+            const float ref = kLift<DT> - m[h];
 #pragma unroll
             for (int kt = 0; kt < kKeyTiles; ++kt) {
                 float p[4];
@@ -329,7 +329,7 @@ sink_fwd_kernel(char *__restrict__ out, float *__restrict__ lse, char *__restric
             store_rest<C>(rest + (((int64_t)it.sample * a.H + head) * ((T + 15) / 16) + (w0 / 16 + h)) * kRestBytes<C>, rw, lane);
         store_tile<C>(os, at_row * a.o.pitch, ow, g, stores_whole_lines(a.o.pitch, C, 0), width);   // rows past T are dropped
         // log2 of the row's sum of exponentials; 0 for a row that does not exist, whose q and dO the backward reads as zeros
-        if (g == 0) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(valid ? m[h] + __builtin_amdgcn_logf(l) : 0.f), ls, at_row * 4, 0, 0);
+        if (g == 0) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(valid ? (m[h] - kLift<DT>) + __builtin_amdgcn_logf(l) : 0.f), ls, at_row * 4, 0, 0);
     }
 }
 

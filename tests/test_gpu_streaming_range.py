@@ -1,7 +1,7 @@
 """Attention of streams where numbers are large or small for their 16-bit type, against its formulas in 64 bits.
 
 `u` is half a step of the type.  fp16 rounds below 2^-14 to multiples of 2^-24, half of one off; the kernels lift what they round: a product with a step of 4 bits so that the
-largest step is 2^7 at least, so that it is off by 2^-32 of that step."""
+largest step is 2^7 at least, so that it is off by 2^-32 of that step; a probability by 2^9, so that it is off by 2^-34 beside one of 1."""
 import pytest
 import torch
 
@@ -104,3 +104,47 @@ def test_rows_in_4_bits_to_the_ends_of_their_type(dtype):
     for c in cache:
         got = streaming.cache_rows(c).transpose(1, 2)
         assert torch.equal(got, value.clamp(-largest, largest).to(dtype))
+
+
+# ------------------------------------------------------------------------------------------------ small shares
+def _sink_and_equals(N, T, H, K, C, dtype, share, rows):
+    """A first token without a value that takes nearly all of every row, and others whose keys are alike, each with a probability of 2^share beside it."""
+    q, k = torch.ones(N, T, H, C), torch.zeros(N, T, K, C)
+    k[:, 0] = -share * 0.6931
+    v = 1 + 0.1 * torch.randn(N, T, K, C, generator=torch.Generator().manual_seed(C))
+    v[:, 0] = 0.0
+    return [x.to(dtype).cuda() for x in (q[:, rows:], k, v)]
+
+
+def _least(dtype, T, v):
+    """Half a step of a result that is small for fp16, and 2^-34 of the largest value for every key (a probability of 1 being the largest at least)."""
+    return 2.0 ** -25 + T * 2.0 ** -34 * float(v.abs().max()) if dtype == torch.float16 else 0.0
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=NAMES)
+@pytest.mark.parametrize("H,K,C,T,W", [(2, 1, 16, 700, 300), (2, 2, 32, 1500, 1500), (4, 1, 64, 2048, 2000), (3, 3, 96, 900, 900), (2, 1, 128, 1100, 700), (64, 8, 64, 2100, 2100)])
+def test_small_shares(H, K, C, T, W, dtype):
+    """Each probability is rounded by itself (half a step of it), as is their sum's share of it and the result: whatever their size beside the largest."""
+    q, k, v = _sink_and_equals(1, T, H, K, C, dtype, -20.4, 0)
+    assert torch.equal(q, torch.ones_like(q))
+    u, f = O.half_step(dtype), O.FP32 * (1 + 20.4 * 0.6931)
+    got = streaming.sink_attention(q, k, v, W, 1, scale=1.0 / C)
+    value = O.attention(q[:, :, :1], k[:, :, :1], v[:, :, :1], W, 1, scale=1.0 / C)["out"][0]
+    for h in range(K):                                                 # (heads differ in their values alone)
+        if h:
+            value = O.attention(q[:, :, :1], k[:, :, :1], v[:, :, h:h + 1], W, 1, scale=1.0 / C)["out"][0]
+        for i in range(h * (H // K), (h + 1) * (H // K)):
+            _near(got[:, :, i:i + 1], value, (3 * u + f) * value.abs() + _least(dtype, W, v))
+    assert float(value.max()) > W * 2.0 ** -20.6 * 0.5
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=NAMES)
+@pytest.mark.parametrize("N,H,K,C,T,n", [(1, 4, 4, 64, 1028, 1), (2, 4, 2, 16, 1500, 1), (3, 8, 2, 128, 3000, 2), (2, 6, 2, 96, 900, 1), (40, 16, 16, 32, 1000, 1), (1, 64, 1, 32, 2000, 3)])
+def test_small_shares_over_a_cache(N, H, K, C, T, n, dtype):
+    q, k, v = _sink_and_equals(N, T, H, K, C, dtype, -20.4, T - n)
+    cache = streaming.new_cache(N, K, T, C, 16, dtype)
+    streaming.cache_append(k, v, *cache, sinks=1)
+    got = streaming.cache_attend(q, *cache, torch.full((N,), T, dtype=torch.int32, device="cuda"), T - n, 1, scale=1.0 / C)
+    value, _ = O.over_history(q, k, v, T - n, 1, [T] * N, scale=1.0 / C)
+    u, f = O.half_step(dtype), O.FP32 * (1 + 20.4 * 0.6931)
+    _near(got, value, (2 * u + f) * value.abs() + _least(dtype, T, v))
