@@ -447,8 +447,8 @@ int na1d_head_backward(const na1d_head *h, void *dx, void *dw, const float *dlos
  *   saved   : what a forward leaves for its backward, na1d_sink_saved_bytes() bytes: 4 to a head's row and a byte to a value of out
  *             (what its rounding lost; head_dim counted as the next of 16, 32, 64, 96, 128); NULL for inference
  * Scores, softmax and sums are in fp32; probabilities are rounded to 16 bits where they are multiplied by v; in the backward they and their
- * gradients are multiplied as two such numbers. Nothing uses atomics: results are the same from call to call.
- * A backward's workspace is 4 bytes to a head's row, and fp32 sums where several workgroups share the rows of a key head (those that are
+ * gradients are multiplied as two such numbers.  What is rounded to fp16 is scaled into its range first.  Nothing uses atomics: results are the same from call to call.
+ * A backward's workspace is 4 bytes to a head's row, in fp16 16 more to every 64 of them, and fp32 sums where several workgroups share the rows of a key head (those that are
  * sinks, and all of them if there are few).
  * head_dim % 8 == 0, up to 128 (NA1D_ERR_HEAD_DIM, NA1D_ERR_UNSUPPORTED); heads % kv_heads == 0, window >= 1, sinks >= 0
  * (NA1D_ERR_SHAPE, NA1D_ERR_WINDOW); all pointers but t_valid 16-byte aligned, strides multiples of 8, row strides at least

@@ -172,6 +172,22 @@ template <class DT> __device__ inline void pack_twice(float x, float y, uint32_t
     rest = Mma<DT>::pack(x - there.x, y - there.y);
 }
 
+// fp16 holds 2^-24 to 65504, and a backward's P and dS may be anywhere: small beside one key that takes nearly all of a row or with a small dO, beyond it with a large one.  Both count
+// 2^kBackLift times where they are rounded (of small ones 2^-35 is lost at most, which their sums of products do not see beside a result's own 2^-25), and dS less than that where it
+// would pass 2^15: dQ's kernel takes a row down, with what it has summed up, when it meets such a value, and leaves the largest of every tile of rows for dK's and dV's, which take P and
+// dS down by the largest that they will meet (a P is then off by 2^-40 of that).  As norms, 4096 tokens of 64 channels, dO of 2^-12 and 2^-16: dQ 7.8e-4 and 7.5e-3 -> 2.5e-4 and
+// 1.0e-3, where the results' rounding alone is 2.1e-4 and 1.0e-3.  (16 x 16 x 1000 rows of 64 channels, fp16, dQ: 49 -> 50.5 us, dK and dV 61 -> 63; these took 64 to 66 looking for
+// large values themselves, or taking down on the way what they had summed up.)
+template <int CTRL> __device__ inline float max_with(float x) {
+    return __builtin_fmaxf(x, __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), CTRL, 0xf, 0xf, true)));
+}
+// Over all lanes: pairs, fours, halves of 16 lanes in reverse, 16 in reverse, then the four groups.
+__device__ inline float wave_max(float x) { return xor_max(max_with<0x140>(max_with<0x141>(max_with<0x4e>(max_with<0xb1>(x))))); }
+template <class DT> constexpr bool kNarrow = DT::tag == NA1D_FP16;
+template <class DT> constexpr int kBackLift = kNarrow<DT> ? 10 : 0;
+constexpr float kTooLarge = 32768.f;        // and what is, is taken down to between 2^14 and 2^15
+__device__ inline int too_much(float high) { return high > kTooLarge ? __builtin_amdgcn_frexp_expf(high) - 15 : 0; }
+
 // =============================================================================
 // Forward
 // =============================================================================
@@ -341,7 +357,7 @@ sink_fwd_kernel(char *__restrict__ out, float *__restrict__ lse, char *__restric
 // 57 and not 48, 5 x 10 x 777, 96 channels, window 100, 24 and not 17.5 (these two before dS went into the product twice).
 template <class DT, int C>
 __global__ void __launch_bounds__(kThreads)
-sink_dq_kernel(char *__restrict__ dq, float *__restrict__ delta, const char *__restrict__ q, const char *__restrict__ k, const char *__restrict__ v,
+sink_dq_kernel(char *__restrict__ dq, float *__restrict__ delta, float *__restrict__ largest, const char *__restrict__ q, const char *__restrict__ k, const char *__restrict__ v,
                const char *__restrict__ out, const char *__restrict__ dout, const float *__restrict__ lse, const char *__restrict__ rest, const int32_t *__restrict__ t_valid,
                uint32_t items, SinkArgs a) {
     constexpr int CT = C / 16, CS = kStaged<C>, kStep = region_bytes<CS>(kKeyTiles);
@@ -394,6 +410,9 @@ sink_dq_kernel(char *__restrict__ dq, float *__restrict__ delta, const char *__r
     for (int ct = 0; ct < CT; ++ct) acc[ct] = f32x4{0.f, 0.f, 0.f, 0.f};
     const KeySight sees(w0, w1, tv, a);
     settle_rows<C>(qop), settle_rows<C>(gop), settle(ref);
+    ref += kBackLift<DT>;
+    int less = 0;                                         // what this row's dS has been taken down by: 2^less
+    float most = 0.f;                                     // the largest of this lane's
     int at = 0;
     while (c < chunks.end) {
         wait_direct();
@@ -408,7 +427,7 @@ sink_dq_kernel(char *__restrict__ dq, float *__restrict__ delta, const char *__r
         if (see == kNothing) continue;
 #pragma unroll
         for (int kt = 0; kt < kKeyTiles; kt += 2) {
-            u32x4 db, rb;
+            float dsv[8];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 RowOperand<C> kop, vop;
@@ -425,11 +444,28 @@ sink_dq_kernel(char *__restrict__ dq, float *__restrict__ delta, const char *__r
                     for (int r = 0; r < 4; ++r)
                         if (!((uint32_t)(d - r) < (uint32_t)a.window || r < stay)) p[r] = 0.f;
                 }
-                uint32_t w[2], r_[2];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) pack_twice<DT>(p[2 * i] * dp[2 * i], p[2 * i + 1] * dp[2 * i + 1], w[i], r_[i]);
-                db[2 * j] = w[0], db[2 * j + 1] = w[1];
-                rb[2 * j] = r_[0], rb[2 * j + 1] = r_[1];
+                for (int r = 0; r < 4; ++r) dsv[4 * j + r] = p[r] * dp[r];
+            }
+            if constexpr (kNarrow<DT>) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) most = __builtin_fmaxf(most, __builtin_fabsf(dsv[i]));
+                if (__builtin_amdgcn_ballot_w64(most > kTooLarge)) {
+                    const int more = too_much(xor_max(most));       // of the four lanes that share the row
+                    const float by = __builtin_amdgcn_ldexpf(1.f, -more);
+                    less += more, ref -= (float)more, most *= by;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) dsv[i] *= by;
+#pragma unroll
+                    for (int ct = 0; ct < CT; ++ct) acc[ct] *= by;
+                }
+            }
+            u32x4 db, rb;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint32_t w, r;
+                pack_twice<DT>(dsv[2 * i], dsv[2 * i + 1], w, r);
+                db[i] = w, rb[i] = r;
             }
             LDS_PTR(char) blk = k_lds + kt * LL::kTileBytes;
 #pragma unroll
@@ -442,10 +478,15 @@ sink_dq_kernel(char *__restrict__ dq, float *__restrict__ delta, const char *__r
         }
     }
     const Rsrc dqs = rows_of(dq + o_off, row0, row_end - row0, a.o.pitch);
+    if constexpr (kNarrow<DT>) {
+        most = wave_max(__builtin_amdgcn_ldexpf(most, less - kBackLift<DT>));
+        if (lane == 0) largest[(((int64_t)it.sample * a.H + head) * a.strips + it.strip) * kWaves + wave] = most;
+    }
+    const float back = __builtin_amdgcn_ldexpf(a.scale, less - kBackLift<DT>);
     u32x2 qw[CT];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-        qw[ct] = pack_acc<DT>(acc[ct], a.scale);
+        qw[ct] = pack_acc<DT>(acc[ct], back);
         if (w0 + n >= tv) qw[ct] = u32x2{0u, 0u};
     }
     store_tile<C>(dqs, (own + n) * a.o.pitch, qw, g, stores_whole_lines(a.o.pitch, C, 0), width);
@@ -474,7 +515,7 @@ template <int C> __device__ inline Partial partial_of(int64_t strip_id, int part
 template <class DT, int C>
 __global__ void __launch_bounds__(kThreads)
 sink_dkv_kernel(char *__restrict__ dk, char *__restrict__ dv, float *__restrict__ partial, const char *__restrict__ q, const char *__restrict__ k,
-                const char *__restrict__ v, const char *__restrict__ dout, const float *__restrict__ lse, const float *__restrict__ delta,
+                const char *__restrict__ v, const char *__restrict__ dout, const float *__restrict__ lse, const float *__restrict__ delta, const float *__restrict__ largest,
                 const int32_t *__restrict__ t_valid, uint32_t rest, uint32_t heads, SinkArgs a) {
     constexpr int CT = C / 16, CS = kStaged<C>, kStep = region_bytes<CS>(kChunkTiles), kBuf = 2 * kStep + 2 * kChunkRows * 4;
     using LL = Lds<CS>;
@@ -554,13 +595,26 @@ sink_dkv_kernel(char *__restrict__ dk, char *__restrict__ dv, float *__restrict_
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) acck[ct] = accv[ct] = f32x4{0.f, 0.f, 0.f, 0.f};
 
+    // P and dS are taken down by 2^less, by the largest dS of all units: a lane has every 64th of them
+    int less = 0;
+    auto largest_of = [&](int i) {
+        const int h = i / nc;
+        const f32x4 x = *reinterpret_cast<const f32x4 *>(largest + (((int64_t)sample * a.H + kv * a.group + h) * a.strips + c_from + i - h * nc) * kWaves);
+        return __builtin_fmaxf(__builtin_fmaxf(x[0], x[1]), __builtin_fmaxf(x[2], x[3]));
+    };
+    float high = 0.f;
+    if (kNarrow<DT> && u + lane < u_end) high = largest_of(u + lane);
     settle_rows<C>(kop), settle_rows<C>(vop);
+    if constexpr (kNarrow<DT>) {
+        for (int i = u + lane + 64; i < u_end; i += 64) high = __builtin_fmaxf(high, largest_of(i));
+        less = uniform(too_much(__builtin_amdgcn_ldexpf(wave_max(high), kBackLift<DT>)));
+    }
     int at = 0;
     for (; u < u_end; ++u) {
         wait_direct();
         {
             // rows past tv: q and dO are zeros there, and so are these
-            const float constant = g == 0 ? -row_lse : -row_delta;
+            const float constant = g == 0 ? (float)(kBackLift<DT> - less) - row_lse : -row_delta;
             if (g < 2) *reinterpret_cast<LDS_PTR(float)>(buf_lds + at + 2 * kStep + (g * kChunkRows + 16 * wave + n) * 4) = constant;
         }
         barrier_lds();
@@ -576,6 +630,7 @@ sink_dkv_kernel(char *__restrict__ dk, char *__restrict__ dv, float *__restrict_
 #pragma unroll
         for (int qi = 0; qi < kChunkTiles; qi += 2) {
             u32x4 pb, db, pr, dr;
+            float dsv[8];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 RowOperand<C> qop, gop;
@@ -594,14 +649,20 @@ sink_dkv_kernel(char *__restrict__ dk, char *__restrict__ dv, float *__restrict_
                     for (int r = 0; r < 4; ++r)
                         if (!((uint32_t)(d + r) < reach)) p[r] = 0.f;
                 }
-                uint32_t w[4], r_[4];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    pack_twice<DT>(p[2 * i], p[2 * i + 1], w[i], r_[i]);
-                    pack_twice<DT>(p[2 * i] * dp[2 * i], p[2 * i + 1] * dp[2 * i + 1], w[2 + i], r_[2 + i]);
+                    uint32_t w, r;
+                    pack_twice<DT>(p[2 * i], p[2 * i + 1], w, r);
+                    pb[2 * j + i] = w, pr[2 * j + i] = r;
                 }
-                pb[2 * j] = w[0], pb[2 * j + 1] = w[1], pr[2 * j] = r_[0], pr[2 * j + 1] = r_[1];
-                db[2 * j] = w[2], db[2 * j + 1] = w[3], dr[2 * j] = r_[2], dr[2 * j + 1] = r_[3];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) dsv[4 * j + r] = p[r] * dp[r];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint32_t w, r;
+                pack_twice<DT>(dsv[2 * i], dsv[2 * i + 1], w, r);
+                db[i] = w, dr[i] = r;
             }
             LDS_PTR(char) qtile = q_lds + qi * LL::kTileBytes;
             LDS_PTR(char) gtile = g_lds + qi * LL::kTileBytes;
@@ -617,6 +678,7 @@ sink_dkv_kernel(char *__restrict__ dk, char *__restrict__ dv, float *__restrict_
             }
         }
     }
+    const float back = __builtin_amdgcn_ldexpf(1.f, less - kBackLift<DT>);
     const bool shared = !far && strip_id >= (uint32_t)a.whole, sinking = a.far && w0 < a.sinks;
     if (shared || far || sinking) {
         if (far && !sinking) return;
@@ -625,8 +687,8 @@ sink_dkv_kernel(char *__restrict__ dk, char *__restrict__ dv, float *__restrict_
         float *to = partial + (shared ? at_.shared : far ? at_.far : at_.near) + (own + n) * C + 4 * g;
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
-            *reinterpret_cast<f32x4 *>(to + 16 * ct) = acck[ct];
-            *reinterpret_cast<f32x4 *>(to + rows * C + 16 * ct) = accv[ct];
+            *reinterpret_cast<f32x4 *>(to + 16 * ct) = acck[ct] * back;
+            *reinterpret_cast<f32x4 *>(to + rows * C + 16 * ct) = accv[ct] * back;
         }
         return;
     }
@@ -636,8 +698,8 @@ sink_dkv_kernel(char *__restrict__ dk, char *__restrict__ dv, float *__restrict_
     u32x2 kw[CT], vw[CT];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-        kw[ct] = pack_acc<DT>(acck[ct], a.scale);
-        vw[ct] = pack_acc<DT>(accv[ct], 1.f);
+        kw[ct] = pack_acc<DT>(acck[ct], a.scale * back);
+        vw[ct] = pack_acc<DT>(accv[ct], back);
         if (key >= tv) kw[ct] = vw[ct] = u32x2{0u, 0u};
     }
     store_tile<C>(dks, (own + n) * a.dkv.pitch, kw, g, stream, width);      // rows past T are dropped
@@ -735,6 +797,7 @@ KeyPlan key_plan(const na1d_sink &h) {
     return p;
 }
 int64_t lse_floats(const na1d_sink &h) { return (h.N * h.heads * h.T + 3) / 4 * 4; }
+int64_t largest_floats(const na1d_sink &h) { return h.dtype == NA1D_FP16 ? h.N * h.heads * ((h.T + kChunkRows - 1) / kChunkRows) * kWaves : 0; }
 bool countable(int64_t items) { return items <= 0x7fffff00LL; }
 
 template <class DT, int C>
@@ -761,14 +824,14 @@ int launch_sink_bwd(const na1d_sink &h, void *dq, void *dk, void *dv, const void
     const KeyPlan p = key_plan(h);
     const int64_t items = h.N * h.heads * a.strips, key_items = p.a.whole + p.rest, join_items = p.joined * ((kChunkRows * (C / 4) + kThreads - 1) / kThreads);
     if (!countable(items) || !countable(p.heads * p.a.strips) || !countable(key_items) || !countable(join_items)) return NA1D_ERR_UNSUPPORTED;
-    float *const delta = ws, *const partial = ws + lse_floats(h);
+    float *const delta = ws, *const largest = ws + lse_floats(h), *const partial = largest + largest_floats(h);
     constexpr size_t dq_lds = 4 * (size_t)region_bytes<kStaged<C>>(kKeyTiles), dkv_lds = 2 * (2 * (size_t)region_bytes<kStaged<C>>(kChunkTiles) + 2 * kChunkRows * sizeof(float));
     if (!allow_lds(sink_dq_kernel<DT, C>, dq_lds) || !allow_lds(sink_dkv_kernel<DT, C>, dkv_lds)) return NA1D_ERR_LAUNCH;
     note_kernel_as("sink_dq_kernel + sink_dkv_kernel<%s, %d>", DT::tag == NA1D_BF16 ? "BF16" : "FP16", C);
-    launch_kernel_span(1, sink_dq_kernel<DT, C>, (unsigned)items, (unsigned)kThreads, dq_lds, s, (char *)dq, delta, (const char *)q, (const char *)k, (const char *)v, (const char *)out,
+    launch_kernel_span(1, sink_dq_kernel<DT, C>, (unsigned)items, (unsigned)kThreads, dq_lds, s, (char *)dq, delta, largest, (const char *)q, (const char *)k, (const char *)v, (const char *)out,
                        (const char *)dout, saved, (const char *)(saved + lse_floats(h)), t_valid, (uint32_t)items, a);
     launch_kernel_span(p.joined ? 0 : 2, sink_dkv_kernel<DT, C>, (unsigned)key_items, (unsigned)kThreads, dkv_lds, s, (char *)dk, (char *)dv, partial, (const char *)q,
-                       (const char *)k, (const char *)v, (const char *)dout, saved, (const float *)delta, t_valid, (uint32_t)p.rest, (uint32_t)p.heads, p.a);
+                       (const char *)k, (const char *)v, (const char *)dout, saved, (const float *)delta, (const float *)largest, t_valid, (uint32_t)p.rest, (uint32_t)p.heads, p.a);
     if (p.joined)
         launch_kernel_span(2, sink_join_kernel<DT, C>, (unsigned)join_items, (unsigned)kThreads, 0, s, (char *)dk, (char *)dv, (const float *)partial, t_valid,
                            (uint32_t)p.heads, p.a);
@@ -795,7 +858,7 @@ int64_t sink_saved_bytes(const na1d_sink &h) {
     return 4 * lse_floats(h) + h.N * h.heads * ((h.T + 15) / 16) * 16 * channels_of(h.head_dim);
 }
 int64_t sink_bwd_workspace_bytes(const na1d_sink &h) {
-    return 4 * (lse_floats(h) + key_plan(h).floats);
+    return 4 * (lse_floats(h) + largest_floats(h) + key_plan(h).floats);
 }
 
 int sink_fwd(const na1d_sink &h, void *out, float *saved, const void *q, const void *k, const void *v, const int32_t *t_valid, hipStream_t s) {

@@ -1,7 +1,7 @@
 """Attention of streams where numbers are large or small for their 16-bit type, against its formulas in 64 bits.
 
 `u` is half a step of the type.  fp16 rounds below 2^-14 to multiples of 2^-24, half of one off; the kernels lift what they round: a product with a step of 4 bits so that the
-largest step is 2^7 at least, so that it is off by 2^-32 of that step; a probability by 2^9, so that it is off by 2^-34 beside one of 1."""
+largest step is 2^7 at least, so that it is off by 2^-32 of that step; a probability by 2^9, so that it is off by 2^-34 beside one of 1; P and dS of a backward by 2^10 unless dS is large."""
 import pytest
 import torch
 
@@ -148,3 +148,60 @@ def test_small_shares_over_a_cache(N, H, K, C, T, n, dtype):
     value, _ = O.over_history(q, k, v, T - n, 1, [T] * N, scale=1.0 / C)
     u, f = O.half_step(dtype), O.FP32 * (1 + 20.4 * 0.6931)
     _near(got, value, (2 * u + f) * value.abs() + _least(dtype, T, v))
+
+
+# ------------------------------------------------------------------------------------------------ gradients
+def _gradients(q, k, v, dout, *args, **kw):
+    q, k, v = (x.detach().requires_grad_(True) for x in (q, k, v))
+    return dict(zip(("dq", "dk", "dv"), torch.autograd.grad(streaming.sink_attention(q, k, v, *args, **kw), [q, k, v], dout)))
+
+
+def _norms_near(got, want, more, part=slice(None)):
+    """As norms: the rounding of the results themselves, as it comes out, and `more` of the whole."""
+    torch.cuda.synchronize()
+    for name, x in got.items():
+        x, value = x[:, part], want[name][0][:, part]
+        assert bool(x.isfinite().all()), name
+        size, off, own = (float(y.norm()) for y in (value, x.double() - value, value.to(x.dtype).double() - value))
+        assert off <= own + more * size, "%s: off by %.3g of it, its rounding %.3g and %.3g more allowed" % (name, off / size, own / size, more)
+
+
+@pytest.mark.parametrize("power", [-16, -12, -8, 0, 6])
+@pytest.mark.parametrize("H,K,C,T,W,Z", [(2, 1, 64, 4096, 4096, 0), (1, 1, 16, 4000, 4000, 3), (2, 2, 32, 3000, 2000, 100), (2, 1, 96, 2500, 2500, 1), (1, 1, 128, 4096, 3000, 4)])
+def test_fp16_gradients_for_any_size_of_what_comes_back(H, K, C, T, W, Z, power):
+    """Beside the results' rounding a delta has what the output's sum lost to roundings of probabilities: independent ones, half a step each at most, u / sqrt(3) of a term of its size;
+    all else (two numbers for P and dS each, fp32) is below a twentieth of u."""
+    g = torch.Generator().manual_seed(C)
+    q, k, v, dout = (torch.randn(1, T, h, C, generator=g) for h in (H, K, K, H))
+    q, k, v, dout = (x.to(torch.float16).cuda() for x in (q, 4 * k, v, 2.0 ** power * dout))
+    u = O.half_step(torch.float16)
+    _norms_near(_gradients(q, k, v, dout, W, Z), O.attention(q, k, v, W, Z, dout=dout), u * (3 ** -0.5 + 0.05))
+
+
+@pytest.mark.parametrize("N,H,K,C,T,W,Z", [(1, 2, 1, 64, 500, 400, 0), (2, 4, 4, 16, 300, 300, 2), (1, 2, 2, 32, 700, 100, 5), (2, 4, 2, 96, 260, 260, 1), (4, 16, 8, 128, 513, 129, 66)])
+def test_fp16_gradients_beyond_the_range_of_their_parts(N, H, K, C, T, W, Z):
+    """dS is beyond 65504 in places where scale * dS * k is not."""
+    g = torch.Generator().manual_seed(C)
+    q, k, v, dout = (torch.randn(N, T, h, C, generator=g) for h in (H, K, K, H))
+    q, k, v, dout = (x.to(torch.float16).cuda() for x in (2 * q, 0.5 * k, 8 * v, 4000 * dout))
+    scale = 1 / 64
+    want = O.attention(q, k, v, W, Z, scale=scale, dout=dout)
+    q_, k_, v_, g_ = (x[:, :64].double().transpose(1, 2).repeat_interleave(H // x.shape[2], 1) for x in (q, k, v, dout))
+    p = torch.softmax((q_ @ k_.transpose(-1, -2) * scale).masked_fill(~torch.ones(64, 64, dtype=torch.bool, device="cuda").tril(), -torch.inf), -1)
+    dp = g_ @ v_.transpose(-1, -2)
+    assert float((p * (dp - (p * dp).sum(-1, keepdim=True))).abs().max()) > 65504
+    assert all(float(want[n][0].abs().max()) < 60000 for n in ("dq", "dk", "dv"))
+    u = O.half_step(torch.float16)
+    _norms_near(_gradients(q, k, v, dout, W, Z, scale=scale), want, u * (3 ** -0.5 + 0.05))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=NAMES)
+@pytest.mark.parametrize("H,K,C,T,W", [(2, 1, 16, 700, 300), (2, 2, 32, 1500, 1500), (4, 1, 64, 2048, 2000), (2, 1, 128, 1100, 700)])
+def test_gradients_of_small_shares(H, K, C, T, W, dtype):
+    """The keys beside a first token that takes nearly all of every row: their P and dS are 2^-20 of it."""
+    q, k, v = _sink_and_equals(1, T, H, K, C, dtype, -20.4, 0)
+    k[:, 1:] = (0.05 * torch.randn(1, T - 1, K, C, generator=torch.Generator().manual_seed(1))).to(dtype)
+    dout = (1 + 0.1 * torch.randn(1, T, H, C, generator=torch.Generator().manual_seed(2))).to(dtype).cuda()
+    want = O.attention(q, k, v, W, 1, scale=1.0 / C, dout=dout)
+    got = _gradients(q, k, v, dout, W, 1, scale=1.0 / C)
+    _norms_near({n: got[n] for n in ("dk", "dv")}, want, O.half_step(dtype) * (3 ** -0.5 + 0.05), slice(1, None))
