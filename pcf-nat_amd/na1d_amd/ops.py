@@ -458,4 +458,5 @@ def sink_attention_op(q: Tensor, k: Tensor, v: Tensor, win_size: int, sinks: int
                       scale: Optional[float] = None) -> Tensor:
     """:func:`na1d_amd.streaming.sink_attention` through the registered op (traceable by ``torch.compile``)."""
     streaming.check_operands(q, k, v, t_valid)
+    streaming.check_tangents(q, k, v)                 # (torch's node for registered ops passes them by where nothing requires a gradient)
     return getattr(torch.ops, NAMESPACE).sink_attention_forward(q, k, v, t_valid, *streaming._window(win_size, sinks), streaming._scale(scale, q.shape[3]))[0]

@@ -4,7 +4,8 @@ tokens, the sinks, that stay visible for good.  Token t sees token u where ``u <
 :func:`sink_attention` is a layer over whole sequences, in training or over a prompt.  Where a stream goes on, its keys and values are in
 caches (:func:`new_cache`) that hold what can still be seen and never grow: :func:`cache_append` puts a prompt there,
 :func:`cache_step` takes the next token or a few, :func:`cache_attend` is a step whose tokens are in the caches already.  A cache has its
-rows in 16 bits or, as :class:`Rows4`, in 4.
+rows in 16 bits or, as :class:`Rows4`, in 4.  None of them has forward-mode derivatives or goes through ``torch.func``'s transforms, and calls over caches
+are not traced by ``torch.jit.trace``: they raise.
 
 Position p of a stream is in row p of its cache where ``p < sinks``, else in row ``sinks + (p - sinks) % (capacity - sinks)``.  ``lengths`` (int32
 ``[N]``, on the GPU) says how many tokens the streams have seen; one whose entry is negative (or above 2^30) is idle: its rows stay as they
@@ -19,6 +20,7 @@ import ctypes
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -175,11 +177,14 @@ def _final(grad):
 
 
 class _SinkAttention(torch.autograd.Function):
+    """Every call goes through it, one without gradients too: forward-mode derivatives and transforms are refused by it, and a tracer sees it."""
     @staticmethod
-    def forward(ctx, q, k, v, t_valid, win_size, sinks, scale):
-        out, saved = sink_forward(q, k, v, t_valid, win_size, sinks, scale, True)
-        ctx.save_for_backward(q, k, v, t_valid, out, saved)
-        ctx.args = (win_size, sinks, scale)
+    def forward(ctx, q, k, v, t_valid, win_size, sinks, scale, grad):
+        want = grad and any(ctx.needs_input_grad)
+        out, saved = sink_forward(q, k, v, t_valid, win_size, sinks, scale, want)
+        if want:
+            ctx.save_for_backward(q, k, v, t_valid, out, saved)
+            ctx.args = (win_size, sinks, scale)
         return out
 
     @staticmethod
@@ -187,7 +192,7 @@ class _SinkAttention(torch.autograd.Function):
         tensors = ctx.saved_tensors
         with torch.no_grad():
             grads = sink_backward(dout, *tensors, *ctx.args)
-        return tuple(_final(g) if want else None for g, want in zip(grads, ctx.needs_input_grad)) + (None,) * 4
+        return tuple(_final(g) if want else None for g, want in zip(grads, ctx.needs_input_grad)) + (None,) * 5
 
 
 def sink_attention(q, k, v, win_size, sinks=0, t_valid=None, scale=None):
@@ -206,9 +211,7 @@ def sink_attention(q, k, v, win_size, sinks=0, t_valid=None, scale=None):
     _check_gpu(q)
     win_size, sinks = _window(win_size, sinks)
     scale = _scale(scale, q.shape[3])
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _SinkAttention.apply(q, k, v, t_valid, win_size, sinks, scale)
-    return sink_forward(q, k, v, t_valid, win_size, sinks, scale, False)[0]
+    return _SinkAttention.apply(q, k, v, t_valid, win_size, sinks, scale, torch.is_grad_enabled() or torch.jit.is_tracing())
 
 
 # ------------------------------------------------------------------------------------------------ caches
@@ -222,6 +225,20 @@ def new_cache(batch, kv_heads, capacity, head_dim, bits=16, dtype=torch.bfloat16
         raise _lib.NA1DError("bits must be 16, or 4 with a head_dim of 32, 64, 96 or 128; got %r and %r" % (bits, head_dim))
     return tuple(Rows4(torch.zeros(batch, kv_heads, capacity, head_dim // 2, dtype=torch.uint8, device=device),
                        torch.zeros(batch, kv_heads, capacity, 2, dtype=dtype, device=device)) for _ in "kv")
+
+
+def _check_untraced():
+    if torch.jit.is_tracing():
+        raise _lib.NA1DError("calls over a cache cannot be traced: a trace would not hold what they write to it and read from it")
+
+
+def _has_tangent(t):
+    return forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None
+
+
+def check_tangents(*tensors):
+    if any(_has_tangent(t) for t in tensors):
+        raise _lib.NA1DError("sink_attention has no forward-mode derivative")
 
 
 def _check_cache(cache, what):
@@ -244,7 +261,7 @@ def _check_cache(cache, what):
     for t in cache if isinstance(cache, Rows4) else (cache,):
         if not t.is_contiguous() or (t.numel() and not t.is_meta and t.data_ptr() % 16):
             raise _lib.NA1DError("%s must be contiguous and 16-byte aligned" % what)
-        if t.requires_grad:
+        if t.requires_grad or _has_tangent(t):
             raise _lib.NA1DError("%s is written to without a gradient: it must not require one" % what)
     return tuple(shape), dtype
 
@@ -315,6 +332,7 @@ def cache_append(k, v, k_cache, v_cache, lengths=None, sinks=0, t_valid=None):
     nodes = _nodes(1, sinks)
     if nodes is not None and nodes.sink_append(k, v, *_parts(k_cache, v_cache), lengths, sinks, t_valid):
         return
+    _check_untraced()
     _, sinks = _window(1, sinks)
     shape, dtype = _check_caches(k_cache, v_cache, sinks)
     device = _device(k_cache)
@@ -340,6 +358,7 @@ def _over_cache(q, k, v, k_cache, v_cache, lengths, win_size, sinks, scale):
     out = None if nodes is None else nodes.sink_over(q, k, v, *_parts(k_cache, v_cache), lengths, win_size, sinks, scale)
     if out is not None:
         return out
+    _check_untraced()
     win_size, sinks = _window(win_size, sinks)
     shape, dtype = _check_caches(k_cache, v_cache, sinks)
     device = _device(k_cache)
@@ -354,7 +373,7 @@ def _over_cache(q, k, v, k_cache, v_cache, lengths, win_size, sinks, scale):
         raise ValueError("lengths must be int32 [%d]" % shape[0])
     check_lengths(lengths, q, "lengths")
     _check_room(shape, win_size, sinks, q.shape[1])
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v)):
+    if any(t is not None and (torch.is_grad_enabled() and t.requires_grad or _has_tangent(t)) for t in (q, k, v)):
         raise _lib.NA1DError("attention over a cache has no gradient: call it under torch.no_grad(), or sink_attention")
     _check_gpu(q)
     scale = _scale(scale, shape[3])
@@ -402,6 +421,8 @@ def cache_rows(cache):
     out = None if nodes is None else nodes.sink_rows(*cache)
     if out is not None:
         return out
+    if isinstance(cache, Rows4):
+        _check_untraced()
     shape, dtype = _check_cache(cache, "cache")
     if not isinstance(cache, Rows4):
         return cache
