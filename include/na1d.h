@@ -452,7 +452,8 @@ int na1d_head_backward(const na1d_head *h, void *dx, void *dw, const float *dlos
  * sinks, and all of them if there are few).
  * head_dim % 8 == 0, up to 128 (NA1D_ERR_HEAD_DIM, NA1D_ERR_UNSUPPORTED); heads % kv_heads == 0, window >= 1, sinks >= 0
  * (NA1D_ERR_SHAPE, NA1D_ERR_WINDOW); all pointers but t_valid 16-byte aligned, strides multiples of 8, row strides at least
- * head_dim.  Limits (NA1D_ERR_UNSUPPORTED): T up to 2^24, row strides to 2^20, heads * head_dim too, N * T * heads to 2^36.
+ * head_dim.  Limits (NA1D_ERR_UNSUPPORTED): T up to 2^24, row strides to 2^20, heads * head_dim too, N * T * heads to 2^36; what a launch holds:
+ * N * heads * ceil(T / 64) below 2^24.
  */
 typedef struct na1d_sink {
     int32_t dtype, heads, kv_heads, head_dim;
@@ -482,8 +483,8 @@ int na1d_sink_backward(const na1d_sink *h, void *dq, void *dk, void *dv, const v
  *   in na1d_sink_forward), the first of them at lengths[n] - fresh (a token before position 0 has output 0).  They are in the cache already.
  * step: the same for tokens that are not: k, v [N, fresh, kv_heads, head_dim] become positions lengths[n] .. lengths[n] + fresh - 1 and are
  *   attended to as the cache holds them.
- * Strides as in na1d_sink.  What a call writes to shares no memory with the rest.  capacity - sinks >= window + fresh - 1 (NA1D_ERR_WINDOW).  capacity * head_dim up to 2^29, N * kv_heads to 2^24,
- * fresh * heads / kv_heads to 2^20, heads to 2^24 (NA1D_ERR_UNSUPPORTED).  All pointers but lengths and t_valid 16-byte aligned.  A workspace is needed where
+ * Strides as in na1d_sink.  What a call writes to shares no memory with the rest.  capacity - sinks >= window + fresh - 1 (NA1D_ERR_WINDOW).  capacity * head_dim up to 2^29,
+ * fresh * heads / kv_heads to 2^20, heads to 2^24, N * kv_heads * ceil(fresh * heads / kv_heads / 64) below 2^24 (NA1D_ERR_UNSUPPORTED).  All pointers but lengths and t_valid 16-byte aligned.  A workspace is needed where
  * na1d_sink_attend_workspace_bytes() is above 0.  rows: what `rows` rows of codes stand for, in `dtype` (its largest number where the last code of a step that was rounded up
  * stands for more).
  */

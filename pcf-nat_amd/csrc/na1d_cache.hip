@@ -782,7 +782,7 @@ int64_t cache_attend_workspace_bytes(const na1d_sink_cache &c, int64_t fresh, in
 int cache_attend(const na1d_sink_cache &c, void *out, const void *q, const void *k, const void *v, const int64_t *q_strides, const int64_t *k_strides, const int64_t *v_strides,
                  const int32_t *lengths, int64_t fresh, int heads, int64_t window, float scale, float *ws, hipStream_t s) {
     CachePlan p = cache_plan(c, fresh, heads, window);
-    if (p.items > 0x7fffff00LL) return NA1D_ERR_UNSUPPORTED;
+    if (!launchable(p.items, 64 * p.waves)) return NA1D_ERR_UNSUPPORTED;
     p.a.scale = scale, p.a.q = rows_by(q_strides);
     if (k) p.a.k = rows_by(k_strides), p.a.v = rows_by(v_strides), p.a.stored = p.a.fresh;
     return c.dtype == NA1D_BF16 ? launch_width<BF16>(c, p, out, q, k, v, lengths, ws, s) : launch_width<FP16>(c, p, out, q, k, v, lengths, ws, s);
@@ -794,7 +794,7 @@ int cache_append(const na1d_sink_cache &c, const void *k, const void *v, const i
     // workgroups fill the card eight times, where there are so many tokens
     const int64_t heads = c.N * c.kv_heads, tokens = std::min(T, c.capacity), slots = kThreads / (c.head_dim <= 32 ? 4 : c.head_dim <= 64 ? 8 : 16);
     const int64_t blocks = std::max<int64_t>(1, std::min((tokens + slots - 1) / slots, 16384 / heads));
-    if (heads * blocks > 0x7fffff00LL) return NA1D_ERR_UNSUPPORTED;
+    if (!launchable(heads * blocks)) return NA1D_ERR_UNSUPPORTED;
     auto go = [&](auto kern) {
         launch_kernel(kern, (unsigned)(heads * blocks), 0, s, (char *)c.k, (char *)c.v, (char *)c.k_ranges, (char *)c.v_ranges, (const char *)k, (const char *)v, lengths, t_valid,
                       (int)T, (int)blocks, p.a);

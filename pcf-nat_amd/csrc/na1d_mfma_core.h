@@ -688,6 +688,9 @@ inline void launch_kernel(K kern, unsigned grid, size_t lds, hipStream_t s, Args
     launch_kernel_block(kern, grid, (unsigned)kThreads, lds, s, args...);
 }
 
+// Whether a launch holds so many workgroups: it has less than 2^32 threads.
+inline bool launchable(int64_t workgroups, int64_t threads = kThreads) { return workgroups < (1ll << 32) / threads; }
+
 // Dynamic LDS above 64 KB has to be allowed per kernel.
 template <class K>
 inline bool allow_lds(K kern, size_t bytes) {

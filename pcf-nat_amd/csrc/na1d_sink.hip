@@ -798,14 +798,13 @@ KeyPlan key_plan(const na1d_sink &h) {
 }
 int64_t lse_floats(const na1d_sink &h) { return (h.N * h.heads * h.T + 3) / 4 * 4; }
 int64_t largest_floats(const na1d_sink &h) { return h.dtype == NA1D_FP16 ? h.N * h.heads * ((h.T + kChunkRows - 1) / kChunkRows) * kWaves : 0; }
-bool countable(int64_t items) { return items <= 0x7fffff00LL; }
 
 template <class DT, int C>
 int launch_sink_fwd(const na1d_sink &h, void *out, float *saved, const void *q, const void *k, const void *v, const int32_t *t_valid, hipStream_t s) {
     const bool two = two_tiles(h);
     const SinkArgs a = sink_args(h, two ? 2 : 1);
     const int64_t items = h.N * h.heads * a.strips;
-    if (!countable(items)) return NA1D_ERR_UNSUPPORTED;
+    if (!launchable(items)) return NA1D_ERR_UNSUPPORTED;
     const size_t lds = 4 * (size_t)region_bytes<kStaged<C>>(kKeyTiles);
     auto go = [&](auto kern) {
         if (!allow_lds(kern, lds)) return (int)NA1D_ERR_LAUNCH;
@@ -823,7 +822,7 @@ int launch_sink_bwd(const na1d_sink &h, void *dq, void *dk, void *dv, const void
     const SinkArgs a = sink_args(h, 1);
     const KeyPlan p = key_plan(h);
     const int64_t items = h.N * h.heads * a.strips, key_items = p.a.whole + p.rest, join_items = p.joined * ((kChunkRows * (C / 4) + kThreads - 1) / kThreads);
-    if (!countable(items) || !countable(p.heads * p.a.strips) || !countable(key_items) || !countable(join_items)) return NA1D_ERR_UNSUPPORTED;
+    if (!launchable(items) || !launchable(p.heads * p.a.strips) || !launchable(key_items) || !launchable(join_items)) return NA1D_ERR_UNSUPPORTED;
     float *const delta = ws, *const largest = ws + lse_floats(h), *const partial = largest + largest_floats(h);
     constexpr size_t dq_lds = 4 * (size_t)region_bytes<kStaged<C>>(kKeyTiles), dkv_lds = 2 * (2 * (size_t)region_bytes<kStaged<C>>(kChunkTiles) + 2 * kChunkRows * sizeof(float));
     if (!allow_lds(sink_dq_kernel<DT, C>, dq_lds) || !allow_lds(sink_dkv_kernel<DT, C>, dkv_lds)) return NA1D_ERR_LAUNCH;
