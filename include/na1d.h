@@ -457,7 +457,7 @@ int na1d_head_backward(const na1d_head *h, void *dx, void *dw, const float *dlos
  */
 typedef struct na1d_sink {
     int32_t dtype, heads, kv_heads, head_dim;
-    float scale;                        /* finite and above 0 */
+    float scale;                        /* above 0, up to 2.3e38 (its product with log2(e) is finite) */
     int64_t N, T, window, sinks;
     int64_t q_strides[3], k_strides[3], v_strides[3];
 } na1d_sink;

@@ -610,6 +610,8 @@ int na1d_head_backward(const na1d_head *h, void *dx, void *dw, const float *dlos
     return na1d::loss::run_backward(*h, dx, dw, dloss, x, w, ids, saved, workspace, (hipStream_t)stream);
 }
 
+// In base 2 the scale has to be finite too: an infinite one times a score of 0 is no number.
+static bool bad_exponent(float scale) { return bad_scale(scale) || !(scale * na1d::kLog2e <= 3.4e38f); }
 static int strides_check(const int64_t *s, int64_t head_dim) {
     if (!s) return NA1D_ERR_NULL;
     if (s[0] < 0 || s[1] < 0 || s[2] < head_dim) return NA1D_ERR_SHAPE;
@@ -623,7 +625,7 @@ static int sink_check(const na1d_sink *h) {
     if (h->head_dim < 1 || h->head_dim % 8) return NA1D_ERR_HEAD_DIM;
     if (h->window < 1 || h->sinks < 0) return NA1D_ERR_WINDOW;
     if (h->N < 0 || h->T < 0 || h->heads < 1 || h->kv_heads < 1 || h->heads % h->kv_heads) return NA1D_ERR_SHAPE;
-    if (bad_scale(h->scale)) return NA1D_ERR_SCALE;
+    if (bad_exponent(h->scale)) return NA1D_ERR_SCALE;
     const int64_t widest = 1 << 20;
     if (h->head_dim > 128 || h->T > (1 << 24) || (int64_t)h->heads * h->head_dim > widest) return NA1D_ERR_UNSUPPORTED;
     if (h->N > (1ll << 36) / h->heads / (h->T > 0 ? h->T : 1)) return NA1D_ERR_UNSUPPORTED;
@@ -698,7 +700,7 @@ static int cache_call(const na1d_sink_cache *c, void *out, const void *q, const 
                       int64_t workspace_bytes, void *stream, bool stores) {
     const int st = cache_check(c, fresh, heads, window);
     if (st < 0) return st;
-    if (bad_scale(scale)) return NA1D_ERR_SCALE;
+    if (bad_exponent(scale)) return NA1D_ERR_SCALE;
     if (st > 0) return NA1D_OK;
     if (!out || !q || !lengths || (stores && (!k || !v))) return NA1D_ERR_NULL;
     for (const int bad : {cache_pointers(c), strides_check(q_strides, c->head_dim), stores ? strides_check(k_strides, c->head_dim) : 0,

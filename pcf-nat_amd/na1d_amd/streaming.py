@@ -200,8 +200,8 @@ def sink_attention(q, k, v, win_size, sinks=0, t_valid=None, scale=None):
 
     q ``[N, T, heads, C]``, k and v ``[N, T, kv_heads, C]``, which may be views of one projection's output (any strides that are
     multiples of 8 with contiguous channels; others are packed first).  ``t_valid`` int32 ``[N]``: tokens from there on do not exist; they
-    may hold anything, and their outputs and gradients are 0.  The tokens before have to be finite.  ``scale`` (finite and above
-    0) defaults to ``C ** -0.5``.  Returns ``[N, T, heads, C]``.  The gradients cannot be differentiated again (asking for it raises).
+    may hold anything, and their outputs and gradients are 0.  The tokens before have to be finite.  ``scale`` (above 0,
+    up to 2.3e38) defaults to ``C ** -0.5``.  Returns ``[N, T, heads, C]``.  The gradients cannot be differentiated again (asking for it raises).
     """
     nodes = _nodes(win_size, sinks)
     out = None if nodes is None else nodes.sink(q, k, v, win_size, sinks, t_valid, scale)

@@ -34,3 +34,18 @@ def test_caches_of_more_workgroups_than_a_launch_has(bits, head_dim, N, kv_heads
     assert lib.na1d_sink_step(ref, 16, 16, 16, 16, s, s, s, 16, fresh, heads, 2, 0.1, 16, 1 << 50, None) == UNSUPPORTED
     if N * kv_heads == 1 << 24:
         assert lib.na1d_sink_append(ref, 16, 16, s, s, None, None, 5, None) == UNSUPPORTED
+
+
+@pytest.mark.parametrize("scale", [2.4e38, 3.0e38])
+def test_scales_whose_product_with_log2_e_is_infinite(scale):
+    """An infinite factor times a score of 0 is no number."""
+    lib, h = _lib.load(), ctypes.byref(_sink(1, 10, 2, 1, scale=scale))
+    assert lib.na1d_sink_saved_bytes(h) == SCALE and lib.na1d_sink_backward_workspace_bytes(h) == SCALE
+    assert lib.na1d_sink_forward(h, 16, None, 0, 16, 16, 16, None, None) == SCALE
+    c, s = ctypes.byref(streaming._Cache(0, 16, 2, 8, 1, 9, 1, 16, 16, None, None)), (ctypes.c_int64 * 3)(16, 8, 16)
+    assert lib.na1d_sink_attend(c, 16, 16, s, 16, 1, 2, 8, scale, 16, 1 << 50, None) == SCALE
+    assert lib.na1d_sink_step(c, 16, 16, 16, 16, s, s, s, 16, 1, 2, 8, scale, 16, 1 << 50, None) == SCALE
+
+
+def test_the_largest_scale():
+    assert _lib.load().na1d_sink_saved_bytes(ctypes.byref(_sink(1, 10, 2, 1, scale=2.3e38))) > 0
