@@ -109,3 +109,37 @@ def over_history(q, k, v, window, sinks, ends, scale=None, four=False):
         bound[i] = (u * o.abs() + u * (p @ rounded) + f * (p @ heads(wide(v[i])))).transpose(0, 1)
     least = 2.0 ** -25 if q.dtype == torch.float16 else 2.0 ** -126
     return out, bound + least * (1 + 16 * sum(x.shape[0] for x in v))
+
+
+def centred(N, T, H, K, C, dtype, mean=0.0):
+    """Standard normal q, k, v, dout, v with a mean."""
+    g = torch.Generator().manual_seed(T + C)
+    q, k, v, dout = (torch.randn(N, T, h, C, generator=g) for h in (H, K, K, H))
+    return [x.to(dtype) for x in (q, k, v + mean, dout)]
+
+
+def more_than_rounding(got, value):
+    """By how much the error of `got`, as a norm, is more than that of the value's rounding, in half steps."""
+    off, own, size = ((x.double() - value).norm() for x in (got, value.to(got.dtype), torch.zeros_like(value)))
+    return float((off - own) / size) / half_step(got.dtype)
+
+
+def rounded_gradients(q, k, v, window, sinks, dout, ds_once=False, p_once=False, bytes_lost=False, bytes_wrong=False):
+    """A head's gradients with the roundings that a backward's kernels have, [1, T, 1, C]: probabilities where they meet v and in their sum, which the backward divides by, and results; and,
+    if asked for, with those that they avoid."""
+    dtype, C, u = q.dtype, q.shape[3], half_step(q.dtype)
+    round_ = lambda x: x.float().to(dtype).double()  # noqa: E731
+    q_, k_, v_, g = (x.double()[0, :, 0] for x in (q, k, v, dout))
+    at = torch.arange(q.shape[1])
+    seen, s = visible(at, at, window, sinks), q_ @ k_.t() * C ** -0.5
+    e = torch.where(seen, (s - s.masked_fill(~seen, -torch.inf).amax(-1, keepdim=True) + 0.3).exp(), 0.0)       # (a reference that is not quite the largest)
+    total = round_(e).sum(-1, keepdim=True)
+    p, out = e / total, round_(e) @ v_ / total
+    if bytes_lost:
+        out = round_(out)
+    if bytes_wrong:
+        out = round_(out) + (2 * torch.rand(out.shape, generator=torch.Generator().manual_seed(0), dtype=torch.float64) - 1) * u * out.abs()
+    ds = p * (g @ v_.t() - (g * out).sum(-1, keepdim=True))
+    ds, p = round_(ds) if ds_once else ds, round_(p) if p_once else p
+    got = {"dq": ds @ k_ * C ** -0.5, "dk": ds.t() @ q_ * C ** -0.5, "dv": p.t() @ g}
+    return {n: x.float().to(dtype)[None, :, None] for n, x in got.items()}

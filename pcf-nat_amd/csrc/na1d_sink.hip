@@ -99,8 +99,8 @@ __device__ inline Rsrc rows_of(const void *base, int row, int rows, int pitch) {
 
 // What outputs lose in rounding, for the backward: delta = rowsum(dO * O) is taken away from every dP of a row, and with O as it is stored, half a step off, that
 // alone made dQ and dK 3.5e-3 (bf16) and 4e-4 (fp16) wrong, as a norm; all else together 2e-3 and 2e-4.  As integers, an fp32 value and the fp32 value of its rounding are
-// apart by half a step of bf16 or fp16 at most, 2^15 or 2^12: a signed byte of that, 2^8 or 2^5 each, leaves 2^-17 or 2^-20 of the value.  (fp16 below its normal range has larger
-// steps: there the byte ends at its range.)  The bytes of a tile of 16 rows lie as dQ's waves read them: channels 32 s + 8 g of row n in the eight bytes of lane
+// apart by half a step of bf16 or fp16 at most, 2^15 or 2^12: a signed byte of that, 2^8 or 2^5 each and rounded down, leaves 2^-15 or 2^-18 of the value at most.  (fp16 below
+// its normal range has larger steps: there the byte ends at its range.)  The bytes of a tile of 16 rows lie as dQ's waves read them: channels 32 s + 8 g of row n in the eight bytes of lane
 // 16 g + n of step s (16 channels: four bytes of a lane).
 template <int C> constexpr int kRestBytes = 16 * C;      // of a tile
 template <class DT> constexpr int kRestShift = DT::tag == NA1D_BF16 ? 8 : 5;
