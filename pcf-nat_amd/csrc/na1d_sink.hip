@@ -186,7 +186,7 @@ __device__ inline float wave_max(float x) { return xor_max(max_with<0x140>(max_w
 template <class DT> constexpr bool kNarrow = DT::tag == NA1D_FP16;
 template <class DT> constexpr int kBackLift = kNarrow<DT> ? 10 : 0;
 constexpr float kTooLarge = 32768.f;        // and what is, is taken down to between 2^14 and 2^15
-__device__ inline int too_much(float high) { return high > kTooLarge ? __builtin_amdgcn_frexp_expf(high) - 15 : 0; }
+__device__ inline int too_much(float high) { return high > kTooLarge && high < __builtin_inff() ? __builtin_amdgcn_frexp_expf(high) - 15 : 0; }
 
 // =============================================================================
 // Forward

@@ -205,3 +205,24 @@ def test_gradients_of_small_shares(H, K, C, T, W, dtype):
     want = O.attention(q, k, v, W, 1, scale=1.0 / C, dout=dout)
     got = _gradients(q, k, v, dout, W, 1, scale=1.0 / C)
     _norms_near({n: got[n] for n in ("dk", "dv")}, want, O.half_step(dtype) * (3 ** -0.5 + 0.05), slice(1, None))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=NAMES)
+@pytest.mark.parametrize("filler", [float("inf"), float("nan")])
+def test_what_comes_back_infinite_stays_where_it_belongs(filler, dtype):
+    """As where a loss's scale was too large: such gradients are no numbers, so that whoever looks for that finds it, and rows that have nothing to do with them are as without."""
+    N, T, H, K, C, W = 2, 640, 4, 2, 64, 64
+    g = torch.Generator().manual_seed(5)
+    q, k, v, dout = (torch.randn(N, T, h, C, generator=g).to(dtype).cuda() for h in (H, K, K, H))
+    clean = _gradients(q, k, v, dout, W)
+    dout[0, 100, 1] = filler
+    got = _gradients(q, k, v, dout, W)
+    torch.cuda.synchronize()
+    bad = torch.zeros(N, T, dtype=torch.bool, device="cuda")
+    bad[0, 100] = True
+    assert not bool(got["dq"][0, 100, 1].isfinite().any())
+    assert torch.equal(got["dq"][~bad], clean["dq"][~bad]) and torch.equal(got["dq"][0, 100, [0, 2, 3]], clean["dq"][0, 100, [0, 2, 3]])
+    for name in ("dk", "dv"):
+        assert not bool(got[name][0, 37:101, 0].isfinite().any())
+        assert torch.equal(got[name][1], clean[name][1]) and torch.equal(got[name][0, :, 1], clean[name][0, :, 1])
+        assert torch.equal(got[name][0, 128:, 0], clean[name][0, 128:, 0])            # (strips of 64 keys that the row's chunk of queries does not see)
