@@ -443,7 +443,7 @@ int na1d_head_backward(const na1d_head *h, void *dx, void *dw, const float *dlos
  *   q [N, T, heads, head_dim], k, v [N, T, kv_heads, head_dim]: {sample, head, row} element strides, channels contiguous
  *   out, dout, dq [N, T, heads, head_dim], dk, dv [N, T, kv_heads, head_dim]: packed
  *   t_valid : int32 [N] or NULL; rows from there on do not exist: they may hold anything, their outputs and gradients are 0.
- *             The rows before have to be finite.
+ *             The rows before have to be finite, scores scale * q . k below 2^26 in size, and v (bf16) below 2^100.
  *   saved   : what a forward leaves for its backward, na1d_sink_saved_bytes() bytes: 4 to a head's row and a byte to a value of out
  *             (what its rounding lost; head_dim counted as the next of 16, 32, 64, 96, 128); NULL for inference
  * Scores, softmax and sums are in fp32; probabilities are rounded to 16 bits where they are multiplied by v; in the backward they and their

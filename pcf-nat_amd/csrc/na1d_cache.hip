@@ -420,7 +420,7 @@ cache_attend_kernel(char *__restrict__ out, float *__restrict__ partial, const c
             for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) high = __builtin_fmaxf(high, s[h][kt][r]);
-            sums.move(h, xor_max(high) * scale2);
+            sums.move(h, reference_of<DT>(xor_max(high) * scale2));
             const float ref = kLift<DT> - sums.m[h];
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt) {

@@ -288,6 +288,9 @@ __device__ inline f32x4 dot_rows_mma(const RowOperand<C> &a, const RowOperand<C>
 // A probability that is rounded to fp16 beside one of 1 loses digits below 2^-14 and is 0 below 2^-25: a few first tokens that take nearly all of a row leave the
 // others there.  The attention of streams rounds 2^kLift times a probability: with a reference that lags by 2^6 that is 2^15 at most.
 template <class DT> constexpr float kLift = DT::tag == NA1D_FP16 ? 9.f : 0.f;
+// The reference of a row whose largest score (times log2(e)) has been rounded to x: in fp16 no smaller than that score itself, since from 2^24 on half a step of x is an octave and
+// more, by which the largest probability would pass 2^15 of lift and lag.
+template <class DT> __device__ inline float reference_of(float x) { return DT::tag == NA1D_FP16 ? __builtin_fmaf(__builtin_fabsf(x), 0x1p-23f, x) : x; }
 
 // Two 16-bit values of a register as floats.
 template <class DT> __device__ inline f32x2 unpack2(uint32_t w);

@@ -292,7 +292,7 @@ sink_fwd_kernel(char *__restrict__ out, float *__restrict__ lse, char *__restric
             // kSlack (probabilities then stay below 2^kSlack, which every format here holds, also 2^kLift times that): most
             // chunks leave the accumulators as they are.
             if (__builtin_amdgcn_ballot_w64(mc > m[h] + kSlack)) {
-                const float m_new = max2(m[h], mc);
+                const float m_new = max2(m[h], reference_of<DT>(mc));
                 const float alpha = __builtin_amdgcn_exp2f(m[h] - m_new);
                 m[h] = m_new;
                 lsum[h] *= alpha;

@@ -226,3 +226,30 @@ def test_what_comes_back_infinite_stays_where_it_belongs(filler, dtype):
         assert not bool(got[name][0, 37:101, 0].isfinite().any())
         assert torch.equal(got[name][1], clean[name][1]) and torch.equal(got[name][0, :, 1], clean[name][0, :, 1])
         assert torch.equal(got[name][0, 128:, 0], clean[name][0, 128:, 0])            # (strips of 64 keys that the row's chunk of queries does not see)
+
+
+# ------------------------------------------------------------------------------------------------ large scores
+@pytest.mark.parametrize("dtype", DTYPES, ids=NAMES)
+@pytest.mark.parametrize("size", [300.0, 1500.0, 6000.0])
+def test_scores_of_many_millions(size, dtype):
+    """Where fp32 has few or no digits behind a score's point a row's output is the value of its largest score, if that is larger than the next by more than sums of 64 products are off by."""
+    N, T, H, K, C, W, Z = 2, 300, 4, 2, 64, 250, 2
+    g = torch.Generator().manual_seed(6)
+    q, k, v = (torch.randn(N, T, h, C, generator=g) for h in (H, K, K))
+    q, k, v = (x.to(dtype).cuda() for x in (size * q, size * k, v))
+    at = torch.arange(T, device="cuda")
+    s = (q.double().transpose(1, 2) @ k.double().transpose(1, 2).repeat_interleave(H // K, 1).transpose(-1, -2) * C ** -0.5).masked_fill(~O.visible(at, at, W, Z), -torch.inf)
+    top = s.topk(2, -1)
+    off = 2.0 ** -20 * (q.double().abs().transpose(1, 2) @ k.double().abs().transpose(1, 2).repeat_interleave(H // K, 1).transpose(-1, -2) * C ** -0.5).amax(-1)
+    clear = top.values[..., 0] - top.values[..., 1] > off + 12          # e^-12 is below half a step
+    assert float(clear.double().mean()) > 0.8
+    want = v.transpose(1, 2).repeat_interleave(H // K, 1).gather(2, top.indices[..., :1].expand(N, H, T, C))
+    out = streaming.sink_attention(q, k, v, W, Z).transpose(1, 2)
+    cache = streaming.new_cache(N, K, T, C, 16, dtype)
+    streaming.cache_append(k, v, *cache, sinks=Z)
+    step = streaming.cache_attend(q[:, -1:], *cache, torch.full((N,), T, dtype=torch.int32, device="cuda"), W, Z).transpose(1, 2)
+    torch.cuda.synchronize()
+    u = O.half_step(dtype)
+    assert bool(out.isfinite().all()) and bool(step.isfinite().all())
+    assert float((out.double() - want)[clear].abs().max()) < 2 * u * float(v.abs().max())
+    assert float((step.double() - want[:, :, -1:])[clear[:, :, -1:]].abs().max()) < 2 * u * float(v.abs().max())
