@@ -699,8 +699,9 @@ struct CachePlan {
     int64_t items;
 };
 // Blocks of 16, 32 or 64 rows of queries.  16-bit rows of up to 64 channels: where the card is not full with a workgroup to every head of keys, and a large one gets through them with at most
-// kSerial units to a wave, that one has them all, and a launch less: one stream's step over 1028 keys, 4 heads of 64, was 7.5 us in 4 workgroups of eight waves (7.0 since), and 6.2 and 3.6 in
-// 16 of four and a join.  (Rows in 4 bits, whose units take longer: 15.6 us in one workgroup of 16 waves to a head, 8.7 and 4.9 in shares, for 5 streams of 2 heads of 64, 2008 keys.)
+// kSerial units to a wave, that one has them all, and a launch less.  With one and with shares, us of a captured step over 1024 and 2048 keys, 16 heads: 5.7 and 6.3, 6.7 and 6.2 (16
+// channels), 5.9 and 6.8, 7.1 and 6.8 (32), 6.5 and 7.3, 8.2 and 7.5 (64: the second are eight units to a wave); 256 heads: 6.2 and 8.4, 7.4 and 9.8 (16), 6.5 and 9.2, 13.2 and 16.0 (32), 14.2 and 16.4 (64,
+// 1024 keys).  (Rows in 4 bits, whose units take longer: 15.6 us in one workgroup of 16 waves to a head, 8.7 and 4.9 in shares, for 5 streams of 2 heads of 64, 2008 keys.)
 // Otherwise workgroups of four waves, as many to a head as occupy the card in whole rounds, with two units of keys to a wave at least, one in 4 bits.
 constexpr int kSerial = 5;
 CachePlan cache_plan(const na1d_sink_cache &c, int64_t fresh, int heads, int64_t window) {

@@ -192,7 +192,7 @@ __device__ inline int too_much(float high) { return high > kTooLarge && high < _
 // Forward
 // =============================================================================
 // What bounds it: with long windows the matrix cores and what a softmax takes of the vector unit, which wait for each other (2 x 16 x 8192 rows of 128 channels, 4 key heads, window 1024:
-// 170 us, 0.77 PFLOP/s of what the mask leaves, matrix cores busy 0.44 of the time; 32 x 16384 over 8, window 2048: 513 us, 1.0 PFLOP/s, 0.53), with short ones memory (16 x 16 x 1000 rows of
+// 170 us, 0.77 PFLOP/s of what the mask leaves, matrix cores busy 0.44 of the time; 32 x 16384 over 8, window 2048: 520 us, 1.0 PFLOP/s, 0.53), with short ones memory (16 x 16 x 1000 rows of
 // 64 channels, window 128: 33 us, 153 MB behind the L2s, 4.6 TB/s), with few rows a chunk's turn, a chain of
 // dependent instructions (4 x 300 rows: 6.7 us; a third chunk on its way does nothing for them).
 template <class DT, int C, int QT>
