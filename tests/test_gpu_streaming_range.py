@@ -253,3 +253,30 @@ def test_scores_of_many_millions(size, dtype):
     assert bool(out.isfinite().all()) and bool(step.isfinite().all())
     assert float((out.double() - want)[clear].abs().max()) < 2 * u * float(v.abs().max())
     assert float((step.double() - want[:, :, -1:])[clear[:, :, -1:]].abs().max()) < 2 * u * float(v.abs().max())
+
+
+def test_a_captured_fp16_step_for_gradients_of_any_size():
+    """What one replay's dS was taken down by is not the next one's."""
+    N, T, H, K, C, W = 2, 300, 4, 2, 64, 100
+    g = torch.Generator().manual_seed(7)
+    q, k, v, base = (torch.randn(N, T, h, C, generator=g).to(torch.float16).cuda() for h in (H, K, K, H))
+    q, k, v = (x.requires_grad_(True) for x in (q, k, v))
+    dout = base.clone()
+
+    def step():
+        return torch.autograd.grad(streaming.sink_attention(q, k, v, W, 2), [q, k, v], dout)
+
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        step()
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for power in (11, -10, 0, 11, -12):
+        dout.copy_(base * 2.0 ** power)
+        want = step()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want)) and all(bool(x.isfinite().all()) for x in want)
